@@ -261,8 +261,16 @@ p2p_status p2p_attn_decode_ragged(p2p_ctx* ctx, const p2p_attn_params* prm, cons
  *   - paged caches (the bundle's PagedAttention layout): k_cache / v_cache are pools of
  *     [kv_rows pages][block_size][Hkv][D] and key j of sequence i is row j % block_size of page
  *     block_table[i * max_blocks + j / block_size].
- * block_size 0 selects the contiguous form of p2p_attn_decode_ragged (offsets). */
-typedef enum p2p_kv_format { P2P_KV_F16 = 0, P2P_KV_I8 = 1 } p2p_kv_format;
+ * block_size 0 selects the contiguous form of p2p_attn_decode_ragged (offsets).
+ *   - 4-bit rows (P2P_KV_Q4; no counterpart in the reference), which carry their own scales:
+ *     the row of one token holds one 36-byte unit per kv head -- 32 bytes of codes (dim 2b in
+ *     the low, dim 2b+1 in the high nibble of byte b), the f16 scale, the f16 lowest value lo
+ *     -- and is padded to p2p_kv_q4_row_bytes(Hkv), the units' bytes rounded up to 16.  With
+ *     lo = min(x) and scale = f16((max(x) - lo) / 15) over the head's 64 values,
+ *     code = clamp(roundeven((x - lo) / scale), 0, 15) (0 when scale is 0) and a value reads
+ *     f32(code) * scale + lo.  A cache row of such a cache is a token row of that many bytes
+ *     (k_scale, v_scale and scale_count are not used); values must be finite. */
+typedef enum p2p_kv_format { P2P_KV_F16 = 0, P2P_KV_I8 = 1, P2P_KV_Q4 = 2 } p2p_kv_format;
 typedef struct p2p_kv_layout {
   int32_t format;              /* p2p_kv_format */
   const float* k_scale;        /* int8: scale_count f32 scales in device memory */
@@ -286,6 +294,108 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
                               void* v_cache, int64_t kv_rows, const int32_t* offsets,
                               const int32_t* past, int32_t nseq, int32_t max_past,
                               int32_t fused_prep, void* out, int64_t ld_o, void* stream);
+
+/* The batched decode over a P2P_KV_Q4 cache: p2p_attn_decode_kv with that format.  It differs
+ * from the other formats in its workspace: a fixed one per context, made by the first such call
+ * (which must not be inside a stream capture: P2P_ERR_INVALID_ARG) and never moved, so that
+ * captured graphs stay valid; calls of one context that use it must not overlap on the GPU.  A
+ * bad block-table entry keeps the sequence's output rows from being written, but with
+ * fused_prep its new row may already be in the cache. */
+
+/* Bytes of one token's row in a P2P_KV_Q4 cache (0 for num_kv_heads <= 0). */
+int64_t p2p_kv_q4_row_bytes(int32_t num_kv_heads);
+/* Converts f16 cache rows [rows][Hkv][D] to P2P_KV_Q4 rows (src and dst 16-byte aligned; the
+ * same rule the appends use; the padding of a row is written as 0). */
+p2p_status p2p_kv_quantize_q4(p2p_ctx* ctx, const void* src, void* dst, int64_t rows,
+                              int32_t num_kv_heads, void* stream);
+
+/* QK_PREP (kernels.js:216-266) of ragged prompt chunks into a cache of any layout.  Rows
+ * row_start[i] .. row_start[i+1]-1 of qkv [n_rows][ld_qkv] (f16, [Hq*D | Hkv*D | Hkv*D]) are the
+ * tokens of sequence i at positions past[i], past[i]+1, ...: q and k are normed (norm_w NULL:
+ * not) and rotated exactly as p2p_qk_prep does it, k and v go to the sequence's cache rows of
+ * those positions in the layout's format, and the rotated q to q_out [n_rows][ld_q] (NULL: not
+ * wanted).  row_start (nseq + 1 values), past and offsets are device int32 arrays; the rope
+ * table holds max_len rows or more.  Rows at and behind row_start[nseq] are left alone, in qkv's
+ * outputs and in the cache.  A sequence with a negative entry, past[i] + rows > max_len, rows
+ * beyond n_rows, kv_rows or max_blocks is skipped, and so is a row whose block-table entry lies
+ * outside the pool; the next p2p_sync then returns P2P_ERR_KV_FULL.  Two sequences must not
+ * name the same cache row.  qkv, q_out, norm_w, rope 8-byte aligned (ld_qkv, ld_q multiples of
+ * 4), cache buffers 16-byte aligned. */
+p2p_status p2p_kv_append(p2p_ctx* ctx, const p2p_attn_params* prm, const p2p_kv_layout* layout,
+                         const void* qkv, int64_t ld_qkv, const void* norm_w, const void* rope,
+                         void* k_cache, void* v_cache, int64_t kv_rows, const int32_t* offsets,
+                         const int32_t* past, const int32_t* row_start, int32_t nseq,
+                         int64_t n_rows, int32_t max_len, void* q_out, int64_t ld_q,
+                         void* stream);
+
+/* Reads cached sequences of any layout back: rows row_start[i] + j of the dense f16 outputs
+ * k_out / v_out [n_rows][Hkv][D] (16-byte aligned; one of them may be NULL) receive the values
+ * of key first[i] + j of sequence i, rounded to f16, for j < row_start[i+1] - row_start[i].  The
+ * sequences are checked as in p2p_kv_append. */
+p2p_status p2p_kv_read(p2p_ctx* ctx, const p2p_kv_layout* layout, int32_t num_kv_heads,
+                       const void* k_cache, const void* v_cache, int64_t kv_rows,
+                       const int32_t* offsets, const int32_t* first, const int32_t* row_start,
+                       int32_t nseq, int64_t n_rows, int32_t max_len, void* k_out, void* v_out,
+                       void* stream);
+
+/* ATTN (kernels.js:268-319) of ragged prompt chunks over a cache of any layout: rotated query
+ * row t of sequence i (row row_start[i] + t of q [n_rows][ld_q]) attends keys 0 .. past[i] + t
+ * of that sequence, which must already be in the cache (p2p_kv_append), and its Hq heads go to
+ * the same row of out [n_rows][ld_o].  Arrays and checks as in p2p_kv_append, except that a bad
+ * block-table entry keeps all rows of the sequence that see it from being written.  q and out
+ * 16-byte aligned (ld_q and ld_o multiples of 8).  Cached values are rounded to f16 once, the
+ * precision of an f16 cache, before they enter the tensor cores.  The workspace is the one of
+ * the 4-bit decode above, under the same rules. */
+p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
+                             const p2p_kv_layout* layout, const void* q, int64_t ld_q,
+                             const void* k_cache, const void* v_cache, int64_t kv_rows,
+                             const int32_t* offsets, const int32_t* past,
+                             const int32_t* row_start, int32_t nseq, int64_t n_rows,
+                             int32_t max_len, void* out, int64_t ld_o, void* stream);
+
+/* The greedy tokens of a batch of logits under penalties, biases and a grammar mask (the batched
+ * counterpart of p2p_argmax_step; the penalties have none in the reference, whose engine hands
+ * the logits to a host-side processor, engine.js:330-361).  For row i and token v, with
+ * n = hist_len[i], p = prompt_len[i] (0 when NULL), seen = v among hist[i][0 .. n), c = the
+ * number of times v is among hist[i][p .. n), all in f32 with one rounding per operation:
+ *   seen:        x = x > 0 ? x / repetition[i] : x * repetition[i]
+ *   c > 0:       x = (x - frequency[i] * c) - presence[i]
+ *   each entry e in bias_start[i] .. bias_start[i+1]-1 with bias_tok[e] = v, in order:
+ *                x = x + bias_val[e]
+ *   mask bit v of row i (bit v % 32 of word v / 32) clear: x = -inf
+ * y = x rounded to the logits' type is stored in out when it is not NULL (out may be logits
+ * itself, with the same ld), and tok[i] is the smallest index of the largest y above -inf (NaN
+ * never wins), or -1 when there is none.  Any of hist, repetition, presence, frequency,
+ * bias_start and mask may be NULL.  Tokens outside the vocabulary are ignored.  With advance != 0,
+ * a token >= 0 is appended to hist[i] and hist_len[i] and past[i] (when not NULL) grow by one,
+ * on the device; when hist_len[i] has reached hist_cap neither changes and the next p2p_sync
+ * returns P2P_ERR_INVALID_ARG.  vocab at most P2P_MAX_VOCAB. */
+#define P2P_MAX_VOCAB 400000
+typedef struct p2p_logits {
+  const void* logits; /* [rows][ld] f16 or f32 */
+  void* out;          /* [rows][ld_out] or NULL */
+  int32_t* tok;       /* [rows] */
+  int64_t ld, ld_out;
+  int32_t rows, vocab;
+  int32_t dtype; /* P2P_F16 or P2P_F32 */
+  int32_t advance;
+  int32_t* hist;     /* [rows][ld_hist] token ids, hist_cap of each row usable */
+  int32_t* hist_len; /* [rows] */
+  const int32_t* prompt_len;
+  int32_t* past; /* [rows] or NULL: advanced with hist_len */
+  int64_t ld_hist;
+  int32_t hist_cap;
+  int32_t n_bias;          /* entries of bias_tok / bias_val */
+  const float* repetition; /* [rows] each */
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_start; /* [rows + 1] */
+  const int32_t* bias_tok;
+  const float* bias_val;
+  const uint32_t* mask; /* [rows][ld_mask], ld_mask >= ceil(vocab / 32) */
+  int64_t ld_mask;
+} p2p_logits;
+p2p_status p2p_logits_pick(p2p_ctx* ctx, const p2p_logits* args, void* stream);
 
 /* Converts f16 cache rows [rows][Hkv][D] to the int8 format above (src 16-byte and dst 8-byte
  * aligned; the same restated rule the decode uses when it appends). */

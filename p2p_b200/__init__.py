@@ -8,9 +8,9 @@ from ._lib import (  # noqa: F401
     LIB_PATH, MAX_LAYERS, P2P_ERR_INVALID_ARG, P2P_ERR_KV_FULL, P2P_ERR_NCCL, P2P_ERR_OOM,
     P2P_ERR_TIMEOUT, KvFullError, OomError, P2PError, lib,
 )
-from .attention import Context, KVCache, LfmAttention, Params  # noqa: F401
+from .attention import Context, KVCache, LfmAttention, Params, kv_q4_row_bytes  # noqa: F401
 from .comm import Comm  # noqa: F401
 
 __all__ = ["Comm", "Context", "KVCache", "LfmAttention", "Params", "P2PError", "KvFullError",
            "OomError", "lib", "LIB_PATH", "MAX_LAYERS", "P2P_ERR_INVALID_ARG", "P2P_ERR_KV_FULL",
-           "P2P_ERR_NCCL", "P2P_ERR_OOM", "P2P_ERR_TIMEOUT"]
+           "P2P_ERR_NCCL", "P2P_ERR_OOM", "P2P_ERR_TIMEOUT", "kv_q4_row_bytes"]

@@ -67,6 +67,35 @@ class KvLayout(C.Structure):
     ]
 
 
+class Logits(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("out", C.c_void_p),
+        ("tok", C.c_void_p),
+        ("ld", C.c_int64),
+        ("ld_out", C.c_int64),
+        ("rows", C.c_int32),
+        ("vocab", C.c_int32),
+        ("dtype", C.c_int32),
+        ("advance", C.c_int32),
+        ("hist", C.c_void_p),
+        ("hist_len", C.c_void_p),
+        ("prompt_len", C.c_void_p),
+        ("past", C.c_void_p),
+        ("ld_hist", C.c_int64),
+        ("hist_cap", C.c_int32),
+        ("n_bias", C.c_int32),
+        ("repetition", C.c_void_p),
+        ("presence", C.c_void_p),
+        ("frequency", C.c_void_p),
+        ("bias_start", C.c_void_p),
+        ("bias_tok", C.c_void_p),
+        ("bias_val", C.c_void_p),
+        ("mask", C.c_void_p),
+        ("ld_mask", C.c_int64),
+    ]
+
+
 class Q4Matrix(C.Structure):
     _fields_ = [
         ("qweight", C.c_void_p),
@@ -79,6 +108,7 @@ class Q4Matrix(C.Structure):
 
 P2P_KV_F16 = 0
 P2P_KV_I8 = 1
+P2P_KV_Q4 = 2
 
 
 class DecodeLayer(C.Structure):
@@ -136,6 +166,18 @@ PROTOTYPES = {
     "p2p_attn_decode_kv": (
         _st, [_v, _pp, C.POINTER(KvLayout), _v, _i64, _v, _v, _v, _v, _i64, _v, _v, _i32, _i32,
               _i32, _v, _i64, _v]),
+    "p2p_kv_q4_row_bytes": (_i64, [_i32]),
+    "p2p_kv_quantize_q4": (_st, [_v, _v, _v, _i64, _i32, _v]),
+    "p2p_kv_append": (
+        _st, [_v, _pp, C.POINTER(KvLayout), _v, _i64, _v, _v, _v, _v, _i64, _v, _v, _v, _i32,
+              _i64, _i32, _v, _i64, _v]),
+    "p2p_kv_read": (
+        _st, [_v, C.POINTER(KvLayout), _i32, _v, _v, _i64, _v, _v, _v, _i32, _i64, _i32, _v, _v,
+              _v]),
+    "p2p_attn_chunk_kv": (
+        _st, [_v, _pp, C.POINTER(KvLayout), _v, _i64, _v, _v, _i64, _v, _v, _v, _i32, _i64, _i32,
+              _v, _i64, _v]),
+    "p2p_logits_pick": (_st, [_v, C.POINTER(Logits), _v]),
     "p2p_kv_quantize_q8": (_st, [_v, _v, _v, _i64, _i32, _v, _i32, _v]),
     "p2p_gemv_q4": (_st, [_v, C.POINTER(Q4Matrix), _v, _v, _i64, _v]),
     "p2p_qkv_gemv_prep": (

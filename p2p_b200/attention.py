@@ -11,6 +11,9 @@ with device memory held in torch tensors and every kernel in libp2pattn.so:
     Context.attn           ATTN      kernels.js:268-319, dispatched engine.js:214-222
     Context.decode_step    QK_PREP + ATTN at M=1 for all attention layers (engine.js:425-429)
     Context.attn_decode_ragged  ATTN at M=1 over many sequences sharing one cache
+    Context.kv_append / kv_read / attn_chunk_kv  QK_PREP and ATTN of ragged prompt chunks over
+                           a cache of any layout (f16, int8 or 4-bit, contiguous or paged)
+    Context.logits_pick    ARGMAX of a batch under penalties, biases and grammar masks
     Context.attn_bidir     VISION_ATTN vision-kernels.js:176-258, dispatched vision.js:271-276
     KVCache                K/V buffers engine.js:152-165 and ensureCapacity engine.js:274-304
     LfmAttention           the per-layer op pair + meta + rope + KV cache of createLfmEngine
@@ -24,9 +27,30 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import AttnParams, DecodeLayer, check, lib
+from ._lib import AttnParams, DecodeLayer, P2PError, check, lib
 
 HEAD_DIM = 64
+
+
+# The current stream's handle on a device (the same as torch.cuda.current_stream(d).cuda_stream,
+# without building a Stream object on every call).
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(
+    torch._C, "_cuda_getCurrentRawStream") else (
+    lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
+def _need(ok: bool, msg: str):
+    if not ok:
+        raise P2PError(_lib.P2P_ERR_INVALID_ARG, msg)
+
+
+def _addr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _table(t):
+    """A rope table: a tensor or what Context.rope_table returned."""
+    return t if t is None or isinstance(t, C.c_void_p) else t.data_ptr()
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -37,6 +61,11 @@ def _stream(stream) -> C.c_void_p:
     if stream is None:
         stream = torch.cuda.current_stream()
     return C.c_void_p(stream.cuda_stream)
+
+
+def kv_q4_row_bytes(num_kv_heads: int) -> int:
+    """Bytes of one token's row in a 4-bit KV cache."""
+    return lib.p2p_kv_q4_row_bytes(num_kv_heads)
 
 
 @dataclass
@@ -240,12 +269,30 @@ class Context:
                        v_scale: Optional[torch.Tensor] = None,
                        block_table: Optional[torch.Tensor] = None, fused_prep: bool = True,
                        kv_rows: Optional[int] = None, stream=None):
-        """Batched decode over an int8 and/or paged KV cache (p2p_attn_decode_kv).
+        """Batched decode over an int8, 4-bit and/or paged KV cache (p2p_attn_decode_kv).
 
         int8 caches (k_cache.dtype == torch.int8) take k_scale / v_scale (f32, 1 or Hkv*64
         values).  Paged caches are [pages][block_size][Hkv][64] with block_table [nseq][max
-        blocks] (int32); contiguous ones [rows][Hkv][64] with offsets (int32)."""
+        blocks] (int32); contiguous ones [rows][Hkv][64] with offsets (int32).  4-bit caches
+        (torch.uint8) hold rows of kv_q4_row_bytes(Hkv) bytes in place of [Hkv][64]."""
         assert past.dtype == torch.int32
+        if k_cache.dtype == torch.uint8:
+            lay, rows = self._layout(prm.num_kv_heads, k_cache, v_cache, past, offsets,
+                                     block_table, None, None)
+            ld_qkv = self._rows(
+                qkv, prm.qkv_width if fused_prep else prm.num_heads * HEAD_DIM, "qkv")
+            ld_o = self._rows(out, prm.num_heads * HEAD_DIM, "out")
+            n = past.shape[0]
+            self._ints(past, n, "past")
+            if n == 0:
+                return
+            _need(qkv.shape[0] >= n and out.shape[0] >= n, "qkv or out has too few rows")
+            self._chk(lib.p2p_attn_decode_kv(
+                self.h, C.byref(prm.c()), C.byref(lay), qkv.data_ptr(), ld_qkv,
+                _addr(norm_w), _table(rope), k_cache.data_ptr(), v_cache.data_ptr(),
+                rows if kv_rows is None else kv_rows, _addr(offsets), past.data_ptr(), n,
+                max_past, int(fused_prep), out.data_ptr(), ld_o, self._stream(stream)))
+            return
         q8 = k_cache.dtype == torch.int8
         lay = _lib.KvLayout()
         lay.format = _lib.P2P_KV_I8 if q8 else _lib.P2P_KV_F16
@@ -267,6 +314,227 @@ class Context:
             rope if isinstance(rope, C.c_void_p) else _ptr(rope), _ptr(k_cache), _ptr(v_cache),
             rows, _ptr(offsets), _ptr(past), past.shape[0], max_past, int(fused_prep),
             _ptr(out), out.stride(0), _stream(stream)))
+
+    # -- caches of any layout: ragged prompt chunks ---------------------------------------------
+    def _stream(self, stream):
+        return _raw_stream(self.device) if stream is None else stream.cuda_stream
+
+    def _rows(self, t: torch.Tensor, width: int, name: str) -> int:
+        """Checks f16 rows of at least `width` values and returns their row stride."""
+        if not (t.dtype == torch.float16 and t.get_device() == self.device and t.dim() == 2 and
+                t.shape[1] >= width and (t.stride(1) == 1 or t.shape[1] == 1)):
+            _need(False, f"{name}: f16 rows of {width} or more values on device {self.device} "
+                  f"needed, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        return t.stride(0) if t.shape[0] > 1 else width
+
+    def _ints(self, t: Optional[torch.Tensor], n: int, name: str):
+        _need(t is not None and t.dtype == torch.int32 and t.get_device() == self.device and
+              t.is_contiguous() and t.numel() >= n,
+              f"{name}: {n} contiguous int32 values on the context's device needed")
+
+    def _layout(self, hkv: int, k_cache, v_cache, past, offsets, block_table, k_scale, v_scale):
+        """The C layout and the cache's rows (or pages) of a pair of cache tensors."""
+        dt = k_cache.dtype
+        q4 = dt == torch.uint8
+        _need(dt in (torch.float16, torch.int8, torch.uint8) and v_cache.dtype == dt and
+              k_cache.shape == v_cache.shape and k_cache.get_device() == self.device and
+              v_cache.get_device() == self.device and k_cache.is_contiguous() and v_cache.is_contiguous(),
+              "k_cache and v_cache: contiguous tensors on the context's device, of one shape and type (f16, int8 "
+              "or uint8) needed")
+        shape = k_cache.shape
+        lead = shape[:-1] if q4 else shape[:-2]
+        want = (kv_q4_row_bytes(hkv),) if q4 else (hkv, HEAD_DIM)
+        _need(tuple(shape[len(lead):]) == want,
+              f"cache rows of shape {want} needed, got {tuple(shape)}")
+        _need(len(lead) == (1 if block_table is None else 2),
+              "[rows] caches with offsets or [pages][block_size] caches with a block table needed")
+        lay = _lib.KvLayout()
+        n = past.numel()
+        if block_table is not None:
+            _need(block_table.dim() == 2 and block_table.shape[0] >= n,
+                  "block_table: [nseq][max_blocks] needed")
+            self._ints(block_table, 0, "block_table")
+            lay.block_size = lead[1]
+            lay.block_table = block_table.data_ptr()
+            lay.max_blocks = block_table.shape[1]
+        else:
+            self._ints(offsets, n, "offsets")
+        if dt == torch.int8:
+            lay.format = _lib.P2P_KV_I8
+            _need(k_scale is not None and v_scale is not None and
+                  k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32 and
+                  k_scale.numel() == v_scale.numel() and k_scale.get_device() == v_scale.get_device() == self.device and
+                  k_scale.is_contiguous() and v_scale.is_contiguous(),
+                  "int8 caches need as many f32 k_scale as v_scale values")
+            lay.k_scale, lay.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+            lay.scale_count = k_scale.numel()
+        else:
+            lay.format = _lib.P2P_KV_Q4 if q4 else _lib.P2P_KV_F16
+        return lay, lead[0]
+
+    def kv_append(self, prm: Params, qkv: torch.Tensor, norm_w: Optional[torch.Tensor], rope,
+                  k_cache: torch.Tensor, v_cache: torch.Tensor, past: torch.Tensor,
+                  row_start: torch.Tensor, *, max_len: int,
+                  q_out: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None,
+                  block_table: Optional[torch.Tensor] = None,
+                  k_scale: Optional[torch.Tensor] = None,
+                  v_scale: Optional[torch.Tensor] = None, stream=None):
+        """QK_PREP of ragged prompt chunks into a cache of any layout (p2p_kv_append): rows
+        row_start[i] .. row_start[i+1] of qkv are sequence i's tokens at positions past[i] and
+        up; their k and v go to the cache, their rotated q to q_out.  The cache tensors are as
+        in attn_decode_kv; the rope table holds max_len rows or more."""
+        lay, rows = self._layout(prm.num_kv_heads, k_cache, v_cache, past, offsets, block_table,
+                                 k_scale, v_scale)
+        n = past.numel()
+        self._ints(past, n, "past")
+        self._ints(row_start, n + 1, "row_start")
+        ld_qkv, ld_q = self._rows(qkv, prm.qkv_width, "qkv"), 0
+        if q_out is not None:
+            ld_q = self._rows(q_out, prm.num_heads * HEAD_DIM, "q_out")
+            _need(q_out.shape[0] >= qkv.shape[0], "q_out has too few rows")
+        if norm_w is not None:
+            _need(norm_w.dtype == torch.float16 and norm_w.numel() == 2 * HEAD_DIM and
+                  norm_w.is_contiguous(), "norm_w: 128 f16 values needed")
+        if isinstance(rope, torch.Tensor):
+            _need(rope.dtype == torch.float16 and rope.is_contiguous() and
+                  rope.numel() >= max_len * HEAD_DIM, f"rope: f16 [{max_len}][64] needed")
+        self._chk(lib.p2p_kv_append(
+            self.h, C.byref(prm.c()), C.byref(lay), qkv.data_ptr(), ld_qkv,
+            _addr(norm_w), _table(rope), k_cache.data_ptr(), v_cache.data_ptr(), rows,
+            _addr(offsets), past.data_ptr(), row_start.data_ptr(), n, qkv.shape[0], max_len,
+            _addr(q_out), ld_q, self._stream(stream)))
+
+    def kv_read(self, prm: Params, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                first: torch.Tensor, row_start: torch.Tensor, k_out: Optional[torch.Tensor],
+                v_out: Optional[torch.Tensor], *, max_len: int,
+                offsets: Optional[torch.Tensor] = None,
+                block_table: Optional[torch.Tensor] = None,
+                k_scale: Optional[torch.Tensor] = None,
+                v_scale: Optional[torch.Tensor] = None, stream=None):
+        """Cached sequences back as f16 values (p2p_kv_read): rows row_start[i] + j of k_out and
+        v_out [rows][Hkv][64] receive key first[i] + j of sequence i."""
+        hkv = prm.num_kv_heads
+        lay, rows = self._layout(hkv, k_cache, v_cache, first, offsets, block_table, k_scale,
+                                 v_scale)
+        n = first.numel()
+        self._ints(first, n, "first")
+        self._ints(row_start, n + 1, "row_start")
+        outs = [t for t in (k_out, v_out) if t is not None]
+        _need(bool(outs), "k_out or v_out needed")
+        for t in outs:
+            _need(t.dtype == torch.float16 and t.get_device() == self.device and t.is_contiguous() and
+                  tuple(t.shape[1:]) == (hkv, HEAD_DIM) and t.shape[0] == outs[0].shape[0],
+                  f"k_out and v_out: contiguous f16 [rows][{hkv}][64] of one length needed")
+        self._chk(lib.p2p_kv_read(
+            self.h, C.byref(lay), hkv, k_cache.data_ptr(), v_cache.data_ptr(), rows,
+            _addr(offsets), first.data_ptr(), row_start.data_ptr(), n,
+            outs[0].shape[0], max_len, _addr(k_out), _addr(v_out),
+            self._stream(stream)))
+
+    def attn_chunk_kv(self, prm: Params, q: torch.Tensor, k_cache: torch.Tensor,
+                      v_cache: torch.Tensor, past: torch.Tensor, row_start: torch.Tensor,
+                      out: torch.Tensor, *, max_len: int,
+                      offsets: Optional[torch.Tensor] = None,
+                      block_table: Optional[torch.Tensor] = None,
+                      k_scale: Optional[torch.Tensor] = None,
+                      v_scale: Optional[torch.Tensor] = None, stream=None):
+        """ATTN of ragged prompt chunks over a cache of any layout (p2p_attn_chunk_kv): rotated
+        query row t of sequence i (row row_start[i] + t) attends keys 0 .. past[i] + t, which
+        kv_append has stored."""
+        lay, rows = self._layout(prm.num_kv_heads, k_cache, v_cache, past, offsets, block_table,
+                                 k_scale, v_scale)
+        n = past.numel()
+        self._ints(past, n, "past")
+        self._ints(row_start, n + 1, "row_start")
+        ld_q = self._rows(q, prm.num_heads * HEAD_DIM, "q")
+        ld_o = self._rows(out, prm.num_heads * HEAD_DIM, "out")
+        _need(out.shape[0] >= q.shape[0], "out has too few rows")
+        self._chk(lib.p2p_attn_chunk_kv(
+            self.h, C.byref(prm.c()), C.byref(lay), q.data_ptr(), ld_q,
+            k_cache.data_ptr(), v_cache.data_ptr(), rows, _addr(offsets), past.data_ptr(),
+            row_start.data_ptr(), n, q.shape[0], max_len, out.data_ptr(), ld_o,
+            self._stream(stream)))
+
+    def kv_quantize_q4(self, src: torch.Tensor, dst: Optional[torch.Tensor] = None,
+                       stream=None) -> torch.Tensor:
+        """f16 cache rows [..., Hkv, 64] -> the rows [..., kv_q4_row_bytes(Hkv)] (uint8) of a
+        4-bit cache."""
+        _need(src.dtype == torch.float16 and src.get_device() == self.device and src.is_contiguous() and
+              src.dim() >= 2 and src.shape[-1] == HEAD_DIM, "src: f16 [..., Hkv, 64] needed")
+        hkv = src.shape[-2]
+        shape = (*src.shape[:-2], kv_q4_row_bytes(hkv))
+        if dst is None:
+            dst = torch.empty(shape, dtype=torch.uint8, device=src.device)
+        _need(dst.dtype == torch.uint8 and tuple(dst.shape) == shape and dst.is_contiguous() and
+              dst.get_device() == self.device, f"dst: contiguous uint8 {shape} needed")
+        self._chk(lib.p2p_kv_quantize_q4(self.h, src.data_ptr(), dst.data_ptr(),
+                                         src.numel() // (hkv * HEAD_DIM), hkv,
+                                         self._stream(stream)))
+        return dst
+
+    def logits_pick(self, logits: torch.Tensor, tok: torch.Tensor, *,
+                    out: Optional[torch.Tensor] = None, hist: Optional[torch.Tensor] = None,
+                    hist_len: Optional[torch.Tensor] = None,
+                    prompt_len: Optional[torch.Tensor] = None,
+                    repetition: Optional[torch.Tensor] = None,
+                    presence: Optional[torch.Tensor] = None,
+                    frequency: Optional[torch.Tensor] = None,
+                    bias_start: Optional[torch.Tensor] = None,
+                    bias_tok: Optional[torch.Tensor] = None,
+                    bias_val: Optional[torch.Tensor] = None,
+                    mask: Optional[torch.Tensor] = None, past: Optional[torch.Tensor] = None,
+                    advance: bool = False, stream=None):
+        """The greedy tokens of a batch of logits [rows][vocab] (f16 or f32) under repetition,
+        presence and frequency penalties over the histories hist [rows][cap], per-row lists of
+        biases and grammar masks [rows][words] (p2p_logits_pick); -1 where nothing is left.
+        The processed logits go to `out` (may be `logits`).  advance appends the tokens to the
+        histories and moves hist_len and past on."""
+        _need(logits.dim() == 2 and logits.get_device() == self.device and logits.stride(1) == 1 and
+              logits.dtype in (torch.float16, torch.float32), "logits: f16 or f32 [rows][vocab]")
+        n, vocab = logits.shape
+        g = _lib.Logits()
+        g.rows, g.vocab, g.advance = n, vocab, int(advance)
+        g.dtype = _lib.P2P_F16 if logits.dtype == torch.float16 else _lib.P2P_F32
+        g.logits = logits.data_ptr()
+        g.ld = logits.stride(0) if n > 1 else vocab
+        self._ints(tok, n, "tok")
+        g.tok = tok.data_ptr()
+        if out is not None:
+            _need(out.shape == logits.shape and out.dtype == logits.dtype and out.get_device() == self.device and
+                  out.stride(1) == 1, "out: the shape and type of the logits needed")
+            g.out, g.ld_out = out.data_ptr(), out.stride(0) if n > 1 else vocab
+        if hist is not None:
+            _need(hist.dtype == torch.int32 and hist.get_device() == self.device and hist.dim() == 2 and
+                  hist.shape[0] >= n and hist.stride(1) == 1, "hist: int32 [rows][cap] needed")
+            self._ints(hist_len, n, "hist_len")
+            g.hist, g.hist_cap = hist.data_ptr(), hist.shape[1]
+            g.ld_hist = hist.stride(0) if hist.shape[0] > 1 else hist.shape[1]
+            g.hist_len = hist_len.data_ptr()
+        for name, t in (("prompt_len", prompt_len), ("past", past)):
+            if t is not None:
+                self._ints(t, n, name)
+                setattr(g, name, t.data_ptr())
+        for name, t in (("repetition", repetition), ("presence", presence),
+                        ("frequency", frequency)):
+            if t is not None:
+                _need(t.dtype == torch.float32 and t.get_device() == self.device and t.is_contiguous() and
+                      t.numel() >= n, f"{name}: {n} f32 values on the device needed")
+                setattr(g, name, t.data_ptr())
+        if bias_start is not None:
+            self._ints(bias_start, n + 1, "bias_start")
+            self._ints(bias_tok, 0, "bias_tok")
+            _need(bias_val is not None and bias_val.dtype == torch.float32 and
+                  bias_val.get_device() == self.device and bias_val.is_contiguous() and
+                  bias_val.numel() >= bias_tok.numel(), "bias_val: an f32 value per bias_tok")
+            g.bias_start, g.bias_tok = bias_start.data_ptr(), bias_tok.data_ptr()
+            g.bias_val, g.n_bias = bias_val.data_ptr(), bias_tok.numel()
+        if mask is not None:
+            _need(mask.dtype == torch.int32 and mask.get_device() == self.device and mask.dim() == 2 and
+                  mask.shape[0] >= n and mask.stride(1) == 1 and
+                  mask.shape[1] >= (vocab + 31) // 32, "mask: int32 [rows][ceil(vocab/32)]")
+            g.mask = mask.data_ptr()
+            g.ld_mask = mask.stride(0) if mask.shape[0] > 1 else mask.shape[1]
+        self._chk(lib.p2p_logits_pick(self.h, C.byref(g), self._stream(stream)))
 
     def kv_quantize_q8(self, src: torch.Tensor, scale: torch.Tensor,
                        dst: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:

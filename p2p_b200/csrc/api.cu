@@ -469,6 +469,10 @@ p2p_status p2p_sync(p2p_ctx* ctx, void* stream) {
       return fail(ctx, P2P_ERR_CUDA,
                   "a kernel's dynamic shared memory did not start on the 1024-byte boundary "
                   "its tiles need; that work was skipped");
+    if (flags & p2p::kErrHistFull)
+      return fail(ctx, P2P_ERR_INVALID_ARG,
+                  "logits_pick: a sequence's history has reached its capacity; its token was not "
+                  "appended");
     if (flags & p2p::kErrOutTokFull)
       return fail(ctx, P2P_ERR_INVALID_ARG,
                   "argmax_step: the step index in the meta buffer reached out_tok's capacity; "
@@ -920,6 +924,39 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
   if (st != P2P_OK) return st;
   if (prm->dtype != P2P_F16)
     return fail(ctx, P2P_ERR_UNSUPPORTED, "decode_kv: q/out must be f16");
+  if (lay->format == P2P_KV_Q4) {
+    p2p::AttnKvArgs q{};
+    st = p2p::make_kv_view(ctx, lay, prm->num_kv_heads, k_cache, v_cache, kv_rows, offsets, nseq,
+                           "decode_kv", &q.kv);
+    if (st != P2P_OK) return st;
+    if (paged && int64_t(max_past) >= (int64_t(lay->max_blocks) << q.kv.shift))
+      return fail(ctx, P2P_ERR_INVALID_ARG, "decode_kv: max_past %d beyond %d blocks of %d",
+                  max_past, lay->max_blocks, lay->block_size);
+    if (max_past == INT32_MAX)
+      return fail(ctx, P2P_ERR_INVALID_ARG, "decode_kv: max_past %d", max_past);
+    if (!aligned16(qkv) || !aligned16(out) || ld_qkv % 8 || ld_o % 8 ||
+        (fused_prep && (!aligned16(rope) || !aligned16(norm_w))))
+      return fail(ctx, P2P_ERR_INVALID_ARG,
+                  "decode_kv: 4-bit caches need 16-byte aligned rows (ld_qkv and ld_o multiples "
+                  "of 8), rope and norm weights");
+    if (nseq == 0) return P2P_OK;
+    q.at = {past, nullptr, nseq, nseq, max_past + 1};
+    q.q = static_cast<const __half*>(qkv);
+    q.ld_q = ld_qkv;
+    q.out = static_cast<__half*>(out);
+    q.ld_o = ld_o;
+    q.hq = prm->num_heads;
+    q.scale_log2 = eff_scale(prm) * 1.4426950408889634f;
+    q.err = ctx->dev_err;
+    q.fused = fused_prep != 0;
+    q.norm_w = static_cast<const __half*>(norm_w);
+    q.rope = static_cast<const __half*>(rope);
+    q.eps = eff_eps(prm);
+    DeviceGuard g(ctx->device);
+    cudaError_t e = p2p::launch_attn_kv(q, pick_stream(ctx, stream));
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "decode_kv launch");
+    return P2P_OK;
+  }
   if (lay->format != P2P_KV_F16 && lay->format != P2P_KV_I8)
     return fail(ctx, P2P_ERR_INVALID_ARG, "decode_kv: format %d", lay->format);
   const int chan = prm->num_kv_heads * prm->head_dim;
@@ -1344,6 +1381,14 @@ p2p_status check_ragged(p2p_ctx* ctx, const p2p_attn_params* prm, const void* qk
         return fail(ctx, P2P_ERR_INVALID_ARG, "%s: rope table of %d rows, max_past %d", who,
                     std::get<0>(kv.first), max_past);
   }
+  return P2P_OK;
+}
+
+p2p_status ctx_check_rope(p2p_ctx* ctx, const void* rope, int32_t max_len, const char* who) {
+  for (const auto& kv : ctx->rope)
+    if (kv.second == rope && std::get<0>(kv.first) < max_len)
+      return fail(ctx, P2P_ERR_INVALID_ARG, "%s: rope table of %d rows, max_len %d", who,
+                  std::get<0>(kv.first), max_len);
   return P2P_OK;
 }
 

@@ -23,6 +23,13 @@ void lib_free(void* p, size_t bytes);
 int32_t* ctx_dev_err(const p2p_ctx* ctx);  // the device error word p2p_sync reports
 int32_t debug_wait_deficit();               // p2p_debug_set_wait_deficit's current value
 
+// A rope table this context built knows its rows: it must hold max_len of them.
+p2p_status ctx_check_rope(p2p_ctx* ctx, const void* rope, int32_t max_len, const char* who);
+// serve_api.cu: the host-side checks of a cache layout, and the layout as the kernels take it.
+p2p_status make_kv_view(p2p_ctx* ctx, const p2p_kv_layout* lay, int32_t hkv, const void* k,
+                        const void* v, int64_t kv_rows, const int32_t* offsets, int32_t nseq,
+                        const char* who, KvView* out);
+
 // Argument checks shared by the ragged decode entry points (`who` prefixes the message).
 p2p_status check_ragged(p2p_ctx* ctx, const p2p_attn_params* prm, const void* qkv,
                         int64_t ld_qkv, const void* rope, const void* k_cache,

@@ -73,7 +73,7 @@ struct DecodeLayer {
 // rows start at offsets[z], past = past_dev[z], q/out rows z*ld.
 // KV-cache storage of the ragged / paged decode: f16 rows, or int8 rows dequantised as
 // f32(q) * scale with one f32 scale per tensor or per (kv head, dim) channel.
-enum KvFormat { kKvF16 = 0, kKvI8 = 1 };
+enum KvFormat { kKvF16 = 0, kKvI8 = 1, kKvQ4 = 2 };
 
 struct DecodeArgs {
   DecodeLayer layers[kMaxLayers];
@@ -247,10 +247,110 @@ struct FlashArgs {
   int32_t num_sms;       // non-causal: > 0 lets the last partial wave run as one-tile CTAs
 };
 
+// ---- caches of any layout (kv_append.cu, attn_kv.cu) ------------------------------------------
+constexpr int kQ4UnitBytes = 36;  // one (token, kv head): 32 bytes of codes, f16 scale, f16 lo
+constexpr int64_t q4_row_bytes(int hkv) { return (int64_t(hkv) * kQ4UnitBytes + 15) / 16 * 16; }
+// Bytes of one cached token row (all kv heads) of format f.
+constexpr int64_t kv_row_bytes(int format, int hkv) {
+  return format == kKvQ4 ? q4_row_bytes(hkv) : int64_t(hkv) * 64 * (format == kKvI8 ? 1 : 2);
+}
+struct KvView {
+  unsigned char* k;
+  unsigned char* v;
+  int64_t kv_rows;         // rows (contiguous) or pages (paged)
+  int64_t row_bytes;       // kv_row_bytes(format, hkv)
+  const int32_t* offsets;  // contiguous: first row of each sequence
+  const int32_t* table;    // paged (nullptr: contiguous): [nseq][max_blocks]
+  int32_t max_blocks, shift;
+  int32_t format, hkv;
+  const float* k_scale;  // int8
+  const float* v_scale;
+  int32_t per_channel;
+};
+// Ragged rows: those of sequence i are row_start[i] .. row_start[i+1]-1 at positions past[i]
+// and up; row_start nullptr: one row per sequence.
+struct ChunkIndex {
+  const int32_t* past;
+  const int32_t* row_start;
+  int32_t nseq;
+  int64_t n_rows;
+  int32_t max_len;
+};
+struct AppendArgs {
+  KvView kv;
+  ChunkIndex at;
+  const __half* qkv;
+  int64_t ld_qkv;
+  const __half* norm_w;
+  const __half* rope;
+  __half* q_out;
+  int64_t ld_q;
+  int32_t hq;
+  float eps;
+  int32_t* err;
+};
+cudaError_t launch_kv_append(const AppendArgs& a, cudaStream_t s);
+struct ReadArgs {
+  KvView kv;
+  ChunkIndex at;
+  __half* k_out;
+  __half* v_out;
+  int32_t* err;
+};
+cudaError_t launch_kv_read(const ReadArgs& a, cudaStream_t s);
+cudaError_t launch_quantize_q4(const void* src, void* dst, int64_t rows, int hkv,
+                               cudaStream_t s);
+struct AttnKvArgs {
+  KvView kv;
+  ChunkIndex at;
+  const __half* q;  // rotated query rows; fused decode: qkv rows
+  int64_t ld_q;
+  __half* out;
+  int64_t ld_o;
+  int32_t hq;
+  float scale_log2;
+  int32_t* err;
+  // fused decode (one row per sequence): q, k, v are normed and rotated here and the new token
+  // is appended
+  int32_t fused;
+  const __half* norm_w;
+  const __half* rope;
+  float eps;
+};
+cudaError_t launch_attn_kv(const AttnKvArgs& a, cudaStream_t s);
+
+// ---- logits_pick.cu ---------------------------------------------------------------------------
+constexpr int kMaxVocab = 400000;
+struct LogitsArgs {
+  const void* logits;
+  void* out;
+  int32_t* tok;
+  int64_t ld, ld_out;
+  int32_t rows, vocab;
+  int32_t advance;
+  int32_t* hist;
+  int32_t* hist_len;
+  const int32_t* prompt_len;
+  int32_t* past;
+  int64_t ld_hist;
+  int32_t hist_cap, n_bias;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_start;
+  const int32_t* bias_tok;
+  const float* bias_val;
+  const uint32_t* mask;
+  int64_t ld_mask;
+  int32_t* err;
+};
+cudaError_t launch_logits_pick(const LogitsArgs& a, int dtype, cudaStream_t s);
+
 // Device error word bits.
 constexpr int kErrPosBeyondCache = 1;
 constexpr int kErrTimeout = 2;  // a bounded device-side wait ran out; that work was not written
 constexpr int kErrOutTokFull = 4;  // argmax_step: the step index reached out_tok's capacity
+constexpr int kErrHistFull = 16;  // logits_pick: a sequence's history reached its capacity
 constexpr int kErrLayout = 8;  // a kernel found its shared memory misplaced; it wrote nothing
 cudaError_t launch_flash(const FlashArgs& a, cudaStream_t s);
 

@@ -1,0 +1,944 @@
+"""The batched serving operators on a B200 against plain implementations in 64 bits: ragged
+appends into f16 / int8 / 4-bit, contiguous and paged caches, reading them back, attention of
+single tokens over 4-bit caches and of prompt chunks over every format, the tokens of a batch of
+logits -- and all of them in the order a server runs them, captured and replayed."""
+import itertools
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+D, UNIT = 64, 36
+FMTS = ("f16", "i8", "q4")
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import p2p_b200
+    c = p2p_b200.Context(0)
+    yield c
+    c.close()
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def i32(x):
+    return torch.tensor(list(x), dtype=torch.int32, device="cuda")
+
+
+def randh(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda", dtype=torch.float16)
+
+
+def row_bytes(hkv):
+    return (hkv * UNIT + 15) // 16 * 16
+
+
+# ---- plain 4-bit rows ---------------------------------------------------------------------------
+def quant4(x):
+    """f16 [..., hkv, 64] -> uint8 [..., row bytes], the rule of the header in torch."""
+    xf = x.float()
+    lo, hi = xf.amin(-1, keepdim=True), xf.amax(-1, keepdim=True)
+    sc = ((hi - lo) / 15).half()
+    s = sc.float()
+    code = torch.where(s > 0, (xf - lo) / s, torch.zeros_like(xf)).round().clamp(0, 15)
+    code = code.to(torch.uint8)
+    unit = torch.cat([code[..., 0::2] | (code[..., 1::2] << 4), sc.view(torch.uint8),
+                      lo.half().view(torch.uint8)], -1)
+    flat = unit.reshape(*x.shape[:-2], -1)
+    out = torch.zeros(*flat.shape[:-1], row_bytes(x.shape[-2]), dtype=torch.uint8, device="cuda")
+    out[..., :flat.shape[-1]] = flat
+    return out
+
+
+def quant8(x, scale, hkv):
+    s = scale.view(hkv, D) if scale.numel() > 1 else scale
+    return (x.float() / s).round().clamp(-128, 127).to(torch.int8)
+
+
+def values64(rows, fmt, hkv, scale):
+    """Cache rows -> their values in f64 [..., hkv, 64]."""
+    if fmt == "f16":
+        return rows.double()
+    if fmt == "i8":
+        return rows.double() * (scale.double().view(hkv, D) if scale.numel() > 1
+                                else scale.double())
+    u = rows[..., :hkv * UNIT].reshape(*rows.shape[:-1], hkv, UNIT)
+    code = torch.stack([u[..., :32] & 15, u[..., :32] >> 4], -1).flatten(-2).double()
+    par = u[..., 32:].contiguous().view(torch.float16).double()
+    return code * par[..., :1] + par[..., 1:]
+
+
+class Cache:
+    """A cache of any layout with `lens` rows reserved per sequence, filled with random rows (so
+    that what lies behind a sequence is not zero)."""
+
+    def __init__(self, seed, fmt, page, hq, hkv, lens, spare=3, per_channel=True, amp=1.0):
+        import p2p_b200
+        g = gen(seed)
+        self.fmt, self.page, self.hkv, self.hq = fmt, page, hkv, hq
+        self.prm = p2p_b200.Params(hq, hkv)
+        n = len(lens)
+        self.table = self.offsets = None
+        if page:
+            need = [max(1, -(-m // page)) for m in lens]
+            pages = sum(need) + spare
+            order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+            self.table = torch.full((n, max(need)), 10**6, dtype=torch.int32, device="cuda")
+            at = 0
+            for i, b in enumerate(need):
+                self.table[i, :b] = order[at:at + b]
+                at += b
+            lead = (pages, page)
+        else:
+            starts = np.concatenate([[1], 1 + np.cumsum([m + 2 for m in lens])])
+            self.offsets = i32(starts[:-1])
+            lead = (int(starts[-1]) + spare,)
+        self.ks = self.vs = None
+        if fmt == "i8":
+            m = hkv * D if per_channel else 1
+            self.ks, self.vs = (0.01 + 0.02 * torch.rand(m, generator=g, device="cuda")
+                                for _ in range(2))
+        k, v = (amp * randh(g, *lead, hkv, D) for _ in range(2))
+        self.k, self.v = self.stored(k, self.ks), self.stored(v, self.vs)
+
+    def stored(self, x, scale):
+        return {"f16": lambda: x.clone(), "i8": lambda: quant8(x, scale, self.hkv),
+                "q4": lambda: quant4(x)}[self.fmt]()
+
+    def kw(self):
+        d = {"offsets": self.offsets, "block_table": self.table}
+        if self.fmt == "i8":
+            d |= {"k_scale": self.ks, "v_scale": self.vs}
+        return d
+
+    def at(self, i, pos):
+        pos = torch.as_tensor(pos, device="cuda")
+        if self.table is not None:
+            return self.table[i].long()[pos // self.page], pos % self.page
+        return (self.offsets[i].long() + pos,)
+
+    def keys64(self, i, n):
+        at = self.at(i, torch.arange(n, device="cuda"))
+        return (values64(self.k[at], self.fmt, self.hkv, self.ks),
+                values64(self.v[at], self.fmt, self.hkv, self.vs))
+
+
+def rope_table(n, theta=1e6):
+    i = torch.arange(32, dtype=torch.float64, device="cuda")
+    a = torch.arange(n, dtype=torch.float64, device="cuda")[:, None] * theta ** (-i / 32)
+    return torch.cat([a.cos(), a.sin()], 1).float().half()
+
+
+def starts_of(lens):
+    return i32(np.concatenate([[0], np.cumsum(lens)]))
+
+
+# ---- append and read back -------------------------------------------------------------------------
+def prep(ctx, prm, qkv, nw, rope, pos0):
+    """QK_PREP of one sequence's rows by the framework's own operator (pinned to the shader)."""
+    m = qkv.shape[0]
+    q = torch.zeros(m, prm.num_heads * D, dtype=torch.float16, device="cuda")
+    k = torch.zeros(pos0 + m, prm.num_kv_heads, D, dtype=torch.float16, device="cuda")
+    v = torch.zeros_like(k)
+    ctx.qk_prep(prm, qkv.contiguous(), nw, rope, q, k, v, pos0=pos0)
+    return q, k[pos0:], v[pos0:]
+
+
+APPENDS = [
+    # heads, page, chunk rows, past
+    ((32, 8), 16, [1], [0]),
+    ((32, 8), 16, [1], [777]),
+    ((16, 8), 0, [33, 1, 0, 7], [0, 15, 9, 100]),
+    ((16, 2), 64, [130, 3, 64], [0, 63, 1]),
+    ((12, 12), 32, [5, 32, 31, 33], [0, 32, 31, 33]),
+    ((6, 3), 16, [17, 2], [14, 31]),
+    ((8, 1), 0, [40], [3]),
+    ((64, 8), 128, [9], [1000]),
+    ((8, 8), 16, [1] * 70, list(range(0, 700, 10))),
+]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("case", APPENDS, ids=lambda c: f"{c[0]}-{c[1]}-{len(c[2])}")
+def test_append_is_qk_prep_into_any_cache(ctx, fmt, case):
+    (hq, hkv), page, rows, past = case
+    total = [p + r for p, r in zip(past, rows)]
+    c = Cache(11, fmt, page, hq, hkv, total)
+    g = gen(12)
+    new, pad = sum(rows), 5
+    wide = randh(g, new + pad, (hq + 2 * hkv) * D + 24)  # rows with a stride, rows behind the last
+    qkv = wide[:, :(hq + 2 * hkv) * D]
+    nw = (1 + 0.1 * torch.randn(2 * D, generator=g, device="cuda")).half()
+    rope = rope_table(max(total) + 1)
+    q_wide = torch.full((new + pad, hq * D + 8), 7.0, dtype=torch.float16, device="cuda")
+    want_k, want_v = c.k.clone(), c.v.clone()
+    want_q = q_wide.clone()
+    at = 0
+    for i, (p, r) in enumerate(zip(past, rows)):
+        if r:
+            q, k, v = prep(ctx, c.prm, qkv[at:at + r], nw, rope, p)
+            want_q[at:at + r, :hq * D] = q
+            idx = c.at(i, p + torch.arange(r, device="cuda"))
+            for pool, x, s in ((want_k, k, c.ks), (want_v, v, c.vs)):
+                used = hkv * UNIT if fmt == "q4" else hkv
+                pool[(*idx, slice(0, used))] = c.stored(x, s)[:, :used]
+        at += r
+    ctx.kv_append(c.prm, qkv, nw, rope, c.k, c.v, i32(past), starts_of(rows),
+                  max_len=max(total), q_out=q_wide[:, :hq * D], **c.kw())
+    ctx.sync()
+    assert torch.equal(q_wide, want_q)
+    assert torch.equal(c.k, want_k) and torch.equal(c.v, want_v)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_append_without_norm_or_q(ctx, fmt):
+    c = Cache(1, fmt, 16, 8, 2, [40], per_channel=False)
+    qkv, rope = randh(gen(2), 40, 12 * D), rope_table(40)
+    _, k, v = prep(ctx, c.prm, qkv, None, rope, 0)
+    ctx.kv_append(c.prm, qkv, None, rope, c.k, c.v, i32([0]), i32([0, 40]), max_len=40, **c.kw())
+    ctx.sync()
+    used = slice(0, 2 * UNIT if fmt == "q4" else 2)
+    at = c.at(0, torch.arange(40, device="cuda"))
+    assert torch.equal(c.k[(*at, used)], c.stored(k, c.ks)[:, used])
+    assert torch.equal(c.v[(*at, used)], c.stored(v, c.vs)[:, used])
+
+
+@pytest.mark.parametrize("fmt,page", list(itertools.product(FMTS, (0, 16, 64))))
+@pytest.mark.parametrize("heads", [(32, 8), (6, 3), (8, 1), (12, 12)])
+def test_read_back(ctx, fmt, page, heads):
+    hq, hkv = heads
+    first, rows = [0, 3, 17, 40], [1, 0, 50, 33]
+    c = Cache(3, fmt, page, hq, hkv, [f + r for f, r in zip(first, rows)])
+    n = sum(rows)
+    k = torch.full((n + 2, hkv, D), 7.0, dtype=torch.float16, device="cuda")
+    v = k.clone()
+    ctx.kv_read(c.prm, c.k, c.v, i32(first), starts_of(rows), k, v, max_len=100, **c.kw())
+    only = torch.full_like(k, 7.0)
+    ctx.kv_read(c.prm, c.k, c.v, i32(first), starts_of(rows), None, only, max_len=100, **c.kw())
+    ctx.sync()
+    at = 0
+    for i, (f, r) in enumerate(zip(first, rows)):
+        wk, wv = c.keys64(i, f + r)
+        # the product of a code (or int8 value) and the scale and the sum with lo round to f32 once
+        # (2^-24) before f16: equal but for ties of f16, which f64 sees the same way
+        assert torch.equal(k[at:at + r], wk[f:].float().half())
+        assert torch.equal(v[at:at + r], wv[f:].float().half())
+        at += r
+    assert (k[n:] == 7).all() and (v[n:] == 7).all()
+    assert torch.equal(only, v)
+
+
+@pytest.mark.parametrize("hkv", [1, 2, 3, 5, 8, 16])
+def test_quantize_q4(ctx, hkv):
+    x = randh(gen(5), 41, hkv, D)
+    x[0] = 0
+    x[1] = 3.25            # a constant row: scale 0
+    x[2, :, ::2] = 65504.0
+    x[2, :, 1::2] = -65504.0
+    x[3] *= 2.0 ** -20     # subnormal values
+    x[4, :, 0] = -0.0
+    x[5, :, 1:] = 1.0
+    x[5, :, 0] = 1.0 + 2.0 ** -10
+    got = ctx.kv_quantize_q4(x)
+    ctx.sync()
+    assert torch.equal(got, quant4(x))
+    # half a step (plus the scale's own rounding over 15 steps) of every value
+    val = values64(got, "q4", hkv, None)
+    step = got[:, :hkv * UNIT].view(41, hkv, UNIT)[..., 32:34].contiguous().view(
+        torch.float16).double()
+    err = (val - x.double()).abs()
+    span = (x.double().amax(-1, keepdim=True) - x.double().amin(-1, keepdim=True))
+    assert (err <= step * 0.5 + span * 2.0 ** -11 + 15 * 2.0 ** -25).all()
+
+
+# ---- attention ------------------------------------------------------------------------------------
+def attention64(c, q, past, rows, chunk):
+    """out and how far a kernel may be from it, [rows][hq][64] in f64 on the GPU.
+
+    The bound counts roundings of half a step: the weights to f16 after an exp2 of 2^-10 relative
+    error (2^-11 + 2^-10) and, for chunks, the cached values to f16 (2^-11 each: a key's shifts its
+    score by up to 2^-11 sum |q k| / 8 and so its weight by that share), and out to f16.  An error
+    e of the weights' own shares moves out by at most sum p |v - out| e.  f32 sums of the scores
+    (64 products, 2^-24 each, twice for the scale and offset of a 4-bit row) and of the weights
+    are below 2^-18 of the magnitudes."""
+    outs, tols = [], []
+    at = 0
+    for i, (p, r) in enumerate(zip(past, rows)):
+        if r == 0:
+            continue
+        k, v = c.keys64(i, p + r)
+        grp = c.hq // c.hkv
+        k, v = (t.repeat_interleave(grp, 1).permute(1, 0, 2) for t in (k, v))  # [hq][keys][64]
+        qi = q[at:at + r].double().view(r, c.hq, D).permute(1, 0, 2)
+        at += r
+        s = qi @ k.transpose(1, 2) / 8
+        mag = qi.abs() @ k.abs().transpose(1, 2) / 8
+        hidden = torch.arange(p + r, device="cuda")[None] > \
+            (p + torch.arange(r, device="cuda"))[:, None]
+        w = torch.softmax(s.masked_fill(hidden, -math.inf), -1)
+        o = w @ v
+        e = 2.0 ** -11 + 2.0 ** -10 + mag * ((2.0 ** -11 if chunk else 0) + 2.0 ** -18)
+        # sum w e |v - o| <= sum w e |v| + |o| sum w e
+        t = (w * e) @ v.abs() + o.abs() * (w * e).sum(-1, keepdim=True)
+        t = t + (w @ v.abs()) * ((2.0 ** -11 if chunk else 0) + 2.0 ** -16)
+        t = t + o.abs() * 2.0 ** -11 + 2.0 ** -24
+        outs.append(o.permute(1, 0, 2))
+        tols.append(t.permute(1, 0, 2))
+    return torch.cat(outs).flatten(1), torch.cat(tols).flatten(1)
+
+
+def assert_within(got, want, tol, what=""):
+    err = (got.double() - want).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} beyond the bound, worst "
+                           f"{float(err.max()):.3e}, {float((err / tol).max()):.2f} of the bound")
+
+
+DECODES = [
+    # heads, page, past
+    ((32, 8), 0, [0]),
+    ((32, 8), 16, [0, 1, 15, 16, 17, 30, 31, 32, 63, 64, 65]),
+    ((32, 8), 0, [1337]),
+    ((32, 8), 16, [4099, 5, 700, 0, 2048]),
+    ((16, 8), 64, [255, 256, 257]),
+    ((16, 2), 16, [333, 40]),
+    ((8, 8), 32, [100, 1000]),
+    ((64, 8), 16, [513, 3]),
+    ((12, 12), 16, [200, 31]),
+    ((6, 3), 0, [77, 500]),
+    ((8, 1), 128, [1500]),
+    ((24, 12), 16, [129]),
+    ((32, 32), 64, [300, 64]),
+    ((40, 20), 0, [90, 21]),
+    ((32, 8), 4096, [9000]),
+    ((32, 8), 16, [20000]),
+    ((16, 8), 16, [(37 * i) % 400 for i in range(200)]),
+]
+
+
+@pytest.mark.parametrize("case", DECODES, ids=lambda c: f"{c[0]}-{c[1]}-{len(c[2])}x{max(c[2])}")
+def test_decode_q4(ctx, case):
+    (hq, hkv), page, past = case
+    n = len(past)
+    c = Cache(21, "q4", page, hq, hkv, [p + 1 for p in past])
+    q = randh(gen(22), n, hq * D + 8)[:, :hq * D]
+    out = torch.full((n + 1, hq * D + 16), 7.0, dtype=torch.float16, device="cuda")
+    ctx.attn_decode_kv(c.prm, q, None, None, c.k, c.v, i32(past), out[:, :hq * D],
+                       max_past=max(past), fused_prep=False, **c.kw())
+    ctx.sync()
+    want, tol = attention64(c, q, past, [1] * n, False)
+    assert_within(out[:n, :hq * D], want, tol)
+    assert (out[n:] == 7).all() and (out[:, hq * D:] == 7).all()
+
+
+@pytest.mark.parametrize("amp", [1e-4, 30.0, 2000.0])
+def test_decode_q4_ranges(ctx, amp):
+    """Caches of tiny and of large values: the scales' range."""
+    c = Cache(23, "q4", 16, 16, 4, [600, 50], amp=amp)
+    q = randh(gen(24), 2, 16 * D) * (0.05 if amp > 1 else 1.0)
+    out = torch.zeros_like(q)
+    ctx.attn_decode_kv(c.prm, q, None, None, c.k, c.v, i32([599, 49]), out, max_past=599,
+                       fused_prep=False, **c.kw())
+    ctx.sync()
+    want, tol = attention64(c, q, [599, 49], [1, 1], False)
+    # f16 weights times the rows' scales have an absolute floor of 2^-27 in a code's weight: 15
+    # codes of 2^-27 for each key whose weight counts
+    assert_within(out, want, tol + 15 * 2.0 ** -27 * 600 ** 0.5)
+
+
+@pytest.mark.parametrize("case", [c for c in DECODES if len(c[2]) < 20],
+                         ids=lambda c: f"{c[0]}-{c[1]}-{len(c[2])}x{max(c[2])}")
+def test_decode_q4_fused_is_append_then_attend(ctx, case):
+    (hq, hkv), page, past = case
+    n = len(past)
+    a = Cache(25, "q4", page, hq, hkv, [p + 1 for p in past])
+    b = Cache(25, "q4", page, hq, hkv, [p + 1 for p in past])
+    g = gen(26)
+    qkv = randh(g, n, (hq + 2 * hkv) * D)
+    nw = (1 + 0.1 * torch.randn(2 * D, generator=g, device="cuda")).half()
+    rope = rope_table(max(past) + 1)
+    q, out, out2 = (torch.zeros(n, hq * D, dtype=torch.float16, device="cuda") for _ in range(3))
+    ctx.kv_append(a.prm, qkv, nw, rope, a.k, a.v, i32(past), i32(range(n + 1)),
+                  max_len=max(past) + 1, q_out=q, **a.kw())
+    ctx.attn_decode_kv(a.prm, q, None, None, a.k, a.v, i32(past), out, max_past=max(past),
+                       fused_prep=False, **a.kw())
+    ctx.attn_decode_kv(b.prm, qkv, nw, rope, b.k, b.v, i32(past), out2, max_past=max(past),
+                       fused_prep=True, **b.kw())
+    ctx.sync()
+    assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+    assert torch.equal(out, out2)
+    want, tol = attention64(a, q, past, [1] * n, False)
+    assert_within(out2, want, tol)
+
+
+CHUNKS = [
+    # heads, page, rows, past
+    ((32, 8), 16, [1], [0]),
+    ((32, 8), 16, [5, 1, 0, 2, 33], [40, 0, 7, 1000, 64]),
+    ((32, 8), 64, [129], [0]),
+    ((32, 8), 16, [128, 127, 31, 32], [0, 1, 97, 128]),
+    ((32, 8), 16, [300], [777]),
+    ((16, 8), 0, [64, 63, 65, 200], [0, 65, 63, 10]),
+    ((16, 2), 32, [40, 3], [500, 2000]),
+    ((8, 8), 16, [150, 6], [33, 128]),
+    ((12, 12), 64, [257], [0]),
+    ((6, 3), 0, [77], [130]),
+    ((8, 1), 128, [50, 16], [0, 300]),
+    ((64, 8), 16, [17, 48], [100, 15]),
+    ((32, 8), 16, [3], [9000]),
+    ((16, 8), 16, [4] * 40, [(53 * i) % 300 for i in range(40)]),
+    ((24, 12), 16, [1024], [100]),
+]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("case", CHUNKS, ids=lambda c: f"{c[0]}-{c[1]}-{len(c[2])}x{max(c[2])}")
+def test_chunk(ctx, fmt, case):
+    (hq, hkv), page, rows, past = case
+    total = [p + r for p, r in zip(past, rows)]
+    c = Cache(31, fmt, page, hq, hkv, total, per_channel=page != 64)
+    n = sum(rows)
+    q = randh(gen(32), n + 3, hq * D + 16)[:, :hq * D]
+    out = torch.full((n + 3, hq * D + 8), 7.0, dtype=torch.float16, device="cuda")
+    ctx.attn_chunk_kv(c.prm, q, c.k, c.v, i32(past), starts_of(rows), out[:, :hq * D],
+                      max_len=max(total), **c.kw())
+    ctx.sync()
+    want, tol = attention64(c, q, past, rows, True)
+    assert_within(out[:n, :hq * D], want, tol)
+    assert (out[n:] == 7).all() and (out[:, hq * D:] == 7).all()
+
+
+def test_rows_behind_a_sequence_do_not_reach_it(ctx):
+    """NaN and infinities behind the sequences' ends (f16 caches) and in their pages' tails."""
+    for page in (0, 64):
+        c = Cache(33, "f16", page, 8, 4, [70, 5])
+        wipe_k, wipe_v = torch.full_like(c.k, math.nan), torch.full_like(c.v, math.inf)
+        for i, m in enumerate([70, 5]):
+            at = c.at(i, torch.arange(m, device="cuda"))
+            wipe_k[at], wipe_v[at] = c.k[at], c.v[at]
+        c.k, c.v = wipe_k, wipe_v
+        q = randh(gen(34), 12, 8 * D)
+        out = torch.zeros_like(q)
+        ctx.attn_chunk_kv(c.prm, q, c.k, c.v, i32([60, 3]), i32([0, 10, 12]), out, max_len=70,
+                          **c.kw())
+        ctx.sync()
+        want, tol = attention64(c, q, [60, 3], [10, 2], True)
+        assert_within(out, want, tol)
+
+
+# ---- refusals on the device -------------------------------------------------------------------------
+@pytest.mark.parametrize("op", ["append", "read", "chunk", "decode", "fused"])
+@pytest.mark.parametrize("page", [0, 16])
+def test_bad_sequences_are_skipped(ctx, op, page):
+    """Sequence 1 does not fit (too long, then a bad page or offset): it is left alone and
+    reported; its neighbours are computed."""
+    import p2p_b200
+    hq, hkv = 8, 2
+    rows = [1, 1, 1] if op in ("decode", "fused") else [20, 9, 3]
+    past = [5, 40, 33]
+    total = [p + r for p, r in zip(past, rows)]
+    for fault in ("length", "place"):
+        c = Cache(41, "q4", page, hq, hkv, total)
+        good_k, good_v = c.k.clone(), c.v.clone()
+        p = list(past)
+        if fault == "length":
+            p[1] = 60 if op != "read" else -1
+        elif page:
+            c.table[1, 2] = len(c.k)  # the page behind the pool
+        else:
+            c.offsets[1] = len(c.k) - 10
+        max_len = 59
+        g = gen(42)
+        n = sum(rows)
+        qkv = randh(g, n, (hq + 2 * hkv) * D)
+        rope = rope_table(max_len)
+        out = torch.full((n, hq * D), 7.0, dtype=torch.float16, device="cuda")
+        with pytest.raises(p2p_b200.KvFullError):
+            if op == "append":
+                ctx.kv_append(c.prm, qkv, None, rope, c.k, c.v, i32(p), starts_of(rows),
+                              max_len=max_len, q_out=out, **c.kw())
+            elif op == "read":
+                k = torch.full((n, hkv, D), 7.0, dtype=torch.float16, device="cuda")
+                ctx.kv_read(c.prm, c.k, c.v, i32(p), starts_of(rows), k, None, max_len=max_len,
+                            **c.kw())
+            elif op == "chunk":
+                ctx.attn_chunk_kv(c.prm, qkv[:, :hq * D].contiguous(), c.k, c.v, i32(p),
+                                  starts_of(rows), out, max_len=max_len, **c.kw())
+            else:
+                ctx.attn_decode_kv(c.prm, qkv, None, rope, c.k, c.v, i32(p), out,
+                                   max_past=47, fused_prep=op == "fused", **c.kw())
+            ctx.sync()
+        ctx.sync()  # reported once
+        a, b = rows[0], rows[0] + rows[1]
+        if op == "read":
+            assert torch.equal(k[:a], c.keys64(0, total[0])[0][p[0]:].float().half())
+            assert torch.equal(k[b:], c.keys64(2, total[2])[0][p[2]:].float().half())
+            # paged: rows 40 .. 47 of the bad page are skipped, row 48 is in the next page
+            if fault == "length" or not page:
+                assert (k[a:b] == 7).all()
+            else:
+                assert (k[a:b - 1] == 7).all()
+            continue
+        if op in ("append", "fused"):
+            for i in (0, 2):
+                at = c.at(i, p[i] + torch.arange(rows[i], device="cuda"))
+                assert not torch.equal(c.k[at], good_k[at])
+                c.k[at], c.v[at] = good_k[at], good_v[at]
+            if op == "append" and page and fault == "place":
+                at = c.at(1, torch.tensor([48], device="cuda"))  # its last row is in a good page
+                c.k[at], c.v[at] = good_k[at], good_v[at]
+            assert torch.equal(c.k, good_k) and torch.equal(c.v, good_v)
+        if op == "append":
+            assert not (out[:a] == 7).any() and not (out[b:] == 7).any()
+            assert (out[a:b - 1] == 7).all()
+            continue
+        assert (out[a:b] == 7).all()
+        if op != "fused":
+            q = qkv[:, :hq * D]
+            for i, s in ((0, slice(0, a)), (2, slice(b, n))):
+                one = Cache(41, "q4", page, hq, hkv, total)
+                one.k, one.v = c.k, c.v
+                if page:
+                    one.table = c.table[i:i + 1]
+                else:
+                    one.offsets = c.offsets[i:i + 1]
+                want, tol = attention64(one, q[s], [p[i]], [rows[i]], True)
+                assert_within(out[s], want, tol, f"sequence {i}")
+
+
+def test_host_refusals(ctx):
+    import p2p_b200
+    c = Cache(43, "q4", 16, 8, 2, [40])
+    q = randh(gen(44), 4, 12 * D)
+    out = torch.zeros(4, 8 * D, dtype=torch.float16, device="cuda")
+    rope = rope_table(40)
+    E = p2p_b200.P2PError
+    ok = dict(max_len=40, **c.kw())
+    rs, z = i32([0, 4]), i32([0])
+
+    def refused(fn, *a, **k):
+        with pytest.raises(E) as e:
+            fn(*a, **k)
+        assert e.value.status in (1, 7), e.value
+    refused(ctx.attn_chunk_kv, c.prm, q.float(), c.k, c.v, z, rs, out, **ok)
+    refused(ctx.attn_chunk_kv, c.prm, q[:, :64], c.k, c.v, z, rs, out, **ok)
+    refused(ctx.attn_chunk_kv, c.prm, q, c.k, c.v[1:], z, rs, out, **ok)
+    refused(ctx.attn_chunk_kv, c.prm, q, c.k, c.v, z.long(), rs, out, **ok)
+    refused(ctx.attn_chunk_kv, c.prm, q, c.k, c.v, z, z, out, **ok)             # row_start short
+    refused(ctx.attn_chunk_kv, c.prm, q, c.k, c.v, z, rs, out[:2], **ok)
+    refused(ctx.attn_chunk_kv, c.prm, q, c.k, c.v, z, rs, out, max_len=-1, **c.kw())
+    refused(ctx.attn_chunk_kv, c.prm, q, c.k, c.v, z, rs, out, max_len=40, offsets=z)
+    shifted = torch.zeros(4 * 12 * D + 8, dtype=torch.float16, device="cuda")[1:]
+    refused(ctx.attn_chunk_kv, c.prm, shifted[:4 * 12 * D].view(4, 12 * D), c.k, c.v, z, rs, out,
+            **ok)
+    refused(ctx.attn_chunk_kv, p2p_b200.Params(6, 2), q, c.k, c.v, z, rs, out, **ok)  # group 3
+    refused(ctx.attn_chunk_kv, p2p_b200.Params(8, 2, dtype=torch.float32), q, c.k, c.v, z, rs, out,
+            **ok)
+    refused(ctx.kv_append, c.prm, q, None, rope[:20], c.k, c.v, z, rs, **ok)    # rope too short
+    refused(ctx.kv_append, c.prm, q, None, ctx.rope_table(39), c.k, c.v, z, rs, **ok)
+    refused(ctx.kv_append, c.prm, q, rope[0], rope, c.k, c.v, z, rs, **ok)      # 64 norm weights
+    refused(ctx.kv_read, c.prm, c.k, c.v, z, rs, None, None, **ok)
+    refused(ctx.attn_decode_kv, c.prm, q, None, rope, c.k, c.v, z, out, max_past=40 + 16, **c.kw())
+    refused(ctx.kv_quantize_q4, q)
+    p = Cache(43, "q4", 0, 8, 2, [40])
+    refused(ctx.attn_chunk_kv, p.prm, q, p.k, p.v, z, rs, out, max_len=40)      # no offsets
+    t8 = Cache(43, "i8", 16, 8, 2, [40])
+    refused(ctx.attn_chunk_kv, t8.prm, q, t8.k, t8.v, z, rs, out, max_len=40, block_table=t8.table)
+
+
+def test_empty_calls(ctx):
+    c = Cache(45, "q4", 16, 8, 2, [40])
+    none = torch.zeros(0, 12 * D, dtype=torch.float16, device="cuda")
+    q = randh(gen(1), 3, 12 * D)
+    out = torch.full((3, 8 * D), 7.0, dtype=torch.float16, device="cuda")
+    empty, rope = i32([]), rope_table(40)
+    ctx.attn_chunk_kv(c.prm, none, c.k, c.v, i32([0]), i32([0, 0]), out, max_len=40, **c.kw())
+    ctx.attn_chunk_kv(c.prm, q, c.k, c.v, i32([0]), i32([0, 0]), out, max_len=40, **c.kw())
+    ctx.attn_chunk_kv(c.prm, q, c.k, c.v, empty, i32([0]), out, max_len=40, **c.kw())
+    ctx.kv_append(c.prm, q, None, rope, c.k, c.v, i32([0]), i32([0, 0]), max_len=40, q_out=out,
+                  **c.kw())
+    ctx.attn_decode_kv(c.prm, q, None, None, c.k, c.v, empty, out, max_past=39, fused_prep=False,
+                       **c.kw())
+    ctx.sync()
+    assert (out == 7).all()
+
+
+# ---- logits -----------------------------------------------------------------------------------------
+def plain_logits(x, hist, hist_len, prompt_len, rep, pres, freq, bias, mask, dt):
+    """One rounding per operation in f32 (numpy), as the header states it."""
+    y = x.float().cpu().numpy().copy()
+    n, vocab = y.shape
+    for i in range(n):
+        h = hist[i][:hist_len[i]] if hist is not None else np.zeros(0, np.int64)
+        made = h[min(max(prompt_len[i], 0), len(h)):] if prompt_len is not None else h
+        inside = h[(h >= 0) & (h < vocab)]
+        made = made[(made >= 0) & (made < vocab)]
+        line = y[i]
+        s = np.unique(inside)
+        if rep is not None:
+            line[s] = np.where(line[s] > 0, line[s] / rep[i], line[s] * rep[i])
+        m, c = np.unique(made, return_counts=True)
+        f = np.float32(freq[i]) if freq is not None else np.float32(0)
+        p = np.float32(pres[i]) if pres is not None else np.float32(0)
+        line[m] = (line[m] - f * c.astype(np.float32)) - p
+        if bias is not None:
+            for t, b in bias[i]:
+                if 0 <= t < vocab:
+                    line[t] = line[t] + np.float32(b)
+        if mask is not None:
+            line[~mask[i]] = -np.inf
+    out = torch.from_numpy(y).to(dt).cuda()
+    toks = []
+    for i in range(n):
+        line = out[i].float().cpu().numpy()
+        live = np.where(np.isnan(line), -np.inf, line)
+        toks.append(int(np.argmax(live)) if live.max() > -np.inf else -1)
+    return out, toks
+
+
+def same_bits(a, b):
+    """Equal values, NaN where NaN."""
+    return bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+LOGITS = [
+    # rows, vocab, history, biases, mask
+    (1, 1, 3, 1, True), (1, 7, 0, 0, False), (2, 31, 5, 3, True), (3, 33, 60, 5, True),
+    (1, 1000, 100, 0, False), (5, 1025, 300, 20, True), (4, 4099, 1000, 300, True),
+    (3, 65536, 2000, 50, True), (2, 131071, 4000, 10, True), (1, 262144, 50, 0, True),
+    (70, 513, 40, 4, True), (1, 400000, 10, 5, True),
+]
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.float32])
+@pytest.mark.parametrize("case", LOGITS, ids=lambda c: f"{c[0]}x{c[1]}")
+def test_logits_pick(ctx, dt, case):
+    n, vocab, cap, nb, with_mask = case
+    rng = np.random.default_rng(n * vocab)
+    g = gen(vocab)
+    for strided in (False, True):
+        wide = (3 * torch.randn(n, vocab + (5 if strided else 0), generator=g,
+                                device="cuda")).to(dt)
+        x = wide[:, :vocab]
+        x[0, vocab // 2] = math.nan
+        x[-1, vocab // 3] = math.inf if vocab > 100 else 1.0
+        out = torch.full((n, vocab + 3), 7.0, dtype=dt, device="cuda")
+        hist = rng.integers(0, vocab, (n, cap + 2))
+        hist[:, ::3] = hist[:, :1]           # one token many times
+        hist[:, 1::7] = -1                   # not a token
+        hist[:, 2::7] = vocab
+        lens = np.minimum(rng.integers(0, cap + 1, n) + cap // 2, cap)
+        lens[-1] = 0
+        plen = lens // 2
+        rep, pres, freq = (1 + rng.random(n), rng.random(n), rng.random(n) / 3)
+        rep, pres, freq = (a.astype(np.float32) for a in (rep, pres, freq))
+        rep[0] = 0.5
+        bias = [[(int(t), float(b)) for t, b in zip(rng.integers(-1, vocab + 1, nb),
+                                                    rng.standard_normal(nb) * 4)]
+                for _ in range(n)]
+        if nb > 2:
+            bias[0][2] = (bias[0][0][0], 1.25)  # the same token twice
+        mask = rng.random((n, vocab)) < 0.5 if with_mask else None
+        kw = {}
+        if nb:
+            kw["bias_start"] = starts_of([len(b) for b in bias])
+            kw["bias_tok"] = i32(t for b in bias for t, _ in b)
+            kw["bias_val"] = torch.tensor([v for b in bias for _, v in b], device="cuda")
+        if mask is not None:
+            words = (vocab + 31) // 32
+            bits = np.zeros((n, words * 32), bool)
+            bits[:, :vocab] = mask
+            packed = np.packbits(bits, axis=1, bitorder="little").view(np.int32)
+            kw["mask"] = torch.from_numpy(packed.copy()).cuda()
+        tok = torch.full((n + 1,), -7, dtype=torch.int32, device="cuda")
+        dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+        want, toks = plain_logits(x, hist, lens, plen, rep, pres, freq, bias if nb else None, mask,
+                                  dt)
+        h = dev(hist.astype(np.int32))
+        kw |= dict(hist=h, hist_len=i32(lens), prompt_len=i32(plen), repetition=dev(rep),
+                   presence=dev(pres), frequency=dev(freq))
+        ctx.logits_pick(x, tok, out=out[:, :vocab], **kw)
+        ctx.sync()
+        assert tok.tolist() == toks + [-7]
+        assert same_bits(out[:, :vocab], want)
+        assert (out[:, vocab:] == 7).all()
+        tok2 = torch.zeros_like(tok)
+        ctx.logits_pick(x, tok2, **kw)       # without an output, and in place
+        keep = wide.clone()
+        ctx.logits_pick(x, tok2, out=x, **kw)
+        ctx.sync()
+        assert tok2.tolist()[:n] == toks and same_bits(x, want)
+        assert torch.equal(wide[:, vocab:], keep[:, vocab:])
+
+
+def test_logits_without_anything_is_argmax(ctx):
+    x = randh(gen(3), 9, 5000)
+    x[0, 77] = x[0, 4000] = 9.0     # a tie: the lowest index
+    x[1] = -math.inf                # nothing left
+    x[2] = math.nan
+    x[3, 1:] = -math.inf
+    x[4] = 0.0
+    x[4, 6] = -0.0                  # equal to +0: index 0
+    tok = torch.zeros(9, dtype=torch.int32, device="cuda")
+    ctx.logits_pick(x, tok)
+    ctx.sync()
+    got = tok.tolist()
+    assert got[:5] == [77, -1, -1, 0, 0]
+    for i in range(5, 9):
+        assert got[i] == int(np.argmax(x[i].float().cpu().numpy()))
+
+
+def test_logits_masks_that_leave_one_or_none(ctx):
+    n, vocab = 3, 70000
+    x = randh(gen(4), n, vocab)
+    mask = torch.zeros(n, (vocab + 31) // 32, dtype=torch.int32, device="cuda")
+    mask[1, 69999 // 32] = 1 << (69999 % 32)
+    mask[2] = -1
+    tok = torch.zeros(n, dtype=torch.int32, device="cuda")
+    hist = torch.zeros(n, 4, dtype=torch.int32, device="cuda")
+    hist_len, past = i32([1, 1, 4]), i32([10, 20, 30])
+    import p2p_b200
+    ctx.logits_pick(x, tok, mask=mask, hist=hist, hist_len=hist_len, past=past, advance=True)
+    with pytest.raises(p2p_b200.P2PError) as e:  # row 2's history is full
+        ctx.sync()
+    assert e.value.status == 1
+    best = int(np.argmax(x[2].float().cpu().numpy()))
+    assert tok.tolist() == [-1, 69999, best]
+    assert hist_len.tolist() == [1, 2, 4] and past.tolist() == [10, 21, 30]
+    assert hist.tolist() == [[0] * 4, [0, 69999, 0, 0], [0] * 4]
+
+
+def test_logits_advance_replays(ctx):
+    """A captured pick that feeds on its own history: each replay picks the next token."""
+    vocab, steps = 3001, 12
+    x = randh(gen(6), 2, vocab)
+    hist = torch.full((2, 40), -1, dtype=torch.int32, device="cuda")
+    hist_len, past = i32([0, 3]), i32([0, 100])
+    hist[1, :3] = torch.tensor([1, 2, 2], dtype=torch.int32)
+    start_hist = hist.cpu().numpy().copy()
+    pres = torch.tensor([100.0, 100.0], device="cuda")  # a picked token never comes again
+    tok = torch.zeros(2, dtype=torch.int32, device="cuda")
+    kw = dict(hist=hist, hist_len=hist_len, past=past, presence=pres, advance=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ctx.logits_pick(x, tok, **kw)
+    for _ in range(steps):
+        graph.replay()
+    ctx.sync()
+    assert hist_len.tolist() == [steps, 3 + steps] and past.tolist() == [steps, 100 + steps]
+    h, lens = start_hist, [0, 3]
+    for _ in range(steps):
+        _, toks = plain_logits(x, h, lens, None, None, [100.0] * 2, None, None, None, x.dtype)
+        for i, t in enumerate(toks):
+            h[i, lens[i]] = t
+            lens[i] += 1
+    assert np.array_equal(h, hist.cpu().numpy())
+
+
+def test_logits_refusals(ctx):
+    import p2p_b200
+    x = randh(gen(7), 2, 100)
+    tok = torch.zeros(2, dtype=torch.int32, device="cuda")
+    f = torch.ones(2, device="cuda")
+    h = torch.zeros(2, 5, dtype=torch.int32, device="cuda")
+
+    def refused(*a, **k):
+        with pytest.raises(p2p_b200.P2PError) as e:
+            ctx.logits_pick(*a, **k)
+        assert e.value.status in (1, 7)
+    refused(x.double(), tok)
+    refused(x[0], tok)
+    refused(x, tok[:1])
+    refused(x, tok.long())
+    refused(x, tok, out=x[:, :50])
+    refused(x, tok, out=x.float())
+    refused(x, tok, hist=h)
+    refused(x, tok, prompt_len=tok)
+    refused(x, tok, repetition=f.half())
+    refused(x, tok, presence=f[:1])
+    refused(x, tok, bias_start=tok, bias_tok=tok, bias_val=f)        # needs rows + 1 starts
+    refused(x, tok, bias_start=h[0], bias_tok=tok)
+    refused(x, tok, mask=h[:, :3])
+    refused(torch.zeros(1, 400001, dtype=torch.float16, device="cuda"), tok)
+
+
+# ---- together ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", FMTS)
+def test_a_server_run(ctx, fmt):
+    """Prompts of a batch appended and attended in chunks, then captured decode steps (append,
+    attention, logits, token), replayed: every row agrees with the 64-bit attention over the
+    cache, and the tokens with the plain picks."""
+    hq, hkv, vocab, steps = 16, 4, 999, 6
+    prompts = [37, 1, 130]
+    n = len(prompts)
+    total = [p + steps + 1 for p in prompts]
+    c = Cache(51, fmt, 16, hq, hkv, total, amp=0.0)
+    prm, g = c.prm, gen(52)
+    nw = (1 + 0.1 * torch.randn(2 * D, generator=g, device="cuda")).half()
+    rope = rope_table(max(total))
+    emb = randh(g, vocab, (hq + 2 * hkv) * D)      # a token's qkv row
+    head = randh(g, hq * D, vocab) * 0.05
+    toks = torch.randint(0, vocab, (sum(prompts),), generator=g, device="cuda")
+    ml = max(total)
+    # prompts in two ragged chunks
+    cut = [p // 2 for p in prompts]
+    rows_of = np.concatenate([[0], np.cumsum(prompts)])
+    for part in range(2):
+        past = [0] * n if part == 0 else cut
+        rows = cut if part == 0 else [p - h for p, h in zip(prompts, cut)]
+        idx = np.concatenate([np.arange(rows_of[i] + past[i], rows_of[i] + past[i] + rows[i])
+                              for i in range(n)]).astype(np.int64)
+        qkv = emb[toks[torch.from_numpy(idx).cuda()]]
+        q, out = (torch.zeros(len(idx), hq * D, dtype=torch.float16, device="cuda")
+                  for _ in range(2))
+        rs, pt = starts_of(rows), i32(past)
+        ctx.kv_append(prm, qkv, nw, rope, c.k, c.v, pt, rs, max_len=ml, q_out=q, **c.kw())
+        ctx.attn_chunk_kv(prm, q, c.k, c.v, pt, rs, out, max_len=ml, **c.kw())
+        ctx.sync()
+        want, tol = attention64(c, q, past, rows, True)
+        assert_within(out, want, tol)
+    last = out[torch.tensor(np.cumsum(rows) - 1).cuda()]
+    hist = torch.full((n, max(prompts) + steps + 2), -1, dtype=torch.int32, device="cuda")
+    for i in range(n):
+        hist[i, :prompts[i]] = toks[rows_of[i]:rows_of[i + 1]].int()
+    hist_len, plen, past = i32(prompts), i32(prompts), i32([p - 1 for p in prompts])
+    kw = dict(hist=hist, hist_len=hist_len, prompt_len=plen,
+              repetition=torch.full((n,), 1.3, device="cuda"),
+              presence=torch.full((n,), 0.5, device="cuda"),
+              frequency=torch.full((n,), 0.25, device="cuda"), past=past, advance=True)
+    tok = torch.zeros(n, dtype=torch.int32, device="cuda")
+    logits = last @ head
+    first = plain_logits(logits, hist.cpu().numpy(), prompts, prompts, [np.float32(1.3)] * n,
+                         [0.5] * n, [0.25] * n, None, None, torch.float16)[1]
+    ctx.logits_pick(logits, tok, **kw)
+    ctx.sync()
+    assert tok.tolist() == first
+    # decode: past now points at the picked token's position
+    q, out = (torch.zeros(n, hq * D, dtype=torch.float16, device="cuda") for _ in range(2))
+    one = i32(range(n + 1))
+
+    def step():
+        qkv = emb[tok.long()]
+        if fmt == "q4":
+            ctx.attn_decode_kv(prm, qkv, nw, rope, c.k, c.v, past, out, max_past=ml - 1, **c.kw())
+        else:
+            ctx.kv_append(prm, qkv, nw, rope, c.k, c.v, past, one, max_len=ml, q_out=q, **c.kw())
+            ctx.attn_chunk_kv(prm, q, c.k, c.v, past, one, out, max_len=ml, **c.kw())
+        ctx.logits_pick(out @ head, tok, **kw)
+
+    keep = [t.clone() for t in (c.k, c.v, hist, hist_len, past, tok)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()  # a warm-up outside the capture: workspaces are made here
+    torch.cuda.current_stream().wait_stream(side)
+    for t, k in zip((c.k, c.v, hist, hist_len, past, tok), keep):
+        t.copy_(k)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    state = (hist.cpu().numpy().copy(), list(prompts))
+    state[0][range(n), prompts] = first
+    lens = [p + 1 for p in prompts]
+    for s in range(steps - 1):
+        before = tok.clone()
+        graph.replay()
+        ctx.sync()
+        pos = [p + s for p in prompts]
+        qs = []
+        for i in range(n):
+            qs.append(prep(ctx, prm, emb[before[i].long()][None], nw, rope, pos[i])[0])
+        want, tol = attention64(c, torch.cat(qs), pos, [1] * n, True)
+        assert_within(out, want, tol, f"step {s}")
+        ref = plain_logits(out @ head, state[0], lens, prompts, [np.float32(1.3)] * n, [0.5] * n,
+                           [0.25] * n, None, None, torch.float16)[1]
+        assert tok.tolist() == ref
+        for i, t in enumerate(ref):
+            state[0][i, lens[i]] = t
+            lens[i] += 1
+    assert np.array_equal(state[0], hist.cpu().numpy())
+    assert past.tolist() == [p + steps - 1 for p in prompts]
+    del graph
+
+
+@pytest.mark.parametrize("op", ["decode", "chunk"])
+def test_two_graphs_of_different_sizes_share_a_context(ctx, op):
+    """A small call captured, a larger one captured and run, the small one replayed."""
+    graphs, checks = [], []
+    for seed, past in ((61, [300, 20]), (62, [5000, 100, 2000, 77])):
+        c = Cache(seed, "q4", 16, 32, 8, [p + 1 for p in past])
+        n = len(past)
+        q = randh(gen(seed), n, 32 * D)
+        out = torch.zeros_like(q)
+        p, rs = i32(past), i32(range(n + 1))
+
+        def call(c=c, q=q, out=out, p=p, rs=rs, top=max(past)):
+            if op == "decode":
+                ctx.attn_decode_kv(c.prm, q, None, None, c.k, c.v, p, out, max_past=top,
+                                   fused_prep=False, **c.kw())
+            else:
+                ctx.attn_chunk_kv(c.prm, q, c.k, c.v, p, rs, out, max_len=top + 1, **c.kw())
+        call()
+        ctx.sync()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call()
+        graphs.append((g, call))
+        checks.append((c, q, out, past, p, rs))
+    for order in ((0, 1), (1, 0), (0, 0)):
+        for k in order:
+            checks[k][2].zero_()
+            graphs[k][0].replay()
+        ctx.sync()
+        for k in order:
+            c, q, out, past, _, _ = checks[k]
+            want, tol = attention64(c, q, past, [1] * len(past), op == "chunk")
+            assert_within(out, want, tol)
+    graphs.clear()
+
+
+@pytest.mark.parametrize("op", ["decode", "chunk"])
+def test_same_bits_every_time(ctx, op):
+    past = [3000, 5, 1200, 64, 900, 2500]
+    c = Cache(71, "q4", 16, 32, 8, [p + 1 for p in past])
+    q = randh(gen(72), len(past), 32 * D)
+    outs = []
+    for _ in range(6):
+        out = torch.zeros_like(q)
+        if op == "decode":
+            ctx.attn_decode_kv(c.prm, q, None, None, c.k, c.v, i32(past), out, max_past=3000,
+                               fused_prep=False, **c.kw())
+        else:
+            ctx.attn_chunk_kv(c.prm, q, c.k, c.v, i32(past), i32(range(len(past) + 1)), out,
+                              max_len=3001, **c.kw())
+        outs.append(out)
+    ctx.sync()
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+def test_another_stream_than_the_current_one(ctx):
+    c = Cache(73, "q4", 16, 16, 8, [513])
+    qkv, rope = randh(gen(74), 513, 32 * D), rope_table(513)
+    q, out, out2 = (torch.zeros(513, 16 * D, dtype=torch.float16, device="cuda")
+                    for _ in range(3))
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    kw = dict(max_len=513, stream=s, **c.kw())
+    z, rs = i32([0]), i32([0, 513])
+    torch.cuda.synchronize()
+    ctx.kv_append(c.prm, qkv, None, rope, c.k, c.v, z, rs, q_out=q, **kw)
+    ctx.attn_chunk_kv(c.prm, q, c.k, c.v, z, rs, out, **kw)
+    with torch.cuda.stream(s):
+        ctx.attn_chunk_kv(c.prm, q, c.k, c.v, z, rs, out2, max_len=513, **c.kw())
+    ctx.sync(s)
+    want, tol = attention64(c, q, [0], [513], True)
+    assert_within(out, want, tol)
+    assert torch.equal(out, out2)
