@@ -41,6 +41,10 @@ struct p2p_ctx {
   size_t partials_bytes = 0;
   int32_t* counters = nullptr;
   size_t counters_bytes = 0;
+  // 4-bit decode and prompt-chunk attention over any cache: a fixed size, made by the first call
+  // and kept until the context goes, so captured graphs never see it move
+  void* serve_ws = nullptr;
+  size_t serve_ws_bytes = 0;
   void* w16 = nullptr;  // prompt-chunk projections: the dequantised f16 weights
   size_t w16_bytes = 0;
   std::map<std::tuple<int, int, double, int>, void*> rope;
@@ -417,6 +421,7 @@ p2p_status p2p_ctx_destroy(p2p_ctx* ctx) {
   dev_free(ctx->partials, ctx->partials_bytes);
   dev_free(ctx->counters, ctx->counters_bytes);
   dev_free(ctx->w16, ctx->w16_bytes);
+  dev_free(ctx->serve_ws, ctx->serve_ws_bytes);
   cudaStreamDestroy(ctx->stream);
   delete ctx;
   return P2P_OK;
@@ -925,7 +930,7 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
   if (prm->dtype != P2P_F16)
     return fail(ctx, P2P_ERR_UNSUPPORTED, "decode_kv: q/out must be f16");
   if (lay->format == P2P_KV_Q4) {
-    p2p::AttnKvArgs q{};
+    p2p::DecodeQ4Args q{};
     st = p2p::make_kv_view(ctx, lay, prm->num_kv_heads, k_cache, v_cache, kv_rows, offsets, nseq,
                            "decode_kv", &q.kv);
     if (st != P2P_OK) return st;
@@ -952,8 +957,18 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
     q.norm_w = static_cast<const __half*>(norm_w);
     q.rope = static_cast<const __half*>(rope);
     q.eps = eff_eps(prm);
+    if (p2p::decode_q4_ctas(ctx->num_sms, prm->num_kv_heads) < 1)
+      return fail(ctx, P2P_ERR_UNSUPPORTED, "decode_kv: %d kv heads in 4 bits",
+                  prm->num_kv_heads);
     DeviceGuard g(ctx->device);
-    cudaError_t e = p2p::launch_attn_kv(q, pick_stream(ctx, stream));
+    cudaStream_t s = pick_stream(ctx, stream);
+    unsigned char* ws = nullptr;
+    st = p2p::ctx_serve_workspace(ctx, s, "decode_kv", &ws);
+    if (st != P2P_OK) return st;
+    q.counters = reinterpret_cast<int32_t*>(ws);
+    q.parts = reinterpret_cast<float*>(ws + p2p::decode_q4_counter_bytes(ctx->num_sms));
+    q.wait_deficit = g_wait_deficit.load();
+    cudaError_t e = p2p::launch_decode_q4(q, ctx->num_sms, s);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "decode_kv launch");
     return P2P_OK;
   }
@@ -1381,6 +1396,41 @@ p2p_status check_ragged(p2p_ctx* ctx, const p2p_attn_params* prm, const void* qk
         return fail(ctx, P2P_ERR_INVALID_ARG, "%s: rope table of %d rows, max_past %d", who,
                     std::get<0>(kv.first), max_past);
   }
+  return P2P_OK;
+}
+
+// The context's workspace of the 4-bit decode and the prompt-chunk attention (counters, zero
+// between launches, then records).  The first call allocates it, which a stream capture forbids.
+p2p_status ctx_serve_workspace(p2p_ctx* ctx, cudaStream_t s, const char* who,
+                               unsigned char** ws) {
+  if (!ctx->serve_ws) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(s, &cap);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return cuda_fail(ctx, e, who);
+    }
+    if (cap != cudaStreamCaptureStatusNone)
+      return fail(ctx, P2P_ERR_INVALID_ARG,
+                  "%s: the first call of a context makes its workspace and cannot be captured",
+                  who);
+    const size_t counters = decode_q4_counter_bytes(ctx->num_sms);
+    const size_t bytes = counters + decode_q4_parts_bytes(ctx->num_sms);
+    void* p = nullptr;
+    if (dev_alloc(&p, bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(ctx, P2P_ERR_OOM, "%s: workspace of %zu bytes", who, bytes);
+    }
+    e = cudaMemset(p, 0, counters);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) {
+      dev_free(p, bytes);
+      return cuda_fail(ctx, e, who);
+    }
+    ctx->serve_ws = p;
+    ctx->serve_ws_bytes = bytes;
+  }
+  *ws = static_cast<unsigned char*>(ctx->serve_ws);
   return P2P_OK;
 }
 

@@ -1,0 +1,749 @@
+// attn_q4.cu -- attention of one token per sequence over a 4-bit KV cache (ATTN at M = 1,
+// src/scripts/lfm-engine/kernels.js:268-319, optionally with QK_PREP, :216-266, in front).
+//
+// Mathematics.  A cached value is code * s + lo with one (s, lo) per (token, kv head), so
+//     q . k_j      = s_j (q . c_j) + lo_j sum(q)
+//     sum_j p_j v_j = sum_j (p_j s_j) c_j + sum_j p_j lo_j
+// and only the codes c enter the tensor cores.  A 4-bit code in the low bits of an f16 is the
+// subnormal c * 2^-24 (c * 2^-20 one nibble higher), which the f16 MMA multiplies exactly: a word
+// of eight codes becomes four f16 pairs with one shift and four ANDs and no conversion.  The odd
+// nibbles' factor 16 goes into q (divided by 16 for those dims; exact down to f16's subnormals)
+// and into the final scale of the odd output dims.
+//     S^T[16 keys x 8 heads] = C_K[16 x 64] . Q^T[64 x 8],   O^T[64 x 8] += C_V^T[64 x 16] . P'^T
+// P' = p * s * 4 is rounded to f16 (2^-11 of a weight, below the rounding of the f16 output; the
+// factor 4 uses the range left by s <= 8734, so weights keep their bits down to small scales);
+// p, the sums of p and of p * lo, the running maximum and O stay in f32.
+//
+// Split.  All sequences' tiles, in order, form one list that is cut into equal parts, one per CTA
+// (two CTAs per SM), so ragged batches balance by themselves whatever the lengths and the grid
+// does not depend on them.  A CTA works on up to 8 kv heads of its tiles, one warp per head (more
+// warps per head when there are fewer heads), because a page's rows are contiguous over heads:
+// one bulk copy per page and pool fetches them, issued by a producer warp into a ring of stages.
+// Sequences that straddle CTAs are joined by the last warp to arrive per head, in two levels of at
+// most kJoin records each; the order of the sums is that of the CTAs, so results repeat bit for bit.
+#include "common.cuh"
+#include "kernels.h"
+#include "kv_view.cuh"
+#include "sm100.cuh"
+
+namespace p2p {
+namespace {
+
+using sm100::fence_barrier_init;
+using sm100::fence_proxy_async_smem;
+using sm100::globaltimer_ns;
+using sm100::mbar_arrive;
+using sm100::mbar_arrive_expect_tx;
+using sm100::mbar_init;
+using sm100::mbar_try_wait;
+using sm100::smem_u32;
+
+constexpr int kWarps = 8;                      // compute warps; warp 8 is the producer
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kBlock = 32;                     // keys per warp and tile
+constexpr int kMaxStages = 8;
+constexpr int kRec = 68;                       // acc[64], max, sum, 2 pad: 17 16-byte pieces
+constexpr int kJoin = 16;                      // records joined by one warp
+constexpr float kNegBig = -1e30f;
+constexpr uint64_t kWaitLimitNs = 1000000000ull;
+
+// Warps per head for a CTA of hb heads (1 .. 8); its tile is kBlock keys per such warp.
+__host__ __device__ constexpr int warps_per_head(int hb) {
+  return hb >= 5 ? 1 : hb >= 3 ? 2 : hb == 2 ? 4 : 8;
+}
+// Bytes of one token's units of hb heads, as copied and as laid out in shared memory.
+__host__ __device__ constexpr int pitch_of(int hb) { return (hb * kQ4UnitBytes + 15) / 16 * 16; }
+__host__ __device__ constexpr int stage_bytes(int hb) {
+  return 2 * kBlock * warps_per_head(hb) * pitch_of(hb);
+}
+
+struct StageMeta {
+  int z;        // sequence
+  int key0;     // first key of the tile
+  int valid;    // its keys
+  int flags;    // kFirst, kLast of this CTA's part of the sequence; kBad
+  long long g;  // position of the sequence's tile 0 in the list of all tiles
+  int tiles;    // the sequence's tiles
+  int pos;      // position of the token (its keys are 0 .. pos)
+};
+constexpr int kFirst = 1, kLast = 2, kBad = 4;
+
+struct Shared {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  StageMeta meta[kMaxStages];
+  long long wsum[kWarps];
+  long long total;
+  int z0, t0;
+  volatile int abort_flag;
+};
+
+__device__ __forceinline__ bool wait_bar(Shared& s, uint64_t* bar, uint32_t parity, int32_t* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (s.abort_flag) return false;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      s.abort_flag = 1;
+      atomicOr(err, kErrTimeout);
+      return false;
+    }
+  }
+}
+
+// Untiled bulk copy: 16-byte aligned addresses, a multiple of 16 bytes.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(dst),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // nibbles 0, 4 and 1, 5 of a word
+
+// A warp's query heads: B fragments of the four k-steps and the heads' sums (columns 2t, 2t+1).
+struct Query {
+  uint32_t b[4][2];
+  float sum[2];
+};
+
+// From the G f16 rows at `q` (row stride 64): lane (gid, t) holds head gid's dims 8t .. 8t+7 and
+// 32 + 8t .. 32 + 8t + 7 in the order the code words give them.
+template <int G>
+__device__ __forceinline__ void load_query(const __half* q, float scale_log2, Query& out) {
+  const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
+  uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (gid < G) {
+    w[0] = *reinterpret_cast<const uint4*>(q + gid * 64 + 8 * t);
+    w[1] = *reinterpret_cast<const uint4*>(q + gid * 64 + 32 + 8 * t);
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t d01 = w[i].x, d23 = w[i].y, d45 = w[i].z, d67 = w[i].w;
+    const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
+    uint32_t e[4] = {__byte_perm(d01, d45, 0x5410), __byte_perm(d01, d45, 0x7632),
+                     __byte_perm(d23, d67, 0x5410), __byte_perm(d23, d67, 0x7632)};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __half2 h = *reinterpret_cast<const __half2*>(&e[k]);
+      const float2 f = __half22float2(h);
+      sum += f.x + f.y;
+      const __half2 s = (k & 1) ? __hmul2(h, sixteenth) : h;
+      out.b[2 * i + (k >> 1)][k & 1] = *reinterpret_cast<const uint32_t*>(&s);
+    }
+  }
+  sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+  sum *= scale_log2;
+  out.sum[0] = __shfl_sync(0xffffffffu, sum, 8 * t);      // lane of head 2t
+  out.sum[1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);  // head 2t + 1
+}
+
+struct State {
+  float m[2], l[2], bias[2];  // heads 2t, 2t+1: maximum (of the warp), partial sums (of the lane)
+  float o[4][4];              // dims 8 gid + 2i (even codes) and 8 gid + 2i + 1, heads 2t, 2t+1
+  __device__ __forceinline__ void clear() {
+    m[0] = m[1] = kNegBig;
+    l[0] = l[1] = bias[0] = bias[1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  }
+};
+
+// One block of 32 keys of one head: rows at ks / vs (this head's unit in the block's first key).
+// Row r of the fragments is key perm(r): eight consecutive rows then read V's words of keys 2t and
+// 2t + 1 from distinct banks (the row pitch is 8 banks modulo 32 for 8 heads).
+__device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned char* vs,
+                                         int pitch, int valid, float scale24, const Query& q,
+                                         State& st) {
+  const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
+  constexpr uint32_t kPerm = 0x57463120u;
+  const int row = (kPerm >> (4 * gid)) & 7;
+  float sc[4][2];  // keys row, row + 8, row + 16, row + 24; heads 2t, 2t + 1
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t* ka = reinterpret_cast<const uint32_t*>(ks + (16 * j + row) * pitch);
+    const uint32_t* kb = reinterpret_cast<const uint32_t*>(ks + (16 * j + row + 8) * pitch);
+    const uint32_t a0 = ka[t], a1 = ka[t + 4], b0 = kb[t], b1 = kb[t + 4];
+    const uint32_t pa = ka[8], pb = kb[8];
+    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+    mma16816(s0, a0 & kEven, b0 & kEven, a0 & kOdd, b0 & kOdd, q.b[0][0], q.b[0][1]);
+    mma16816(s1, (a0 >> 8) & kEven, (b0 >> 8) & kEven, (a0 >> 8) & kOdd, (b0 >> 8) & kOdd,
+             q.b[1][0], q.b[1][1]);
+    mma16816(s0, a1 & kEven, b1 & kEven, a1 & kOdd, b1 & kOdd, q.b[2][0], q.b[2][1]);
+    mma16816(s1, (a1 >> 8) & kEven, (b1 >> 8) & kEven, (a1 >> 8) & kOdd, (b1 >> 8) & kOdd,
+             q.b[3][0], q.b[3][1]);
+    float s, lo;
+    q4_unpack(pa, s, lo);
+    s *= scale24;
+    sc[2 * j][0] = fmaf(s0[0] + s1[0], s, lo * q.sum[0]);
+    sc[2 * j][1] = fmaf(s0[1] + s1[1], s, lo * q.sum[1]);
+    q4_unpack(pb, s, lo);
+    s *= scale24;
+    sc[2 * j + 1][0] = fmaf(s0[2] + s1[2], s, lo * q.sum[0]);
+    sc[2 * j + 1][1] = fmaf(s0[3] + s1[3], s, lo * q.sum[1]);
+  }
+  if (valid < kBlock) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (8 * k + row >= valid) sc[k][0] = sc[k][1] = -INFINITY;
+  }
+  const float mb0 = fmaxf(fmaxf(sc[0][0], sc[1][0]), fmaxf(sc[2][0], sc[3][0]));
+  const float mb1 = fmaxf(fmaxf(sc[0][1], sc[1][1]), fmaxf(sc[2][1], sc[3][1]));
+  // the maximum rarely grows after the first blocks: only then is it joined and O rescaled
+  if (__any_sync(0xffffffffu, mb0 > st.m[0] || mb1 > st.m[1])) {
+    float n0 = mb0, n1 = mb1;
+#pragma unroll
+    for (int o = 4; o <= 16; o <<= 1) {
+      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
+      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+    }
+    n0 = fmaxf(n0, st.m[0]);
+    n1 = fmaxf(n1, st.m[1]);
+    const float c0 = fast_exp2(st.m[0] - n0), c1 = fast_exp2(st.m[1] - n1);
+    st.m[0] = n0;
+    st.m[1] = n1;
+    st.l[0] *= c0;
+    st.l[1] *= c1;
+    st.bias[0] *= c0;
+    st.bias[1] *= c1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      st.o[i][0] *= c0;
+      st.o[i][1] *= c1;
+      st.o[i][2] *= c0;
+      st.o[i][3] *= c1;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    // weights of keys row and row + 8 of this half, scaled by the keys' value scales
+    float w[4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t pv = reinterpret_cast<const uint32_t*>(vs + (16 * j + row + 8 * k) * pitch)[8];
+      // rows behind the last key hold whatever the stage held before: no weight, no parameters
+      if (valid < kBlock && 16 * j + 8 * k + row >= valid) pv = 0u;
+      float s, lo;
+      q4_unpack(pv, s, lo);
+      s *= 4.f;
+      const float p0 = fast_exp2(sc[2 * j + k][0] - st.m[0]);
+      const float p1 = fast_exp2(sc[2 * j + k][1] - st.m[1]);
+      st.l[0] += p0;
+      st.l[1] += p1;
+      st.bias[0] = fmaf(p0, lo, st.bias[0]);
+      st.bias[1] = fmaf(p1, lo, st.bias[1]);
+      w[2 * k] = p0 * s;
+      w[2 * k + 1] = p1 * s;
+    }
+    const uint32_t b0 = movmatrix_trans(pack_h2(w[0], w[1]));
+    const uint32_t b1 = movmatrix_trans(pack_h2(w[2], w[3]));
+    const unsigned char* v0 = vs + (16 * j + ((kPerm >> (8 * t)) & 7)) * pitch + 4 * gid;
+    const unsigned char* v1 = vs + (16 * j + ((kPerm >> (8 * t + 4)) & 7)) * pitch + 4 * gid;
+    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(v0);
+    const uint32_t w1 = *reinterpret_cast<const uint32_t*>(v1);
+    const uint32_t w2 = *reinterpret_cast<const uint32_t*>(v0 + 8 * pitch);
+    const uint32_t w3 = *reinterpret_cast<const uint32_t*>(v1 + 8 * pitch);
+    // pairs of keys: codes 0..3 of both words, then codes 4..7
+    const uint32_t x = __byte_perm(w0, w1, 0x5410), y = __byte_perm(w0, w1, 0x7632);
+    const uint32_t x2 = __byte_perm(w2, w3, 0x5410), y2 = __byte_perm(w2, w3, 0x7632);
+    mma16816(st.o[0], x & kEven, x & kOdd, x2 & kEven, x2 & kOdd, b0, b1);
+    mma16816(st.o[1], (x >> 8) & kEven, (x >> 8) & kOdd, (x2 >> 8) & kEven, (x2 >> 8) & kOdd, b0,
+             b1);
+    mma16816(st.o[2], y & kEven, y & kOdd, y2 & kEven, y2 & kOdd, b0, b1);
+    mma16816(st.o[3], (y >> 8) & kEven, (y >> 8) & kOdd, (y2 >> 8) & kEven, (y2 >> 8) & kOdd, b0,
+             b1);
+  }
+}
+
+// The CTA (of w) that owns tile i of `total`: part b starts at tile total * b / w.
+__device__ __forceinline__ int owner_of(long long i, long long total, int w) {
+  return int(((i + 1) * w - 1) / total);
+}
+
+// A warp's part of one head: lane (gid, t) holds dims 8 gid .. 8 gid + 7 of heads 2t and 2t + 1.
+struct Part {
+  float acc[2][8], m[2], l[2];
+};
+__device__ __forceinline__ void store_part(float* rec, const Part& p, int g_count) {
+  const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int g = 2 * t + e;
+    if (g >= g_count) continue;
+    float* r = rec + g * kRec;
+    *reinterpret_cast<float4*>(r + 8 * gid) =
+        make_float4(p.acc[e][0], p.acc[e][1], p.acc[e][2], p.acc[e][3]);
+    *reinterpret_cast<float4*>(r + 8 * gid + 4) =
+        make_float4(p.acc[e][4], p.acc[e][5], p.acc[e][6], p.acc[e][7]);
+    if (gid == 0) *reinterpret_cast<float2*>(r + 64) = make_float2(p.m[e], p.l[e]);
+  }
+}
+template <bool GLOBAL>
+__device__ __forceinline__ float4 load_f4(const float* p) {
+  if (GLOBAL) return __ldcg(reinterpret_cast<const float4*>(p));
+  return *reinterpret_cast<const float4*>(p);
+}
+// The join of n records (rec(i) of them), in order; a record with a negative sum makes the join one.
+template <bool GLOBAL, class Rec>
+__device__ __forceinline__ void join_parts(Part& p, int n, int g_count, Rec rec) {
+  const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int g = min(2 * t + e, g_count - 1);
+    float mx = kNegBig;
+    bool bad = false;
+    for (int i = 0; i < n; ++i) {
+      const float4 ml = load_f4<GLOBAL>(rec(i) + g * kRec + 64);
+      mx = fmaxf(mx, ml.x);
+      bad |= ml.y < 0.f;
+    }
+    float l = 0.f, acc[8] = {};
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float* r = rec(i) + g * kRec;
+      const float4 ml = load_f4<GLOBAL>(r + 64);
+      const float4 a = load_f4<GLOBAL>(r + 8 * gid), b = load_f4<GLOBAL>(r + 8 * gid + 4);
+      const float c = fast_exp2(ml.x - mx);
+      l = fmaf(ml.y, c, l);
+      acc[0] = fmaf(a.x, c, acc[0]);
+      acc[1] = fmaf(a.y, c, acc[1]);
+      acc[2] = fmaf(a.z, c, acc[2]);
+      acc[3] = fmaf(a.w, c, acc[3]);
+      acc[4] = fmaf(b.x, c, acc[4]);
+      acc[5] = fmaf(b.y, c, acc[5]);
+      acc[6] = fmaf(b.z, c, acc[6]);
+      acc[7] = fmaf(b.w, c, acc[7]);
+    }
+    p.m[e] = mx;
+    p.l[e] = bad ? -1.f : l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p.acc[e][i] = acc[i];
+  }
+}
+
+// The tiles of a CTA's part, in order, sequence by sequence.
+struct Walk {
+  const KvView& kv;
+  const ChunkIndex& at;
+  int tile, z, t, tiles;
+  SeqSpan sp;
+  __device__ Walk(const KvView& k, const ChunkIndex& x, int tile_, int z0, int t0)
+      : kv(k), at(x), tile(tile_), z(z0), t(t0), sp(seq_span(k, x, z0)) {
+    tiles = (sp.past + tile) / tile;  // of past + 1 keys
+  }
+  // Moves on to the next sequence that has tiles when this one's are done.
+  __device__ void settle() {
+    if (t < tiles) return;
+    do {
+      ++z;
+      sp = seq_span(kv, at, z);
+    } while (!sp.ok);
+    tiles = (sp.past + tile) / tile;
+    t = 0;
+  }
+};
+
+// Announces this warp's record at `counter`; true for the last of n (which resets it).
+__device__ __forceinline__ bool last_of(int32_t* counter, int n) {
+  __threadfence();
+  __syncwarp();
+  int old = 0;
+  if ((threadIdx.x & 31) == 0) old = atomicAdd(counter, 1);
+  old = __shfl_sync(0xffffffffu, old, 0);
+  if (old != n - 1) return false;
+  if ((threadIdx.x & 31) == 0) *counter = 0;
+  __threadfence();
+  return true;
+}
+
+template <int G, bool FUSED>
+__global__ void __launch_bounds__(kThreads, 2)
+    attn_decode_q4_kernel(const __grid_constant__ DecodeQ4Args a) {
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ Shared s;
+  __shared__ __align__(16) __half q_s[FUSED ? kWarps : 1][FUSED ? G : 1][64];
+  __shared__ __align__(16) __half new_s[FUSED ? kWarps : 1][2][64];
+  __shared__ uint32_t unit_s[FUSED ? kWarps : 1][2][9];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int grp = blockIdx.y;
+  const int hb = min(8, a.kv.hkv - 8 * grp), wph = warps_per_head(hb);
+  const int tile = kBlock * wph, pitch = pitch_of(hb), sbytes = 2 * tile * pitch;
+  const int n_groups = gridDim.y;
+
+  // ---- the CTA's part of the list of tiles
+  const int per = (a.at.nseq + kWarps * 32 - 1) / (kWarps * 32);
+  long long mine = 0, upto = 0;
+  if (tid == 0) {
+    for (int i = 0; i < a.stages; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], kWarps);
+    }
+    s.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp < kWarps) {
+    for (int z = tid * per; z < min((tid + 1) * per, a.at.nseq); ++z) {
+      const SeqSpan sp = seq_span(a.kv, a.at, z);
+      if (sp.ok) mine += (sp.past + tile) / tile;  // tiles of past + 1 keys
+      else if (blockIdx.x == 0 && grp == 0) atomicOr(a.err, kErrPosBeyondCache);
+    }
+    upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) s.wsum[warp] = upto;
+  }
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) upto += total;
+    total += s.wsum[w];
+  }
+  const int parts = int(min(static_cast<long long>(gridDim.x),
+                            (total + a.min_tiles - 1) / a.min_tiles));
+  const int b = blockIdx.x;
+  if (b >= parts) return;
+  const long long lo = total * b / parts;
+  const int n_tiles = int(total * (b + 1) / parts - lo);
+  if (warp < kWarps && lo < upto && lo >= upto - mine) {
+    long long at = upto - mine;
+    for (int z = tid * per;; ++z) {
+      const SeqSpan sp = seq_span(a.kv, a.at, z);
+      const int tz = sp.ok ? (sp.past + tile) / tile : 0;
+      if (lo < at + tz) {
+        s.z0 = z;
+        s.t0 = int(lo - at);
+        break;
+      }
+      at += tz;
+    }
+  }
+  __syncthreads();
+
+  if (warp == kWarps) {
+    // ------------------------------------------------------------------ producer
+    Walk w(a.kv, a.at, tile, s.z0, s.t0);
+    // keys of one contiguous run: the cache's rows are whole tokens, so a run can span keys only
+    // when one group of heads is the whole row
+    const int run = n_groups > 1 ? 1 : a.kv.table ? min(1 << a.kv.shift, tile) : tile;
+    int issued = 0;
+    for (int i = 0; i < n_tiles; ++i, ++w.t) {
+      w.settle();
+      const int st = i % a.stages;
+      if (i >= a.stages) {
+        bool ok = true;
+        if (lane == 0) ok = wait_bar(s, &s.empty[st], (i / a.stages - 1) & 1, a.err);
+        if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) break;
+      }
+      const int z = w.z, key0 = w.t * tile, len = w.sp.past + 1, valid = min(tile, len - key0);
+      const int n_copy = FUSED && key0 + valid == len ? valid - 1 : valid;
+      const int runs = (n_copy + run - 1) / run;
+      bool bad = false;
+      for (int k = lane; k < runs; k += 32) bad |= kv_row(a.kv, z, key0 + k * run) < 0;
+      if (FUSED && key0 + valid == len) bad |= kv_row(a.kv, z, w.sp.past) < 0;
+      bad = __any_sync(0xffffffffu, bad);
+      if (lane == 0) {
+        if (bad) atomicOr(a.err, kErrPosBeyondCache);
+        StageMeta& m = s.meta[st];
+        m.z = z;
+        m.key0 = key0;
+        m.valid = valid;
+        m.flags = (i == 0 || w.t == 0 ? kFirst : 0) |
+                  (i == n_tiles - 1 || w.t == w.tiles - 1 ? kLast : 0) | (bad ? kBad : 0);
+        m.g = lo + i - w.t;
+        m.tiles = w.tiles;
+        m.pos = w.sp.past;
+        mbar_arrive_expect_tx(&s.full[st],
+                              uint32_t(bad ? 0 : 2 * n_copy * pitch) +
+                                  uint32_t(i == 0 ? a.wait_deficit : 0));
+      }
+      __syncwarp();
+      if (!bad) {
+        const uint32_t dst = smem_u32(ring) + uint32_t(st * sbytes);
+        for (int k = lane; k < 2 * runs; k += 32) {
+          const int pool = k >= runs, r = k - pool * runs;
+          const int n = min(run, n_copy - r * run);
+          const int64_t row = kv_row(a.kv, z, key0 + r * run);
+          bulk_load(dst + uint32_t((pool * tile + r * run) * pitch),
+                    (pool ? a.kv.v : a.kv.k) + row * a.kv.row_bytes + grp * 8 * kQ4UnitBytes,
+                    uint32_t(n * pitch), &s.full[st]);
+        }
+      }
+      issued = i + 1;
+    }
+    if (s.abort_flag) {  // let the copies already in flight land before the CTA exits
+      for (int i = max(0, issued - a.stages); i < issued; ++i) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&s.full[i % a.stages], (i / a.stages) & 1) &&
+               globaltimer_ns() - t0 < kWaitLimitNs) {
+        }
+      }
+    }
+    return;
+  }
+
+  // -------------------------------------------------------------------- compute warps
+  const int h = warp % hb, sub = warp / hb;
+  const bool active = sub < wph;
+  const int kh = grp * 8 + h;
+  const float scale24 = a.scale_log2 * 16777216.f;
+  float* merge = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // [warp][G][kRec]
+  Query q;
+  State state;
+  bool bad = false, seg_first = true;
+  int segs = 0;  // parts of sequences ended
+  // Ends this CTA's part of sequence z (whose `tiles` tiles begin at g0 of the list): the warps of
+  // a head meet, and the sequence's output is written or its record left for the last to arrive.
+  auto finish = [&](Part& p, int z, long long g0, int tiles) {
+    if (wph > 1) {  // the warps of a head meet in shared memory
+      if (active) store_part(merge + warp * G * kRec, p, G);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (sub == 0)
+        join_parts<false>(p, wph, G, [&](int k) { return merge + (k * hb + h) * G * kRec; });
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    const bool whole_seq = lo <= g0 && lo + n_tiles >= g0 + tiles;
+    bool write = active && sub == 0;
+    if (!whole_seq && write) {
+      const int slot = seg_first ? 0 : 1;
+      const int first = owner_of(g0, total, parts), last = owner_of(g0 + tiles - 1, total, parts);
+      const int n = last - first + 1, me = b - first;
+      // CTA first + i: the sequence is its first part, except that `first` may begin with another
+      const int slot0 = total * first / parts < g0 ? 1 : 0;
+      auto place = [&](int i) {
+        return ((int64_t(grp) * gridDim.x + first + i) * 2 + (i == 0 ? slot0 : 0)) * 8 + h;
+      };
+      auto rec = [&](int i) { return a.parts + place(i) * (G * kRec); };
+      store_part(a.parts + (((int64_t(grp) * gridDim.x + b) * 2 + slot) * 8 + h) * (G * kRec), p,
+                 G);
+      const int lead = me / kJoin * kJoin, n_here = min(kJoin, n - lead);
+      write = last_of(a.counters + 2 * place(lead), n_here);
+      if (write) join_parts<true>(p, n_here, G, [&](int k) { return rec(lead + k); });
+      if (write && n > kJoin) {
+        store_part(rec(lead), p, G);
+        const int n_lead = (n + kJoin - 1) / kJoin;
+        write = last_of(a.counters + 2 * place(0) + 1, n_lead);
+        if (write) join_parts<true>(p, n_lead, G, [&](int k) { return rec(k * kJoin); });
+      }
+    }
+    if (write) {
+      const int gid = lane >> 2, t = lane & 3;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (2 * t + e >= G || p.l[e] < 0.f) continue;
+        const float inv = __fdiv_rn(1.f, p.l[e]);
+        *reinterpret_cast<uint4*>(a.out + int64_t(z) * a.ld_o + (kh * G + 2 * t + e) * 64 +
+                                  8 * gid) =
+            make_uint4(pack_h2(p.acc[e][0] * inv, p.acc[e][1] * inv),
+                       pack_h2(p.acc[e][2] * inv, p.acc[e][3] * inv),
+                       pack_h2(p.acc[e][4] * inv, p.acc[e][5] * inv),
+                       pack_h2(p.acc[e][6] * inv, p.acc[e][7] * inv));
+      }
+    }
+    seg_first = false;
+    ++segs;
+  };
+  int i = 0;
+  for (; i < n_tiles; ++i) {
+    const int st = i % a.stages;
+    const bool ok = wait_bar(s, &s.full[st], (i / a.stages) & 1, a.err);
+    if (!__all_sync(0xffffffffu, ok)) break;
+    const StageMeta m = s.meta[st];
+    unsigned char* ks = ring + st * sbytes + sub * kBlock * pitch + h * kQ4UnitBytes;
+    unsigned char* vs = ks + tile * pitch;
+    const bool has_new = FUSED && m.key0 + m.valid == m.pos + 1;
+    if (m.flags & kFirst) {
+      state.clear();
+      bad = false;
+      if (active) {
+        const __half* row = a.q + int64_t(m.z) * a.ld_q;
+        if (FUSED) {
+          const float cs = to_f32(a.rope[int64_t(m.pos) * 64 + lane]);
+          const float sn = to_f32(a.rope[int64_t(m.pos) * 64 + 32 + lane]);
+          const __half* src = row + kh * G * 64;
+          float x[G][2];
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            x[g][0] = to_f32(src[g * 64 + lane]);
+            x[g][1] = to_f32(src[g * 64 + 32 + lane]);
+          }
+          const bool nw = a.norm_w != nullptr;
+          const float w0 = nw ? to_f32(a.norm_w[lane]) : 0.f;
+          const float w1 = nw ? to_f32(a.norm_w[32 + lane]) : 0.f;
+          __syncwarp();  // q_s of the sequence before has been read
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            float r0, r1;
+            norm_rope_vals<__half>(x[g][0], x[g][1], w0, w1, nw, a.eps, cs, sn, r0, r1);
+            q_s[warp][g][lane] = __float2half_rn(r0);
+            q_s[warp][g][32 + lane] = __float2half_rn(r1);
+          }
+          __syncwarp();
+          load_query<G>(&q_s[warp][0][0], a.scale_log2, q);
+        } else {
+          load_query<G>(row + kh * G * 64, a.scale_log2, q);
+        }
+      }
+    }
+    if (m.flags & kBad) bad = true;
+    const int valid = m.valid - sub * kBlock;
+    if (active && valid > 0 && !bad) {
+      if (has_new && valid <= kBlock) {
+        // the new token's unit of this head: normed, rotated, quantised, into the cache and over
+        // the stage's row (which the copy left out)
+        const __half* row = a.q + int64_t(m.z) * a.ld_q;
+        const float cs = to_f32(a.rope[int64_t(m.pos) * 64 + lane]);
+        const float sn = to_f32(a.rope[int64_t(m.pos) * 64 + 32 + lane]);
+        const __half* kn = row + (a.hq + kh) * 64;
+        const __half* vn = row + (a.hq + a.kv.hkv + kh) * 64;
+        float r0, r1;
+        norm_rope_head<__half>(to_f32(kn[lane]), to_f32(kn[32 + lane]),
+                               a.norm_w ? a.norm_w + 64 : nullptr, a.norm_w != nullptr, a.eps, cs,
+                               sn, r0, r1);
+        __syncwarp();
+        new_s[warp][0][lane] = __float2half_rn(r0);
+        new_s[warp][0][32 + lane] = __float2half_rn(r1);
+        new_s[warp][1][lane] = vn[lane];
+        new_s[warp][1][32 + lane] = vn[32 + lane];
+        __syncwarp();
+        float x[8];  // lanes 0-7: k's unit, 8-15: v's (the others repeat them)
+        const int sl = lane & 7, kv = (lane >> 3) & 1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[k] = to_f32(new_s[warp][kv][4 * sl + k]);
+          x[4 + k] = to_f32(new_s[warp][kv][32 + 4 * sl + k]);
+        }
+        q4_store_unit(x, unit_s[warp][kv], lane < 16);
+        __syncwarp();
+        if (lane < 18) {
+          const int pool = lane / 9, w = lane % 9;
+          const uint32_t v = unit_s[warp][pool][w];
+          const int64_t at = kv_row(a.kv, m.z, m.pos);
+          reinterpret_cast<uint32_t*>((pool ? a.kv.v : a.kv.k) + at * a.kv.row_bytes +
+                                      kh * kQ4UnitBytes)[w] = v;
+          reinterpret_cast<uint32_t*>((pool ? vs : ks) + (valid - 1) * pitch)[w] = v;
+        }
+        fence_proxy_async_smem();  // a later copy into this stage comes after these writes
+        __syncwarp();
+      }
+      attend32(ks, vs, pitch, min(valid, kBlock), scale24, q, state);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.empty[st]);
+    if (!(m.flags & kLast)) continue;
+
+    // ---- this CTA's part of the sequence is done
+    Part p;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int o = 4; o <= 16; o <<= 1) {
+        state.l[e] += __shfl_xor_sync(0xffffffffu, state.l[e], o);
+        state.bias[e] += __shfl_xor_sync(0xffffffffu, state.bias[e], o);
+      }
+      p.m[e] = state.m[e];
+      p.l[e] = bad ? -1.f : state.l[e];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        p.acc[e][2 * k] = fmaf(state.o[k][e], 4194304.f, state.bias[e]);         // 2^24 / 4
+        p.acc[e][2 * k + 1] = fmaf(state.o[k][2 + e], 262144.f, state.bias[e]);  // 2^20 / 4
+      }
+    }
+    finish(p, m.z, m.g, m.tiles);
+  }
+  if (i == n_tiles) return;
+  // A wait ran out: the parts that are left end as bad ones, so that no other warp or CTA waits or
+  // joins in vain and the counters return to zero.
+  Walk w(a.kv, a.at, tile, s.z0, s.t0);
+  int done = segs;
+  for (int k = 0; k < n_tiles; ++k, ++w.t) {
+    w.settle();
+    if (!(k == n_tiles - 1 || w.t == w.tiles - 1) || done-- > 0) continue;
+    Part p = {};
+    p.m[0] = p.m[1] = kNegBig;
+    p.l[0] = p.l[1] = -1.f;
+    finish(p, w.z, lo + k - w.t, w.tiles);
+  }
+}
+
+template <int G>
+const void* pick(bool fused) {
+  return fused ? reinterpret_cast<const void*>(&attn_decode_q4_kernel<G, true>)
+               : reinterpret_cast<const void*>(&attn_decode_q4_kernel<G, false>);
+}
+const void* pick(int group, bool fused) {
+  switch (group) {
+    case 1: return pick<1>(fused);
+    case 2: return pick<2>(fused);
+    case 4: return pick<4>(fused);
+    case 8: return pick<8>(fused);
+    default: return nullptr;
+  }
+}
+
+constexpr int kRingBytes = 94 * 1024;  // two CTAs per SM
+
+}  // namespace
+
+int decode_q4_ctas(int num_sms, int hkv) {
+  const int groups = (hkv + 7) / 8;
+  return groups > 2 * num_sms ? 0 : 2 * num_sms / groups;
+}
+
+size_t decode_q4_parts_bytes(int num_sms) {
+  return size_t(2 * num_sms) * 2 * 8 * 8 * kRec * sizeof(float);
+}
+size_t decode_q4_counter_bytes(int num_sms) { return size_t(2 * num_sms) * 2 * 8 * 2 * 4; }
+
+cudaError_t launch_decode_q4(const DecodeQ4Args& args, int num_sms, cudaStream_t s) {
+  DecodeQ4Args a = args;
+  const int group = a.hq / a.kv.hkv, groups = (a.kv.hkv + 7) / 8;
+  const void* fn = pick(group, a.fused != 0);
+  const int ctas = decode_q4_ctas(num_sms, a.kv.hkv);
+  if (!fn || ctas < 1) return cudaErrorInvalidValue;
+  // the groups' stages: 8 heads each, the last one the rest
+  const int rest = a.kv.hkv - 8 * (groups - 1);
+  a.stage_bytes = stage_bytes(rest);
+  if (groups > 1 && a.stage_bytes < stage_bytes(8)) a.stage_bytes = stage_bytes(8);
+  const int merge = warps_per_head(rest) > 1 ? kWarps * group * kRec * 4 : 0;
+  a.stages = (kRingBytes - merge) / a.stage_bytes;
+  if (a.stages > kMaxStages) a.stages = kMaxStages;
+  a.min_tiles = 1;
+  const size_t smem = size_t(a.stages) * a.stage_bytes + merge;
+  static PerDeviceOnce attrs[8];
+  const int slot = (group == 1 ? 0 : group == 2 ? 1 : group == 4 ? 2 : 3) * 2 + (a.fused ? 1 : 0);
+  const cudaError_t e = per_device_once(attrs[slot], [&](int&) {
+    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  });
+  if (e != cudaSuccess) return e;
+  void* argv[] = {&a};
+  return cudaLaunchKernel(fn, dim3(unsigned(ctas), unsigned(groups)), dim3(kThreads), argv, smem,
+                          s);
+}
+
+}  // namespace p2p

@@ -23,6 +23,7 @@ void lib_free(void* p, size_t bytes);
 int32_t* ctx_dev_err(const p2p_ctx* ctx);  // the device error word p2p_sync reports
 int32_t debug_wait_deficit();               // p2p_debug_set_wait_deficit's current value
 
+p2p_status ctx_serve_workspace(p2p_ctx* ctx, cudaStream_t s, const char* who, unsigned char** ws);
 // A rope table this context built knows its rows: it must hold max_len of them.
 p2p_status ctx_check_rope(p2p_ctx* ctx, const void* rope, int32_t max_len, const char* who);
 // serve_api.cu: the host-side checks of a cache layout, and the layout as the kernels take it.

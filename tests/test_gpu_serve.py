@@ -268,7 +268,12 @@ def attention64(c, q, past, rows, chunk):
     score by up to 2^-11 sum |q k| / 8 and so its weight by that share), and out to f16.  An error
     e of the weights' own shares moves out by at most sum p |v - out| e.  f32 sums of the scores
     (64 products, 2^-24 each, twice for the scale and offset of a 4-bit row) and of the weights
-    are below 2^-18 of the magnitudes."""
+    are below 2^-18 of the magnitudes.
+
+    A 4-bit value is lo + s c.  The decode sums (p s) c with p s rounded to f16 and p lo with p in
+    f32, apart from each other: the rounding of a weight by up to 2^-11 then moves out by
+    2^-11 w s c = 2^-11 w (v - lo), which |v| does not bound (v may be near 0 with lo far below):
+    sum w 2^-11 (v - lo) is added for single tokens over 4-bit caches."""
     outs, tols = [], []
     at = 0
     for i, (p, r) in enumerate(zip(past, rows)):
@@ -290,6 +295,9 @@ def attention64(c, q, past, rows, chunk):
         t = (w * e) @ v.abs() + o.abs() * (w * e).sum(-1, keepdim=True)
         t = t + (w @ v.abs()) * ((2.0 ** -11 if chunk else 0) + 2.0 ** -16)
         t = t + o.abs() * 2.0 ** -11 + 2.0 ** -24
+        if c.fmt == "q4" and not chunk:
+            lo = v.amin(-1, keepdim=True)  # a row's smallest value has code 0
+            t = t + 2.0 ** -11 * (w @ (v - lo))
         outs.append(o.permute(1, 0, 2))
         tols.append(t.permute(1, 0, 2))
     return torch.cat(outs).flatten(1), torch.cat(tols).flatten(1)
@@ -856,7 +864,7 @@ def test_a_server_run(ctx, fmt):
         qs = []
         for i in range(n):
             qs.append(prep(ctx, prm, emb[before[i].long()][None], nw, rope, pos[i])[0])
-        want, tol = attention64(c, torch.cat(qs), pos, [1] * n, True)
+        want, tol = attention64(c, torch.cat(qs), pos, [1] * n, fmt != "q4")
         assert_within(out, want, tol, f"step {s}")
         ref = plain_logits(out @ head, state[0], lens, prompts, [np.float32(1.3)] * n, [0.5] * n,
                            [0.25] * n, None, None, torch.float16)[1]
@@ -942,3 +950,33 @@ def test_another_stream_than_the_current_one(ctx):
     want, tol = attention64(c, q, [0], [513], True)
     assert_within(out, want, tol)
     assert torch.equal(out, out2)
+
+
+@pytest.mark.parametrize("heads", [(32, 8), (16, 2)])
+def test_decode_wait_runs_out(ctx, heads):
+    """A copy that never completes (more bytes expected than come): the kernel gives up after its
+    limit, writes nothing and reports it; the next call works, so no counter was left behind."""
+    import p2p_b200
+    hq, hkv = heads
+    past = [3000, 40, 700]
+    c = Cache(75, "q4", 16, hq, hkv, [p + 1 for p in past])
+    q = randh(gen(76), 3, hq * D)
+    out = torch.full_like(q, 7.0)
+    args = (c.prm, q, None, None, c.k, c.v, i32(past), out)
+    kw = dict(max_past=3000, fused_prep=False, **c.kw())
+    ctx.attn_decode_kv(*args, **kw)
+    ctx.sync()
+    good = out.clone()
+    out.fill_(7.0)
+    try:
+        p2p_b200.lib.p2p_debug_set_wait_deficit(16)
+        ctx.attn_decode_kv(*args, **kw)
+        with pytest.raises(p2p_b200.P2PError) as e:
+            ctx.sync()
+    finally:
+        p2p_b200.lib.p2p_debug_set_wait_deficit(0)
+    assert e.value.status == p2p_b200.P2P_ERR_TIMEOUT
+    assert (out == 7).all()
+    ctx.attn_decode_kv(*args, **kw)
+    ctx.sync()
+    assert torch.equal(out, good)
