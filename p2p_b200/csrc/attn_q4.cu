@@ -57,7 +57,7 @@ __host__ __device__ constexpr int stage_bytes(int hb) {
   return 2 * kBlock * warps_per_head(hb) * pitch_of(hb);
 }
 
-struct StageMeta {
+struct __align__(16) StageMeta {
   int z;        // sequence
   int key0;     // first key of the tile
   int valid;    // its keys
@@ -282,11 +282,11 @@ __device__ __forceinline__ int owner_of(long long i, long long total, int w) {
   return int(((i + 1) * w - 1) / total);
 }
 
-// A warp's part of one head: lane (gid, t) holds dims 8 gid .. 8 gid + 7 of heads 2t and 2t + 1.
-struct Part {
-  float acc[2][8], m[2], l[2];
-};
-__device__ __forceinline__ void store_part(float* rec, const Part& p, int g_count) {
+// A warp's part of one head's G query heads as a record [G][acc[64] | max | sum]: from the
+// fragments (acc[e][i]: dim 8 gid + i of head 2t + e) ...
+__device__ __forceinline__ void store_fragments(float* rec, const float (&acc)[2][8],
+                                                const float (&m)[2], const float (&l)[2],
+                                                int g_count) {
   const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -294,54 +294,104 @@ __device__ __forceinline__ void store_part(float* rec, const Part& p, int g_coun
     if (g >= g_count) continue;
     float* r = rec + g * kRec;
     *reinterpret_cast<float4*>(r + 8 * gid) =
-        make_float4(p.acc[e][0], p.acc[e][1], p.acc[e][2], p.acc[e][3]);
+        make_float4(acc[e][0], acc[e][1], acc[e][2], acc[e][3]);
     *reinterpret_cast<float4*>(r + 8 * gid + 4) =
-        make_float4(p.acc[e][4], p.acc[e][5], p.acc[e][6], p.acc[e][7]);
-    if (gid == 0) *reinterpret_cast<float2*>(r + 64) = make_float2(p.m[e], p.l[e]);
+        make_float4(acc[e][4], acc[e][5], acc[e][6], acc[e][7]);
+    if (gid == 0) *reinterpret_cast<float2*>(r + 64) = make_float2(m[e], l[e]);
   }
 }
-template <bool GLOBAL>
-__device__ __forceinline__ float4 load_f4(const float* p) {
-  if (GLOBAL) return __ldcg(reinterpret_cast<const float4*>(p));
-  return *reinterpret_cast<const float4*>(p);
-}
-// The join of n records (rec(i) of them), in order; a record with a negative sum makes the join one.
-template <bool GLOBAL, class Rec>
-__device__ __forceinline__ void join_parts(Part& p, int n, int g_count, Rec rec) {
-  const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int g = min(2 * t + e, g_count - 1);
-    float mx = kNegBig;
-    bool bad = false;
-    for (int i = 0; i < n; ++i) {
-      const float4 ml = load_f4<GLOBAL>(rec(i) + g * kRec + 64);
-      mx = fmaxf(mx, ml.x);
-      bad |= ml.y < 0.f;
-    }
-    float l = 0.f, acc[8] = {};
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float* r = rec(i) + g * kRec;
-      const float4 ml = load_f4<GLOBAL>(r + 64);
-      const float4 a = load_f4<GLOBAL>(r + 8 * gid), b = load_f4<GLOBAL>(r + 8 * gid + 4);
-      const float c = fast_exp2(ml.x - mx);
-      l = fmaf(ml.y, c, l);
-      acc[0] = fmaf(a.x, c, acc[0]);
-      acc[1] = fmaf(a.y, c, acc[1]);
-      acc[2] = fmaf(a.z, c, acc[2]);
-      acc[3] = fmaf(a.w, c, acc[3]);
-      acc[4] = fmaf(b.x, c, acc[4]);
-      acc[5] = fmaf(b.y, c, acc[5]);
-      acc[6] = fmaf(b.z, c, acc[6]);
-      acc[7] = fmaf(b.w, c, acc[7]);
-    }
-    p.m[e] = mx;
-    p.l[e] = bad ? -1.f : l;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p.acc[e][i] = acc[i];
+
+// ... or joined from several: piece lane + 32 k of the G x 16 16-byte pieces, so that a record is
+// one or a few coalesced loads of the warp.  Piece k belongs to head 2k + lane / 16.
+template <int G>
+struct Joined {
+  static constexpr int kPieces = (G + 1) / 2;
+  float4 acc[kPieces];
+  float m[kPieces], l[kPieces];  // l < 0: some page of the sequence was refused
+
+  __device__ __forceinline__ static bool has(int k) { return G > 1 || (threadIdx.x & 31) < 16; }
+  __device__ __forceinline__ static int head(int k) {
+    return G > 1 ? 2 * k + ((threadIdx.x & 31) >> 4) : 0;
   }
-}
+
+  // The n <= kJoin records rec(i), in order.  Lane i (and i + 16) first takes record i's maximum
+  // and sum, so that all of them are one load; then the accumulators, several records in flight.
+  template <bool GLOBAL, class Rec>
+  __device__ __forceinline__ void join(int n, Rec rec) {
+    const int lane = threadIdx.x & 31;
+    float c[kPieces];
+    const float* mine = rec(min(lane & 15, n - 1));
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      float2 ml;
+      if (GLOBAL) ml = __ldcg(reinterpret_cast<const float2*>(mine + head(k) * kRec + 64));
+      else ml = *reinterpret_cast<const float2*>(mine + head(k) * kRec + 64);
+      if ((lane & 15) >= n) ml = make_float2(kNegBig, 0.f);
+      m[k] = ml.x;
+      l[k] = ml.y;
+    }
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const uint32_t refused = __ballot_sync(0xffffffffu, l[k] < 0.f);
+      float mx = m[k];
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      c[k] = fast_exp2(m[k] - mx);
+      float sum = l[k] * c[k];
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      m[k] = mx;
+      l[k] = ((refused >> (lane & 16)) & 0xffffu) ? -1.f : sum;
+      acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    constexpr int kBatch = kPieces > 2 ? 4 : 8;
+    for (int i0 = 0; i0 < n; i0 += kBatch) {
+      float4 x[kBatch][kPieces];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float* r = rec(min(i0 + i, n - 1));
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+          const float4* p = reinterpret_cast<const float4*>(r + head(k) * kRec) + (lane & 15);
+          if (GLOBAL) x[i][k] = __ldcg(p);
+          else x[i][k] = *p;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+          // 0 behind the last record: lanes n .. 15 hold exp2(-1e30 - max)
+          const float w = __shfl_sync(0xffffffffu, c[k], min(i0 + i, 15) | (lane & 16));
+          if (i0 + i < n) {
+            acc[k].x = fmaf(x[i][k].x, w, acc[k].x);
+            acc[k].y = fmaf(x[i][k].y, w, acc[k].y);
+            acc[k].z = fmaf(x[i][k].z, w, acc[k].z);
+            acc[k].w = fmaf(x[i][k].w, w, acc[k].w);
+          }
+        }
+    }
+  }
+  __device__ __forceinline__ void store(float* rec) const {
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      if (!has(k)) continue;
+      float* r = rec + head(k) * kRec;
+      reinterpret_cast<float4*>(r)[threadIdx.x & 15] = acc[k];
+      if ((threadIdx.x & 15) == 0) *reinterpret_cast<float2*>(r + 64) = make_float2(m[k], l[k]);
+    }
+  }
+  __device__ __forceinline__ void write(__half* out) const {  // [G][64]
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      if (!has(k) || l[k] < 0.f) continue;
+      const float inv = __fdiv_rn(1.f, l[k]);
+      reinterpret_cast<uint2*>(out + head(k) * 64)[threadIdx.x & 15] =
+          make_uint2(pack_h2(acc[k].x * inv, acc[k].y * inv),
+                     pack_h2(acc[k].z * inv, acc[k].w * inv));
+    }
+  }
+};
 
 // The tiles of a CTA's part, in order, sequence by sequence.
 struct Walk {
@@ -378,7 +428,58 @@ __device__ __forceinline__ bool last_of(int32_t* counter, int n) {
   return true;
 }
 
-template <int G, bool FUSED>
+// Where the CTAs' parts lie in the list of tiles and their records in the workspace.
+struct Parts {
+  float* parts;
+  int32_t* counters;
+  long long total;
+  int n_parts;
+  // record of head h of CTA b (of gridDim.x per group): slot 0 its first sequence, 1 its last
+  __device__ __forceinline__ int64_t place(int b, int slot, int h) const {
+    return ((int64_t(blockIdx.y) * gridDim.x + b) * 2 + slot) * 8 + h;
+  }
+};
+
+// After this warp's record of head h of a sequence (tiles g0 .. g0 + tiles - 1 of the list) is
+// stored: the last warp to arrive joins the records and writes the output rows `out` [G][64].
+template <int G>
+__device__ __forceinline__ void join_sequence(const Parts& x, int h, long long g0, int tiles,
+                                              __half* out) {
+  // the sequence spans CTAs first .. last; it is each one's first part, except that `first` may
+  // begin with another sequence
+  const int first = owner_of(g0, x.total, x.n_parts),
+            last = owner_of(g0 + tiles - 1, x.total, x.n_parts);
+  const int n = last - first + 1, slot0 = x.total * first / x.n_parts < g0 ? 1 : 0;
+  auto place = [&](int i) { return x.place(first + i, i == 0 ? slot0 : 0, h); };
+  auto rec = [&](int i) { return x.parts + place(i) * (G * kRec); };
+  const int lead = (int(blockIdx.x) - first) / kJoin * kJoin, n_here = min(kJoin, n - lead);
+  if (!last_of(x.counters + 2 * place(lead), n_here)) return;
+  Joined<G> j;
+  j.template join<true>(n_here, [&](int k) { return rec(lead + k); });
+  if (n > kJoin) {
+    j.store(rec(lead));
+    const int n_lead = (n + kJoin - 1) / kJoin;
+    if (!last_of(x.counters + 2 * place(0) + 1, n_lead)) return;
+    // more than kJoin^2 CTAs are joined a stretch of leaders at a time, into the first of each
+    int step = kJoin;
+    if (n_lead > kJoin) {
+      for (int k0 = 0; k0 < n_lead; k0 += kJoin) {
+        j.template join<true>(min(kJoin, n_lead - k0),
+                              [&](int k) { return rec((k0 + k) * kJoin); });
+        j.store(rec(k0 * kJoin));
+      }
+      __threadfence();
+      __syncwarp();
+      step = kJoin * kJoin;
+    }
+    j.template join<true>((n + step - 1) / step, [&](int k) { return rec(k * step); });
+  }
+  j.write(out);
+}
+
+// HB: the kv heads of every group when that number is 8, 4, 2 or 1 (row pitches are then constants
+// in the addresses), or 0.
+template <int G, bool FUSED, int HB>
 __global__ void __launch_bounds__(kThreads, 2)
     attn_decode_q4_kernel(const __grid_constant__ DecodeQ4Args a) {
   extern __shared__ __align__(128) unsigned char ring[];
@@ -388,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   __shared__ uint32_t unit_s[FUSED ? kWarps : 1][2][9];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grp = blockIdx.y;
-  const int hb = min(8, a.kv.hkv - 8 * grp), wph = warps_per_head(hb);
+  const int hb = HB ? HB : min(8, a.kv.hkv - 8 * grp), wph = warps_per_head(hb);
   const int tile = kBlock * wph, pitch = pitch_of(hb), sbytes = 2 * tile * pitch;
   const int n_groups = gridDim.y;
 
@@ -451,13 +552,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     // keys of one contiguous run: the cache's rows are whole tokens, so a run can span keys only
     // when one group of heads is the whole row
     const int run = n_groups > 1 ? 1 : a.kv.table ? min(1 << a.kv.shift, tile) : tile;
-    int issued = 0;
+    int issued = 0, st = 0;
+    uint32_t round = 0;  // parity of the stages' current use
     for (int i = 0; i < n_tiles; ++i, ++w.t) {
       w.settle();
-      const int st = i % a.stages;
       if (i >= a.stages) {
         bool ok = true;
-        if (lane == 0) ok = wait_bar(s, &s.empty[st], (i / a.stages - 1) & 1, a.err);
+        if (lane == 0) ok = wait_bar(s, &s.empty[st], round ^ 1, a.err);
         if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) break;
       }
       const int z = w.z, key0 = w.t * tile, len = w.sp.past + 1, valid = min(tile, len - key0);
@@ -495,6 +596,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
       issued = i + 1;
+      if (++st == a.stages) {
+        st = 0;
+        round ^= 1;
+      }
     }
     if (s.abort_flag) {  // let the copies already in flight land before the CTA exits
       for (int i = max(0, issued - a.stages); i < issued; ++i) {
@@ -512,79 +617,76 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool active = sub < wph;
   const int kh = grp * 8 + h;
   const float scale24 = a.scale_log2 * 16777216.f;
-  float* merge = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // [warp][G][kRec]
   Query q;
   State state;
-  bool bad = false, seg_first = true;
+  bool bad = false;
   int segs = 0;  // parts of sequences ended
+  const Parts x{a.parts, a.counters, total, parts};
+  float* merge = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // [warp][G][kRec]
+  auto out_of = [&](int z) { return a.out + int64_t(z) * a.ld_o + kh * G * 64; };
+  auto whole = [&](long long g0, int tiles) { return lo <= g0 && lo + n_tiles >= g0 + tiles; };
   // Ends this CTA's part of sequence z (whose `tiles` tiles begin at g0 of the list): the warps of
-  // a head meet, and the sequence's output is written or its record left for the last to arrive.
-  auto finish = [&](Part& p, int z, long long g0, int tiles) {
-    if (wph > 1) {  // the warps of a head meet in shared memory
-      if (active) store_part(merge + warp * G * kRec, p, G);
+  // a head meet, and the output is written, or a record when other CTAs have parts of it too.
+  auto end_part = [&](const float (&acc)[2][8], const float (&m)[2], const float (&l)[2], int z,
+                      long long g0, int tiles, bool seg_first) {
+    float* own = x.parts + x.place(b, seg_first ? 0 : 1, h) * (G * kRec);
+    if (wph > 1) {
+      if (active) store_fragments(merge + warp * G * kRec, acc, m, l, G);
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (sub == 0)
-        join_parts<false>(p, wph, G, [&](int k) { return merge + (k * hb + h) * G * kRec; });
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-    }
-    const bool whole_seq = lo <= g0 && lo + n_tiles >= g0 + tiles;
-    bool write = active && sub == 0;
-    if (!whole_seq && write) {
-      const int slot = seg_first ? 0 : 1;
-      const int first = owner_of(g0, total, parts), last = owner_of(g0 + tiles - 1, total, parts);
-      const int n = last - first + 1, me = b - first;
-      // CTA first + i: the sequence is its first part, except that `first` may begin with another
-      const int slot0 = total * first / parts < g0 ? 1 : 0;
-      auto place = [&](int i) {
-        return ((int64_t(grp) * gridDim.x + first + i) * 2 + (i == 0 ? slot0 : 0)) * 8 + h;
-      };
-      auto rec = [&](int i) { return a.parts + place(i) * (G * kRec); };
-      store_part(a.parts + (((int64_t(grp) * gridDim.x + b) * 2 + slot) * 8 + h) * (G * kRec), p,
-                 G);
-      const int lead = me / kJoin * kJoin, n_here = min(kJoin, n - lead);
-      write = last_of(a.counters + 2 * place(lead), n_here);
-      if (write) join_parts<true>(p, n_here, G, [&](int k) { return rec(lead + k); });
-      if (write && n > kJoin) {
-        store_part(rec(lead), p, G);
-        const int n_lead = (n + kJoin - 1) / kJoin;
-        write = last_of(a.counters + 2 * place(0) + 1, n_lead);
-        if (write) join_parts<true>(p, n_lead, G, [&](int k) { return rec(k * kJoin); });
+      if (sub == 0) {
+        Joined<G> j;
+        j.template join<false>(wph, [&](int k) { return merge + (k * hb + h) * G * kRec; });
+        if (whole(g0, tiles)) j.write(out_of(z));
+        else j.store(own);
       }
-    }
-    if (write) {
-      const int gid = lane >> 2, t = lane & 3;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    } else if (active) {
+      if (!whole(g0, tiles)) {
+        store_fragments(own, acc, m, l, G);
+      } else {
+        const int gid = lane >> 2, t = lane & 3;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (2 * t + e >= G || p.l[e] < 0.f) continue;
-        const float inv = __fdiv_rn(1.f, p.l[e]);
-        *reinterpret_cast<uint4*>(a.out + int64_t(z) * a.ld_o + (kh * G + 2 * t + e) * 64 +
-                                  8 * gid) =
-            make_uint4(pack_h2(p.acc[e][0] * inv, p.acc[e][1] * inv),
-                       pack_h2(p.acc[e][2] * inv, p.acc[e][3] * inv),
-                       pack_h2(p.acc[e][4] * inv, p.acc[e][5] * inv),
-                       pack_h2(p.acc[e][6] * inv, p.acc[e][7] * inv));
+        for (int e = 0; e < 2; ++e) {
+          if (2 * t + e >= G || l[e] < 0.f) continue;
+          const float inv = __fdiv_rn(1.f, l[e]);
+          *reinterpret_cast<uint4*>(out_of(z) + (2 * t + e) * 64 + 8 * gid) =
+              make_uint4(pack_h2(acc[e][0] * inv, acc[e][1] * inv),
+                         pack_h2(acc[e][2] * inv, acc[e][3] * inv),
+                         pack_h2(acc[e][4] * inv, acc[e][5] * inv),
+                         pack_h2(acc[e][6] * inv, acc[e][7] * inv));
+        }
       }
     }
-    seg_first = false;
-    ++segs;
   };
-  int i = 0;
+  int i = 0, st = 0;
+  uint32_t round = 0;
+  int z = s.z0, tiles = 0;  // the sequence at hand
+  long long g0 = 0;
+  state.clear();
+  q = Query{};
   for (; i < n_tiles; ++i) {
-    const int st = i % a.stages;
-    const bool ok = wait_bar(s, &s.full[st], (i / a.stages) & 1, a.err);
+    const bool ok = wait_bar(s, &s.full[st], round, a.err);
     if (!__all_sync(0xffffffffu, ok)) break;
-    const StageMeta m = s.meta[st];
+    const StageMeta& m = s.meta[st];
+    const int4 head = *reinterpret_cast<const int4*>(&m);  // z, key0, valid, flags
+    const int flags = head.w;
+    int pos = 0;
+    if (flags & (kFirst | kLast)) {
+      z = head.x;
+      pos = m.pos;
+      tiles = m.tiles;
+      g0 = m.g;
+    }
     unsigned char* ks = ring + st * sbytes + sub * kBlock * pitch + h * kQ4UnitBytes;
     unsigned char* vs = ks + tile * pitch;
-    const bool has_new = FUSED && m.key0 + m.valid == m.pos + 1;
-    if (m.flags & kFirst) {
-      state.clear();
-      bad = false;
+    // the sequence's last tile ends this part
+    const bool has_new = FUSED && (flags & kLast) && head.y + head.z == pos + 1;
+    if (flags & kFirst) {
       if (active) {
-        const __half* row = a.q + int64_t(m.z) * a.ld_q;
+        const __half* row = a.q + int64_t(z) * a.ld_q;
         if (FUSED) {
-          const float cs = to_f32(a.rope[int64_t(m.pos) * 64 + lane]);
-          const float sn = to_f32(a.rope[int64_t(m.pos) * 64 + 32 + lane]);
+          const float cs = to_f32(a.rope[int64_t(pos) * 64 + lane]);
+          const float sn = to_f32(a.rope[int64_t(pos) * 64 + 32 + lane]);
           const __half* src = row + kh * G * 64;
           float x[G][2];
 #pragma unroll
@@ -610,15 +712,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     }
-    if (m.flags & kBad) bad = true;
-    const int valid = m.valid - sub * kBlock;
+    if (flags & kBad) bad = true;
+    const int valid = head.z - sub * kBlock;
     if (active && valid > 0 && !bad) {
       if (has_new && valid <= kBlock) {
         // the new token's unit of this head: normed, rotated, quantised, into the cache and over
         // the stage's row (which the copy left out)
-        const __half* row = a.q + int64_t(m.z) * a.ld_q;
-        const float cs = to_f32(a.rope[int64_t(m.pos) * 64 + lane]);
-        const float sn = to_f32(a.rope[int64_t(m.pos) * 64 + 32 + lane]);
+        const __half* row = a.q + int64_t(z) * a.ld_q;
+        const float cs = to_f32(a.rope[int64_t(pos) * 64 + lane]);
+        const float sn = to_f32(a.rope[int64_t(pos) * 64 + 32 + lane]);
         const __half* kn = row + (a.hq + kh) * 64;
         const __half* vn = row + (a.hq + a.kv.hkv + kh) * 64;
         float r0, r1;
@@ -643,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (lane < 18) {
           const int pool = lane / 9, w = lane % 9;
           const uint32_t v = unit_s[warp][pool][w];
-          const int64_t at = kv_row(a.kv, m.z, m.pos);
+          const int64_t at = kv_row(a.kv, z, pos);
           reinterpret_cast<uint32_t*>((pool ? a.kv.v : a.kv.k) + at * a.kv.row_bytes +
                                       kh * kQ4UnitBytes)[w] = v;
           reinterpret_cast<uint32_t*>((pool ? vs : ks) + (valid - 1) * pitch)[w] = v;
@@ -655,10 +757,14 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&s.empty[st]);
-    if (!(m.flags & kLast)) continue;
+    if (++st == a.stages) {
+      st = 0;
+      round ^= 1;
+    }
+    if (!(flags & kLast)) continue;
 
     // ---- this CTA's part of the sequence is done
-    Part p;
+    float acc[2][8], mx[2], sum[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -666,44 +772,77 @@ __global__ void __launch_bounds__(kThreads, 2)
         state.l[e] += __shfl_xor_sync(0xffffffffu, state.l[e], o);
         state.bias[e] += __shfl_xor_sync(0xffffffffu, state.bias[e], o);
       }
-      p.m[e] = state.m[e];
-      p.l[e] = bad ? -1.f : state.l[e];
+      mx[e] = state.m[e];
+      sum[e] = bad ? -1.f : state.l[e];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        p.acc[e][2 * k] = fmaf(state.o[k][e], 4194304.f, state.bias[e]);         // 2^24 / 4
-        p.acc[e][2 * k + 1] = fmaf(state.o[k][2 + e], 262144.f, state.bias[e]);  // 2^20 / 4
+        acc[e][2 * k] = fmaf(state.o[k][e], 4194304.f, state.bias[e]);         // 2^24 / 4
+        acc[e][2 * k + 1] = fmaf(state.o[k][2 + e], 262144.f, state.bias[e]);  // 2^20 / 4
       }
     }
-    finish(p, m.z, m.g, m.tiles);
+    end_part(acc, mx, sum, z, g0, tiles, segs == 0);
+    ++segs;
+    state.clear();
+    q = Query{};
+    bad = false;
   }
-  if (i == n_tiles) return;
-  // A wait ran out: the parts that are left end as bad ones, so that no other warp or CTA waits or
-  // joins in vain and the counters return to zero.
-  Walk w(a.kv, a.at, tile, s.z0, s.t0);
-  int done = segs;
-  for (int k = 0; k < n_tiles; ++k, ++w.t) {
-    w.settle();
-    if (!(k == n_tiles - 1 || w.t == w.tiles - 1) || done-- > 0) continue;
-    Part p = {};
-    p.m[0] = p.m[1] = kNegBig;
-    p.l[0] = p.l[1] = -1.f;
-    finish(p, w.z, lo + k - w.t, w.tiles);
+  if (i < n_tiles) {
+    // A wait ran out: the parts that are left end as bad ones, so that no other warp or CTA waits
+    // or joins in vain and the counters return to zero.
+    Walk w(a.kv, a.at, tile, s.z0, s.t0);
+    int done = segs;
+    for (int k = 0; k < n_tiles; ++k, ++w.t) {
+      w.settle();
+      if (!(k == n_tiles - 1 || w.t == w.tiles - 1) || done-- > 0) continue;
+      const float acc[2][8] = {}, mx[2] = {kNegBig, kNegBig}, sum[2] = {-1.f, -1.f};
+      z = w.z;
+      g0 = lo + k - w.t;
+      tiles = w.tiles;
+      end_part(acc, mx, sum, z, g0, tiles, segs == 0);
+      ++segs;
+    }
   }
+  // The sequences that straddle CTAs: the first part's and the last one's.  They are joined here,
+  // behind the loop, which keeps its registers to itself; nothing waits for a join.
+  if (!active || sub != 0) return;
+  if (segs > 1) {
+    const SeqSpan sp = seq_span(a.kv, a.at, s.z0);
+    const int t0 = (sp.past + tile) / tile;
+    if (!whole(lo - s.t0, t0)) join_sequence<G>(x, h, lo - s.t0, t0, out_of(s.z0));
+  }
+  if (!whole(g0, tiles)) join_sequence<G>(x, h, g0, tiles, out_of(z));
 }
 
-template <int G>
+struct Pick {
+  const void* fn;
+  int id;  // of 4 groups x 2 x 5 head counts
+};
+template <int G, int HB>
 const void* pick(bool fused) {
-  return fused ? reinterpret_cast<const void*>(&attn_decode_q4_kernel<G, true>)
-               : reinterpret_cast<const void*>(&attn_decode_q4_kernel<G, false>);
+  return fused ? reinterpret_cast<const void*>(&attn_decode_q4_kernel<G, true, HB>)
+               : reinterpret_cast<const void*>(&attn_decode_q4_kernel<G, false, HB>);
 }
-const void* pick(int group, bool fused) {
-  switch (group) {
-    case 1: return pick<1>(fused);
-    case 2: return pick<2>(fused);
-    case 4: return pick<4>(fused);
-    case 8: return pick<8>(fused);
-    default: return nullptr;
+template <int G>
+Pick pick(bool fused, int hb) {
+  const int id = fused ? 5 : 0;
+  switch (hb) {
+    case 8: return {pick<G, 8>(fused), id};
+    case 4: return {pick<G, 4>(fused), id + 1};
+    case 2: return {pick<G, 2>(fused), id + 2};
+    case 1: return {pick<G, 1>(fused), id + 3};
+    default: return {pick<G, 0>(fused), id + 4};
   }
+}
+Pick pick(int group, bool fused, int hkv) {
+  const int hb = hkv % 8 == 0 ? 8 : hkv < 8 ? hkv : 0;
+  Pick p{nullptr, 0};
+  switch (group) {
+    case 1: p = pick<1>(fused, hb); break;
+    case 2: p = pick<2>(fused, hb); p.id += 10; break;
+    case 4: p = pick<4>(fused, hb); p.id += 20; break;
+    case 8: p = pick<8>(fused, hb); p.id += 30; break;
+  }
+  return p;
 }
 
 constexpr int kRingBytes = 94 * 1024;  // two CTAs per SM
@@ -723,7 +862,8 @@ size_t decode_q4_counter_bytes(int num_sms) { return size_t(2 * num_sms) * 2 * 8
 cudaError_t launch_decode_q4(const DecodeQ4Args& args, int num_sms, cudaStream_t s) {
   DecodeQ4Args a = args;
   const int group = a.hq / a.kv.hkv, groups = (a.kv.hkv + 7) / 8;
-  const void* fn = pick(group, a.fused != 0);
+  const Pick k = pick(group, a.fused != 0, a.kv.hkv);
+  const void* fn = k.fn;
   const int ctas = decode_q4_ctas(num_sms, a.kv.hkv);
   if (!fn || ctas < 1) return cudaErrorInvalidValue;
   // the groups' stages: 8 heads each, the last one the rest
@@ -735,9 +875,8 @@ cudaError_t launch_decode_q4(const DecodeQ4Args& args, int num_sms, cudaStream_t
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   a.min_tiles = 1;
   const size_t smem = size_t(a.stages) * a.stage_bytes + merge;
-  static PerDeviceOnce attrs[8];
-  const int slot = (group == 1 ? 0 : group == 2 ? 1 : group == 4 ? 2 : 3) * 2 + (a.fused ? 1 : 0);
-  const cudaError_t e = per_device_once(attrs[slot], [&](int&) {
+  static PerDeviceOnce attrs[40];
+  const cudaError_t e = per_device_once(attrs[k.id], [&](int&) {
     return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
   });
   if (e != cudaSuccess) return e;
