@@ -965,8 +965,8 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
     unsigned char* ws = nullptr;
     st = p2p::ctx_serve_workspace(ctx, s, "decode_kv", &ws);
     if (st != P2P_OK) return st;
-    q.counters = reinterpret_cast<int32_t*>(ws);
-    q.parts = reinterpret_cast<float*>(ws + p2p::decode_q4_counter_bytes(ctx->num_sms));
+    q.joins = reinterpret_cast<int4*>(ws);
+    q.parts = reinterpret_cast<float*>(ws + p2p::decode_q4_join_bytes(ctx->num_sms));
     q.wait_deficit = g_wait_deficit.load();
     cudaError_t e = p2p::launch_decode_q4(q, ctx->num_sms, s);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "decode_kv launch");
@@ -1399,8 +1399,8 @@ p2p_status check_ragged(p2p_ctx* ctx, const p2p_attn_params* prm, const void* qk
   return P2P_OK;
 }
 
-// The context's workspace of the 4-bit decode and the prompt-chunk attention (counters, zero
-// between launches, then records).  The first call allocates it, which a stream capture forbids.
+// The context's workspace of the 4-bit decode and the prompt-chunk attention; nothing in it
+// outlives a call.  The first call allocates it, which a stream capture forbids.
 p2p_status ctx_serve_workspace(p2p_ctx* ctx, cudaStream_t s, const char* who,
                                unsigned char** ws) {
   if (!ctx->serve_ws) {
@@ -1414,18 +1414,11 @@ p2p_status ctx_serve_workspace(p2p_ctx* ctx, cudaStream_t s, const char* who,
       return fail(ctx, P2P_ERR_INVALID_ARG,
                   "%s: the first call of a context makes its workspace and cannot be captured",
                   who);
-    const size_t counters = decode_q4_counter_bytes(ctx->num_sms);
-    const size_t bytes = counters + decode_q4_parts_bytes(ctx->num_sms);
+    const size_t bytes = decode_q4_join_bytes(ctx->num_sms) + decode_q4_parts_bytes(ctx->num_sms);
     void* p = nullptr;
     if (dev_alloc(&p, bytes) != cudaSuccess) {
       cudaGetLastError();
       return fail(ctx, P2P_ERR_OOM, "%s: workspace of %zu bytes", who, bytes);
-    }
-    e = cudaMemset(p, 0, counters);
-    if (e == cudaSuccess) e = cudaDeviceSynchronize();
-    if (e != cudaSuccess) {
-      dev_free(p, bytes);
-      return cuda_fail(ctx, e, who);
     }
     ctx->serve_ws = p;
     ctx->serve_ws_bytes = bytes;

@@ -10,8 +10,8 @@
 // nibbles' factor 16 goes into q (divided by 16 for those dims; exact down to f16's subnormals)
 // and into the final scale of the odd output dims.
 //     S^T[16 keys x 8 heads] = C_K[16 x 64] . Q^T[64 x 8],   O^T[64 x 8] += C_V^T[64 x 16] . P'^T
-// P' = p * s * 4 is rounded to f16 (2^-11 of a weight, below the rounding of the f16 output; the
-// factor 4 uses the range left by s <= 8734, so weights keep their bits down to small scales);
+// P' = p * s is rounded to f16 (2^-11 of a weight, below the rounding of the f16 output; p goes up to
+// 4, which uses the range left by s <= 8734, so weights keep their bits down to small scales);
 // p, the sums of p and of p * lo, the running maximum and O stay in f32.
 //
 // Split.  All sequences' tiles, in order, form one list that is cut into equal parts, one per CTA
@@ -19,8 +19,13 @@
 // does not depend on them.  A CTA works on up to 8 kv heads of its tiles, one warp per head (more
 // warps per head when there are fewer heads), because a page's rows are contiguous over heads:
 // one bulk copy per page and pool fetches them, issued by a producer warp into a ring of stages.
-// Sequences that straddle CTAs are joined by the last warp to arrive per head, in two levels of at
-// most kJoin records each; the order of the sums is that of the CTAs, so results repeat bit for bit.
+// Sequences that straddle CTAs leave a record per CTA, head and query head, which a second kernel
+// joins; it is launched as a programmatic dependent, so it is resident when the first one ends.  The
+// order of the sums is that of the CTAs, so results repeat bit for bit, and nothing in the
+// workspace outlives a call.
+// Measured on the way (4 sequences, 390k keys, 8 kv heads x 4): joining by the last warp to arrive
+// (a fence, an atomic and the loads of up to 16 records per level, all one after the other) took
+// 8 us of a short call and 19 us of this one.
 #include "common.cuh"
 #include "kernels.h"
 #include "kv_view.cuh"
@@ -45,6 +50,8 @@ constexpr int kMaxStages = 8;
 constexpr int kRec = 68;                       // acc[64], max, sum, 2 pad: 17 16-byte pieces
 constexpr int kJoin = 16;                      // records joined by one warp
 constexpr float kNegBig = -1e30f;
+// Weights are 2^(score - m) with m two below the maximum, so at most 4: p * s <= 4 * 8734 < 65504
+constexpr float kUp = 2.f;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 
 // Warps per head for a CTA of hb heads (1 .. 8); its tile is kBlock keys per such warp.
@@ -161,7 +168,7 @@ __device__ __forceinline__ void load_query(const __half* q, float scale_log2, Qu
 }
 
 struct State {
-  float m[2], l[2], bias[2];  // heads 2t, 2t+1: maximum (of the warp), partial sums (of the lane)
+  float m[2], l[2], bias[2];  // heads 2t, 2t+1: reference (of the warp), partial sums (of the lane)
   float o[4][4];              // dims 8 gid + 2i (even codes) and 8 gid + 2i + 1, heads 2t, 2t+1
   __device__ __forceinline__ void clear() {
     m[0] = m[1] = kNegBig;
@@ -212,15 +219,15 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
   const float mb0 = fmaxf(fmaxf(sc[0][0], sc[1][0]), fmaxf(sc[2][0], sc[3][0]));
   const float mb1 = fmaxf(fmaxf(sc[0][1], sc[1][1]), fmaxf(sc[2][1], sc[3][1]));
   // the maximum rarely grows after the first blocks: only then is it joined and O rescaled
-  if (__any_sync(0xffffffffu, mb0 > st.m[0] || mb1 > st.m[1])) {
+  if (__any_sync(0xffffffffu, mb0 - kUp > st.m[0] || mb1 - kUp > st.m[1])) {
     float n0 = mb0, n1 = mb1;
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) {
       n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
       n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
     }
-    n0 = fmaxf(n0, st.m[0]);
-    n1 = fmaxf(n1, st.m[1]);
+    n0 = fmaxf(n0 - kUp, st.m[0]);
+    n1 = fmaxf(n1 - kUp, st.m[1]);
     const float c0 = fast_exp2(st.m[0] - n0), c1 = fast_exp2(st.m[1] - n1);
     st.m[0] = n0;
     st.m[1] = n1;
@@ -247,7 +254,6 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
       if (valid < kBlock && 16 * j + 8 * k + row >= valid) pv = 0u;
       float s, lo;
       q4_unpack(pv, s, lo);
-      s *= 4.f;
       const float p0 = fast_exp2(sc[2 * j + k][0] - st.m[0]);
       const float p1 = fast_exp2(sc[2 * j + k][1] - st.m[1]);
       st.l[0] += p0;
@@ -275,11 +281,6 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
     mma16816(st.o[3], (y >> 8) & kEven, (y >> 8) & kOdd, (y2 >> 8) & kEven, (y2 >> 8) & kOdd, b0,
              b1);
   }
-}
-
-// The CTA (of w) that owns tile i of `total`: part b starts at tile total * b / w.
-__device__ __forceinline__ int owner_of(long long i, long long total, int w) {
-  return int(((i + 1) * w - 1) / total);
 }
 
 // A warp's part of one head's G query heads as a record [G][acc[64] | max | sum]: from the
@@ -314,6 +315,27 @@ struct Joined {
     return G > 1 ? 2 * k + ((threadIdx.x & 31) >> 4) : 0;
   }
 
+  __device__ __forceinline__ void none() {
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      m[k] = kNegBig;
+      l[k] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void add(const Joined& x) {
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const float mx = fmaxf(m[k], x.m[k]);
+      const float c = fast_exp2(m[k] - mx), d = fast_exp2(x.m[k] - mx);
+      l[k] = l[k] < 0.f || x.l[k] < 0.f ? -1.f : fmaf(l[k], c, x.l[k] * d);
+      m[k] = mx;
+      acc[k].x = fmaf(acc[k].x, c, x.acc[k].x * d);
+      acc[k].y = fmaf(acc[k].y, c, x.acc[k].y * d);
+      acc[k].z = fmaf(acc[k].z, c, x.acc[k].z * d);
+      acc[k].w = fmaf(acc[k].w, c, x.acc[k].w * d);
+    }
+  }
   // The n <= kJoin records rec(i), in order.  Lane i (and i + 16) first takes record i's maximum
   // and sum, so that all of them are one load; then the accumulators, several records in flight.
   template <bool GLOBAL, class Rec>
@@ -415,66 +437,10 @@ struct Walk {
   }
 };
 
-// Announces this warp's record at `counter`; true for the last of n (which resets it).
-__device__ __forceinline__ bool last_of(int32_t* counter, int n) {
-  __threadfence();
-  __syncwarp();
-  int old = 0;
-  if ((threadIdx.x & 31) == 0) old = atomicAdd(counter, 1);
-  old = __shfl_sync(0xffffffffu, old, 0);
-  if (old != n - 1) return false;
-  if ((threadIdx.x & 31) == 0) *counter = 0;
-  __threadfence();
-  return true;
-}
-
-// Where the CTAs' parts lie in the list of tiles and their records in the workspace.
-struct Parts {
-  float* parts;
-  int32_t* counters;
-  long long total;
-  int n_parts;
-  // record of head h of CTA b (of gridDim.x per group): slot 0 its first sequence, 1 its last
-  __device__ __forceinline__ int64_t place(int b, int slot, int h) const {
-    return ((int64_t(blockIdx.y) * gridDim.x + b) * 2 + slot) * 8 + h;
-  }
-};
-
-// After this warp's record of head h of a sequence (tiles g0 .. g0 + tiles - 1 of the list) is
-// stored: the last warp to arrive joins the records and writes the output rows `out` [G][64].
-template <int G>
-__device__ __forceinline__ void join_sequence(const Parts& x, int h, long long g0, int tiles,
-                                              __half* out) {
-  // the sequence spans CTAs first .. last; it is each one's first part, except that `first` may
-  // begin with another sequence
-  const int first = owner_of(g0, x.total, x.n_parts),
-            last = owner_of(g0 + tiles - 1, x.total, x.n_parts);
-  const int n = last - first + 1, slot0 = x.total * first / x.n_parts < g0 ? 1 : 0;
-  auto place = [&](int i) { return x.place(first + i, i == 0 ? slot0 : 0, h); };
-  auto rec = [&](int i) { return x.parts + place(i) * (G * kRec); };
-  const int lead = (int(blockIdx.x) - first) / kJoin * kJoin, n_here = min(kJoin, n - lead);
-  if (!last_of(x.counters + 2 * place(lead), n_here)) return;
-  Joined<G> j;
-  j.template join<true>(n_here, [&](int k) { return rec(lead + k); });
-  if (n > kJoin) {
-    j.store(rec(lead));
-    const int n_lead = (n + kJoin - 1) / kJoin;
-    if (!last_of(x.counters + 2 * place(0) + 1, n_lead)) return;
-    // more than kJoin^2 CTAs are joined a stretch of leaders at a time, into the first of each
-    int step = kJoin;
-    if (n_lead > kJoin) {
-      for (int k0 = 0; k0 < n_lead; k0 += kJoin) {
-        j.template join<true>(min(kJoin, n_lead - k0),
-                              [&](int k) { return rec((k0 + k) * kJoin); });
-        j.store(rec(k0 * kJoin));
-      }
-      __threadfence();
-      __syncwarp();
-      step = kJoin * kJoin;
-    }
-    j.template join<true>((n + step - 1) / step, [&](int k) { return rec(k * step); });
-  }
-  j.write(out);
+// The record of head h of CTA b (of `ctas` per group of heads): slot 0 its first sequence, 1 its
+// last.
+__device__ __forceinline__ int64_t record_of(int grp, int ctas, int b, int slot, int h) {
+  return ((int64_t(grp) * ctas + b) * 2 + slot) * 8 + h;
 }
 
 // HB: the kv heads of every group when that number is 8, 4, 2 or 1 (row pitches are then constants
@@ -528,6 +494,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int parts = int(min(static_cast<long long>(gridDim.x),
                             (total + a.min_tiles - 1) / a.min_tiles));
   const int b = blockIdx.x;
+  launch_dependents();  // the joining kernel may take the slots that become free
+  if (tid == 0) a.joins[grp * gridDim.x + b] = make_int4(-1, 0, 0, 0);
   if (b >= parts) return;
   const long long lo = total * b / parts;
   const int n_tiles = int(total * (b + 1) / parts - lo);
@@ -621,7 +589,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   State state;
   bool bad = false;
   int segs = 0;  // parts of sequences ended
-  const Parts x{a.parts, a.counters, total, parts};
   float* merge = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // [warp][G][kRec]
   auto out_of = [&](int z) { return a.out + int64_t(z) * a.ld_o + kh * G * 64; };
   auto whole = [&](long long g0, int tiles) { return lo <= g0 && lo + n_tiles >= g0 + tiles; };
@@ -629,7 +596,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   // a head meet, and the output is written, or a record when other CTAs have parts of it too.
   auto end_part = [&](const float (&acc)[2][8], const float (&m)[2], const float (&l)[2], int z,
                       long long g0, int tiles, bool seg_first) {
-    float* own = x.parts + x.place(b, seg_first ? 0 : 1, h) * (G * kRec);
+    float* own = a.parts + record_of(grp, gridDim.x, b, seg_first ? 0 : 1, h) * (G * kRec);
+    if (tid == 0 && lo <= g0 && !whole(g0, tiles)) {  // it begins here: what there is to join
+      const int last = int(((g0 + tiles) * parts - 1) / total);  // the CTA of its last tile
+      a.joins[grp * gridDim.x + b] = make_int4(z, seg_first ? 0 : 1, last - b + 1, 0);
+    }
     if (wph > 1) {
       if (active) store_fragments(merge + warp * G * kRec, acc, m, l, G);
       asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -776,8 +747,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       sum[e] = bad ? -1.f : state.l[e];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        acc[e][2 * k] = fmaf(state.o[k][e], 4194304.f, state.bias[e]);         // 2^24 / 4
-        acc[e][2 * k + 1] = fmaf(state.o[k][2 + e], 262144.f, state.bias[e]);  // 2^20 / 4
+        acc[e][2 * k] = fmaf(state.o[k][e], 16777216.f, state.bias[e]);         // 2^24
+        acc[e][2 * k + 1] = fmaf(state.o[k][2 + e], 1048576.f, state.bias[e]);  // 2^20
       }
     }
     end_part(acc, mx, sum, z, g0, tiles, segs == 0);
@@ -802,15 +773,52 @@ __global__ void __launch_bounds__(kThreads, 2)
       ++segs;
     }
   }
-  // The sequences that straddle CTAs: the first part's and the last one's.  They are joined here,
-  // behind the loop, which keeps its registers to itself; nothing waits for a join.
-  if (!active || sub != 0) return;
-  if (segs > 1) {
-    const SeqSpan sp = seq_span(a.kv, a.at, s.z0);
-    const int t0 = (sp.past + tile) / tile;
-    if (!whole(lo - s.t0, t0)) join_sequence<G>(x, h, lo - s.t0, t0, out_of(s.z0));
+}
+
+// CTA (c, h): joins head h of the sequences that began in CTAs kJoinWarps c .. of the first kernel
+// and went on in others.  Up to kJoin records are one warp's; more are spread over the warps, which
+// meet in shared memory.
+constexpr int kJoinWarps = 8;
+template <int G>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    join_q4_kernel(const float* parts, const int4* joins, __half* out, int64_t ld_o, int hkv,
+                   int ctas) {
+  __shared__ __align__(16) float meet[kJoinWarps][G * kRec];
+  __shared__ int4 many[kJoinWarps];
+  const int warp = threadIdx.x >> 5, b0 = blockIdx.x * kJoinWarps, kh = blockIdx.y;
+  const int grp = kh >> 3, h = kh & 7;
+  grid_dependency_wait();
+  // sequence (-1: none), first slot, records
+  int4 d = make_int4(-1, 0, 0, 0);
+  if (b0 + warp < ctas) d = joins[grp * ctas + b0 + warp];
+  if ((threadIdx.x & 31) == 0) many[warp] = d.x >= 0 && d.z > kJoin ? d : make_int4(-1, 0, 0, 0);
+  auto rec = [&](int b, int slot, int i) {
+    return parts + record_of(grp, ctas, b + i, i == 0 ? slot : 0, h) * (G * kRec);
+  };
+  Joined<G> j;
+  if (d.x >= 0 && d.z <= kJoin) {
+    j.template join<true>(d.z, [&](int k) { return rec(b0 + warp, d.y, k); });
+    j.write(out + int64_t(d.x) * ld_o + kh * G * 64);
   }
-  if (!whole(g0, tiles)) join_sequence<G>(x, h, g0, tiles, out_of(z));
+  __syncthreads();
+  for (int w = 0; w < kJoinWarps; ++w) {
+    d = many[w];
+    if (d.x < 0) continue;
+    j.none();
+    for (int i0 = warp; i0 < d.z; i0 += kJoinWarps * kJoin) {
+      Joined<G> x;
+      x.template join<true>(min(kJoin, (d.z - i0 + kJoinWarps - 1) / kJoinWarps),
+                            [&](int k) { return rec(b0 + w, d.y, i0 + k * kJoinWarps); });
+      j.add(x);
+    }
+    j.store(meet[warp]);
+    __syncthreads();
+    if (warp == 0) {
+      j.template join<false>(kJoinWarps, [&](int k) { return meet[k]; });
+      j.write(out + int64_t(d.x) * ld_o + kh * G * 64);
+    }
+    __syncthreads();
+  }
 }
 
 struct Pick {
@@ -857,7 +865,7 @@ int decode_q4_ctas(int num_sms, int hkv) {
 size_t decode_q4_parts_bytes(int num_sms) {
   return size_t(2 * num_sms) * 2 * 8 * 8 * kRec * sizeof(float);
 }
-size_t decode_q4_counter_bytes(int num_sms) { return size_t(2 * num_sms) * 2 * 8 * 2 * 4; }
+size_t decode_q4_join_bytes(int num_sms) { return size_t(2 * num_sms) * sizeof(int4); }
 
 cudaError_t launch_decode_q4(const DecodeQ4Args& args, int num_sms, cudaStream_t s) {
   DecodeQ4Args a = args;
@@ -881,8 +889,27 @@ cudaError_t launch_decode_q4(const DecodeQ4Args& args, int num_sms, cudaStream_t
   });
   if (e != cudaSuccess) return e;
   void* argv[] = {&a};
-  return cudaLaunchKernel(fn, dim3(unsigned(ctas), unsigned(groups)), dim3(kThreads), argv, smem,
-                          s);
+  cudaError_t le = cudaLaunchKernel(fn, dim3(unsigned(ctas), unsigned(groups)), dim3(kThreads),
+                                    argv, smem, s);
+  if (le != cudaSuccess) return le;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned((ctas + kJoinWarps - 1) / kJoinWarps), unsigned(a.kv.hkv));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  const float* pp = a.parts;
+  const int4* pj = a.joins;
+  auto join = [&](auto kernel) {
+    return cudaLaunchKernelEx(&cfg, kernel, pp, pj, a.out, a.ld_o, a.kv.hkv, ctas);
+  };
+  return group == 1   ? join(&join_q4_kernel<1>)
+         : group == 2 ? join(&join_q4_kernel<2>)
+         : group == 4 ? join(&join_q4_kernel<4>)
+                      : join(&join_q4_kernel<8>);
 }
 
 }  // namespace p2p

@@ -321,14 +321,14 @@ cudaError_t launch_attn_kv(const AttnKvArgs& a, cudaStream_t s);
 
 // ---- attn_q4.cu -------------------------------------------------------------------------------
 struct DecodeQ4Args : AttnKvArgs {
-  float* parts;       // decode_q4_parts_bytes(): records of sequences that straddle CTAs
-  int32_t* counters;  // decode_q4_counter_bytes(), zero between launches
+  float* parts;  // decode_q4_parts_bytes(): records of sequences that straddle CTAs
+  int4* joins;   // decode_q4_join_bytes(): per CTA the sequence to join, if any
   int32_t wait_deficit;
   // set by the launcher
   int32_t stages, stage_bytes, min_tiles;
 };
 size_t decode_q4_parts_bytes(int num_sms);
-size_t decode_q4_counter_bytes(int num_sms);
+size_t decode_q4_join_bytes(int num_sms);
 // CTAs per group of 8 kv heads; 0 when there are more heads than the workspace is made for.
 int decode_q4_ctas(int num_sms, int hkv);
 cudaError_t launch_decode_q4(const DecodeQ4Args& a, int num_sms, cudaStream_t s);
