@@ -10,9 +10,11 @@
 // nibbles' factor 16 goes into q (divided by 16 for those dims; exact down to f16's subnormals)
 // and into the final scale of the odd output dims.
 //     S^T[16 keys x 8 heads] = C_K[16 x 64] . Q^T[64 x 8],   O^T[64 x 8] += C_V^T[64 x 16] . P'^T
-// P' = p * s is rounded to f16 (2^-11 of a weight, below the rounding of the f16 output; p goes up to
-// 4, which uses the range left by s <= 8734, so weights keep their bits down to small scales);
-// p, the sums of p and of p * lo, the running maximum and O stay in f32.
+// P' = p * s goes in as a high and a low f16 in the columns that up to four query heads leave free
+// (22 bits of the weight); eight heads fill the columns and P' is rounded to f16 (2^-11 of a weight,
+// below the rounding of the f16 output).  p goes up to 4, which uses the range left by s <= 8734,
+// so weights keep their bits down to small scales.  p, the sums of p and of p * lo, the running
+// maximum and O stay in f32.
 //
 // Split.  All sequences' tiles, in order, form one list that is cut into equal parts, one per CTA
 // (two CTAs per SM), so ragged batches balance by themselves whatever the lengths and the grid
@@ -128,21 +130,32 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 
 constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // nibbles 0, 4 and 1, 5 of a word
 
-// A warp's query heads: B fragments of the four k-steps and the heads' sums (columns 2t, 2t+1).
+// Query heads per lane.  Up to four heads, head t sits in lane column 2t of the fragments' eight and
+// column 2t + 1 is free: it takes no score, so that a lane's softmax works on one head instead of
+// two (half of them empty), and carries the low part of the weights through the P.V product.  Eight
+// heads fill the columns: heads 2t and 2t + 1 are lane t's.
+template <int G>
+constexpr int heads_per_lane() {
+  return G > 4 ? 2 : 1;
+}
+
+// A warp's query heads: B fragments of the four k-steps and the lane's heads' sums.
+template <int H>
 struct Query {
   uint32_t b[4][2];
-  float sum[2];
+  float sum[H];
 };
 
-// From the G f16 rows at `q` (row stride 64): lane (gid, t) holds head gid's dims 8t .. 8t+7 and
-// 32 + 8t .. 32 + 8t + 7 in the order the code words give them.
-template <int G>
-__device__ __forceinline__ void load_query(const __half* q, float scale_log2, Query& out) {
+// From the G f16 rows at `q` (row stride 64): lane (gid, t) holds column gid's head, dims 8t .. 8t+7
+// and 32 + 8t .. 32 + 8t + 7 in the order the code words give them.
+template <int G, int H>
+__device__ __forceinline__ void load_query(const __half* q, float scale_log2, Query<H>& out) {
   const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
   uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  if (gid < G) {
-    w[0] = *reinterpret_cast<const uint4*>(q + gid * 64 + 8 * t);
-    w[1] = *reinterpret_cast<const uint4*>(q + gid * 64 + 32 + 8 * t);
+  const int head = H == 2 ? gid : (gid & 1) ? G : gid >> 1;
+  if (head < G) {
+    w[0] = *reinterpret_cast<const uint4*>(q + head * 64 + 8 * t);
+    w[1] = *reinterpret_cast<const uint4*>(q + head * 64 + 32 + 8 * t);
   }
   float sum = 0.f;
 #pragma unroll
@@ -163,16 +176,23 @@ __device__ __forceinline__ void load_query(const __half* q, float scale_log2, Qu
   sum += __shfl_xor_sync(0xffffffffu, sum, 1);
   sum += __shfl_xor_sync(0xffffffffu, sum, 2);
   sum *= scale_log2;
-  out.sum[0] = __shfl_sync(0xffffffffu, sum, 8 * t);      // lane of head 2t
-  out.sum[1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);  // head 2t + 1
+#pragma unroll
+  for (int e = 0; e < H; ++e)  // from a lane of column 2t + e
+    out.sum[e] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
 }
 
+template <int H>
 struct State {
-  float m[2], l[2], bias[2];  // heads 2t, 2t+1: reference (of the warp), partial sums (of the lane)
-  float o[4][4];              // dims 8 gid + 2i (even codes) and 8 gid + 2i + 1, heads 2t, 2t+1
+  float m[H], l[H], bias[H];  // reference (of the warp), partial sums (of the lane)
+  // [i][c]: dim 8 gid + 2i of column 2t + c (even codes); [i][2 + c]: dim 8 gid + 2i + 1 (odd ones).
+  // H = 1: the sums over the high (c = 0) and low (c = 1) parts of the weights.
+  float o[4][4];
   __device__ __forceinline__ void clear() {
-    m[0] = m[1] = kNegBig;
-    l[0] = l[1] = bias[0] = bias[1] = 0.f;
+#pragma unroll
+    for (int e = 0; e < H; ++e) {
+      m[e] = kNegBig;
+      l[e] = bias[e] = 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   }
@@ -181,13 +201,14 @@ struct State {
 // One block of 32 keys of one head: rows at ks / vs (this head's unit in the block's first key).
 // Row r of the fragments is key perm(r): eight consecutive rows then read V's words of keys 2t and
 // 2t + 1 from distinct banks (the row pitch is 8 banks modulo 32 for 8 heads).
+template <int H>
 __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned char* vs,
-                                         int pitch, int valid, float scale24, const Query& q,
-                                         State& st) {
+                                         int pitch, int valid, float scale24, const Query<H>& q,
+                                         State<H>& st) {
   const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
   constexpr uint32_t kPerm = 0x57463120u;
   const int row = (kPerm >> (4 * gid)) & 7;
-  float sc[4][2];  // keys row, row + 8, row + 16, row + 24; heads 2t, 2t + 1
+  float sc[4][H];  // keys row, row + 8, row + 16, row + 24
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const uint32_t* ka = reinterpret_cast<const uint32_t*>(ks + (16 * j + row) * pitch);
@@ -204,67 +225,76 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
     float s, lo;
     q4_unpack(pa, s, lo);
     s *= scale24;
-    sc[2 * j][0] = fmaf(s0[0] + s1[0], s, lo * q.sum[0]);
-    sc[2 * j][1] = fmaf(s0[1] + s1[1], s, lo * q.sum[1]);
+#pragma unroll
+    for (int e = 0; e < H; ++e) sc[2 * j][e] = fmaf(s0[e] + s1[e], s, lo * q.sum[e]);
     q4_unpack(pb, s, lo);
     s *= scale24;
-    sc[2 * j + 1][0] = fmaf(s0[2] + s1[2], s, lo * q.sum[0]);
-    sc[2 * j + 1][1] = fmaf(s0[3] + s1[3], s, lo * q.sum[1]);
+#pragma unroll
+    for (int e = 0; e < H; ++e) sc[2 * j + 1][e] = fmaf(s0[2 + e] + s1[2 + e], s, lo * q.sum[e]);
   }
   if (valid < kBlock) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (8 * k + row >= valid) sc[k][0] = sc[k][1] = -INFINITY;
+      if (8 * k + row >= valid)
+#pragma unroll
+        for (int e = 0; e < H; ++e) sc[k][e] = -INFINITY;
   }
-  const float mb0 = fmaxf(fmaxf(sc[0][0], sc[1][0]), fmaxf(sc[2][0], sc[3][0]));
-  const float mb1 = fmaxf(fmaxf(sc[0][1], sc[1][1]), fmaxf(sc[2][1], sc[3][1]));
+  float top[H];
+  bool grows = false;
+#pragma unroll
+  for (int e = 0; e < H; ++e) {
+    top[e] = fmaxf(fmaxf(sc[0][e], sc[1][e]), fmaxf(sc[2][e], sc[3][e])) - kUp;
+    grows |= top[e] > st.m[e];
+  }
   // the maximum rarely grows after the first blocks: only then is it joined and O rescaled
-  if (__any_sync(0xffffffffu, mb0 - kUp > st.m[0] || mb1 - kUp > st.m[1])) {
-    float n0 = mb0, n1 = mb1;
+  if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-    for (int o = 4; o <= 16; o <<= 1) {
-      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
-      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
-    }
-    n0 = fmaxf(n0 - kUp, st.m[0]);
-    n1 = fmaxf(n1 - kUp, st.m[1]);
-    const float c0 = fast_exp2(st.m[0] - n0), c1 = fast_exp2(st.m[1] - n1);
-    st.m[0] = n0;
-    st.m[1] = n1;
-    st.l[0] *= c0;
-    st.l[1] *= c1;
-    st.bias[0] *= c0;
-    st.bias[1] *= c1;
+    for (int e = 0; e < H; ++e) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      st.o[i][0] *= c0;
-      st.o[i][1] *= c1;
-      st.o[i][2] *= c0;
-      st.o[i][3] *= c1;
+      for (int o = 4; o <= 16; o <<= 1)
+        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
+      top[e] = fmaxf(top[e], st.m[e]);
+      const float c = fast_exp2(st.m[e] - top[e]);
+      st.m[e] = top[e];
+      st.l[e] *= c;
+      st.bias[e] *= c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        st.o[i][e] *= c;
+        st.o[i][2 + e] *= c;
+        if (H == 1) {
+          st.o[i][1] *= c;
+          st.o[i][3] *= c;
+        }
+      }
     }
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    // weights of keys row and row + 8 of this half, scaled by the keys' value scales
-    float w[4];
+    // weights of keys row and row + 8 of this half, scaled by the keys' value scales: columns 2t
+    // and 2t + 1 of the fragment
+    uint32_t w[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       uint32_t pv = reinterpret_cast<const uint32_t*>(vs + (16 * j + row + 8 * k) * pitch)[8];
       // rows behind the last key hold whatever the stage held before: no weight, no parameters
       if (valid < kBlock && 16 * j + 8 * k + row >= valid) pv = 0u;
-      float s, lo;
+      float s, lo, ps[2];
       q4_unpack(pv, s, lo);
-      const float p0 = fast_exp2(sc[2 * j + k][0] - st.m[0]);
-      const float p1 = fast_exp2(sc[2 * j + k][1] - st.m[1]);
-      st.l[0] += p0;
-      st.l[1] += p1;
-      st.bias[0] = fmaf(p0, lo, st.bias[0]);
-      st.bias[1] = fmaf(p1, lo, st.bias[1]);
-      w[2 * k] = p0 * s;
-      w[2 * k + 1] = p1 * s;
+#pragma unroll
+      for (int e = 0; e < H; ++e) {
+        const float p = fast_exp2(sc[2 * j + k][e] - st.m[e]);
+        st.l[e] += p;
+        st.bias[e] = fmaf(p, lo, st.bias[e]);
+        ps[e] = p * s;
+      }
+      if (H == 1) {  // high and low part: 22 bits of the weight
+        const float hi = __half2float(__float2half_rn(ps[0]));
+        ps[1] = ps[0] - hi;
+      }
+      w[k] = pack_h2(ps[0], ps[1]);
     }
-    const uint32_t b0 = movmatrix_trans(pack_h2(w[0], w[1]));
-    const uint32_t b1 = movmatrix_trans(pack_h2(w[2], w[3]));
+    const uint32_t b0 = movmatrix_trans(w[0]), b1 = movmatrix_trans(w[1]);
     const unsigned char* v0 = vs + (16 * j + ((kPerm >> (8 * t)) & 7)) * pitch + 4 * gid;
     const unsigned char* v1 = vs + (16 * j + ((kPerm >> (8 * t + 4)) & 7)) * pitch + 4 * gid;
     const uint32_t w0 = *reinterpret_cast<const uint32_t*>(v0);
@@ -284,15 +314,15 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
 }
 
 // A warp's part of one head's G query heads as a record [G][acc[64] | max | sum]: from the
-// fragments (acc[e][i]: dim 8 gid + i of head 2t + e) ...
-__device__ __forceinline__ void store_fragments(float* rec, const float (&acc)[2][8],
-                                                const float (&m)[2], const float (&l)[2],
-                                                int g_count) {
+// fragments (acc[e][i]: dim 8 gid + i of the lane's head e) ...
+template <int G, int H>
+__device__ __forceinline__ void store_fragments(float* rec, const float (&acc)[H][8],
+                                                const float (&m)[H], const float (&l)[H]) {
   const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int g = 2 * t + e;
-    if (g >= g_count) continue;
+  for (int e = 0; e < H; ++e) {
+    const int g = H * t + e;
+    if (g >= G) continue;
     float* r = rec + g * kRec;
     *reinterpret_cast<float4*>(r + 8 * gid) =
         make_float4(acc[e][0], acc[e][1], acc[e][2], acc[e][3]);
@@ -415,24 +445,36 @@ struct Joined {
   }
 };
 
-// The tiles of a CTA's part, in order, sequence by sequence.
+// The tiles of a CTA's part, in order, sequence by sequence.  The next sequence's length and offset
+// are loaded while this one's tiles go by.
 struct Walk {
   const KvView& kv;
   const ChunkIndex& at;
-  int tile, z, t, tiles;
+  int tile, z, t, tiles, off, next_past, next_off;
   SeqSpan sp;
-  __device__ Walk(const KvView& k, const ChunkIndex& x, int tile_, int z0, int t0)
-      : kv(k), at(x), tile(tile_), z(z0), t(t0), sp(seq_span(k, x, z0)) {
+  __device__ __forceinline__ Walk(const KvView& k, const ChunkIndex& x, int tile_, int z0, int t0)
+      : kv(k), at(x), tile(tile_), z(z0), t(t0) {
+    fetch(z0);
+    take();
+  }
+  __device__ __forceinline__ void fetch(int i) {
+    next_past = i < at.nseq ? at.past[i] : -1;
+    next_off = kv.table == nullptr && i < at.nseq ? kv.offsets[i] : 0;
+  }
+  __device__ __forceinline__ void take() {
+    sp.past = next_past;
+    off = next_off;
+    sp.ok = one_token_fits(kv, at, sp.past, off);
     tiles = (sp.past + tile) / tile;  // of past + 1 keys
+    fetch(z + 1);
   }
   // Moves on to the next sequence that has tiles when this one's are done.
-  __device__ void settle() {
+  __device__ __forceinline__ void settle() {
     if (t < tiles) return;
     do {
       ++z;
-      sp = seq_span(kv, at, z);
-    } while (!sp.ok);
-    tiles = (sp.past + tile) / tile;
+      take();
+    } while (!sp.ok && z < at.nseq);
     t = 0;
   }
 };
@@ -519,23 +561,54 @@ __global__ void __launch_bounds__(kThreads, 2)
     Walk w(a.kv, a.at, tile, s.z0, s.t0);
     // keys of one contiguous run: the cache's rows are whole tokens, so a run can span keys only
     // when one group of heads is the whole row
-    const int run = n_groups > 1 ? 1 : a.kv.table ? min(1 << a.kv.shift, tile) : tile;
+    const bool paged = a.kv.table != nullptr;
+    const int shift = a.kv.shift;
+    const int run = n_groups > 1 ? 1 : paged ? min(1 << shift, tile) : tile;
+    // The block table's entries pass through a window of 32 in the lanes, with the next 32 on their
+    // way: a load per tile would put its latency (more than a tile takes) in front of every copy.
+    // A tile covers 1, 2, 4, 8 or 16 pages, or part of one, so it never straddles two windows.
+    int page0 = 0;
+    int32_t pages = 0, next_pages = 0;
+    auto table_at = [&](int z, int p) {
+      return p < a.kv.max_blocks ? a.kv.table[int64_t(z) * a.kv.max_blocks + p] : -1;
+    };
     int issued = 0, st = 0;
     uint32_t round = 0;  // parity of the stages' current use
     for (int i = 0; i < n_tiles; ++i, ++w.t) {
       w.settle();
+      const int z = w.z, key0 = w.t * tile, len = w.sp.past + 1, valid = min(tile, len - key0);
+      const int n_copy = FUSED && key0 + valid == len ? valid - 1 : valid;
+      if (paged) {
+        const int p = key0 >> shift;
+        if (i == 0 || w.t == 0) {
+          page0 = p;
+          pages = table_at(z, p + lane);
+          next_pages = table_at(z, p + 32 + lane);
+        } else if (p >= page0 + 32) {
+          page0 += 32;
+          pages = next_pages;
+          next_pages = table_at(z, page0 + 32 + lane);
+        }
+      }
+      // cache row of the tile's key k, -1 when its page is outside the pool (whole warps call it)
+      auto row_at = [&](int k) -> int64_t {
+        const int pos = key0 + k;
+        if (!paged) return int64_t(w.off) + pos;
+        const int32_t pg = __shfl_sync(0xffffffffu, pages, (pos >> shift) - page0);
+        if (pg < 0 || int64_t(pg) >= a.kv.kv_rows) return -1;
+        return (int64_t(pg) << shift) | (pos & ((1 << shift) - 1));
+      };
+      bool bad = false;
+      for (int k = 0; k < valid; k += 32 * run) {
+        const int mine = k + lane * run;
+        bad |= row_at(min(mine, valid - 1)) < 0;
+      }
+      bad = __any_sync(0xffffffffu, bad);
       if (i >= a.stages) {
         bool ok = true;
         if (lane == 0) ok = wait_bar(s, &s.empty[st], round ^ 1, a.err);
         if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) break;
       }
-      const int z = w.z, key0 = w.t * tile, len = w.sp.past + 1, valid = min(tile, len - key0);
-      const int n_copy = FUSED && key0 + valid == len ? valid - 1 : valid;
-      const int runs = (n_copy + run - 1) / run;
-      bool bad = false;
-      for (int k = lane; k < runs; k += 32) bad |= kv_row(a.kv, z, key0 + k * run) < 0;
-      if (FUSED && key0 + valid == len) bad |= kv_row(a.kv, z, w.sp.past) < 0;
-      bad = __any_sync(0xffffffffu, bad);
       if (lane == 0) {
         if (bad) atomicOr(a.err, kErrPosBeyondCache);
         StageMeta& m = s.meta[st];
@@ -554,13 +627,14 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
       if (!bad) {
         const uint32_t dst = smem_u32(ring) + uint32_t(st * sbytes);
-        for (int k = lane; k < 2 * runs; k += 32) {
-          const int pool = k >= runs, r = k - pool * runs;
-          const int n = min(run, n_copy - r * run);
-          const int64_t row = kv_row(a.kv, z, key0 + r * run);
-          bulk_load(dst + uint32_t((pool * tile + r * run) * pitch),
-                    (pool ? a.kv.v : a.kv.k) + row * a.kv.row_bytes + grp * 8 * kQ4UnitBytes,
-                    uint32_t(n * pitch), &s.full[st]);
+        const int runs = (n_copy + run - 1) / run;
+        for (int k0 = 0; k0 < 2 * runs; k0 += 32) {
+          const int k = k0 + lane, pool = k >= runs, r = k - pool * runs;
+          const int64_t row = row_at(min(r * run, valid - 1));
+          if (k < 2 * runs)
+            bulk_load(dst + uint32_t((pool * tile + r * run) * pitch),
+                      (pool ? a.kv.v : a.kv.k) + row * a.kv.row_bytes + grp * 8 * kQ4UnitBytes,
+                      uint32_t(min(run, n_copy - r * run) * pitch), &s.full[st]);
         }
       }
       issued = i + 1;
@@ -585,8 +659,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool active = sub < wph;
   const int kh = grp * 8 + h;
   const float scale24 = a.scale_log2 * 16777216.f;
-  Query q;
-  State state;
+  constexpr int H = heads_per_lane<G>();
+  Query<H> q;
+  State<H> state;
   bool bad = false;
   int segs = 0;  // parts of sequences ended
   float* merge = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // [warp][G][kRec]
@@ -594,7 +669,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   auto whole = [&](long long g0, int tiles) { return lo <= g0 && lo + n_tiles >= g0 + tiles; };
   // Ends this CTA's part of sequence z (whose `tiles` tiles begin at g0 of the list): the warps of
   // a head meet, and the output is written, or a record when other CTAs have parts of it too.
-  auto end_part = [&](const float (&acc)[2][8], const float (&m)[2], const float (&l)[2], int z,
+  auto end_part = [&](const float (&acc)[H][8], const float (&m)[H], const float (&l)[H], int z,
                       long long g0, int tiles, bool seg_first) {
     float* own = a.parts + record_of(grp, gridDim.x, b, seg_first ? 0 : 1, h) * (G * kRec);
     if (tid == 0 && lo <= g0 && !whole(g0, tiles)) {  // it begins here: what there is to join
@@ -602,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       a.joins[grp * gridDim.x + b] = make_int4(z, seg_first ? 0 : 1, last - b + 1, 0);
     }
     if (wph > 1) {
-      if (active) store_fragments(merge + warp * G * kRec, acc, m, l, G);
+      if (active) store_fragments<G>(merge + warp * G * kRec, acc, m, l);
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (sub == 0) {
         Joined<G> j;
@@ -613,14 +688,14 @@ __global__ void __launch_bounds__(kThreads, 2)
       asm volatile("bar.sync 1, 256;" ::: "memory");
     } else if (active) {
       if (!whole(g0, tiles)) {
-        store_fragments(own, acc, m, l, G);
+        store_fragments<G>(own, acc, m, l);
       } else {
         const int gid = lane >> 2, t = lane & 3;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (2 * t + e >= G || l[e] < 0.f) continue;
+        for (int e = 0; e < H; ++e) {
+          if (H * t + e >= G || l[e] < 0.f) continue;
           const float inv = __fdiv_rn(1.f, l[e]);
-          *reinterpret_cast<uint4*>(out_of(z) + (2 * t + e) * 64 + 8 * gid) =
+          *reinterpret_cast<uint4*>(out_of(z) + (H * t + e) * 64 + 8 * gid) =
               make_uint4(pack_h2(acc[e][0] * inv, acc[e][1] * inv),
                          pack_h2(acc[e][2] * inv, acc[e][3] * inv),
                          pack_h2(acc[e][4] * inv, acc[e][5] * inv),
@@ -634,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   int z = s.z0, tiles = 0;  // the sequence at hand
   long long g0 = 0;
   state.clear();
-  q = Query{};
+  q = Query<H>{};
   for (; i < n_tiles; ++i) {
     const bool ok = wait_bar(s, &s.full[st], round, a.err);
     if (!__all_sync(0xffffffffu, ok)) break;
@@ -677,9 +752,9 @@ __global__ void __launch_bounds__(kThreads, 2)
             q_s[warp][g][32 + lane] = __float2half_rn(r1);
           }
           __syncwarp();
-          load_query<G>(&q_s[warp][0][0], a.scale_log2, q);
+          load_query<G, H>(&q_s[warp][0][0], a.scale_log2, q);
         } else {
-          load_query<G>(row + kh * G * 64, a.scale_log2, q);
+          load_query<G, H>(row + kh * G * 64, a.scale_log2, q);
         }
       }
     }
@@ -724,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         fence_proxy_async_smem();  // a later copy into this stage comes after these writes
         __syncwarp();
       }
-      attend32(ks, vs, pitch, min(valid, kBlock), scale24, q, state);
+      attend32<H>(ks, vs, pitch, min(valid, kBlock), scale24, q, state);
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&s.empty[st]);
@@ -735,9 +810,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (!(flags & kLast)) continue;
 
     // ---- this CTA's part of the sequence is done
-    float acc[2][8], mx[2], sum[2];
+    float acc[H][8], mx[H], sum[H];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < H; ++e) {
 #pragma unroll
       for (int o = 4; o <= 16; o <<= 1) {
         state.l[e] += __shfl_xor_sync(0xffffffffu, state.l[e], o);
@@ -747,14 +822,16 @@ __global__ void __launch_bounds__(kThreads, 2)
       sum[e] = bad ? -1.f : state.l[e];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        acc[e][2 * k] = fmaf(state.o[k][e], 16777216.f, state.bias[e]);         // 2^24
-        acc[e][2 * k + 1] = fmaf(state.o[k][2 + e], 1048576.f, state.bias[e]);  // 2^20
+        const float even = H == 2 ? state.o[k][e] : state.o[k][0] + state.o[k][1];
+        const float odd = H == 2 ? state.o[k][2 + e] : state.o[k][2] + state.o[k][3];
+        acc[e][2 * k] = fmaf(even, 16777216.f, state.bias[e]);     // 2^24
+        acc[e][2 * k + 1] = fmaf(odd, 1048576.f, state.bias[e]);   // 2^20
       }
     }
     end_part(acc, mx, sum, z, g0, tiles, segs == 0);
     ++segs;
     state.clear();
-    q = Query{};
+    q = Query<H>{};
     bad = false;
   }
   if (i < n_tiles) {
@@ -765,7 +842,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int k = 0; k < n_tiles; ++k, ++w.t) {
       w.settle();
       if (!(k == n_tiles - 1 || w.t == w.tiles - 1) || done-- > 0) continue;
-      const float acc[2][8] = {}, mx[2] = {kNegBig, kNegBig}, sum[2] = {-1.f, -1.f};
+      float acc[H][8] = {}, mx[H], sum[H];
+#pragma unroll
+      for (int e = 0; e < H; ++e) mx[e] = kNegBig, sum[e] = -1.f;
       z = w.z;
       g0 = lo + k - w.t;
       tiles = w.tiles;

@@ -19,6 +19,20 @@ struct SeqSpan {
   bool ok;
 };
 
+__host__ __device__ __forceinline__ bool span_fits(const KvView& c, const ChunkIndex& x, int past,
+                                                  int row0, int len, int off) {
+  const int64_t end = int64_t(past) + len;
+  return past >= 0 && row0 >= 0 && len >= 0 && int64_t(row0) + len <= x.n_rows &&
+         end <= x.max_len &&
+         (c.table != nullptr ? end <= 0 || ((end - 1) >> c.shift) < c.max_blocks
+                             : off >= 0 && int64_t(off) + end <= c.kv_rows);
+}
+// The same for one token behind `past` keys (no chunk rows to check).
+__host__ __device__ __forceinline__ bool one_token_fits(const KvView& c, const ChunkIndex& x,
+                                                       int past, int off) {
+  return span_fits(c, x, past, 0, 1, off);
+}
+
 __host__ __device__ __forceinline__ SeqSpan seq_span(const KvView& c, const ChunkIndex& x, int i) {
   SeqSpan s;
   s.past = x.past[i];
@@ -29,15 +43,7 @@ __host__ __device__ __forceinline__ SeqSpan seq_span(const KvView& c, const Chun
     s.row0 = i;
     s.len = 1;
   }
-  const int64_t end = int64_t(s.past) + s.len;
-  s.ok = s.past >= 0 && s.row0 >= 0 && s.len >= 0 && int64_t(s.row0) + s.len <= x.n_rows &&
-         end <= x.max_len;
-  if (c.table != nullptr) {
-    s.ok = s.ok && (end <= 0 || ((end - 1) >> c.shift) < c.max_blocks);
-  } else {
-    const int off = c.offsets[i];
-    s.ok = s.ok && off >= 0 && int64_t(off) + end <= c.kv_rows;
-  }
+  s.ok = span_fits(c, x, s.past, s.row0, s.len, c.table == nullptr ? c.offsets[i] : 0);
   return s;
 }
 
