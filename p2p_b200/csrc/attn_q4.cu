@@ -56,14 +56,14 @@ constexpr float kNegBig = -1e30f;
 constexpr float kUp = 2.f;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 
-// Warps per head for a CTA of hb heads (1 .. 8); its tile is kBlock keys per such warp.
+// Warps per head for a CTA of hb heads (1 .. 8); its tile is `blocks` (1 or 2) blocks per such warp.
 __host__ __device__ constexpr int warps_per_head(int hb) {
   return hb >= 5 ? 1 : hb >= 3 ? 2 : hb == 2 ? 4 : 8;
 }
 // Bytes of one token's units of hb heads, as copied and as laid out in shared memory.
 __host__ __device__ constexpr int pitch_of(int hb) { return (hb * kQ4UnitBytes + 15) / 16 * 16; }
-__host__ __device__ constexpr int stage_bytes(int hb) {
-  return 2 * kBlock * warps_per_head(hb) * pitch_of(hb);
+__host__ __device__ constexpr int stage_bytes(int hb, int blocks) {
+  return 2 * kBlock * blocks * warps_per_head(hb) * pitch_of(hb);
 }
 
 struct __align__(16) StageMeta {
@@ -183,16 +183,17 @@ __device__ __forceinline__ void load_query(const __half* q, float scale_log2, Qu
 
 template <int H>
 struct State {
-  float m[H], l[H], bias[H];  // reference (of the warp), partial sums (of the lane)
+  // The reference that weights are taken against (the warp's; at most kUp below the maximum when it
+  // was set) and, of the lane, the sums of the weights and of weight * lo.
+  float m[H], l[H], bias[H];
   // [i][c]: dim 8 gid + 2i of column 2t + c (even codes); [i][2 + c]: dim 8 gid + 2i + 1 (odd ones).
   // H = 1: the sums over the high (c = 0) and low (c = 1) parts of the weights.
   float o[4][4];
+  bool fresh;  // no block yet: the reference is to be set, whatever it is
   __device__ __forceinline__ void clear() {
+    fresh = true;
 #pragma unroll
-    for (int e = 0; e < H; ++e) {
-      m[e] = kNegBig;
-      l[e] = bias[e] = 0.f;
-    }
+    for (int e = 0; e < H; ++e) m[e] = l[e] = bias[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   }
@@ -201,38 +202,40 @@ struct State {
 // One block of 32 keys of one head: rows at ks / vs (this head's unit in the block's first key).
 // Row r of the fragments is key perm(r): eight consecutive rows then read V's words of keys 2t and
 // 2t + 1 from distinct banks (the row pitch is 8 banks modulo 32 for 8 heads).
-template <int H>
+// FULL: all 32 keys are there; else the rows behind `valid` hold whatever the stage held before and
+// get neither weight nor parameters.
+template <int H, bool FULL>
 __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned char* vs,
                                          int pitch, int valid, float scale24, const Query<H>& q,
                                          State<H>& st) {
   const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
   constexpr uint32_t kPerm = 0x57463120u;
   const int row = (kPerm >> (4 * gid)) & 7;
-  float sc[4][H];  // keys row, row + 8, row + 16, row + 24
+  float sc[4][H];  // log2 weights of keys row, row + 8, row + 16, row + 24
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const uint32_t* ka = reinterpret_cast<const uint32_t*>(ks + (16 * j + row) * pitch);
     const uint32_t* kb = reinterpret_cast<const uint32_t*>(ks + (16 * j + row + 8) * pitch);
     const uint32_t a0 = ka[t], a1 = ka[t + 4], b0 = kb[t], b1 = kb[t + 4];
     const uint32_t pa = ka[8], pb = kb[8];
-    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-    mma16816(s0, a0 & kEven, b0 & kEven, a0 & kOdd, b0 & kOdd, q.b[0][0], q.b[0][1]);
-    mma16816(s1, (a0 >> 8) & kEven, (b0 >> 8) & kEven, (a0 >> 8) & kOdd, (b0 >> 8) & kOdd,
+    float r[4] = {0.f, 0.f, 0.f, 0.f};
+    mma16816(r, a0 & kEven, b0 & kEven, a0 & kOdd, b0 & kOdd, q.b[0][0], q.b[0][1]);
+    mma16816(r, (a0 >> 8) & kEven, (b0 >> 8) & kEven, (a0 >> 8) & kOdd, (b0 >> 8) & kOdd,
              q.b[1][0], q.b[1][1]);
-    mma16816(s0, a1 & kEven, b1 & kEven, a1 & kOdd, b1 & kOdd, q.b[2][0], q.b[2][1]);
-    mma16816(s1, (a1 >> 8) & kEven, (b1 >> 8) & kEven, (a1 >> 8) & kOdd, (b1 >> 8) & kOdd,
+    mma16816(r, a1 & kEven, b1 & kEven, a1 & kOdd, b1 & kOdd, q.b[2][0], q.b[2][1]);
+    mma16816(r, (a1 >> 8) & kEven, (b1 >> 8) & kEven, (a1 >> 8) & kOdd, (b1 >> 8) & kOdd,
              q.b[3][0], q.b[3][1]);
     float s, lo;
     q4_unpack(pa, s, lo);
     s *= scale24;
 #pragma unroll
-    for (int e = 0; e < H; ++e) sc[2 * j][e] = fmaf(s0[e] + s1[e], s, lo * q.sum[e]);
+    for (int e = 0; e < H; ++e) sc[2 * j][e] = fmaf(r[e], s, fmaf(lo, q.sum[e], -st.m[e]));
     q4_unpack(pb, s, lo);
     s *= scale24;
 #pragma unroll
-    for (int e = 0; e < H; ++e) sc[2 * j + 1][e] = fmaf(s0[2 + e] + s1[2 + e], s, lo * q.sum[e]);
+    for (int e = 0; e < H; ++e) sc[2 * j + 1][e] = fmaf(r[2 + e], s, fmaf(lo, q.sum[e], -st.m[e]));
   }
-  if (valid < kBlock) {
+  if (!FULL) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (8 * k + row >= valid)
@@ -240,11 +243,11 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
         for (int e = 0; e < H; ++e) sc[k][e] = -INFINITY;
   }
   float top[H];
-  bool grows = false;
+  bool grows = st.fresh;
 #pragma unroll
   for (int e = 0; e < H; ++e) {
-    top[e] = fmaxf(fmaxf(sc[0][e], sc[1][e]), fmaxf(sc[2][e], sc[3][e])) - kUp;
-    grows |= top[e] > st.m[e];
+    top[e] = fmaxf(fmaxf(sc[0][e], sc[1][e]), fmaxf(sc[2][e], sc[3][e]));
+    grows |= top[e] > kUp;
   }
   // the maximum rarely grows after the first blocks: only then is it joined and O rescaled
   if (__any_sync(0xffffffffu, grows)) {
@@ -253,11 +256,13 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
 #pragma unroll
       for (int o = 4; o <= 16; o <<= 1)
         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
-      top[e] = fmaxf(top[e], st.m[e]);
-      const float c = fast_exp2(st.m[e] - top[e]);
-      st.m[e] = top[e];
+      const float up = st.fresh ? top[e] - kUp : fmaxf(top[e] - kUp, 0.f);
+      const float c = st.fresh ? 0.f : fast_exp2(-up);
+      st.m[e] += up;
       st.l[e] *= c;
       st.bias[e] *= c;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sc[k][e] -= up;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         st.o[i][e] *= c;
@@ -268,6 +273,7 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
         }
       }
     }
+    st.fresh = false;
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -277,13 +283,12 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       uint32_t pv = reinterpret_cast<const uint32_t*>(vs + (16 * j + row + 8 * k) * pitch)[8];
-      // rows behind the last key hold whatever the stage held before: no weight, no parameters
-      if (valid < kBlock && 16 * j + 8 * k + row >= valid) pv = 0u;
+      if (!FULL && 16 * j + 8 * k + row >= valid) pv = 0u;
       float s, lo, ps[2];
       q4_unpack(pv, s, lo);
 #pragma unroll
       for (int e = 0; e < H; ++e) {
-        const float p = fast_exp2(sc[2 * j + k][e] - st.m[e]);
+        const float p = fast_exp2(sc[2 * j + k][e]);
         st.l[e] += p;
         st.bias[e] = fmaf(p, lo, st.bias[e]);
         ps[e] = p * s;
@@ -498,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grp = blockIdx.y;
   const int hb = HB ? HB : min(8, a.kv.hkv - 8 * grp), wph = warps_per_head(hb);
-  const int tile = kBlock * wph, pitch = pitch_of(hb), sbytes = 2 * tile * pitch;
+  const int tile = kBlock * a.blocks * wph, pitch = pitch_of(hb), sbytes = 2 * tile * pitch;
   const int n_groups = gridDim.y;
 
   // ---- the CTA's part of the list of tiles
@@ -723,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       tiles = m.tiles;
       g0 = m.g;
     }
-    unsigned char* ks = ring + st * sbytes + sub * kBlock * pitch + h * kQ4UnitBytes;
+    unsigned char* ks = ring + st * sbytes + sub * (tile / wph) * pitch + h * kQ4UnitBytes;
     unsigned char* vs = ks + tile * pitch;
     // the sequence's last tile ends this part
     const bool has_new = FUSED && (flags & kLast) && head.y + head.z == pos + 1;
@@ -759,9 +764,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
     if (flags & kBad) bad = true;
-    const int valid = head.z - sub * kBlock;
-    if (active && valid > 0 && !bad) {
-      if (has_new && valid <= kBlock) {
+    int valid = head.z - sub * (tile / wph);
+    if (!active || bad) valid = 0;
+    if (FUSED && has_new) {
+      const int at = valid - 1;  // the new token's row, if it is among this warp's
+      if (at >= 0 && at < tile / wph) {
         // the new token's unit of this head: normed, rotated, quantised, into the cache and over
         // the stage's row (which the copy left out)
         const __half* row = a.q + int64_t(z) * a.ld_q;
@@ -791,15 +798,20 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (lane < 18) {
           const int pool = lane / 9, w = lane % 9;
           const uint32_t v = unit_s[warp][pool][w];
-          const int64_t at = kv_row(a.kv, z, pos);
-          reinterpret_cast<uint32_t*>((pool ? a.kv.v : a.kv.k) + at * a.kv.row_bytes +
+          const int64_t cached = kv_row(a.kv, z, pos);
+          reinterpret_cast<uint32_t*>((pool ? a.kv.v : a.kv.k) + cached * a.kv.row_bytes +
                                       kh * kQ4UnitBytes)[w] = v;
-          reinterpret_cast<uint32_t*>((pool ? vs : ks) + (valid - 1) * pitch)[w] = v;
+          reinterpret_cast<uint32_t*>((pool ? vs : ks) + at * pitch)[w] = v;
         }
         fence_proxy_async_smem();  // a later copy into this stage comes after these writes
         __syncwarp();
       }
-      attend32<H>(ks, vs, pitch, min(valid, kBlock), scale24, q, state);
+    }
+    for (int k = 0; k < a.blocks && valid > 0; ++k, valid -= kBlock) {
+      if (valid >= kBlock) attend32<H, true>(ks, vs, pitch, kBlock, scale24, q, state);
+      else attend32<H, false>(ks, vs, pitch, valid, scale24, q, state);
+      ks += kBlock * pitch;
+      vs += kBlock * pitch;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&s.empty[st]);
@@ -818,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         state.l[e] += __shfl_xor_sync(0xffffffffu, state.l[e], o);
         state.bias[e] += __shfl_xor_sync(0xffffffffu, state.bias[e], o);
       }
-      mx[e] = state.m[e];
+      mx[e] = state.fresh ? kNegBig : state.m[e];
       sum[e] = bad ? -1.f : state.l[e];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -932,7 +944,7 @@ Pick pick(int group, bool fused, int hkv) {
   return p;
 }
 
-constexpr int kRingBytes = 94 * 1024;  // two CTAs per SM
+constexpr int kSmemBytes = 113 * 1024;  // of a CTA, static ones included: two CTAs per SM
 
 }  // namespace
 
@@ -955,18 +967,26 @@ cudaError_t launch_decode_q4(const DecodeQ4Args& args, int num_sms, cudaStream_t
   if (!fn || ctas < 1) return cudaErrorInvalidValue;
   // the groups' stages: 8 heads each, the last one the rest
   const int rest = a.kv.hkv - 8 * (groups - 1);
-  a.stage_bytes = stage_bytes(rest);
-  if (groups > 1 && a.stage_bytes < stage_bytes(8)) a.stage_bytes = stage_bytes(8);
+  a.blocks = 2;
+  a.stage_bytes = stage_bytes(rest, a.blocks);
+  if (groups > 1 && a.stage_bytes < stage_bytes(8, a.blocks))
+    a.stage_bytes = stage_bytes(8, a.blocks);
   const int merge = warps_per_head(rest) > 1 ? kWarps * group * kRec * 4 : 0;
-  a.stages = (kRingBytes - merge) / a.stage_bytes;
+  static PerDeviceOnce attrs[40];
+  int fixed = 0;  // the kernel's static shared memory
+  const cudaError_t e = per_device_once(attrs[k.id], [&](int& value) {
+    cudaFuncAttributes fa;
+    cudaError_t r = cudaFuncGetAttributes(&fa, fn);
+    if (r != cudaSuccess) return r;
+    value = int(fa.sharedSizeBytes);
+    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kSmemBytes - value);
+  }, &fixed);
+  if (e != cudaSuccess) return e;
+  a.stages = (kSmemBytes - fixed - merge) / a.stage_bytes;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   a.min_tiles = 1;
   const size_t smem = size_t(a.stages) * a.stage_bytes + merge;
-  static PerDeviceOnce attrs[40];
-  const cudaError_t e = per_device_once(attrs[k.id], [&](int&) {
-    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
-  });
-  if (e != cudaSuccess) return e;
   void* argv[] = {&a};
   cudaError_t le = cudaLaunchKernel(fn, dim3(unsigned(ctas), unsigned(groups)), dim3(kThreads),
                                     argv, smem, s);
