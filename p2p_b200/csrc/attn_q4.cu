@@ -199,21 +199,21 @@ struct State {
   }
 };
 
-// One block of 32 keys of one head: rows at ks / vs (this head's unit in the block's first key).
+// A block of 16 NJ keys of one head: rows at ks / vs (this head's unit in the block's first key).
 // Row r of the fragments is key perm(r): eight consecutive rows then read V's words of keys 2t and
 // 2t + 1 from distinct banks (the row pitch is 8 banks modulo 32 for 8 heads).
-// FULL: all 32 keys are there; else the rows behind `valid` hold whatever the stage held before and
+// FULL: all the keys are there; else the rows behind `valid` hold whatever the stage held before and
 // get neither weight nor parameters.
-template <int H, bool FULL>
-__device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned char* vs,
+template <int H, bool FULL, int NJ>
+__device__ __forceinline__ void attend(const unsigned char* ks, const unsigned char* vs,
                                          int pitch, int valid, float scale24, const Query<H>& q,
                                          State<H>& st) {
   const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
   constexpr uint32_t kPerm = 0x57463120u;
   const int row = (kPerm >> (4 * gid)) & 7;
-  float sc[4][H];  // log2 weights of keys row, row + 8, row + 16, row + 24
+  float sc[2 * NJ][H];  // log2 weights of keys row, row + 8, row + 16, ...
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < NJ; ++j) {
     const uint32_t* ka = reinterpret_cast<const uint32_t*>(ks + (16 * j + row) * pitch);
     const uint32_t* kb = reinterpret_cast<const uint32_t*>(ks + (16 * j + row + 8) * pitch);
     const uint32_t a0 = ka[t], a1 = ka[t + 4], b0 = kb[t], b1 = kb[t + 4];
@@ -237,7 +237,7 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
   }
   if (!FULL) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 2 * NJ; ++k)
       if (8 * k + row >= valid)
 #pragma unroll
         for (int e = 0; e < H; ++e) sc[k][e] = -INFINITY;
@@ -246,7 +246,9 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
   bool grows = st.fresh;
 #pragma unroll
   for (int e = 0; e < H; ++e) {
-    top[e] = fmaxf(fmaxf(sc[0][e], sc[1][e]), fmaxf(sc[2][e], sc[3][e]));
+    top[e] = sc[0][e];
+#pragma unroll
+    for (int k = 1; k < 2 * NJ; ++k) top[e] = fmaxf(top[e], sc[k][e]);
     grows |= top[e] > kUp;
   }
   // the maximum rarely grows after the first blocks: only then is it joined and O rescaled
@@ -262,7 +264,7 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
       st.l[e] *= c;
       st.bias[e] *= c;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sc[k][e] -= up;
+      for (int k = 0; k < 2 * NJ; ++k) sc[k][e] -= up;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         st.o[i][e] *= c;
@@ -276,7 +278,7 @@ __device__ __forceinline__ void attend32(const unsigned char* ks, const unsigned
     st.fresh = false;
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < NJ; ++j) {
     // weights of keys row and row + 8 of this half, scaled by the keys' value scales: columns 2t
     // and 2t + 1 of the fragment
     uint32_t w[2];
@@ -807,11 +809,14 @@ __global__ void __launch_bounds__(kThreads, 2)
         __syncwarp();
       }
     }
-    for (int k = 0; k < a.blocks && valid > 0; ++k, valid -= kBlock) {
-      if (valid >= kBlock) attend32<H, true>(ks, vs, pitch, kBlock, scale24, q, state);
-      else attend32<H, false>(ks, vs, pitch, valid, scale24, q, state);
-      ks += kBlock * pitch;
-      vs += kBlock * pitch;
+    if (valid >= 2 * kBlock && a.blocks == 2) {
+      attend<H, true, 4>(ks, vs, pitch, 2 * kBlock, scale24, q, state);
+    } else {
+      for (int k = 0; k < a.blocks && valid > 0; ++k, valid -= kBlock) {
+        attend<H, false, 2>(ks, vs, pitch, valid, scale24, q, state);
+        ks += kBlock * pitch;
+        vs += kBlock * pitch;
+      }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&s.empty[st]);
