@@ -1414,7 +1414,9 @@ p2p_status ctx_serve_workspace(p2p_ctx* ctx, cudaStream_t s, const char* who,
       return fail(ctx, P2P_ERR_INVALID_ARG,
                   "%s: the first call of a context makes its workspace and cannot be captured",
                   who);
-    const size_t bytes = decode_q4_join_bytes(ctx->num_sms) + decode_q4_parts_bytes(ctx->num_sms);
+    const size_t bytes =
+        std::max(decode_q4_join_bytes(ctx->num_sms) + decode_q4_parts_bytes(ctx->num_sms),
+                 chunk_join_bytes(ctx->num_sms) + chunk_parts_bytes(ctx->num_sms));
     void* p = nullptr;
     if (dev_alloc(&p, bytes) != cudaSuccess) {
       cudaGetLastError();

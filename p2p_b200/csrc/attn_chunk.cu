@@ -1,0 +1,857 @@
+// attn_chunk.cu -- attention of ragged prompt chunks over a KV cache of any layout on the 5th
+// generation tensor cores (ATTN for M > 1, src/scripts/lfm-engine/kernels.js:268-319, for several
+// sequences at once over paged / int8 / 4-bit caches).
+//
+// Work.  An item is 256 query rows of one sequence and kv head: 256 / G tokens times the G query
+// heads that share the kv head, so that one pass over the keys serves all of them and short chunks
+// of grouped heads fill the tensor cores' 128 rows.  An item runs over its keys in tiles of 128.
+//   few items: all tiles of all items form one list that is cut into equal parts, one per SM; an
+//     item that straddles CTAs leaves records (unnormalised rows, maxima, sums) which a dependent
+//     kernel joins in CTA order;
+//   many items: one CTA per item, the longest of each sequence first.
+// The choice goes by the number of items the call can have, against four per SM: records cost 70 KB
+// of traffic per straddling item and CTA, an uneven last wave a part of an item's time.
+//
+// Roles of a CTA (16 warps): two softmax warpgroups, one query row per thread, 128 rows each; one
+// warp that issues the MMAs; seven that load.  f16 rows come by TMA, a box per page; int8 and 4-bit
+// rows are converted by the loading warps while the previous tiles are at work, each value rounded
+// to f16 once, straight into the swizzled operand layout.  The eight codes of a 4-bit word become
+// one 16-byte piece in the order 0 4 1 5 2 6 3 7 (the order in which masking a word yields pairs);
+// the query's dims are stored in the same order and the output's are put back at the end.
+//   S_w = Q_w K^T (M128 N128 K64) -> TMEM; P_w to TMEM as f16; O_w += P_w V (M128 N64 K128).
+// The softmax is that of the prompt kernel: exp2 with the scale folded in, partly by a cubic on the
+// FMA pipe, lazily rescaled (only when a row's maximum grows by 2^8).
+//
+// Every wait is bounded; one that gives up sets the error word, the other roles stop, the CTA frees
+// its TMEM and writes nothing more.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "kv_view.cuh"
+#include "sm100.cuh"
+
+namespace p2p {
+namespace {
+
+using namespace sm100;
+
+constexpr int BM = 128, BN = 128, D = kHeadDim;
+constexpr int kRows = 2 * BM;  // rows of an item
+constexpr int kStages = 5;
+constexpr int kThreads = 512;
+constexpr int kMmaWarp = 8, kLoadWarp0 = 9, kLoadWarps = 7;
+constexpr int kLoaders = kLoadWarps * 32;
+// setmaxnreg splits the 512 x 128 registers of the launch: 256 x 192 + 256 x 64
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 192, kOtherRegs = 64;
+static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
+constexpr uint32_t kTmemCols = 512;
+constexpr uint64_t kWaitLimitNs = 1000000000ull;
+constexpr float kRescaleLog2 = 8.0f;
+constexpr int kPolyPairs = 5;  // of every 16 exp pairs, these use the cubic
+constexpr int kRec = 68;       // a record's row: acc[64], max, sum, 2 pad
+constexpr int kMaxItemsPerSm = 4;
+
+__device__ __forceinline__ uint32_t col_s(int w) { return uint32_t(w) * 256u; }
+__device__ __forceinline__ uint32_t col_p(int w) { return uint32_t(w) * 256u + 128u; }
+__device__ __forceinline__ uint32_t col_o(int w) { return uint32_t(w) * 256u + 192u; }
+
+struct __align__(128) Smem {
+  __half q[2][BM * D];
+  __half kv[kStages][2][BN * D];  // K, V
+  uint64_t q_full, q_free;
+  uint64_t kv_full[kStages], kv_empty[kStages];
+  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];
+  long long wsum[8];
+  int z0, qt0, kh0, k0, n_tiles;
+  volatile int bad[8];  // of part i & 7 of this CTA: some page was refused
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+__device__ __forceinline__ bool wait_bar(Smem& s, uint64_t* bar, uint32_t parity, int32_t* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (s.abort_flag) return false;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      s.abort_flag = 1;
+      atomicOr(err, kErrTimeout);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One item: rows of tokens tok0 .. of sequence z for kv head kh.
+struct Item {
+  int z, kh, qt;
+  int past, row0, len;  // of the sequence
+  int group;
+
+  __device__ __forceinline__ int tok0() const { return qt * (kRows / group); }
+  __device__ __forceinline__ int rows() const { return min(kRows, (len - tok0()) * group); }
+  // valid rows of half w, and the keys its last row sees
+  __device__ __forceinline__ int rows_of(int w) const { return max(0, min(BM, rows() - BM * w)); }
+  __device__ __forceinline__ int key_end(int w) const {
+    const int r = rows_of(w);
+    return r == 0 ? 0 : past + tok0() + (BM * w + r - 1) / group + 1;
+  }
+  __device__ __forceinline__ int key_end() const {
+    return past + tok0() + (rows() - 1) / group + 1;
+  }
+  __device__ __forceinline__ int tiles() const { return (key_end() + BN - 1) / BN; }
+  __device__ __forceinline__ int tiles_of(int w) const { return (key_end(w) + BN - 1) / BN; }
+};
+
+__host__ __device__ constexpr int q_tiles(int len, int group) {
+  return (len * group + kRows - 1) / kRows;
+}
+// Key tiles of all items of one kv head of a sequence.
+__device__ __forceinline__ long long seq_tiles(const SeqSpan& sp, int group) {
+  long long n = 0;
+  const int nq = q_tiles(sp.len, group), per = kRows / group;
+  for (int q = 0; q < nq; ++q) n += (sp.past + min(sp.len, (q + 1) * per) + BN - 1) / BN;
+  return n;
+}
+
+// The items in list order: sequences, their query tiles from the last (the longest) to the first,
+// the kv heads of each.
+struct ItemWalk {
+  const KvView& kv;
+  const ChunkIndex& at;
+  Item it;
+  __device__ __forceinline__ ItemWalk(const KvView& k, const ChunkIndex& x, int group, int z,
+                                      int qt, int kh)
+      : kv(k), at(x) {
+    it.group = group;
+    it.z = z;
+    it.qt = qt;
+    it.kh = kh;
+    take();
+  }
+  __device__ __forceinline__ bool take() {
+    const SeqSpan sp = seq_span(kv, at, it.z);
+    it.past = sp.past;
+    it.row0 = sp.row0;
+    it.len = sp.ok ? sp.len : 0;
+    return it.len > 0;
+  }
+  __device__ __forceinline__ void next() {
+    if (++it.kh < kv.hkv) return;
+    it.kh = 0;
+    if (--it.qt >= 0) return;
+    do ++it.z;
+    while (it.z < at.nseq && !take());
+    it.qt = q_tiles(it.len, it.group) - 1;
+  }
+};
+
+// Eight 4-bit codes of a word as f16 values code * s + lo (one rounding: an f16 multiply-add), in
+// the order 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ uint4 q4_piece(uint32_t w, uint32_t params) {
+  const uint32_t s2 = __byte_perm(params, params, 0x1010), l2 = __byte_perm(params, params, 0x3232);
+  const __half2 s = *reinterpret_cast<const __half2*>(&s2);
+  const __half2 lo = *reinterpret_cast<const __half2*>(&l2);
+  const __half2 base = __floats2half2_rn(1024.f, 1024.f);
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t c = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;  // 1024 + code
+    const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s, lo);
+    r[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+// Position of dim d (0 .. 7) of a piece in that order.
+__device__ __forceinline__ constexpr int q4_place(int d) { return d < 4 ? 2 * d : 2 * d - 7; }
+
+template <int KVF>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_chunk_kernel(const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v,
+                      const __grid_constant__ ChunkArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                     ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = a.hq / a.kv.hkv;
+
+  // ---- this CTA's part of the list
+  const int per = (a.at.nseq + 255) / 256;
+  long long mine = 0, upto = 0, total = 0;
+  if (tid < 256) {
+    for (int z = tid * per; z < min((tid + 1) * per, a.at.nseq); ++z) {
+      const SeqSpan sp = seq_span(a.kv, a.at, z);
+      if (!sp.ok) {
+        if (blockIdx.x == 0) atomicOr(a.err, kErrPosBeyondCache);
+      } else if (sp.len > 0) {
+        mine += a.kv.hkv * (a.split ? seq_tiles(sp, group)
+                                    : static_cast<long long>(q_tiles(sp.len, group)));
+      }
+    }
+    upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) s.wsum[warp] = upto;
+  }
+  if (tid == 0) {
+    mbar_init(&s.q_full, kLoadWarps);
+    mbar_init(&s.q_free, 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s.kv_full[i], KVF == kKvF16 ? 1 : kLoadWarps);
+      mbar_init(&s.kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.s_free[i], 4);
+      mbar_init(&s.p_full[i], 4);
+      mbar_init(&s.pv_done[i], 1);
+      mbar_init(&s.o_free[i], 4);
+    }
+    for (int i = 0; i < 8; ++i) s.bad[i] = 0;
+    s.abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    if (w == warp) upto += total;
+    total += s.wsum[w];
+  }
+  const int parts = int(min(static_cast<long long>(gridDim.x), total));
+  const int b = blockIdx.x;
+  launch_dependents();
+  if (a.split && tid == 0) a.joins[b] = make_int4(-1, 0, 0, 0);
+  if (b >= parts) return;
+  const long long lo = a.split ? total * b / parts : b;
+  if (tid < 256 && lo < upto && lo >= upto - mine) {
+    long long at = upto - mine;
+    for (int z = tid * per;; ++z) {
+      const SeqSpan sp = seq_span(a.kv, a.at, z);
+      if (!sp.ok || sp.len <= 0) continue;
+      const int nq = q_tiles(sp.len, group);
+      bool found = false;
+      for (int qt = nq - 1; qt >= 0 && !found; --qt) {
+        const Item it{z, 0, qt, sp.past, sp.row0, sp.len, group};
+        const int nk = it.tiles(), unit = a.split ? nk : 1;
+        if (lo < at + static_cast<long long>(unit) * a.kv.hkv) {
+          const long long r = lo - at;
+          s.z0 = z;
+          s.qt0 = qt;
+          s.kh0 = int(r / unit);
+          s.k0 = a.split ? int(r % unit) : 0;
+          s.n_tiles = a.split ? int(total * (b + 1) / parts - lo) : nk;
+          found = true;
+        }
+        at += static_cast<long long>(unit) * a.kv.hkv;
+      }
+      if (found) break;
+    }
+  }
+  if (warp == kMmaWarp) tmem_alloc(&s.tmem_base, kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  const int n_tiles = s.n_tiles;
+
+  if (warp >= 8) {
+    regs_dec<kOtherRegs>();
+    if (warp == kMmaWarp) {
+      // ---------------------------------------------------------------- MMA issuer
+      constexpr uint32_t idesc_s = idesc_f16_f32(BM, BN, 0, 0);
+      constexpr uint32_t idesc_pv = idesc_f16_f32(BM, D, 0, 1);
+      static_assert(sizeof(s.q[0]) == 16384 && sizeof(s.kv[0]) == 32768, "16 KB tiles");
+      const uint64_t qdesc0 = smem_desc_sw128(smem_u32(s.q[0]), 16, 1024);
+      const uint64_t kdesc0 = smem_desc_sw128(smem_u32(s.kv[0][0]), 16, 1024);
+      const uint64_t vdesc0 = smem_desc_sw128(smem_u32(s.kv[0][1]), 0, 1024);
+      auto issue_s = [&](int w, int st) {  // S_w = Q_w K_st^T
+        if (elect_one()) {
+          const uint64_t qd = qdesc0 + uint64_t(w) * 1024, kd = kdesc0 + uint64_t(st) * 2048;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_f16_ss(tmem + col_s(w), qd + 2 * kk, kd + 2 * kk, idesc_s, kk > 0);
+          mma_commit(&s.s_full[w]);
+        }
+        __syncwarp();
+      };
+      auto issue_pv = [&](int w, int st, bool acc) {  // O_w += P_w V_st
+        if (elect_one()) {
+          const uint64_t vd = vdesc0 + uint64_t(st) * 2048;
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk)
+            mma_f16_ts(tmem + col_o(w), tmem + col_p(w) + kk * 8, vd + 128 * kk, idesc_pv,
+                       (acc || kk > 0) ? 1u : 0u);
+          mma_commit(&s.pv_done[w]);
+        }
+        __syncwarp();
+      };
+      auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+        bool r = true;
+        if (lane == 0) r = wait_bar(s, bar, parity, a.err);
+        return __shfl_sync(0xffffffffu, r ? 1 : 0, 0) != 0;
+      };
+      ItemWalk w8(a.kv, a.at, group, s.z0, s.qt0, s.kh0);
+      int c = 0, seg = 0;                  // tiles and parts so far
+      int n_s[2] = {0, 0}, n_pv[2] = {0, 0}, n_o[2] = {0, 0};  // S, P.V, ended O per half
+      bool ok = true;
+      for (int k0 = s.k0, left = n_tiles; ok && left > 0; k0 = 0, ++seg, w8.next()) {
+        const Item it = w8.it;
+        const int k1 = min(it.tiles(), k0 + left);
+        const int nk0 = it.tiles_of(0), nk1 = it.tiles_of(1);
+        left -= k1 - k0;
+        auto score = [&](int w, int jj, int cc) {  // S of half w for key tile jj, when it has rows
+          if (jj >= (w ? nk1 : nk0)) return true;
+          if (n_s[w] > 0 && !wait_warp(&s.s_free[w], (n_s[w] - 1) & 1)) return false;
+          tc_fence_after();
+          issue_s(w, cc % kStages);
+          ++n_s[w];
+          return true;
+        };
+        if (!wait_warp(&s.q_full, seg & 1)) { ok = false; break; }
+        for (int jj = k0; ok && jj < k1; ++jj, ++c) {
+          const int st = c % kStages;
+          if (jj == k0) {
+            ok = wait_warp(&s.kv_full[st], (c / kStages) & 1);
+            tc_fence_after();
+            ok = ok && score(0, jj, c) && score(1, jj, c);
+          }
+          if (ok && jj + 1 < k1) {  // the next tile's scores, while the softmax of this one runs
+            ok = wait_warp(&s.kv_full[(c + 1) % kStages], ((c + 1) / kStages) & 1);
+            tc_fence_after();
+            ok = ok && score(0, jj + 1, c + 1) && score(1, jj + 1, c + 1);
+          }
+          if (!ok) break;
+          if (jj == k1 - 1 && elect_one()) mma_commit(&s.q_free);
+          __syncwarp();
+          const int tail = it.key_end() - jj * BN;
+          if (KVF == kKvF16 && tail < BN) {
+            // Rows behind the last key may hold anything; P is 0 there, but 0 * NaN is NaN
+            uint4* vrow = reinterpret_cast<uint4*>(s.kv[st][1]);
+            for (int i = tail * 8 + lane; i < BN * 8; i += 32) vrow[i] = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (!ok || jj >= (w ? nk1 : nk0)) continue;
+            if (jj == k0 && n_o[w] > 0) ok = wait_warp(&s.o_free[w], (n_o[w] - 1) & 1);
+            ok = ok && wait_warp(&s.p_full[w], n_pv[w] & 1);
+            if (!ok) continue;
+            tc_fence_after();
+            issue_pv(w, st, jj > k0);
+            ++n_pv[w];
+          }
+          if (!ok) break;
+          if (elect_one()) mma_commit(&s.kv_empty[st]);
+          __syncwarp();
+        }
+        if (k0 < nk0) ++n_o[0];
+        if (k0 < nk1) ++n_o[1];
+      }
+    } else {
+      // ---------------------------------------------------------------- loading warps
+      const int lt = tid - kLoadWarp0 * 32;
+      const int w = lt & 7;  // 16-byte piece of a row (kLoaders is a multiple of 8)
+      constexpr int kTasks = (2 * BN * 8 + kLoaders - 1) / kLoaders;
+      const bool paged = a.kv.table != nullptr;
+      ItemWalk walk(a.kv, a.at, group, s.z0, s.qt0, s.kh0);
+      int c = 0, seg = 0;
+      bool ok = true;
+      float ksc[KVF == kKvI8 ? 8 : 1], vsc[KVF == kKvI8 ? 8 : 1];
+      if (KVF == kKvF16 && lt == 0) {
+        prefetch_tensormap(&tm_k);
+        prefetch_tensormap(&tm_v);
+      }
+      for (int k0 = s.k0, left = n_tiles; ok && left > 0; k0 = 0, ++seg, walk.next()) {
+        const Item it = walk.it;
+        const int k1 = min(it.tiles(), k0 + left), key_end = it.key_end();
+        left -= k1 - k0;
+        if (KVF == kKvI8) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int ch = a.kv.per_channel ? it.kh * 64 + 8 * w + i : 0;
+            ksc[i] = a.kv.k_scale[ch];
+            vsc[i] = a.kv.v_scale[ch];
+          }
+        }
+        // Q: the 16-byte pieces of the item's rows, zeros behind them
+        if (seg > 0) {
+          ok = wait_bar(s, &s.q_free, (seg - 1) & 1, a.err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        // The mark of four parts ahead is cleared: no loading warp is there yet (each part's Q
+        // waits for the products of the one before), and the part that used it last has ended
+        // (three parts back, before this one's Q could be asked for).
+        if (lt == 0) s.bad[(seg + 4) & 7] = 0;
+        const int rows = it.rows();
+        for (int i = lt; i < kRows * 8; i += kLoaders) {
+          const int r = i >> 3;
+          if (r >= BM && rows <= BM) break;
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (r < rows)
+            x = *reinterpret_cast<const uint4*>(
+                a.q + (int64_t(it.row0) + it.tok0() + r / group) * a.ld_q +
+                (it.kh * group + r % group) * D + w * 8);
+          if (KVF == kKvQ4)
+            x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632),
+                           __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+          *reinterpret_cast<uint4*>(reinterpret_cast<char*>(s.q[r / BM]) + (r % BM) * 128 +
+                                    ((w ^ (r & 7)) << 4)) = x;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.q_full);
+
+        for (int jj = k0; ok && jj < k1; ++jj, ++c) {
+          const int st = c % kStages, key0 = jj * BN, valid = min(BN, key_end - key0);
+          if constexpr (KVF == kKvF16) {
+            if (warp != kLoadWarp0) continue;
+            // one box per page (or one of 128 rows)
+            const int box = paged ? min(1 << a.kv.shift, BN) : BN;
+            const int boxes = (valid + box - 1) / box;
+            int64_t row = 0;
+            if (lane < boxes) row = kv_row(a.kv, it.z, key0 + lane * box);
+            const bool bad = __any_sync(0xffffffffu, row < 0);
+            if (lane == 0 && c >= kStages)
+              ok = wait_bar(s, &s.kv_empty[st], (c / kStages - 1) & 1, a.err);
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            if (!ok) break;
+            if (lane == 0) {
+              if (bad) {
+                s.bad[seg & 7] = 1;
+                atomicOr(a.err, kErrPosBeyondCache);
+              }
+              mbar_arrive_expect_tx(&s.kv_full[st],
+                                    uint32_t(bad ? 0 : 2 * boxes * box * 128) +
+                                        uint32_t(c == 0 ? a.wait_deficit : 0));
+            }
+            __syncwarp();
+            if (!bad && lane < boxes) {
+              tma_load_2d(&s.kv[st][0][lane * box * D], &tm_k, it.kh * D, int32_t(row),
+                          &s.kv_full[st]);
+              tma_load_2d(&s.kv[st][1][lane * box * D], &tm_v, it.kh * D, int32_t(row),
+                          &s.kv_full[st]);
+            }
+          } else {
+            uint32_t raw[kTasks][2];
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < kTasks; ++i) {
+              const int u = (i * kLoaders + lt) >> 3, key = u & (BN - 1);
+              raw[i][0] = raw[i][1] = 0u;  // rows behind the last key: zeros
+              if (u >= 2 * BN || key >= valid) continue;
+              const int64_t row = kv_row(a.kv, it.z, key0 + key);
+              if (row < 0) {
+                bad = true;
+                continue;
+              }
+              const unsigned char* src = (u >= BN ? a.kv.v : a.kv.k) + row * a.kv.row_bytes;
+              if (KVF == kKvQ4) {
+                const uint32_t* unit =
+                    reinterpret_cast<const uint32_t*>(src + it.kh * kQ4UnitBytes);
+                raw[i][0] = unit[w];
+                raw[i][1] = unit[8];
+              } else {
+                const uint2 x = *reinterpret_cast<const uint2*>(src + it.kh * D + 8 * w);
+                raw[i][0] = x.x;
+                raw[i][1] = x.y;
+              }
+            }
+            if (bad) {
+              s.bad[seg & 7] = 1;
+              atomicOr(a.err, kErrPosBeyondCache);
+            }
+            if (c >= kStages) ok = wait_bar(s, &s.kv_empty[st], (c / kStages - 1) & 1, a.err);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < kTasks; ++i) {
+              const int u = (i * kLoaders + lt) >> 3, key = u & (BN - 1);
+              if (u >= 2 * BN) continue;
+              uint4 x;
+              if constexpr (KVF == kKvQ4) {
+                x = q4_piece(raw[i][0], raw[i][1]);
+              } else {
+                float f[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  f[k] = float(static_cast<int8_t>(raw[i][k >> 2] >> (8 * (k & 3)))) *
+                         (u >= BN ? vsc[k] : ksc[k]);
+                x = make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]),
+                               pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
+              }
+              *reinterpret_cast<uint4*>(reinterpret_cast<char*>(s.kv[st][u >= BN ? 1 : 0]) +
+                                        key * 128 + ((w ^ (key & 7)) << 4)) = x;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (c == 0 && lt == 0 && a.wait_deficit)
+                mbar_arrive_expect_tx(&s.kv_full[st], uint32_t(a.wait_deficit));
+              else
+                mbar_arrive(&s.kv_full[st]);
+            }
+          }
+        }
+      }
+      if (KVF == kKvF16 && warp == kLoadWarp0 && s.abort_flag) {
+        // let the copies already in flight land before the CTA exits
+        for (int i = max(0, c - kStages); i < c; ++i) {
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(&s.kv_full[i % kStages], (i / kStages) & 1) &&
+                 globaltimer_ns() - t0 < kWaitLimitNs) {
+          }
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax warpgroups
+    regs_inc<kSoftmaxRegs>();
+    const int w = warp >> 2;
+    const int r = tid & 127;  // row of the half = TMEM lane
+    const uint32_t lane_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
+    const float sl2 = a.scale_log2;
+    ItemWalk walk(a.kv, a.at, group, s.z0, s.qt0, s.kh0);
+    int n = 0, seg = 0;  // tiles of this half, parts
+    bool ok = true;
+    for (int k0 = s.k0, left = n_tiles; ok && left > 0; k0 = 0, ++seg, walk.next()) {
+      const Item it = walk.it;
+      const int nk = it.tiles(), k1 = min(nk, k0 + left);
+      left -= k1 - k0;
+      const int rows = it.rows_of(w), mine_end = min(k1, it.tiles_of(w));
+      if (rows == 0) continue;
+      const int first_lim = it.past + it.tok0() + BM * w / group + 1;  // keys the first row sees
+      const int key_lim = first_lim + r / group;
+      float m_raw = -INFINITY, l_run = 0.f;
+      for (int j = k0; j < mine_end; ++j, ++n) {
+        ok = wait_bar(s, &s.s_full[w], n & 1, a.err);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t sv[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32(lane_addr + col_s(w) + q * 32, sv[q]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.s_free[w]);
+        const int key0 = j * BN;
+        if (key0 + BN > first_lim) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (key0 + q * 32 + i >= key_lim) sv[q][i] = __float_as_uint(-INFINITY);
+        }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            m4[(i >> 1) & 3] = fmax3(m4[(i >> 1) & 3], __uint_as_float(sv[q][i]),
+                                     __uint_as_float(sv[q][i + 1]));
+        const float mx = fmax3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
+        const bool grow = (mx - m_raw) * sl2 > kRescaleLog2;
+        const float alpha = grow ? fast_exp2((m_raw - mx) * sl2) : 1.0f;
+        if (grow) m_raw = mx;
+        const float neg = (m_raw == -INFINITY) ? 0.f : -m_raw * sl2;
+        uint32_t pk[2][32];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const int q = half * 2 + cc;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float x0, x1;
+              fma2(__uint_as_float(sv[q][2 * i]), __uint_as_float(sv[q][2 * i + 1]), sl2, neg, x0,
+                   x1);
+              pk[half][cc * 16 + i] = i < kPolyPairs ? ex2_poly_f16x2(x0, x1) : ex2_f16x2(x0, x1);
+            }
+          }
+        float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const uint32_t* q4 = &pk[half][4 * g];
+            ps[g & 3] =
+                add_f16x2_to_f32(hadd2(hadd2(q4[0], q4[1]), hadd2(q4[2], q4[3])), ps[g & 3]);
+          }
+        // P is free (and O holds the tiles before) once the last P.V has completed
+        if (j > k0) {
+          ok = wait_bar(s, &s.pv_done[w], (n - 1) & 1, a.err);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+        }
+        tc_fence_after();
+        tmem_st32(lane_addr + col_p(w), pk[0]);
+        tmem_st32(lane_addr + col_p(w) + 32, pk[1]);
+        tmem_st_wait();
+        l_run = fmaf(l_run, alpha, (ps[0] + ps[1]) + (ps[2] + ps[3]));
+        if (j > k0 && __any_sync(0xffffffffu, grow)) {
+          uint32_t ov[2][32];
+          tmem_ld32(lane_addr + col_o(w), ov[0]);
+          tmem_ld32(lane_addr + col_o(w) + 32, ov[1]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            ov[0][i] = __float_as_uint(__uint_as_float(ov[0][i]) * alpha);
+            ov[1][i] = __float_as_uint(__uint_as_float(ov[1][i]) * alpha);
+          }
+          tmem_st32(lane_addr + col_o(w), ov[0]);
+          tmem_st32(lane_addr + col_o(w) + 32, ov[1]);
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.p_full[w]);
+      }
+      if (!ok) break;
+      const bool whole = k0 == 0 && k1 == nk;
+      uint32_t ov[2][32];
+      if (k0 < mine_end) {
+        ok = wait_bar(s, &s.pv_done[w], (n - 1) & 1, a.err);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        tmem_ld32(lane_addr + col_o(w), ov[0]);
+        tmem_ld32(lane_addr + col_o(w) + 32, ov[1]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.o_free[w]);
+      } else {  // this half's keys all lie in other CTAs' parts
+#pragma unroll
+        for (int i = 0; i < 32; ++i) ov[0][i] = ov[1][i] = 0u;
+      }
+      if (KVF == kKvQ4) {  // the dims back in their order
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int g = 0; g < 32; g += 8) {
+            uint32_t t[8];
+#pragma unroll
+            for (int d = 0; d < 8; ++d) t[d] = ov[h][g + q4_place(d)];
+#pragma unroll
+            for (int d = 0; d < 8; ++d) ov[h][g + d] = t[d];
+          }
+      }
+      const bool bad = s.bad[seg & 7] != 0;
+      if (!whole && tid == 0 && k0 == 0) {  // the item begins here: what there is to join
+        const long long end = lo + (n_tiles - left) + (nk - k1);  // list position behind the item
+        const int last = int((end * parts - 1) / total);
+        a.joins[b] = make_int4(it.z, it.kh, it.qt, ((last - b + 1) << 1) | (seg == 0 ? 0 : 1));
+      }
+      if (r < rows) {
+        if (whole) {
+          if (!bad) {
+            const float inv = __fdiv_rn(1.0f, l_run);
+            uint4* dst = reinterpret_cast<uint4*>(
+                a.out + (int64_t(it.row0) + it.tok0() + (BM * w + r) / group) * a.ld_o +
+                (it.kh * group + r % group) * D);
+#pragma unroll
+            for (int i = 0; i < D; i += 8) {
+              const uint32_t* o = &ov[i >> 5][i & 31];
+              dst[i / 8] = make_uint4(
+                  pack_half2(__uint_as_float(o[0]) * inv, __uint_as_float(o[1]) * inv),
+                  pack_half2(__uint_as_float(o[2]) * inv, __uint_as_float(o[3]) * inv),
+                  pack_half2(__uint_as_float(o[4]) * inv, __uint_as_float(o[5]) * inv),
+                  pack_half2(__uint_as_float(o[6]) * inv, __uint_as_float(o[7]) * inv));
+            }
+          }
+        } else {
+          float4* rec = reinterpret_cast<float4*>(
+              a.parts + ((int64_t(b) * 2 + (seg == 0 ? 0 : 1)) * kRows + BM * w + r) * kRec);
+#pragma unroll
+          for (int i = 0; i < D; i += 4) {
+            const uint32_t* o = &ov[i >> 5][i & 31];
+            rec[i / 4] = make_float4(__uint_as_float(o[0]), __uint_as_float(o[1]),
+                                     __uint_as_float(o[2]), __uint_as_float(o[3]));
+          }
+          // log2 units; a sum below 0: some page was refused
+          const float m2 = m_raw == -INFINITY ? -1e30f : m_raw * sl2;
+          rec[16] = make_float4(m2, bad ? -1.f : l_run, 0.f, 0.f);
+        }
+      }
+    }
+    // a wait ran out: a part that others join is marked, the rest stays as it was
+    if (!ok && a.split) {
+      ItemWalk again(a.kv, a.at, group, s.z0, s.qt0, s.kh0);
+      int i = 0;
+      for (int k0 = s.k0, left = n_tiles; left > 0; k0 = 0, ++i, again.next()) {
+        const Item it = again.it;
+        const int nk = it.tiles(), k1 = min(nk, k0 + left);
+        left -= k1 - k0;
+        if (i < seg || (k0 == 0 && k1 == nk) || r >= it.rows_of(w)) continue;
+        float* rec = a.parts + ((int64_t(b) * 2 + (i == 0 ? 0 : 1)) * kRows + BM * w + r) * kRec;
+        rec[64] = -1e30f;
+        rec[65] = -1.f;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// CTA (b, y): rows 32 y .. of the item that began in CTA b and went on in others.  Half a warp per
+// row (16 lanes of 4 dims), records in CTA order.
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads)
+    join_chunk_kernel(const __grid_constant__ ChunkArgs a) {
+  grid_dependency_wait();
+  const int4 d = a.joins[blockIdx.x];
+  if (d.x < 0) return;
+  const int group = a.hq / a.kv.hkv, b = blockIdx.x, n = d.w >> 1, slot = d.w & 1;
+  const SeqSpan sp = seq_span(a.kv, a.at, d.x);
+  const Item it{d.x, d.y, d.z, sp.past, sp.row0, sp.len, group};
+  const int l16 = threadIdx.x & 15;
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {
+    const int r = blockIdx.y * 32 + pass * 16 + (threadIdx.x >> 4);
+    if (r >= it.rows()) return;
+    auto rec = [&](int i) {
+      return a.parts + ((int64_t(b + i) * 2 + (i == 0 ? slot : 0)) * kRows + r) * kRec;
+    };
+    float mx = -1e30f, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    bool bad = false;
+    for (int i0 = 0; i0 < n; i0 += 8) {  // eight records in flight
+      float2 ml[8];
+      float4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float* p = rec(min(i0 + i, n - 1));
+        ml[i] = __ldcg(reinterpret_cast<const float2*>(p + 64));
+        x[i] = __ldcg(reinterpret_cast<const float4*>(p) + l16);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i0 + i >= n) continue;
+        bad |= ml[i].y < 0.f;
+        const float m = fmaxf(mx, ml[i].x), c = fast_exp2(mx - m), e = fast_exp2(ml[i].x - m);
+        mx = m;
+        l = fmaf(l, c, ml[i].y * e);
+        acc.x = fmaf(acc.x, c, x[i].x * e);
+        acc.y = fmaf(acc.y, c, x[i].y * e);
+        acc.z = fmaf(acc.z, c, x[i].z * e);
+        acc.w = fmaf(acc.w, c, x[i].w * e);
+      }
+    }
+    if (bad) continue;
+    const float inv = __fdiv_rn(1.f, l);
+    reinterpret_cast<uint2*>(a.out + (int64_t(it.row0) + it.tok0() + r / group) * a.ld_o +
+                             (it.kh * group + r % group) * D)[l16] =
+        make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+
+// f16 pool as [rows][hkv * 64], boxes of 64 values x `box` rows, 128-byte swizzle.
+bool make_map(CUtensorMap* m, const void* base, int64_t width, int64_t rows, int box_rows) {
+  auto enc = get_encode();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {cuuint64_t(width), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(width) * 2};
+  cuuint32_t box[2] = {64, cuuint32_t(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+size_t chunk_parts_bytes(int num_sms) {
+  return size_t(num_sms) * 2 * kRows * kRec * sizeof(float);
+}
+size_t chunk_join_bytes(int num_sms) { return size_t(num_sms) * sizeof(int4); }
+
+cudaError_t launch_attn_chunk(const ChunkArgs& args, int num_sms, cudaStream_t s) {
+  ChunkArgs a = args;
+  CUtensorMap tk{}, tv{};
+  if (a.kv.format == kKvF16) {
+    const int64_t rows = a.kv.kv_rows << a.kv.shift;  // shift 0 when contiguous
+    const int box = a.kv.table && (1 << a.kv.shift) < BN ? 1 << a.kv.shift : BN;
+    if (rows > INT32_MAX) return cudaErrorInvalidValue;
+    if (!make_map(&tk, a.kv.k, int64_t(a.kv.hkv) * D, rows, box) ||
+        !make_map(&tv, a.kv.v, int64_t(a.kv.hkv) * D, rows, box))
+      return cudaErrorInvalidValue;
+  }
+  const int group = a.hq / a.kv.hkv;
+  // the items this call can have: every sequence may end in a part of one
+  const int64_t items = (a.at.n_rows * group / kRows + a.at.nseq) * a.kv.hkv;
+  a.split = items <= int64_t(kMaxItemsPerSm) * num_sms;
+  const int64_t ctas = a.split ? num_sms : items;
+  if (ctas > INT32_MAX) return cudaErrorInvalidValue;
+  const void* fn = a.kv.format == kKvF16  ? reinterpret_cast<const void*>(&attn_chunk_kernel<kKvF16>)
+                   : a.kv.format == kKvI8 ? reinterpret_cast<const void*>(&attn_chunk_kernel<kKvI8>)
+                                          : reinterpret_cast<const void*>(&attn_chunk_kernel<kKvQ4>);
+  const int smem = int(sizeof(Smem)) + 1024;
+  static PerDeviceOnce attrs[3];
+  const cudaError_t e = per_device_once(attrs[a.kv.format], [&](int&) {
+    // the split of the registers needs the launch to have them all: without, a warpgroup would
+    // wait for registers for good
+    cudaFuncAttributes fa;
+    cudaError_t r = cudaFuncGetAttributes(&fa, fn);
+    if (r != cudaSuccess) return r;
+    if (fa.numRegs != kLaunchRegs) return cudaErrorNotSupported;
+    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  });
+  if (e != cudaSuccess) return e;
+  void* argv[] = {&tk, &tv, &a};
+  cudaError_t le =
+      cudaLaunchKernel(fn, dim3(unsigned(ctas)), dim3(kThreads), argv, size_t(smem), s);
+  if (le != cudaSuccess || !a.split) return le;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(num_sms), kRows / 32);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_chunk_kernel, a);
+}
+
+}  // namespace p2p

@@ -247,7 +247,7 @@ struct FlashArgs {
   int32_t num_sms;       // non-causal: > 0 lets the last partial wave run as one-tile CTAs
 };
 
-// ---- caches of any layout (kv_append.cu, attn_kv.cu) ------------------------------------------
+// ---- caches of any layout (kv_append.cu) -------------------------------------------------------
 constexpr int kQ4UnitBytes = 36;  // one (token, kv head): 32 bytes of codes, f16 scale, f16 lo
 constexpr int64_t q4_row_bytes(int hkv) { return (int64_t(hkv) * kQ4UnitBytes + 15) / 16 * 16; }
 // Bytes of one cached token row (all kv heads) of format f.
@@ -317,7 +317,17 @@ struct AttnKvArgs {
   const __half* rope;
   float eps;
 };
-cudaError_t launch_attn_kv(const AttnKvArgs& a, cudaStream_t s);
+
+// ---- attn_chunk.cu ----------------------------------------------------------------------------
+struct ChunkArgs : AttnKvArgs {
+  float* parts;  // chunk_parts_bytes(): records of items that straddle CTAs
+  int4* joins;   // chunk_join_bytes(): per CTA the item to join, if any
+  int32_t wait_deficit;
+  int32_t split;  // set by the launcher: tiles cut into equal parts, else one CTA per item
+};
+size_t chunk_parts_bytes(int num_sms);
+size_t chunk_join_bytes(int num_sms);
+cudaError_t launch_attn_chunk(const ChunkArgs& a, int num_sms, cudaStream_t s);
 
 // ---- attn_q4.cu -------------------------------------------------------------------------------
 struct DecodeQ4Args : AttnKvArgs {

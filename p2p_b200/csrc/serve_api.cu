@@ -221,7 +221,7 @@ p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
   if (!ctx) return P2P_ERR_INVALID_ARG;
   p2p_status st = check_f16(ctx, prm, "attn_chunk_kv");
   if (st != P2P_OK) return st;
-  p2p::AttnKvArgs a{};
+  p2p::ChunkArgs a{};
   st = p2p::make_kv_view(ctx, layout, prm->num_kv_heads, k_cache, v_cache, kv_rows, offsets, nseq,
                          "attn_chunk_kv", &a.kv);
   if (st != P2P_OK) return st;
@@ -243,8 +243,17 @@ p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
   a.hq = prm->num_heads;
   a.scale_log2 = p2p::eff_scale_log2(prm);
   a.err = p2p::ctx_dev_err(ctx);
+  if (a.kv.format == P2P_KV_F16 && (a.kv.kv_rows << a.kv.shift) > INT32_MAX)
+    return fail(ctx, P2P_ERR_UNSUPPORTED, "attn_chunk_kv: f16 caches of more than 2^31 rows");
   OnDevice g(p2p::ctx_device(ctx));
-  return launched(ctx, p2p::launch_attn_kv(a, static_cast<cudaStream_t>(stream)),
+  unsigned char* ws = nullptr;
+  st = p2p::ctx_serve_workspace(ctx, static_cast<cudaStream_t>(stream), "attn_chunk_kv", &ws);
+  if (st != P2P_OK) return st;
+  a.joins = reinterpret_cast<int4*>(ws);
+  a.parts = reinterpret_cast<float*>(ws + p2p::chunk_join_bytes(p2p::ctx_num_sms(ctx)));
+  a.wait_deficit = p2p::debug_wait_deficit();
+  return launched(ctx, p2p::launch_attn_chunk(a, p2p::ctx_num_sms(ctx),
+                                              static_cast<cudaStream_t>(stream)),
                   "attn_chunk_kv launch");
 }
 

@@ -404,6 +404,9 @@ CHUNKS = [
     ((32, 8), 16, [3], [9000]),
     ((16, 8), 16, [4] * 40, [(53 * i) % 300 for i in range(40)]),
     ((24, 12), 16, [1024], [100]),
+    # more items than the equal parts are for: a CTA each
+    ((64, 8), 64, [2400, 5, 77], [3, 0, 500]),
+    ((16, 16), 16, [5] * 48, [(31 * i) % 500 for i in range(48)]),
 ]
 
 
@@ -950,6 +953,34 @@ def test_another_stream_than_the_current_one(ctx):
     want, tol = attention64(c, q, [0], [513], True)
     assert_within(out, want, tol)
     assert torch.equal(out, out2)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows", [[70, 3], [4900, 100]])
+def test_chunk_wait_runs_out(ctx, fmt, rows):
+    import p2p_b200
+    past = [900, 40]
+    c = Cache(77, fmt, 16, 32, 8, [p + r for p, r in zip(past, rows)])
+    q = randh(gen(78), sum(rows), 32 * D)
+    out = torch.full_like(q, 7.0)
+    args = (c.prm, q, c.k, c.v, i32(past), starts_of(rows), out)
+    kw = dict(max_len=6000, **c.kw())
+    ctx.attn_chunk_kv(*args, **kw)
+    ctx.sync()
+    good = out.clone()
+    out.fill_(7.0)
+    try:
+        p2p_b200.lib.p2p_debug_set_wait_deficit(16)
+        ctx.attn_chunk_kv(*args, **kw)
+        with pytest.raises(p2p_b200.P2PError) as e:
+            ctx.sync()
+    finally:
+        p2p_b200.lib.p2p_debug_set_wait_deficit(0)
+    assert e.value.status == p2p_b200.P2P_ERR_TIMEOUT
+    assert (out == 7).all()
+    ctx.attn_chunk_kv(*args, **kw)
+    ctx.sync()
+    assert torch.equal(out, good)
 
 
 @pytest.mark.parametrize("heads", [(32, 8), (16, 2)])
