@@ -45,8 +45,8 @@ constexpr int kStages = 5;
 constexpr int kThreads = 512;
 constexpr int kMmaWarp = 8, kLoadWarp0 = 9, kLoadWarps = 7;
 constexpr int kLoaders = kLoadWarps * 32;
-// setmaxnreg splits the 512 x 128 registers of the launch: 256 x 192 + 256 x 64
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 192, kOtherRegs = 64;
+// setmaxnreg splits the 512 x 128 registers of the launch: 256 x 176 + 256 x 80
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kOtherRegs = 80;
 static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
@@ -67,6 +67,8 @@ struct __align__(128) Smem {
   uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];
   long long wsum[8];
   int z0, qt0, kh0, k0, n_tiles;
+  int4 part[8];  // of part i & 7, for the MMA warp: first and end key tile, the halves' tiles
+  int part_tail[8];  // its item's keys
   volatile int bad[8];  // of part i & 7 of this CTA: some page was refused
   uint32_t tmem_base;
   volatile int abort_flag;
@@ -303,63 +305,81 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) r = wait_bar(s, bar, parity, a.err);
         return __shfl_sync(0xffffffffu, r ? 1 : 0, 0) != 0;
       };
-      ItemWalk w8(a.kv, a.at, group, s.z0, s.qt0, s.kh0);
-      int c = 0, seg = 0;                  // tiles and parts so far
-      int n_s[2] = {0, 0}, n_pv[2] = {0, 0}, n_o[2] = {0, 0};  // S, P.V, ended O per half
-      bool ok = true;
-      for (int k0 = s.k0, left = n_tiles; ok && left > 0; k0 = 0, ++seg, w8.next()) {
-        const Item it = w8.it;
-        const int k1 = min(it.tiles(), k0 + left);
-        const int nk0 = it.tiles_of(0), nk1 = it.tiles_of(1);
-        left -= k1 - k0;
-        auto score = [&](int w, int jj, int cc) {  // S of half w for key tile jj, when it has rows
-          if (jj >= (w ? nk1 : nk0)) return true;
-          if (n_s[w] > 0 && !wait_warp(&s.s_free[w], (n_s[w] - 1) & 1)) return false;
-          tc_fence_after();
-          issue_s(w, cc % kStages);
-          ++n_s[w];
+      int st = 0, st1 = 1 % kStages;       // stage of this tile and of the next
+      uint32_t ph = 0, ph1 = 0;            // their parities
+      uint32_t n_s0 = 0, n_s1 = 0, n_pv0 = 0, n_pv1 = 0, n_o0 = 0, n_o1 = 0;  // per half: S, P.V,
+      bool ok = true;                                                         // ended O
+      uint32_t seg = 0;
+      for (int left = n_tiles; ok && left > 0; ++seg) {
+        ok = wait_warp(&s.q_full, seg & 1);
+        if (!ok) break;
+        const int4 part = s.part[seg & 7];
+        const int k1 = part.y, nk0 = part.z, nk1 = part.w;
+        left -= k1 - part.x;
+        // S of both halves for key tile jj in stage x, where they have rows that see it
+        auto score = [&](int jj, int x) {
+          if (jj < nk0) {
+            if (n_s0 > 0 && !wait_warp(&s.s_free[0], (n_s0 - 1) & 1)) return false;
+            tc_fence_after();
+            issue_s(0, x);
+            ++n_s0;
+          }
+          if (jj < nk1) {
+            if (n_s1 > 0 && !wait_warp(&s.s_free[1], (n_s1 - 1) & 1)) return false;
+            tc_fence_after();
+            issue_s(1, x);
+            ++n_s1;
+          }
           return true;
         };
-        if (!wait_warp(&s.q_full, seg & 1)) { ok = false; break; }
-        for (int jj = k0; ok && jj < k1; ++jj, ++c) {
-          const int st = c % kStages;
-          if (jj == k0) {
-            ok = wait_warp(&s.kv_full[st], (c / kStages) & 1);
+        ok = wait_warp(&s.kv_full[st], ph);
+        tc_fence_after();
+        ok = ok && score(part.x, st);
+        for (int jj = part.x; ok && jj < k1; ++jj) {
+          if (jj + 1 < k1) {  // the next tile's scores, while the softmax of this one runs
+            ok = wait_warp(&s.kv_full[st1], ph1);
             tc_fence_after();
-            ok = ok && score(0, jj, c) && score(1, jj, c);
-          }
-          if (ok && jj + 1 < k1) {  // the next tile's scores, while the softmax of this one runs
-            ok = wait_warp(&s.kv_full[(c + 1) % kStages], ((c + 1) / kStages) & 1);
-            tc_fence_after();
-            ok = ok && score(0, jj + 1, c + 1) && score(1, jj + 1, c + 1);
-          }
-          if (!ok) break;
-          if (jj == k1 - 1 && elect_one()) mma_commit(&s.q_free);
-          __syncwarp();
-          const int tail = it.key_end() - jj * BN;
-          if (KVF == kKvF16 && tail < BN) {
-            // Rows behind the last key may hold anything; P is 0 there, but 0 * NaN is NaN
-            uint4* vrow = reinterpret_cast<uint4*>(s.kv[st][1]);
-            for (int i = tail * 8 + lane; i < BN * 8; i += 32) vrow[i] = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
+            ok = ok && score(jj + 1, st1);
+            if (!ok) break;
+          } else {
+            if (elect_one()) mma_commit(&s.q_free);
             __syncwarp();
+            const int tail = s.part_tail[seg & 7] - jj * BN;
+            if (KVF == kKvF16 && tail < BN) {
+              // Rows behind the last key may hold anything; P is 0 there, but 0 * NaN is NaN
+              uint4* vrow = reinterpret_cast<uint4*>(s.kv[st][1]);
+              for (int i = tail * 8 + lane; i < BN * 8; i += 32) vrow[i] = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
           }
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            if (!ok || jj >= (w ? nk1 : nk0)) continue;
-            if (jj == k0 && n_o[w] > 0) ok = wait_warp(&s.o_free[w], (n_o[w] - 1) & 1);
-            ok = ok && wait_warp(&s.p_full[w], n_pv[w] & 1);
-            if (!ok) continue;
+          if (jj < nk0) {
+            if (jj == part.x && n_o0 > 0) ok = wait_warp(&s.o_free[0], (n_o0 - 1) & 1);
+            ok = ok && wait_warp(&s.p_full[0], n_pv0 & 1);
+            if (!ok) break;
             tc_fence_after();
-            issue_pv(w, st, jj > k0);
-            ++n_pv[w];
+            issue_pv(0, st, jj > part.x);
+            ++n_pv0;
           }
-          if (!ok) break;
+          if (jj < nk1) {
+            if (jj == part.x && n_o1 > 0) ok = wait_warp(&s.o_free[1], (n_o1 - 1) & 1);
+            ok = ok && wait_warp(&s.p_full[1], n_pv1 & 1);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(1, st, jj > part.x);
+            ++n_pv1;
+          }
           if (elect_one()) mma_commit(&s.kv_empty[st]);
           __syncwarp();
+          st = st1;
+          ph = ph1;
+          if (++st1 == kStages) {
+            st1 = 0;
+            ph1 ^= 1;
+          }
         }
-        if (k0 < nk0) ++n_o[0];
-        if (k0 < nk1) ++n_o[1];
+        if (part.x < nk0) ++n_o0;
+        if (part.x < nk1) ++n_o1;
       }
     } else {
       // ---------------------------------------------------------------- loading warps
@@ -370,6 +390,54 @@ __global__ void __launch_bounds__(kThreads, 1)
       ItemWalk walk(a.kv, a.at, group, s.z0, s.qt0, s.kh0);
       int c = 0, seg = 0;
       bool ok = true;
+      // int8 and 4-bit rows on their way to a tile: this thread's pieces, loaded together (all page
+      // numbers, then all words), one tile ahead
+      uint32_t raw[KVF == kKvF16 ? 1 : kTasks][2];
+      auto fetch = [&](const Item& it, int key0, int valid, int seg) {
+        if constexpr (KVF != kKvF16) {
+          // a tile has at most 8 pages: their numbers, a load per warp
+          int32_t pages = 0, off = 0;
+          if (paged) {
+            const int p = (key0 >> a.kv.shift) + lane;
+            if (lane <= ((valid - 1) + (key0 & ((1 << a.kv.shift) - 1))) >> a.kv.shift)
+              pages = a.kv.table[int64_t(it.z) * a.kv.max_blocks + p];
+            if (__any_sync(0xffffffffu, pages < 0 || int64_t(pages) >= a.kv.kv_rows)) {
+              if (lane == 0) {
+                s.bad[seg & 7] = 1;
+                atomicOr(a.err, kErrPosBeyondCache);
+              }
+              valid = 0;  // nothing of this tile is read
+            }
+          } else {
+            off = a.kv.offsets[it.z];
+          }
+          const int mask = (1 << a.kv.shift) - 1;
+#pragma unroll
+          for (int i = 0; i < kTasks; ++i) {
+            const int u = (i * kLoaders + lt) >> 3, key = u & (BN - 1);
+            int64_t row = int64_t(off) + key0 + key;
+            if (paged) {
+              const int32_t pg = __shfl_sync(0xffffffffu, pages,
+                                             ((key0 & mask) + key) >> a.kv.shift);
+              row = (int64_t(pg) << a.kv.shift) | ((key0 + key) & mask);
+            }
+            raw[i][0] = raw[i][1] = 0u;  // rows behind the last key: zeros
+            if (u < 2 * BN && key < valid) {
+              const unsigned char* src = (u >= BN ? a.kv.v : a.kv.k) + row * a.kv.row_bytes;
+              if (KVF == kKvQ4) {
+                const uint32_t* unit =
+                    reinterpret_cast<const uint32_t*>(src + it.kh * kQ4UnitBytes);
+                raw[i][0] = unit[w];
+                raw[i][1] = unit[8];
+              } else {
+                const uint2 x = *reinterpret_cast<const uint2*>(src + it.kh * D + 8 * w);
+                raw[i][0] = x.x;
+                raw[i][1] = x.y;
+              }
+            }
+          }
+        }
+      };
       float ksc[KVF == kKvI8 ? 8 : 1], vsc[KVF == kKvI8 ? 8 : 1];
       if (KVF == kKvF16 && lt == 0) {
         prefetch_tensormap(&tm_k);
@@ -414,6 +482,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
+        if (lt == 0) {
+          s.part[seg & 7] = make_int4(k0, k1, it.tiles_of(0), it.tiles_of(1));
+          s.part_tail[seg & 7] = key_end;
+        }
         if (lane == 0) mbar_arrive(&s.q_full);
 
         for (int jj = k0; ok && jj < k1; ++jj, ++c) {
@@ -447,34 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                           &s.kv_full[st]);
             }
           } else {
-            uint32_t raw[kTasks][2];
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < kTasks; ++i) {
-              const int u = (i * kLoaders + lt) >> 3, key = u & (BN - 1);
-              raw[i][0] = raw[i][1] = 0u;  // rows behind the last key: zeros
-              if (u >= 2 * BN || key >= valid) continue;
-              const int64_t row = kv_row(a.kv, it.z, key0 + key);
-              if (row < 0) {
-                bad = true;
-                continue;
-              }
-              const unsigned char* src = (u >= BN ? a.kv.v : a.kv.k) + row * a.kv.row_bytes;
-              if (KVF == kKvQ4) {
-                const uint32_t* unit =
-                    reinterpret_cast<const uint32_t*>(src + it.kh * kQ4UnitBytes);
-                raw[i][0] = unit[w];
-                raw[i][1] = unit[8];
-              } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(src + it.kh * D + 8 * w);
-                raw[i][0] = x.x;
-                raw[i][1] = x.y;
-              }
-            }
-            if (bad) {
-              s.bad[seg & 7] = 1;
-              atomicOr(a.err, kErrPosBeyondCache);
-            }
+            if (jj == k0) fetch(it, key0, valid, seg);  // else on its way since the tile before
             if (c >= kStages) ok = wait_bar(s, &s.kv_empty[st], (c / kStages - 1) & 1, a.err);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -505,6 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               else
                 mbar_arrive(&s.kv_full[st]);
             }
+            if (jj + 1 < k1) fetch(it, key0 + BN, min(BN, key_end - key0 - BN), seg);
           }
         }
       }
