@@ -5,19 +5,20 @@
 // Work.  An item is 256 query rows of one sequence and kv head: 256 / G tokens times the G query
 // heads that share the kv head, so that one pass over the keys serves all of them and short chunks
 // of grouped heads fill the tensor cores' 128 rows.  An item runs over its keys in tiles of 128.
-//   few items: all tiles of all items form one list that is cut into equal parts, one per SM; an
-//     item that straddles CTAs leaves records (unnormalised rows, maxima, sums) which a dependent
-//     kernel joins in CTA order;
-//   many items: one CTA per item, the longest of each sequence first.
-// The choice goes by the number of items the call can have, against four per SM: records cost 70 KB
-// of traffic per straddling item and CTA, an uneven last wave a part of an item's time.
+// All tiles of all items form one list, the longest items of each sequence first, that is cut into
+// equal parts, one per SM, so ragged batches and causal prompts balance by themselves and a CTA's
+// roles run on from item to item.  An item counts kSetup units more than its tiles, for the start
+// and the end of its pipeline (without, the CTAs with a prompt's short first items took 2.5 times
+// as long as the others).  An item that straddles CTAs leaves records (unnormalised rows,
+// maxima, sums; at most two a CTA, 20 MB in all) which a dependent kernel joins in CTA order.
 //
 // Roles of a CTA (16 warps): two softmax warpgroups, one query row per thread, 128 rows each; one
-// warp that issues the MMAs; seven that load.  f16 rows come by TMA, a box per page; int8 and 4-bit
-// rows are converted by the loading warps while the previous tiles are at work, each value rounded
-// to f16 once, straight into the swizzled operand layout.  The eight codes of a 4-bit word become
-// one 16-byte piece in the order 0 4 1 5 2 6 3 7 (the order in which masking a word yields pairs);
-// the query's dims are stored in the same order and the output's are put back at the end.
+// warp that issues the MMAs; one that issues TMA loads: Q (a 3-D box: the group's heads of 128 / G
+// tokens), two items deep, and f16 rows, a box per page; four that convert int8 and 4-bit rows, each
+// value rounded to f16 once, into the swizzled operand layout.  A converting thread has one key of
+// the tile, its K and its V: the row's address is then worked out once per 128 values (eight lanes
+// per row took three times the instructions), and its page's number is loaded two tiles early and
+// its words one, into registers.
 //   S_w = Q_w K^T (M128 N128 K64) -> TMEM; P_w to TMEM as f16; O_w += P_w V (M128 N64 K128).
 // The softmax is that of the prompt kernel: exp2 with the scale folded in, partly by a cubic on the
 // FMA pipe, lazily rescaled (only when a row's maximum grows by 2^8).
@@ -41,35 +42,35 @@ using namespace sm100;
 
 constexpr int BM = 128, BN = 128, D = kHeadDim;
 constexpr int kRows = 2 * BM;  // rows of an item
-constexpr int kStages = 5;
 constexpr int kThreads = 512;
-constexpr int kMmaWarp = 8, kLoadWarp0 = 9, kLoadWarps = 7;
-constexpr int kLoaders = kLoadWarps * 32;
+constexpr int kMmaWarp = 8, kTmaWarp = 9, kLoadWarp0 = 12, kLoadWarps = 4;
+constexpr int kMarks = 16;
+constexpr int kSetup = 1;
 // setmaxnreg splits the 512 x 128 registers of the launch: 256 x 176 + 256 x 80
 constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kOtherRegs = 80;
 static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
+constexpr int kStages = 4;  // K/V tiles in flight
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kPolyPairs = 5;  // of every 16 exp pairs, these use the cubic
 constexpr int kRec = 68;       // a record's row: acc[64], max, sum, 2 pad
-constexpr int kMaxItemsPerSm = 4;
 
 __device__ __forceinline__ uint32_t col_s(int w) { return uint32_t(w) * 256u; }
 __device__ __forceinline__ uint32_t col_p(int w) { return uint32_t(w) * 256u + 128u; }
 __device__ __forceinline__ uint32_t col_o(int w) { return uint32_t(w) * 256u + 192u; }
 
 struct __align__(128) Smem {
-  __half q[2][BM * D];
+  __half q[2][2][BM * D];         // two items, two halves
   __half kv[kStages][2][BN * D];  // K, V
-  uint64_t q_full, q_free;
+  uint64_t q_full[2], q_free[2];
   uint64_t kv_full[kStages], kv_empty[kStages];
   uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];
   long long wsum[8];
-  int z0, qt0, kh0, k0, n_tiles;
+  int z0, qt0, kh0, off0, n_units;  // the first item of the CTA's part, and where in it
   int4 part[8];  // of part i & 7, for the MMA warp: first and end key tile, the halves' tiles
   int part_tail[8];  // its item's keys
-  volatile int bad[8];  // of part i & 7 of this CTA: some page was refused
+  volatile int bad[kMarks];  // of part i % kMarks of this CTA: some page was refused
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -78,7 +79,7 @@ __device__ __forceinline__ bool wait_bar(Smem& s, uint64_t* bar, uint32_t parity
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait_for(bar, parity, 2000)) return true;
     if (s.abort_flag) return false;
     if (globaltimer_ns() - t0 > kWaitLimitNs) {
       s.abort_flag = 1;
@@ -117,12 +118,31 @@ struct Item {
 __host__ __device__ constexpr int q_tiles(int len, int group) {
   return (len * group + kRows - 1) / kRows;
 }
-// Key tiles of all items of one kv head of a sequence.
-__device__ __forceinline__ long long seq_tiles(const SeqSpan& sp, int group) {
-  long long n = 0;
-  const int nq = q_tiles(sp.len, group), per = kRows / group;
-  for (int q = 0; q < nq; ++q) n += (sp.past + min(sp.len, (q + 1) * per) + BN - 1) / BN;
-  return n;
+// Key tiles of query tiles 0 .. n - 1 of a sequence: the sum of ceil(keys / 128), where tile q's last
+// row sees past + (q + 1) * per keys (`per` a power of two) but the sequence's last tile past + len.
+__host__ __device__ inline long long tiles_before(int past, int len, int group, int n) {
+  const int per = kRows / group, total = q_tiles(len, group);
+  const int full = n == total ? n - 1 : n;  // tiles whose tokens are all there, at least
+  long long sum = 0;
+  if (full > 0) {
+    if (per >= BN) {  // (past + 127) / 128 + q * (per / 128), q = 1 .. full
+      const long long a = (static_cast<long long>(past) + BN - 1) / BN;
+      sum = a * full + static_cast<long long>(per / BN) * full * (full + 1LL) / 2;
+    } else {  // floor((u + q) / k), u = (past + 127) / per, k = 128 / per
+      const long long k = BN / per, u = (static_cast<long long>(past) + BN - 1) / per;
+      auto upto = [k](long long m) {  // sum over 0 .. m of i / k
+        const long long t = m / k;
+        return k * (t * (t - 1) / 2) + t * (m - k * t + 1);
+      };
+      sum = upto(u + full) - upto(u);
+    }
+  }
+  if (full < n) sum += (static_cast<long long>(past) + len + BN - 1) / BN;
+  return sum;
+}
+
+__host__ __device__ inline long long units_before(int past, int len, int group, int n) {
+  return tiles_before(past, len, group, n) + static_cast<long long>(kSetup) * n;
 }
 
 // The items in list order: sequences, their query tiles from the last (the longest) to the first,
@@ -157,35 +177,79 @@ struct ItemWalk {
   }
 };
 
-// Eight 4-bit codes of a word as f16 values code * s + lo (one rounding: an f16 multiply-add), in
-// the order 0 4 1 5 2 6 3 7.
+// A CTA's parts of items, one after the other: the key tiles k0 .. k1 - 1 of each.
+struct PartWalk {
+  ItemWalk walk;
+  int off, left;  // unit of the item where the part begins, units of the CTA from there
+  int nk, k0, k1, seg;
+  bool live;
+  __device__ __forceinline__ PartWalk(const KvView& k, const ChunkIndex& x, int group,
+                                      const Smem& s)
+      : walk(k, x, group, s.z0, s.qt0, s.kh0), off(s.off0), left(s.n_units), seg(0) {
+    set();
+  }
+  __device__ __forceinline__ void set() {
+    nk = walk.it.tiles();
+    k0 = max(0, off - kSetup);
+    k1 = min(nk, off + left - kSetup);
+    live = k1 > k0;  // a CTA's units may end before the item's first tile
+  }
+  __device__ __forceinline__ void next() {
+    left -= kSetup + nk - off;
+    off = 0;
+    ++seg;
+    live = false;
+    if (left <= 0) return;
+    walk.next();
+    set();
+  }
+  __device__ __forceinline__ const Item& it() const { return walk.it; }
+};
+// Their tiles, one after the other.
+struct TileStream {
+  PartWalk part;
+  int jj;
+  __device__ __forceinline__ TileStream(const KvView& k, const ChunkIndex& x, int group,
+                                        const Smem& s)
+      : part(k, x, group, s), jj(part.k0) {}
+  __device__ __forceinline__ bool done() const { return !part.live; }
+  __device__ __forceinline__ void next() {
+    if (++jj < part.k1) return;
+    part.next();
+    jj = part.k0;
+  }
+  __device__ __forceinline__ const Item& it() const { return part.walk.it; }
+  __device__ __forceinline__ int valid() const { return min(BN, it().key_end() - jj * BN); }
+};
+
+// Eight 4-bit codes of a word as f16 values code * s + lo (one rounding: an f16 multiply-add).
 __device__ __forceinline__ uint4 q4_piece(uint32_t w, uint32_t params) {
   const uint32_t s2 = __byte_perm(params, params, 0x1010), l2 = __byte_perm(params, params, 0x3232);
   const __half2 s = *reinterpret_cast<const __half2*>(&s2);
   const __half2 lo = *reinterpret_cast<const __half2*>(&l2);
   const __half2 base = __floats2half2_rn(1024.f, 1024.f);
-  uint32_t r[4];
+  uint32_t r[4];  // values i and i + 4
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t c = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;  // 1024 + code
     const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s, lo);
     r[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
-  return make_uint4(r[0], r[1], r[2], r[3]);
+  return make_uint4(__byte_perm(r[0], r[1], 0x5410), __byte_perm(r[2], r[3], 0x5410),
+                    __byte_perm(r[0], r[1], 0x7632), __byte_perm(r[2], r[3], 0x7632));
 }
-// Position of dim d (0 .. 7) of a piece in that order.
-__device__ __forceinline__ constexpr int q4_place(int d) { return d < 4 ? 2 * d : 2 * d - 7; }
 
 template <int KVF>
 __global__ void __launch_bounds__(kThreads, 1)
-    attn_chunk_kernel(const __grid_constant__ CUtensorMap tm_k,
+    attn_chunk_kernel(const __grid_constant__ CUtensorMap tm_q,
+                      const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ ChunkArgs a) {
   extern __shared__ uint8_t smem_raw[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                      ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int group = a.hq / a.kv.hkv;
+  const int group = a.hq / a.kv.hkv, gshift = __ffs(group) - 1;
 
   // ---- this CTA's part of the list
   const int per = (a.at.nseq + 255) / 256;
@@ -196,8 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!sp.ok) {
         if (blockIdx.x == 0) atomicOr(a.err, kErrPosBeyondCache);
       } else if (sp.len > 0) {
-        mine += a.kv.hkv * (a.split ? seq_tiles(sp, group)
-                                    : static_cast<long long>(q_tiles(sp.len, group)));
+        mine += a.kv.hkv * units_before(sp.past, sp.len, group, q_tiles(sp.len, group));
       }
     }
     upto = mine;
@@ -209,20 +272,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 31) s.wsum[warp] = upto;
   }
   if (tid == 0) {
-    mbar_init(&s.q_full, kLoadWarps);
-    mbar_init(&s.q_free, 1);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.kv_full[i], KVF == kKvF16 ? 1 : kLoadWarps);
       mbar_init(&s.kv_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.q_full[i], 1);
+      mbar_init(&s.q_free[i], 1);
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.s_free[i], 4);
       mbar_init(&s.p_full[i], 4);
       mbar_init(&s.pv_done[i], 1);
       mbar_init(&s.o_free[i], 4);
     }
-    for (int i = 0; i < 8; ++i) s.bad[i] = 0;
+    for (int i = 0; i < kMarks; ++i) s.bad[i] = 0;
     s.abort_flag = 0;
     fence_barrier_init();
   }
@@ -235,31 +298,36 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int parts = int(min(static_cast<long long>(gridDim.x), total));
   const int b = blockIdx.x;
   launch_dependents();
-  if (a.split && tid == 0) a.joins[b] = make_int4(-1, 0, 0, 0);
+  if (tid == 0) a.joins[b] = make_int4(-1, 0, 0, 0);
   if (b >= parts) return;
-  const long long lo = a.split ? total * b / parts : b;
+  const long long lo = total * b / parts;
   if (tid < 256 && lo < upto && lo >= upto - mine) {
     long long at = upto - mine;
     for (int z = tid * per;; ++z) {
       const SeqSpan sp = seq_span(a.kv, a.at, z);
       if (!sp.ok || sp.len <= 0) continue;
       const int nq = q_tiles(sp.len, group);
-      bool found = false;
-      for (int qt = nq - 1; qt >= 0 && !found; --qt) {
-        const Item it{z, 0, qt, sp.past, sp.row0, sp.len, group};
-        const int nk = it.tiles(), unit = a.split ? nk : 1;
-        if (lo < at + static_cast<long long>(unit) * a.kv.hkv) {
-          const long long r = lo - at;
-          s.z0 = z;
-          s.qt0 = qt;
-          s.kh0 = int(r / unit);
-          s.k0 = a.split ? int(r % unit) : 0;
-          s.n_tiles = a.split ? int(total * (b + 1) / parts - lo) : nk;
-          found = true;
-        }
-        at += static_cast<long long>(unit) * a.kv.hkv;
+      const long long all = units_before(sp.past, sp.len, group, nq);
+      const long long r = lo - at;  // the sequence's query tiles come last one first
+      at += all * a.kv.hkv;
+      if (lo >= at) continue;
+      int first = 0, last = nq - 1;  // the tile qt with after(qt) <= r < after(qt - 1)
+      auto after = [&](int qt) {
+        return (all - units_before(sp.past, sp.len, group, qt + 1)) * a.kv.hkv;
+      };
+      while (first < last) {
+        const int mid = (first + last) / 2;
+        if (after(mid) <= r) last = mid;
+        else first = mid + 1;
       }
-      if (found) break;
+      const int unit = Item{z, 0, first, sp.past, sp.row0, sp.len, group}.tiles() + kSetup;
+      const long long in = r - after(first);
+      s.z0 = z;
+      s.qt0 = first;
+      s.kh0 = int(in / unit);
+      s.off0 = int(in % unit);
+      s.n_units = int(total * (b + 1) / parts - lo);
+      break;
     }
   }
   if (warp == kMmaWarp) tmem_alloc(&s.tmem_base, kTmemCols);
@@ -267,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
-  const int n_tiles = s.n_tiles;
+  const int n_units = s.n_units;
 
   if (warp >= 8) {
     regs_dec<kOtherRegs>();
@@ -275,13 +343,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------------------------------------------------------- MMA issuer
       constexpr uint32_t idesc_s = idesc_f16_f32(BM, BN, 0, 0);
       constexpr uint32_t idesc_pv = idesc_f16_f32(BM, D, 0, 1);
-      static_assert(sizeof(s.q[0]) == 16384 && sizeof(s.kv[0]) == 32768, "16 KB tiles");
-      const uint64_t qdesc0 = smem_desc_sw128(smem_u32(s.q[0]), 16, 1024);
+      static_assert(sizeof(s.q[0]) == 32768 && sizeof(s.kv[0]) == 32768, "16 KB tiles");
+      const uint64_t qdesc0 = smem_desc_sw128(smem_u32(s.q[0][0]), 16, 1024);
       const uint64_t kdesc0 = smem_desc_sw128(smem_u32(s.kv[0][0]), 16, 1024);
       const uint64_t vdesc0 = smem_desc_sw128(smem_u32(s.kv[0][1]), 0, 1024);
+      uint32_t seg = 0;  // parts so far
       auto issue_s = [&](int w, int st) {  // S_w = Q_w K_st^T
         if (elect_one()) {
-          const uint64_t qd = qdesc0 + uint64_t(w) * 1024, kd = kdesc0 + uint64_t(st) * 2048;
+          const uint64_t qd = qdesc0 + uint64_t((seg & 1) * 2 + w) * 1024,
+                         kd = kdesc0 + uint64_t(st) * 2048;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
             mma_f16_ss(tmem + col_s(w), qd + 2 * kk, kd + 2 * kk, idesc_s, kk > 0);
@@ -309,13 +379,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t ph = 0, ph1 = 0;            // their parities
       uint32_t n_s0 = 0, n_s1 = 0, n_pv0 = 0, n_pv1 = 0, n_o0 = 0, n_o1 = 0;  // per half: S, P.V,
       bool ok = true;                                                         // ended O
-      uint32_t seg = 0;
-      for (int left = n_tiles; ok && left > 0; ++seg) {
-        ok = wait_warp(&s.q_full, seg & 1);
+      while (ok) {
+        ok = wait_warp(&s.q_full[seg & 1], (seg >> 1) & 1);
         if (!ok) break;
         const int4 part = s.part[seg & 7];
         const int k1 = part.y, nk0 = part.z, nk1 = part.w;
-        left -= k1 - part.x;
+        if (k1 == 0) break;  // behind the last part
         // S of both halves for key tile jj in stage x, where they have rows that see it
         auto score = [&](int jj, int x) {
           if (jj < nk0) {
@@ -342,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = ok && score(jj + 1, st1);
             if (!ok) break;
           } else {
-            if (elect_one()) mma_commit(&s.q_free);
+            if (elect_one()) mma_commit(&s.q_free[seg & 1]);
             __syncwarp();
             const int tail = s.part_tail[seg & 7] - jj * BN;
             if (KVF == kKvF16 && tail < BN) {
@@ -380,131 +449,85 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (part.x < nk0) ++n_o0;
         if (part.x < nk1) ++n_o1;
+        ++seg;
       }
-    } else {
-      // ---------------------------------------------------------------- loading warps
-      const int lt = tid - kLoadWarp0 * 32;
-      const int w = lt & 7;  // 16-byte piece of a row (kLoaders is a multiple of 8)
-      constexpr int kTasks = (2 * BN * 8 + kLoaders - 1) / kLoaders;
+    } else if (warp == kTmaWarp) {
+      // ---------------------------------------------------------------- TMA producer
       const bool paged = a.kv.table != nullptr;
-      ItemWalk walk(a.kv, a.at, group, s.z0, s.qt0, s.kh0);
-      int c = 0, seg = 0;
+      const int mask = (1 << a.kv.shift) - 1;
+      PartWalk walk(a.kv, a.at, group, s);
+      int c = 0, n_q = 0;
       bool ok = true;
-      // int8 and 4-bit rows on their way to a tile: this thread's pieces, loaded together (all page
-      // numbers, then all words), one tile ahead
-      uint32_t raw[KVF == kKvF16 ? 1 : kTasks][2];
-      auto fetch = [&](const Item& it, int key0, int valid, int seg) {
-        if constexpr (KVF != kKvF16) {
-          // a tile has at most 8 pages: their numbers, a load per warp
-          int32_t pages = 0, off = 0;
-          if (paged) {
-            const int p = (key0 >> a.kv.shift) + lane;
-            if (lane <= ((valid - 1) + (key0 & ((1 << a.kv.shift) - 1))) >> a.kv.shift)
-              pages = a.kv.table[int64_t(it.z) * a.kv.max_blocks + p];
-            if (__any_sync(0xffffffffu, pages < 0 || int64_t(pages) >= a.kv.kv_rows)) {
-              if (lane == 0) {
-                s.bad[seg & 7] = 1;
-                atomicOr(a.err, kErrPosBeyondCache);
-              }
-              valid = 0;  // nothing of this tile is read
-            }
-          } else {
-            off = a.kv.offsets[it.z];
-          }
-          const int mask = (1 << a.kv.shift) - 1;
-#pragma unroll
-          for (int i = 0; i < kTasks; ++i) {
-            const int u = (i * kLoaders + lt) >> 3, key = u & (BN - 1);
-            int64_t row = int64_t(off) + key0 + key;
-            if (paged) {
-              const int32_t pg = __shfl_sync(0xffffffffu, pages,
-                                             ((key0 & mask) + key) >> a.kv.shift);
-              row = (int64_t(pg) << a.kv.shift) | ((key0 + key) & mask);
-            }
-            raw[i][0] = raw[i][1] = 0u;  // rows behind the last key: zeros
-            if (u < 2 * BN && key < valid) {
-              const unsigned char* src = (u >= BN ? a.kv.v : a.kv.k) + row * a.kv.row_bytes;
-              if (KVF == kKvQ4) {
-                const uint32_t* unit =
-                    reinterpret_cast<const uint32_t*>(src + it.kh * kQ4UnitBytes);
-                raw[i][0] = unit[w];
-                raw[i][1] = unit[8];
-              } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(src + it.kh * D + 8 * w);
-                raw[i][0] = x.x;
-                raw[i][1] = x.y;
-              }
-            }
-          }
+      if (lane == 0) {
+        prefetch_tensormap(&tm_q);
+        if (KVF == kKvF16) {
+          prefetch_tensormap(&tm_k);
+          prefetch_tensormap(&tm_v);
         }
-      };
-      float ksc[KVF == kKvI8 ? 8 : 1], vsc[KVF == kKvI8 ? 8 : 1];
-      if (KVF == kKvF16 && lt == 0) {
-        prefetch_tensormap(&tm_k);
-        prefetch_tensormap(&tm_v);
       }
-      for (int k0 = s.k0, left = n_tiles; ok && left > 0; k0 = 0, ++seg, walk.next()) {
-        const Item it = walk.it;
-        const int k1 = min(it.tiles(), k0 + left), key_end = it.key_end();
-        left -= k1 - k0;
-        if (KVF == kKvI8) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int ch = a.kv.per_channel ? it.kh * 64 + 8 * w + i : 0;
-            ksc[i] = a.kv.k_scale[ch];
-            vsc[i] = a.kv.v_scale[ch];
-          }
-        }
-        // Q: the 16-byte pieces of the item's rows, zeros behind them
-        if (seg > 0) {
-          ok = wait_bar(s, &s.q_free, (seg - 1) & 1, a.err);
-          ok = __all_sync(0xffffffffu, ok);
+      for (bool more = true; more; walk.next()) {
+        const Item it = walk.it();
+        const int seg = walk.seg, k0 = walk.k0, k1 = walk.k1, key_end = it.key_end();
+        more = walk.live;
+        // Q (and what the MMA warp has to know) once the products of two items before are done
+        if (seg > 1) {
+          if (lane == 0) ok = wait_bar(s, &s.q_free[seg & 1], ((seg >> 1) - 1) & 1, a.err);
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
           if (!ok) break;
         }
-        // The mark of four parts ahead is cleared: no loading warp is there yet (each part's Q
-        // waits for the products of the one before), and the part that used it last has ended
-        // (three parts back, before this one's Q could be asked for).
-        if (lt == 0) s.bad[(seg + 4) & 7] = 0;
-        const int rows = it.rows();
-        for (int i = lt; i < kRows * 8; i += kLoaders) {
-          const int r = i >> 3;
-          if (r >= BM && rows <= BM) break;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (r < rows)
-            x = *reinterpret_cast<const uint4*>(
-                a.q + (int64_t(it.row0) + it.tok0() + r / group) * a.ld_q +
-                (it.kh * group + r % group) * D + w * 8);
-          if (KVF == kKvQ4)
-            x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632),
-                           __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
-          *reinterpret_cast<uint4*>(reinterpret_cast<char*>(s.q[r / BM]) + (r % BM) * 128 +
-                                    ((w ^ (r & 7)) << 4)) = x;
+        if (!more) {  // tells the MMA warp that the part before was the last
+          if (lane == 0) {
+            s.part[seg & 7] = make_int4(0, 0, 0, 0);
+            mbar_arrive(&s.q_full[seg & 1]);
+          }
+          break;
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lt == 0) {
+        if (lane == 0) {
+          // The mark of eight parts ahead is cleared.  Nobody sets it yet: the MMA warp is at this
+          // part at most, the converting warps are up to kStages tiles ahead of it and their loads
+          // two more.  The part that used it last is eight back, and ended long ago.
+          s.bad[(seg + kMarks / 2) % kMarks] = 0;
           s.part[seg & 7] = make_int4(k0, k1, it.tiles_of(0), it.tiles_of(1));
           s.part_tail[seg & 7] = key_end;
+          const int halves = it.rows() > BM ? 2 : 1;
+          mbar_arrive_expect_tx(&s.q_full[seg & 1], uint32_t(halves * BM * D * 2));
+          for (int h = 0; h < halves; ++h)
+            tma_load_3d(s.q[seg & 1][h], &tm_q, 0, it.kh * group,
+                        it.row0 + it.tok0() + h * (BM >> gshift), &s.q_full[seg & 1]);
         }
-        if (lane == 0) mbar_arrive(&s.q_full);
-
-        for (int jj = k0; ok && jj < k1; ++jj, ++c) {
-          const int st = c % kStages, key0 = jj * BN, valid = min(BN, key_end - key0);
-          if constexpr (KVF == kKvF16) {
-            if (warp != kLoadWarp0) continue;
-            // one box per page (or one of 128 rows)
-            const int box = paged ? min(1 << a.kv.shift, BN) : BN;
-            const int boxes = (valid + box - 1) / box;
-            int64_t row = 0;
-            if (lane < boxes) row = kv_row(a.kv, it.z, key0 + lane * box);
-            const bool bad = __any_sync(0xffffffffu, row < 0);
+        n_q = seg + 1;
+        if constexpr (KVF == kKvF16) {
+          int32_t pages = 0;
+          const int off = paged ? 0 : a.kv.offsets[it.z];
+          for (int jj = k0; jj < k1; ++jj, ++c) {
+            const int st = c % kStages, key0 = jj * BN, valid = min(BN, key_end - key0);
             if (lane == 0 && c >= kStages)
               ok = wait_bar(s, &s.kv_empty[st], (c / kStages - 1) & 1, a.err);
             ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
             if (!ok) break;
+            // one box per page (or one of 128 rows)
+            const int box = paged ? min(1 << a.kv.shift, BN) : BN;
+            const int boxes = (valid + box - 1) / box;
+            int64_t row = int64_t(off) + key0;
+            if (paged) {
+              const int in = (jj - k0) & 3;  // the pages of four tiles at a time, at most 32
+              if (in == 0) {
+                pages = 0;
+                const int p = (key0 >> a.kv.shift) + lane;
+                if (p <= (key_end - 1) >> a.kv.shift)
+                  pages = a.kv.table[int64_t(it.z) * a.kv.max_blocks + p];
+              }
+              const int at = key0 + min(lane, boxes - 1) * box;
+              const int32_t pg = __shfl_sync(
+                  0xffffffffu, pages, (at >> a.kv.shift) - ((key0 - in * BN) >> a.kv.shift));
+              row = pg < 0 || int64_t(pg) >= a.kv.kv_rows
+                        ? -1
+                        : (int64_t(pg) << a.kv.shift) | (at & mask);
+            }
+            const bool bad = __any_sync(0xffffffffu, row < 0);
             if (lane == 0) {
               if (bad) {
-                s.bad[seg & 7] = 1;
+                s.bad[seg % kMarks] = 1;
                 atomicOr(a.err, kErrPosBeyondCache);
               }
               mbar_arrive_expect_tx(&s.kv_full[st],
@@ -518,49 +541,145 @@ __global__ void __launch_bounds__(kThreads, 1)
               tma_load_2d(&s.kv[st][1][lane * box * D], &tm_v, it.kh * D, int32_t(row),
                           &s.kv_full[st]);
             }
-          } else {
-            if (jj == k0) fetch(it, key0, valid, seg);  // else on its way since the tile before
-            if (c >= kStages) ok = wait_bar(s, &s.kv_empty[st], (c / kStages - 1) & 1, a.err);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-#pragma unroll
-            for (int i = 0; i < kTasks; ++i) {
-              const int u = (i * kLoaders + lt) >> 3, key = u & (BN - 1);
-              if (u >= 2 * BN) continue;
-              uint4 x;
-              if constexpr (KVF == kKvQ4) {
-                x = q4_piece(raw[i][0], raw[i][1]);
-              } else {
-                float f[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                  f[k] = float(static_cast<int8_t>(raw[i][k >> 2] >> (8 * (k & 3)))) *
-                         (u >= BN ? vsc[k] : ksc[k]);
-                x = make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]),
-                               pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
-              }
-              *reinterpret_cast<uint4*>(reinterpret_cast<char*>(s.kv[st][u >= BN ? 1 : 0]) +
-                                        key * 128 + ((w ^ (key & 7)) << 4)) = x;
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (c == 0 && lt == 0 && a.wait_deficit)
-                mbar_arrive_expect_tx(&s.kv_full[st], uint32_t(a.wait_deficit));
-              else
-                mbar_arrive(&s.kv_full[st]);
-            }
-            if (jj + 1 < k1) fetch(it, key0 + BN, min(BN, key_end - key0 - BN), seg);
           }
         }
+        if (!ok) break;
       }
-      if (KVF == kKvF16 && warp == kLoadWarp0 && s.abort_flag) {
-        // let the copies already in flight land before the CTA exits
-        for (int i = max(0, c - kStages); i < c; ++i) {
-          const uint64_t t0 = globaltimer_ns();
+      // after a wait that ran out: let the copies already in flight land before the CTA exits
+      if (lane == 0 && s.abort_flag) {
+        const uint64_t t0 = globaltimer_ns();
+        for (int i = max(0, n_q - 2); i < n_q; ++i)
+          while (!mbar_try_wait(&s.q_full[i & 1], (i >> 1) & 1) &&
+                 globaltimer_ns() - t0 < kWaitLimitNs) {
+          }
+        for (int i = max(0, c - kStages); i < c; ++i)
           while (!mbar_try_wait(&s.kv_full[i % kStages], (i / kStages) & 1) &&
                  globaltimer_ns() - t0 < kWaitLimitNs) {
           }
+      }
+    } else if (KVF != kKvF16 && warp >= kLoadWarp0) {
+      // ---------------------------------------------------------------- converting warps
+      constexpr int kWords = KVF == kKvQ4 ? 9 : 16;  // of a head's row
+      const int key = tid - kLoadWarp0 * 32;
+      const bool paged = a.kv.table != nullptr;
+      // Three tiles in a line: `now` is converted, the words of `words` are on their way, and the
+      // page number of `ahead`.
+      TileStream ahead(a.kv, a.at, group, s);
+      int32_t page = 0;
+      auto find = [&] {
+        if (ahead.done()) return;
+        page = 0;
+        if (!paged) page = a.kv.offsets[ahead.it().z];
+        else if (key < ahead.valid())
+          page = a.kv.table[int64_t(ahead.it().z) * a.kv.max_blocks +
+                            ((ahead.jj * BN + key) >> a.kv.shift)];
+      };
+      uint32_t raw[2][kWords];
+      int64_t at = 0;        // byte offset of the head's row in either pool
+      bool there = false;    // the key exists
+      int kh = 0;
+      auto place = [&] {  // takes `ahead` over as the tile whose words are loaded
+        if (ahead.done()) return;
+        const int pos = ahead.jj * BN + key;
+        kh = ahead.it().kh;
+        there = key < ahead.valid();
+        int64_t row = int64_t(page) + pos;
+        if (paged) {
+          if (there && (page < 0 || int64_t(page) >= a.kv.kv_rows)) {
+            there = false;  // a page outside the pool is not read
+            s.bad[ahead.part.seg % kMarks] = 1;
+            atomicOr(a.err, kErrPosBeyondCache);
+          }
+          row = (int64_t(page) << a.kv.shift) | (pos & ((1 << a.kv.shift) - 1));
+        }
+        at = row * a.kv.row_bytes + kh * (KVF == kKvQ4 ? kQ4UnitBytes : D);
+        ahead.next();
+        find();
+      };
+      auto load = [&](int pool) {
+        const unsigned char* src = (pool ? a.kv.v : a.kv.k) + at;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) raw[pool][i] = 0u;  // rows behind the last key: zeros
+        if (!there) return;
+        if constexpr (KVF == kKvQ4) {
+#pragma unroll
+          for (int i = 0; i < kWords; ++i)
+            raw[pool][i] = reinterpret_cast<const uint32_t*>(src)[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < kWords; i += 4) {
+            const uint4 x = reinterpret_cast<const uint4*>(src)[i / 4];
+            raw[pool][i] = x.x;
+            raw[pool][i + 1] = x.y;
+            raw[pool][i + 2] = x.z;
+            raw[pool][i + 3] = x.w;
+          }
+        }
+      };
+      auto convert = [&](int st, int pool, int head) {
+        char* dst = reinterpret_cast<char*>(s.kv[st][pool]) + key * 128;
+        const float4* scale = reinterpret_cast<const float4*>(
+            (pool ? a.kv.v_scale : a.kv.k_scale) + (a.kv.per_channel ? head * D : 0));
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          uint4 x;
+          if constexpr (KVF == kKvQ4) {
+            x = q4_piece(raw[pool][w], raw[pool][8]);
+          } else {
+            float sc[8];
+            if (a.kv.per_channel && (reinterpret_cast<uintptr_t>(scale) & 15u) != 0) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) sc[k] = reinterpret_cast<const float*>(scale)[8 * w + k];
+            } else if (a.kv.per_channel) {
+              const float4 a4 = scale[2 * w], b4 = scale[2 * w + 1];
+              sc[0] = a4.x, sc[1] = a4.y, sc[2] = a4.z, sc[3] = a4.w;
+              sc[4] = b4.x, sc[5] = b4.y, sc[6] = b4.z, sc[7] = b4.w;
+            } else {
+              const float one = *reinterpret_cast<const float*>(scale);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) sc[k] = one;
+            }
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              f[k] = float(static_cast<int8_t>(raw[pool][2 * w + (k >> 2)] >> (8 * (k & 3)))) *
+                     sc[k];
+            x = make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]),
+                           pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
+          }
+          *reinterpret_cast<uint4*>(dst + ((w ^ (key & 7)) << 4)) = x;
+        }
+      };
+      find();
+      bool more = !ahead.done();
+      place();
+      load(0);
+      load(1);
+      int head = kh, st = 0;
+      uint32_t ph = 1;
+      for (int c = 0; more; ++c) {
+        bool ok = true;
+        if (lane == 0 && c >= kStages) ok = wait_bar(s, &s.kv_empty[st], ph, a.err);
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok) break;
+        more = !ahead.done();
+        if (more) place();
+        convert(st, 0, head);
+        if (more) load(0);
+        convert(st, 1, head);
+        if (more) load(1);
+        head = kh;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (c == 0 && key == 0 && a.wait_deficit)
+            mbar_arrive_expect_tx(&s.kv_full[st], uint32_t(a.wait_deficit));
+          else
+            mbar_arrive(&s.kv_full[st]);
+        }
+        if (++st == kStages) {
+          st = 0;
+          ph ^= 1;
         }
       }
     }
@@ -571,13 +690,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = tid & 127;  // row of the half = TMEM lane
     const uint32_t lane_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
     const float sl2 = a.scale_log2;
-    ItemWalk walk(a.kv, a.at, group, s.z0, s.qt0, s.kh0);
-    int n = 0, seg = 0;  // tiles of this half, parts
+    PartWalk walk(a.kv, a.at, group, s);
+    int n = 0;  // tiles of this half
     bool ok = true;
-    for (int k0 = s.k0, left = n_tiles; ok && left > 0; k0 = 0, ++seg, walk.next()) {
-      const Item it = walk.it;
-      const int nk = it.tiles(), k1 = min(nk, k0 + left);
-      left -= k1 - k0;
+    for (; walk.live; walk.next()) {
+      const Item it = walk.it();
+      const int seg = walk.seg, nk = walk.nk, k0 = walk.k0, k1 = walk.k1;
       const int rows = it.rows_of(w), mine_end = min(k1, it.tiles_of(w));
       if (rows == 0) continue;
       const int first_lim = it.past + it.tok0() + BM * w / group + 1;  // keys the first row sees
@@ -691,21 +809,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) ov[0][i] = ov[1][i] = 0u;
       }
-      if (KVF == kKvQ4) {  // the dims back in their order
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int g = 0; g < 32; g += 8) {
-            uint32_t t[8];
-#pragma unroll
-            for (int d = 0; d < 8; ++d) t[d] = ov[h][g + q4_place(d)];
-#pragma unroll
-            for (int d = 0; d < 8; ++d) ov[h][g + d] = t[d];
-          }
-      }
-      const bool bad = s.bad[seg & 7] != 0;
+      const bool bad = s.bad[seg % kMarks] != 0;
       if (!whole && tid == 0 && k0 == 0) {  // the item begins here: what there is to join
-        const long long end = lo + (n_tiles - left) + (nk - k1);  // list position behind the item
+        // list position behind the item
+        const long long end = lo + (n_units - walk.left) - walk.off + kSetup + nk;
         const int last = int((end * parts - 1) / total);
         a.joins[b] = make_int4(it.z, it.kh, it.qt, ((last - b + 1) << 1) | (seg == 0 ? 0 : 1));
       }
@@ -742,14 +849,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     // a wait ran out: a part that others join is marked, the rest stays as it was
-    if (!ok && a.split) {
-      ItemWalk again(a.kv, a.at, group, s.z0, s.qt0, s.kh0);
-      int i = 0;
-      for (int k0 = s.k0, left = n_tiles; left > 0; k0 = 0, ++i, again.next()) {
-        const Item it = again.it;
-        const int nk = it.tiles(), k1 = min(nk, k0 + left);
-        left -= k1 - k0;
-        if (i < seg || (k0 == 0 && k1 == nk) || r >= it.rows_of(w)) continue;
+    if (!ok) {
+      PartWalk again(a.kv, a.at, group, s);
+      for (; again.live; again.next()) {
+        const int i = again.seg;
+        if (i < walk.seg || (again.k0 == 0 && again.k1 == again.nk) ||
+            r >= again.it().rows_of(w))
+          continue;
         float* rec = a.parts + ((int64_t(b) * 2 + (i == 0 ? 0 : 1)) * kRows + BM * w + r) * kRec;
         rec[64] = -1e30f;
         rec[65] = -1.f;
@@ -845,6 +951,20 @@ bool make_map(CUtensorMap* m, const void* base, int64_t width, int64_t rows, int
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// q rows as [rows][hq][64] (row pitch ld), boxes of a group's heads of 128 / group rows.
+bool make_q_map(CUtensorMap* m, const void* q, int hq, int64_t rows, int64_t ld, int group) {
+  auto enc = get_encode();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {64, cuuint64_t(hq), cuuint64_t(rows)};
+  cuuint64_t strides[2] = {128, cuuint64_t(ld) * 2};
+  cuuint32_t box[3] = {64, cuuint32_t(group), cuuint32_t(BM / group)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace
 
 size_t chunk_parts_bytes(int num_sms) {
@@ -854,7 +974,9 @@ size_t chunk_join_bytes(int num_sms) { return size_t(num_sms) * sizeof(int4); }
 
 cudaError_t launch_attn_chunk(const ChunkArgs& args, int num_sms, cudaStream_t s) {
   ChunkArgs a = args;
-  CUtensorMap tk{}, tv{};
+  const int group = a.hq / a.kv.hkv;
+  CUtensorMap tq{}, tk{}, tv{};
+  if (!make_q_map(&tq, a.q, a.hq, a.at.n_rows, a.ld_q, group)) return cudaErrorInvalidValue;
   if (a.kv.format == kKvF16) {
     const int64_t rows = a.kv.kv_rows << a.kv.shift;  // shift 0 when contiguous
     const int box = a.kv.table && (1 << a.kv.shift) < BN ? 1 << a.kv.shift : BN;
@@ -863,12 +985,6 @@ cudaError_t launch_attn_chunk(const ChunkArgs& args, int num_sms, cudaStream_t s
         !make_map(&tv, a.kv.v, int64_t(a.kv.hkv) * D, rows, box))
       return cudaErrorInvalidValue;
   }
-  const int group = a.hq / a.kv.hkv;
-  // the items this call can have: every sequence may end in a part of one
-  const int64_t items = (a.at.n_rows * group / kRows + a.at.nseq) * a.kv.hkv;
-  a.split = items <= int64_t(kMaxItemsPerSm) * num_sms;
-  const int64_t ctas = a.split ? num_sms : items;
-  if (ctas > INT32_MAX) return cudaErrorInvalidValue;
   const void* fn = a.kv.format == kKvF16  ? reinterpret_cast<const void*>(&attn_chunk_kernel<kKvF16>)
                    : a.kv.format == kKvI8 ? reinterpret_cast<const void*>(&attn_chunk_kernel<kKvI8>)
                                           : reinterpret_cast<const void*>(&attn_chunk_kernel<kKvQ4>);
@@ -884,10 +1000,10 @@ cudaError_t launch_attn_chunk(const ChunkArgs& args, int num_sms, cudaStream_t s
     return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (e != cudaSuccess) return e;
-  void* argv[] = {&tk, &tv, &a};
+  void* argv[] = {&tq, &tk, &tv, &a};
   cudaError_t le =
-      cudaLaunchKernel(fn, dim3(unsigned(ctas)), dim3(kThreads), argv, size_t(smem), s);
-  if (le != cudaSuccess || !a.split) return le;
+      cudaLaunchKernel(fn, dim3(unsigned(num_sms)), dim3(kThreads), argv, size_t(smem), s);
+  if (le != cudaSuccess) return le;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(num_sms), kRows / 32);
   cfg.blockDim = dim3(kJoinThreads);

@@ -323,7 +323,6 @@ struct ChunkArgs : AttnKvArgs {
   float* parts;  // chunk_parts_bytes(): records of items that straddle CTAs
   int4* joins;   // chunk_join_bytes(): per CTA the item to join, if any
   int32_t wait_deficit;
-  int32_t split;  // set by the launcher: tiles cut into equal parts, else one CTA per item
 };
 size_t chunk_parts_bytes(int num_sms);
 size_t chunk_join_bytes(int num_sms);
