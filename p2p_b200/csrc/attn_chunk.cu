@@ -45,7 +45,7 @@ constexpr int kRows = 2 * BM;  // rows of an item
 constexpr int kThreads = 512;
 constexpr int kMmaWarp = 8, kTmaWarp = 9, kLoadWarp0 = 12, kLoadWarps = 4;
 constexpr int kMarks = 16;
-constexpr int kSetup = 1;
+constexpr int kSetup = 2;
 // setmaxnreg splits the 512 x 128 registers of the launch: 256 x 176 + 256 x 80
 constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kOtherRegs = 80;
 static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
