@@ -9,8 +9,11 @@
 // ones are read once per row: each CTA takes a part and counts every token straight into the owning
 // CTA's shared memory (distributed shared memory).  Counts are whole numbers, so the order of the
 // atomics does not matter.
-//   Biased tokens are few: the streaming pass leaves them out, and a thread per token then does
-// the whole computation with the token's biases in the order of the list.
+//   The touched tokens -- penalised or biased -- are few.  Threads take one each, compute its value in
+// f32 and leave it in the token's count word, with a bit in a map of the slice; the streaming pass
+// looks at the map and otherwise only masks, stores and compares.  (With the penalties in the
+// streaming pass nearly every warp ran their divisions for one lane or another: 74 instructions per
+// token.)
 // The CTAs' best tokens meet in the first CTA's shared memory, one slot each (a 64-bit maximum on
 // distributed shared memory from several CTAs at once lost values).
 #include <cooperative_groups.h>
@@ -26,13 +29,12 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512;
 constexpr int kMaxCluster = 8;
 constexpr int kLocalHist = 4096;
-constexpr int kMaxBiases = 512;            // of a slice, for the pass of their own
+constexpr int kMaxBiases = 512;            // of a slice, gathered in shared memory
 constexpr uint32_t kSeen = 0x80000000u;    // in the prompt (or generated: the count says so)
-constexpr uint32_t kBiased = 0x40000000u;  // some bias entry names the token
-constexpr uint32_t kCount = 0x3fffffffu;   // times generated
+constexpr uint32_t kCount = 0x7fffffffu;   // times generated
 constexpr int kAhead = 4;                  // pieces of logits loaded before the history is read
 
-// Larger value first, then smaller index; 0 is no token.  -0 and +0 are the same value.
+// Larger value first, then smaller index; 0 is no token (y = -inf).  -0 and +0 are the same value.
 __device__ __forceinline__ unsigned long long pick_key(float y, uint32_t v) {
   if (!(y > -INFINITY)) return 0ull;
   uint32_t b = __float_as_uint(y + 0.0f);
@@ -66,40 +68,22 @@ struct Piece {  // 16 bytes of logits
   }
 };
 
-struct Penalty {
-  float rep, pres, freq;
-  bool has_rep;
-  __device__ __forceinline__ float apply(float x, uint32_t c) const {
-    if (has_rep) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-    if (c & kCount) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, float(c & kCount))), pres);
-    return x;
-  }
-};
-
-// Words in front of the counts of CTA `rank` of row i (its `pad`, see the kernel): slices are whole
-// pieces apart, so all CTAs of a row have the same unless theirs ends before the boundary.
-template <class T>
-__device__ __forceinline__ int pad_of(const LogitsArgs& a, int i, int rank, int slice) {
-  constexpr int kN = Piece<T>::kN;
-  const uintptr_t p =
-      reinterpret_cast<uintptr_t>(static_cast<const T*>(a.logits) + int64_t(i) * a.ld);
-  const int n = min(slice, a.vocab - rank * slice);
-  const int lead = min(n, int((16u - uint32_t(p & 15u)) & 15u) / int(sizeof(T)));
-  return (kN - lead) % kN;
-}
-
-// cnt[] holds the slice's counts behind `pad` words, so that the counts of a 16-byte piece of
-// logits start on 16 bytes whatever the row's alignment.
 template <class T>
 __global__ void __launch_bounds__(kThreads)
     logits_pick_kernel(const __grid_constant__ LogitsArgs a, int slice) {
   constexpr int kN = Piece<T>::kN;
-  extern __shared__ __align__(16) uint32_t cnt[];  // [slice + kN]
-  __shared__ unsigned long long warp_best[kThreads / 32];
+  // per token of the slice a count, later the value of a touched token; the map of touched tokens;
+  // the counted tokens (short histories)
+  extern __shared__ __align__(16) uint32_t cnt[];
+  uint32_t* map = cnt + slice;
+  uint16_t* list = reinterpret_cast<uint16_t*>(map + slice / 32);
+  __shared__ float warp_y[kThreads / 32];
+  __shared__ uint32_t warp_v[kThreads / 32];
   __shared__ unsigned long long cta_best[kMaxCluster];  // rank 0's: one slot per CTA
   __shared__ int bias_tok[kMaxBiases];
-  __shared__ float bias_val[kMaxBiases], bias_x[kMaxBiases];
+  __shared__ float bias_val[kMaxBiases];
   __shared__ int warp_n[kThreads / 32];
+  __shared__ int n_list;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = int(cl.block_rank()), csize = int(cl.num_blocks());
   const int i = blockIdx.x / csize, t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -109,16 +93,13 @@ __global__ void __launch_bounds__(kThreads)
   // tokens in front of the first 16-byte boundary; whole pieces behind it
   const int lead =
       min(n, int((16u - uint32_t(reinterpret_cast<uintptr_t>(src) & 15u)) & 15u) / int(sizeof(T)));
-  const int pad = (kN - lead) % kN, pieces = (n - lead) / kN;
+  const int pieces = (n - lead) / kN;
   const uint4* body = reinterpret_cast<const uint4*>(src + lead);
   Piece<T> ahead[kAhead];
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)
     if (t + k * kThreads < pieces) ahead[k].w = body[t + k * kThreads];
 
-  const bool remote = a.hist != nullptr && a.hist_cap > kLocalHist;
-  for (int k = t; k < (slice + kN) / 4; k += kThreads)
-    reinterpret_cast<uint4*>(cnt)[k] = make_uint4(0, 0, 0, 0);
   int len = 0, prompt = 0, e0 = 0, e1 = 0;
   if (a.hist != nullptr) {
     len = min(max(a.hist_len[i], 0), a.hist_cap);
@@ -128,121 +109,130 @@ __global__ void __launch_bounds__(kThreads)
     e0 = min(max(a.bias_start[i], 0), a.n_bias);
     e1 = min(max(a.bias_start[i + 1], e0), a.n_bias);
   }
-  Penalty pen;
-  pen.has_rep = a.repetition != nullptr;
-  pen.rep = a.repetition ? a.repetition[i] : 1.f;
-  pen.pres = a.presence ? a.presence[i] : 0.f;
-  pen.freq = a.frequency ? a.frequency[i] : 0.f;
-  const int32_t* hist = a.hist + int64_t(i) * a.ld_hist;
-  if (remote) cl.sync();
-  else __syncthreads();
-  if (remote) {
-    for (int k = rank * kThreads + t; k < len; k += csize * kThreads) {
-      const int v = hist[k];
-      if (v < 0 || v >= a.vocab) continue;
-      uint32_t* c = cl.map_shared_rank(cnt, v / slice) + pad_of<T>(a, i, v / slice, slice) +
-                    v % slice;
-      if (k >= prompt) atomicAdd(c, 1u);
-      else atomicOr(c, kSeen);
-    }
-  } else {
-#pragma unroll 4
-    for (int k = t; k < len; k += kThreads) {
-      const int v = hist[k] - v0;
-      if (v < 0 || v >= n) continue;
-      if (k >= prompt) atomicAdd(&cnt[pad + v], 1u);
-      else atomicOr(&cnt[pad + v], kSeen);
-    }
-  }
-  // the slice's biases, in the order of the list
-  int n_bias = 0;
-  bool scan = false;  // too many of them: the streaming pass looks each biased token up
-  for (int k0 = e0; k0 < e1; k0 += kThreads) {
-    const int k = k0 + t;
-    const int v = k < e1 ? a.bias_tok[k] - v0 : -1;
-    const bool mine = v >= 0 && v < n;
-    const uint32_t votes = __ballot_sync(0xffffffffu, mine);
-    if (lane == 0) warp_n[warp] = __popc(votes);
-    __syncthreads();
-    int at = n_bias + __popc(votes & ((1u << lane) - 1u));
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) at += warp_n[w];
-      n_bias += warp_n[w];
-    }
-    if (mine && at < kMaxBiases) {
-      bias_tok[at] = v;
-      bias_val[at] = a.bias_val[k];
-      bias_x[at] = to_f32(src[v]);  // before the streaming pass may store over it
-    }
-    __syncthreads();
-  }
-  scan = n_bias > kMaxBiases;
-  if (remote) cl.sync();
-  else __syncthreads();
-  if (n_bias > 0) {  // the counts are complete
-    if (scan) {
-      for (int k = e0 + t; k < e1; k += kThreads) {
-        const int v = a.bias_tok[k] - v0;
-        if (v >= 0 && v < n) atomicOr(&cnt[pad + v], kBiased);
+  const bool touched = a.hist != nullptr || a.bias_start != nullptr;
+  if (touched) {
+    const bool remote = a.hist_cap > kLocalHist;
+    const bool has_rep = a.repetition != nullptr;
+    const float rep = has_rep ? a.repetition[i] : 1.f;
+    const float pres = a.presence ? a.presence[i] : 0.f;
+    const float freq = a.frequency ? a.frequency[i] : 0.f;
+    for (int k = t; k < (slice + slice / 32) / 4; k += kThreads)
+      reinterpret_cast<uint4*>(cnt)[k] = make_uint4(0, 0, 0, 0);
+    if (t == 0) n_list = 0;
+    if (remote) cl.sync();
+    else __syncthreads();
+    const int32_t* hist = a.hist + int64_t(i) * a.ld_hist;
+    if (remote) {
+      for (int k = rank * kThreads + t; k < len; k += csize * kThreads) {
+        const int v = hist[k];
+        if (v < 0 || v >= a.vocab) continue;
+        uint32_t* c = cl.map_shared_rank(cnt, v / slice) + v % slice;
+        if (k >= prompt) atomicAdd(c, 1u);
+        else atomicOr(c, kSeen);
       }
+      cl.sync();
     } else {
-      for (int k = t; k < n_bias; k += kThreads) atomicOr(&cnt[pad + bias_tok[k]], kBiased);
+#pragma unroll 4
+      for (int k = t; k < len; k += kThreads) {
+        const int v = hist[k] - v0;
+        if (v < 0 || v >= n) continue;
+        const uint32_t old = k >= prompt ? atomicAdd(&cnt[v], 1u) : atomicOr(&cnt[v], kSeen);
+        if (old == 0u) list[atomicAdd(&n_list, 1)] = uint16_t(v);  // the first to touch it
+      }
+      __syncthreads();
+    }
+    auto penalise = [&](int v) {
+      const uint32_t c = cnt[v];
+      float x = to_f32(src[v]);
+      if (has_rep) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+      if (c & kCount) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, float(c & kCount))), pres);
+      cnt[v] = __float_as_uint(x);
+      atomicOr(&map[v >> 5], 1u << (v & 31));
+    };
+    if (remote) {
+      for (int v = t; v < n; v += kThreads)
+        if (cnt[v] != 0u) penalise(v);
+    } else {
+      for (int k = t; k < n_list; k += kThreads) penalise(list[k]);
+    }
+    // the slice's biases, in the order of the list, kMaxBiases at a time
+    for (int k0 = e0; k0 < e1; k0 += kThreads) {
+      static_assert(kMaxBiases == kThreads, "a round's entries fit");
+      const int k = k0 + t;
+      const int v = k < e1 ? a.bias_tok[k] - v0 : -1;
+      const bool mine = v >= 0 && v < n;
+      const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+      if (lane == 0) warp_n[warp] = __popc(votes);
+      __syncthreads();  // also: the penalties, or the round before, are in place
+      int at = __popc(votes & ((1u << lane) - 1u)), all = 0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) at += warp_n[w];
+        all += warp_n[w];
+      }
+      if (mine) {
+        bias_tok[at] = v;
+        bias_val[at] = a.bias_val[k];
+      }
+      __syncthreads();
+      if (t < all) {  // a token's first entry adds all of them, in order
+        const int u = bias_tok[t];
+        bool first = true;
+        for (int j = 0; j < t; ++j) first = first && bias_tok[j] != u;
+        if (first) {
+          const bool known = (map[u >> 5] >> (u & 31)) & 1u;
+          float x = known ? __uint_as_float(cnt[u]) : to_f32(src[u]);
+          for (int j = t; j < all; ++j)
+            if (bias_tok[j] == u) x = __fadd_rn(x, bias_val[j]);
+          cnt[u] = __float_as_uint(x);
+          atomicOr(&map[u >> 5], 1u << (u & 31));
+        }
+      }
+      __syncthreads();
     }
     __syncthreads();
   }
-  const uint32_t* mask = a.mask ? a.mask + int64_t(i) * a.ld_mask : nullptr;
-  unsigned long long best = 0ull;
-  // the stored value of token v of the slice; biased ones are done later unless `scan`
-  auto process = [&](float x, uint32_t c, int v, bool allowed) {
-    if (c) {
-      if (c & ~kBiased) x = pen.apply(x, c);
-      if (scan && (c & kBiased)) {
-        for (int k = e0; k < e1; ++k)
-          if (a.bias_tok[k] == v0 + v) x = __fadd_rn(x, a.bias_val[k]);
-      }
-    }
-    return to_f32(from_f32<T>(allowed ? x : -INFINITY));
-  };
-  auto consider = [&](float y, uint32_t c, int v) {
-    if ((c & kBiased) && !scan) return;
-    const unsigned long long key = pick_key(y, uint32_t(v0 + v));
-    if (key > best) best = key;
-  };
-  auto allowed_bits = [&](int v) {  // of tokens v .. of the slice, at least kN of them
-    if (mask == nullptr) return 0xffffffffu;
-    const int g = v0 + v, w = g >> 5, sh = g & 31;
-    uint32_t bits = mask[w] >> sh;
-    if (sh + kN > 32 && (w + 1) * 32 < a.vocab) bits |= mask[w + 1] << (32 - sh);
+  const uint32_t* mask = a.mask ? a.mask + int64_t(i) * a.ld_mask + v0 / 32 : nullptr;
+  // bits of the kN tokens from v on, out of a word a 32 tokens (v0 is a multiple of 32)
+  auto bits_of = [&](const uint32_t* words, int v) {
+    const int w = v >> 5, sh = v & 31;
+    uint32_t bits = words[w] >> sh;
+    if (sh + kN > 32 && (w + 1) * 32 < n) bits |= words[w + 1] << (32 - sh);
     return bits;
   };
+  float best = -INFINITY;  // NaN and -inf never win
+  uint32_t best_v = 0xffffffffu;
   const bool wide_out = dst != nullptr && (reinterpret_cast<uintptr_t>(dst + lead) & 15u) == 0;
-  auto piece = [&](const Piece<T>& in, int k) {
+  auto piece = [&](Piece<T> in, int k) {
     const int v = lead + k * kN;
-    uint32_t c[kN];
+    float y[kN];
 #pragma unroll
-    for (int j = 0; j < kN; j += 4) {
-      const uint4 q = *reinterpret_cast<const uint4*>(&cnt[pad + v + j]);
-      c[j] = q.x, c[j + 1] = q.y, c[j + 2] = q.z, c[j + 3] = q.w;
+    for (int j = 0; j < kN; ++j) y[j] = in.get(j);
+    const uint32_t hit = touched ? bits_of(map, v) & ((1u << kN) - 1u) : 0u;
+    if (hit) {
+#pragma unroll
+      for (int j = 0; j < kN; ++j)
+        if ((hit >> j) & 1u) y[j] = round_st<T>(__uint_as_float(cnt[v + j]));
     }
-    const uint32_t bits = allowed_bits(v);
-    float y[kN], top = -INFINITY;
+    if (mask != nullptr) {
+      const uint32_t bits = bits_of(mask, v);
 #pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      y[j] = process(in.get(j), c[j], v + j, (bits >> j) & 1u);
-      if (!(c[j] & kBiased) || scan) top = fmaxf(top, y[j]);
+      for (int j = 0; j < kN; ++j)
+        if (!((bits >> j) & 1u)) y[j] = -INFINITY;
     }
-    // a piece whose best does not beat the thread's changes nothing (NaN never wins; an equal value
-    // of a later token neither)
-    if (pick_key(top, 0u) > best) {
+    float top = y[0];
 #pragma unroll
-      for (int j = 0; j < kN; ++j) consider(y[j], c[j], v + j);
+    for (int j = 1; j < kN; ++j) top = fmaxf(top, y[j]);
+    if (top > best) {  // a thread's pieces come in the order of their tokens
+      best = top;
+#pragma unroll
+      for (int j = kN - 1; j >= 0; --j)
+        if (y[j] == top) best_v = uint32_t(v0 + v + j);
     }
     if (dst != nullptr) {
       if (wide_out) {
-        Piece<T> o;
-        o.set(y);
-        *reinterpret_cast<uint4*>(dst + v) = o.w;
+        in.set(y);
+        *reinterpret_cast<uint4*>(dst + v) = in.w;
       } else {
 #pragma unroll
         for (int j = 0; j < kN; ++j) dst[v + j] = from_f32<T>(y[j]);
@@ -264,42 +254,37 @@ __global__ void __launch_bounds__(kThreads)
   const int tail = lead + pieces * kN;
   for (int k = t; k < lead + (n - tail); k += kThreads) {
     const int v = k < lead ? k : tail + k - lead;
-    const uint32_t c = cnt[pad + v];
-    const float y = process(to_f32(src[v]), c, v, allowed_bits(v) & 1u);
+    float y = to_f32(src[v]);
+    if (touched && ((map[v >> 5] >> (v & 31)) & 1u)) y = round_st<T>(__uint_as_float(cnt[v]));
+    if (mask != nullptr && !((mask[v >> 5] >> (v & 31)) & 1u)) y = -INFINITY;
     if (dst) dst[v] = from_f32<T>(y);
-    consider(y, c, v);
-  }
-  if (n_bias > 0 && !scan) {
-    __syncthreads();  // the pieces around them are stored
-    for (int k = t; k < n_bias; k += kThreads) {
-      const int v = bias_tok[k];
-      bool first = true;
-      for (int j = 0; j < k; ++j) first = first && bias_tok[j] != v;
-      if (!first) continue;
-      const uint32_t c = cnt[pad + v];
-      float x = bias_x[k];
-      if (c & ~kBiased) x = pen.apply(x, c);
-      for (int j = k; j < n_bias; ++j)
-        if (bias_tok[j] == v) x = __fadd_rn(x, bias_val[j]);
-      if (!(allowed_bits(v) & 1u)) x = -INFINITY;
-      const T y = from_f32<T>(x);
-      if (dst) dst[v] = y;
-      const unsigned long long key = pick_key(to_f32(y), uint32_t(v0 + v));
-      if (key > best) best = key;
+    if (y > best || (y == best && uint32_t(v0 + v) < best_v)) {
+      best = y;
+      best_v = uint32_t(v0 + v);
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-    if (other > best) best = other;
+    const float y = __shfl_xor_sync(0xffffffffu, best, o);
+    const uint32_t v = __shfl_xor_sync(0xffffffffu, best_v, o);
+    if (y > best || (y == best && v < best_v)) {
+      best = y;
+      best_v = v;
+    }
   }
-  if (lane == 0) warp_best[warp] = best;
+  if (lane == 0) {
+    warp_y[warp] = best;
+    warp_v[warp] = best_v;
+  }
   __syncthreads();
   if (t == 0) {
 #pragma unroll
     for (int w = 1; w < kThreads / 32; ++w)
-      if (warp_best[w] > best) best = warp_best[w];
-    *cl.map_shared_rank(&cta_best[rank], 0) = best;
+      if (warp_y[w] > best || (warp_y[w] == best && warp_v[w] < best_v)) {
+        best = warp_y[w];
+        best_v = warp_v[w];
+      }
+    *cl.map_shared_rank(&cta_best[rank], 0) = pick_key(best, best_v);
   }
   cl.sync();
   if (rank == 0 && t == 0) {
@@ -325,17 +310,24 @@ __global__ void __launch_bounds__(kThreads)
 }  // namespace
 
 cudaError_t launch_logits_pick(const LogitsArgs& a, int dtype, cudaStream_t s) {
-  // slices of at least 1024 tokens, a multiple of 32 (whole mask words)
+  // slices of at least 1024 tokens, a multiple of 128 (whole words of masks and 16 bytes of the map)
   int c = 1;
   while (c < kMaxCluster && a.vocab > c * 1024) c *= 2;
-  const int slice = ((a.vocab + c - 1) / c + 31) / 32 * 32;
-  const size_t smem = size_t(slice + 8) * 4;
+  const int slice = ((a.vocab + c - 1) / c + 127) / 128 * 128;
+  constexpr int kMaxSlice = ((kMaxVocab + kMaxCluster - 1) / kMaxCluster + 127) / 128 * 128;
+  static_assert(kMaxSlice <= 65536, "a slice's tokens in 16 bits");
+  auto bytes = [](int slice, int hist) {
+    return size_t(slice) * 4 + size_t(slice) / 8 + size_t(hist) * 2;
+  };
+  const bool touched = a.hist != nullptr || a.bias_start != nullptr;
+  const bool listed = a.hist != nullptr && a.hist_cap <= kLocalHist;
+  const size_t smem = touched ? bytes(slice, listed ? a.hist_cap : 0) : 0;
   const void* fn = dtype == 0 ? reinterpret_cast<const void*>(&logits_pick_kernel<__half>)
                               : reinterpret_cast<const void*>(&logits_pick_kernel<float>);
   static PerDeviceOnce attrs[2];
   const cudaError_t e = per_device_once(attrs[dtype == 0 ? 0 : 1], [&](int&) {
     return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (((kMaxVocab + kMaxCluster - 1) / kMaxCluster + 31) / 32 * 32 + 8) * 4);
+                                int(bytes(kMaxSlice, kLocalHist)));
   });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
