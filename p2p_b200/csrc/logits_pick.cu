@@ -26,10 +26,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
 constexpr int kMaxCluster = 8;
 constexpr int kLocalHist = 4096;
-constexpr int kMaxBiases = 512;            // of a slice, gathered in shared memory
+// Threads of a CTA: 256 up to this slice (four CTAs per SM: 64 rows of 65536 in 11.2 us, 15.8 with
+// 512), 512 above, where the counts leave room for two or three CTAs (128 rows of 131071 f32 in 58
+// us, 73 with 256).
+constexpr int kSmallSlice = 12288;
 constexpr uint32_t kSeen = 0x80000000u;    // in the prompt (or generated: the count says so)
 constexpr uint32_t kCount = 0x7fffffffu;   // times generated
 constexpr int kAhead = 4;                  // pieces of logits loaded before the history is read
@@ -68,20 +70,21 @@ struct Piece {  // 16 bytes of logits
   }
 };
 
-template <class T>
+template <class T, int kThreads>
 __global__ void __launch_bounds__(kThreads)
     logits_pick_kernel(const __grid_constant__ LogitsArgs a, int slice) {
   constexpr int kN = Piece<T>::kN;
-  // per token of the slice a count, later the value of a touched token; the map of touched tokens;
+  // per token of the slice a count, later the value of a touched token; a bit each: touched, allowed;
   // the counted tokens (short histories)
   extern __shared__ __align__(16) uint32_t cnt[];
-  uint32_t* map = cnt + slice;
-  uint16_t* list = reinterpret_cast<uint16_t*>(map + slice / 32);
+  uint32_t* map = cnt + (a.hist != nullptr || a.bias_start != nullptr ? slice : 0);
+  uint32_t* mask = map + slice / 32;
+  uint16_t* list = reinterpret_cast<uint16_t*>(mask + slice / 32);
   __shared__ float warp_y[kThreads / 32];
   __shared__ uint32_t warp_v[kThreads / 32];
   __shared__ unsigned long long cta_best[kMaxCluster];  // rank 0's: one slot per CTA
-  __shared__ int bias_tok[kMaxBiases];
-  __shared__ float bias_val[kMaxBiases];
+  __shared__ int bias_tok[kThreads];
+  __shared__ float bias_val[kThreads];
   __shared__ int warp_n[kThreads / 32];
   __shared__ int n_list;
   cg::cluster_group cl = cg::this_cluster();
@@ -100,6 +103,21 @@ __global__ void __launch_bounds__(kThreads)
   for (int k = 0; k < kAhead; ++k)
     if (t + k * kThreads < pieces) ahead[k].w = body[t + k * kThreads];
 
+  // ... and everything else the CTA is going to look at is asked for now, before any of it is
+  // needed: the row's history (short ones whole; what lies behind its length is dropped later), the
+  // first of its biases, the slice's mask words
+  const bool remote = a.hist_cap > kLocalHist;
+  const int32_t* hist = a.hist + int64_t(i) * a.ld_hist;
+  constexpr int kHist = kLocalHist / kThreads;
+  int early[kHist];
+  if (a.hist != nullptr && !remote) {
+#pragma unroll
+    for (int k = 0; k < kHist; ++k)
+      early[k] = t + k * kThreads < a.hist_cap ? hist[t + k * kThreads] : -1;
+  }
+  const int words = a.mask ? (n + 31) / 32 : 0;
+  const uint32_t* mask_row = a.mask ? a.mask + int64_t(i) * a.ld_mask + v0 / 32 : nullptr;
+  const uint32_t early_mask = t < words ? mask_row[t] : 0u;
   int len = 0, prompt = 0, e0 = 0, e1 = 0;
   if (a.hist != nullptr) {
     len = min(max(a.hist_len[i], 0), a.hist_cap);
@@ -109,9 +127,12 @@ __global__ void __launch_bounds__(kThreads)
     e0 = min(max(a.bias_start[i], 0), a.n_bias);
     e1 = min(max(a.bias_start[i + 1], e0), a.n_bias);
   }
+  const int early_tok = e0 + t < e1 ? a.bias_tok[e0 + t] : -1;
+  const float early_val = e0 + t < e1 ? a.bias_val[e0 + t] : 0.f;
+  if (t < words) mask[t] = early_mask;
+  for (int k = t + kThreads; k < words; k += kThreads) mask[k] = mask_row[k];
   const bool touched = a.hist != nullptr || a.bias_start != nullptr;
   if (touched) {
-    const bool remote = a.hist_cap > kLocalHist;
     const bool has_rep = a.repetition != nullptr;
     const float rep = has_rep ? a.repetition[i] : 1.f;
     const float pres = a.presence ? a.presence[i] : 0.f;
@@ -121,7 +142,6 @@ __global__ void __launch_bounds__(kThreads)
     if (t == 0) n_list = 0;
     if (remote) cl.sync();
     else __syncthreads();
-    const int32_t* hist = a.hist + int64_t(i) * a.ld_hist;
     if (remote) {
       for (int k = rank * kThreads + t; k < len; k += csize * kThreads) {
         const int v = hist[k];
@@ -132,18 +152,24 @@ __global__ void __launch_bounds__(kThreads)
       }
       cl.sync();
     } else {
-#pragma unroll 4
-      for (int k = t; k < len; k += kThreads) {
-        const int v = hist[k] - v0;
-        if (v < 0 || v >= n) continue;
-        const uint32_t old = k >= prompt ? atomicAdd(&cnt[v], 1u) : atomicOr(&cnt[v], kSeen);
-        if (old == 0u) list[atomicAdd(&n_list, 1)] = uint16_t(v);  // the first to touch it
+#pragma unroll
+      for (int j = 0; j < kHist; ++j) {
+        if (j * kThreads >= len) break;
+        const int k = t + j * kThreads, v = early[j] - v0;
+        bool fresh = false;
+        if (k < len && v >= 0 && v < n)
+          fresh = (k >= prompt ? atomicAdd(&cnt[v], 1u) : atomicOr(&cnt[v], kSeen)) == 0u;
+        // the first to touch a token lists it; one count a warp
+        const uint32_t votes = __ballot_sync(0xffffffffu, fresh);
+        int at = 0;
+        if (lane == 0 && votes) at = atomicAdd(&n_list, __popc(votes));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(votes & ((1u << lane) - 1u));
+        if (fresh) list[at] = uint16_t(v);
       }
       __syncthreads();
     }
-    auto penalise = [&](int v) {
+    auto penalise = [&](int v, float x) {
       const uint32_t c = cnt[v];
-      float x = to_f32(src[v]);
       if (has_rep) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
       if (c & kCount) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, float(c & kCount))), pres);
       cnt[v] = __float_as_uint(x);
@@ -151,16 +177,24 @@ __global__ void __launch_bounds__(kThreads)
     };
     if (remote) {
       for (int v = t; v < n; v += kThreads)
-        if (cnt[v] != 0u) penalise(v);
+        if (cnt[v] != 0u) penalise(v, to_f32(src[v]));
     } else {
-      for (int k = t; k < n_list; k += kThreads) penalise(list[k]);
+      for (int k0 = t; k0 < n_list; k0 += 4 * kThreads) {  // four logits on their way
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (k0 + j * kThreads < n_list) x[j] = to_f32(src[list[k0 + j * kThreads]]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (k0 + j * kThreads < n_list) penalise(list[k0 + j * kThreads], x[j]);
+      }
     }
-    // the slice's biases, in the order of the list, kMaxBiases at a time
+    // the slice's biases, in the order of the list, a round of kThreads entries at a time
     for (int k0 = e0; k0 < e1; k0 += kThreads) {
-      static_assert(kMaxBiases == kThreads, "a round's entries fit");
       const int k = k0 + t;
-      const int v = k < e1 ? a.bias_tok[k] - v0 : -1;
-      const bool mine = v >= 0 && v < n;
+      const int tok = k0 == e0 ? early_tok : k < e1 ? a.bias_tok[k] : -1;
+      const int v = tok - v0;
+      const bool mine = tok >= 0 && v >= 0 && v < n;
       const uint32_t votes = __ballot_sync(0xffffffffu, mine);
       if (lane == 0) warp_n[warp] = __popc(votes);
       __syncthreads();  // also: the penalties, or the round before, are in place
@@ -172,7 +206,7 @@ __global__ void __launch_bounds__(kThreads)
       }
       if (mine) {
         bias_tok[at] = v;
-        bias_val[at] = a.bias_val[k];
+        bias_val[at] = k0 == e0 ? early_val : a.bias_val[k];
       }
       __syncthreads();
       if (t < all) {  // a token's first entry adds all of them, in order
@@ -190,9 +224,8 @@ __global__ void __launch_bounds__(kThreads)
       }
       __syncthreads();
     }
-    __syncthreads();
   }
-  const uint32_t* mask = a.mask ? a.mask + int64_t(i) * a.ld_mask + v0 / 32 : nullptr;
+  __syncthreads();
   // bits of the kN tokens from v on, out of a word a 32 tokens (v0 is a multiple of 32)
   auto bits_of = [&](const uint32_t* words, int v) {
     const int w = v >> 5, sh = v & 31;
@@ -214,7 +247,7 @@ __global__ void __launch_bounds__(kThreads)
       for (int j = 0; j < kN; ++j)
         if ((hit >> j) & 1u) y[j] = round_st<T>(__uint_as_float(cnt[v + j]));
     }
-    if (mask != nullptr) {
+    if (words) {
       const uint32_t bits = bits_of(mask, v);
 #pragma unroll
       for (int j = 0; j < kN; ++j)
@@ -256,7 +289,7 @@ __global__ void __launch_bounds__(kThreads)
     const int v = k < lead ? k : tail + k - lead;
     float y = to_f32(src[v]);
     if (touched && ((map[v >> 5] >> (v & 31)) & 1u)) y = round_st<T>(__uint_as_float(cnt[v]));
-    if (mask != nullptr && !((mask[v >> 5] >> (v & 31)) & 1u)) y = -INFINITY;
+    if (words && !((mask[v >> 5] >> (v & 31)) & 1u)) y = -INFINITY;
     if (dst) dst[v] = from_f32<T>(y);
     if (y > best || (y == best && uint32_t(v0 + v) < best_v)) {
       best = y;
@@ -317,22 +350,26 @@ cudaError_t launch_logits_pick(const LogitsArgs& a, int dtype, cudaStream_t s) {
   constexpr int kMaxSlice = ((kMaxVocab + kMaxCluster - 1) / kMaxCluster + 127) / 128 * 128;
   static_assert(kMaxSlice <= 65536, "a slice's tokens in 16 bits");
   auto bytes = [](int slice, int hist) {
-    return size_t(slice) * 4 + size_t(slice) / 8 + size_t(hist) * 2;
+    return size_t(slice) * 4 + size_t(slice) / 4 + size_t(hist) * 2;
   };
   const bool touched = a.hist != nullptr || a.bias_start != nullptr;
   const bool listed = a.hist != nullptr && a.hist_cap <= kLocalHist;
-  const size_t smem = touched ? bytes(slice, listed ? a.hist_cap : 0) : 0;
-  const void* fn = dtype == 0 ? reinterpret_cast<const void*>(&logits_pick_kernel<__half>)
-                              : reinterpret_cast<const void*>(&logits_pick_kernel<float>);
-  static PerDeviceOnce attrs[2];
-  const cudaError_t e = per_device_once(attrs[dtype == 0 ? 0 : 1], [&](int&) {
+  const size_t smem = touched ? bytes(slice, listed ? a.hist_cap : 0) : size_t(slice) / 4;
+  const int which = (dtype == 0 ? 0 : 2) + (slice > kSmallSlice ? 1 : 0);
+  const int threads = slice > kSmallSlice ? 512 : 256;
+  const void* fn = which == 0   ? reinterpret_cast<const void*>(&logits_pick_kernel<__half, 256>)
+                   : which == 1 ? reinterpret_cast<const void*>(&logits_pick_kernel<__half, 512>)
+                   : which == 2 ? reinterpret_cast<const void*>(&logits_pick_kernel<float, 256>)
+                                : reinterpret_cast<const void*>(&logits_pick_kernel<float, 512>);
+  static PerDeviceOnce attrs[4];
+  const cudaError_t e = per_device_once(attrs[which], [&](int&) {
     return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 int(bytes(kMaxSlice, kLocalHist)));
   });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(a.rows) * unsigned(c));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(unsigned(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at{};
