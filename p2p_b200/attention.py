@@ -21,6 +21,7 @@ with device memory held in torch tensors and every kernel in libp2pattn.so:
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -39,18 +40,12 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(
     lambda d: torch.cuda.current_stream(d).cuda_stream)
 
 
-def _need(ok: bool, msg: str):
-    if not ok:
-        raise P2PError(_lib.P2P_ERR_INVALID_ARG, msg)
+def _refuse(msg: str):
+    raise P2PError(_lib.P2P_ERR_INVALID_ARG, msg)
 
 
 def _addr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
-
-
-def _table(t):
-    """A rope table: a tensor or what Context.rope_table returned."""
-    return t if t is None or isinstance(t, C.c_void_p) else t.data_ptr()
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -63,6 +58,11 @@ def _stream(stream) -> C.c_void_p:
     return C.c_void_p(stream.cuda_stream)
 
 
+_KV_FORMATS = {torch.float16: _lib.P2P_KV_F16, torch.int8: _lib.P2P_KV_I8,
+               torch.uint8: _lib.P2P_KV_Q4}
+
+
+@functools.lru_cache(maxsize=None)
 def kv_q4_row_bytes(num_kv_heads: int) -> int:
     """Bytes of one token's row in a 4-bit KV cache."""
     return lib.p2p_kv_q4_row_bytes(num_kv_heads)
@@ -84,6 +84,15 @@ class Params:
         dt = {torch.float16: _lib.P2P_F16, torch.float32: _lib.P2P_F32}[self.dtype]
         return AttnParams(self.num_heads, self.num_kv_heads, self.head_dim, self.scale,
                           self.eps, dt)
+
+    def ref(self):
+        """The C view by reference, kept while the fields stay as they are."""
+        key = (self.num_heads, self.num_kv_heads, self.head_dim, self.scale, self.eps, self.dtype)
+        kept = self.__dict__.get("_c")
+        if kept is None or kept[0] != key:
+            c = self.c()
+            kept = self.__dict__["_c"] = (key, c, C.byref(c))
+        return kept[2]
 
     @property
     def qkv_width(self) -> int:
@@ -277,21 +286,8 @@ class Context:
         (torch.uint8) hold rows of kv_q4_row_bytes(Hkv) bytes in place of [Hkv][64]."""
         assert past.dtype == torch.int32
         if k_cache.dtype == torch.uint8:
-            lay, rows = self._layout(prm.num_kv_heads, k_cache, v_cache, past, offsets,
-                                     block_table, None, None)
-            ld_qkv = self._rows(
-                qkv, prm.qkv_width if fused_prep else prm.num_heads * HEAD_DIM, "qkv")
-            ld_o = self._rows(out, prm.num_heads * HEAD_DIM, "out")
-            n = past.shape[0]
-            self._ints(past, n, "past")
-            if n == 0:
-                return
-            _need(qkv.shape[0] >= n and out.shape[0] >= n, "qkv or out has too few rows")
-            self._chk(lib.p2p_attn_decode_kv(
-                self.h, C.byref(prm.c()), C.byref(lay), qkv.data_ptr(), ld_qkv,
-                _addr(norm_w), _table(rope), k_cache.data_ptr(), v_cache.data_ptr(),
-                rows if kv_rows is None else kv_rows, _addr(offsets), past.data_ptr(), n,
-                max_past, int(fused_prep), out.data_ptr(), ld_o, self._stream(stream)))
+            self._decode_q4(prm, qkv, norm_w, rope, k_cache, v_cache, past, out, max_past,
+                            offsets, block_table, fused_prep, kv_rows, stream)
             return
         q8 = k_cache.dtype == torch.int8
         lay = _lib.KvLayout()
@@ -321,56 +317,103 @@ class Context:
 
     def _rows(self, t: torch.Tensor, width: int, name: str) -> int:
         """Checks f16 rows of at least `width` values and returns their row stride."""
-        if not (t.dtype == torch.float16 and t.get_device() == self.device and t.dim() == 2 and
-                t.shape[1] >= width and (t.stride(1) == 1 or t.shape[1] == 1)):
-            _need(False, f"{name}: f16 rows of {width} or more values on device {self.device} "
-                  f"needed, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        return t.stride(0) if t.shape[0] > 1 else width
+        shape = t.shape
+        if t.dtype is not torch.float16 or t.get_device() != self.device or len(shape) != 2 or \
+                shape[1] < width or t.stride(1) != 1:
+            _refuse(f"{name}: f16 rows of {width} or more values on device {self.device} needed, "
+                    f"got {tuple(shape)} {t.dtype} on {t.device}")
+        return t.stride(0) if shape[0] > 1 else width
 
-    def _ints(self, t: Optional[torch.Tensor], n: int, name: str):
-        _need(t is not None and t.dtype == torch.int32 and t.get_device() == self.device and
-              t.is_contiguous() and t.numel() >= n,
-              f"{name}: {n} contiguous int32 values on the context's device needed")
+    def _ints(self, t: Optional[torch.Tensor], n: int, name: str) -> int:
+        """Checks n int32 values and returns their address."""
+        if t is None or t.dtype is not torch.int32 or t.get_device() != self.device or \
+                t.numel() < n or not t.is_contiguous():
+            _refuse(f"{name}: {n} contiguous int32 values on device {self.device} needed")
+        return t.data_ptr()
 
-    def _layout(self, hkv: int, k_cache, v_cache, past, offsets, block_table, k_scale, v_scale):
-        """The C layout and the cache's rows (or pages) of a pair of cache tensors."""
-        dt = k_cache.dtype
-        q4 = dt == torch.uint8
-        _need(dt in (torch.float16, torch.int8, torch.uint8) and v_cache.dtype == dt and
-              k_cache.shape == v_cache.shape and k_cache.get_device() == self.device and
-              v_cache.get_device() == self.device and k_cache.is_contiguous() and v_cache.is_contiguous(),
-              "k_cache and v_cache: contiguous tensors on the context's device, of one shape and type (f16, int8 "
-              "or uint8) needed")
-        shape = k_cache.shape
-        lead = shape[:-1] if q4 else shape[:-2]
-        want = (kv_q4_row_bytes(hkv),) if q4 else (hkv, HEAD_DIM)
-        _need(tuple(shape[len(lead):]) == want,
-              f"cache rows of shape {want} needed, got {tuple(shape)}")
-        _need(len(lead) == (1 if block_table is None else 2),
-              "[rows] caches with offsets or [pages][block_size] caches with a block table needed")
+    def _floats(self, t: Optional[torch.Tensor], n: int, name: str) -> int:
+        if t is None or t.dtype is not torch.float32 or t.get_device() != self.device or \
+                t.numel() < n or not t.is_contiguous():
+            _refuse(f"{name}: {n} contiguous f32 values on device {self.device} needed")
+        return t.data_ptr()
+
+    def _layout(self, hkv: int, k_cache, v_cache, n: int, offsets, block_table, k_scale, v_scale):
+        """Checks a pair of cache tensors for n sequences: the C layout, the cache's rows (or
+        pages) and the address of the offsets."""
+        dt, shape, dev = k_cache.dtype, k_cache.shape, self.device
+        fmt = _KV_FORMATS.get(dt)
+        if fmt is None or v_cache.dtype is not dt or v_cache.shape != shape or \
+                k_cache.get_device() != dev or v_cache.get_device() != dev or \
+                not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+            _refuse(f"k_cache and v_cache: contiguous tensors of one shape and type (f16, int8 or "
+                    f"uint8) on device {dev} needed")
+        lead = 1 if block_table is None else 2
+        if fmt == _lib.P2P_KV_Q4:
+            if len(shape) != lead + 1 or shape[lead] != kv_q4_row_bytes(hkv):
+                _refuse(f"a 4-bit cache's rows are {kv_q4_row_bytes(hkv)} bytes behind [rows] or "
+                        f"[pages][block_size], got {tuple(shape)}")
+        elif len(shape) != lead + 2 or shape[lead] != hkv or shape[lead + 1] != HEAD_DIM:
+            _refuse(f"[rows] caches with offsets or [pages][block_size] caches with a block table, "
+                    f"of [{hkv}][{HEAD_DIM}] values, needed, got {tuple(shape)}")
         lay = _lib.KvLayout()
-        n = past.numel()
+        lay.format = fmt
+        offs = None
         if block_table is not None:
-            _need(block_table.dim() == 2 and block_table.shape[0] >= n,
-                  "block_table: [nseq][max_blocks] needed")
-            self._ints(block_table, 0, "block_table")
-            lay.block_size = lead[1]
-            lay.block_table = block_table.data_ptr()
-            lay.max_blocks = block_table.shape[1]
+            tab = block_table.shape
+            if len(tab) != 2 or tab[0] < n:
+                _refuse(f"block_table: [{n}][max_blocks] needed, got {tuple(tab)}")
+            lay.block_table = self._ints(block_table, 0, "block_table")
+            lay.block_size = shape[1]
+            lay.max_blocks = tab[1]
         else:
-            self._ints(offsets, n, "offsets")
-        if dt == torch.int8:
-            lay.format = _lib.P2P_KV_I8
-            _need(k_scale is not None and v_scale is not None and
-                  k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32 and
-                  k_scale.numel() == v_scale.numel() and k_scale.get_device() == v_scale.get_device() == self.device and
-                  k_scale.is_contiguous() and v_scale.is_contiguous(),
-                  "int8 caches need as many f32 k_scale as v_scale values")
-            lay.k_scale, lay.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+            offs = self._ints(offsets, n, "offsets")
+        if fmt == _lib.P2P_KV_I8:
+            lay.k_scale = self._floats(k_scale, 1, "k_scale")
             lay.scale_count = k_scale.numel()
+            lay.v_scale = self._floats(v_scale, lay.scale_count, "v_scale")
+        return lay, shape[0], offs
+
+    def _weights(self, norm_w, rope, max_len: int):
+        """The addresses of the norm weights and of the rope table (a tensor, or what rope_table
+        returned)."""
+        nw = None
+        if norm_w is not None:
+            if norm_w.dtype is not torch.float16 or norm_w.numel() != 2 * HEAD_DIM or \
+                    norm_w.get_device() != self.device or not norm_w.is_contiguous():
+                _refuse(f"norm_w: {2 * HEAD_DIM} f16 values on device {self.device} needed")
+            nw = norm_w.data_ptr()
+        if isinstance(rope, torch.Tensor):
+            if rope.dtype is not torch.float16 or rope.numel() < max_len * HEAD_DIM or \
+                    rope.get_device() != self.device or not rope.is_contiguous():
+                _refuse(f"rope: f16 [{max_len}][{HEAD_DIM}] on device {self.device} needed")
+            rope = rope.data_ptr()
+        return nw, rope
+
+    def _decode_q4(self, prm: Params, qkv, norm_w, rope, k_cache, v_cache, past, out, max_past,
+                   offsets, block_table, fused_prep, kv_rows, stream):
+        """attn_decode_kv over a 4-bit cache."""
+        n = past.numel()
+        lay, rows, offs = self._layout(prm.num_kv_heads, k_cache, v_cache, n, offsets, block_table,
+                                       None, None)
+        width = prm.num_heads * HEAD_DIM
+        ld_qkv = self._rows(qkv, prm.qkv_width if fused_prep else width, "qkv")
+        ld_o = self._rows(out, width, "out")
+        nw = None
+        if fused_prep:
+            nw, rope = self._weights(norm_w, rope, max_past + 1)
         else:
-            lay.format = _lib.P2P_KV_Q4 if q4 else _lib.P2P_KV_F16
-        return lay, lead[0]
+            rope = None
+        at = self._ints(past, n, "past")
+        if n == 0:
+            return
+        if qkv.shape[0] < n or out.shape[0] < n:
+            _refuse(f"qkv and out: {n} rows needed")
+        st = lib.p2p_attn_decode_kv(
+            self.h, prm.ref(), C.byref(lay), qkv.data_ptr(), ld_qkv, nw, rope,
+            k_cache.data_ptr(), v_cache.data_ptr(), rows if kv_rows is None else kv_rows, offs, at,
+            n, max_past, 1 if fused_prep else 0, out.data_ptr(), ld_o, self._stream(stream))
+        if st:
+            self._chk(st)
 
     def kv_append(self, prm: Params, qkv: torch.Tensor, norm_w: Optional[torch.Tensor], rope,
                   k_cache: torch.Tensor, v_cache: torch.Tensor, past: torch.Tensor,
@@ -383,26 +426,24 @@ class Context:
         row_start[i] .. row_start[i+1] of qkv are sequence i's tokens at positions past[i] and
         up; their k and v go to the cache, their rotated q to q_out.  The cache tensors are as
         in attn_decode_kv; the rope table holds max_len rows or more."""
-        lay, rows = self._layout(prm.num_kv_heads, k_cache, v_cache, past, offsets, block_table,
-                                 k_scale, v_scale)
         n = past.numel()
-        self._ints(past, n, "past")
-        self._ints(row_start, n + 1, "row_start")
-        ld_qkv, ld_q = self._rows(qkv, prm.qkv_width, "qkv"), 0
+        lay, rows, offs = self._layout(prm.num_kv_heads, k_cache, v_cache, n, offsets, block_table,
+                                       k_scale, v_scale)
+        ld_qkv, m = self._rows(qkv, prm.qkv_width, "qkv"), qkv.shape[0]
+        q_at, ld_q = None, 0
         if q_out is not None:
             ld_q = self._rows(q_out, prm.num_heads * HEAD_DIM, "q_out")
-            _need(q_out.shape[0] >= qkv.shape[0], "q_out has too few rows")
-        if norm_w is not None:
-            _need(norm_w.dtype == torch.float16 and norm_w.numel() == 2 * HEAD_DIM and
-                  norm_w.is_contiguous(), "norm_w: 128 f16 values needed")
-        if isinstance(rope, torch.Tensor):
-            _need(rope.dtype == torch.float16 and rope.is_contiguous() and
-                  rope.numel() >= max_len * HEAD_DIM, f"rope: f16 [{max_len}][64] needed")
-        self._chk(lib.p2p_kv_append(
-            self.h, C.byref(prm.c()), C.byref(lay), qkv.data_ptr(), ld_qkv,
-            _addr(norm_w), _table(rope), k_cache.data_ptr(), v_cache.data_ptr(), rows,
-            _addr(offsets), past.data_ptr(), row_start.data_ptr(), n, qkv.shape[0], max_len,
-            _addr(q_out), ld_q, self._stream(stream)))
+            if q_out.shape[0] < m:
+                _refuse(f"q_out: {m} rows needed")
+            q_at = q_out.data_ptr()
+        nw, rope = self._weights(norm_w, rope, max_len)
+        st = lib.p2p_kv_append(
+            self.h, prm.ref(), C.byref(lay), qkv.data_ptr(), ld_qkv, nw, rope,
+            k_cache.data_ptr(), v_cache.data_ptr(), rows, offs, self._ints(past, n, "past"),
+            self._ints(row_start, n + 1, "row_start"), n, m, max_len, q_at, ld_q,
+            self._stream(stream))
+        if st:
+            self._chk(st)
 
     def kv_read(self, prm: Params, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 first: torch.Tensor, row_start: torch.Tensor, k_out: Optional[torch.Tensor],
@@ -413,23 +454,25 @@ class Context:
                 v_scale: Optional[torch.Tensor] = None, stream=None):
         """Cached sequences back as f16 values (p2p_kv_read): rows row_start[i] + j of k_out and
         v_out [rows][Hkv][64] receive key first[i] + j of sequence i."""
-        hkv = prm.num_kv_heads
-        lay, rows = self._layout(hkv, k_cache, v_cache, first, offsets, block_table, k_scale,
-                                 v_scale)
-        n = first.numel()
-        self._ints(first, n, "first")
-        self._ints(row_start, n + 1, "row_start")
-        outs = [t for t in (k_out, v_out) if t is not None]
-        _need(bool(outs), "k_out or v_out needed")
-        for t in outs:
-            _need(t.dtype == torch.float16 and t.get_device() == self.device and t.is_contiguous() and
-                  tuple(t.shape[1:]) == (hkv, HEAD_DIM) and t.shape[0] == outs[0].shape[0],
-                  f"k_out and v_out: contiguous f16 [rows][{hkv}][64] of one length needed")
-        self._chk(lib.p2p_kv_read(
-            self.h, C.byref(lay), hkv, k_cache.data_ptr(), v_cache.data_ptr(), rows,
-            _addr(offsets), first.data_ptr(), row_start.data_ptr(), n,
-            outs[0].shape[0], max_len, _addr(k_out), _addr(v_out),
-            self._stream(stream)))
+        hkv, n = prm.num_kv_heads, first.numel()
+        lay, rows, offs = self._layout(hkv, k_cache, v_cache, n, offsets, block_table, k_scale,
+                                       v_scale)
+        one = k_out if k_out is not None else v_out
+        if one is None:
+            _refuse("k_out or v_out needed")
+        m = one.shape[0]
+        for t in (k_out, v_out):
+            if t is not None and (t.dtype is not torch.float16 or t.get_device() != self.device or
+                                  tuple(t.shape) != (m, hkv, HEAD_DIM) or
+                                  not t.is_contiguous()):
+                _refuse(f"k_out and v_out: contiguous f16 [rows][{hkv}][{HEAD_DIM}] of one length "
+                        f"on device {self.device} needed")
+        st = lib.p2p_kv_read(
+            self.h, C.byref(lay), hkv, k_cache.data_ptr(), v_cache.data_ptr(), rows, offs,
+            self._ints(first, n, "first"), self._ints(row_start, n + 1, "row_start"), n, m,
+            max_len, _addr(k_out), _addr(v_out), self._stream(stream))
+        if st:
+            self._chk(st)
 
     def attn_chunk_kv(self, prm: Params, q: torch.Tensor, k_cache: torch.Tensor,
                       v_cache: torch.Tensor, past: torch.Tensor, row_start: torch.Tensor,
@@ -441,32 +484,36 @@ class Context:
         """ATTN of ragged prompt chunks over a cache of any layout (p2p_attn_chunk_kv): rotated
         query row t of sequence i (row row_start[i] + t) attends keys 0 .. past[i] + t, which
         kv_append has stored."""
-        lay, rows = self._layout(prm.num_kv_heads, k_cache, v_cache, past, offsets, block_table,
-                                 k_scale, v_scale)
         n = past.numel()
-        self._ints(past, n, "past")
-        self._ints(row_start, n + 1, "row_start")
-        ld_q = self._rows(q, prm.num_heads * HEAD_DIM, "q")
-        ld_o = self._rows(out, prm.num_heads * HEAD_DIM, "out")
-        _need(out.shape[0] >= q.shape[0], "out has too few rows")
-        self._chk(lib.p2p_attn_chunk_kv(
-            self.h, C.byref(prm.c()), C.byref(lay), q.data_ptr(), ld_q,
-            k_cache.data_ptr(), v_cache.data_ptr(), rows, _addr(offsets), past.data_ptr(),
-            row_start.data_ptr(), n, q.shape[0], max_len, out.data_ptr(), ld_o,
-            self._stream(stream)))
+        lay, rows, offs = self._layout(prm.num_kv_heads, k_cache, v_cache, n, offsets, block_table,
+                                       k_scale, v_scale)
+        width, m = prm.num_heads * HEAD_DIM, q.shape[0]
+        ld_q = self._rows(q, width, "q")
+        ld_o = self._rows(out, width, "out")
+        if out.shape[0] < m:
+            _refuse(f"out: {m} rows needed")
+        st = lib.p2p_attn_chunk_kv(
+            self.h, prm.ref(), C.byref(lay), q.data_ptr(), ld_q, k_cache.data_ptr(),
+            v_cache.data_ptr(), rows, offs, self._ints(past, n, "past"),
+            self._ints(row_start, n + 1, "row_start"), n, m, max_len, out.data_ptr(), ld_o,
+            self._stream(stream))
+        if st:
+            self._chk(st)
 
     def kv_quantize_q4(self, src: torch.Tensor, dst: Optional[torch.Tensor] = None,
                        stream=None) -> torch.Tensor:
         """f16 cache rows [..., Hkv, 64] -> the rows [..., kv_q4_row_bytes(Hkv)] (uint8) of a
         4-bit cache."""
-        _need(src.dtype == torch.float16 and src.get_device() == self.device and src.is_contiguous() and
-              src.dim() >= 2 and src.shape[-1] == HEAD_DIM, "src: f16 [..., Hkv, 64] needed")
+        if src.dtype is not torch.float16 or src.get_device() != self.device or src.dim() < 2 or \
+                src.shape[-1] != HEAD_DIM or not src.is_contiguous():
+            _refuse(f"src: contiguous f16 [..., Hkv, {HEAD_DIM}] on device {self.device} needed")
         hkv = src.shape[-2]
         shape = (*src.shape[:-2], kv_q4_row_bytes(hkv))
         if dst is None:
             dst = torch.empty(shape, dtype=torch.uint8, device=src.device)
-        _need(dst.dtype == torch.uint8 and tuple(dst.shape) == shape and dst.is_contiguous() and
-              dst.get_device() == self.device, f"dst: contiguous uint8 {shape} needed")
+        if dst.dtype is not torch.uint8 or tuple(dst.shape) != shape or \
+                dst.get_device() != self.device or not dst.is_contiguous():
+            _refuse(f"dst: contiguous uint8 {shape} on device {self.device} needed")
         self._chk(lib.p2p_kv_quantize_q4(self.h, src.data_ptr(), dst.data_ptr(),
                                          src.numel() // (hkv * HEAD_DIM), hkv,
                                          self._stream(stream)))
@@ -489,52 +536,58 @@ class Context:
         biases and grammar masks [rows][words] (p2p_logits_pick); -1 where nothing is left.
         The processed logits go to `out` (may be `logits`).  advance appends the tokens to the
         histories and moves hist_len and past on."""
-        _need(logits.dim() == 2 and logits.get_device() == self.device and logits.stride(1) == 1 and
-              logits.dtype in (torch.float16, torch.float32), "logits: f16 or f32 [rows][vocab]")
-        n, vocab = logits.shape
+        dt, shape, dev = logits.dtype, logits.shape, self.device
+        if dt not in (torch.float16, torch.float32) or len(shape) != 2 or \
+                logits.get_device() != dev or logits.stride(1) != 1 and shape[1] != 1:
+            _refuse(f"logits: f16 or f32 [rows][vocab] on device {dev} needed")
+        n, vocab = shape
         g = _lib.Logits()
-        g.rows, g.vocab, g.advance = n, vocab, int(advance)
-        g.dtype = _lib.P2P_F16 if logits.dtype == torch.float16 else _lib.P2P_F32
+        g.rows, g.vocab = n, vocab
+        g.advance = 1 if advance else 0
+        g.dtype = _lib.P2P_F16 if dt is torch.float16 else _lib.P2P_F32
         g.logits = logits.data_ptr()
         g.ld = logits.stride(0) if n > 1 else vocab
-        self._ints(tok, n, "tok")
-        g.tok = tok.data_ptr()
+        g.tok = self._ints(tok, n, "tok")
         if out is not None:
-            _need(out.shape == logits.shape and out.dtype == logits.dtype and out.get_device() == self.device and
-                  out.stride(1) == 1, "out: the shape and type of the logits needed")
-            g.out, g.ld_out = out.data_ptr(), out.stride(0) if n > 1 else vocab
+            if out.shape != shape or out.dtype is not dt or out.get_device() != dev or \
+                    out.stride(1) != 1 and vocab != 1:
+                _refuse("out: the shape, type and device of the logits needed")
+            g.out = out.data_ptr()
+            g.ld_out = out.stride(0) if n > 1 else vocab
         if hist is not None:
-            _need(hist.dtype == torch.int32 and hist.get_device() == self.device and hist.dim() == 2 and
-                  hist.shape[0] >= n and hist.stride(1) == 1, "hist: int32 [rows][cap] needed")
-            self._ints(hist_len, n, "hist_len")
-            g.hist, g.hist_cap = hist.data_ptr(), hist.shape[1]
-            g.ld_hist = hist.stride(0) if hist.shape[0] > 1 else hist.shape[1]
-            g.hist_len = hist_len.data_ptr()
-        for name, t in (("prompt_len", prompt_len), ("past", past)):
-            if t is not None:
-                self._ints(t, n, name)
-                setattr(g, name, t.data_ptr())
-        for name, t in (("repetition", repetition), ("presence", presence),
-                        ("frequency", frequency)):
-            if t is not None:
-                _need(t.dtype == torch.float32 and t.get_device() == self.device and t.is_contiguous() and
-                      t.numel() >= n, f"{name}: {n} f32 values on the device needed")
-                setattr(g, name, t.data_ptr())
+            hs = hist.shape
+            if hist.dtype is not torch.int32 or hist.get_device() != dev or len(hs) != 2 or \
+                    hs[0] < n or hist.stride(1) != 1 and hs[1] > 1:
+                _refuse(f"hist: int32 [{n}][capacity] on device {dev} needed")
+            g.hist = hist.data_ptr()
+            g.hist_cap = hs[1]
+            g.ld_hist = hist.stride(0) if hs[0] > 1 else hs[1]
+            g.hist_len = self._ints(hist_len, n, "hist_len")
+        if prompt_len is not None:
+            g.prompt_len = self._ints(prompt_len, n, "prompt_len")
+        if past is not None:
+            g.past = self._ints(past, n, "past")
+        if repetition is not None:
+            g.repetition = self._floats(repetition, n, "repetition")
+        if presence is not None:
+            g.presence = self._floats(presence, n, "presence")
+        if frequency is not None:
+            g.frequency = self._floats(frequency, n, "frequency")
         if bias_start is not None:
-            self._ints(bias_start, n + 1, "bias_start")
-            self._ints(bias_tok, 0, "bias_tok")
-            _need(bias_val is not None and bias_val.dtype == torch.float32 and
-                  bias_val.get_device() == self.device and bias_val.is_contiguous() and
-                  bias_val.numel() >= bias_tok.numel(), "bias_val: an f32 value per bias_tok")
-            g.bias_start, g.bias_tok = bias_start.data_ptr(), bias_tok.data_ptr()
-            g.bias_val, g.n_bias = bias_val.data_ptr(), bias_tok.numel()
+            g.bias_start = self._ints(bias_start, n + 1, "bias_start")
+            g.bias_tok = self._ints(bias_tok, 0, "bias_tok")
+            g.n_bias = bias_tok.numel()
+            g.bias_val = self._floats(bias_val, g.n_bias, "bias_val")
         if mask is not None:
-            _need(mask.dtype == torch.int32 and mask.get_device() == self.device and mask.dim() == 2 and
-                  mask.shape[0] >= n and mask.stride(1) == 1 and
-                  mask.shape[1] >= (vocab + 31) // 32, "mask: int32 [rows][ceil(vocab/32)]")
+            ms = mask.shape
+            if mask.dtype is not torch.int32 or mask.get_device() != dev or len(ms) != 2 or \
+                    ms[0] < n or ms[1] < (vocab + 31) // 32 or mask.stride(1) != 1 and ms[1] > 1:
+                _refuse(f"mask: int32 [{n}][{(vocab + 31) // 32}] on device {dev} needed")
             g.mask = mask.data_ptr()
-            g.ld_mask = mask.stride(0) if mask.shape[0] > 1 else mask.shape[1]
-        self._chk(lib.p2p_logits_pick(self.h, C.byref(g), self._stream(stream)))
+            g.ld_mask = mask.stride(0) if ms[0] > 1 else ms[1]
+        st = lib.p2p_logits_pick(self.h, C.byref(g), self._stream(stream))
+        if st:
+            self._chk(st)
 
     def kv_quantize_q8(self, src: torch.Tensor, scale: torch.Tensor,
                        dst: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
