@@ -33,13 +33,11 @@ __device__ __forceinline__ uint2 round4(float a, float b, float c, float d) {
   return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
-// x (8 values of a unit per lane) normed and rounded to f16.  The sum of squares follows the
-// shader's tree (kernels.js:246-251: t[i] = v[i]^2 + v[i+32]^2, then pairs 16, 8, 4, 2, 1 apart),
+// The sum of squares of a unit (x: 8 values per lane), in the shader's tree (kernels.js:246-251: t[i] = v[i]^2 + v[i+32]^2, then pairs 16, 8, 4, 2, 1 apart),
 // each IEEE operation on its own, so it is bit-identical to it (an addition's order of operands
 // does not matter).  Lane l holds t[4l .. 4l+3]: pairs 16 and 8 apart lie 4 and 2 lanes away, and a
 // lane keeps only half of its sums at each of these steps.
-__device__ __forceinline__ void norm_unit(const float (&x)[8], const float (&w)[8], int s,
-                                          float eps, float (&y)[8]) {
+__device__ __forceinline__ float square_sum(const float (&x)[8], int s) {
   float t[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -54,14 +52,20 @@ __device__ __forceinline__ void norm_unit(const float (&x)[8], const float (&w)[
   float r = __fadd_rn(odd ? p1 : p0, g2);
   r = __fadd_rn(r, __shfl_xor_sync(0xffffffffu, r, 1));  // 4 apart
   r = __fadd_rn(r, __shfl_xor_sync(0xffffffffu, r, 4));  // 2 apart: sums c and c + 2
-  r = __fadd_rn(r, __shfl_xor_sync(0xffffffffu, r, 2));  // 1 apart
-  const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(r, 0.015625f), eps)));
+  return __fadd_rn(r, __shfl_xor_sync(0xffffffffu, r, 2));  // 1 apart
+}
+
+// x normed with the weights w (packed) and rounded to f16.
+__device__ __forceinline__ void norm_unit(float (&x)[8], const uint2 (&w)[2], float inv) {
+  float f[8];
+  widen4(w[0], f);
+  widen4(w[1], f + 4);
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    const float2 f = __half22float2(__floats2half2_rn(
-        __fmul_rn(__fmul_rn(x[i], inv), w[i]), __fmul_rn(__fmul_rn(x[i + 1], inv), w[i + 1])));
-    y[i] = f.x;
-    y[i + 1] = f.y;
+    const float2 y = __half22float2(__floats2half2_rn(
+        __fmul_rn(__fmul_rn(x[i], inv), f[i]), __fmul_rn(__fmul_rn(x[i + 1], inv), f[i + 1])));
+    x[i] = y.x;
+    x[i + 1] = y.y;
   }
 }
 
@@ -122,6 +126,26 @@ __global__ void __launch_bounds__(kThreads)
   load4(a.rope + int64_t(pos) * 64 + 4 * s, cs);
   load4(a.rope + int64_t(pos) * 64 + 32 + 4 * s, sn);
   const bool norm = a.norm_w != nullptr;
+  uint2 wq[2] = {}, wk[2] = {};  // this lane's norm weights of q and of k units
+  float inv = 0.f;
+  if (norm) {
+    const __half* nw = a.norm_w + 4 * s;
+    wq[0] = *reinterpret_cast<const uint2*>(nw);
+    wq[1] = *reinterpret_cast<const uint2*>(nw + 32);
+    wk[0] = *reinterpret_cast<const uint2*>(nw + 64);
+    wk[1] = *reinterpret_cast<const uint2*>(nw + 96);
+    // lane s works out 1 / sqrt for group s % kIter; the others take it from there
+    float mean = 0.f;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      float x[8];
+      widen4(raw[i][0], x);
+      widen4(raw[i][1], x + 4);
+      const float r = square_sum(x, s);
+      if (s % kIter == i) mean = __fmul_rn(r, 0.015625f);
+    }
+    inv = __frcp_rn(__fsqrt_rn(__fadd_rn(mean, a.eps)));
+  }
 #pragma unroll
   for (int i = 0; i < kIter; ++i) {
     const int u = u0 + 4 * i, first = u - (lane >> 3);
@@ -132,14 +156,10 @@ __global__ void __launch_bounds__(kThreads)
       float x[8];
       widen4(lo, x);
       widen4(hi, x + 4);
-      if (norm) {  // the shuffles inside are warp-wide instructions: v units run them too
-        float w[8], y[8];
-        const __half* nw = a.norm_w + (is_q ? 0 : 64) + 4 * s;
-        load4(nw, w);
-        load4(nw + 32, w + 4);
-        norm_unit(x, w, s, a.eps, y);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = y[k];
+      if (norm) {
+        const float mine = __shfl_sync(0xffffffffu, inv, (lane & 24) + i);
+        const uint2 w[2] = {is_q ? wq[0] : wk[0], is_q ? wq[1] : wk[1]};
+        norm_unit(x, w, mine);
       }
       if (is_q || is_k) rotate_unit(x, cs, sn, lo, hi);
     }
