@@ -79,7 +79,7 @@ __device__ __forceinline__ bool wait_bar(Smem& s, uint64_t* bar, uint32_t parity
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   while (true) {
-    if (mbar_try_wait_for(bar, parity, 2000)) return true;
+    if (mbar_try_wait(bar, parity)) return true;
     if (s.abort_flag) return false;
     if (globaltimer_ns() - t0 > kWaitLimitNs) {
       s.abort_flag = 1;
@@ -237,6 +237,14 @@ __device__ __forceinline__ uint4 q4_piece(uint32_t w, uint32_t params) {
   }
   return make_uint4(__byte_perm(r[0], r[1], 0x5410), __byte_perm(r[2], r[3], 0x5410),
                     __byte_perm(r[0], r[1], 0x7632), __byte_perm(r[2], r[3], 0x7632));
+}
+
+// Bytes 2k, 2k + 1 of a word as signed values: the byte x ^ 0x80 under the f16 pattern 0x64xx is
+// 1024 + 128 + x (no conversion instructions, which would share the exponentials' unit).
+__device__ __forceinline__ float2 s8_pair(uint32_t w, int k) {
+  const uint32_t h = __byte_perm(w ^ 0x80808080u, 0x64646464u, k ? 0x4342 : 0x4140);
+  return __half22float2(
+      __hsub2(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(1152.f, 1152.f)));
 }
 
 template <int KVF>
@@ -639,13 +647,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int k = 0; k < 8; ++k) sc[k] = one;
             }
-            float f[8];
+            uint32_t h[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              f[k] = float(static_cast<int8_t>(raw[pool][2 * w + (k >> 2)] >> (8 * (k & 3)))) *
-                     sc[k];
-            x = make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]),
-                           pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
+            for (int k = 0; k < 4; ++k) {
+              const float2 v = s8_pair(raw[pool][2 * w + (k >> 1)], k & 1);
+              h[k] = pack_half2(v.x * sc[2 * k], v.y * sc[2 * k + 1]);
+            }
+            x = make_uint4(h[0], h[1], h[2], h[3]);
           }
           *reinterpret_cast<uint4*>(dst + ((w ^ (key & 7)) << 4)) = x;
         }
