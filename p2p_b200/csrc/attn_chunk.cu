@@ -63,6 +63,7 @@ __device__ __forceinline__ uint32_t col_o(int w) { return uint32_t(w) * 256u + 1
 struct __align__(128) Smem {
   __half q[2][2][BM * D];         // two items, two halves
   __half kv[kStages][2][BN * D];  // K, V
+  float scale[kLoadWarps][2][D];  // int8: the head's scales, a copy per converting warp
   uint64_t q_full[2], q_free[2];
   uint64_t kv_full[kStages], kv_empty[kStages];
   uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];
@@ -624,29 +625,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       };
-      auto convert = [&](int st, int pool, int head) {
+      auto convert = [&](int st, int pool) {
         char* dst = reinterpret_cast<char*>(s.kv[st][pool]) + key * 128;
-        const float4* scale = reinterpret_cast<const float4*>(
-            (pool ? a.kv.v_scale : a.kv.k_scale) + (a.kv.per_channel ? head * D : 0));
+        const float4* scale = reinterpret_cast<const float4*>(s.scale[warp - kLoadWarp0][pool]);
 #pragma unroll
         for (int w = 0; w < 8; ++w) {
           uint4 x;
           if constexpr (KVF == kKvQ4) {
             x = q4_piece(raw[pool][w], raw[pool][8]);
           } else {
-            float sc[8];
-            if (a.kv.per_channel && (reinterpret_cast<uintptr_t>(scale) & 15u) != 0) {
-#pragma unroll
-              for (int k = 0; k < 8; ++k) sc[k] = reinterpret_cast<const float*>(scale)[8 * w + k];
-            } else if (a.kv.per_channel) {
-              const float4 a4 = scale[2 * w], b4 = scale[2 * w + 1];
-              sc[0] = a4.x, sc[1] = a4.y, sc[2] = a4.z, sc[3] = a4.w;
-              sc[4] = b4.x, sc[5] = b4.y, sc[6] = b4.z, sc[7] = b4.w;
-            } else {
-              const float one = *reinterpret_cast<const float*>(scale);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) sc[k] = one;
-            }
+            const float4 lo = scale[2 * w], hi = scale[2 * w + 1];
+            const float sc[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
             uint32_t h[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -663,20 +652,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       place();
       load(0);
       load(1);
-      int head = kh, st = 0;
+      int head = -1, next_head = kh, st = 0;
       uint32_t ph = 1;
       for (int c = 0; more; ++c) {
         bool ok = true;
         if (lane == 0 && c >= kStages) ok = wait_bar(s, &s.kv_empty[st], ph, a.err);
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         if (!ok) break;
+        if (KVF == kKvI8 && next_head != head) {
+          __syncwarp();
+#pragma unroll
+          for (int pool = 0; pool < 2; ++pool)
+#pragma unroll
+            for (int d = lane; d < D; d += 32)
+              s.scale[warp - kLoadWarp0][pool][d] =
+                  (pool ? a.kv.v_scale
+                        : a.kv.k_scale)[a.kv.per_channel ? next_head * D + d : 0];
+          __syncwarp();
+        }
+        head = next_head;
         more = !ahead.done();
         if (more) place();
-        convert(st, 0, head);
+        convert(st, 0);
         if (more) load(0);
-        convert(st, 1, head);
+        convert(st, 1);
         if (more) load(1);
-        head = kh;
+        next_head = kh;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
