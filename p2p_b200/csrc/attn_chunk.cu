@@ -46,6 +46,7 @@ constexpr int kThreads = 512;
 constexpr int kMmaWarp = 8, kTmaWarp = 9, kLoadWarp0 = 12, kLoadWarps = 4;
 constexpr int kMarks = 16;
 constexpr int kSetup = 2;
+constexpr int kMinUnits = 3;  // of a CTA: fewer make more records than they save time
 // setmaxnreg splits the 512 x 128 registers of the launch: 256 x 176 + 256 x 80
 constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kOtherRegs = 80;
 static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
@@ -304,7 +305,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (w == warp) upto += total;
     total += s.wsum[w];
   }
-  const int parts = int(min(static_cast<long long>(gridDim.x), total));
+  const int parts = int(min(static_cast<long long>(gridDim.x),
+                            (total + kMinUnits - 1) / kMinUnits));
   const int b = blockIdx.x;
   launch_dependents();
   if (tid == 0) a.joins[b] = make_int4(-1, 0, 0, 0);
@@ -881,9 +883,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // CTA (b, y): rows 32 y .. of the item that began in CTA b and went on in others.  Half a warp per
-// row (16 lanes of 4 dims), records in CTA order.
+// row (16 lanes of 4 dims), records in CTA order, eight of them in flight.
 constexpr int kJoinThreads = 256;
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(kJoinThreads, 4)
     join_chunk_kernel(const __grid_constant__ ChunkArgs a) {
   grid_dependency_wait();
   const int4 d = a.joins[blockIdx.x];
@@ -891,18 +893,16 @@ __global__ void __launch_bounds__(kJoinThreads)
   const int group = a.hq / a.kv.hkv, b = blockIdx.x, n = d.w >> 1, slot = d.w & 1;
   const SeqSpan sp = seq_span(a.kv, a.at, d.x);
   const Item it{d.x, d.y, d.z, sp.past, sp.row0, sp.len, group};
-  const int l16 = threadIdx.x & 15;
-#pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    const int r = blockIdx.y * 32 + pass * 16 + (threadIdx.x >> 4);
-    if (r >= it.rows()) return;
+  const int l16 = threadIdx.x & 15, end = min(it.rows(), int(blockIdx.y) * 32 + 32);
+#pragma unroll 1
+  for (int r = blockIdx.y * 32 + (threadIdx.x >> 4); r < end; r += 16) {
     auto rec = [&](int i) {
       return a.parts + ((int64_t(b + i) * 2 + (i == 0 ? slot : 0)) * kRows + r) * kRec;
     };
     float mx = -1e30f, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     bool bad = false;
-    for (int i0 = 0; i0 < n; i0 += 8) {  // eight records in flight
+    for (int i0 = 0; i0 < n; i0 += 8) {
       float2 ml[8];
       float4 x[8];
 #pragma unroll
@@ -915,13 +915,13 @@ __global__ void __launch_bounds__(kJoinThreads)
       for (int i = 0; i < 8; ++i) {
         if (i0 + i >= n) continue;
         bad |= ml[i].y < 0.f;
-        const float m = fmaxf(mx, ml[i].x), c = fast_exp2(mx - m), e = fast_exp2(ml[i].x - m);
+        const float m = fmaxf(mx, ml[i].x), c = fast_exp2(mx - m), w = fast_exp2(ml[i].x - m);
         mx = m;
-        l = fmaf(l, c, ml[i].y * e);
-        acc.x = fmaf(acc.x, c, x[i].x * e);
-        acc.y = fmaf(acc.y, c, x[i].y * e);
-        acc.z = fmaf(acc.z, c, x[i].z * e);
-        acc.w = fmaf(acc.w, c, x[i].w * e);
+        l = fmaf(l, c, ml[i].y * w);
+        acc.x = fmaf(acc.x, c, x[i].x * w);
+        acc.y = fmaf(acc.y, c, x[i].y * w);
+        acc.z = fmaf(acc.z, c, x[i].z * w);
+        acc.w = fmaf(acc.w, c, x[i].w * w);
       }
     }
     if (bad) continue;
