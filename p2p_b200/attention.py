@@ -556,6 +556,8 @@ class Context:
             g.ld_out = out.stride(0) if n > 1 else vocab
         if hist is not None:
             hs = hist.shape
+            if len(hs) == 2 and hs[1] == 0:
+                _refuse("hist: a capacity of at least one token needed")
             if hist.dtype is not torch.int32 or hist.get_device() != dev or len(hs) != 2 or \
                     hs[0] < n or hist.stride(1) != 1 and hs[1] > 1:
                 _refuse(f"hist: int32 [{n}][capacity] on device {dev} needed")
@@ -563,6 +565,8 @@ class Context:
             g.hist_cap = hs[1]
             g.ld_hist = hist.stride(0) if hs[0] > 1 else hs[1]
             g.hist_len = self._ints(hist_len, n, "hist_len")
+        elif hist_len is not None:
+            _refuse("hist_len without hist")
         if prompt_len is not None:
             g.prompt_len = self._ints(prompt_len, n, "prompt_len")
         if past is not None:

@@ -22,6 +22,11 @@
 //   S_w = Q_w K^T (M128 N128 K64) -> TMEM; P_w to TMEM as f16; O_w += P_w V (M128 N64 K128).
 // The softmax is that of the prompt kernel: exp2 with the scale folded in, partly by a cubic on the
 // FMA pipe, lazily rescaled (only when a row's maximum grows by 2^8).
+//   A key that a row may not see has weight 0, but 0 * inf and 0 * NaN are NaN: a token whose V
+// overflowed would reach the tokens in front of it in its tile.  A row whose sums are not finite
+// though it does not see all keys of its tiles is looked at again when the CTA's parts are done,
+// and worked out key by key if such a V is the cause.  (Looking through those tiles of V before they
+// are multiplied cost 4 prompts of 4096 tokens 384 -> 479 us; this costs nothing that can be seen.)
 //
 // Every wait is bounded; one that gives up sets the error word, the other roles stop, the CTA frees
 // its TMEM and writes nothing more.
@@ -73,6 +78,7 @@ struct __align__(128) Smem {
   int4 part[8];  // of part i & 7, for the MMA warp: first and end key tile, the halves' tiles
   int part_tail[8];  // its item's keys
   volatile int bad[kMarks];  // of part i % kMarks of this CTA: some page was refused
+  volatile int odd;          // some row that does not see all keys of its tiles is not finite
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -113,6 +119,8 @@ struct Item {
   __device__ __forceinline__ int key_end() const {
     return past + tok0() + (rows() - 1) / group + 1;
   }
+  // keys that row r sees
+  __device__ __forceinline__ int key_lim(int r) const { return past + tok0() + r / group + 1; }
   __device__ __forceinline__ int tiles() const { return (key_end() + BN - 1) / BN; }
   __device__ __forceinline__ int tiles_of(int w) const { return (key_end(w) + BN - 1) / BN; }
 };
@@ -249,6 +257,93 @@ __device__ __forceinline__ float2 s8_pair(uint32_t w, int k) {
       __hsub2(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(1152.f, 1152.f)));
 }
 
+// The maximum of three, NaN when one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Dims 8 i .. 8 i + 7 of a cached row as the MMAs see them.
+__device__ __forceinline__ void cached_piece(const KvView& kv, int pool, int64_t row, int kh, int i,
+                                             float (&x)[8]) {
+  const unsigned char* src = (pool ? kv.v : kv.k) + row * kv.row_bytes;
+  uint4 h;
+  if (kv.format == kKvF16) {
+    h = reinterpret_cast<const uint4*>(src + kh * 128)[i];
+  } else if (kv.format == kKvQ4) {
+    const uint32_t* unit = reinterpret_cast<const uint32_t*>(src + kh * kQ4UnitBytes);
+    h = q4_piece(unit[i], unit[8]);
+  } else {
+    const float* sc = pool ? kv.v_scale : kv.k_scale;
+    float v[8];
+    for (int k = 0; k < 8; ++k)
+      v[k] = float(reinterpret_cast<const int8_t*>(src)[kh * D + 8 * i + k]) *
+             sc[kv.per_channel ? kh * D + 8 * i + k : 0];
+    h = make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]),
+                   pack_half2(v[6], v[7]));
+  }
+  const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+    x[2 * k] = f.x;
+    x[2 * k + 1] = f.y;
+  }
+}
+
+// Row r of an item over the keys k0 .. k1 - 1 of its tiles, of which it sees those below its limit:
+// if a V behind the limit is not finite, the row is worked out again without it, into the f16
+// output or the f32 record that the calling thread wrote before.
+__device__ __noinline__ void redo_row(const ChunkArgs& a, const Item& it, int r, int k0, int k1,
+                                      __half* out, float* rec) {
+  const int lim = min(k1, it.key_lim(r));
+  float x[8], acc[D], m = -INFINITY, l = 0.f;
+  bool odd = false;
+  for (int key = max(k0, it.key_lim(r)); key < k1; ++key) {
+    const int64_t row = kv_row(a.kv, it.z, key);
+    if (row < 0) return;  // refused: the row was not written
+    for (int i = 0; i < 8; ++i) {
+      cached_piece(a.kv, 1, row, it.kh, i, x);
+      for (int k = 0; k < 8; ++k) odd |= !(fabsf(x[k]) < INFINITY);
+    }
+  }
+  if (!odd) return;
+  const __half* q = a.q + (int64_t(it.row0) + it.tok0() + r / it.group) * a.ld_q +
+                    (it.kh * it.group + r % it.group) * D;
+  for (int d = 0; d < D; ++d) acc[d] = 0.f;
+  for (int key = k0; key < lim; ++key) {
+    const int64_t row = kv_row(a.kv, it.z, key);
+    if (row < 0) return;
+    float sc = 0.f;
+    for (int i = 0; i < 8; ++i) {
+      cached_piece(a.kv, 0, row, it.kh, i, x);
+      for (int k = 0; k < 8; ++k) sc = fmaf(__half2float(q[8 * i + k]), x[k], sc);
+    }
+    sc *= a.scale_log2;
+    if (sc == -INFINITY) continue;
+    if (sc > m) {
+      const float c = fast_exp2(m - sc);
+      m = sc;
+      l *= c;
+      for (int d = 0; d < D; ++d) acc[d] *= c;
+    }
+    const float p = fast_exp2(sc - m);
+    l += p;
+    for (int i = 0; i < 8; ++i) {
+      cached_piece(a.kv, 1, row, it.kh, i, x);
+      for (int k = 0; k < 8; ++k) acc[8 * i + k] = fmaf(p, x[k], acc[8 * i + k]);
+    }
+  }
+  if (out) {
+    const float inv = __fdiv_rn(1.0f, l);
+    for (int d = 0; d < D; ++d) out[d] = __float2half_rn(acc[d] * inv);
+  } else {
+    for (int d = 0; d < D; ++d) rec[d] = acc[d];
+    rec[D] = m == -INFINITY ? -1e30f : m;
+    rec[D + 1] = l;
+  }
+}
+
 template <int KVF>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_chunk_kernel(const __grid_constant__ CUtensorMap tm_q,
@@ -296,6 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s.o_free[i], 4);
     }
     for (int i = 0; i < kMarks; ++i) s.bad[i] = 0;
+    s.odd = 0;
     s.abort_flag = 0;
     fence_barrier_init();
   }
@@ -709,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int seg = walk.seg, nk = walk.nk, k0 = walk.k0, k1 = walk.k1;
       const int rows = it.rows_of(w), mine_end = min(k1, it.tiles_of(w));
       if (rows == 0) continue;
-      const int first_lim = it.past + it.tok0() + BM * w / group + 1;  // keys the first row sees
+      const int first_lim = it.key_lim(BM * w);  // keys the first row sees
       const int key_lim = first_lim + r / group;
       float m_raw = -INFINITY, l_run = 0.f;
       for (int j = k0; j < mine_end; ++j, ++n) {
@@ -739,13 +835,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int i = 0; i < 32; i += 2)
-            m4[(i >> 1) & 3] = fmax3(m4[(i >> 1) & 3], __uint_as_float(sv[q][i]),
-                                     __uint_as_float(sv[q][i + 1]));
-        const float mx = fmax3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
+            m4[(i >> 1) & 3] = max3_nan(m4[(i >> 1) & 3], __uint_as_float(sv[q][i]),
+                                        __uint_as_float(sv[q][i + 1]));
+        const float mx = max3_nan(m4[0], max3_nan(m4[1], m4[1], m4[2]), m4[3]);
         const bool grow = (mx - m_raw) * sl2 > kRescaleLog2;
         const float alpha = grow ? fast_exp2((m_raw - mx) * sl2) : 1.0f;
         if (grow) m_raw = mx;
-        const float neg = (m_raw == -INFINITY) ? 0.f : -m_raw * sl2;
+        // a NaN score makes all of the row's weights NaN (the cubic alone would lose it)
+        const float neg = mx != mx ? mx : (m_raw == -INFINITY) ? 0.f : -m_raw * sl2;
         uint32_t pk[2][32];
 #pragma unroll
         for (int half = 0; half < 2; ++half)
@@ -816,6 +913,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.o_free[w]);
+        if (mine_end * BN > first_lim) {  // some row does not see all keys of its tiles
+          float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 64; ++i) t[i & 3] += __uint_as_float(ov[i >> 5][i & 31]);
+          const float sum = (t[0] + t[1]) + (t[2] + t[3]);
+          if (!(fabsf(sum) < INFINITY) && r < rows) s.odd = 1;
+        }
       } else {  // this half's keys all lie in other CTAs' parts
 #pragma unroll
         for (int i = 0; i < 32; ++i) ov[0][i] = ov[1][i] = 0u;
@@ -870,6 +974,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         float* rec = a.parts + ((int64_t(b) * 2 + (i == 0 ? 0 : 1)) * kRows + BM * w + r) * kRec;
         rec[64] = -1e30f;
         rec[65] = -1.f;
+      }
+    } else if (s.odd) {
+      PartWalk again(a.kv, a.at, group, s);
+      for (; again.live; again.next()) {
+        const Item it = again.it();
+        const int row = BM * w + r, first = again.k0 * BN;
+        const int end = min(min(again.k1, it.tiles_of(w)) * BN, it.key_end());
+        if (row >= it.rows() || end <= it.key_lim(row) || end <= first) continue;
+        const bool whole = again.k0 == 0 && again.k1 == again.nk;
+        __half* out = a.out + (int64_t(it.row0) + it.tok0() + row / group) * a.ld_o +
+                      (it.kh * group + row % group) * D;
+        float* rec = a.parts +
+                     ((int64_t(b) * 2 + (again.seg == 0 ? 0 : 1)) * kRows + row) * kRec;
+        bool finite = true;
+        for (int d = 0; d < D; ++d)
+          finite = finite && fabsf(whole ? __half2float(out[d]) : rec[d]) < INFINITY;
+        if (finite || (!whole && rec[D + 1] < 0.f)) continue;  // < 0: a page was refused
+        redo_row(a, it, row, first, end, whole ? out : nullptr, rec);
       }
     }
   }

@@ -103,10 +103,14 @@ __global__ void __launch_bounds__(kThreads)
   for (int k = 0; k < kAhead; ++k)
     if (t + k * kThreads < pieces) ahead[k].w = body[t + k * kThreads];
 
+  // Another CTA's shared memory is not touched before that CTA runs: everyone reports here and waits
+  // in front of the first access.
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+
   // ... and everything else the CTA is going to look at is asked for now, before any of it is
   // needed: the row's history (short ones whole; what lies behind its length is dropped later), the
   // first of its biases, the slice's mask words
-  const bool remote = a.hist_cap > kLocalHist;
+  const bool remote = a.hist != nullptr && a.hist_cap > kLocalHist;
   const int32_t* hist = a.hist + int64_t(i) * a.ld_hist;
   constexpr int kHist = kLocalHist / kThreads;
   int early[kHist];
@@ -140,8 +144,12 @@ __global__ void __launch_bounds__(kThreads)
     for (int k = t; k < (slice + slice / 32) / 4; k += kThreads)
       reinterpret_cast<uint4*>(cnt)[k] = make_uint4(0, 0, 0, 0);
     if (t == 0) n_list = 0;
-    if (remote) cl.sync();
-    else __syncthreads();
+    if (remote) {
+      asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+      cl.sync();  // the counts are clear
+    } else {
+      __syncthreads();
+    }
     if (remote) {
       for (int k = rank * kThreads + t; k < len; k += csize * kThreads) {
         const int v = hist[k];
@@ -309,6 +317,7 @@ __global__ void __launch_bounds__(kThreads)
     warp_y[warp] = best;
     warp_v[warp] = best_v;
   }
+  if (!remote) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   __syncthreads();
   if (t == 0) {
 #pragma unroll

@@ -86,6 +86,8 @@ p2p_status make_kv_view(p2p_ctx* ctx, const p2p_kv_layout* lay, int32_t hkv, con
       return fail(ctx, P2P_ERR_INVALID_ARG,
                   "%s: int8 caches need k/v scales, 1 or %d of them (got %d)", who, chan,
                   lay->scale_count);
+    if (!aligned(lay->k_scale, 4) || !aligned(lay->v_scale, 4))
+      return fail(ctx, P2P_ERR_INVALID_ARG, "%s: scales not aligned to their type", who);
     c.k_scale = lay->k_scale;
     c.v_scale = lay->v_scale;
     c.per_channel = lay->scale_count > 1 ? 1 : 0;
@@ -284,7 +286,7 @@ p2p_status p2p_logits_pick(p2p_ctx* ctx, const p2p_logits* args, void* stream) {
                 g.hist_cap, (long long)g.ld_hist);
   if (!g.hist && (g.hist_len || g.prompt_len))
     return fail(ctx, P2P_ERR_INVALID_ARG, "logits_pick: hist_len or prompt_len without hist");
-  if (g.bias_start && (!g.bias_tok || !g.bias_val || g.n_bias < 0))
+  if (g.bias_start && (g.n_bias < 0 || (g.n_bias > 0 && (!g.bias_tok || !g.bias_val))))
     return fail(ctx, P2P_ERR_INVALID_ARG, "logits_pick: bias_start needs bias_tok and bias_val");
   if (g.mask && g.ld_mask < (int64_t(g.vocab) + 31) / 32)
     return fail(ctx, P2P_ERR_INVALID_ARG, "logits_pick: ld_mask %lld for vocab %d",
@@ -308,7 +310,7 @@ p2p_status p2p_logits_pick(p2p_ctx* ctx, const p2p_logits* args, void* stream) {
   a.repetition = g.repetition;
   a.presence = g.presence;
   a.frequency = g.frequency;
-  a.bias_start = g.bias_start;
+  a.bias_start = g.n_bias > 0 ? g.bias_start : nullptr;
   a.bias_tok = g.bias_tok;
   a.bias_val = g.bias_val;
   a.mask = g.mask;

@@ -445,6 +445,66 @@ def test_rows_behind_a_sequence_do_not_reach_it(ctx):
         assert_within(out, want, tol)
 
 
+@pytest.mark.parametrize("fmt", ["f16", "q4"])
+@pytest.mark.parametrize("page", [0, 16, 256])
+@pytest.mark.parametrize("case", [
+    # heads, past, rows, the tokens whose V overflowed (sequence, row of the chunk)
+    ((32, 8), [0, 130, 40], [70, 5, 300], [(0, 69), (1, 3), (2, 100), (2, 101), (2, 270)]),
+    ((16, 16), [500], [400], [(0, 0), (0, 255), (0, 256), (0, 399)]),
+    ((8, 1), [5000], [33], [(0, 17)]),
+    # more items than the equal parts are for: a CTA each
+    ((64, 8), [3, 0], [2400, 77], [(0, 1200), (0, 2399), (1, 40)]),
+], ids=lambda c: f"{c[0]}-{len(c[2])}x{max(c[2])}")
+def test_values_that_overflowed_reach_no_earlier_token(ctx, fmt, page, case):
+    """A token's infinite or NaN K and V: the rows in front of it are as without (within the bound
+    of a chunk), those that see an infinity of V get it in its dims (f16: dim 3 inf, dim 10 NaN,
+    the rest as without; 4 bits: the whole head), and those that see a NaN K are NaN."""
+    (hq, hkv), past, rows, odd = case
+    c = Cache(35, fmt, page, hq, hkv, [p + r for p, r in zip(past, rows)])
+    n = sum(rows)
+    q, first = randh(gen(36), n, hq * D), [sum(rows[:i]) for i in range(len(rows))]
+
+    want, tol = (t.view(n, hq, D) for t in attention64(c, q, past, rows, True))
+
+    def check(what):
+        out = torch.full_like(q, math.nan)
+        ctx.attn_chunk_kv(c.prm, q, c.k, c.v, i32(past), starts_of(rows), out, max_len=6000,
+                          **c.kw())
+        ctx.sync()
+        got = out.view(n, hq, D)
+        live = want.isfinite()
+        assert same_bits(got.double()[~live], want[~live]), what
+        assert_within(got[live], want[live], tol[live], what)
+    check("clean")
+    grp, last = hq // hkv, hkv - 1
+    for i, r in odd:
+        at = tuple(x if torch.is_tensor(x) and x.dim() == 0 else torch.as_tensor(x, device="cuda")
+                   for x in c.at(i, past[i] + r))
+        sees = want[first[i] + r:first[i] + rows[i]]
+        if fmt == "f16":
+            c.v[(*at, 0, 3)], c.v[(*at, 0, 10)] = math.inf, math.nan
+            sees[:, :grp, 3], sees[:, :grp, 10] = math.inf, math.nan
+            c.v[(*at, last, 63)] = -math.inf
+            sees[:, last * grp:, 63] = -math.inf
+        else:
+            unit = c.v[at]
+            unit[34:36] = torch.tensor([math.inf], dtype=torch.float16,
+                                       device="cuda").view(torch.uint8)
+            c.v[at] = unit
+            sees[:, :grp] = math.inf
+    check("V")
+    i, r = odd[-1]
+    at = tuple(torch.as_tensor(x, device="cuda") for x in c.at(i, past[i] + r))
+    row = c.k[at]
+    if fmt == "f16":
+        row[0] = math.nan
+    else:
+        row[32:34] = torch.tensor([math.nan], dtype=torch.float16, device="cuda").view(torch.uint8)
+    c.k[at] = row
+    want[first[i] + r:first[i] + rows[i], :grp] = math.nan
+    check("K")
+
+
 # ---- refusals on the device -------------------------------------------------------------------------
 @pytest.mark.parametrize("op", ["append", "read", "chunk", "decode", "fused"])
 @pytest.mark.parametrize("page", [0, 16])
@@ -626,6 +686,9 @@ LOGITS = [
     (1, 1000, 100, 0, False), (5, 1025, 300, 20, True), (4, 4099, 1000, 300, True),
     (3, 65536, 2000, 50, True), (2, 131071, 4000, 10, True), (1, 262144, 50, 0, True),
     (70, 513, 40, 4, True), (1, 400000, 10, 5, True),
+    # long histories; more biases than threads
+    (2, 900, 4097, 2000, True), (3, 65536, 9000, 700, True), (2, 131071, 20000, 5000, False),
+    (1, 262144, 5000, 0, False), (1, 400000, 4097, 1, True), (2, 30, 6000, 600, False),
 ]
 
 
@@ -688,6 +751,17 @@ def test_logits_pick(ctx, dt, case):
         ctx.sync()
         assert tok2.tolist()[:n] == toks and same_bits(x, want)
         assert torch.equal(wide[:, vocab:], keep[:, vocab:])
+
+
+def test_logits_empty_lists(ctx):
+    x, tok = randh(gen(8), 2, 300), torch.zeros(2, dtype=torch.int32, device="cuda")
+    none, f = i32([]), torch.zeros(0, device="cuda")
+    out = torch.zeros_like(x)
+    ctx.logits_pick(x, tok, out=out, bias_start=i32([0, 0, 0]), bias_tok=none, bias_val=f)
+    ctx.logits_pick(x[:0], tok)
+    ctx.sync()
+    assert torch.equal(out, x)
+    assert tok.tolist() == [int(np.argmax(r)) for r in x.float().cpu().numpy()]
 
 
 def test_logits_without_anything_is_argmax(ctx):
@@ -772,6 +846,8 @@ def test_logits_refusals(ctx):
     refused(x, tok, out=x[:, :50])
     refused(x, tok, out=x.float())
     refused(x, tok, hist=h)
+    refused(x, tok, hist_len=tok)
+    refused(x, tok, hist=h[:, :0], hist_len=tok)
     refused(x, tok, prompt_len=tok)
     refused(x, tok, repetition=f.half())
     refused(x, tok, presence=f[:1])
@@ -914,6 +990,46 @@ def test_two_graphs_of_different_sizes_share_a_context(ctx, op):
             want, tol = attention64(c, q, past, [1] * len(past), op == "chunk")
             assert_within(out, want, tol)
     graphs.clear()
+
+
+@pytest.mark.parametrize("op", ["decode", "chunk"])
+def test_the_workspace_is_made_outside_captures_and_may_not_fit(op):
+    import p2p_b200
+    past = [300, 20]
+    c = Cache(63, "q4", 16, 16, 4, [p + 1 for p in past])
+    q = randh(gen(64), 2, 16 * D)
+    out = torch.full_like(q, 7.0)
+    p, rs = i32(past), i32([0, 1, 2])
+    fresh = p2p_b200.Context(0)
+    try:
+        def call():
+            if op == "decode":
+                fresh.attn_decode_kv(c.prm, q, None, None, c.k, c.v, p, out, max_past=300,
+                                     fused_prep=False, **c.kw())
+            else:
+                fresh.attn_chunk_kv(c.prm, q, c.k, c.v, p, rs, out, max_len=301, **c.kw())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out.fill_(7.0)
+            with pytest.raises(p2p_b200.P2PError) as e:
+                call()
+        assert e.value.status == p2p_b200.P2P_ERR_INVALID_ARG
+        g.replay()
+        torch.cuda.synchronize()
+        assert (out == 7).all()
+        try:
+            p2p_b200.lib.p2p_debug_set_alloc_limit(0)
+            with pytest.raises(p2p_b200.P2PError) as e:
+                call()
+            assert e.value.status == p2p_b200.P2P_ERR_OOM
+        finally:
+            p2p_b200.lib.p2p_debug_set_alloc_limit(-1)
+        call()
+        fresh.sync()
+        want, tol = attention64(c, q, past, [1, 1], op == "chunk")
+        assert_within(out, want, tol)
+    finally:
+        fresh.close()
 
 
 @pytest.mark.parametrize("op", ["decode", "chunk"])
