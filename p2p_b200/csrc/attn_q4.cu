@@ -129,6 +129,10 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 }
 
 constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;  // nibbles 0, 4 and 1, 5 of a word
+// V's codes sit two bits higher, c * 2^-22 and c * 2^-18: measured, the sums of the lower nibbles were
+// off by 16 times as much as those of the higher ones (a subnormal seems to be aligned by the smallest
+// exponent, not by its leading bit), and two bits up leave nothing that can be seen.
+constexpr uint32_t kLow = kEven << 2, kHigh = kOdd << 2;
 
 // Query heads per lane.  Up to four heads, head t sits in lane column 2t of the fragments' eight and
 // column 2t + 1 is free: it takes no score, so that a lane's softmax works on one head instead of
@@ -277,6 +281,11 @@ __device__ __forceinline__ void attend(const unsigned char* ks, const unsigned c
     }
     st.fresh = false;
   }
+  // A block's products are summed apart and then added: the MMA truncates what it adds to its
+  // accumulators, and codes are never negative, so over thousands of keys the losses of a running sum
+  // would all go one way (4 x 131071 keys: 6.5e-4 of the outputs' norm from
+  // the exact ones; summed apart 2.1e-4, which is the rounding to f16).
+  float o[4][4] = {};
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     // weights of keys row and row + 8 of this half, scaled by the keys' value scales: columns 2t
@@ -311,13 +320,15 @@ __device__ __forceinline__ void attend(const unsigned char* ks, const unsigned c
     // pairs of keys: codes 0..3 of both words, then codes 4..7
     const uint32_t x = __byte_perm(w0, w1, 0x5410), y = __byte_perm(w0, w1, 0x7632);
     const uint32_t x2 = __byte_perm(w2, w3, 0x5410), y2 = __byte_perm(w2, w3, 0x7632);
-    mma16816(st.o[0], x & kEven, x & kOdd, x2 & kEven, x2 & kOdd, b0, b1);
-    mma16816(st.o[1], (x >> 8) & kEven, (x >> 8) & kOdd, (x2 >> 8) & kEven, (x2 >> 8) & kOdd, b0,
-             b1);
-    mma16816(st.o[2], y & kEven, y & kOdd, y2 & kEven, y2 & kOdd, b0, b1);
-    mma16816(st.o[3], (y >> 8) & kEven, (y >> 8) & kOdd, (y2 >> 8) & kEven, (y2 >> 8) & kOdd, b0,
-             b1);
+    mma16816(o[0], (x << 2) & kLow, (x << 2) & kHigh, (x2 << 2) & kLow, (x2 << 2) & kHigh, b0, b1);
+    mma16816(o[1], (x >> 6) & kLow, (x >> 6) & kHigh, (x2 >> 6) & kLow, (x2 >> 6) & kHigh, b0, b1);
+    mma16816(o[2], (y << 2) & kLow, (y << 2) & kHigh, (y2 << 2) & kLow, (y2 << 2) & kHigh, b0, b1);
+    mma16816(o[3], (y >> 6) & kLow, (y >> 6) & kHigh, (y2 >> 6) & kLow, (y2 >> 6) & kHigh, b0, b1);
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) st.o[i][k] += o[i][k];
 }
 
 // A warp's part of one head's G query heads as a record [G][acc[64] | max | sum]: from the
@@ -841,8 +852,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int k = 0; k < 4; ++k) {
         const float even = H == 2 ? state.o[k][e] : state.o[k][0] + state.o[k][1];
         const float odd = H == 2 ? state.o[k][2 + e] : state.o[k][2] + state.o[k][3];
-        acc[e][2 * k] = fmaf(even, 16777216.f, state.bias[e]);     // 2^24
-        acc[e][2 * k + 1] = fmaf(odd, 1048576.f, state.bias[e]);   // 2^20
+        acc[e][2 * k] = fmaf(even, 4194304.f, state.bias[e]);     // 2^22
+        acc[e][2 * k + 1] = fmaf(odd, 262144.f, state.bias[e]);   // 2^18
       }
     }
     end_part(acc, mx, sum, z, g0, tiles, segs == 0);
