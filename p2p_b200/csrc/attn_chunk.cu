@@ -20,13 +20,13 @@
 // per row took three times the instructions), and its page's number is loaded two tiles early and
 // its words one, into registers.
 //   S_w = Q_w K^T (M128 N128 K64) -> TMEM; P_w to TMEM as f16; O_w += P_w V (M128 N64 K128).
-// The softmax is that of the prompt kernel: exp2 with the scale folded in, partly by a cubic on the
-// FMA pipe, lazily rescaled (only when a row's maximum grows by 2^8).
+// The softmax: exp2 with the scale folded in, lazily rescaled (only when a row's maximum grows by
+// 2^8).
 //   A key that a row may not see has weight 0, but 0 * inf and 0 * NaN are NaN: a token whose V
 // overflowed would reach the tokens in front of it in its tile.  A row whose sums are not finite
 // though it does not see all keys of its tiles is looked at again when the CTA's parts are done,
 // and worked out key by key if such a V is the cause.  (Looking through those tiles of V before they
-// are multiplied cost 4 prompts of 4096 tokens 384 -> 479 us; this costs nothing that can be seen.)
+// are multiplied cost 4 prompts of 4096 tokens 384 -> 479 us, this 384 -> 389.)
 //
 // Every wait is bounded; one that gives up sets the error word, the other roles stop, the CTA frees
 // its TMEM and writes nothing more.
@@ -59,7 +59,13 @@ constexpr int kStages = 4;  // K/V tiles in flight
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 constexpr float kRescaleLog2 = 8.0f;
-constexpr int kPolyPairs = 5;  // of every 16 exp pairs, these use the cubic
+// Every fourth pair of exponentials is a cubic on the FMA pipe, over f16 caches (4096 rows over 28000
+// keys: 1507 us, 1670 with none; the first 5 of 16 pairs in a row: 1628).  Over int8 and 4-bit caches
+// the converting warps need that pipe's issue slots: none (4 bits: 1804 us, 1818 with a fourth; 16
+// sequences of 5 rows over up to 4096 keys: 42.6 us, 45.3).  The others are f32 exponentials rounded
+// once; packed f16 ones round their argument (errors of up to 2^-9 of a weight) and took as long.
+template <int KVF>
+constexpr bool kCubic = KVF == kKvF16;
 constexpr int kRec = 68;       // a record's row: acc[64], max, sum, 2 pad
 
 __device__ __forceinline__ uint32_t col_s(int w) { return uint32_t(w) * 256u; }
@@ -854,7 +860,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               float x0, x1;
               fma2(__uint_as_float(sv[q][2 * i]), __uint_as_float(sv[q][2 * i + 1]), sl2, neg, x0,
                    x1);
-              pk[half][cc * 16 + i] = i < kPolyPairs ? ex2_poly_f16x2(x0, x1) : ex2_f16x2(x0, x1);
+              pk[half][cc * 16 + i] = kCubic<KVF> && (i & 3) == 0
+                                          ? ex2_poly_f16x2(x0, x1)
+                                          : pack_half2(fast_exp2(x0), fast_exp2(x1));
             }
           }
         float ps[4] = {0.f, 0.f, 0.f, 0.f};
