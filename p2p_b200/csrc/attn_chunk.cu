@@ -34,6 +34,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -47,37 +48,53 @@ using namespace sm100;
 
 constexpr int BM = 128, BN = 128, D = kHeadDim;
 constexpr int kRows = 2 * BM;  // rows of an item
-constexpr int kThreads = 512;
 constexpr int kMmaWarp = 8, kTmaWarp = 9, kLoadWarp0 = 12, kLoadWarps = 4;
 constexpr int kMarks = 16;
 constexpr int kSetup = 2;
 constexpr int kMinUnits = 3;  // of a CTA: fewer make more records than they save time
-// setmaxnreg splits the 512 x 128 registers of the launch: 256 x 176 + 256 x 80
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kOtherRegs = 80;
-static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
-constexpr int kStages = 4;  // K/V tiles in flight
+constexpr int kMaxStages = 4;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 constexpr float kRescaleLog2 = 8.0f;
-// Every fourth pair of exponentials is a cubic on the FMA pipe, over f16 caches (4096 rows over 28000
-// keys: 1507 us, 1670 with none; the first 5 of 16 pairs in a row: 1628).  Over int8 and 4-bit caches
-// the converting warps need that pipe's issue slots: none (4 bits: 1804 us, 1818 with a fourth; 16
-// sequences of 5 rows over up to 4096 keys: 42.6 us, 45.3).  The others are f32 exponentials rounded
-// once; packed f16 ones round their argument (errors of up to 2^-9 of a weight) and took as long.
+// What differs by the cache's format.
+// kMoveF16: f16 tiles only move.  Nothing but the softmax asks for issue slots then: every fourth pair of
+//   exponentials is a cubic on the FMA pipe and the row sums are taken in f32 (4096 rows over 28000 keys:
+//   1450 us; with f16 pair sums 1507, without the cubic 1670).  The converting warps of the other formats
+//   need the slots: no cubic, and the rounded weights are summed in f16 by fours (4 bits: 1800 us; with
+//   f32 sums and the cubic 2377).  The exponentials are f32 ones rounded once; packed f16 ones round their
+//   argument (errors of up to 2^-9 of a weight) and took as long.
+// kStages: K/V tiles in flight.  3 leave more of the SM to the L1 cache (4 prompts of up to 4096 tokens:
+//   350 us, 368 with 4); converting warps want 4 (4 bits: 1800 us, 2589 with 3).
+// Registers: setmaxnreg splits what the launch gives (kThreads x kLaunchRegs) among the two softmax
+//   warpgroups, that of the issuing warps and that of the converting ones.  The f16 kernel has no converting
+//   warps and gives theirs to the others (4 prompts: 350 -> 335 us).  Converting int8 rows in 80 registers
+//   spilled in its loop (512 rows over 32000 keys: 490 us; 280 with 96).
 template <int KVF>
-constexpr bool kCubic = KVF == kKvF16;
+struct Conf {
+  static constexpr bool kMoveF16 = KVF == kKvF16;
+  static constexpr int kStages = kMoveF16 ? 3 : 4;
+  static constexpr int kThreads = kMoveF16 ? 384 : 512, kLaunchRegs = kMoveF16 ? 168 : 128;
+  static constexpr int kSoftmaxRegs = kMoveF16 ? 184 : 176,
+                       kIssueRegs = kMoveF16 ? 136 : KVF == kKvI8 ? 64 : 80,
+                       kLoadRegs = kMoveF16 ? 0 : KVF == kKvI8 ? 96 : 80;
+  static_assert(256 * kSoftmaxRegs + 128 * (kIssueRegs + kLoadRegs) <= kThreads * kLaunchRegs,
+                "register split");
+};
 constexpr int kRec = 68;       // a record's row: acc[64], max, sum, 2 pad
 
 __device__ __forceinline__ uint32_t col_s(int w) { return uint32_t(w) * 256u; }
 __device__ __forceinline__ uint32_t col_p(int w) { return uint32_t(w) * 256u + 128u; }
 __device__ __forceinline__ uint32_t col_o(int w) { return uint32_t(w) * 256u + 192u; }
 
+template <int S>
+struct __align__(1024) Tiles {
+  __half q[2][2][BM * D];   // two items, two halves
+  __half kv[S][2][BN * D];  // K, V
+};
 struct __align__(128) Smem {
-  __half q[2][2][BM * D];         // two items, two halves
-  __half kv[kStages][2][BN * D];  // K, V
   float scale[kLoadWarps][2][D];  // int8: the head's scales, a copy per converting warp
   uint64_t q_full[2], q_free[2];
-  uint64_t kv_full[kStages], kv_empty[kStages];
+  uint64_t kv_full[kMaxStages], kv_empty[kMaxStages];
   uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];
   long long wsum[8];
   int z0, qt0, kh0, off0, n_units;  // the first item of the CTA's part, and where in it
@@ -270,6 +287,18 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return r;
 }
 
+// acc += (a, b), a pair of f32 sums; and their total.
+__device__ __forceinline__ void add_pair(uint64_t& acc, float a, float b) {
+  uint64_t x;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(x));
+}
+__device__ __forceinline__ float pair_sum(uint64_t acc) {
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(acc));
+  return a + b;
+}
+
 // Dims 8 i .. 8 i + 7 of a cached row as the MMAs see them.
 __device__ __forceinline__ void cached_piece(const KvView& kv, int pool, int64_t row, int kh, int i,
                                              float (&x)[8]) {
@@ -351,14 +380,17 @@ __device__ __noinline__ void redo_row(const ChunkArgs& a, const Item& it, int r,
 }
 
 template <int KVF>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
     attn_chunk_kernel(const __grid_constant__ CUtensorMap tm_q,
                       const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ ChunkArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                     ~uintptr_t(1023));
+  constexpr int kStages = Conf<KVF>::kStages;
+  constexpr bool kMoveF16 = Conf<KVF>::kMoveF16;
+  auto& tiles = *reinterpret_cast<Tiles<kStages>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Smem& s = *reinterpret_cast<Smem*>(&tiles + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.hq / a.kv.hkv, gshift = __ffs(group) - 1;
 
@@ -450,16 +482,142 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = s.tmem_base;
   const int n_units = s.n_units;
 
-  if (warp >= 8) {
-    regs_dec<kOtherRegs>();
+  if (!kMoveF16 && warp >= kLoadWarp0) {
+    if constexpr (!kMoveF16) regs_dec<Conf<KVF>::kLoadRegs>();
+    // ---------------------------------------------------------------- converting warps
+    constexpr int kWords = KVF == kKvQ4 ? 9 : 16;  // of a head's row
+    const int key = tid - kLoadWarp0 * 32;
+    const bool paged = a.kv.table != nullptr;
+    // Three tiles in a line: `now` is converted, the words of `words` are on their way, and the
+    // page number of `ahead`.
+    TileStream ahead(a.kv, a.at, group, s);
+    int32_t page = 0;
+    auto find = [&] {
+      if (ahead.done()) return;
+      page = 0;
+      if (!paged) page = a.kv.offsets[ahead.it().z];
+      else if (key < ahead.valid())
+        page = a.kv.table[int64_t(ahead.it().z) * a.kv.max_blocks +
+                          ((ahead.jj * BN + key) >> a.kv.shift)];
+    };
+    uint32_t raw[2][kWords];
+    int64_t at = 0;        // byte offset of the head's row in either pool
+    bool there = false;    // the key exists
+    int kh = 0;
+    auto place = [&] {  // takes `ahead` over as the tile whose words are loaded
+      if (ahead.done()) return;
+      const int pos = ahead.jj * BN + key;
+      kh = ahead.it().kh;
+      there = key < ahead.valid();
+      int64_t row = int64_t(page) + pos;
+      if (paged) {
+        if (there && (page < 0 || int64_t(page) >= a.kv.kv_rows)) {
+          there = false;  // a page outside the pool is not read
+          s.bad[ahead.part.seg % kMarks] = 1;
+          atomicOr(a.err, kErrPosBeyondCache);
+        }
+        row = (int64_t(page) << a.kv.shift) | (pos & ((1 << a.kv.shift) - 1));
+      }
+      at = row * a.kv.row_bytes + kh * (KVF == kKvQ4 ? kQ4UnitBytes : D);
+      ahead.next();
+      find();
+    };
+    auto load = [&](int pool) {
+      const unsigned char* src = (pool ? a.kv.v : a.kv.k) + at;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) raw[pool][i] = 0u;  // rows behind the last key: zeros
+      if (!there) return;
+      if constexpr (KVF == kKvQ4) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+          raw[pool][i] = reinterpret_cast<const uint32_t*>(src)[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < kWords; i += 4) {
+          const uint4 x = reinterpret_cast<const uint4*>(src)[i / 4];
+          raw[pool][i] = x.x;
+          raw[pool][i + 1] = x.y;
+          raw[pool][i + 2] = x.z;
+          raw[pool][i + 3] = x.w;
+        }
+      }
+    };
+    auto convert = [&](int st, int pool) {
+      char* dst = reinterpret_cast<char*>(tiles.kv[st][pool]) + key * 128;
+      const float4* scale = reinterpret_cast<const float4*>(s.scale[warp - kLoadWarp0][pool]);
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        uint4 x;
+        if constexpr (KVF == kKvQ4) {
+          x = q4_piece(raw[pool][w], raw[pool][8]);
+        } else {
+          const float4 lo = scale[2 * w], hi = scale[2 * w + 1];
+          const float sc[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          uint32_t h[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 v = s8_pair(raw[pool][2 * w + (k >> 1)], k & 1);
+            h[k] = pack_half2(v.x * sc[2 * k], v.y * sc[2 * k + 1]);
+          }
+          x = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        *reinterpret_cast<uint4*>(dst + ((w ^ (key & 7)) << 4)) = x;
+      }
+    };
+    find();
+    bool more = !ahead.done();
+    place();
+    load(0);
+    load(1);
+    int head = -1, next_head = kh, st = 0;
+    uint32_t ph = 1;
+    for (int c = 0; more; ++c) {
+      bool ok = true;
+      if (lane == 0 && c >= kStages) ok = wait_bar(s, &s.kv_empty[st], ph, a.err);
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      if (!ok) break;
+      if (KVF == kKvI8 && next_head != head) {
+        __syncwarp();
+#pragma unroll
+        for (int pool = 0; pool < 2; ++pool)
+#pragma unroll
+          for (int d = lane; d < D; d += 32)
+            s.scale[warp - kLoadWarp0][pool][d] =
+                (pool ? a.kv.v_scale
+                      : a.kv.k_scale)[a.kv.per_channel ? next_head * D + d : 0];
+        __syncwarp();
+      }
+      head = next_head;
+      more = !ahead.done();
+      if (more) place();
+      convert(st, 0);
+      if (more) load(0);
+      convert(st, 1);
+      if (more) load(1);
+      next_head = kh;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (c == 0 && key == 0 && a.wait_deficit)
+          mbar_arrive_expect_tx(&s.kv_full[st], uint32_t(a.wait_deficit));
+        else
+          mbar_arrive(&s.kv_full[st]);
+      }
+      if (++st == kStages) {
+        st = 0;
+        ph ^= 1;
+      }
+    }
+  } else if (warp >= 8) {
+    regs_dec<Conf<KVF>::kIssueRegs>();
     if (warp == kMmaWarp) {
       // ---------------------------------------------------------------- MMA issuer
       constexpr uint32_t idesc_s = idesc_f16_f32(BM, BN, 0, 0);
       constexpr uint32_t idesc_pv = idesc_f16_f32(BM, D, 0, 1);
-      static_assert(sizeof(s.q[0]) == 32768 && sizeof(s.kv[0]) == 32768, "16 KB tiles");
-      const uint64_t qdesc0 = smem_desc_sw128(smem_u32(s.q[0][0]), 16, 1024);
-      const uint64_t kdesc0 = smem_desc_sw128(smem_u32(s.kv[0][0]), 16, 1024);
-      const uint64_t vdesc0 = smem_desc_sw128(smem_u32(s.kv[0][1]), 0, 1024);
+      static_assert(sizeof(tiles.q[0]) == 32768 && sizeof(tiles.kv[0]) == 32768, "16 KB tiles");
+      const uint64_t qdesc0 = smem_desc_sw128(smem_u32(tiles.q[0][0]), 16, 1024);
+      const uint64_t kdesc0 = smem_desc_sw128(smem_u32(tiles.kv[0][0]), 16, 1024);
+      const uint64_t vdesc0 = smem_desc_sw128(smem_u32(tiles.kv[0][1]), 0, 1024);
       uint32_t seg = 0;  // parts so far
       auto issue_s = [&](int w, int st) {  // S_w = Q_w K_st^T
         if (elect_one()) {
@@ -529,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int tail = s.part_tail[seg & 7] - jj * BN;
             if (KVF == kKvF16 && tail < BN) {
               // Rows behind the last key may hold anything; P is 0 there, but 0 * NaN is NaN
-              uint4* vrow = reinterpret_cast<uint4*>(s.kv[st][1]);
+              uint4* vrow = reinterpret_cast<uint4*>(tiles.kv[st][1]);
               for (int i = tail * 8 + lane; i < BN * 8; i += 32) vrow[i] = make_uint4(0, 0, 0, 0);
               fence_proxy_async_smem();
               __syncwarp();
@@ -605,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int halves = it.rows() > BM ? 2 : 1;
           mbar_arrive_expect_tx(&s.q_full[seg & 1], uint32_t(halves * BM * D * 2));
           for (int h = 0; h < halves; ++h)
-            tma_load_3d(s.q[seg & 1][h], &tm_q, 0, it.kh * group,
+            tma_load_3d(tiles.q[seg & 1][h], &tm_q, 0, it.kh * group,
                         it.row0 + it.tok0() + h * (BM >> gshift), &s.q_full[seg & 1]);
         }
         n_q = seg + 1;
@@ -649,9 +807,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
             if (!bad && lane < boxes) {
-              tma_load_2d(&s.kv[st][0][lane * box * D], &tm_k, it.kh * D, int32_t(row),
+              tma_load_2d(&tiles.kv[st][0][lane * box * D], &tm_k, it.kh * D, int32_t(row),
                           &s.kv_full[st]);
-              tma_load_2d(&s.kv[st][1][lane * box * D], &tm_v, it.kh * D, int32_t(row),
+              tma_load_2d(&tiles.kv[st][1][lane * box * D], &tm_v, it.kh * D, int32_t(row),
                           &s.kv_full[st]);
             }
           }
@@ -670,135 +828,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                  globaltimer_ns() - t0 < kWaitLimitNs) {
           }
       }
-    } else if (KVF != kKvF16 && warp >= kLoadWarp0) {
-      // ---------------------------------------------------------------- converting warps
-      constexpr int kWords = KVF == kKvQ4 ? 9 : 16;  // of a head's row
-      const int key = tid - kLoadWarp0 * 32;
-      const bool paged = a.kv.table != nullptr;
-      // Three tiles in a line: `now` is converted, the words of `words` are on their way, and the
-      // page number of `ahead`.
-      TileStream ahead(a.kv, a.at, group, s);
-      int32_t page = 0;
-      auto find = [&] {
-        if (ahead.done()) return;
-        page = 0;
-        if (!paged) page = a.kv.offsets[ahead.it().z];
-        else if (key < ahead.valid())
-          page = a.kv.table[int64_t(ahead.it().z) * a.kv.max_blocks +
-                            ((ahead.jj * BN + key) >> a.kv.shift)];
-      };
-      uint32_t raw[2][kWords];
-      int64_t at = 0;        // byte offset of the head's row in either pool
-      bool there = false;    // the key exists
-      int kh = 0;
-      auto place = [&] {  // takes `ahead` over as the tile whose words are loaded
-        if (ahead.done()) return;
-        const int pos = ahead.jj * BN + key;
-        kh = ahead.it().kh;
-        there = key < ahead.valid();
-        int64_t row = int64_t(page) + pos;
-        if (paged) {
-          if (there && (page < 0 || int64_t(page) >= a.kv.kv_rows)) {
-            there = false;  // a page outside the pool is not read
-            s.bad[ahead.part.seg % kMarks] = 1;
-            atomicOr(a.err, kErrPosBeyondCache);
-          }
-          row = (int64_t(page) << a.kv.shift) | (pos & ((1 << a.kv.shift) - 1));
-        }
-        at = row * a.kv.row_bytes + kh * (KVF == kKvQ4 ? kQ4UnitBytes : D);
-        ahead.next();
-        find();
-      };
-      auto load = [&](int pool) {
-        const unsigned char* src = (pool ? a.kv.v : a.kv.k) + at;
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) raw[pool][i] = 0u;  // rows behind the last key: zeros
-        if (!there) return;
-        if constexpr (KVF == kKvQ4) {
-#pragma unroll
-          for (int i = 0; i < kWords; ++i)
-            raw[pool][i] = reinterpret_cast<const uint32_t*>(src)[i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < kWords; i += 4) {
-            const uint4 x = reinterpret_cast<const uint4*>(src)[i / 4];
-            raw[pool][i] = x.x;
-            raw[pool][i + 1] = x.y;
-            raw[pool][i + 2] = x.z;
-            raw[pool][i + 3] = x.w;
-          }
-        }
-      };
-      auto convert = [&](int st, int pool) {
-        char* dst = reinterpret_cast<char*>(s.kv[st][pool]) + key * 128;
-        const float4* scale = reinterpret_cast<const float4*>(s.scale[warp - kLoadWarp0][pool]);
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          uint4 x;
-          if constexpr (KVF == kKvQ4) {
-            x = q4_piece(raw[pool][w], raw[pool][8]);
-          } else {
-            const float4 lo = scale[2 * w], hi = scale[2 * w + 1];
-            const float sc[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-            uint32_t h[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 v = s8_pair(raw[pool][2 * w + (k >> 1)], k & 1);
-              h[k] = pack_half2(v.x * sc[2 * k], v.y * sc[2 * k + 1]);
-            }
-            x = make_uint4(h[0], h[1], h[2], h[3]);
-          }
-          *reinterpret_cast<uint4*>(dst + ((w ^ (key & 7)) << 4)) = x;
-        }
-      };
-      find();
-      bool more = !ahead.done();
-      place();
-      load(0);
-      load(1);
-      int head = -1, next_head = kh, st = 0;
-      uint32_t ph = 1;
-      for (int c = 0; more; ++c) {
-        bool ok = true;
-        if (lane == 0 && c >= kStages) ok = wait_bar(s, &s.kv_empty[st], ph, a.err);
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        if (!ok) break;
-        if (KVF == kKvI8 && next_head != head) {
-          __syncwarp();
-#pragma unroll
-          for (int pool = 0; pool < 2; ++pool)
-#pragma unroll
-            for (int d = lane; d < D; d += 32)
-              s.scale[warp - kLoadWarp0][pool][d] =
-                  (pool ? a.kv.v_scale
-                        : a.kv.k_scale)[a.kv.per_channel ? next_head * D + d : 0];
-          __syncwarp();
-        }
-        head = next_head;
-        more = !ahead.done();
-        if (more) place();
-        convert(st, 0);
-        if (more) load(0);
-        convert(st, 1);
-        if (more) load(1);
-        next_head = kh;
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          if (c == 0 && key == 0 && a.wait_deficit)
-            mbar_arrive_expect_tx(&s.kv_full[st], uint32_t(a.wait_deficit));
-          else
-            mbar_arrive(&s.kv_full[st]);
-        }
-        if (++st == kStages) {
-          st = 0;
-          ph ^= 1;
-        }
-      }
     }
   } else {
     // ------------------------------------------------------------------ softmax warpgroups
-    regs_inc<kSoftmaxRegs>();
+    regs_inc<Conf<KVF>::kSoftmaxRegs>();
     const int w = warp >> 2;
     const int r = tid & 127;  // row of the half = TMEM lane
     const uint32_t lane_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
@@ -850,6 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // a NaN score makes all of the row's weights NaN (the cubic alone would lose it)
         const float neg = mx != mx ? mx : (m_raw == -INFINITY) ? 0.f : -m_raw * sl2;
         uint32_t pk[2][32];
+        uint64_t ps[4] = {0, 0, 0, 0};  // f32 pairs
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -860,20 +894,30 @@ __global__ void __launch_bounds__(kThreads, 1)
               float x0, x1;
               fma2(__uint_as_float(sv[q][2 * i]), __uint_as_float(sv[q][2 * i + 1]), sl2, neg, x0,
                    x1);
-              pk[half][cc * 16 + i] = kCubic<KVF> && (i & 3) == 0
-                                          ? ex2_poly_f16x2(x0, x1)
-                                          : pack_half2(fast_exp2(x0), fast_exp2(x1));
+              if (kMoveF16 && (i & 3) == 0) {
+                ex2_poly(x0, x1);
+              } else {
+                x0 = fast_exp2(x0);
+                x1 = fast_exp2(x1);
+              }
+              if constexpr (kMoveF16) add_pair(ps[i & 3], x0, x1);
+              pk[half][cc * 16 + i] = pack_half2(x0, x1);
             }
           }
-        float ps[4] = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+        if constexpr (kMoveF16) {
+          sum = (pair_sum(ps[0]) + pair_sum(ps[1])) + (pair_sum(ps[2]) + pair_sum(ps[3]));
+        } else {
+          float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const uint32_t* q4 = &pk[half][4 * g];
-            ps[g & 3] =
-                add_f16x2_to_f32(hadd2(hadd2(q4[0], q4[1]), hadd2(q4[2], q4[3])), ps[g & 3]);
-          }
+            for (int g = 0; g < 8; ++g) {
+              const uint32_t* q4 = &pk[half][4 * g];
+              t[g & 3] = add_f16x2_to_f32(hadd2(hadd2(q4[0], q4[1]), hadd2(q4[2], q4[3])), t[g & 3]);
+            }
+          sum = (t[0] + t[1]) + (t[2] + t[3]);
+        }
         // P is free (and O holds the tiles before) once the last P.V has completed
         if (j > k0) {
           ok = wait_bar(s, &s.pv_done[w], (n - 1) & 1, a.err);
@@ -886,7 +930,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st32(lane_addr + col_p(w), pk[0]);
         tmem_st32(lane_addr + col_p(w) + 32, pk[1]);
         tmem_st_wait();
-        l_run = fmaf(l_run, alpha, (ps[0] + ps[1]) + (ps[2] + ps[3]));
+        l_run = fmaf(l_run, alpha, sum);
         if (j > k0 && __any_sync(0xffffffffu, grow)) {
           uint32_t ov[2][32];
           tmem_ld32(lane_addr + col_o(w), ov[0]);
@@ -1124,24 +1168,33 @@ cudaError_t launch_attn_chunk(const ChunkArgs& args, int num_sms, cudaStream_t s
         !make_map(&tv, a.kv.v, int64_t(a.kv.hkv) * D, rows, box))
       return cudaErrorInvalidValue;
   }
-  const void* fn = a.kv.format == kKvF16  ? reinterpret_cast<const void*>(&attn_chunk_kernel<kKvF16>)
-                   : a.kv.format == kKvI8 ? reinterpret_cast<const void*>(&attn_chunk_kernel<kKvI8>)
-                                          : reinterpret_cast<const void*>(&attn_chunk_kernel<kKvQ4>);
-  const int smem = int(sizeof(Smem)) + 1024;
+  struct Kernel {
+    const void* fn;
+    int threads, regs, smem;
+  };
+  auto kernel = [](auto fmt) {
+    constexpr int kFmt = decltype(fmt)::value;
+    using C = Conf<kFmt>;
+    return Kernel{reinterpret_cast<const void*>(&attn_chunk_kernel<kFmt>), C::kThreads,
+                  C::kLaunchRegs, int(sizeof(Tiles<C::kStages>) + sizeof(Smem)) + 1024};
+  };
+  const Kernel k = a.kv.format == kKvF16  ? kernel(std::integral_constant<int, kKvF16>{})
+                   : a.kv.format == kKvI8 ? kernel(std::integral_constant<int, kKvI8>{})
+                                          : kernel(std::integral_constant<int, kKvQ4>{});
   static PerDeviceOnce attrs[3];
   const cudaError_t e = per_device_once(attrs[a.kv.format], [&](int&) {
     // the split of the registers needs the launch to have them all: without, a warpgroup would
     // wait for registers for good
     cudaFuncAttributes fa;
-    cudaError_t r = cudaFuncGetAttributes(&fa, fn);
+    cudaError_t r = cudaFuncGetAttributes(&fa, k.fn);
     if (r != cudaSuccess) return r;
-    if (fa.numRegs != kLaunchRegs) return cudaErrorNotSupported;
-    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (fa.numRegs != k.regs) return cudaErrorNotSupported;
+    return cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
   });
   if (e != cudaSuccess) return e;
   void* argv[] = {&tq, &tk, &tv, &a};
-  cudaError_t le =
-      cudaLaunchKernel(fn, dim3(unsigned(num_sms)), dim3(kThreads), argv, size_t(smem), s);
+  cudaError_t le = cudaLaunchKernel(k.fn, dim3(unsigned(num_sms)), dim3(unsigned(k.threads)), argv,
+                                    size_t(k.smem), s);
   if (le != cudaSuccess) return le;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(num_sms), kRows / 32);

@@ -297,7 +297,7 @@ __device__ __forceinline__ uint32_t ex2_f16x2(float a, float b) {
 // error on [-0.5, 0.5]: 7.5e-5, below half an f16 ulp), 2^n added into the exponent field,
 // then the same rounding cvt to f16x2 as ex2_f16x2.  Arguments below -125 (masked keys) are
 // clamped there; their f16 result is 0.
-__device__ __forceinline__ uint32_t ex2_poly_f16x2(float a, float b) {
+__device__ __forceinline__ void ex2_poly(float& a, float& b) {
   constexpr uint64_t kShift = 0x4B4000004B400000ull;  // (1.5 * 2^23, 1.5 * 2^23)
   constexpr uint64_t kC0 = 0x3F7FFB493F7FFB49ull;     // 0.99992806
   constexpr uint64_t kC1 = 0x3F31798D3F31798Dull;     // 0.69326097
@@ -317,9 +317,14 @@ __device__ __forceinline__ uint32_t ex2_poly_f16x2(float a, float b) {
   asm("mov.b64 {%0, %1}, %2;" : "=r"(t0), "=r"(t1) : "l"(t));
   asm("mov.b64 {%0, %1}, %2;" : "=r"(q0), "=r"(q1) : "l"(q));
   // the shifter's low bits hold n: (t << 23) mod 2^32 == n << 23
-  const uint32_t e0 = t0 * 8388608u + q0, e1 = t1 * 8388608u + q1;
+  a = __uint_as_float(t0 * 8388608u + q0);
+  b = __uint_as_float(t1 * 8388608u + q1);
+}
+// The same rounded to a packed f16x2.
+__device__ __forceinline__ uint32_t ex2_poly_f16x2(float a, float b) {
+  ex2_poly(a, b);
   uint32_t h;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(__uint_as_float(e1)), "f"(__uint_as_float(e0)));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(b), "f"(a));
   return h;
 }
 // Packed f16x2 sum.
