@@ -12,7 +12,7 @@
 // as long as the others).  An item that straddles CTAs leaves records (unnormalised rows,
 // maxima, sums; at most two a CTA, 20 MB in all) which a dependent kernel joins in CTA order.
 //
-// Roles of a CTA (16 warps): two softmax warpgroups, one query row per thread, 128 rows each; one
+// Roles of a CTA (16 warps, 12 over f16 caches): two softmax warpgroups, one query row per thread, 128 rows each; one
 // warp that issues the MMAs; one that issues TMA loads: Q (a 3-D box: the group's heads of 128 / G
 // tokens), two items deep, and f16 rows, a box per page; four that convert int8 and 4-bit rows, each
 // value rounded to f16 once, into the swizzled operand layout.  A converting thread has one key of
@@ -27,6 +27,13 @@
 // though it does not see all keys of its tiles is looked at again when the CTA's parts are done,
 // and worked out key by key if such a V is the cause.  (Looking through those tiles of V before they
 // are multiplied cost 4 prompts of 4096 tokens 384 -> 479 us, this 384 -> 389.)
+//
+// What bounds it.  Long chunks: the two softmax warps of each scheduler (4096 rows of 32 heads over
+// 28000 f16 keys: 1430 us, 700 TFLOP/s) or the converting warps (the same over 4 bits: 1830 us, 550
+// TFLOP/s; rows fetched by TMA instead of by their threads: 1785, but int8 280 -> 293).  Prompts of
+// up to 4096 tokens: 335 us for four, 576 TFLOP/s of the causal half.  Short chunks: latency, 2.3 us
+// to cut the list, 5 us to the first scores, 2.2 us a tile whatever its rows (a warp has a row per
+// lane and all 128 keys), 5 us to join (16 sequences of 5 tokens over up to 4096 4-bit keys: 44 us).
 //
 // Every wait is bounded; one that gives up sets the error word, the other roles stop, the CTA frees
 // its TMEM and writes nothing more.
@@ -57,18 +64,19 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 constexpr float kRescaleLog2 = 8.0f;
 // What differs by the cache's format.
-// kMoveF16: f16 tiles only move.  Nothing but the softmax asks for issue slots then: every fourth pair of
-//   exponentials is a cubic on the FMA pipe and the row sums are taken in f32 (4096 rows over 28000 keys:
-//   1450 us; with f16 pair sums 1507, without the cubic 1670).  The converting warps of the other formats
-//   need the slots: no cubic, and the rounded weights are summed in f16 by fours (4 bits: 1800 us; with
-//   f32 sums and the cubic 2377).  The exponentials are f32 ones rounded once; packed f16 ones round their
-//   argument (errors of up to 2^-9 of a weight) and took as long.
-// kStages: K/V tiles in flight.  3 leave more of the SM to the L1 cache (4 prompts of up to 4096 tokens:
-//   350 us, 368 with 4); converting warps want 4 (4 bits: 1800 us, 2589 with 3).
+// kMoveF16: f16 tiles only move.  Nothing but the softmax asks for issue slots then: every fourth
+//   pair of exponentials is a cubic on the FMA pipe and the row sums are taken in f32 (4096 rows
+//   over 28000 keys: 1450 us; with f16 pair sums 1507, without the cubic 1670).  The converting
+//   warps of the other formats need the slots: no cubic, and the rounded weights are summed in f16
+//   by fours (4 bits: 1800 us; with f32 sums and the cubic 2377).  The exponentials are f32 ones
+//   rounded once; packed f16 ones round their argument (errors of up to 2^-9 of a weight) and took
+//   as long.
+// kStages: K/V tiles in flight.  3 leave more of the SM to the L1 cache (4 prompts of up to 4096
+//   tokens: 350 us, 368 with 4); converting warps want 4 (4 bits: 1800 us, 2589 with 3).
 // Registers: setmaxnreg splits what the launch gives (kThreads x kLaunchRegs) among the two softmax
-//   warpgroups, that of the issuing warps and that of the converting ones.  The f16 kernel has no converting
-//   warps and gives theirs to the others (4 prompts: 350 -> 335 us).  Converting int8 rows in 80 registers
-//   spilled in its loop (512 rows over 32000 keys: 490 us; 280 with 96).
+//   warpgroups, that of the issuing warps and that of the converting ones.  The f16 kernel has no
+//   converting warps and gives theirs to the others (4 prompts: 350 -> 335 us).  Converting int8
+//   rows in 80 registers spilled in its loop (512 rows over 32000 keys: 490 us; 280 with 96).
 template <int KVF>
 struct Conf {
   static constexpr bool kMoveF16 = KVF == kKvF16;

@@ -14,6 +14,10 @@
 // looks at the map and otherwise only masks, stores and compares.  (With the penalties in the
 // streaming pass nearly every warp ran their divisions for one lane or another: 74 instructions per
 // token.)
+//   One row of 65536 f16 logits takes 4.6 us, which is latency (launch, history, counts, stream, cluster
+// barrier); 64 rows with everything 11.4 us; 128 rows of 131071 f32 logits, 4000 tokens of history and 300
+// biases each, 59 us (2.3 TB/s): two CTAs per SM, which is what the counts leave room for, wait at their
+// barriers.
 // The CTAs' best tokens meet in the first CTA's shared memory, one slot each (a 64-bit maximum on
 // distributed shared memory from several CTAs at once lost values).
 #include <cooperative_groups.h>
@@ -28,9 +32,9 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxCluster = 8;
 constexpr int kLocalHist = 4096;
-// Threads of a CTA: 256 up to this slice (four CTAs per SM: 64 rows of 65536 in 11.2 us, 15.8 with
-// 512), 512 above, where the counts leave room for two or three CTAs (128 rows of 131071 f32 in 58
-// us, 73 with 256).
+// Threads of a CTA: 256 up to this slice (four CTAs per SM: 64 rows of 65536 in 11.4 us, 15.8 with
+// 512), 512 above, where the counts leave room for two CTAs (128 rows of 131071 f32 in 59 us, 73 with
+// 256).
 constexpr int kSmallSlice = 12288;
 constexpr uint32_t kSeen = 0x80000000u;    // in the prompt (or generated: the count says so)
 constexpr uint32_t kCount = 0x7fffffffu;   // times generated
@@ -105,7 +109,7 @@ __global__ void __launch_bounds__(kThreads)
 
   // Another CTA's shared memory is not touched before that CTA runs: everyone reports here and waits
   // in front of the first access.
-  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   // ... and everything else the CTA is going to look at is asked for now, before any of it is
   // needed: the row's history (short ones whole; what lies behind its length is dropped later), the
