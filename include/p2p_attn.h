@@ -6,7 +6,11 @@
  *   QK_PREP      src/scripts/lfm-engine/kernels.js:216-266   -> p2p_qk_prep
  *   ATTN         src/scripts/lfm-engine/kernels.js:268-319   -> p2p_attn (prefill and decode)
  *   QK_PREP+ATTN at M=1 for every attention layer of a step  -> p2p_decode_step
- *   ATTN over many independent sequences (ragged KV cache)   -> p2p_attn_decode_ragged
+ *   ATTN over many independent sequences (ragged KV cache)   -> p2p_attn_decode_ragged,
+ *                p2p_attn_decode_kv (int8, 4-bit and/or paged caches)
+ *   QK_PREP and ATTN of ragged prompt chunks over those caches -> p2p_kv_append,
+ *                p2p_attn_chunk_kv; the cached rows back        -> p2p_kv_read
+ *   ARGMAX of a batch under penalties, biases and grammar masks -> p2p_logits_pick
  *   VISION_ATTN  src/scripts/lfm-engine/vision-kernels.js:176-258 -> p2p_attn_bidir
  *   ropeTable    src/scripts/lfm-engine/engine.js:60-71      -> p2p_rope_table
  *   meta buffer  src/scripts/lfm-engine/engine.js:144,388,422 -> p2p_meta / p2p_meta_write
@@ -342,10 +346,12 @@ p2p_status p2p_kv_read(p2p_ctx* ctx, const p2p_kv_layout* layout, int32_t num_kv
  * row t of sequence i (row row_start[i] + t of q [n_rows][ld_q]) attends keys 0 .. past[i] + t
  * of that sequence, which must already be in the cache (p2p_kv_append), and its Hq heads go to
  * the same row of out [n_rows][ld_o].  Arrays and checks as in p2p_kv_append, except that a bad
- * block-table entry keeps all rows of the sequence that see it from being written.  q and out
- * 16-byte aligned (ld_q and ld_o multiples of 8).  Cached values are rounded to f16 once, the
- * precision of an f16 cache, before they enter the tensor cores.  The workspace is the one of
- * the 4-bit decode above, under the same rules. */
+ * block-table entry keeps all rows of the sequence that see it, and up to 256 / (Hq / Hkv)
+ * tokens in front of them, from being written.  q and out 16-byte aligned (ld_q and ld_o
+ * multiples of 8), not overlapping; at most 2^31 - 1 rows of an f16 cache.  Cached values are
+ * rounded to f16 once, the precision of an f16 cache, before they enter the tensor cores.  A row
+ * is not touched by keys that it does not see, whatever their values (infinities, NaN).  The
+ * workspace is the one of the 4-bit decode above, under the same rules. */
 p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
                              const p2p_kv_layout* layout, const void* q, int64_t ld_q,
                              const void* k_cache, const void* v_cache, int64_t kv_rows,
@@ -364,7 +370,7 @@ p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
  *                x = x + bias_val[e]
  *   mask bit v of row i (bit v % 32 of word v / 32) clear: x = -inf
  * y = x rounded to the logits' type is stored in out when it is not NULL (out may be logits
- * itself, with the same ld), and tok[i] is the smallest index of the largest y above -inf (NaN
+ * itself, with the same ld, and must not overlap it otherwise), and tok[i] is the smallest index of the largest y above -inf (NaN
  * never wins), or -1 when there is none.  Any of hist, repetition, presence, frequency,
  * bias_start and mask may be NULL.  Tokens outside the vocabulary are ignored.  With advance != 0,
  * a token >= 0 is appended to hist[i] and hist_len[i] and past[i] (when not NULL) grow by one,

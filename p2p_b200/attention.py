@@ -13,6 +13,8 @@ with device memory held in torch tensors and every kernel in libp2pattn.so:
     Context.attn_decode_ragged  ATTN at M=1 over many sequences sharing one cache
     Context.kv_append / kv_read / attn_chunk_kv  QK_PREP and ATTN of ragged prompt chunks over
                            a cache of any layout (f16, int8 or 4-bit, contiguous or paged)
+    Context.attn_decode_kv ATTN at M=1 over int8, 4-bit and / or paged caches; 4-bit rows are made
+                           by kv_append, by the fused decode or by kv_quantize_q4
     Context.logits_pick    ARGMAX of a batch under penalties, biases and grammar masks
     Context.attn_bidir     VISION_ATTN vision-kernels.js:176-258, dispatched vision.js:271-276
     KVCache                K/V buffers engine.js:152-165 and ensureCapacity engine.js:274-304

@@ -14,14 +14,17 @@
 //
 // Roles of a CTA (16 warps, 12 over f16 caches): two softmax warpgroups, one query row per thread, 128 rows each; one
 // warp that issues the MMAs; one that issues TMA loads: Q (a 3-D box: the group's heads of 128 / G
-// tokens), two items deep, and f16 rows, a box per page; four that convert int8 and 4-bit rows, each
-// value rounded to f16 once, into the swizzled operand layout.  A converting thread has one key of
-// the tile, its K and its V: the row's address is then worked out once per 128 values (eight lanes
-// per row took three times the instructions), and its page's number is loaded two tiles early and
-// its words one, into registers.
+// tokens), two items deep, and the cached rows, a box per page: f16 ones into the operand tiles,
+// others into a ring (of a 4-bit row the 48 aligned bytes that hold the head's 36); four that convert
+// int8 and 4-bit rows, a key per thread, each value rounded to f16 once, into the swizzled operand
+// layout.  Their loops are rolled: unrolled they took the instruction cache from the softmax (16
+// sequences of 5 tokens: 38 us, 45 unrolled; 4096 4-bit rows over 28000 keys: 1720 us, 1785).
 //   S_w = Q_w K^T (M128 N128 K64) -> TMEM; P_w to TMEM as f16; O_w += P_w V (M128 N64 K128).
 // The softmax: exp2 with the scale folded in, lazily rescaled (only when a row's maximum grows by
-// 2^8).
+// 2^8).  Every fourth pair of exponentials is a cubic on the FMA pipe (4096 f16 rows over 28000 keys:
+// 1450 us, 1670 with none; the first 5 of 16 pairs in a row: 1628), the others are f32 ones rounded
+// once (packed f16 ones round their argument, errors of up to 2^-9 of a weight, and took as long); the
+// row sums are taken in f32.
 //   A key that a row may not see has weight 0, but 0 * inf and 0 * NaN are NaN: a token whose V
 // overflowed would reach the tokens in front of it in its tile.  A row whose sums are not finite
 // though it does not see all keys of its tiles is looked at again when the CTA's parts are done,
@@ -29,11 +32,11 @@
 // are multiplied cost 4 prompts of 4096 tokens 384 -> 479 us, this 384 -> 389.)
 //
 // What bounds it.  Long chunks: the two softmax warps of each scheduler (4096 rows of 32 heads over
-// 28000 f16 keys: 1430 us, 700 TFLOP/s) or the converting warps (the same over 4 bits: 1830 us, 550
-// TFLOP/s; rows fetched by TMA instead of by their threads: 1785, but int8 280 -> 293).  Prompts of
-// up to 4096 tokens: 335 us for four, 576 TFLOP/s of the causal half.  Short chunks: latency, 2.3 us
-// to cut the list, 5 us to the first scores, 2.2 us a tile whatever its rows (a warp has a row per
-// lane and all 128 keys), 5 us to join (16 sequences of 5 tokens over up to 4096 4-bit keys: 44 us).
+// 28000 keys: 1430 us in f16, 705 TFLOP/s, 1580 us in 4 bits, 640; int8 is converted at its softmax's
+// expense, 1900 us).  Prompts of up to 4096 tokens: 334 us for four, 579 TFLOP/s of the causal half.
+// Short chunks: latency, 2.3 us to cut the list, 5 us to the first scores, about 2 us a tile whatever
+// its rows (a warp has a row per lane and all 128 keys), 5 us to join (16 sequences of 5 tokens over
+// up to 4096 4-bit keys: 39 us).
 //
 // Every wait is bounded; one that gives up sets the error word, the other roles stop, the CTA frees
 // its TMEM and writes nothing more.
@@ -63,28 +66,25 @@ constexpr int kMaxStages = 4;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 constexpr float kRescaleLog2 = 8.0f;
-// What differs by the cache's format.
-// kMoveF16: f16 tiles only move.  Nothing but the softmax asks for issue slots then: every fourth
-//   pair of exponentials is a cubic on the FMA pipe and the row sums are taken in f32 (4096 rows
-//   over 28000 keys: 1450 us; with f16 pair sums 1507, without the cubic 1670).  The converting
-//   warps of the other formats need the slots: no cubic, and the rounded weights are summed in f16
-//   by fours (4 bits: 1800 us; with f32 sums and the cubic 2377).  The exponentials are f32 ones
-//   rounded once; packed f16 ones round their argument (errors of up to 2^-9 of a weight) and took
-//   as long.
-// kStages: K/V tiles in flight.  3 leave more of the SM to the L1 cache (4 prompts of up to 4096
-//   tokens: 350 us, 368 with 4); converting warps want 4 (4 bits: 1800 us, 2589 with 3).
+// What differs by the cache's format: f16 tiles only move (kMoveF16), int8 and 4-bit rows are copied
+// into a ring of kRaw tiles first (4096 4-bit rows over 28000 keys: 2 and 3 of them take as long).
+// kStages: operand tiles.  3, not 4, leave more of the SM to the L1 cache (4 prompts of up to 4096
+//   tokens: 350 us, 368 with 4).
 // Registers: setmaxnreg splits what the launch gives (kThreads x kLaunchRegs) among the two softmax
 //   warpgroups, that of the issuing warps and that of the converting ones.  The f16 kernel has no
-//   converting warps and gives theirs to the others (4 prompts: 350 -> 335 us).  Converting int8
-//   rows in 80 registers spilled in its loop (512 rows over 32000 keys: 490 us; 280 with 96).
+//   converting warps and gives theirs to the others (4 prompts: 350 -> 335 us).  int8: 270 us for 512
+//   rows over 32000 keys, 284 with the 4-bit split; 4 bits: 51 us for 512 rows over 3600 keys, 53 with
+//   192, 72 and 56.
 template <int KVF>
 struct Conf {
   static constexpr bool kMoveF16 = KVF == kKvF16;
-  static constexpr int kStages = kMoveF16 ? 3 : 4;
+  static constexpr int kStages = 3;
+  static constexpr int kRaw = kMoveF16 ? 0 : 2;
+  static constexpr int kRowBytes = kMoveF16 ? 128 : KVF == kKvI8 ? 64 : 48;  // of a copied row
   static constexpr int kThreads = kMoveF16 ? 384 : 512, kLaunchRegs = kMoveF16 ? 168 : 128;
-  static constexpr int kSoftmaxRegs = kMoveF16 ? 184 : 176,
-                       kIssueRegs = kMoveF16 ? 136 : KVF == kKvI8 ? 64 : 80,
-                       kLoadRegs = kMoveF16 ? 0 : KVF == kKvI8 ? 96 : 80;
+  static constexpr int kSoftmaxRegs = KVF == kKvI8 ? 176 : 184,
+                       kIssueRegs = kMoveF16 ? 136 : KVF == kKvI8 ? 64 : 72,
+                       kLoadRegs = kMoveF16 ? 0 : KVF == kKvI8 ? 96 : 72;
   static_assert(256 * kSoftmaxRegs + 128 * (kIssueRegs + kLoadRegs) <= kThreads * kLaunchRegs,
                 "register split");
 };
@@ -94,15 +94,18 @@ __device__ __forceinline__ uint32_t col_s(int w) { return uint32_t(w) * 256u; }
 __device__ __forceinline__ uint32_t col_p(int w) { return uint32_t(w) * 256u + 128u; }
 __device__ __forceinline__ uint32_t col_o(int w) { return uint32_t(w) * 256u + 192u; }
 
-template <int S>
+template <int KVF>
 struct __align__(1024) Tiles {
   __half q[2][2][BM * D];   // two items, two halves
-  __half kv[S][2][BN * D];  // K, V
+  __half kv[Conf<KVF>::kStages][2][BN * D];  // K, V
+  unsigned char raw[Conf<KVF>::kRaw ? Conf<KVF>::kRaw : 1][2]
+                   [Conf<KVF>::kRaw ? BN * Conf<KVF>::kRowBytes : 16];  // int8, 4 bits: their rows
 };
 struct __align__(128) Smem {
   float scale[kLoadWarps][2][D];  // int8: the head's scales, a copy per converting warp
   uint64_t q_full[2], q_free[2];
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages];
+  uint64_t raw_full[kMaxStages], raw_empty[kMaxStages];
   uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];
   long long wsum[8];
   int z0, qt0, kh0, off0, n_units;  // the first item of the CTA's part, and where in it
@@ -396,7 +399,7 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   constexpr int kStages = Conf<KVF>::kStages;
   constexpr bool kMoveF16 = Conf<KVF>::kMoveF16;
-  auto& tiles = *reinterpret_cast<Tiles<kStages>*>(
+  auto& tiles = *reinterpret_cast<Tiles<KVF>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Smem& s = *reinterpret_cast<Smem*>(&tiles + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -426,6 +429,10 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.kv_full[i], KVF == kKvF16 ? 1 : kLoadWarps);
       mbar_init(&s.kv_empty[i], 1);
+    }
+    for (int i = 0; i < Conf<KVF>::kRaw; ++i) {
+      mbar_init(&s.raw_full[i], 1);
+      mbar_init(&s.raw_empty[i], kLoadWarps);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.q_full[i], 1);
@@ -493,127 +500,73 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
   if (!kMoveF16 && warp >= kLoadWarp0) {
     if constexpr (!kMoveF16) regs_dec<Conf<KVF>::kLoadRegs>();
     // ---------------------------------------------------------------- converting warps
-    constexpr int kWords = KVF == kKvQ4 ? 9 : 16;  // of a head's row
+    constexpr int kRaw = Conf<KVF>::kRaw ? Conf<KVF>::kRaw : 1, kRowBytes = Conf<KVF>::kRowBytes;
     const int key = tid - kLoadWarp0 * 32;
-    const bool paged = a.kv.table != nullptr;
-    // Three tiles in a line: `now` is converted, the words of `words` are on their way, and the
-    // page number of `ahead`.
-    TileStream ahead(a.kv, a.at, group, s);
-    int32_t page = 0;
-    auto find = [&] {
-      if (ahead.done()) return;
-      page = 0;
-      if (!paged) page = a.kv.offsets[ahead.it().z];
-      else if (key < ahead.valid())
-        page = a.kv.table[int64_t(ahead.it().z) * a.kv.max_blocks +
-                          ((ahead.jj * BN + key) >> a.kv.shift)];
-    };
-    uint32_t raw[2][kWords];
-    int64_t at = 0;        // byte offset of the head's row in either pool
-    bool there = false;    // the key exists
-    int kh = 0;
-    auto place = [&] {  // takes `ahead` over as the tile whose words are loaded
-      if (ahead.done()) return;
-      const int pos = ahead.jj * BN + key;
-      kh = ahead.it().kh;
-      there = key < ahead.valid();
-      int64_t row = int64_t(page) + pos;
-      if (paged) {
-        if (there && (page < 0 || int64_t(page) >= a.kv.kv_rows)) {
-          there = false;  // a page outside the pool is not read
-          s.bad[ahead.part.seg % kMarks] = 1;
-          atomicOr(a.err, kErrPosBeyondCache);
-        }
-        row = (int64_t(page) << a.kv.shift) | (pos & ((1 << a.kv.shift) - 1));
-      }
-      at = row * a.kv.row_bytes + kh * (KVF == kKvQ4 ? kQ4UnitBytes : D);
-      ahead.next();
-      find();
-    };
-    auto load = [&](int pool) {
-      const unsigned char* src = (pool ? a.kv.v : a.kv.k) + at;
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) raw[pool][i] = 0u;  // rows behind the last key: zeros
-      if (!there) return;
-      if constexpr (KVF == kKvQ4) {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i)
-          raw[pool][i] = reinterpret_cast<const uint32_t*>(src)[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < kWords; i += 4) {
-          const uint4 x = reinterpret_cast<const uint4*>(src)[i / 4];
-          raw[pool][i] = x.x;
-          raw[pool][i + 1] = x.y;
-          raw[pool][i + 2] = x.z;
-          raw[pool][i + 3] = x.w;
-        }
-      }
-    };
-    auto convert = [&](int st, int pool) {
-      char* dst = reinterpret_cast<char*>(tiles.kv[st][pool]) + key * 128;
-      const float4* scale = reinterpret_cast<const float4*>(s.scale[warp - kLoadWarp0][pool]);
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        uint4 x;
-        if constexpr (KVF == kKvQ4) {
-          x = q4_piece(raw[pool][w], raw[pool][8]);
-        } else {
-          const float4 lo = scale[2 * w], hi = scale[2 * w + 1];
-          const float sc[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-          uint32_t h[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 v = s8_pair(raw[pool][2 * w + (k >> 1)], k & 1);
-            h[k] = pack_half2(v.x * sc[2 * k], v.y * sc[2 * k + 1]);
-          }
-          x = make_uint4(h[0], h[1], h[2], h[3]);
-        }
-        *reinterpret_cast<uint4*>(dst + ((w ^ (key & 7)) << 4)) = x;
-      }
-    };
-    find();
-    bool more = !ahead.done();
-    place();
-    load(0);
-    load(1);
-    int head = -1, next_head = kh, st = 0;
-    uint32_t ph = 1;
-    for (int c = 0; more; ++c) {
-      bool ok = true;
-      if (lane == 0 && c >= kStages) ok = wait_bar(s, &s.kv_empty[st], ph, a.err);
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      if (!ok) break;
-      if (KVF == kKvI8 && next_head != head) {
+    TileStream tile(a.kv, a.at, group, s);
+    int head = -1, st = 0, rs = 0;
+    uint32_t ph = 1, rph = 0;
+    for (int c = 0; !tile.done(); ++c, tile.next()) {
+      const int kh = tile.it().kh;
+      const bool there = key < tile.valid();  // rows behind the last key: zeros
+      bool ok = wait_bar(s, &s.raw_full[rs], rph, a.err);
+      if (ok && c >= kStages) ok = wait_bar(s, &s.kv_empty[st], ph, a.err);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (KVF == kKvI8 && kh != head) {
         __syncwarp();
 #pragma unroll
         for (int pool = 0; pool < 2; ++pool)
 #pragma unroll
           for (int d = lane; d < D; d += 32)
             s.scale[warp - kLoadWarp0][pool][d] =
-                (pool ? a.kv.v_scale
-                      : a.kv.k_scale)[a.kv.per_channel ? next_head * D + d : 0];
+                (pool ? a.kv.v_scale : a.kv.k_scale)[a.kv.per_channel ? kh * D + d : 0];
         __syncwarp();
+        head = kh;
       }
-      head = next_head;
-      more = !ahead.done();
-      if (more) place();
-      convert(st, 0);
-      if (more) load(0);
-      convert(st, 1);
-      if (more) load(1);
-      next_head = kh;
+#pragma unroll 1
+      for (int pool = 0; pool < 2; ++pool) {
+        const unsigned char* src = &tiles.raw[rs][pool][key * kRowBytes];
+        char* dst = reinterpret_cast<char*>(tiles.kv[st][pool]) + key * 128;
+        if constexpr (KVF == kKvQ4) {
+          // the unit's 9 words among the 12 that were copied
+          const uint32_t* unit = reinterpret_cast<const uint32_t*>(src) + (kh & 3);
+          const uint32_t params = there ? unit[8] : 0u;
+#pragma unroll 2
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(dst + ((i ^ (key & 7)) << 4)) =
+                q4_piece(there ? unit[i] : 0u, params);
+        } else {
+          const float4* scale = reinterpret_cast<const float4*>(s.scale[warp - kLoadWarp0][pool]);
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {  // 16-byte pieces, swizzled over 8 rows by the copy
+            const uint4 w =
+                there ? *reinterpret_cast<const uint4*>(src + ((i ^ ((key >> 1) & 3)) << 4))
+                      : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float4 lo = scale[4 * i + 2 * k], hi = scale[4 * i + 2 * k + 1];
+              const uint32_t w0 = k ? w.z : w.x, w1 = k ? w.w : w.y;
+              const float2 a0 = s8_pair(w0, 0), a1 = s8_pair(w0, 1), a2 = s8_pair(w1, 0),
+                           a3 = s8_pair(w1, 1);
+              *reinterpret_cast<uint4*>(dst + (((2 * i + k) ^ (key & 7)) << 4)) = make_uint4(
+                  pack_half2(a0.x * lo.x, a0.y * lo.y), pack_half2(a1.x * lo.z, a1.y * lo.w),
+                  pack_half2(a2.x * hi.x, a2.y * hi.y), pack_half2(a3.x * hi.z, a3.y * hi.w));
+            }
+          }
+        }
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if (c == 0 && key == 0 && a.wait_deficit)
-          mbar_arrive_expect_tx(&s.kv_full[st], uint32_t(a.wait_deficit));
-        else
-          mbar_arrive(&s.kv_full[st]);
+        mbar_arrive(&s.raw_empty[rs]);
+        mbar_arrive(&s.kv_full[st]);
       }
       if (++st == kStages) {
         st = 0;
         ph ^= 1;
+      }
+      if (++rs == kRaw) {
+        rs = 0;
+        rph ^= 1;
       }
     }
   } else if (warp >= 8) {
@@ -732,6 +685,12 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
       }
     } else if (warp == kTmaWarp) {
       // ---------------------------------------------------------------- TMA producer
+      // f16 rows go straight to the operand tiles, others to the ring of the converting warps
+      constexpr int kRing = kMoveF16 ? kStages : Conf<KVF>::kRaw, kRowBytes = Conf<KVF>::kRowBytes;
+      uint64_t* full = kMoveF16 ? s.kv_full : s.raw_full;
+      uint64_t* empty = kMoveF16 ? s.kv_empty : s.raw_empty;
+      unsigned char* ring =
+          kMoveF16 ? reinterpret_cast<unsigned char*>(tiles.kv) : &tiles.raw[0][0][0];
       const bool paged = a.kv.table != nullptr;
       const int mask = (1 << a.kv.shift) - 1;
       PartWalk walk(a.kv, a.at, group, s);
@@ -739,10 +698,8 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
       bool ok = true;
       if (lane == 0) {
         prefetch_tensormap(&tm_q);
-        if (KVF == kKvF16) {
-          prefetch_tensormap(&tm_k);
-          prefetch_tensormap(&tm_v);
-        }
+        prefetch_tensormap(&tm_k);
+        prefetch_tensormap(&tm_v);
       }
       for (bool more = true; more; walk.next()) {
         const Item it = walk.it();
@@ -762,9 +719,8 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
           break;
         }
         if (lane == 0) {
-          // The mark of eight parts ahead is cleared.  Nobody sets it yet: the MMA warp is at this
-          // part at most, the converting warps are up to kStages tiles ahead of it and their loads
-          // two more.  The part that used it last is eight back, and ended long ago.
+          // The mark of eight parts ahead is cleared.  The part that used it last is eight back,
+          // and ended long ago.
           s.bad[(seg + kMarks / 2) % kMarks] = 0;
           s.part[seg & 7] = make_int4(k0, k1, it.tiles_of(0), it.tiles_of(1));
           s.part_tail[seg & 7] = key_end;
@@ -775,51 +731,49 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
                         it.row0 + it.tok0() + h * (BM >> gshift), &s.q_full[seg & 1]);
         }
         n_q = seg + 1;
-        if constexpr (KVF == kKvF16) {
-          int32_t pages = 0;
-          const int off = paged ? 0 : a.kv.offsets[it.z];
-          for (int jj = k0; jj < k1; ++jj, ++c) {
-            const int st = c % kStages, key0 = jj * BN, valid = min(BN, key_end - key0);
-            if (lane == 0 && c >= kStages)
-              ok = wait_bar(s, &s.kv_empty[st], (c / kStages - 1) & 1, a.err);
-            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-            if (!ok) break;
-            // one box per page (or one of 128 rows)
-            const int box = paged ? min(1 << a.kv.shift, BN) : BN;
-            const int boxes = (valid + box - 1) / box;
-            int64_t row = int64_t(off) + key0;
-            if (paged) {
-              const int in = (jj - k0) & 3;  // the pages of four tiles at a time, at most 32
-              if (in == 0) {
-                pages = 0;
-                const int p = (key0 >> a.kv.shift) + lane;
-                if (p <= (key_end - 1) >> a.kv.shift)
-                  pages = a.kv.table[int64_t(it.z) * a.kv.max_blocks + p];
-              }
-              const int at = key0 + min(lane, boxes - 1) * box;
-              const int32_t pg = __shfl_sync(
-                  0xffffffffu, pages, (at >> a.kv.shift) - ((key0 - in * BN) >> a.kv.shift));
-              row = pg < 0 || int64_t(pg) >= a.kv.kv_rows
-                        ? -1
-                        : (int64_t(pg) << a.kv.shift) | (at & mask);
+        const int x = KVF == kKvQ4 ? it.kh * kQ4UnitBytes / 16 * 16 : it.kh * D;
+        int32_t pages = 0;
+        const int off = paged ? 0 : a.kv.offsets[it.z];
+        for (int jj = k0; jj < k1; ++jj, ++c) {
+          const int st = c % kRing, key0 = jj * BN, valid = min(BN, key_end - key0);
+          if (lane == 0 && c >= kRing)
+            ok = wait_bar(s, &empty[st], (c / kRing - 1) & 1, a.err);
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+          if (!ok) break;
+          // one box per page (or one of 128 rows)
+          const int box = paged ? min(1 << a.kv.shift, BN) : BN;
+          const int boxes = (valid + box - 1) / box;
+          int64_t row = int64_t(off) + key0;
+          if (paged) {
+            const int in = (jj - k0) & 3;  // the pages of four tiles at a time, at most 32
+            if (in == 0) {
+              pages = 0;
+              const int p = (key0 >> a.kv.shift) + lane;
+              if (p <= (key_end - 1) >> a.kv.shift)
+                pages = a.kv.table[int64_t(it.z) * a.kv.max_blocks + p];
             }
-            const bool bad = __any_sync(0xffffffffu, row < 0);
-            if (lane == 0) {
-              if (bad) {
-                s.bad[seg % kMarks] = 1;
-                atomicOr(a.err, kErrPosBeyondCache);
-              }
-              mbar_arrive_expect_tx(&s.kv_full[st],
-                                    uint32_t(bad ? 0 : 2 * boxes * box * 128) +
-                                        uint32_t(c == 0 ? a.wait_deficit : 0));
+            const int at = key0 + min(lane, boxes - 1) * box;
+            const int32_t pg = __shfl_sync(
+                0xffffffffu, pages, (at >> a.kv.shift) - ((key0 - in * BN) >> a.kv.shift));
+            row = pg < 0 || int64_t(pg) >= a.kv.kv_rows
+                      ? -1
+                      : (int64_t(pg) << a.kv.shift) | (at & mask);
+          }
+          const bool bad = __any_sync(0xffffffffu, row < 0);
+          if (lane == 0) {
+            if (bad) {
+              s.bad[seg % kMarks] = 1;
+              atomicOr(a.err, kErrPosBeyondCache);
             }
-            __syncwarp();
-            if (!bad && lane < boxes) {
-              tma_load_2d(&tiles.kv[st][0][lane * box * D], &tm_k, it.kh * D, int32_t(row),
-                          &s.kv_full[st]);
-              tma_load_2d(&tiles.kv[st][1][lane * box * D], &tm_v, it.kh * D, int32_t(row),
-                          &s.kv_full[st]);
-            }
+            mbar_arrive_expect_tx(&full[st],
+                                  uint32_t(bad ? 0 : 2 * boxes * box * kRowBytes) +
+                                      uint32_t(c == 0 ? a.wait_deficit : 0));
+          }
+          __syncwarp();
+          if (!bad && lane < boxes) {
+            unsigned char* dst = ring + st * 2 * BN * kRowBytes + lane * box * kRowBytes;
+            tma_load_2d(dst, &tm_k, x, int32_t(row), &full[st]);
+            tma_load_2d(dst + BN * kRowBytes, &tm_v, x, int32_t(row), &full[st]);
           }
         }
         if (!ok) break;
@@ -831,8 +785,8 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
           while (!mbar_try_wait(&s.q_full[i & 1], (i >> 1) & 1) &&
                  globaltimer_ns() - t0 < kWaitLimitNs) {
           }
-        for (int i = max(0, c - kStages); i < c; ++i)
-          while (!mbar_try_wait(&s.kv_full[i % kStages], (i / kStages) & 1) &&
+        for (int i = max(0, c - kRing); i < c; ++i)
+          while (!mbar_try_wait(&full[i % kRing], (i / kRing) & 1) &&
                  globaltimer_ns() - t0 < kWaitLimitNs) {
           }
       }
@@ -902,30 +856,17 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
               float x0, x1;
               fma2(__uint_as_float(sv[q][2 * i]), __uint_as_float(sv[q][2 * i + 1]), sl2, neg, x0,
                    x1);
-              if (kMoveF16 && (i & 3) == 0) {
+              if ((i & 3) == 0) {
                 ex2_poly(x0, x1);
               } else {
                 x0 = fast_exp2(x0);
                 x1 = fast_exp2(x1);
               }
-              if constexpr (kMoveF16) add_pair(ps[i & 3], x0, x1);
+              add_pair(ps[i & 3], x0, x1);
               pk[half][cc * 16 + i] = pack_half2(x0, x1);
             }
           }
-        float sum = 0.f;
-        if constexpr (kMoveF16) {
-          sum = (pair_sum(ps[0]) + pair_sum(ps[1])) + (pair_sum(ps[2]) + pair_sum(ps[3]));
-        } else {
-          float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-              const uint32_t* q4 = &pk[half][4 * g];
-              t[g & 3] = add_f16x2_to_f32(hadd2(hadd2(q4[0], q4[1]), hadd2(q4[2], q4[3])), t[g & 3]);
-            }
-          sum = (t[0] + t[1]) + (t[2] + t[3]);
-        }
+        const float sum = (pair_sum(ps[0]) + pair_sum(ps[1])) + (pair_sum(ps[2]) + pair_sum(ps[3]));
         // P is free (and O holds the tiles before) once the last P.V has completed
         if (j > k0) {
           ok = wait_bar(s, &s.pv_done[w], (n - 1) & 1, a.err);
@@ -1128,16 +1069,21 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
   return fn;
 }
 
-// f16 pool as [rows][hkv * 64], boxes of 64 values x `box` rows, 128-byte swizzle.
-bool make_map(CUtensorMap* m, const void* base, int64_t width, int64_t rows, int box_rows) {
+// A pool as [rows][the row's values], boxes of one head x `box_rows` rows: f16 in the operands' swizzle,
+// int8 in one without bank conflicts for a row per lane; 4 bits as the 48 bytes that hold a unit.
+bool make_map(CUtensorMap* m, const void* base, const KvView& kv, int64_t rows, int box_rows) {
   auto enc = get_encode();
   if (!enc) return false;
-  cuuint64_t dims[2] = {cuuint64_t(width), cuuint64_t(rows)};
-  cuuint64_t strides[1] = {cuuint64_t(width) * 2};
-  cuuint32_t box[2] = {64, cuuint32_t(box_rows)};
+  const bool f16 = kv.format == kKvF16;
+  cuuint64_t dims[2] = {cuuint64_t(f16 ? kv.row_bytes / 2 : kv.row_bytes), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(kv.row_bytes)};
+  cuuint32_t box[2] = {kv.format == kKvQ4 ? 48u : 64u, cuuint32_t(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box,
-             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  return enc(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
+             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             f16                     ? CU_TENSOR_MAP_SWIZZLE_128B
+             : kv.format == kKvI8 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                    : CU_TENSOR_MAP_SWIZZLE_NONE,
              CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1168,14 +1114,11 @@ cudaError_t launch_attn_chunk(const ChunkArgs& args, int num_sms, cudaStream_t s
   const int group = a.hq / a.kv.hkv;
   CUtensorMap tq{}, tk{}, tv{};
   if (!make_q_map(&tq, a.q, a.hq, a.at.n_rows, a.ld_q, group)) return cudaErrorInvalidValue;
-  if (a.kv.format == kKvF16) {
-    const int64_t rows = a.kv.kv_rows << a.kv.shift;  // shift 0 when contiguous
-    const int box = a.kv.table && (1 << a.kv.shift) < BN ? 1 << a.kv.shift : BN;
-    if (rows > INT32_MAX) return cudaErrorInvalidValue;
-    if (!make_map(&tk, a.kv.k, int64_t(a.kv.hkv) * D, rows, box) ||
-        !make_map(&tv, a.kv.v, int64_t(a.kv.hkv) * D, rows, box))
-      return cudaErrorInvalidValue;
-  }
+  const int64_t rows = a.kv.kv_rows << a.kv.shift;  // shift 0 when contiguous
+  const int box = a.kv.table && (1 << a.kv.shift) < BN ? 1 << a.kv.shift : BN;
+  if (rows > INT32_MAX) return cudaErrorInvalidValue;
+  if (!make_map(&tk, a.kv.k, a.kv, rows, box) || !make_map(&tv, a.kv.v, a.kv, rows, box))
+    return cudaErrorInvalidValue;
   struct Kernel {
     const void* fn;
     int threads, regs, smem;
@@ -1184,7 +1127,7 @@ cudaError_t launch_attn_chunk(const ChunkArgs& args, int num_sms, cudaStream_t s
     constexpr int kFmt = decltype(fmt)::value;
     using C = Conf<kFmt>;
     return Kernel{reinterpret_cast<const void*>(&attn_chunk_kernel<kFmt>), C::kThreads,
-                  C::kLaunchRegs, int(sizeof(Tiles<C::kStages>) + sizeof(Smem)) + 1024};
+                  C::kLaunchRegs, int(sizeof(Tiles<kFmt>) + sizeof(Smem)) + 1024};
   };
   const Kernel k = a.kv.format == kKvF16  ? kernel(std::integral_constant<int, kKvF16>{})
                    : a.kv.format == kKvI8 ? kernel(std::integral_constant<int, kKvI8>{})

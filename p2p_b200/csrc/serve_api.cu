@@ -245,8 +245,8 @@ p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
   a.hq = prm->num_heads;
   a.scale_log2 = p2p::eff_scale_log2(prm);
   a.err = p2p::ctx_dev_err(ctx);
-  if (a.kv.format == P2P_KV_F16 && (a.kv.kv_rows << a.kv.shift) > INT32_MAX)
-    return fail(ctx, P2P_ERR_UNSUPPORTED, "attn_chunk_kv: f16 caches of more than 2^31 rows");
+  if (a.kv.kv_rows > (int64_t(INT32_MAX) >> a.kv.shift))
+    return fail(ctx, P2P_ERR_UNSUPPORTED, "attn_chunk_kv: caches of more than 2^31 - 1 rows");
   OnDevice g(p2p::ctx_device(ctx));
   unsigned char* ws = nullptr;
   st = p2p::ctx_serve_workspace(ctx, static_cast<cudaStream_t>(stream), "attn_chunk_kv", &ws);
