@@ -211,6 +211,25 @@ def test_append_without_norm_or_q(ctx, fmt):
     assert torch.equal(c.v[(*at, used)], c.stored(v, c.vs)[:, used])
 
 
+@pytest.mark.parametrize("rows", [[3, 40], [1500, 700]])
+def test_append_with_q_in_place(ctx, rows):
+    past = [5, 0]
+    c = Cache(15, "f16", 16, 32, 8, [p + r for p, r in zip(past, rows)])
+    qkv, rope = randh(gen(16), sum(rows), 48 * D), rope_table(2000)
+    nw = randh(gen(17), 2 * D)
+    q = torch.zeros(sum(rows), 32 * D, dtype=torch.float16, device="cuda")
+    args = (i32(past), starts_of(rows))
+    ctx.kv_append(c.prm, qkv, nw, rope, c.k, c.v, *args, max_len=2000, q_out=q, **c.kw())
+    ctx.sync()
+    k, v = c.k.clone(), c.v.clone()
+    same = qkv.clone()
+    ctx.kv_append(c.prm, same, nw, rope, c.k, c.v, *args, max_len=2000, q_out=same[:, :32 * D],
+                  **c.kw())
+    ctx.sync()
+    assert torch.equal(same[:, :32 * D], q) and torch.equal(same[:, 32 * D:], qkv[:, 32 * D:])
+    assert torch.equal(c.k, k) and torch.equal(c.v, v)
+
+
 @pytest.mark.parametrize("fmt,page", list(itertools.product(FMTS, (0, 16, 64))))
 @pytest.mark.parametrize("heads", [(32, 8), (6, 3), (8, 1), (12, 12)])
 def test_read_back(ctx, fmt, page, heads):
