@@ -12,31 +12,32 @@
 // as long as the others).  An item that straddles CTAs leaves records (unnormalised rows,
 // maxima, sums; at most two a CTA, 20 MB in all) which a dependent kernel joins in CTA order.
 //
-// Roles of a CTA (16 warps, 12 over f16 caches): two softmax warpgroups, one query row per thread, 128 rows each; one
-// warp that issues the MMAs; one that issues TMA loads: Q (a 3-D box: the group's heads of 128 / G
-// tokens), two items deep, and the cached rows, a box per page: f16 ones into the operand tiles,
-// others into a ring (of a 4-bit row the 48 aligned bytes that hold the head's 36); four that convert
-// int8 and 4-bit rows, a key per thread, each value rounded to f16 once, into the swizzled operand
-// layout.  Their loops are rolled: unrolled they took the instruction cache from the softmax (16
-// sequences of 5 tokens: 38 us, 45 unrolled; 4096 4-bit rows over 28000 keys: 1720 us, 1785).
-//   S_w = Q_w K^T (M128 N128 K64) -> TMEM; P_w to TMEM as f16; O_w += P_w V (M128 N64 K128).
-// The softmax: exp2 with the scale folded in, lazily rescaled (only when a row's maximum grows by
-// 2^8).  Every fourth pair of exponentials is a cubic on the FMA pipe (4096 f16 rows over 28000 keys:
-// 1450 us, 1670 with none; the first 5 of 16 pairs in a row: 1628), the others are f32 ones rounded
-// once (packed f16 ones round their argument, errors of up to 2^-9 of a weight, and took as long); the
-// row sums are taken in f32.
+// Roles of a CTA (16 warps, 12 over f16 caches): two softmax warpgroups, one query row per thread,
+// 128 rows each; one warp that issues the MMAs; one that issues TMA loads: Q (a 3-D box: the
+// group's heads of 128 / G tokens), two items deep, and the cached rows, a box per page: f16 ones
+// into the operand tiles, others into a ring (of a 4-bit row the 48 aligned bytes that hold the
+// head's 36); four that convert int8 and 4-bit rows, a key per thread, each value rounded to f16
+// once, into the swizzled operand layout.  Their loops are rolled: unrolled they took the
+// instruction cache from the softmax (16 sequences of 5 tokens: 38 us, 45 unrolled; 4096 4-bit rows
+// over 28000 keys: 1720 us, 1785).
+//   S_w = Q_w K^T (M128 N128 K64) -> TMEM; P_w to TMEM as f16; O_w += P_w V (M128 N64 K128). The
+// softmax: exp2 with the scale folded in, lazily rescaled (only when a row's maximum grows by
+// 2^8).  Every fourth pair of exponentials is a cubic on the FMA pipe (4096 f16 rows over 28000
+// keys: 1450 us, 1670 with none; the first 5 of 16 pairs in a row: 1628), the others are f32 ones
+// rounded once (packed f16 ones round their argument, errors of up to 2^-9 of a weight, and took
+// as long); the row sums are taken in f32.
 //   A key that a row may not see has weight 0, but 0 * inf and 0 * NaN are NaN: a token whose V
 // overflowed would reach the tokens in front of it in its tile.  A row whose sums are not finite
 // though it does not see all keys of its tiles is looked at again when the CTA's parts are done,
-// and worked out key by key if such a V is the cause.  (Looking through those tiles of V before they
-// are multiplied cost 4 prompts of 4096 tokens 384 -> 479 us, this 384 -> 389.)
+// and worked out key by key if such a V is the cause.  (Looking through those tiles of V before
+// they are multiplied cost 4 prompts of 4096 tokens 384 -> 479 us, this 384 -> 389.)
 //
 // What bounds it.  Long chunks: the two softmax warps of each scheduler (4096 rows of 32 heads over
-// 28000 keys: 1430 us in f16, 705 TFLOP/s, 1580 us in 4 bits, 640; int8 is converted at its softmax's
-// expense, 1900 us).  Prompts of up to 4096 tokens: 334 us for four, 579 TFLOP/s of the causal half.
-// Short chunks: latency, 2.3 us to cut the list, 5 us to the first scores, about 2 us a tile whatever
-// its rows (a warp has a row per lane and all 128 keys), 5 us to join (16 sequences of 5 tokens over
-// up to 4096 4-bit keys: 39 us).
+// 28000 keys: 1430 us in f16, 705 TFLOP/s, 1580 us in 4 bits, 640; int8 is converted at its
+// softmax's expense, 1900 us).  Prompts of up to 4096 tokens: 334 us for four, 579 TFLOP/s of the
+// causal half. Short chunks: latency, 2.3 us to cut the list, 5 us to the first scores, about 2 us
+// a tile whatever its rows (a warp has a row per lane and all 128 keys), 5 us to join (16 sequences
+// of 5 tokens over up to 4096 4-bit keys: 39 us).
 //
 // Every wait is bounded; one that gives up sets the error word, the other roles stop, the CTA frees
 // its TMEM and writes nothing more.

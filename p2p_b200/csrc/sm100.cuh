@@ -291,12 +291,11 @@ __device__ __forceinline__ uint32_t ex2_f16x2(float a, float b) {
   asm("ex2.approx.f16x2 %0, %1;" : "=r"(e) : "r"(h));
   return e;
 }
-// exp2 of two f32 arguments as one packed f16x2, evaluated on the FMA pipe instead of the
+// exp2 of two f32 arguments, in place, evaluated on the FMA pipe instead of the
 // MUFU: n = rint(x) with the 1.5 * 2^23 shifter, f = x - n in [-0.5, 0.5], 2^f by a cubic
 // (coefficients fitted for this kernel by a linear program minimising the maximum relative
-// error on [-0.5, 0.5]: 7.5e-5, below half an f16 ulp), 2^n added into the exponent field,
-// then the same rounding cvt to f16x2 as ex2_f16x2.  Arguments below -125 (masked keys) are
-// clamped there; their f16 result is 0.
+// error on [-0.5, 0.5]: 7.5e-5, below half an f16 ulp), 2^n added into the exponent field.
+// Arguments below -125 (masked keys) are clamped there; rounded to f16 the result is 0.
 __device__ __forceinline__ void ex2_poly(float& a, float& b) {
   constexpr uint64_t kShift = 0x4B4000004B400000ull;  // (1.5 * 2^23, 1.5 * 2^23)
   constexpr uint64_t kC0 = 0x3F7FFB493F7FFB49ull;     // 0.99992806
@@ -320,7 +319,7 @@ __device__ __forceinline__ void ex2_poly(float& a, float& b) {
   a = __uint_as_float(t0 * 8388608u + q0);
   b = __uint_as_float(t1 * 8388608u + q1);
 }
-// The same rounded to a packed f16x2.
+// The same as one packed f16x2, with the rounding cvt of ex2_f16x2.
 __device__ __forceinline__ uint32_t ex2_poly_f16x2(float a, float b) {
   ex2_poly(a, b);
   uint32_t h;
