@@ -33,8 +33,7 @@
 // they are multiplied cost 4 prompts of 4096 tokens 384 -> 479 us, this 384 -> 389.)
 //
 // What bounds it.  Long chunks: the two softmax warps of each scheduler (4096 rows of 32 heads over
-// 28000 keys: 1430 us in f16, 705 TFLOP/s, 1580 us in 4 bits, 640; int8 is converted at its
-// softmax's expense, 1900 us).  Prompts of up to 4096 tokens: 334 us for four, 579 TFLOP/s of the
+// 28000 keys: 1425 us in f16, 708 TFLOP/s, 1580 us in 4 bits, 640, 1660 us in int8, 608).  Prompts of up to 4096 tokens: 334 us for four, 579 TFLOP/s of the
 // causal half. Short chunks: latency, 2.3 us to cut the list, 5 us to the first scores, about 2 us
 // a tile whatever its rows (a warp has a row per lane and all 128 keys), 5 us to join (16 sequences
 // of 5 tokens over up to 4096 4-bit keys: 39 us).
@@ -73,8 +72,8 @@ constexpr float kRescaleLog2 = 8.0f;
 //   tokens: 350 us, 368 with 4).
 // Registers: setmaxnreg splits what the launch gives (kThreads x kLaunchRegs) among the two softmax
 //   warpgroups, that of the issuing warps and that of the converting ones.  The f16 kernel has no
-//   converting warps and gives theirs to the others (4 prompts: 350 -> 335 us).  int8: 270 us for 512
-//   rows over 32000 keys, 284 with the 4-bit split; 4 bits: 51 us for 512 rows over 3600 keys, 53 with
+//   converting warps and gives theirs to the others (4 prompts: 350 -> 335 us).  int8: 245 us for 512
+//   rows over 32000 keys, 287 with the 4-bit split; 4 bits: 51 us for 512 rows over 3600 keys, 53 with
 //   192, 72 and 56.
 template <int KVF>
 struct Conf {
@@ -284,12 +283,20 @@ __device__ __forceinline__ uint4 q4_piece(uint32_t w, uint32_t params) {
                     __byte_perm(r[0], r[1], 0x7632), __byte_perm(r[2], r[3], 0x7632));
 }
 
-// Bytes 2k, 2k + 1 of a word as signed values: the byte x ^ 0x80 under the f16 pattern 0x64xx is
-// 1024 + 128 + x (no conversion instructions, which would share the exponentials' unit).
-__device__ __forceinline__ float2 s8_pair(uint32_t w, int k) {
-  const uint32_t h = __byte_perm(w ^ 0x80808080u, 0x64646464u, k ? 0x4342 : 0x4140);
-  return __half22float2(
-      __hsub2(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(1152.f, 1152.f)));
+// Bytes 2k, 2k + 1 of x ^ 0x80808080 (x: signed bytes) times their scales, rounded to f16 once: under
+// the f32 pattern of 2^23 a byte is 2^23 + 128 + its value (no conversion instructions, which would
+// share the exponentials' unit).
+__device__ __forceinline__ uint32_t s8_scaled(uint32_t w, int k, float s0, float s1) {
+  const float f0 = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + 2 * k));
+  const float f1 = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441 + 2 * k));
+  uint64_t x, s;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(f0), "f"(f1));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(s) : "f"(s0), "f"(s1));
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(0xcb000080cb000080ull));  // -(2^23 + 128)
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(s));
+  float v0, v1;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v0), "=f"(v1) : "l"(x));
+  return pack_half2(v0, v1);
 }
 
 // The maximum of three, NaN when one of them is.
@@ -545,12 +552,10 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const float4 lo = scale[4 * i + 2 * k], hi = scale[4 * i + 2 * k + 1];
-              const uint32_t w0 = k ? w.z : w.x, w1 = k ? w.w : w.y;
-              const float2 a0 = s8_pair(w0, 0), a1 = s8_pair(w0, 1), a2 = s8_pair(w1, 0),
-                           a3 = s8_pair(w1, 1);
-              *reinterpret_cast<uint4*>(dst + (((2 * i + k) ^ (key & 7)) << 4)) = make_uint4(
-                  pack_half2(a0.x * lo.x, a0.y * lo.y), pack_half2(a1.x * lo.z, a1.y * lo.w),
-                  pack_half2(a2.x * hi.x, a2.y * hi.y), pack_half2(a3.x * hi.z, a3.y * hi.w));
+              const uint32_t w0 = (k ? w.z : w.x) ^ 0x80808080u, w1 = (k ? w.w : w.y) ^ 0x80808080u;
+              *reinterpret_cast<uint4*>(dst + (((2 * i + k) ^ (key & 7)) << 4)) =
+                  make_uint4(s8_scaled(w0, 0, lo.x, lo.y), s8_scaled(w0, 1, lo.z, lo.w),
+                             s8_scaled(w1, 0, hi.x, hi.y), s8_scaled(w1, 1, hi.z, hi.w));
             }
           }
         }
