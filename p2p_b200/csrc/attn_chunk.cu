@@ -33,10 +33,11 @@
 // they are multiplied cost 4 prompts of 4096 tokens 384 -> 479 us, this 384 -> 389.)
 //
 // What bounds it.  Long chunks: the two softmax warps of each scheduler (4096 rows of 32 heads over
-// 28000 keys: 1425 us in f16, 708 TFLOP/s, 1580 us in 4 bits, 640, 1660 us in int8, 608).  Prompts of up to 4096 tokens: 334 us for four, 579 TFLOP/s of the
-// causal half. Short chunks: latency, 2.3 us to cut the list, 5 us to the first scores, about 2 us
-// a tile whatever its rows (a warp has a row per lane and all 128 keys), 5 us to join (16 sequences
-// of 5 tokens over up to 4096 4-bit keys: 39 us).
+// 28000 keys: 1425 us in f16, 708 TFLOP/s, 1580 us in 4 bits, 640, 1660 us in int8, 608).  Prompts
+// of up to 4096 tokens: 334 us for four, 579 TFLOP/s of the causal half. Short chunks: latency, 2.3
+// us to cut the list, 5 us to the first scores, about 2 us a tile whatever its rows (a warp has a
+// row per lane and all 128 keys), 5 us to join (16 sequences of 5 tokens over up to 4096 4-bit
+// keys: 39 us).
 //
 // Every wait is bounded; one that gives up sets the error word, the other roles stop, the CTA frees
 // its TMEM and writes nothing more.
