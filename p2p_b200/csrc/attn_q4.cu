@@ -11,10 +11,13 @@
 // and into the final scale of the odd output dims.
 //     S^T[16 keys x 8 heads] = C_K[16 x 64] . Q^T[64 x 8],   O^T[64 x 8] += C_V^T[64 x 16] . P'^T
 // P' = p * s goes in as a high and a low f16 in the columns that up to four query heads leave free
-// (22 bits of the weight); eight heads fill the columns and P' is rounded to f16 (2^-11 of a weight,
-// below the rounding of the f16 output).  p goes up to 4, which uses the range left by s <= 8734,
-// so weights keep their bits down to small scales.  p, the sums of p and of p * lo, the running
-// maximum and O stay in f32.
+// (22 bits of the weight); eight heads fill the columns and P' is rounded to f16: 2^-11 of w (v - lo),
+// about twice the rounding of the output where the values have no common sign.  The reference that
+// weights are taken against follows the largest p * s, not the largest p, and puts it at 2^12 or more:
+// a key keeps its bits down to 2^-26 of the largest weight times scale and is lost below 2^-37 of it,
+// whatever the scales are.  (Against the largest p, a tail of 131071 keys of amplitude 0.03 behind a key
+// 14 nats above it lost its codes: 3.5e-2 of the outputs' norm off, now 2.1e-4; it costs 2 % of the
+// time.)  p, the sums of p and of p * lo, the reference and O stay in f32.
 //
 // Split.  All sequences' tiles, in order, form one list that is cut into equal parts, one per CTA
 // (two CTAs per SM), so ragged batches balance by themselves whatever the lengths and the grid
@@ -56,8 +59,9 @@ constexpr int kMaxStages = 8;
 constexpr int kRec = 68;                       // acc[64], max, sum, 2 pad: 17 16-byte pieces
 constexpr int kJoin = 16;                      // records joined by one warp
 constexpr float kNegBig = -1e30f;
-// Weights are 2^(score - m) with m two below the maximum, so at most 4: p * s <= 4 * 8734 < 65504
-constexpr float kUp = 2.f;
+// log2 of where the largest weight * scale is put when the reference is set, and from where on it is
+// set again: 2^15.5 is below f16's 65504 with what log2_scale may be off.
+constexpr float kUp = 12.f, kTop = 15.5f;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 
 // Warps per head for a CTA of hb heads (1 .. 8); its tile is `blocks` (1 or 2) blocks per such warp.
@@ -189,10 +193,20 @@ __device__ __forceinline__ void load_query(const __half* q, float scale_log2, Qu
     out.sum[e] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
 }
 
+// kLogBias + x + log2 of the scale in a unit's parameters, from the bits of the f16: 0 to 0.09 too low
+// for normal numbers, for the others as for 2^-15 (more: their rows' codes are below the output's
+// rounding anyway).  The bias leaves a sum 2^-10.
+constexpr float kLogBias = 8192.f + 15.f;
+__device__ __forceinline__ float add_log2_scale(float x, uint32_t params) {
+  // 2^23 + the bits
+  const float bits = __uint_as_float(__byte_perm(params, 0x4b000000u, 0x7610));
+  return fmaf(bits, 0.0009765625f, x);
+}
+
 template <int H>
 struct State {
-  // The reference that weights are taken against (the warp's; at most kUp below the maximum when it
-  // was set) and, of the lane, the sums of the weights and of weight * lo.
+  // The reference that weights are taken against (the warp's; kUp below the largest score + log2 of
+  // the value scale when it was set) and, of the lane, the sums of the weights and of weight * lo.
   float m[H], l[H], bias[H];
   // [i][c]: dim 8 gid + 2i of column 2t + c (even codes); [i][2 + c]: dim 8 gid + 2i + 1 (odd ones).
   // H = 1: the sums over the high (c = 0) and low (c = 1) parts of the weights.
@@ -250,23 +264,40 @@ __device__ __forceinline__ void attend(const unsigned char* ks, const unsigned c
 #pragma unroll
         for (int e = 0; e < H; ++e) sc[k][e] = -INFINITY;
   }
-  float top[H];
-  bool grows = st.fresh;
+  uint32_t pv[2 * NJ];  // the keys' parameters of V
 #pragma unroll
-  for (int e = 0; e < H; ++e) {
-    top[e] = sc[0][e];
-#pragma unroll
-    for (int k = 1; k < 2 * NJ; ++k) top[e] = fmaxf(top[e], sc[k][e]);
-    grows |= top[e] > kUp;
+  for (int k = 0; k < 2 * NJ; ++k) {
+    pv[k] = reinterpret_cast<const uint32_t*>(vs + (row + 8 * k) * pitch)[8];
+    if (!FULL && 8 * k + row >= valid) pv[k] = 0u;
   }
-  // the maximum rarely grows after the first blocks: only then is it joined and O rescaled
-  if (__any_sync(0xffffffffu, grows)) {
+  // The reference rarely has to move after the first blocks: only then are the lanes' maxima joined and
+  // O rescaled.  (Scores of 2^24 and more may need it again, rounded as their differences are.)
+#pragma unroll 1
+  for (int pass = 0; pass < 4; ++pass) {
+    float top[H];
+    bool grows = st.fresh;
 #pragma unroll
     for (int e = 0; e < H; ++e) {
+      top[e] = add_log2_scale(sc[0][e], pv[0]);
 #pragma unroll
-      for (int o = 4; o <= 16; o <<= 1)
+      for (int k = 1; k < 2 * NJ; ++k) top[e] = fmaxf(top[e], add_log2_scale(sc[k][e], pv[k]));
+      grows |= top[e] > kTop + kLogBias;
+    }
+    if (!__any_sync(0xffffffffu, grows)) break;
+#pragma unroll
+    for (int e = 0; e < H; ++e) {
+      float most = sc[0][e];
+#pragma unroll
+      for (int k = 1; k < 2 * NJ; ++k) most = fmaxf(most, sc[k][e]);
+#pragma unroll
+      for (int o = 4; o <= 16; o <<= 1) {
         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
-      const float up = st.fresh ? top[e] - kUp : fmaxf(top[e] - kUp, 0.f);
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      }
+      // a whole number away from the largest score, whose weight then is a power of two and its
+      // product with the scale exact
+      const float rise = most + floorf(top[e] - kLogBias - kUp - most);
+      const float up = st.fresh ? rise : fmaxf(rise, 0.f);
       const float c = st.fresh ? 0.f : fast_exp2(-up);
       st.m[e] += up;
       st.l[e] *= c;
@@ -297,10 +328,8 @@ __device__ __forceinline__ void attend(const unsigned char* ks, const unsigned c
     uint32_t w[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      uint32_t pv = reinterpret_cast<const uint32_t*>(vs + (16 * j + row + 8 * k) * pitch)[8];
-      if (!FULL && 16 * j + 8 * k + row >= valid) pv = 0u;
       float s, lo, ps[2];
-      q4_unpack(pv, s, lo);
+      q4_unpack(pv[2 * j + k], s, lo);
 #pragma unroll
       for (int e = 0; e < H; ++e) {
         const float p = fast_exp2(sc[2 * j + k][e]);

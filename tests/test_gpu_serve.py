@@ -1146,3 +1146,142 @@ def test_decode_wait_runs_out(ctx, heads):
     ctx.attn_decode_kv(*args, **kw)
     ctx.sync()
     assert torch.equal(out, good)
+
+
+# ---- the weights' range of the 4-bit decode ---------------------------------------------------------
+def decode_of_constant_keys(c, q, n):
+    """One token over the n keys of a 4-bit cache whose K rows are constant (codes of 0, so that a
+    score is lo * sum(q) / 8 in plain f32): out [hq][64] in f64 and how far a kernel may be from it.
+
+    Weights.  A score in log2 units is a sum of 64 f16 values, a product and two additions: 24
+    roundings of 2^-24 of its size, of the reference's (kept 12 below the largest score + log2 of the
+    scale or of 2^-14) and of the differences; exp2 is off by 2^-22.  An error e of a
+    weight moves out by w e |v - out|.
+    A weight times the scale goes into the product sum in two f16 parts (2^-22) or, for 8 query heads
+    per kv head, in one (2^-11), which moves out by that share of w (v - lo); below f16's normal numbers
+    by 2^-25 with the largest product at 2^12 or more: 2^-37 of it in each code's weight.
+    The product sums of 64 keys are four MMAs, each of up to 17 addends cut off at 2^-22 of the
+    largest, which is below 2^-14 (a subnormal code) times the largest weight, or the sum so far; the
+    result counts 2^22.  The other sums are f32: a lane's 8 keys of a block, its blocks, of 64 keys each,
+    and the joins, below 64 + n / 64 roundings of 2^-24."""
+    grp = c.hq // c.hkv
+    at = c.at(0, torch.arange(n, device="cuda"))
+    lo_k = c.k[at][:, :c.hkv * UNIT].reshape(n, c.hkv, UNIT)
+    assert not lo_k[..., :34].any()  # codes and scale
+    lo_k = lo_k[..., 34:].contiguous().view(torch.float16).double()[..., 0]    # [n][hkv]
+    u = c.v[at][:, :c.hkv * UNIT].reshape(n, c.hkv, UNIT)
+    par = u[..., 32:].contiguous().view(torch.float16).double()
+    scale, lo = par[..., 0], par[..., 1]
+    outs, tols = [], []
+    for h in range(c.hkv):
+        qs = q.view(c.hq, D)[h * grp:(h + 1) * grp].double()
+        s = qs.sum(-1, keepdim=True) * lo_k[None, :, h] / 8                       # [grp][n]
+        w = torch.softmax(s, -1)
+        code = torch.stack([u[:, h, :32] & 15, u[:, h, :32] >> 4], -1).flatten(-2).double()
+        above = code * scale[:, h, None]                                          # v - lo
+        v = above + lo[:, h, None]
+        o = w @ v
+        e = 2.0 ** -21 + 2.0 ** -24 * 24 * (s.abs().amax() / math.log(2) + 40)
+        t = e * (w @ v.abs() + o.abs())
+        t = t + (2.0 ** -11 if grp == 8 else 2.0 ** -22) * (w @ above)
+        t = t + 2.0 ** -37 * (w * scale[:, h].clamp(min=2.0 ** -14)).amax(-1, keepdim=True) * code.sum(0)
+        ws = torch.nn.functional.pad(w * scale[:, h], (0, -n % 64)).view(grp, -1, 64)
+        t = t + 68 * 2.0 ** -14 * ws.amax(-1).sum(-1, keepdim=True)
+        t = t + (68 * 2.0 ** -22 + (64 + n / 64) * 2.0 ** -24) * (w @ above + w @ lo[:, h].abs()[:, None])
+        t = t + o.abs() * 2.0 ** -11 + 2.0 ** -25
+        outs.append(o)
+        tols.append(t)
+    return torch.cat(outs), torch.cat(tols)
+
+
+def decode_constant_keys(ctx, hq, hkv, page, k, v, copies=1):
+    """One token of each of `copies` sequences over the same n keys: k [n][hkv] (the rows' only value),
+    v f16 [n][hkv][64].  (One sequence's keys are spread over all SMs; of hundreds, each is one CTA's.)"""
+    n = len(k)
+    c = Cache(91, "q4", page, hq, hkv, [n])
+    at = c.at(0, torch.arange(n, device="cuda"))
+    c.k[at] = quant4(k.half()[..., None].expand(n, hkv, D).contiguous())
+    c.v[at] = quant4(v)
+    q = torch.ones(copies, hq * D, dtype=torch.float16, device="cuda")
+    out = torch.zeros_like(q)
+    if page:
+        c.table = c.table.repeat(copies, 1)
+    else:
+        c.offsets = c.offsets.repeat(copies)
+    ctx.attn_decode_kv(c.prm, q, None, None, c.k, c.v, i32([n - 1] * copies), out, max_past=n - 1,
+                       fused_prep=False, **c.kw())
+    ctx.sync()
+    want, tol = decode_of_constant_keys(c, q[0], n)
+    return out.view(copies, hq, D), want, tol
+
+
+@pytest.mark.parametrize("amp", [1.0, 0.1, 0.03, 0.01, 1e-4])
+@pytest.mark.parametrize("heads,n,gap", [((8, 8), 8192, 14), ((16, 8), 8192, 13), ((32, 8), 8192, 14),
+                                         ((64, 8), 8192, 14), ((8, 1), 8192, 12), ((4, 1), 32768, 13),
+                                         ((32, 8), 131071, 14), ((8, 1), 131071, 14)],
+                         ids=lambda x: str(x).replace(" ", ""))
+def test_decode_q4_strong_first_key(ctx, heads, n, gap, amp):
+    """A key far above a long tail, whose weights times small scales are tiny: the tail counts."""
+    hq, hkv = heads
+    k = torch.zeros(n, hkv, device="cuda")
+    k[0] = gap / 8
+    v = amp * randh(gen(92), n, hkv, D)
+    for copies in (1, 600 if n < 30000 else 300):
+        got, want, tol = decode_constant_keys(ctx, hq, hkv, 64, k, v, copies)
+        assert_within(got, want, tol, f"{copies} sequences")
+        assert float(((got.double() - want).norm(dim=(1, 2)) / want.norm()).max()) < 1e-3
+
+
+@pytest.mark.parametrize("heads", [(8, 8), (32, 8), (64, 8), (8, 1), (12, 12)])
+@pytest.mark.parametrize("kind", ["mixed scales", "a loud key of no weight", "rising scores"])
+def test_decode_q4_scales_of_all_sizes(ctx, heads, kind):
+    hq, hkv = heads
+    n, g = 9000, gen(93)
+    v = torch.randn(n, hkv, D, generator=g, device="cuda")
+    k = torch.randn(n, hkv, generator=g, device="cuda") / 2
+    if kind == "mixed scales":
+        v = v * 2.0 ** (22 * torch.rand(n, hkv, 1, generator=g, device="cuda") - 12)
+        v[::7] = v[::7, :, :1]  # constant rows: a scale of 0
+    elif kind == "rising scores":
+        k = (k / 4 + torch.arange(n, device="cuda")[:, None] * (8 / n))
+        v = v * 0.01
+    else:
+        k, v = k / 4, v * 0.01
+        k[0] = 14 / 8 + 0.5
+        k[n // 2], v[n // 2] = -4, 2000 * v[0]
+    for copies in (1, 600):
+        got, want, tol = decode_constant_keys(ctx, hq, hkv, 16, k, v.half(), copies)
+        assert_within(got, want, tol, f"{copies} sequences")
+
+
+@pytest.mark.parametrize("gap", [3.0, 3.125, 3.25, 3.375])
+@pytest.mark.parametrize("heads", [(8, 8), (16, 8), (32, 8), (4, 1)])
+def test_decode_q4_weights_in_two_parts(ctx, heads, gap):
+    """Equal weights whose product with the scale is no f16: up to four query heads per kv head keep
+    22 bits of them, which shows where the values' mean is near 0 and their lowest value is not."""
+    hq, hkv = heads
+    n = 8192
+    k = torch.zeros(n, hkv, device="cuda")
+    k[0] = gap / 8
+    v = torch.full((n, hkv, D), -1 + 7 * 2 / 15, device="cuda")
+    v[1::2] = -1 + 8 * 2 / 15
+    v[..., 0], v[..., 1] = -1, 1
+    got, want, tol = decode_constant_keys(ctx, hq, hkv, 0, k, v.half())
+    assert_within(got, want, tol)
+    assert (tol[:, 2:] < 2.0 ** -13).all()  # one f16 would be off by up to 2^-11
+
+
+@pytest.mark.parametrize("amp", [1e-4, 0.01, 30.0, 2000.0])
+@pytest.mark.parametrize("heads", [(8, 8), (8, 4), (16, 4), (64, 8), (8, 1)])
+def test_decode_q4_ranges_of_every_group(ctx, heads, amp):
+    """Tiny and large caches, with the bound of ordinary ones."""
+    hq, hkv = heads
+    c = Cache(94, "q4", 16, hq, hkv, [600, 50, 2000], amp=amp)
+    q = randh(gen(95), 3, hq * D) * (0.05 if amp > 1 else 1.0)
+    out = torch.zeros_like(q)
+    past = [599, 49, 1999]
+    ctx.attn_decode_kv(c.prm, q, None, None, c.k, c.v, i32(past), out, max_past=1999,
+                       fused_prep=False, **c.kw())
+    ctx.sync()
+    want, tol = attention64(c, q, past, [1] * 3, False)
+    assert_within(out, want, tol)
