@@ -849,8 +849,9 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
         const bool grow = (mx - m_raw) * sl2 > kRescaleLog2;
         const float alpha = grow ? fast_exp2((m_raw - mx) * sl2) : 1.0f;
         if (grow) m_raw = mx;
-        // a NaN score makes all of the row's weights NaN (the cubic alone would lose it)
-        const float neg = mx != mx ? mx : (m_raw == -INFINITY) ? 0.f : -m_raw * sl2;
+        // a score of NaN or +inf makes all of the row's weights NaN (inf - inf is NaN for that key
+        // alone, and the cubic would lose it)
+        const float neg = !(mx < INFINITY) ? NAN : (m_raw == -INFINITY) ? 0.f : -m_raw * sl2;
         uint32_t pk[2][32];
         uint64_t ps[4] = {0, 0, 0, 0};  // f32 pairs
 #pragma unroll
@@ -932,6 +933,9 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) ov[0][i] = ov[1][i] = 0u;
       }
+      // No key that counts so far (scores of -inf, or none in this part): the cubic has left 2^-125 per
+      // masked key.  With 0 the row is NaN if that stays all of it, and a record adds nothing.
+      if (m_raw == -INFINITY) l_run *= 0.f;
       const bool bad = s.bad[seg % kMarks] != 0;
       if (!whole && tid == 0 && k0 == 0) {  // the item begins here: what there is to join
         // list position behind the item

@@ -1285,3 +1285,87 @@ def test_decode_q4_ranges_of_every_group(ctx, heads, amp):
     ctx.sync()
     want, tol = attention64(c, q, past, [1] * 3, False)
     assert_within(out, want, tol)
+
+
+# ---- infinite scores in prompt chunks ----------------------------------------------------------------
+def chunk_with_infinite_keys(ctx, case, page, keys, sign):
+    """One sequence whose keys `keys` have a K of sign * inf in dim 5 of kv head 0: out and the 64-bit
+    one [rows][hq][64], with the bound of attention64 (the infinite products left out of its sizes: a
+    score of -inf has weight 0, one of +inf makes the row NaN)."""
+    (hq, hkv), past, rows = case
+    n, grp = past + rows, hq // hkv
+    c = Cache(96, "f16", page, hq, hkv, [n])
+    q = randh(gen(97), rows, hq * D)
+    k, v = c.keys64(0, n)
+    at = c.at(0, torch.as_tensor(keys, device="cuda"))
+    c.k[(*at, 0, 5)] = sign * math.inf
+    out = torch.full_like(q, 7.0)
+    ctx.attn_chunk_kv(c.prm, q, c.k, c.v, i32([past]), i32([0, rows]), out, max_len=n, **c.kw())
+    ctx.sync()
+    k, v = (t.repeat_interleave(grp, 1).permute(1, 0, 2) for t in (k, v))
+    qi = q.double().view(rows, hq, D).permute(1, 0, 2)
+    s, mag = qi @ k.transpose(1, 2) / 8, qi.abs() @ k.abs().transpose(1, 2) / 8
+    s[:grp, :, keys] = sign * math.inf * qi[:grp, :, 5].sign()[..., None]
+    hidden = torch.arange(n, device="cuda")[None] > \
+        (past + torch.arange(rows, device="cuda"))[:, None]
+    w = torch.softmax(s.masked_fill(hidden, -math.inf), -1)
+    o = w @ v
+    e = 2.0 ** -11 + 2.0 ** -10 + mag * (2.0 ** -11 + 2.0 ** -18)
+    t = (w * e) @ v.abs() + o.abs() * (w * e).sum(-1, keepdim=True)
+    t = t + (w @ v.abs()) * (2.0 ** -11 + 2.0 ** -16) + o.abs() * 2.0 ** -11 + 2.0 ** -24
+    return out.view(rows, hq, D), o.permute(1, 0, 2), t.permute(1, 0, 2)
+
+
+def assert_nan_or_within(got, want, tol, what):
+    odd = want.isnan()
+    assert torch.equal(got.isnan(), odd), (what, int((got.isnan() != odd).sum()))
+    assert_within(got[~odd], want[~odd], tol[~odd], what)
+
+
+INFINITE = [
+    # heads, past, rows: items that one CTA works on alone, and items split over several
+    ((32, 8), 0, 40), ((32, 8), 130, 70), ((32, 8), 3000, 33), ((8, 1), 9000, 5), ((16, 16), 700, 257),
+]
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("case", INFINITE, ids=str)
+def test_an_infinite_key_at_any_place(ctx, case, sign):
+    (hq, hkv), past, rows = case
+    n = past + rows
+    for j in range(8):
+        for key in {j, n - 17 + j, n // 2 // 8 * 8 + j}:
+            got, want, tol = chunk_with_infinite_keys(ctx, case, 16, [key], sign)
+            assert_nan_or_within(got, want, tol, f"key {key}")
+            # the other kv heads do not see it
+            assert hkv == 1 or not want[:, hq // hkv:].isnan().any()
+
+
+@pytest.mark.parametrize("page", [0, 64])
+@pytest.mark.parametrize("case", INFINITE, ids=str)
+def test_rows_of_infinite_scores(ctx, case, page):
+    """All of a kv head's keys infinite, its first ones, its last ones, all but one."""
+    _, past, rows = case
+    n = past + rows
+    for keys in (range(n), range(min(n - 1, 200)), range(n // 2, n), range(1, n)):
+        for sign in (1, -1):
+            got, want, tol = chunk_with_infinite_keys(ctx, case, page, list(keys), sign)
+            assert_nan_or_within(got, want, tol, f"{sign} * inf at {keys}")
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("case", INFINITE, ids=str)
+def test_an_infinite_query_is_its_rows_alone(ctx, fmt, case):
+    (hq, hkv), past, rows = case
+    c = Cache(98, fmt, 16, hq, hkv, [past + rows])
+    q = randh(gen(99), rows, hq * D)
+    want, tol = (t.view(rows, hq, D) for t in attention64(c, q, [past], [rows], True))
+    for r, h, d, x in ((0, 1, 3, math.inf), (rows - 1, hq - 1, 60, -math.inf), (rows // 2, 0, 0, math.nan)):
+        q[r, h * D + d] = x
+        want[r, h] = math.nan
+    out = torch.zeros_like(q)
+    ctx.attn_chunk_kv(c.prm, q, c.k, c.v, i32([past]), i32([0, rows]), out, max_len=past + rows, **c.kw())
+    ctx.sync()
+    got = out.view(rows, hq, D)
+    # (the first row of the first case sees one key: a score of -inf or +inf, NaN either way)
+    assert_nan_or_within(got, want, tol, "q")
