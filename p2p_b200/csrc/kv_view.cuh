@@ -55,24 +55,34 @@ __host__ __device__ __forceinline__ int64_t kv_row(const KvView& c, int i, int p
   return (int64_t(pg) << c.shift) | (pos & ((1 << c.shift) - 1));
 }
 
-// The sequence whose chunk holds row r, by the whole warp: the number of i in [1, nseq] with
-// row_start[i] <= r, 32 entries a step.  -1 when no sequence's rows reach r.
-__device__ __forceinline__ int warp_find_seq(const int32_t* row_start, int nseq, int64_t r) {
-  const int lane = threadIdx.x & 31;
+// The sequence whose chunk holds row r: the number of i in [1, nseq] with row_start[i] <= r, 32
+// entries a step.  -1 when no sequence's rows reach r, and whatever row_start holds, a sequence that is
+// returned has r among its rows.  count(f): for how many of the 32 lanes f(lane) holds.
+template <class Count>
+__host__ __device__ __forceinline__ int find_seq(const int32_t* row_start, int nseq, int64_t r,
+                                                 Count count) {
   int lo = 0, n = nseq;  // candidates lo .. lo + n - 1; every entry before lo is <= r
   while (n > 32) {
     const int step = (n + 31) / 32;
-    const int at = lo + min((lane + 1) * step, n) - 1;  // last candidate of the lane's part
-    const int below = __popc(__ballot_sync(0xffffffffu, row_start[at + 1] <= r));
+    const int below = count([&](int lane) {  // the last candidate of the lane's part
+      const int end = (lane + 1) * step;
+      return row_start[lo + (end < n ? end : n)] <= r;
+    });
     if (below == 32) return -1;
-    const int skip = min(below * step, n);
+    const int skip = below * step < n ? below * step : n;
     lo += skip;
-    n = min(step, n - skip);
+    n = step < n - skip ? step : n - skip;
     if (n <= 0) return -1;
   }
-  const bool le = lane < n && row_start[lo + lane + 1] <= r;
-  const int seq = lo + __popc(__ballot_sync(0xffffffffu, le));
-  return seq < nseq && seq < lo + n && row_start[seq] <= r ? seq : -1;
+  const int seq =
+      lo + count([&](int lane) { return lane < n && row_start[lo + lane + 1] <= r; });
+  return seq < nseq && seq < lo + n && row_start[seq] <= r && r < row_start[seq + 1] ? seq : -1;
+}
+// The same by a whole warp.
+__device__ __forceinline__ int warp_find_seq(const int32_t* row_start, int nseq, int64_t r) {
+  const int lane = threadIdx.x & 31;
+  return find_seq(row_start, nseq, r,
+                  [&](auto f) { return __popc(__ballot_sync(0xffffffffu, f(lane))); });
 }
 
 // ---- the 4-bit rows ---------------------------------------------------------------------------

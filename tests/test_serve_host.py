@@ -111,3 +111,60 @@ def test_paged_rows(host_rows):
     assert host_rows(True, 9, 30, 0, 4, 4, 60, table=t) == \
         (True, [2 * 16 + 14, 2 * 16 + 15, -1, -1])
     assert host_rows(True, 10, 15, 0, 2, 4, 60, table=[7, -1, 9]) == (True, [7 * 16 + 15, -1])
+
+
+@pytest.fixture(scope="module")
+def find_seq(tmp_path_factory):
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("p2p_build", ROOT / "p2p_b200" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    exe = tmp_path_factory.mktemp("find_seq") / "find_seq_host"
+    subprocess.run([build.nvcc(), *build.ARCH, "-std=c++17", "--expt-relaxed-constexpr",
+                    "--extended-lambda", "-I", str(build.CSRC),
+                    str(ROOT / "tests" / "find_seq_host.cu"), "-o", str(exe)],
+                   check=True, capture_output=True)
+
+    def ask(cases):
+        """cases: (row_start, rows) pairs -> the sequences of the rows."""
+        lines = [" ".join(map(str, [len(s) - 1, *s, len(r), *r])) for s, r in cases]
+        out = subprocess.run([str(exe)], input="\n".join(lines) + "\n", capture_output=True,
+                             text=True, check=True).stdout.splitlines()
+        return [[int(x) for x in line.split()] for line in out]
+    return ask
+
+
+def test_a_rows_sequence(find_seq):
+    """Every row of rising starts is found, empty sequences are passed over."""
+    import random
+    rng = random.Random(3)
+    cases = []
+    for n in (1, 2, 31, 32, 33, 64, 65, 1000, 1025, 3000):
+        for top in (0, 1, 3):
+            lens = [rng.randint(0, top) for _ in range(n)]
+            start = [rng.randint(0, 2)]
+            for x in lens:
+                start.append(start[-1] + x)
+            cases.append((start, range(0, start[-1] + 3)))
+    for (start, rows), got in zip(cases, find_seq(cases)):
+        want = {r: i for i in range(len(start) - 1) for r in range(start[i], start[i + 1])}
+        assert got == [want.get(r, -1) for r in rows]
+
+
+def test_falling_starts_never_give_a_row_to_a_sequence_that_ends_before_it(find_seq):
+    """Whatever row_start holds, the sequence that a row is given has it among its rows (a position
+    behind a sequence's checked end would lie outside its pages)."""
+    import random
+    rng = random.Random(4)
+    cases = [([0, 100, 2, 4], range(105))]
+    for n in (3, 5, 32, 40, 100, 700, 2000):
+        for _ in range(60):
+            start = [rng.randint(-3, 2 * n) for _ in range(n + 1)]
+            if rng.random() < 0.5:  # nearly rising
+                start.sort()
+                for _ in range(rng.randint(1, 4)):
+                    start[rng.randrange(n + 1)] = rng.randint(-3, 2 * n)
+            cases.append((start, [rng.randint(0, 2 * n) for _ in range(60)]))
+    for (start, rows), got in zip(cases, find_seq(cases)):
+        for r, i in zip(rows, got):
+            assert i == -1 or start[i] <= r < start[i + 1], (start, r, i)
