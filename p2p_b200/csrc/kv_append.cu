@@ -95,13 +95,25 @@ __device__ __forceinline__ uint32_t pack_q8(const float* x, const float* sc, int
   return w;
 }
 
+// The first block of a launch reports the sequences that do not fit, by themselves: those whose rows
+// all lie behind n_rows, or that a falling row_start leaves without any, belong to no row's warp.
+__device__ __forceinline__ void report_misfits(const KvView& kv, const ChunkIndex& at, int32_t* err) {
+  bool bad = false;
+  for (int z = threadIdx.x; z < at.nseq; z += kThreads) {
+    const SeqSpan span = seq_span(kv, at, z);
+    bad |= span.len != 0 && !span.ok;
+  }
+  if (bad) atomicOr(err, kErrPosBeyondCache);
+}
+
 // One warp per (row, 4 kIter consecutive units of its Hq + 2 Hkv).
 template <int KVF, int kIter>
 __global__ void __launch_bounds__(kThreads)
     kv_append_kernel(const __grid_constant__ AppendArgs a) {
+  if (blockIdx.x == 0) return report_misfits(a.kv, a.at, a.err);
   const int lane = threadIdx.x & 31, s = lane & 7;
   const int units = a.hq + 2 * a.kv.hkv, groups = (units + 4 * kIter - 1) / (4 * kIter);
-  const int64_t item = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  const int64_t item = (int64_t(blockIdx.x - 1) * kThreads + threadIdx.x) >> 5;
   const int64_t row = item / groups;
   if (row >= a.at.n_rows) return;
   const int u0 = int(item - row * groups) * 4 * kIter + (lane >> 3);
@@ -117,7 +129,7 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
   const int seq = warp_find_seq(a.at.row_start, a.at.nseq, row);
-  if (seq < 0) return;  // behind the last sequence
+  if (seq < 0) return;  // no sequence's row
   const SeqSpan span = seq_span(a.kv, a.at, seq);
   const int pos = span.past + int(row - span.row0);
   const int64_t at = span.ok ? kv_row(a.kv, seq, pos) : -1;
@@ -203,9 +215,10 @@ __global__ void __launch_bounds__(kThreads)
 // One warp per (row, 4 kIter consecutive units of K and V); lane s of a unit: dims 8s .. 8s+7.
 template <int KVF, int kIter>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadArgs a) {
+  if (blockIdx.x == 0) return report_misfits(a.kv, a.at, a.err);
   const int lane = threadIdx.x & 31, s = lane & 7;
   const int hkv = a.kv.hkv, units = 2 * hkv, groups = (units + 4 * kIter - 1) / (4 * kIter);
-  const int64_t item = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  const int64_t item = (int64_t(blockIdx.x - 1) * kThreads + threadIdx.x) >> 5;
   const int64_t row = item / groups;
   if (row >= a.at.n_rows) return;
   const int seq = warp_find_seq(a.at.row_start, a.at.nseq, row);
@@ -302,8 +315,8 @@ static cudaError_t launch_rows(const A& a, int64_t units, cudaStream_t s) {
   const bool w = wide(a.at.n_rows, units);
   const int64_t groups = w ? (units + 15) / 16 : (units + 3) / 4;
   const int64_t blocks = (a.at.n_rows * groups * 32 + kThreads - 1) / kThreads;
-  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  const dim3 g{unsigned(blocks)};
+  if (blocks >= INT32_MAX) return cudaErrorInvalidValue;
+  const dim3 g{unsigned(blocks + 1)};  // and the one that reports
   if (a.kv.format == kKvF16) w ? K<kKvF16, 4>::run(g, s, a) : K<kKvF16, 1>::run(g, s, a);
   else if (a.kv.format == kKvI8) w ? K<kKvI8, 4>::run(g, s, a) : K<kKvI8, 1>::run(g, s, a);
   else w ? K<kKvQ4, 4>::run(g, s, a) : K<kKvQ4, 1>::run(g, s, a);

@@ -1369,3 +1369,46 @@ def test_an_infinite_query_is_its_rows_alone(ctx, fmt, case):
     got = out.view(rows, hq, D)
     # (the first row of the first case sees one key: a score of -inf or +inf, NaN either way)
     assert_nan_or_within(got, want, tol, "q")
+
+
+@pytest.mark.parametrize("op", ["append", "read"])
+@pytest.mark.parametrize("page", [0, 16])
+@pytest.mark.parametrize("starts,done", [
+    ([0, 4, 8, 12], [(0, 0, 4), (1, 4, 8)]),   # of 8 rows: the last sequence's all lie behind them
+    ([0, 4, 8, 8], [(0, 0, 4), (1, 4, 8)]),    # nothing wrong
+    ([0, 6, 2, 4], [(0, 0, 2)]),               # falling: sequence 1 has -4 rows
+], ids=str)
+def test_rows_without_a_sequence_are_left_alone_and_reported(ctx, op, page, starts, done):
+    import p2p_b200
+    hq, hkv, past, n = 8, 2, [5, 40, 33], 8
+    c = Cache(47, "q4", page, hq, hkv, [60, 60, 60])
+    good_k, good_v = c.k.clone(), c.v.clone()
+    qkv, rope = randh(gen(48), n, 12 * D), rope_table(60)
+    out = torch.full((n, hq * D), 7.0, dtype=torch.float16, device="cuda")
+    back = torch.full((n, hkv, D), 7.0, dtype=torch.float16, device="cuda")
+    if op == "append":
+        ctx.kv_append(c.prm, qkv, None, rope, c.k, c.v, i32(past), i32(starts), max_len=60,
+                      q_out=out, **c.kw())
+    else:
+        ctx.kv_read(c.prm, c.k, c.v, i32(past), i32(starts), back, None, max_len=60, **c.kw())
+    if starts[-1] == n:
+        ctx.sync()
+    else:
+        with pytest.raises(p2p_b200.KvFullError):
+            ctx.sync()
+    ctx.sync()
+    left = torch.ones(n, dtype=torch.bool, device="cuda")
+    for i, a, b in done:
+        left[a:b] = False
+        if op == "read":
+            assert torch.equal(back[a:b], c.keys64(i, 60)[0][past[i]:past[i] + b - a].float().half())
+            continue
+        assert not (out[a:b] == 7).any()
+        at = c.at(i, past[i] + torch.arange(b - a, device="cuda"))
+        _, k, v = prep(ctx, c.prm, qkv[a:b], None, rope, past[i])
+        used = slice(0, hkv * UNIT)
+        assert torch.equal(c.k[(*at, used)], quant4(k)[:, used])
+        assert torch.equal(c.v[(*at, used)], quant4(v)[:, used])
+        c.k[at], c.v[at] = good_k[at], good_v[at]
+    assert (out[left] == 7).all() and (back[left] == 7).all()
+    assert torch.equal(c.k, good_k) and torch.equal(c.v, good_v)
