@@ -88,17 +88,19 @@ class Params:
                           self.eps, dt)
 
     def ref(self):
-        """The C view by reference, kept while the fields stay as they are."""
-        key = (self.num_heads, self.num_kv_heads, self.head_dim, self.scale, self.eps, self.dtype)
-        kept = self.__dict__.get("_c")
-        if kept is None or kept[0] != key:
-            c = self.c()
-            kept = self.__dict__["_c"] = (key, c, C.byref(c))
-        return kept[2]
+        """The C view by reference, made once for these values (kept outside the instance, which
+        stays an ordinary dataclass that can be copied and pickled)."""
+        return _params_ref(self.num_heads, self.num_kv_heads, self.head_dim, self.scale, self.eps,
+                           self.dtype)
 
     @property
     def qkv_width(self) -> int:
         return (self.num_heads + 2 * self.num_kv_heads) * self.head_dim
+
+
+@functools.lru_cache(maxsize=256)
+def _params_ref(*fields):
+    return C.byref(Params(*fields).c())
 
 
 class Context:

@@ -168,3 +168,18 @@ def test_falling_starts_never_give_a_row_to_a_sequence_that_ends_before_it(find_
     for (start, rows), got in zip(cases, find_seq(cases)):
         for r, i in zip(rows, got):
             assert i == -1 or start[i] <= r < start[i + 1], (start, r, i)
+
+
+def test_parameters_stay_plain_values():
+    """Parameters that were used in a call can be copied, sent and changed like others."""
+    import copy
+    import pickle
+    import p2p_b200
+    prm = p2p_b200.Params(8, 2, scale=0.5)
+    c = prm.ref()._obj
+    assert (c.num_heads, c.num_kv_heads, c.head_dim, c.scale, c.dtype) == (8, 2, 64, 0.5, 0)
+    assert copy.deepcopy(prm) == prm and pickle.loads(pickle.dumps(prm)) == prm
+    assert vars(prm) == vars(p2p_b200.Params(8, 2, scale=0.5))
+    prm.num_heads, prm.dtype = 16, torch.float32
+    c = prm.ref()._obj
+    assert (c.num_heads, c.scale, c.dtype) == (16, 0.5, 1)
