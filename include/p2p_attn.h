@@ -318,7 +318,7 @@ p2p_status p2p_kv_quantize_q4(p2p_ctx* ctx, const void* src, void* dst, int64_t 
  * tokens of sequence i at positions past[i], past[i]+1, ...: q and k are normed (norm_w NULL:
  * not) and rotated exactly as p2p_qk_prep does it, k and v go to the sequence's cache rows of
  * those positions in the layout's format, and the rotated q to q_out [n_rows][ld_q] (NULL: not
- * wanted; the q columns of qkv itself are fine).  row_start (nseq + 1 values), past and offsets
+ * wanted; qkv itself with ld_q = ld_qkv is fine, any other overlap with its rows is refused).  row_start (nseq + 1 values), past and offsets
  * are device int32 arrays; the rope table holds max_len rows or more.  Rows at and behind row_start[nseq] are left alone, in qkv's
  * outputs and in the cache.  A sequence with a negative entry or a negative number of rows,
  * past[i] + rows > max_len, rows beyond n_rows, kv_rows or max_blocks is skipped, and so is a row

@@ -12,6 +12,7 @@
 #pragma GCC visibility pop
 #include "host_internal.h"
 #include "kernels.h"
+#include "rows.h"
 
 static_assert(P2P_MAX_VOCAB == p2p::kMaxVocab, "vocabulary limit");
 static_assert(P2P_KV_F16 == int(p2p::kKvF16) && P2P_KV_I8 == int(p2p::kKvI8) &&
@@ -172,6 +173,11 @@ p2p_status p2p_kv_append(p2p_ctx* ctx, const p2p_attn_params* prm, const p2p_kv_
     return fail(ctx, P2P_ERR_INVALID_ARG,
                 "kv_append: qkv, q_out, norm_w and rope must be 8-byte aligned, ld_qkv and ld_q "
                 "multiples of 4");
+  if (q_out && !(q_out == qkv && (ld_q == ld_qkv || n_rows == 1)) &&
+      p2p::rows_overlap(qkv, ld_qkv * 2, row * 2, q_out, ld_q * 2, qw * 2, n_rows))
+    return fail(ctx, P2P_ERR_INVALID_ARG,
+                "kv_append: q_out overlaps qkv (in place it starts with it and has its pitch, %lld)",
+                (long long)ld_qkv);
   if ((st = p2p::ctx_check_rope(ctx, rope, max_len, "kv_append")) != P2P_OK) return st;
   a.at = {past, row_start, nseq, n_rows, max_len};
   a.qkv = static_cast<const __half*>(qkv);

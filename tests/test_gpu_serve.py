@@ -1412,3 +1412,32 @@ def test_rows_without_a_sequence_are_left_alone_and_reported(ctx, op, page, star
         c.k[at], c.v[at] = good_k[at], good_v[at]
     assert (out[left] == 7).all() and (back[left] == 7).all()
     assert torch.equal(c.k, good_k) and torch.equal(c.v, good_v)
+
+
+def test_append_refuses_a_q_that_overlaps_qkv(ctx):
+    import p2p_b200
+    c = Cache(49, "f16", 16, 8, 2, [40])
+    buf = randh(gen(50), 4, 24 * D)
+    qkv, rope = buf[:, :12 * D], rope_table(40)
+    keep, k, v = buf.clone(), c.k.clone(), c.v.clone()
+    args, kw = (c.k, c.v, i32([3]), i32([0, 4])), dict(max_len=40, **c.kw())
+    flat = buf.view(-1)
+    for bad in (flat[:4 * 8 * D].view(4, 8 * D),              # in place with its own pitch
+                buf[:, 4 * D:12 * D],                         # shifted by heads
+                flat[24 * D:24 * D * 4 + 8 * D].as_strided((3, 8 * D), (24 * D, 1)),
+                flat[8 * D:].as_strided((4, 8 * D), (16 * D, 1))):
+        with pytest.raises(p2p_b200.P2PError) as e:
+            ctx.kv_append(c.prm, qkv[:len(bad)], None, rope, *args, q_out=bad, **kw)
+        assert e.value.status == p2p_b200.P2P_ERR_INVALID_ARG
+    ctx.sync()
+    assert torch.equal(buf, keep) and torch.equal(c.k, k) and torch.equal(c.v, v)
+    # beside it, in place with its pitch, and one row in place are fine
+    q = torch.zeros(4, 8 * D, dtype=torch.float16, device="cuda")
+    ctx.kv_append(c.prm, qkv, None, rope, *args, q_out=q, **kw)
+    ctx.kv_append(c.prm, qkv, None, rope, *args, q_out=buf[:, 12 * D:20 * D], **kw)
+    one = buf[:1, :12 * D].clone()
+    ctx.kv_append(c.prm, one, None, rope, c.k, c.v, i32([3]), i32([0, 1]), q_out=one[:, :8 * D], **kw)
+    ctx.kv_append(c.prm, qkv, None, rope, *args, q_out=buf[:, :8 * D], **kw)
+    ctx.sync()
+    assert torch.equal(buf[:, 12 * D:20 * D], q) and torch.equal(buf[:, :8 * D], q)
+    assert torch.equal(one[:, :8 * D], q[:1])

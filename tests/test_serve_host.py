@@ -183,3 +183,31 @@ def test_parameters_stay_plain_values():
     prm.num_heads, prm.dtype = 16, torch.float32
     c = prm.ref()._obj
     assert (c.num_heads, c.scale, c.dtype) == (16, 0.5, 1)
+
+
+def test_rows_overlap(tmp_path):
+    """Strided rows against the sets of their bytes: shifted, interleaved, of other pitches."""
+    import random
+    exe = tmp_path / "rows_host"
+    subprocess.run(["g++", "-std=c++17", "-I", str(ROOT / "p2p_b200" / "csrc"),
+                    str(ROOT / "tests" / "rows_host.cpp"), "-o", str(exe)], check=True,
+                   capture_output=True)
+    rng = random.Random(5)
+    cases = []
+    for _ in range(6000):
+        n, pa = rng.randint(1, 6), rng.randint(1, 12)
+        pb = pa if rng.random() < 0.6 else rng.randint(1, 12)
+        cases.append((rng.randint(100, 160), pa, rng.randint(1, pa), rng.randint(100, 160), pb,
+                      rng.randint(1, pb), n))
+        if n == 1:  # a single row may be wider than its pitch
+            cases.append((*cases[-1][:2], 9, *cases[-1][3:5], 7, 1))
+    big = 2**40
+    cases += [(big, 2**20, 2**19, big + 2**19, 2**20, 2**19, 2**31 - 1),      # side by side
+              (big, 2**20, 2**19 + 1, big + 2**19, 2**20, 2**19, 2**31 - 1)]  # one byte shared
+    out = subprocess.run([str(exe)], input="\n".join(" ".join(map(str, c)) for c in cases) + "\n",
+                         capture_output=True, text=True, check=True).stdout.split()
+    for (a, pa, wa, b, pb, wb, n), got in zip(cases[:-2], out):
+        one, two = ({at + i * p + j for i in range(n) for j in range(w)}
+                    for at, p, w in ((a, pa, wa), (b, pb, wb)))
+        assert bool(int(got)) == bool(one & two), (a, pa, wa, b, pb, wb, n)
+    assert out[-2:] == ["0", "1"]
