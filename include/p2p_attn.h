@@ -350,7 +350,7 @@ p2p_status p2p_kv_read(p2p_ctx* ctx, const p2p_kv_layout* layout, int32_t num_kv
  * the same row of out [n_rows][ld_o].  Arrays and checks as in p2p_kv_append, except that a bad
  * block-table entry keeps all rows of the sequence that see it, and up to 256 / (Hq / Hkv)
  * tokens in front of them, from being written.  q and out 16-byte aligned (ld_q and ld_o
- * multiples of 8), not overlapping; at most 2^31 - 1 rows of an f16 cache.  Cached values are
+ * multiples of 8), not overlapping (refused); at most 2^31 - 1 rows of an f16 cache.  Cached values are
  * rounded to f16 once, the precision of an f16 cache, before they enter the tensor cores.  A row
  * is not touched by keys that it does not see, whatever their values (infinities, NaN); a head's
  * row is NaN where a score that it sees is NaN or +inf, or where all of them are -inf.  The

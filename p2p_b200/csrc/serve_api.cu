@@ -243,6 +243,8 @@ p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
   if (!aligned(q, 16) || !aligned(out, 16) || ld_q % 8 || ld_o % 8)
     return fail(ctx, P2P_ERR_INVALID_ARG,
                 "attn_chunk_kv: q and out must be 16-byte aligned, ld_q and ld_o multiples of 8");
+  if (p2p::rows_overlap(q, ld_q * 2, qw * 2, out, ld_o * 2, qw * 2, n_rows))
+    return fail(ctx, P2P_ERR_INVALID_ARG, "attn_chunk_kv: q and out overlap");
   a.at = {past, row_start, nseq, n_rows, max_len};
   a.q = static_cast<const __half*>(q);
   a.ld_q = ld_q;

@@ -1441,3 +1441,25 @@ def test_append_refuses_a_q_that_overlaps_qkv(ctx):
     ctx.sync()
     assert torch.equal(buf[:, 12 * D:20 * D], q) and torch.equal(buf[:, :8 * D], q)
     assert torch.equal(one[:, :8 * D], q[:1])
+
+
+def test_chunk_refuses_an_out_that_overlaps_q(ctx):
+    import p2p_b200
+    c = Cache(51, "q4", 16, 8, 2, [40])
+    buf = randh(gen(52), 9, 24 * D)
+    keep = buf.clone()
+    q = buf[:4, :8 * D]
+    args, kw = (c.k, c.v, i32([3]), i32([0, 4])), dict(max_len=40, **c.kw())
+    for bad in (q, buf[1:5, :8 * D], buf[:4, 4 * D:12 * D], buf[3:7, 7 * D:15 * D],
+                buf.view(-1)[16 * D:].as_strided((4, 8 * D), (16 * D, 1))):
+        with pytest.raises(p2p_b200.P2PError) as e:
+            ctx.attn_chunk_kv(c.prm, q, *args, bad, **kw)
+        assert e.value.status == p2p_b200.P2P_ERR_INVALID_ARG
+    ctx.sync()
+    assert torch.equal(buf, keep)
+    out = torch.zeros(4, 8 * D, dtype=torch.float16, device="cuda")
+    ctx.attn_chunk_kv(c.prm, q, *args, out, **kw)
+    for beside in (buf[:4, 8 * D:16 * D], buf[4:8, :8 * D], buf[2:6, 16 * D:]):
+        ctx.attn_chunk_kv(c.prm, q, *args, beside, **kw)
+        ctx.sync()
+        assert torch.equal(beside, out) and torch.equal(q, keep[:4, :8 * D])
