@@ -373,8 +373,8 @@ p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
  *                x = x + bias_val[e]
  *   mask bit v of row i (bit v % 32 of word v / 32) clear: x = -inf
  * y = x rounded to the logits' type is stored in out when it is not NULL (out may be logits
- * itself, with the same ld, and must not overlap it otherwise), and tok[i] is the smallest index of the largest y above -inf (NaN
- * never wins), or -1 when there is none.  Any of hist, repetition, presence, frequency,
+ * itself, with the same ld; any other overlap is refused), and tok[i] is the smallest index of the
+ * largest y above -inf (NaN never wins), or -1 when there is none.  Any of hist, repetition, presence, frequency,
  * bias_start and mask may be NULL.  Tokens outside the vocabulary are ignored.  With advance != 0,
  * a token >= 0 is appended to hist[i] and hist_len[i] and past[i] (when not NULL) grow by one,
  * on the device; when hist_len[i] has reached hist_cap neither changes and the next p2p_sync

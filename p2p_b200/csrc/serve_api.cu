@@ -288,6 +288,10 @@ p2p_status p2p_logits_pick(p2p_ctx* ctx, const p2p_logits* args, void* stream) {
   const unsigned es = g.dtype == P2P_F32 ? 4 : 2;
   if (!aligned(g.logits, es) || !aligned(g.out, es))
     return fail(ctx, P2P_ERR_INVALID_ARG, "logits_pick: logits not aligned to their type");
+  if (g.out && g.out != g.logits &&
+      p2p::rows_overlap(g.logits, g.ld * es, int64_t(g.vocab) * es, g.out, g.ld_out * es,
+                        int64_t(g.vocab) * es, g.rows))
+    return fail(ctx, P2P_ERR_INVALID_ARG, "logits_pick: out overlaps logits other than in place");
   if (g.hist && (!g.hist_len || g.hist_cap < 0 || g.ld_hist < g.hist_cap))
     return fail(ctx, P2P_ERR_INVALID_ARG,
                 "logits_pick: hist needs hist_len and 0 <= hist_cap %d <= ld_hist %lld",

@@ -1463,3 +1463,23 @@ def test_chunk_refuses_an_out_that_overlaps_q(ctx):
         ctx.attn_chunk_kv(c.prm, q, *args, beside, **kw)
         ctx.sync()
         assert torch.equal(beside, out) and torch.equal(q, keep[:4, :8 * D])
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.float32])
+def test_logits_refuse_an_out_that_overlaps_them(ctx, dt):
+    import p2p_b200
+    buf = randh(gen(53), 7, 1500).to(dt)
+    keep = buf.clone()
+    x, tok = buf[:4, :500], torch.full((4,), -7, dtype=torch.int32, device="cuda")
+    for bad in (buf[:4, 1:501], buf[1:5, :500], buf[:4, 499:999],
+                buf.view(-1)[1000:].as_strided((4, 500), (1000, 1))):
+        with pytest.raises(p2p_b200.P2PError) as e:
+            ctx.logits_pick(x, tok, out=bad)
+        assert e.value.status == p2p_b200.P2P_ERR_INVALID_ARG
+    ctx.sync()
+    assert torch.equal(buf, keep) and tok.tolist() == [-7] * 4
+    want = [int(np.argmax(r)) for r in x.float().cpu().numpy()]
+    for fine in (buf[:4, 500:1000], buf[3:7, 1000:], x):
+        ctx.logits_pick(x, tok, out=fine)
+        ctx.sync()
+        assert torch.equal(fine, keep[:4, :500]) and tok.tolist() == want
