@@ -7,8 +7,9 @@
 // and only the codes c enter the tensor cores.  A 4-bit code in the low bits of an f16 is the
 // subnormal c * 2^-24 (c * 2^-20 one nibble higher), which the f16 MMA multiplies exactly: a word
 // of eight codes becomes four f16 pairs with one shift and four ANDs and no conversion.  The odd
-// nibbles' factor 16 goes into q (divided by 16 for those dims; exact down to f16's subnormals)
-// and into the final scale of the odd output dims.
+// nibbles' factor 16 goes into q (divided by 16 for those dims) and into the final scale of the odd
+// output dims.  A head's q enters times the power of two that puts its largest value at 2^14, taken
+// out of the scores again: divided by 16 as they were, values below 2^-10 lost bits.
 //     S^T[16 keys x 8 heads] = C_K[16 x 64] . Q^T[64 x 8],   O^T[64 x 8] += C_V^T[64 x 16] . P'^T
 // P' = p * s goes in as a high and a low f16 in the columns that up to four query heads leave free
 // (22 bits of the weight); eight heads fill the columns and P' is rounded to f16: 2^-11 of w (v - lo),
@@ -151,11 +152,12 @@ constexpr int heads_per_lane() {
   return G > 4 ? 2 : 1;
 }
 
-// A warp's query heads: B fragments of the four k-steps and the lane's heads' sums.
+// A warp's query heads: B fragments of the four k-steps, and the lane's heads' sums and the factors of
+// their products with the codes.
 template <int H>
 struct Query {
   uint32_t b[4][2];
-  float sum[H];
+  float sum[H], scale[H];
 };
 
 // From the G f16 rows at `q` (row stride 64): lane (gid, t) holds column gid's head, dims 8t .. 8t+7
@@ -169,11 +171,24 @@ __device__ __forceinline__ void load_query(const __half* q, float scale_log2, Qu
     w[0] = *reinterpret_cast<const uint4*>(q + head * 64 + 8 * t);
     w[1] = *reinterpret_cast<const uint4*>(q + head * 64 + 32 + 8 * t);
   }
+  // the head's largest value, as bits; 2^14 over its power of two (1 for zeros, infinities and NaN)
+  uint32_t top = 0u;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    top = __vmaxu2(top, __vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu));
+    top = __vmaxu2(top, __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
+  }
+  top = max(top & 0xffffu, top >> 16);
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const uint32_t expo =  // of the f32
+      __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(top)))) >> 23;
+  const uint32_t shift = top == 0u || top >= 0x7c00u ? 127u : 141u - expo + 127u;
+  const float up = __uint_as_float(shift << 23), down = __uint_as_float((254u - shift) << 23);
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t d01 = w[i].x, d23 = w[i].y, d45 = w[i].z, d67 = w[i].w;
-    const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
     uint32_t e[4] = {__byte_perm(d01, d45, 0x5410), __byte_perm(d01, d45, 0x7632),
                      __byte_perm(d23, d67, 0x5410), __byte_perm(d23, d67, 0x7632)};
 #pragma unroll
@@ -181,16 +196,18 @@ __device__ __forceinline__ void load_query(const __half* q, float scale_log2, Qu
       const __half2 h = *reinterpret_cast<const __half2*>(&e[k]);
       const float2 f = __half22float2(h);
       sum += f.x + f.y;
-      const __half2 s = (k & 1) ? __hmul2(h, sixteenth) : h;
-      out.b[2 * i + (k >> 1)][k & 1] = *reinterpret_cast<const uint32_t*>(&s);
+      const float by = (k & 1) ? 0.0625f * up : up;
+      out.b[2 * i + (k >> 1)][k & 1] = pack_h2(f.x * by, f.y * by);
     }
   }
   sum += __shfl_xor_sync(0xffffffffu, sum, 1);
   sum += __shfl_xor_sync(0xffffffffu, sum, 2);
   sum *= scale_log2;
 #pragma unroll
-  for (int e = 0; e < H; ++e)  // from a lane of column 2t + e
+  for (int e = 0; e < H; ++e) {  // from a lane of column 2t + e
     out.sum[e] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
+    out.scale[e] = scale_log2 * 16777216.f * __shfl_sync(0xffffffffu, down, 8 * t + 4 * e);
+  }
 }
 
 // kLogBias + x + log2 of the scale in a unit's parameters, from the bits of the f16: 0 to 0.09 too low
@@ -228,8 +245,7 @@ struct State {
 // get neither weight nor parameters.
 template <int H, bool FULL, int NJ>
 __device__ __forceinline__ void attend(const unsigned char* ks, const unsigned char* vs,
-                                         int pitch, int valid, float scale24, const Query<H>& q,
-                                         State<H>& st) {
+                                         int pitch, int valid, const Query<H>& q, State<H>& st) {
   const int lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
   constexpr uint32_t kPerm = 0x57463120u;
   const int row = (kPerm >> (4 * gid)) & 7;
@@ -249,13 +265,13 @@ __device__ __forceinline__ void attend(const unsigned char* ks, const unsigned c
              q.b[3][0], q.b[3][1]);
     float s, lo;
     q4_unpack(pa, s, lo);
-    s *= scale24;
 #pragma unroll
-    for (int e = 0; e < H; ++e) sc[2 * j][e] = fmaf(r[e], s, fmaf(lo, q.sum[e], -st.m[e]));
+    for (int e = 0; e < H; ++e)
+      sc[2 * j][e] = fmaf(r[e], s * q.scale[e], fmaf(lo, q.sum[e], -st.m[e]));
     q4_unpack(pb, s, lo);
-    s *= scale24;
 #pragma unroll
-    for (int e = 0; e < H; ++e) sc[2 * j + 1][e] = fmaf(r[2 + e], s, fmaf(lo, q.sum[e], -st.m[e]));
+    for (int e = 0; e < H; ++e)
+      sc[2 * j + 1][e] = fmaf(r[2 + e], s * q.scale[e], fmaf(lo, q.sum[e], -st.m[e]));
   }
   if (!FULL) {
 #pragma unroll
@@ -709,7 +725,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int h = warp % hb, sub = warp / hb;
   const bool active = sub < wph;
   const int kh = grp * 8 + h;
-  const float scale24 = a.scale_log2 * 16777216.f;
   constexpr int H = heads_per_lane<G>();
   Query<H> q;
   State<H> state;
@@ -854,10 +869,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
     if (valid >= 2 * kBlock && a.blocks == 2) {
-      attend<H, true, 4>(ks, vs, pitch, 2 * kBlock, scale24, q, state);
+      attend<H, true, 4>(ks, vs, pitch, 2 * kBlock, q, state);
     } else {
       for (int k = 0; k < a.blocks && valid > 0; ++k, valid -= kBlock) {
-        attend<H, false, 2>(ks, vs, pitch, valid, scale24, q, state);
+        attend<H, false, 2>(ks, vs, pitch, valid, q, state);
         ks += kBlock * pitch;
         vs += kBlock * pitch;
       }

@@ -1483,3 +1483,56 @@ def test_logits_refuse_an_out_that_overlaps_them(ctx, dt):
         ctx.logits_pick(x, tok, out=fine)
         ctx.sync()
         assert torch.equal(fine, keep[:4, :500]) and tok.tolist() == want
+
+
+@pytest.mark.parametrize("amp", [1e-5, 1e-4, 1e-3, 3e3])
+@pytest.mark.parametrize("heads", [(8, 8), (16, 4), (64, 8), (8, 1)])
+def test_decode_q4_queries_of_any_size(ctx, heads, amp):
+    """Queries down to f16's subnormal numbers over keys that make up for it: scores of the usual size
+    and the bound of attention64, with the MMAs' share of a score's error for 4-bit codes: four of them,
+    each of up to 17 addends cut off at 2^-22 of the largest, which is below 2^-14 (a subnormal code)
+    times the head's largest query value and counts 2^24 times the key's scale."""
+    import p2p_b200
+    hq, hkv = heads
+    past = [11, 40, 0, 333]
+    k_amp = min(1e4, 1.0 / amp)
+    c = Cache(54, "q4", 16, hq, hkv, [p + 1 for p in past])
+    c.k = quant4((k_amp * randh(gen(55), *c.k.shape[:2], hkv, D).float()).clamp(-6e4, 6e4).half())
+    scale = 0.8 / (amp * k_amp)
+    c.prm = p2p_b200.Params(hq, hkv, scale=scale)
+    q = (amp * randh(gen(56), 4, hq * D).float()).half()
+    q[0, :D] = 0
+    q[3, D:D + 40] = 0
+    out = torch.zeros_like(q)
+    ctx.attn_decode_kv(c.prm, q, None, None, c.k, c.v, i32(past), out, max_past=333,
+                       fused_prep=False, **c.kw())
+    ctx.sync()
+    grp = hq // hkv
+    for i, p in enumerate(past):
+        k, v = (t.repeat_interleave(grp, 1).permute(1, 0, 2) for t in c.keys64(i, p + 1))
+        qi = q[i].double().view(hq, 1, D)
+        s = scale * qi @ k.transpose(1, 2)                                 # [hq][1][keys]
+        w = torch.softmax(s, -1)
+        o = w @ v
+        lo = v.amin(-1, keepdim=True)
+        step = (k.amax(-1) - k.amin(-1))[:, None] / 14                     # the scale or more
+        e = 2.0 ** -11 + 2.0 ** -10 + scale * (qi.abs() @ k.abs().transpose(1, 2)) * 2.0 ** -18
+        e = e + 68 * 2.0 ** -12 * scale * qi.abs().amax(-1, keepdim=True) * step
+        t = (w * e) @ v.abs() + o.abs() * (w * e).sum(-1, keepdim=True)
+        t = t + (w @ v.abs()) * 2.0 ** -16 + 2.0 ** -11 * (w @ (v - lo)) + o.abs() * 2.0 ** -11 + 2.0 ** -24
+        assert_within(out[i].view(hq, D), o[:, 0], t[:, 0], f"sequence {i}")
+
+
+def test_decode_q4_infinite_queries_are_their_rows_alone(ctx):
+    past, hq, hkv = [300, 5, 0], 16, 4
+    c = Cache(57, "q4", 16, hq, hkv, [p + 1 for p in past])
+    q = randh(gen(58), 3, hq * D)
+    want, tol = (t.view(3, hq, D) for t in attention64(c, q, past, [1] * 3, False))
+    for r, h, d, x in ((0, 1, 3, math.inf), (1, 15, 60, -math.inf), (2, 0, 0, math.nan)):
+        q[r, h * D + d] = x
+        want[r, h] = math.nan
+    out = torch.zeros_like(q)
+    ctx.attn_decode_kv(c.prm, q, None, None, c.k, c.v, i32(past), out, max_past=300,
+                       fused_prep=False, **c.kw())
+    ctx.sync()
+    assert_nan_or_within(out.view(3, hq, D), want, tol, "q")
