@@ -63,14 +63,14 @@ constexpr int kMmaWarp = 8, kTmaWarp = 9, kLoadWarp0 = 12, kLoadWarps = 4;
 constexpr int kMarks = 16;
 constexpr int kSetup = 2;
 constexpr int kMinUnits = 3;  // of a CTA: fewer make more records than they save time
-constexpr int kMaxStages = 4;
+constexpr int kStages = 3, kMaxRaw = 2;  // operand tiles; copied rows of int8 and 4-bit caches
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 constexpr float kRescaleLog2 = 8.0f;
+// 3 operand tiles, not 4, leave more of the SM to the L1 cache (4 prompts of up to 4096 tokens: 350 us,
+// 368 with 4).
 // What differs by the cache's format: f16 tiles only move (kMoveF16), int8 and 4-bit rows are copied
 // into a ring of kRaw tiles first (4096 4-bit rows over 28000 keys: 2 and 3 of them take as long).
-// kStages: operand tiles.  3, not 4, leave more of the SM to the L1 cache (4 prompts of up to 4096
-//   tokens: 350 us, 368 with 4).
 // Registers: setmaxnreg splits what the launch gives (kThreads x kLaunchRegs) among the two softmax
 //   warpgroups, that of the issuing warps and that of the converting ones.  The f16 kernel has no
 //   converting warps and gives theirs to the others (4 prompts: 350 -> 335 us).  int8: 245 us for 512
@@ -79,8 +79,7 @@ constexpr float kRescaleLog2 = 8.0f;
 template <int KVF>
 struct Conf {
   static constexpr bool kMoveF16 = KVF == kKvF16;
-  static constexpr int kStages = 3;
-  static constexpr int kRaw = kMoveF16 ? 0 : 2;
+  static constexpr int kRaw = kMoveF16 ? 0 : kMaxRaw;
   static constexpr int kRowBytes = kMoveF16 ? 128 : KVF == kKvI8 ? 64 : 48;  // of a copied row
   static constexpr int kThreads = kMoveF16 ? 384 : 512, kLaunchRegs = kMoveF16 ? 168 : 128;
   static constexpr int kSoftmaxRegs = KVF == kKvI8 ? 176 : 184,
@@ -98,15 +97,15 @@ __device__ __forceinline__ uint32_t col_o(int w) { return uint32_t(w) * 256u + 1
 template <int KVF>
 struct __align__(1024) Tiles {
   __half q[2][2][BM * D];   // two items, two halves
-  __half kv[Conf<KVF>::kStages][2][BN * D];  // K, V
+  __half kv[kStages][2][BN * D];  // K, V
   unsigned char raw[Conf<KVF>::kRaw ? Conf<KVF>::kRaw : 1][2]
                    [Conf<KVF>::kRaw ? BN * Conf<KVF>::kRowBytes : 16];  // int8, 4 bits: their rows
 };
 struct __align__(128) Smem {
   float scale[kLoadWarps][2][D];  // int8: the head's scales, a copy per converting warp
   uint64_t q_full[2], q_free[2];
-  uint64_t kv_full[kMaxStages], kv_empty[kMaxStages];
-  uint64_t raw_full[kMaxStages], raw_empty[kMaxStages];
+  uint64_t kv_full[kStages], kv_empty[kStages];
+  uint64_t raw_full[kMaxRaw], raw_empty[kMaxRaw];
   uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];
   long long wsum[8];
   int z0, qt0, kh0, off0, n_units;  // the first item of the CTA's part, and where in it
@@ -406,7 +405,6 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
                       const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ ChunkArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  constexpr int kStages = Conf<KVF>::kStages;
   constexpr bool kMoveF16 = Conf<KVF>::kMoveF16;
   auto& tiles = *reinterpret_cast<Tiles<KVF>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));

@@ -55,7 +55,7 @@ using sm100::smem_u32;
 
 constexpr int kWarps = 8;                      // compute warps; warp 8 is the producer
 constexpr int kThreads = (kWarps + 1) * 32;
-constexpr int kBlock = 32;                     // keys per warp and tile
+constexpr int kBlock = 64;                     // keys per warp and tile
 constexpr int kMaxStages = 8;
 constexpr int kRec = 68;                       // acc[64], max, sum, 2 pad: 17 16-byte pieces
 constexpr int kJoin = 16;                      // records joined by one warp
@@ -65,14 +65,14 @@ constexpr float kNegBig = -1e30f;
 constexpr float kUp = 12.f, kTop = 15.5f;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 
-// Warps per head for a CTA of hb heads (1 .. 8); its tile is `blocks` (1 or 2) blocks per such warp.
+// Warps per head for a CTA of hb heads (1 .. 8); its tile is kBlock keys per such warp.
 __host__ __device__ constexpr int warps_per_head(int hb) {
   return hb >= 5 ? 1 : hb >= 3 ? 2 : hb == 2 ? 4 : 8;
 }
 // Bytes of one token's units of hb heads, as copied and as laid out in shared memory.
 __host__ __device__ constexpr int pitch_of(int hb) { return (hb * kQ4UnitBytes + 15) / 16 * 16; }
-__host__ __device__ constexpr int stage_bytes(int hb, int blocks) {
-  return 2 * kBlock * blocks * warps_per_head(hb) * pitch_of(hb);
+__host__ __device__ constexpr int stage_bytes(int hb) {
+  return 2 * kBlock * warps_per_head(hb) * pitch_of(hb);
 }
 
 struct __align__(16) StageMeta {
@@ -90,7 +90,6 @@ struct Shared {
   uint64_t full[kMaxStages], empty[kMaxStages];
   StageMeta meta[kMaxStages];
   long long wsum[kWarps];
-  long long total;
   int z0, t0;
   volatile int abort_flag;
 };
@@ -565,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grp = blockIdx.y;
   const int hb = HB ? HB : min(8, a.kv.hkv - 8 * grp), wph = warps_per_head(hb);
-  const int tile = kBlock * a.blocks * wph, pitch = pitch_of(hb), sbytes = 2 * tile * pitch;
+  const int tile = kBlock * wph, pitch = pitch_of(hb), sbytes = 2 * tile * pitch;
   const int n_groups = gridDim.y;
 
   // ---- the CTA's part of the list of tiles
@@ -600,8 +599,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (w == warp) upto += total;
     total += s.wsum[w];
   }
-  const int parts = int(min(static_cast<long long>(gridDim.x),
-                            (total + a.min_tiles - 1) / a.min_tiles));
+  const int parts = int(min(static_cast<long long>(gridDim.x), total));
   const int b = blockIdx.x;
   launch_dependents();  // the joining kernel may take the slots that become free
   if (tid == 0) a.joins[grp * gridDim.x + b] = make_int4(-1, 0, 0, 0);
@@ -868,13 +866,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         __syncwarp();
       }
     }
-    if (valid >= 2 * kBlock && a.blocks == 2) {
-      attend<H, true, 4>(ks, vs, pitch, 2 * kBlock, q, state);
-    } else {
-      for (int k = 0; k < a.blocks && valid > 0; ++k, valid -= kBlock) {
+    if (valid >= kBlock) {
+      attend<H, true, 4>(ks, vs, pitch, kBlock, q, state);
+    } else {  // the sequence's last keys, in two halves
+      for (int k = 0; k < 2 && valid > 0; ++k, valid -= kBlock / 2) {
         attend<H, false, 2>(ks, vs, pitch, valid, q, state);
-        ks += kBlock * pitch;
-        vs += kBlock * pitch;
+        ks += kBlock / 2 * pitch;
+        vs += kBlock / 2 * pitch;
       }
     }
     __syncwarp();
@@ -911,8 +909,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     bad = false;
   }
   if (i < n_tiles) {
-    // A wait ran out: the parts that are left end as bad ones, so that no other warp or CTA waits
-    // or joins in vain and the counters return to zero.
+    // A wait ran out: the parts that are left end as bad ones, so that no other warp waits in vain and
+    // the joining kernel writes none of them.
     Walk w(a.kv, a.at, tile, s.z0, s.t0);
     int done = segs;
     for (int k = 0; k < n_tiles; ++k, ++w.t) {
@@ -1031,10 +1029,8 @@ cudaError_t launch_decode_q4(const DecodeQ4Args& args, int num_sms, cudaStream_t
   if (!fn || ctas < 1) return cudaErrorInvalidValue;
   // the groups' stages: 8 heads each, the last one the rest
   const int rest = a.kv.hkv - 8 * (groups - 1);
-  a.blocks = 2;
-  a.stage_bytes = stage_bytes(rest, a.blocks);
-  if (groups > 1 && a.stage_bytes < stage_bytes(8, a.blocks))
-    a.stage_bytes = stage_bytes(8, a.blocks);
+  a.stage_bytes = stage_bytes(rest);
+  if (groups > 1 && a.stage_bytes < stage_bytes(8)) a.stage_bytes = stage_bytes(8);
   const int merge = warps_per_head(rest) > 1 ? kWarps * group * kRec * 4 : 0;
   static PerDeviceOnce attrs[40];
   int fixed = 0;  // the kernel's static shared memory
@@ -1048,8 +1044,8 @@ cudaError_t launch_decode_q4(const DecodeQ4Args& args, int num_sms, cudaStream_t
   }, &fixed);
   if (e != cudaSuccess) return e;
   a.stages = (kSmemBytes - fixed - merge) / a.stage_bytes;
+  if (a.stages < 1) return cudaErrorInvalidValue;  // (1 for one kv head of 8 query heads)
   if (a.stages > kMaxStages) a.stages = kMaxStages;
-  a.min_tiles = 1;
   const size_t smem = size_t(a.stages) * a.stage_bytes + merge;
   void* argv[] = {&a};
   cudaError_t le = cudaLaunchKernel(fn, dim3(unsigned(ctas), unsigned(groups)), dim3(kThreads),

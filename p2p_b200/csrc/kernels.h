@@ -334,7 +334,7 @@ struct DecodeQ4Args : AttnKvArgs {
   int4* joins;   // decode_q4_join_bytes(): per CTA the sequence to join, if any
   int32_t wait_deficit;
   // set by the launcher
-  int32_t stages, stage_bytes, min_tiles, blocks;
+  int32_t stages, stage_bytes;
 };
 size_t decode_q4_parts_bytes(int num_sms);
 size_t decode_q4_join_bytes(int num_sms);
