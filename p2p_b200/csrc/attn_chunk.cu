@@ -22,7 +22,9 @@
 // over 28000 keys: 1720 us, 1785).
 //   S_w = Q_w K^T (M128 N128 K64) -> TMEM; P_w to TMEM as f16; O_w += P_w V (M128 N64 K128). The
 // softmax: exp2 with the scale folded in, lazily rescaled (only when a row's maximum grows by
-// 2^8).  Every fourth pair of exponentials is a cubic on the FMA pipe (4096 f16 rows over 28000
+// 2^5); the largest weight is put at 2^10, so that as f16 one keeps its bits down to 2^-24 of it and
+// is lost below 2^-35 (put at 1, a row over a first key of no value and a tail 17 nats below it was
+// 44 % off; the times are the same).  Every fourth pair of exponentials is a cubic on the FMA pipe (4096 f16 rows over 28000
 // keys: 1450 us, 1670 with none; the first 5 of 16 pairs in a row: 1628), the others are f32 ones
 // rounded once (packed f16 ones round their argument, errors of up to 2^-9 of a weight, and took
 // as long); the row sums are taken in f32.
@@ -66,7 +68,9 @@ constexpr int kMinUnits = 3;  // of a CTA: fewer make more records than they sav
 constexpr int kStages = 3, kMaxRaw = 2;  // operand tiles; copied rows of int8 and 4-bit caches
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
-constexpr float kRescaleLog2 = 8.0f;
+// log2 of where a row's largest weight is put, and of how far it may grow before the row is rescaled:
+// together below f16's 2^16.
+constexpr float kUp = 10.0f, kRescaleLog2 = 5.0f;
 // 3 operand tiles, not 4, leave more of the SM to the L1 cache (4 prompts of up to 4096 tokens: 350 us,
 // 368 with 4).
 // What differs by the cache's format: f16 tiles only move (kMoveF16), int8 and 4-bit rows are copied
@@ -849,7 +853,7 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
         if (grow) m_raw = mx;
         // a score of NaN or +inf makes all of the row's weights NaN (inf - inf is NaN for that key
         // alone, and the cubic would lose it)
-        const float neg = !(mx < INFINITY) ? NAN : (m_raw == -INFINITY) ? 0.f : -m_raw * sl2;
+        const float neg = !(mx < INFINITY) ? NAN : (m_raw == -INFINITY) ? 0.f : kUp - m_raw * sl2;
         uint32_t pk[2][32];
         uint64_t ps[4] = {0, 0, 0, 0};  // f32 pairs
 #pragma unroll
@@ -968,7 +972,7 @@ __global__ void __launch_bounds__(Conf<KVF>::kThreads, 1)
                                      __uint_as_float(o[2]), __uint_as_float(o[3]));
           }
           // log2 units; a sum below 0: some page was refused
-          const float m2 = m_raw == -INFINITY ? -1e30f : m_raw * sl2;
+          const float m2 = m_raw == -INFINITY ? -1e30f : m_raw * sl2 - kUp;
           rec[16] = make_float4(m2, bad ? -1.f : l_run, 0.f, 0.f);
         }
       }

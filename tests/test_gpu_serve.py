@@ -1536,3 +1536,31 @@ def test_decode_q4_infinite_queries_are_their_rows_alone(ctx):
                        fused_prep=False, **c.kw())
     ctx.sync()
     assert_nan_or_within(out.view(3, hq, D), want, tol, "q")
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("gap", [13, 15, 17, 18])
+@pytest.mark.parametrize("heads,n,rows,copies", [((32, 8), 8192, 2, 60), ((32, 8), 32768, 2, 24),
+                                                 ((8, 1), 32768, 40, 150)], ids=str)
+def test_chunk_behind_a_strong_first_key(ctx, fmt, gap, heads, n, rows, copies):
+    """A first key of no value far above a long tail: the rows are what the tail's small weights make
+    of it.  (Hundreds of items over the same keys: each is one CTA's or two.)"""
+    (hq, hkv), g = heads, gen(60)
+    c = Cache(59, fmt, 64, hq, hkv, [n], per_channel=False)
+    at = c.at(0, torch.arange(n, device="cuda"))
+    v = 1 + 0.5 * randh(g, n, hkv, D)
+    v[0] = 0
+    k = torch.zeros(n, hkv, D, dtype=torch.float16, device="cuda")
+    k[0] = gap / 8
+    if fmt == "i8":
+        c.ks.fill_(1 / 64)
+        c.vs.fill_(1 / 32)
+    c.k[at], c.v[at] = c.stored(k, c.ks), c.stored(v, c.vs)
+    q = torch.ones(copies * rows, hq * D, dtype=torch.float16, device="cuda")
+    out = torch.zeros_like(q)
+    kw = c.kw() | {"block_table": c.table.repeat(copies, 1)}
+    ctx.attn_chunk_kv(c.prm, q, c.k, c.v, i32([n - rows] * copies), i32(range(0, len(q) + 1, rows)), out,
+                      max_len=n, **kw)
+    ctx.sync()
+    want, tol = attention64(c, q[:rows], [n - rows], [rows], True)
+    assert_within(out.view(copies, rows, hq * D), want, tol)
