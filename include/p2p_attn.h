@@ -304,7 +304,7 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
  * (which must not be inside a stream capture: P2P_ERR_INVALID_ARG) and never moved, so that
  * captured graphs stay valid; calls of one context that use it must not overlap on the GPU.  A
  * bad block-table entry keeps the sequence's output rows from being written, but with
- * fused_prep its new row may already be in the cache. */
+ * fused_prep its new row may already be in the cache.  A sequence has at most 2^31 - 4097 tokens. */
 
 /* Bytes of one token's row in a P2P_KV_Q4 cache (0 for num_kv_heads <= 0). */
 int64_t p2p_kv_q4_row_bytes(int32_t num_kv_heads);
@@ -318,15 +318,16 @@ p2p_status p2p_kv_quantize_q4(p2p_ctx* ctx, const void* src, void* dst, int64_t 
  * tokens of sequence i at positions past[i], past[i]+1, ...: q and k are normed (norm_w NULL:
  * not) and rotated exactly as p2p_qk_prep does it, k and v go to the sequence's cache rows of
  * those positions in the layout's format, and the rotated q to q_out [n_rows][ld_q] (NULL: not
- * wanted; qkv itself with ld_q = ld_qkv is fine, any other overlap with its rows is refused).  row_start (nseq + 1 values), past and offsets
- * are device int32 arrays; the rope table holds max_len rows or more.  Rows at and behind row_start[nseq] are left alone, in qkv's
- * outputs and in the cache.  A sequence with a negative entry or a negative number of rows,
- * past[i] + rows > max_len, rows beyond n_rows, kv_rows or max_blocks is skipped, and so is a row
- * whose block-table entry lies outside the pool; the next p2p_sync then returns P2P_ERR_KV_FULL.
- * (A sequence of no rows has nothing to skip.  Rows in front of row_start[0] are left alone, and
- * where row_start falls, so may be rows of the sequences around.)  Two sequences must not name the
- * same cache row.  qkv, q_out, norm_w, rope 8-byte aligned (ld_qkv, ld_q multiples of 4), cache
- * buffers 16-byte aligned. */
+ * wanted; qkv itself with ld_q = ld_qkv is fine, any other overlap with its rows is refused).
+ * row_start (nseq + 1 values), past and offsets are device int32 arrays; the rope table holds
+ * max_len rows or more.  Rows at and behind row_start[nseq] are left alone, in qkv's outputs and
+ * in the cache.  A sequence with a negative entry or a negative number of rows, past[i] + rows >
+ * max_len, rows beyond n_rows, kv_rows or max_blocks, or more than 2^31 - 4097 tokens is skipped,
+ * and so is a row whose block-table entry lies outside the pool; the next p2p_sync then returns
+ * P2P_ERR_KV_FULL.  (A sequence of no rows has nothing to skip.  Rows in front of row_start[0] are
+ * left alone, and where row_start falls, so may be rows of the sequences around.)  Two sequences
+ * must not name the same cache row.  qkv, q_out, norm_w, rope 8-byte aligned (ld_qkv, ld_q
+ * multiples of 4), cache buffers 16-byte aligned. */
 p2p_status p2p_kv_append(p2p_ctx* ctx, const p2p_attn_params* prm, const p2p_kv_layout* layout,
                          const void* qkv, int64_t ld_qkv, const void* norm_w, const void* rope,
                          void* k_cache, void* v_cache, int64_t kv_rows, const int32_t* offsets,
