@@ -304,7 +304,10 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
  * (which must not be inside a stream capture: P2P_ERR_INVALID_ARG) and never moved, so that
  * captured graphs stay valid; calls of one context that use it must not overlap on the GPU.  A
  * bad block-table entry keeps the sequence's output rows from being written, but with
- * fused_prep its new row may already be in the cache.  A sequence has at most 2^31 - 4097 tokens. */
+ * fused_prep its new row may already be in the cache.  A sequence of more than 2^31 - 4097 keys is
+ * skipped and reported as well.  Errors of the output: its rounding to f16, 2^-11 of the weights
+ * with 8 query heads per kv head (2^-22 with fewer), and what f32 sums of the scores lose; a key
+ * counts down to 2^-37 of the largest weight times its value scale. */
 
 /* Bytes of one token's row in a P2P_KV_Q4 cache (0 for num_kv_heads <= 0). */
 int64_t p2p_kv_q4_row_bytes(int32_t num_kv_heads);
@@ -322,9 +325,8 @@ p2p_status p2p_kv_quantize_q4(p2p_ctx* ctx, const void* src, void* dst, int64_t 
  * row_start (nseq + 1 values), past and offsets are device int32 arrays; the rope table holds
  * max_len rows or more.  Rows at and behind row_start[nseq] are left alone, in qkv's outputs and
  * in the cache.  A sequence with a negative entry or a negative number of rows, past[i] + rows >
- * max_len, rows beyond n_rows, kv_rows or max_blocks, or more than 2^31 - 4097 tokens is skipped,
- * and so is a row whose block-table entry lies outside the pool; the next p2p_sync then returns
- * P2P_ERR_KV_FULL.  (A sequence of no rows has nothing to skip.  Rows in front of row_start[0] are
+ * max_len, rows beyond n_rows, kv_rows or max_blocks is skipped, and so is a row whose
+ * block-table entry lies outside the pool; the next p2p_sync then returns P2P_ERR_KV_FULL.  (A sequence of no rows has nothing to skip.  Rows in front of row_start[0] are
  * left alone, and where row_start falls, so may be rows of the sequences around.)  Two sequences
  * must not name the same cache row.  qkv, q_out, norm_w, rope 8-byte aligned (ld_qkv, ld_q
  * multiples of 4), cache buffers 16-byte aligned. */
@@ -348,14 +350,16 @@ p2p_status p2p_kv_read(p2p_ctx* ctx, const p2p_kv_layout* layout, int32_t num_kv
 /* ATTN (kernels.js:268-319) of ragged prompt chunks over a cache of any layout: rotated query
  * row t of sequence i (row row_start[i] + t of q [n_rows][ld_q]) attends keys 0 .. past[i] + t
  * of that sequence, which must already be in the cache (p2p_kv_append), and its Hq heads go to
- * the same row of out [n_rows][ld_o].  Arrays and checks as in p2p_kv_append, except that a bad
- * block-table entry keeps all rows of the sequence that see it, and up to 256 / (Hq / Hkv)
- * tokens in front of them, from being written.  q and out 16-byte aligned (ld_q and ld_o
- * multiples of 8), not overlapping (refused); at most 2^31 - 1 rows of an f16 cache.  Cached values are
- * rounded to f16 once, the precision of an f16 cache, before they enter the tensor cores.  A row
- * is not touched by keys that it does not see, whatever their values (infinities, NaN); a head's
- * row is NaN where a score that it sees is NaN or +inf, or where all of them are -inf.  The
- * workspace is the one of the 4-bit decode above, under the same rules. */
+ * the same row of out [n_rows][ld_o].  Arrays and checks as in p2p_kv_append, except that a
+ * sequence of more than 2^31 - 4097 keys is skipped too, and that a bad block-table entry keeps
+ * all rows of the sequence that see it, and up to 256 / (Hq / Hkv) tokens in front of them, from
+ * being written.  q and out 16-byte aligned (ld_q and ld_o multiples of 8), not overlapping
+ * (refused); at most 2^31 - 1 rows of a cache, whatever its format.  Cached values are rounded to
+ * f16 once, the precision of an f16 cache, before they enter the tensor cores (one beyond 65504,
+ * which a rounded scale can give, is infinite there).  A row is not touched by keys that it does
+ * not see, whatever their values (infinities, NaN); a head's row is NaN where a score that it sees
+ * is NaN or +inf, or where all of them are -inf.  The workspace is the one of the 4-bit decode
+ * above, under the same rules. */
 p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
                              const p2p_kv_layout* layout, const void* q, int64_t ld_q,
                              const void* k_cache, const void* v_cache, int64_t kv_rows,

@@ -945,7 +945,7 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
                   "decode_kv: 4-bit caches need 16-byte aligned rows (ld_qkv and ld_o multiples "
                   "of 8), rope and norm weights");
     if (nseq == 0) return P2P_OK;
-    q.at = {past, nullptr, nseq, nseq, max_past + 1};
+    q.at = {past, nullptr, nseq, nseq, std::min(max_past + 1, p2p::kMaxKeys)};
     q.q = static_cast<const __half*>(qkv);
     q.ld_q = ld_qkv;
     q.out = static_cast<__half*>(out);

@@ -269,6 +269,9 @@ struct KvView {
 };
 // Ragged rows: those of sequence i are row_start[i] .. row_start[i+1]-1 at positions past[i]
 // and up; row_start nullptr: one row per sequence.
+// The attention kernels take max_len up to kMaxKeys: their sums of a key and a tile's length stay below
+// 2^31.  (A cache holds that many only where its pages repeat.)
+constexpr int32_t kMaxKeys = INT32_MAX - 4096;
 struct ChunkIndex {
   const int32_t* past;
   const int32_t* row_start;
@@ -289,7 +292,7 @@ struct AppendArgs {
   float eps;
   int32_t* err;
 };
-cudaError_t launch_kv_append(const AppendArgs& a, cudaStream_t s);
+cudaError_t launch_kv_append(const AppendArgs& a, int num_sms, cudaStream_t s);
 struct ReadArgs {
   KvView kv;
   ChunkIndex at;
@@ -297,8 +300,8 @@ struct ReadArgs {
   __half* v_out;
   int32_t* err;
 };
-cudaError_t launch_kv_read(const ReadArgs& a, cudaStream_t s);
-cudaError_t launch_quantize_q4(const void* src, void* dst, int64_t rows, int hkv,
+cudaError_t launch_kv_read(const ReadArgs& a, int num_sms, cudaStream_t s);
+cudaError_t launch_quantize_q4(const void* src, void* dst, int64_t rows, int hkv, int num_sms,
                                cudaStream_t s);
 struct AttnKvArgs {
   KvView kv;

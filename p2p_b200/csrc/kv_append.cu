@@ -307,12 +307,12 @@ __global__ void __launch_bounds__(kThreads)
 // A warp takes four groups of units of a row when that still fills the SMs' 32 warps twice over
 // (11.4k rows of 48 units into f16 pages: 35 us against 46 with one), else one (1 row: 2.7 us against
 // 3.7).
-static bool wide(int64_t rows, int64_t units) {
-  return rows * ((units + 15) / 16) >= int64_t(148) * 32 * 2;
+static bool wide(int64_t rows, int64_t units, int num_sms) {
+  return rows * ((units + 15) / 16) >= int64_t(num_sms) * 32 * 2;
 }
 template <template <int, int> class K, class A>
-static cudaError_t launch_rows(const A& a, int64_t units, cudaStream_t s) {
-  const bool w = wide(a.at.n_rows, units);
+static cudaError_t launch_rows(const A& a, int64_t units, int num_sms, cudaStream_t s) {
+  const bool w = wide(a.at.n_rows, units, num_sms);
   const int64_t groups = w ? (units + 15) / 16 : (units + 3) / 4;
   const int64_t blocks = (a.at.n_rows * groups * 32 + kThreads - 1) / kThreads;
   if (blocks >= INT32_MAX) return cudaErrorInvalidValue;
@@ -335,19 +335,19 @@ struct Read {
   }
 };
 
-cudaError_t launch_kv_append(const AppendArgs& a, cudaStream_t s) {
-  return launch_rows<Append>(a, a.hq + 2 * a.kv.hkv, s);
+cudaError_t launch_kv_append(const AppendArgs& a, int num_sms, cudaStream_t s) {
+  return launch_rows<Append>(a, a.hq + 2 * a.kv.hkv, num_sms, s);
 }
 
-cudaError_t launch_kv_read(const ReadArgs& a, cudaStream_t s) {
-  return launch_rows<Read>(a, 2 * a.kv.hkv, s);
+cudaError_t launch_kv_read(const ReadArgs& a, int num_sms, cudaStream_t s) {
+  return launch_rows<Read>(a, 2 * a.kv.hkv, num_sms, s);
 }
 
-cudaError_t launch_quantize_q4(const void* src, void* dst, int64_t rows, int hkv,
+cudaError_t launch_quantize_q4(const void* src, void* dst, int64_t rows, int hkv, int num_sms,
                                cudaStream_t s) {
   const int64_t units = rows * hkv;
   const int64_t want = (units * 8 + kThreads - 1) / kThreads;
-  const int blocks = int(want < 148 * 16 ? want : 148 * 16);
+  const int blocks = int(want < num_sms * 16 ? want : num_sms * 16);
   quantize_q4_kernel<<<blocks, kThreads, 0, s>>>(static_cast<const __half*>(src),
                                                  static_cast<unsigned char*>(dst), units, hkv,
                                                  q4_row_bytes(hkv));

@@ -19,15 +19,11 @@ struct SeqSpan {
   bool ok;
 };
 
-// A sequence's most keys: the kernels' sums of a key and a tile's length stay below 2^31.  (A cache
-// holds that many only where its pages repeat.)
-constexpr int kMaxKeys = INT32_MAX - 4096;
-
 __host__ __device__ __forceinline__ bool span_fits(const KvView& c, const ChunkIndex& x, int past,
                                                   int row0, int len, int off) {
   const int64_t end = int64_t(past) + len;
   return past >= 0 && row0 >= 0 && len >= 0 && int64_t(row0) + len <= x.n_rows &&
-         end <= x.max_len && end <= kMaxKeys &&
+         end <= x.max_len &&
          (c.table != nullptr ? end <= 0 || ((end - 1) >> c.shift) < c.max_blocks
                              : off >= 0 && int64_t(off) + end <= c.kv_rows);
 }

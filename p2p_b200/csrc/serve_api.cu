@@ -3,6 +3,7 @@
 // logits.  Host-side checks only; the kernels check what lives in device memory.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 
@@ -145,6 +146,7 @@ p2p_status p2p_kv_quantize_q4(p2p_ctx* ctx, const void* src, void* dst, int64_t 
     return fail(ctx, P2P_ERR_INVALID_ARG, "kv_quantize_q4: buffers must be 16-byte aligned");
   OnDevice g(p2p::ctx_device(ctx));
   return launched(ctx, p2p::launch_quantize_q4(src, dst, rows, num_kv_heads,
+                                               p2p::ctx_num_sms(ctx),
                                                static_cast<cudaStream_t>(stream)),
                   "kv_quantize_q4 launch");
 }
@@ -190,7 +192,8 @@ p2p_status p2p_kv_append(p2p_ctx* ctx, const p2p_attn_params* prm, const p2p_kv_
   a.eps = p2p::eff_eps_of(prm);
   a.err = p2p::ctx_dev_err(ctx);
   OnDevice g(p2p::ctx_device(ctx));
-  return launched(ctx, p2p::launch_kv_append(a, static_cast<cudaStream_t>(stream)),
+  return launched(ctx, p2p::launch_kv_append(a, p2p::ctx_num_sms(ctx),
+                                             static_cast<cudaStream_t>(stream)),
                   "kv_append launch");
 }
 
@@ -216,7 +219,8 @@ p2p_status p2p_kv_read(p2p_ctx* ctx, const p2p_kv_layout* layout, int32_t num_kv
   a.v_out = static_cast<__half*>(v_out);
   a.err = p2p::ctx_dev_err(ctx);
   OnDevice g(p2p::ctx_device(ctx));
-  return launched(ctx, p2p::launch_kv_read(a, static_cast<cudaStream_t>(stream)),
+  return launched(ctx, p2p::launch_kv_read(a, p2p::ctx_num_sms(ctx),
+                                           static_cast<cudaStream_t>(stream)),
                   "kv_read launch");
 }
 
@@ -245,7 +249,7 @@ p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
                 "attn_chunk_kv: q and out must be 16-byte aligned, ld_q and ld_o multiples of 8");
   if (p2p::rows_overlap(q, ld_q * 2, qw * 2, out, ld_o * 2, qw * 2, n_rows))
     return fail(ctx, P2P_ERR_INVALID_ARG, "attn_chunk_kv: q and out overlap");
-  a.at = {past, row_start, nseq, n_rows, max_len};
+  a.at = {past, row_start, nseq, n_rows, std::min(max_len, p2p::kMaxKeys)};
   a.q = static_cast<const __half*>(q);
   a.ld_q = ld_q;
   a.out = static_cast<__half*>(out);

@@ -1564,3 +1564,27 @@ def test_chunk_behind_a_strong_first_key(ctx, fmt, gap, heads, n, rows, copies):
     ctx.sync()
     want, tol = attention64(c, q[:rows], [n - rows], [rows], True)
     assert_within(out.view(copies, rows, hq * D), want, tol)
+
+
+@pytest.mark.parametrize("fmt,op", [("f16", "chunk"), ("i8", "chunk"), ("q4", "chunk"), ("q4", "decode")])
+def test_sequences_near_the_end_of_32_bits_are_refused(ctx, fmt, op):
+    """A table whose entries repeat one page of 4096 tokens: from 2^31 - 4096 keys on, a sequence is
+    skipped and reported, and its neighbour is computed."""
+    import p2p_b200
+    c = Cache(61, fmt, 4096, 8, 1, [4096])
+    n, top = 2**31 // 4096, 2**31 - 4096
+    c.table = c.table.expand(2, 1).repeat(1, n).contiguous()
+    q = randh(gen(62), 2, 8 * D)
+    for past in (top - 1, 2**31 - 2):
+        out = torch.full_like(q, 7.0)
+        if op == "chunk":
+            ctx.attn_chunk_kv(c.prm, q, c.k, c.v, i32([past, 600]), i32([0, 1, 2]), out,
+                              max_len=2**31 - 1, **c.kw())
+        else:
+            ctx.attn_decode_kv(c.prm, q, None, None, c.k, c.v, i32([past, 600]), out,
+                               max_past=2**31 - 2, fused_prep=False, **c.kw())
+        with pytest.raises(p2p_b200.KvFullError):
+            ctx.sync()
+        want, tol = attention64(c, q[1:], [600], [1], op == "chunk")
+        assert (out[0] == 7).all()
+        assert_within(out[1:], want, tol)

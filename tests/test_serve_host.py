@@ -211,16 +211,3 @@ def test_rows_overlap(tmp_path):
                     for at, p, w in ((a, pa, wa), (b, pb, wb)))
         assert bool(int(got)) == bool(one & two), (a, pa, wa, b, pb, wb, n)
     assert out[-2:] == ["0", "1"]
-
-
-def test_the_longest_sequence(host_rows):
-    """Pages that repeat can make a sequence as long as its table: up to 2^31 - 4097 tokens fit, so that
-    a position plus a tile stays below 2^31."""
-    top = I32_MAX - 4096
-    table = [5] * (2**31 // 4096)
-    for past, rows, fits in ((top - 2, 2, True), (top - 1, 2, False), (top, 1, False), (top, 0, True),
-                             (I32_MAX - 1, 1, False), (2**30, 2, True)):
-        ok, at = host_rows(True, 8, past, 0, rows, rows, I32_MAX, shift=12, table=table)
-        assert ok == fits
-        if ok:
-            assert at == [5 * 4096 + (past + j) % 4096 for j in range(rows)]
