@@ -34,12 +34,12 @@
 // and worked out key by key if such a V is the cause.  (Looking through those tiles of V before
 // they are multiplied cost 4 prompts of 4096 tokens 384 -> 479 us, this 384 -> 389.)
 //
-// What bounds it.  Long chunks: the two softmax warps of each scheduler (4096 rows of 32 heads over
-// 28000 keys: 1425 us in f16, 708 TFLOP/s, 1580 us in 4 bits, 640, 1660 us in int8, 608).  Prompts
-// of up to 4096 tokens: 334 us for four, 579 TFLOP/s of the causal half. Short chunks: latency, 2.3
+// What bounds it.  Long chunks: a tile's chain in the two softmax warps of each scheduler (4096 rows of
+// 32 heads over 28000 keys: 1455 us in f16, 693 TFLOP/s, 1580 us in 4 bits, 638, 1670 us in int8, 604).
+// Prompts of up to 4096 tokens: 336 us for four, 576 TFLOP/s of the causal half. Short chunks: latency, 2.3
 // us to cut the list, 5 us to the first scores, about 2 us a tile whatever its rows (a warp has a
 // row per lane and all 128 keys), 5 us to join (16 sequences of 5 tokens over up to 4096 4-bit
-// keys: 39 us).
+// keys: 40 us).
 //
 // Every wait is bounded; one that gives up sets the error word, the other roles stop, the CTA frees
 // its TMEM and writes nothing more.

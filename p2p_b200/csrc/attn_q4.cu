@@ -29,9 +29,9 @@
 // joins; it is launched as a programmatic dependent, so it is resident when the first one ends.  The
 // order of the sums is that of the CTAs, so results repeat bit for bit, and nothing in the
 // workspace outlives a call.
-// What bounds it.  4 sequences of up to 131071 keys (240 MB of rows, 32 heads on 8): 58 us, 4.1 TB/s,
-// 63 % of the copy rate, at 57 % of the issue slots: 460 instructions per head and 64 keys, each block
-// a chain of dependent steps.  64 sequences of up to 8191 (167 MB): 46 us.  One of 1337: 9.9 us, latency.  (Three CTAs
+// What bounds it.  4 sequences of up to 131071 keys (240 MB of rows, 32 heads on 8): 59 us, 4.0 TB/s,
+// 62 % of the copy rate, at 58 % of the issue slots: 470 instructions per head and 64 keys, each block
+// a chain of dependent steps.  64 sequences of up to 8191 (167 MB): 47 us.  One of 1337: 9.7 us, latency.  (Three CTAs
 // per SM with 72 registers were slower, and so were 32 keys a stage: 70 us.)
 // Measured on the way (4 sequences, 390k keys, 8 kv heads x 4): joining by the last warp to arrive
 // (a fence, an atomic and the loads of up to 16 records per level, all one after the other) took

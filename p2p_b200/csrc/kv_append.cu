@@ -9,8 +9,8 @@
 // one row: their loads are all on their way before the row's sequence, position, page and rope row
 // are looked up, one after the other, once for all of them.
 //   Bound by issue: 12 prompts (11.4k rows of 32 + 8 + 8 heads, 142 MB) take 35 us, 62 % of the copy rate,
-// at 81 % of the issue slots (220 instructions a group); small calls by latency (one row: 2.7 us).  4-bit
-// units halve the bytes written but not the instructions (509 rows appended and read back: 9.7 us).
+// at 83 % of the issue slots (225 instructions a group); small calls by latency (one row: 2.8 us).  4-bit
+// units halve the bytes written but not the instructions (509 rows appended and read back: 10.1 us).
 #include "common.cuh"
 #include "kernels.h"
 #include "kv_view.cuh"
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kThreads)
 }  // namespace
 
 // A warp takes four groups of units of a row when that still fills the SMs' 32 warps twice over
-// (11.4k rows of 48 units into f16 pages: 35 us against 46 with one), else one (1 row: 2.7 us against
+// (11.4k rows of 48 units into f16 pages: 35 us against 46 with one), else one (1 row: 2.8 us against
 // 3.7).
 static bool wide(int64_t rows, int64_t units, int num_sms) {
   return rows * ((units + 15) / 16) >= int64_t(num_sms) * 32 * 2;
