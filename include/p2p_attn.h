@@ -305,7 +305,8 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
  * captured graphs stay valid; calls of one context that use it must not overlap on the GPU.  A
  * bad block-table entry keeps the sequence's output rows from being written, but with
  * fused_prep its new row may already be in the cache.  A sequence of more than 2^31 - 4097 keys is
- * skipped and reported as well.  Errors of the output: its rounding to f16, 2^-11 of the weights
+ * skipped and reported as well.  out may be qkv itself with ld_o = ld_qkv (the q columns are then
+ * replaced); any other overlap is refused.  Errors of the output: its rounding to f16, 2^-11 of the weights
  * with 8 query heads per kv head (2^-22 with fewer), and what f32 sums of the scores lose; a key
  * counts down to 2^-37 of the largest weight times its value scale. */
 

@@ -428,7 +428,8 @@ class Context:
                   v_scale: Optional[torch.Tensor] = None, stream=None):
         """QK_PREP of ragged prompt chunks into a cache of any layout (p2p_kv_append): rows
         row_start[i] .. row_start[i+1] of qkv are sequence i's tokens at positions past[i] and
-        up; their k and v go to the cache, their rotated q to q_out.  The cache tensors are as
+        up; their k and v go to the cache, their rotated q to q_out (qkv's own q columns, or rows
+        apart from it).  The cache tensors are as
         in attn_decode_kv; the rope table holds max_len rows or more."""
         n = past.numel()
         lay, rows, offs = self._layout(prm.num_kv_heads, k_cache, v_cache, n, offsets, block_table,

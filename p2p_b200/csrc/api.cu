@@ -28,6 +28,7 @@
 #pragma GCC visibility pop
 #include "host_internal.h"
 #include "kernels.h"
+#include "rows.h"
 
 struct p2p_ctx {
   int device = 0;
@@ -945,6 +946,13 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
                   "decode_kv: 4-bit caches need 16-byte aligned rows (ld_qkv and ld_o multiples "
                   "of 8), rope and norm weights");
     if (nseq == 0) return P2P_OK;
+    const int64_t qw = int64_t(prm->num_heads) * 64;
+    const int64_t row = fused_prep ? qw + 2 * int64_t(prm->num_kv_heads) * 64 : qw;
+    if (!(out == qkv && (ld_o == ld_qkv || nseq == 1)) &&
+        p2p::rows_overlap(qkv, ld_qkv * 2, row * 2, out, ld_o * 2, qw * 2, nseq))
+      return fail(ctx, P2P_ERR_INVALID_ARG,
+                  "decode_kv: out overlaps qkv (in place it starts with it and has its pitch, %lld)",
+                  (long long)ld_qkv);
     q.at = {past, nullptr, nseq, nseq, std::min(max_past + 1, p2p::kMaxKeys)};
     q.q = static_cast<const __half*>(qkv);
     q.ld_q = ld_qkv;

@@ -1588,3 +1588,33 @@ def test_sequences_near_the_end_of_32_bits_are_refused(ctx, fmt, op):
         want, tol = attention64(c, q[1:], [600], [1], op == "chunk")
         assert (out[0] == 7).all()
         assert_within(out[1:], want, tol)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("heads", [(32, 8), (8, 1), (72, 9)])
+def test_decode_q4_in_place_or_apart(ctx, heads, fused):
+    """out over the q columns gives what it gives apart; any other overlap with qkv is refused."""
+    import p2p_b200
+    (hq, hkv), past = heads, [700, 3, 64, 20, 5000]
+    n, w = len(past), hq * D
+    g = gen(63)
+    wide = (hq + 2 * hkv) * D
+    buf = randh(g, n + 1, wide + 24)
+    rope = rope_table(5001)
+
+    def call(c, x, out):
+        ctx.attn_decode_kv(c.prm, x[:, :wide], None, rope, c.k, c.v, i32(past), out, max_past=5000,
+                           fused_prep=fused, **c.kw())
+        ctx.sync()
+    a, b = (Cache(64, "q4", 16, hq, hkv, [p + 1 for p in past]) for _ in range(2))
+    keep, out = buf.clone(), torch.zeros(n, w, dtype=torch.float16, device="cuda")
+    call(a, buf[:n], out)
+    k = a.k.clone()
+    for bad in (buf[:n, 16:16 + w], buf[1:, :w], buf.view(-1)[:n * w].view(n, w)):
+        with pytest.raises(p2p_b200.P2PError) as e:
+            call(a, buf[:n], bad)
+        assert e.value.status == p2p_b200.P2P_ERR_INVALID_ARG
+    assert torch.equal(buf, keep) and torch.equal(a.k, k)
+    call(b, buf[:n], buf[:n, :w])
+    assert torch.equal(buf[:n, :w], out) and torch.equal(b.k, a.k) and torch.equal(b.v, a.v)
+    assert torch.equal(buf[:, w:], keep[:, w:]) and torch.equal(buf[n], keep[n])
