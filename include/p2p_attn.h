@@ -306,9 +306,9 @@ p2p_status p2p_attn_decode_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
  * bad block-table entry keeps the sequence's output rows from being written, but with
  * fused_prep its new row may already be in the cache.  A sequence of more than 2^31 - 4097 keys is
  * skipped and reported as well.  out may be qkv itself with ld_o = ld_qkv (the q columns are then
- * replaced); any other overlap is refused.  Errors of the output: its rounding to f16, 2^-11 of the weights
- * with 8 query heads per kv head (2^-22 with fewer), and what f32 sums of the scores lose; a key
- * counts down to 2^-37 of the largest weight times its value scale. */
+ * replaced); any other overlap is refused.  Errors of the output: its rounding to f16, 2^-11 of
+ * the weights with 8 query heads per kv head (2^-22 with fewer), and what f32 sums of the scores
+ * lose; a key counts down to 2^-37 of the largest weight times its value scale. */
 
 /* Bytes of one token's row in a P2P_KV_Q4 cache (0 for num_kv_heads <= 0). */
 int64_t p2p_kv_q4_row_bytes(int32_t num_kv_heads);
@@ -327,10 +327,11 @@ p2p_status p2p_kv_quantize_q4(p2p_ctx* ctx, const void* src, void* dst, int64_t 
  * max_len rows or more.  Rows at and behind row_start[nseq] are left alone, in qkv's outputs and
  * in the cache.  A sequence with a negative entry or a negative number of rows, past[i] + rows >
  * max_len, rows beyond n_rows, kv_rows or max_blocks is skipped, and so is a row whose
- * block-table entry lies outside the pool; the next p2p_sync then returns P2P_ERR_KV_FULL.  (A sequence of no rows has nothing to skip.  Rows in front of row_start[0] are
- * left alone, and where row_start falls, so may be rows of the sequences around.)  Two sequences
- * must not name the same cache row.  qkv, q_out, norm_w, rope 8-byte aligned (ld_qkv, ld_q
- * multiples of 4), cache buffers 16-byte aligned. */
+ * block-table entry lies outside the pool; the next p2p_sync then returns P2P_ERR_KV_FULL.  (A
+ * sequence of no rows has nothing to skip.  Rows in front of row_start[0] are left alone, and
+ * where row_start falls, so may be rows of the sequences around.)  Two sequences must not name the
+ * same cache row.  qkv, q_out, norm_w, rope 8-byte aligned (ld_qkv, ld_q multiples of 4), cache
+ * buffers 16-byte aligned. */
 p2p_status p2p_kv_append(p2p_ctx* ctx, const p2p_attn_params* prm, const p2p_kv_layout* layout,
                          const void* qkv, int64_t ld_qkv, const void* norm_w, const void* rope,
                          void* k_cache, void* v_cache, int64_t kv_rows, const int32_t* offsets,
@@ -380,9 +381,9 @@ p2p_status p2p_attn_chunk_kv(p2p_ctx* ctx, const p2p_attn_params* prm,
  *   mask bit v of row i (bit v % 32 of word v / 32) clear: x = -inf
  * y = x rounded to the logits' type is stored in out when it is not NULL (out may be logits
  * itself, with the same ld; any other overlap is refused), and tok[i] is the smallest index of the
- * largest y above -inf (NaN never wins), or -1 when there is none.  Any of hist, repetition, presence, frequency,
- * bias_start and mask may be NULL.  Tokens outside the vocabulary are ignored.  With advance != 0,
- * a token >= 0 is appended to hist[i] and hist_len[i] and past[i] (when not NULL) grow by one,
+ * largest y above -inf (NaN never wins), or -1 when there is none.  Any of hist, repetition,
+ * presence, frequency, bias_start and mask may be NULL.  Tokens outside the vocabulary are ignored.
+ * With advance != 0, a token >= 0 is appended to hist[i] and hist_len[i] and past[i] (when not NULL) grow by one,
  * on the device; when hist_len[i] has reached hist_cap neither changes and the next p2p_sync
  * returns P2P_ERR_INVALID_ARG.  vocab at most P2P_MAX_VOCAB. */
 #define P2P_MAX_VOCAB 400000

@@ -61,7 +61,7 @@ constexpr int kRec = 68;                       // acc[64], max, sum, 2 pad: 17 1
 constexpr int kJoin = 16;                      // records joined by one warp
 constexpr float kNegBig = -1e30f;
 // log2 of where the largest weight * scale is put when the reference is set, and from where on it is
-// set again: 2^15.5 is below f16's 65504 with what log2_scale may be off.
+// set again: 2^15.5 is below f16's 65504 with what add_log2_scale may be off.
 constexpr float kUp = 12.f, kTop = 15.5f;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
 
