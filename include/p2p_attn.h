@@ -413,6 +413,73 @@ typedef struct p2p_logits {
 } p2p_logits;
 p2p_status p2p_logits_pick(p2p_ctx* ctx, const p2p_logits* args, void* stream);
 
+/* The parts of a decoder layer around its attention, in 8-bit integers: rows of codes with one f32
+ * scale each (a token's activations, or an output channel of a weight), value = code * scale.
+ *   p2p_read_rows_q8      rows of a table as values (the embedding lookup), or int8 rows read back
+ *   p2p_add_norm_q8       the residual addition and RMS norm (ADD_RMS, kernels.js:146-182)
+ *   p2p_gemm_q8           a projection, with a bias and the residual addition behind it; the LM head
+ *   p2p_gate_q8           gate and up projections with SILU_MUL (kernels.js:321-339) behind them
+ *   p2p_quantize_rows_q8  weights (once, from p2p_q4_to_f16's rows or any f16 / f32 ones) and
+ *                         activations between two products
+ * codes: rows of `cols` bytes, ld apart (q 16-byte aligned, ld a multiple of 16; what lies between
+ * two rows is neither read nor written); scale 4-byte aligned.  The entry points below refuse (but
+ * for what each says) outputs that overlap inputs or each other.  They use no workspace. */
+#define P2P_MAX_Q8_COLS 65536
+typedef struct p2p_q8_rows {
+  void* q;       /* int8 [rows][ld] */
+  float* scale;  /* [rows] */
+  int64_t ld;
+  int32_t rows;
+  int32_t cols;  /* at most P2P_MAX_Q8_COLS */
+} p2p_q8_rows;
+
+/* dst row i = codes of src row i (f16 or f32 [dst->rows][ld_src]): with a = max |x| over the row,
+ * scale = a / 127 and code = roundeven(127 x / a), in f32 (ties of f16 rows are exact).  A row whose a is below 2^-100 has
+ * scale 0 and codes 0; one that holds an infinity or a NaN has scale NaN and codes 0 (all that is
+ * made of it is NaN). */
+p2p_status p2p_quantize_rows_q8(p2p_ctx* ctx, const void* src, int64_t ld_src, int32_t dtype,
+                                const p2p_q8_rows* dst, void* stream);
+
+/* out row i [rows][ld_out] (f16 or f32) = (code * scale) * factor of src row index[i] (device int32
+ * array; NULL: row i, and then rows <= src->rows), rounded once to out's type.  An index of -1 (what
+ * p2p_logits_pick stores where no token is left) gives a row of zeros; another one outside the table
+ * gives zeros and P2P_ERR_INVALID_ARG at the next p2p_sync. */
+p2p_status p2p_read_rows_q8(p2p_ctx* ctx, const p2p_q8_rows* src, const int32_t* index, int64_t rows,
+                            float factor, void* out, int64_t ld_out, int32_t dtype, void* stream);
+
+/* For every row, in f32:  s = x + residual, rounded to dtype;  y = (s * weight) / sqrt(mean(s^2) + eps);
+ * s goes to sum, y (rounded to dtype) to y, and y's codes and scale (of the unrounded y, by the rule of
+ * p2p_quantize_rows_q8) to out.  residual, weight (then 1), sum, y and out.q may be NULL; without out.q,
+ * out.scale is not used.  out.rows and out.cols are the call's in any case.  sum or y may be x or residual themselves, with the same pitch.  A row whose sum of
+ * squares is not finite gives y NaN, scale NaN, codes 0.  (f32 rows: values below 2^60.) */
+typedef struct p2p_add_norm {
+  const void* x;        /* [rows][ld_x], f16 or f32 */
+  const void* residual; /* [rows][ld_r] */
+  const void* weight;   /* [cols] f16 */
+  void* sum;            /* [rows][ld_sum] */
+  void* y;              /* [rows][ld_y] */
+  int64_t ld_x, ld_r, ld_sum, ld_y;
+  p2p_q8_rows out;
+  int32_t dtype;
+  float eps; /* 0 selects 1e-5 */
+} p2p_add_norm;
+p2p_status p2p_add_norm_q8(p2p_ctx* ctx, const p2p_add_norm* args, void* stream);
+
+/* y[m][n] = (f32(sum_k x[m][k] * w[n][k]) * x.scale[m]) * w.scale[n] (+ bias[n]) (+ residual[m][n]),
+ * rounded to y's type (f16 or f32, dtype; the residual has the same type).  The sums are whole numbers,
+ * exact in 32 bits (any codes, -128 too).  x->cols = w->cols; y [x->rows][ld_y], w->rows values a row; bias f32
+ * or NULL; residual [x->rows][ld_r] or NULL, y itself with ld_r = ld_y included. */
+p2p_status p2p_gemm_q8(p2p_ctx* ctx, const p2p_q8_rows* w, const p2p_q8_rows* x, const float* bias,
+                       const void* residual, int64_t ld_r, void* y, int64_t ld_y, int32_t dtype,
+                       void* stream);
+
+/* h[m][n] = f16(act(g) * u), g and u the products of x with gate and up as in p2p_gemm_q8 (f32, no
+ * bias): act P2P_ACT_SILU g / (1 + exp(-g)), P2P_ACT_GELU (tanh form) g / (1 + exp(-2c (g + 0.044715 g^3))),
+ * c = sqrt(2 / pi).  gate and up have the same rows and cols; h [x->rows][ld_h]. */
+typedef enum p2p_act { P2P_ACT_SILU = 0, P2P_ACT_GELU = 1 } p2p_act;
+p2p_status p2p_gate_q8(p2p_ctx* ctx, const p2p_q8_rows* gate, const p2p_q8_rows* up,
+                       const p2p_q8_rows* x, int32_t act, void* h, int64_t ld_h, void* stream);
+
 /* Converts f16 cache rows [rows][Hkv][D] to the int8 format above (src 16-byte and dst 8-byte
  * aligned; the same restated rule the decode uses when it appends). */
 p2p_status p2p_kv_quantize_q8(p2p_ctx* ctx, const void* src, void* dst, int64_t rows,

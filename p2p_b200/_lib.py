@@ -96,6 +96,33 @@ class Logits(C.Structure):
     ]
 
 
+class Q8Rows(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("scale", C.c_void_p),
+        ("ld", C.c_int64),
+        ("rows", C.c_int32),
+        ("cols", C.c_int32),
+    ]
+
+
+class AddNorm(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("sum", C.c_void_p),
+        ("y", C.c_void_p),
+        ("ld_x", C.c_int64),
+        ("ld_r", C.c_int64),
+        ("ld_sum", C.c_int64),
+        ("ld_y", C.c_int64),
+        ("out", Q8Rows),
+        ("dtype", C.c_int32),
+        ("eps", C.c_float),
+    ]
+
+
 class Q4Matrix(C.Structure):
     _fields_ = [
         ("qweight", C.c_void_p),
@@ -106,6 +133,8 @@ class Q4Matrix(C.Structure):
     ]
 
 
+P2P_ACT_SILU = 0
+P2P_ACT_GELU = 1
 P2P_KV_F16 = 0
 P2P_KV_I8 = 1
 P2P_KV_Q4 = 2
@@ -178,6 +207,14 @@ PROTOTYPES = {
         _st, [_v, _pp, C.POINTER(KvLayout), _v, _i64, _v, _v, _i64, _v, _v, _v, _i32, _i64, _i32,
               _v, _i64, _v]),
     "p2p_logits_pick": (_st, [_v, C.POINTER(Logits), _v]),
+    "p2p_quantize_rows_q8": (_st, [_v, _v, _i64, _i32, C.POINTER(Q8Rows), _v]),
+    "p2p_read_rows_q8": (
+        _st, [_v, C.POINTER(Q8Rows), _v, _i64, C.c_float, _v, _i64, _i32, _v]),
+    "p2p_add_norm_q8": (_st, [_v, C.POINTER(AddNorm), _v]),
+    "p2p_gemm_q8": (
+        _st, [_v, C.POINTER(Q8Rows), C.POINTER(Q8Rows), _v, _v, _i64, _v, _i64, _i32, _v]),
+    "p2p_gate_q8": (
+        _st, [_v, C.POINTER(Q8Rows), C.POINTER(Q8Rows), C.POINTER(Q8Rows), _i32, _v, _i64, _v]),
     "p2p_kv_quantize_q8": (_st, [_v, _v, _v, _i64, _i32, _v, _i32, _v]),
     "p2p_gemv_q4": (_st, [_v, C.POINTER(Q4Matrix), _v, _v, _i64, _v]),
     "p2p_qkv_gemv_prep": (

@@ -16,6 +16,11 @@ with device memory held in torch tensors and every kernel in libp2pattn.so:
     Context.attn_decode_kv ATTN at M=1 over int8, 4-bit and / or paged caches; 4-bit rows are made
                            by kv_append, by the fused decode or by kv_quantize_q4
     Context.logits_pick    ARGMAX of a batch under penalties, biases and grammar masks
+    Context.add_norm_q8    ADD_RMS kernels.js:146-182, with int8 rows and a scale per token
+    Context.gemm_q8 / gate_q8  projections of int8 rows (bias, residual; gate and up with SILU_MUL
+                           kernels.js:321-339 behind them)
+    Context.quantize_rows_q8 / read_rows_q8  f16 / f32 rows to int8 ones and back (the embedding
+                           lookup)
     Context.attn_bidir     VISION_ATTN vision-kernels.js:176-258, dispatched vision.js:271-276
     KVCache                K/V buffers engine.js:152-165 and ensureCapacity engine.js:274-304
     LfmAttention           the per-layer op pair + meta + rope + KV cache of createLfmEngine
@@ -62,6 +67,10 @@ def _stream(stream) -> C.c_void_p:
 
 _KV_FORMATS = {torch.float16: _lib.P2P_KV_F16, torch.int8: _lib.P2P_KV_I8,
                torch.uint8: _lib.P2P_KV_Q4}
+
+
+_ROW_TYPES = {torch.float16: _lib.P2P_F16, torch.float32: _lib.P2P_F32}
+_ACTS = {"silu": _lib.P2P_ACT_SILU, "gelu": _lib.P2P_ACT_GELU}
 
 
 @functools.lru_cache(maxsize=None)
@@ -609,6 +618,129 @@ class Context:
         self._chk(lib.p2p_kv_quantize_q8(self.h, _ptr(src), _ptr(dst), rows, hkv, _ptr(scale),
                                          scale.numel(), _stream(stream)))
         return dst
+
+    # -- 8-bit rows: the layer around its attention ----------------------------------------------
+    def _values(self, t: torch.Tensor, name: str, dtype=None, rows: int = -1, cols: int = -1) -> int:
+        """Checks f16 or f32 rows (of `dtype`, [rows][cols], where given) and returns their row
+        stride."""
+        shape, dt = t.shape, t.dtype
+        if (dt is not dtype if dtype is not None else dt not in _ROW_TYPES) or \
+                t.get_device() != self.device or len(shape) != 2 or \
+                rows >= 0 and shape[0] != rows or cols >= 0 and shape[1] != cols or \
+                shape[1] > 1 and t.stride(1) != 1:
+            _refuse(f"{name}: {dtype or 'f16 or f32'} [{rows if rows >= 0 else 'rows'}]"
+                    f"[{cols if cols >= 0 else 'cols'}] on device {self.device} needed, "
+                    f"got {tuple(shape)} {dt} on {t.device}")
+        return t.stride(0) if shape[0] > 1 else shape[1]
+
+    def _q8(self, q: torch.Tensor, scale: torch.Tensor, name: str) -> "_lib.Q8Rows":
+        """Checks int8 rows and their scales and returns the C view."""
+        shape = q.shape
+        if q.dtype is not torch.int8 or q.get_device() != self.device or len(shape) != 2 or \
+                shape[1] > 1 and q.stride(1) != 1:
+            _refuse(f"{name}: int8 [rows][cols] on device {self.device} needed, "
+                    f"got {tuple(shape)} {q.dtype} on {q.device}")
+        n, k = shape
+        return _lib.Q8Rows(q.data_ptr(), self._floats(scale, n, name + " scales"),
+                           q.stride(0) if n > 1 else (k + 15) & -16, n, k)
+
+    def _new_q8(self, q, scale, rows: int, cols: int, device):
+        """int8 rows on 16-byte boundaries and their scales, where the caller has none."""
+        if q is None:
+            q = torch.empty((rows, (cols + 15) & -16), dtype=torch.int8, device=device)[:, :cols]
+        if scale is None:
+            scale = torch.empty(rows, dtype=torch.float32, device=device)
+        if tuple(q.shape) != (rows, cols):
+            _refuse(f"q: [{rows}][{cols}] needed, got {tuple(q.shape)}")
+        return q, scale
+
+    def quantize_rows_q8(self, src: torch.Tensor, q: Optional[torch.Tensor] = None,
+                         scale: Optional[torch.Tensor] = None, stream=None):
+        """f16 or f32 rows [rows][cols] -> int8 rows and a scale for each (p2p_quantize_rows_q8):
+        (q, scale).  A weight's rows are its output channels."""
+        ld = self._values(src, "src")
+        q, scale = self._new_q8(q, scale, *src.shape, src.device)
+        d = self._q8(q, scale, "q")
+        st = lib.p2p_quantize_rows_q8(self.h, src.data_ptr(), ld, _ROW_TYPES[src.dtype],
+                                      C.byref(d), self._stream(stream))
+        if st:
+            self._chk(st)
+        return q, scale
+
+    def read_rows_q8(self, q: torch.Tensor, scale: torch.Tensor, out: torch.Tensor, *,
+                     index: Optional[torch.Tensor] = None, factor: float = 1.0, stream=None):
+        """Rows index[i] (without index: row i) of int8 rows as values times `factor`, into out
+        [rows][cols] (f16 or f32): the embedding lookup (p2p_read_rows_q8).  index -1 gives
+        zeros."""
+        s = self._q8(q, scale, "q")
+        ld, n = self._values(out, "out", cols=s.cols), out.shape[0]
+        st = lib.p2p_read_rows_q8(
+            self.h, C.byref(s), None if index is None else self._ints(index, n, "index"), n,
+            factor, out.data_ptr(), ld, _ROW_TYPES[out.dtype], self._stream(stream))
+        if st:
+            self._chk(st)
+        return out
+
+    def add_norm_q8(self, x: torch.Tensor, weight: Optional[torch.Tensor],
+                    q: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, *,
+                    residual: Optional[torch.Tensor] = None,
+                    sum_out: Optional[torch.Tensor] = None, y: Optional[torch.Tensor] = None,
+                    eps: float = 1e-5, stream=None):
+        """Residual addition and RMS norm (p2p_add_norm_q8): sum_out = x + residual (may be
+        either of them), y the normed rows, (q, scale) their int8 rows; returns (q, scale)."""
+        dt, (m, k) = x.dtype, x.shape
+        g = _lib.AddNorm()
+        g.x, g.ld_x = x.data_ptr(), self._values(x, "x")
+        if residual is not None:
+            g.residual, g.ld_r = residual.data_ptr(), self._values(residual, "residual", dt, m, k)
+        if weight is not None:
+            if weight.dtype is not torch.float16 or weight.get_device() != self.device or \
+                    weight.numel() != k or not weight.is_contiguous():
+                _refuse(f"weight: {k} contiguous f16 values on device {self.device} needed")
+            g.weight = weight.data_ptr()
+        if sum_out is not None:
+            g.sum, g.ld_sum = sum_out.data_ptr(), self._values(sum_out, "sum_out", dt, m, k)
+        if y is not None:
+            g.y, g.ld_y = y.data_ptr(), self._values(y, "y", dt, m, k)
+        q, scale = self._new_q8(q, scale, m, k, x.device)
+        g.out = self._q8(q, scale, "q")
+        g.dtype, g.eps = _ROW_TYPES[dt], eps
+        st = lib.p2p_add_norm_q8(self.h, C.byref(g), self._stream(stream))
+        if st:
+            self._chk(st)
+        return q, scale
+
+    def gemm_q8(self, w, x: torch.Tensor, x_scale: torch.Tensor, y: torch.Tensor, *,
+                bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                stream=None):
+        """y = x . w^T of int8 rows x [M][K] and w = (codes [N][K], scales), times both scales,
+        plus bias [N] (f32) and residual [M][N] (may be y), into y (f16 or f32; p2p_gemm_q8)."""
+        wr, xr = self._q8(w[0], w[1], "w"), self._q8(x, x_scale, "x")
+        ld_y, dt = self._values(y, "y", None, xr.rows, wr.rows), y.dtype
+        r_at, ld_r = None, 0
+        if residual is not None:
+            ld_r = self._values(residual, "residual", dt, xr.rows, wr.rows)
+            r_at = residual.data_ptr()
+        st = lib.p2p_gemm_q8(
+            self.h, C.byref(wr), C.byref(xr),
+            None if bias is None else self._floats(bias, wr.rows, "bias"), r_at, ld_r,
+            y.data_ptr(), ld_y, _ROW_TYPES[dt], self._stream(stream))
+        if st:
+            self._chk(st)
+
+    def gate_q8(self, gate, up, x: torch.Tensor, x_scale: torch.Tensor, h: torch.Tensor, *,
+                act: str = "silu", stream=None):
+        """h = act(x . gate^T) * (x . up^T) of int8 rows, into f16 h [M][F] (p2p_gate_q8); gate
+        and up are (codes [F][K], scales); act "silu" or "gelu" (tanh form)."""
+        gr, ur = self._q8(gate[0], gate[1], "gate"), self._q8(up[0], up[1], "up")
+        xr = self._q8(x, x_scale, "x")
+        if act not in _ACTS:
+            _refuse(f"act: one of {sorted(_ACTS)} needed, got {act!r}")
+        ld_h = self._values(h, "h", torch.float16, xr.rows, gr.rows)
+        st = lib.p2p_gate_q8(self.h, C.byref(gr), C.byref(ur), C.byref(xr), _ACTS[act],
+                             h.data_ptr(), ld_h, self._stream(stream))
+        if st:
+            self._chk(st)
 
     @staticmethod
     def q4(w) -> "_lib.Q4Matrix":

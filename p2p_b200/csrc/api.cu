@@ -475,6 +475,9 @@ p2p_status p2p_sync(p2p_ctx* ctx, void* stream) {
       return fail(ctx, P2P_ERR_CUDA,
                   "a kernel's dynamic shared memory did not start on the 1024-byte boundary "
                   "its tiles need; that work was skipped");
+    if (flags & p2p::kErrIndex)
+      return fail(ctx, P2P_ERR_INVALID_ARG,
+                  "read_rows_q8: a row index lies outside the table; zeros were written for it");
     if (flags & p2p::kErrHistFull)
       return fail(ctx, P2P_ERR_INVALID_ARG,
                   "logits_pick: a sequence's history has reached its capacity; its token was not "

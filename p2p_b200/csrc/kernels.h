@@ -372,11 +372,56 @@ struct LogitsArgs {
 };
 cudaError_t launch_logits_pick(const LogitsArgs& a, int dtype, cudaStream_t s);
 
+// ---- rows_q8.cu, gemm_q8.cu: 8-bit integer rows with a scale each --------------------------------
+struct Q8Rows {
+  int8_t* q;      // [rows][ld], 16-byte aligned rows
+  float* scale;   // [rows]
+  int64_t ld;
+  int32_t rows, cols;
+};
+struct RowsQ8Args {  // add_norm, or (norm 0) the quantisation of rows alone
+  const void* x;
+  const void* r;      // nullptr: none
+  const __half* w;    // nullptr: ones
+  void* sum;          // nullptr: not wanted; likewise y and out.q
+  void* y;
+  Q8Rows out;         // rows and cols are the call's
+  int64_t ld_x, ld_r, ld_sum, ld_y;
+  float eps;
+  int32_t norm;
+};
+cudaError_t launch_rows_q8(const RowsQ8Args& a, int dtype, int num_sms, cudaStream_t s);
+struct ReadQ8Args {
+  Q8Rows src;
+  const int32_t* index;  // nullptr: rows in order
+  int64_t rows;
+  float factor;
+  void* out;
+  int64_t ld_out;
+  int32_t* err;
+};
+cudaError_t launch_read_q8(const ReadQ8Args& a, int dtype, cudaStream_t s);
+
+constexpr int kActSilu = 0, kActGelu = 1;
+struct GemmQ8Args {
+  Q8Rows x, w;
+  Q8Rows up;          // gate form: w holds the gate's rows (up.q nullptr: a single product)
+  int32_t act;
+  const float* bias;  // [w.rows] or nullptr
+  const void* res;    // rows of y's type or nullptr
+  int64_t ld_res;
+  void* y;
+  int64_t ld_y;
+  int32_t* err;
+};
+cudaError_t launch_gemm_q8(const GemmQ8Args& a, int dtype, int num_sms, cudaStream_t s);
+
 // Device error word bits.
 constexpr int kErrPosBeyondCache = 1;
 constexpr int kErrTimeout = 2;  // a bounded device-side wait ran out; that work was not written
 constexpr int kErrOutTokFull = 4;  // argmax_step: the step index reached out_tok's capacity
 constexpr int kErrHistFull = 16;  // logits_pick: a sequence's history reached its capacity
+constexpr int kErrIndex = 32;     // read_rows_q8: a row index outside the table
 constexpr int kErrLayout = 8;  // a kernel found its shared memory misplaced; it wrote nothing
 cudaError_t launch_flash(const FlashArgs& a, cudaStream_t s);
 

@@ -1,0 +1,220 @@
+"""The 8-bit layer operators without a GPU: what their host side refuses, with made-up addresses and
+launchers that only count, and what the Python layer refuses before it."""
+import ctypes as C
+import subprocess
+
+import pytest
+
+from conftest import ROOT
+
+torch = pytest.importorskip("torch")
+
+BAD, UNSUPPORTED = 1, 7
+I32_MAX = 2**31 - 1
+MB = 1 << 20
+
+
+@pytest.fixture(scope="module")
+def api(tmp_path_factory):
+    import importlib.util
+    from p2p_b200._lib import PROTOTYPES
+    spec = importlib.util.spec_from_file_location("p2p_build", ROOT / "p2p_b200" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    so = tmp_path_factory.mktemp("q8_api") / "q8_api_host.so"
+    subprocess.run([build.nvcc(), *build.ARCH, *build.NVCC_FLAGS, "-shared", "-cudart", "static",
+                    str(ROOT / "tests" / "q8_api_host.cu"), "-o", str(so)], check=True,
+                   capture_output=True)
+    lib = C.CDLL(str(so))
+    for name in ("p2p_quantize_rows_q8", "p2p_read_rows_q8", "p2p_add_norm_q8", "p2p_gemm_q8",
+                 "p2p_gate_q8"):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = PROTOTYPES[name]
+    lib.host_message.restype = C.c_char_p
+    return lib
+
+
+def rows(at, n=4, k=64, ld=None, scale=None):
+    """int8 rows at a made-up address, their scales 2^16 bytes behind them unless given."""
+    from p2p_b200._lib import Q8Rows
+    return Q8Rows(at, at + 65536 if scale is None else scale, (k + 15) // 16 * 16 if ld is None
+                  else ld, n, k)
+
+
+def said(api, status, want, text=None):
+    assert status == want, api.host_message()
+    if text:
+        assert text in api.host_message().decode(), api.host_message()
+
+
+CTX = 1  # not NULL
+
+
+def test_null_context_is_a_status():
+    from p2p_b200 import _lib, lib
+    r, g = _lib.Q8Rows(), _lib.AddNorm()
+    assert lib.p2p_quantize_rows_q8(None, None, 0, 0, C.byref(r), None) == BAD
+    assert lib.p2p_read_rows_q8(None, C.byref(r), None, 0, 1.0, None, 0, 0, None) == BAD
+    assert lib.p2p_add_norm_q8(None, C.byref(g), None) == BAD
+    assert lib.p2p_gemm_q8(None, C.byref(r), C.byref(r), None, None, 0, None, 0, 0, None) == BAD
+    assert lib.p2p_gate_q8(None, C.byref(r), C.byref(r), C.byref(r), 0, None, 0, None) == BAD
+
+
+def quantize(api, dst, src=MB, ld=64, dtype=0):
+    return api.p2p_quantize_rows_q8(CTX, src, ld, dtype, C.byref(dst) if dst else None, None)
+
+
+def test_quantize_refusals(api):
+    before = api.host_launches()
+    good = rows(4 * MB)
+    said(api, quantize(api, good), 0)
+    assert api.host_launches() == before + 1
+    said(api, quantize(api, rows(4 * MB, n=0), src=None), 0)  # nothing to do
+    said(api, quantize(api, None), BAD, "NULL")
+    said(api, quantize(api, good, dtype=2), UNSUPPORTED)
+    said(api, quantize(api, good, src=None), BAD)
+    said(api, quantize(api, good, src=MB + 1), BAD)
+    said(api, quantize(api, good, src=MB + 2, dtype=1), BAD)
+    said(api, quantize(api, good, ld=63), BAD)
+    for bad in (rows(4 * MB, n=-1), rows(4 * MB, k=0), rows(4 * MB, k=65537), rows(4 * MB + 8),
+                rows(4 * MB, ld=72), rows(4 * MB, ld=48), rows(4 * MB, scale=5 * MB + 2),
+                rows(0, scale=MB)):
+        said(api, quantize(api, bad), BAD)
+    bad = rows(4 * MB)
+    bad.scale = None
+    said(api, quantize(api, bad), BAD)
+    # overlaps: codes in the source, scales in the source, scales in the codes
+    said(api, quantize(api, rows(MB + 128)), BAD, "overlaps")
+    said(api, quantize(api, rows(4 * MB, scale=MB + 64)), BAD, "overlaps")
+    said(api, quantize(api, rows(4 * MB, scale=4 * MB + 192)), BAD, "overlaps")
+    # columns of one buffer beside each other are apart
+    said(api, quantize(api, rows(MB + 128, ld=256), ld=128), 0)
+    assert api.host_launches() == before + 2
+
+
+def read(api, src, n=4, index=None, out=MB, ld=64, dtype=0, factor=1.0):
+    return api.p2p_read_rows_q8(CTX, C.byref(src) if src else None, index, n, factor, out, ld, dtype,
+                                None)
+
+
+def test_read_refusals(api):
+    before = api.host_launches()
+    good = rows(4 * MB)
+    said(api, read(api, good), 0)
+    said(api, read(api, good, n=9, index=8 * MB), 0)
+    said(api, read(api, good, n=0, out=None), 0)
+    assert api.host_launches() == before + 2
+    said(api, read(api, None), BAD)
+    said(api, read(api, good, n=5), BAD)  # more rows than there are, in order
+    said(api, read(api, good, n=-1, index=8 * MB), BAD)
+    said(api, read(api, good, n=I32_MAX + 1, index=8 * MB), BAD)
+    said(api, read(api, good, index=8 * MB + 2), BAD)
+    said(api, read(api, good, dtype=5), UNSUPPORTED)
+    said(api, read(api, good, out=None), BAD)
+    said(api, read(api, good, ld=63), BAD)
+    said(api, read(api, good, out=4 * MB + 64), BAD, "overlaps")
+    said(api, read(api, good, out=4 * MB + 65536), BAD, "overlaps")
+    said(api, read(api, good, n=9, index=MB + 8), BAD, "overlaps")
+    assert api.host_launches() == before + 2
+
+
+def norm(api, **kw):
+    from p2p_b200._lib import AddNorm
+    g = AddNorm()
+    g.x, g.residual, g.weight, g.sum, g.y = MB, 2 * MB, 3 * MB, 5 * MB, 6 * MB
+    g.ld_x = g.ld_r = g.ld_sum = g.ld_y = 64
+    g.out = rows(4 * MB)
+    for k, v in kw.items():
+        setattr(g, k, v)
+    return api.p2p_add_norm_q8(CTX, C.byref(g), None)
+
+
+def test_norm_refusals(api):
+    from p2p_b200._lib import Q8Rows
+    before = api.host_launches()
+    said(api, norm(api), 0)
+    said(api, norm(api, residual=None, weight=None, sum=None, y=None), 0)
+    said(api, norm(api, out=Q8Rows(None, None, 0, 4, 64)), 0)  # no codes wanted
+    said(api, norm(api, sum=MB), 0)                            # in place
+    said(api, norm(api, sum=2 * MB, y=MB), 0)
+    assert api.host_launches() == before + 5
+    said(api, norm(api, out=rows(4 * MB, n=0), x=None), 0)
+    said(api, api.p2p_add_norm_q8(CTX, None, None), BAD)
+    said(api, norm(api, out=Q8Rows(None, None, 0, 4, 64), sum=None, y=None), BAD, "all NULL")
+    said(api, norm(api, out=Q8Rows(None, None, 0, 4, 0)), BAD)
+    said(api, norm(api, out=Q8Rows(None, None, 0, -1, 64)), BAD)
+    said(api, norm(api, out=rows(4 * MB, ld=72)), BAD)
+    said(api, norm(api, dtype=3), UNSUPPORTED)
+    for eps in (-1.0, float("nan"), float("inf")):
+        said(api, norm(api, eps=eps), BAD, "eps")
+    for bad in ({"x": None}, {"x": MB + 1}, {"ld_x": 63}, {"ld_r": 63}, {"ld_sum": 63},
+                {"ld_y": 63}, {"weight": 3 * MB + 1}, {"y": 6 * MB + 1}):
+        said(api, norm(api, **bad), BAD)
+    for bad in ({"sum": MB, "ld_sum": 80}, {"sum": MB + 2}, {"y": 2 * MB + 128}, {"y": 5 * MB},
+                {"sum": 3 * MB}, {"sum": 4 * MB}, {"y": 4 * MB + 65536}, {"out": rows(MB)},
+                {"out": rows(3 * MB)}, {"out": rows(4 * MB, scale=MB + 4)}):
+        said(api, norm(api, **bad), BAD, "overlaps")
+    assert api.host_launches() == before + 5
+
+
+def gemm(api, w=None, x=None, bias=None, res=None, ld_r=0, y=MB, ld_y=32, dtype=0):
+    w = w or rows(4 * MB, n=32)
+    x = x or rows(8 * MB)
+    return api.p2p_gemm_q8(CTX, C.byref(w), C.byref(x), bias, res, ld_r, y, ld_y, dtype, None)
+
+
+def test_gemm_refusals(api):
+    before = api.host_launches()
+    said(api, gemm(api), 0)
+    said(api, gemm(api, bias=2 * MB, res=3 * MB, ld_r=40, dtype=1), 0)
+    said(api, gemm(api, res=MB, ld_r=32), 0)  # in place
+    said(api, gemm(api, x=rows(8 * MB, n=1), res=MB, ld_r=99), 0)
+    assert api.host_launches() == before + 4
+    said(api, gemm(api, x=rows(8 * MB, n=0), y=None), 0)
+    said(api, gemm(api, w=rows(8 * MB, n=0), y=None), 0)
+    said(api, gemm(api, x=rows(8 * MB, k=65)), BAD, "64 and 65")
+    said(api, gemm(api, dtype=2), UNSUPPORTED)
+    for bad in ({"y": None}, {"ld_y": 31}, {"y": MB + 1}, {"y": MB + 2, "dtype": 1},
+                {"res": 3 * MB, "ld_r": 31}, {"res": 3 * MB + 1, "ld_r": 32}, {"bias": 2 * MB + 2},
+                {"w": rows(4 * MB + 4, n=32)}, {"x": rows(8 * MB, ld=80 + 8)}):
+        said(api, gemm(api, **bad), BAD)
+    for bad in ({"res": MB, "ld_r": 48}, {"res": MB + 64, "ld_r": 32}, {"y": 4 * MB},
+                {"y": 8 * MB}, {"y": 8 * MB + 65536}, {"bias": MB + 64}):
+        said(api, gemm(api, **bad), BAD, "overlaps")
+    assert api.host_launches() == before + 4
+
+
+def gate(api, g=None, u=None, x=None, act=0, h=MB, ld_h=32):
+    g = g or rows(4 * MB, n=32)
+    u = u or rows(6 * MB, n=32)
+    x = x or rows(8 * MB)
+    return api.p2p_gate_q8(CTX, C.byref(g), C.byref(u), C.byref(x), act, h, ld_h, None)
+
+
+def test_gate_refusals(api):
+    before = api.host_launches()
+    said(api, gate(api), 0)
+    said(api, gate(api, act=1), 0)
+    said(api, gate(api, u=rows(4 * MB, n=32)), 0)  # the same weights twice
+    assert api.host_launches() == before + 3
+    said(api, gate(api, x=rows(8 * MB, n=0), h=None), 0)
+    for bad in ({"act": 2}, {"act": -1}, {"u": rows(6 * MB, n=31)}, {"u": rows(6 * MB, n=32, k=63)},
+                {"x": rows(8 * MB, k=63)}, {"h": None}, {"h": MB + 1}, {"ld_h": 31},
+                {"g": rows(4 * MB + 1, n=32)}):
+        said(api, gate(api, **bad), BAD)
+    for bad in ({"h": 4 * MB}, {"h": 6 * MB + 64}, {"h": 8 * MB}):
+        said(api, gate(api, **bad), BAD, "overlaps")
+    assert api.host_launches() == before + 3
+
+
+def test_python_refusals():
+    import p2p_b200
+    ctx = object.__new__(p2p_b200.Context)
+    ctx.h, ctx.device = None, 0
+    f = torch.zeros(3, 64, dtype=torch.float16)
+    q, s = torch.zeros(3, 64, dtype=torch.int8), torch.zeros(3)
+    for call in (lambda: ctx.quantize_rows_q8(f), lambda: ctx.read_rows_q8(q, s, f),
+                 lambda: ctx.add_norm_q8(f, None), lambda: ctx.gemm_q8((q, s), q, s, f),
+                 lambda: ctx.gate_q8((q, s), (q, s), q, s, f)):
+        with pytest.raises(p2p_b200.P2PError):  # nothing of this is on a device
+            call()
