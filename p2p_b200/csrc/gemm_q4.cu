@@ -26,13 +26,12 @@
 // word, every role of the CTA stops, the copies and MMAs in flight are waited for, the TMEM is
 // freed and the CTA returns.
 #include <cuda.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <climits>
-#include <mutex>
 
 #include "common.cuh"
+#include "gemm_common.cuh"
 #include "kernels.h"
 #include "qk_row.cuh"
 #include "sm100.cuh"
@@ -48,7 +47,6 @@ constexpr int kEpiWarps = 8;  // two per TMEM lane quarter, each owning 128 of t
 constexpr int kTmaWarp = kEpiWarps, kMmaWarp = kEpiWarps + 1;
 constexpr int kGemmThreads = 32 * (kEpiWarps + 2);
 constexpr uint32_t kATile = GBM * GBK * 2;  // 16 KB
-constexpr uint64_t kGemmWaitNs = 1000000000ull;
 
 // Output tile width BN (a multiple of the 64-column head).  PAIR = false: one CTA computes a
 // 128 x BN tile; PAIR = true: a cluster of two CTAs computes a 256 x BN tile with one
@@ -98,29 +96,6 @@ struct GemmParams {
   int32_t pos0;
   int32_t* err;
 };
-
-__device__ __forceinline__ bool gemm_wait(volatile int& abort_flag, uint64_t* bar,
-                                          uint32_t parity, int32_t* err) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (abort_flag) return false;
-    if (globaltimer_ns() - t0 > kGemmWaitNs) {
-      abort_flag = 1;
-      atomicOr(err, kErrTimeout);
-      return false;
-    }
-  }
-}
-
-// A wait of a warp: lane 0 polls, the verdict is shared.
-__device__ __forceinline__ bool gemm_wait_warp(volatile int& abort_flag, uint64_t* bar,
-                                               uint32_t parity, int32_t* err, int lane) {
-  bool r = true;
-  if (lane == 0) r = gemm_wait(abort_flag, bar, parity, err);
-  return __shfl_sync(0xffffffffu, r ? 1 : 0, 0) != 0;
-}
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -515,20 +490,6 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < 8; ++i) vals[i] = (float((word >> (4 * i)) & 15u) - z) * sc;
     store8(dst + idx * 8, vals);
   }
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  });
-  return fn;
 }
 
 // f16 [rows][width] with row pitch ld elements, boxes of 64 (k) x box_rows, 128-byte swizzle.
