@@ -2,13 +2,12 @@
 // the residual addition and RMS norm of a decoder layer (ADD_RMS,
 // src/scripts/lfm-engine/kernels.js:146-182), and read back as values (the embedding lookup).
 //
-// All three move bytes: a row is read once, kept in registers, reduced and written once.  A code is
-// 127 v / a, a = max |v|, rounded to even.  It is taken as v * (127 / a); a product so near a half that
-// its two roundings could have moved it is divided anew (half of the largest value is exactly 63.5, and
-// rows of f16 hold such values), so that ties of f16 rows are ties.  For the norm, v = (s * w) * rstd and rounding is monotone,
-// so max |v| = max |s * w| * rstd exactly: the sum of squares and the maximum go through one
-// reduction, and the row's values are not touched again until they are written.  Maxima are taken
-// over the bits of |v| as whole numbers, in which infinities and NaN come out largest.
+// All three move bytes: a row is read once, kept in registers (as it lies in memory, 4 words for 16
+// bytes), reduced and written once.  A code is 127 v / a, a = max |v|, rounded to even.  It is taken as
+// v * (127 / a); a product so near a half that its two roundings could have moved it is divided anew
+// (half of the largest value is exactly 63.5, and rows of f16 hold such values), so that ties of f16
+// rows are ties.  For the norm, v = (s * w) * rstd and rounding is monotone, so max |v| = max |s * w| *
+// rstd exactly: the sum of squares and the maximum go through one reduction.
 #include <algorithm>
 
 #include "common.cuh"
@@ -21,45 +20,155 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr float kTiny = 0x1p-100f;  // a row below it counts as zeros (127 / a stays finite)
 
-// 16 bytes of a row: V values.
-template <class T>
-struct Piece {
-  static constexpr int V = 16 / sizeof(T);
-  T e[V];
+// Two f32 operations in one instruction.
+union Pair {
+  uint64_t w;
+  float f[2];
 };
-
-// Values [0, n) of the V at p, the others 0.  Whole pieces in one load where rows are aligned.
-template <class T, int V>
-__device__ __forceinline__ void load_piece(const T* p, int n, bool wide, float (&v)[V]) {
-  union {
-    uint4 u;
-    T e[V];
-  } w;
-  if (wide && n >= V) {
-    w.u = *reinterpret_cast<const uint4*>(p);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) w.e[i] = i < n ? p[i] : from_f32<T>(0.f);
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = to_f32(w.e[i]);
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair p;
+  p.f[0] = a;
+  p.f[1] = b;
+  return p;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.w) : "l"(b.w));
+  return a;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.w) : "l"(b.w));
+  return a;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.w) : "l"(a.w), "l"(b.w));
+  return c;
+}
+// max(|a|, |b|, |c|), NaN if one of them is.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
-template <class T, int V>
-__device__ __forceinline__ void store_piece(T* p, int n, bool wide, const float (&v)[V]) {
-  union {
-    uint4 u;
-    T e[V];
-  } w;
-#pragma unroll
-  for (int i = 0; i < V; ++i) w.e[i] = from_f32<T>(v[i]);
-  if (wide && n >= V) {
-    *reinterpret_cast<uint4*>(p) = w.u;
+// 16 bytes of a row as they lie in memory: V values.
+template <class T>
+union Piece {
+  static constexpr int V = 16 / sizeof(T);
+  uint4 u;
+  T e[V];
+  __half2 h[4];
+  __device__ __forceinline__ Pair get(int i) const {  // values 2i and 2i + 1
+    if constexpr (sizeof(T) == 2) {
+      const float2 f = __half22float2(h[i]);
+      return pair(f.x, f.y);
+    } else {
+      return pair(e[2 * i], e[2 * i + 1]);
+    }
+  }
+  __device__ __forceinline__ void set(int i, Pair p) {
+    if constexpr (sizeof(T) == 2) {
+      h[i] = __floats2half2_rn(p.f[0], p.f[1]);
+    } else {
+      e[2 * i] = p.f[0];
+      e[2 * i + 1] = p.f[1];
+    }
+  }
+};
+
+// The columns of a row over the threads that hold it: a thread's piece is V neighbours, whatever the
+// rows' alignment (so that sums, and with them all results, do not depend on it).
+template <int V>
+struct Columns {
+  int first, threads, cols;  // the thread's place among those of the row
+  __device__ __forceinline__ int at(int piece, int e = 0) const {
+    return (piece * threads + first) * V + e;
+  }
+  __device__ __forceinline__ bool whole(int piece) const { return at(piece, V - 1) < cols; }
+};
+
+// Rows that start on 16-byte boundaries (WIDE) are read and written piece by piece.  Others go value by
+// value, neighbours in neighbouring lanes, so that each access of a warp is still one contiguous stretch,
+// and change hands through a warp's 512 bytes of shared memory (`turn`).  Value j of lane l is then the
+// warp's value 32 j + l.
+template <bool WIDE, class T>
+__device__ __forceinline__ void load_piece(Piece<T>& w, const T* row, const Columns<Piece<T>::V>& c,
+                                           int piece) {
+  constexpr int V = Piece<T>::V;
+  const int lane = threadIdx.x & 31, col = c.at(piece) - lane * V + lane;
+  if (WIDE && c.whole(piece)) {
+    w.u = *reinterpret_cast<const uint4*>(row + c.at(piece));
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < n) p[i] = w.e[i];
+    for (int j = 0; j < V; ++j) {
+      const int at = WIDE ? c.at(piece, j) : col + 32 * j;
+      w.e[j] = at < c.cols ? row[at] : from_f32<T>(0.f);
+    }
   }
+}
+// A loaded piece's values to the threads they belong to.
+template <bool WIDE, class T>
+__device__ __forceinline__ void turn_loaded(Piece<T>& w, uint4* turn) {
+  if constexpr (!WIDE) {
+    const int lane = threadIdx.x & 31;
+    T* t = reinterpret_cast<T*>(turn);
+#pragma unroll
+    for (int j = 0; j < Piece<T>::V; ++j) t[32 * j + lane] = w.e[j];
+    __syncwarp();
+    w.u = turn[lane];
+    __syncwarp();
+  }
+}
+template <bool WIDE, class T>
+__device__ __forceinline__ void store_piece(const Piece<T>& w, T* row, const Columns<Piece<T>::V>& c,
+                                            int piece, uint4* turn) {
+  constexpr int V = Piece<T>::V;
+  const int lane = threadIdx.x & 31;
+  if constexpr (WIDE) {
+    if (c.whole(piece)) {
+      *reinterpret_cast<uint4*>(row + c.at(piece)) = w.u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (c.at(piece, j) < c.cols) row[c.at(piece, j)] = w.e[j];
+    }
+  } else {
+    const int col = c.at(piece) - lane * V + lane;
+    const T* t = reinterpret_cast<const T*>(turn);
+    turn[lane] = w.u;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (col + 32 * j < c.cols) row[col + 32 * j] = t[32 * j + lane];
+    __syncwarp();
+  }
+}
+// The V norm weights of a piece (0 behind the row's end; ones without weights).
+template <bool WIDE, int V>
+__device__ __forceinline__ void load_weights(__half2 (&w)[V / 2], const __half* row,
+                                             const Columns<V>& c, int piece) {
+  union {
+    uint4 u4;
+    uint2 u2;
+    __half e[V];
+    __half2 h[V / 2];
+  } x;
+  if (!row) {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) x.h[j] = __float2half2_rn(1.f);
+  } else if (WIDE && c.whole(piece)) {
+    if constexpr (V == 8) x.u4 = *reinterpret_cast<const uint4*>(row + c.at(piece));
+    else x.u2 = *reinterpret_cast<const uint2*>(row + c.at(piece));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      x.e[j] = c.at(piece, j) < c.cols ? row[c.at(piece, j)] : __half(0.f);
+  }
+#pragma unroll
+  for (int j = 0; j < V / 2; ++j) w[j] = x.h[j];
+}
+__device__ __forceinline__ Pair wide2(__half2 h) {
+  const float2 f = __half22float2(h);
+  return pair(f.x, f.y);
 }
 
 // What a row's values are multiplied with, and its scale.  inv 0: all codes are 0.
@@ -69,56 +178,65 @@ struct RowScale {
 
 // Adding 1.5 * 2^23 rounds to a whole number, whose low byte is the code.
 template <int V>
-__device__ __forceinline__ void store_codes(int8_t* p, int n, const float (&v)[V],
-                                            const RowScale& sc) {
+__device__ __forceinline__ void store_codes(int8_t* row, const Columns<V>& c, int piece,
+                                            const Pair (&v)[V / 2], const RowScale& sc) {
   constexpr float kRound = 12582912.f;
-  float t[V];
-  bool near = false;
+  const Pair inv = pair(sc.inv, sc.inv), up = pair(kRound, kRound), down = pair(-kRound, -kRound);
+  const Pair minus = pair(-1.f, -1.f);
+  Pair t[V / 2];
+  float far = 0.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float c = v[i] * sc.inv;
-    t[i] = __fadd_rn(c, kRound);
-    near |= fabsf(__fsub_rn(c, __fsub_rn(t[i], kRound))) > 0.49996f;  // 127 * 2^-22 from a half
+  for (int i = 0; i < V / 2; ++i) {
+    const Pair q = mul2(v[i], inv);
+    t[i] = add2(q, up);
+    const Pair d = fma2(add2(t[i], down), minus, q);  // q less its code
+    far = max_abs3(far, d.f[0], d.f[1]);
   }
-  if (near) {
+  if (far > 0.49996f) {  // 127 * 2^-22 from a half
 #pragma unroll
-    for (int i = 0; i < V; ++i) t[i] = __fadd_rn(__fdiv_rn(__fmul_rn(v[i], 127.f), sc.top), kRound);
+    for (int i = 0; i < V / 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        t[i].f[j] = __fadd_rn(__fdiv_rn(__fmul_rn(v[i].f[j], 127.f), sc.top), kRound);
   }
   uint32_t u[V / 4];
 #pragma unroll
   for (int i = 0; i < V / 4; ++i) {
-    const uint32_t lo = __byte_perm(__float_as_uint(t[4 * i]), __float_as_uint(t[4 * i + 1]), 0x0040),
-                   hi = __byte_perm(__float_as_uint(t[4 * i + 2]), __float_as_uint(t[4 * i + 3]), 0x0040);
+    const uint32_t lo = __byte_perm(__float_as_uint(t[2 * i].f[0]), __float_as_uint(t[2 * i].f[1]),
+                                    0x0040),
+                   hi = __byte_perm(__float_as_uint(t[2 * i + 1].f[0]),
+                                    __float_as_uint(t[2 * i + 1].f[1]), 0x0040);
     u[i] = sc.inv == 0.f ? 0u : __byte_perm(lo, hi, 0x5410);
   }
-  if (n >= V) {
+  if (c.whole(piece)) {
+    int8_t* p = row + c.at(piece);
     if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
     else *reinterpret_cast<uint32_t*>(p) = u[0];
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < n) p[i] = int8_t(u[i / 4] >> (8 * (i % 4)));
+    for (int j = 0; j < V; ++j)
+      if (c.at(piece, j) < c.cols) row[c.at(piece, j)] = int8_t(u[j / 4] >> (8 * (j % 4)));
   }
 }
 
 struct RowSums {
-  uint32_t top;  // bits of the largest |value|
-  float ss;
+  float top, ss;  // the largest |value|, the sum of squares
 };
 
-// The sums of the threads of a row: `warps` consecutive warps of the block, `first` the row's first.
-__device__ __forceinline__ RowSums row_reduce(RowSums r, int warps, int first, int warp, int lane,
+// The sums of the threads of a row: a warp, or the `warps` of the block.
+__device__ __forceinline__ RowSums row_reduce(RowSums r, int warps, int warp, int lane,
                                               RowSums* part) {
-  r.top = __reduce_max_sync(0xffffffffu, r.top);
+  // as whole numbers, infinities and NaN come out largest
+  r.top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(r.top)));
 #pragma unroll
   for (int o = 16; o; o >>= 1) r.ss += __shfl_xor_sync(0xffffffffu, r.ss, o);
   if (warps == 1) return r;
   if (lane == 0) part[warp] = r;
-  asm volatile("bar.sync %0, %1;" ::"r"(1 + first), "r"(32 * warps) : "memory");
-  r = part[first];
+  __syncthreads();
+  r = part[0];
   for (int i = 1; i < warps; ++i) {
-    r.top = max(r.top, part[first + i].top);
-    r.ss += part[first + i].ss;
+    r.top = max_abs3(r.top, part[i].top, 0.f);
+    r.ss += part[i].ss;
   }
   return r;
 }
@@ -132,7 +250,7 @@ __device__ __forceinline__ RowScale row_scale(RowSums r, int cols, float eps) {
     s.rstd = r.ss <= 3.4028235e38f
                  ? __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(r.ss, float(cols)) + eps))
                  : nan;
-  const float a = s.top = __uint_as_float(r.top) * s.rstd;
+  const float a = s.top = r.top * s.rstd;
   if (a < kTiny) {
     s.inv = s.scale = 0.f;
   } else if (a <= 3.4028235e38f) {
@@ -145,190 +263,215 @@ __device__ __forceinline__ RowScale row_scale(RowSums r, int cols, float eps) {
   return s;
 }
 
-// A row in the registers of `warps` warps, NP pieces a lane.
-template <class T, int NP, bool NORM>
-__global__ void __launch_bounds__(kThreads)
-    rows_kernel(const __grid_constant__ RowsQ8Args a, int warps, int wide) {
-  constexpr int V = Piece<T>::V;
-  __shared__ RowSums part[kWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = warp / warps * warps;
-  const int64_t row = int64_t(blockIdx.x) * (kWarps / warps) + warp / warps;
-  grid_dependency_wait();
-  launch_dependents();
-  if (row >= a.out.rows) return;
-  const int cols = a.out.cols, step = warps * 32 * V;
-  const int col0 = ((warp - first) * 32 + lane) * V;
-  const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
-  float v[NP][V];
+// s = x + r as it is stored.  (Two f16 values add up to the same f16 value in one rounding and through
+// f32: what a f32 sum drops lies below half of the f16 sum's last place, and never on it.)
+template <class T>
+__device__ __forceinline__ void add_piece(Piece<T>& x, const Piece<T>& r) {
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int i = 0; i < NP; ++i)
-    load_piece<T, V>(x + col0 + i * step, cols - (col0 + i * step), wide, v[i]);
-  RowSums sums{0u, 0.f};
-  if constexpr (NORM) {
-    if (a.r) {
-      const T* r = static_cast<const T*>(a.r) + row * a.ld_r;
-      float u[NP][V];
+    for (int j = 0; j < 4; ++j) x.h[j] = __hadd2(x.h[j], r.h[j]);
+  } else {
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
-        load_piece<T, V>(r + col0 + i * step, cols - (col0 + i * step), wide, u[i]);
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = round_st<T>(v[i][j] + u[i][j]);
-    }
-    if (a.sum) {
-      T* s = static_cast<T*>(a.sum) + row * a.ld_sum;
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        store_piece<T, V>(s + col0 + i * step, cols - (col0 + i * step), wide, v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int c = col0 + i * step + j;
-        sums.ss += v[i][j] * v[i][j];
-        if (a.w) v[i][j] *= c < cols ? __half2float(a.w[c]) : 0.f;
-      }
-    }
+    for (int j = 0; j < 2; ++j) x.set(j, add2(x.get(j), r.get(j)));
   }
+}
+
+// A piece's part of the row's sums.
+template <bool NORM, bool WIDE, class T>
+__device__ __forceinline__ void sum_piece(RowSums& sums, Pair& ss, const Piece<T>& x,
+                                          const RowsQ8Args& a,
+                                          const Columns<Piece<T>::V>& c, int piece) {
+  constexpr int V = Piece<T>::V;
+  __half2 w[V / 2];
+  if constexpr (NORM) load_weights<WIDE, V>(w, a.w, c, piece);
 #pragma unroll
-  for (int i = 0; i < NP; ++i)
+  for (int j = 0; j < V / 2; ++j) {
+    Pair v = x.get(j);
+    if constexpr (NORM) {
+      ss = fma2(v, v, ss);
+      v = mul2(v, wide2(w[j]));
+    }
+    sums.top = max_abs3(sums.top, v.f[0], v.f[1]);
+  }
+}
+// A piece of what the call stores behind the reduction.
+template <bool NORM, bool WIDE, class T>
+__device__ __forceinline__ void finish_piece(const Piece<T>& x, const RowScale& sc,
+                                             const RowsQ8Args& a, int64_t row,
+                                             const Columns<Piece<T>::V>& c, int piece,
+                                             uint4* turn) {
+  constexpr int V = Piece<T>::V;
+  Pair v[V / 2];
+  __half2 w[V / 2];
+  if constexpr (NORM) load_weights<WIDE, V>(w, a.w, c, piece);
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      sums.top = max(sums.top, __float_as_uint(v[i][j]) & 0x7fffffffu);
-  sums = row_reduce(sums, warps, first, warp, lane, part);
-  const RowScale sc = row_scale<NORM>(sums, cols, a.eps);
+  for (int j = 0; j < V / 2; ++j) {
+    v[j] = x.get(j);
+    if constexpr (NORM) v[j] = mul2(mul2(v[j], wide2(w[j])), pair(sc.rstd, sc.rstd));
+  }
   if constexpr (NORM) {
-#pragma unroll
-    for (int i = 0; i < NP; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] *= sc.rstd;
     if (a.y) {
-      T* y = static_cast<T*>(a.y) + row * a.ld_y;
+      Piece<T> y;
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
-        store_piece<T, V>(y + col0 + i * step, cols - (col0 + i * step), wide, v[i]);
+      for (int j = 0; j < V / 2; ++j) y.set(j, v[j]);
+      store_piece<WIDE>(y, static_cast<T*>(a.y) + row * a.ld_y, c, piece, turn);
     }
     if (!a.out.q) return;
   }
-  int8_t* q = a.out.q + row * a.out.ld;
+  store_codes<V>(a.out.q + row * a.out.ld, c, piece, v, sc);
+}
+
+// The words of a piece as they are: what was computed from them before is not kept beside them.
+template <class T>
+__device__ __forceinline__ void keep_words(Piece<T>& x) {
+  asm volatile("" : "+r"(x.u.x), "+r"(x.u.y), "+r"(x.u.z), "+r"(x.u.w));
+}
+
+// A row in the registers of a warp (warps 1: a row a warp) or of a block of `warps` warps, NP pieces a
+// lane.
+template <class T, int NP, bool NORM, bool WIDE>
+__global__ void __launch_bounds__(kThreads)
+    rows_kernel(const __grid_constant__ RowsQ8Args a, int warps) {
+  __shared__ RowSums part[kWarps];
+  __shared__ uint4 turns[WIDE ? 1 : kWarps][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = warps == 1 ? int64_t(blockIdx.x) * kWarps + warp : blockIdx.x;
+  const int part_of = warps == 1 ? 0 : warp;
+  grid_dependency_wait();
+  launch_dependents();
+  if (row >= a.out.rows) return;
+  const Columns<Piece<T>::V> c{part_of * 32 + lane, warps * 32, a.out.cols};
+  uint4* turn = turns[WIDE ? 0 : warp];
+  const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+  Piece<T> v[NP];
 #pragma unroll
-  for (int i = 0; i < NP; ++i)
-    store_codes<V>(q + col0 + i * step, cols - (col0 + i * step), v[i], sc);
-  if (warp == first && lane == 0) a.out.scale[row] = sc.scale;
+  for (int i = 0; i < NP; ++i) load_piece<WIDE>(v[i], x, c, i);
+  if constexpr (NORM) {
+    if (a.r) {  // added as the two were loaded
+      const T* r = static_cast<const T*>(a.r) + row * a.ld_r;
+      Piece<T> u[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) load_piece<WIDE>(u[i], r, c, i);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) add_piece(v[i], u[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NP; ++i) turn_loaded<WIDE>(v[i], turn);
+  if constexpr (NORM) {
+    if (a.sum) {
+      T* s = static_cast<T*>(a.sum) + row * a.ld_sum;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) store_piece<WIDE>(v[i], s, c, i, turn);
+    }
+  }
+  RowSums sums{0.f, 0.f};
+  Pair ss = pair(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) sum_piece<NORM, WIDE>(sums, ss, v[i], a, c, i);
+  sums.ss = ss.f[0] + ss.f[1];
+  sums = row_reduce(sums, warps, warp, lane, part);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) keep_words(v[i]);
+  const RowScale sc = row_scale<NORM>(sums, a.out.cols, a.eps);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) finish_piece<NORM, WIDE>(v[i], sc, a, row, c, i, turn);
+  if (a.out.q && part_of == 0 && lane == 0) a.out.scale[row] = sc.scale;
 }
 
 // Rows too long for the registers of a block: read twice, a block a row.  The second reading takes
 // s from where the first one stored it (sum may be x or r).
-template <class T, bool NORM>
+template <class T, bool NORM, bool WIDE>
 __global__ void __launch_bounds__(kThreads)
-    long_rows_kernel(const __grid_constant__ RowsQ8Args a, int wide) {
-  constexpr int V = Piece<T>::V;
+    long_rows_kernel(const __grid_constant__ RowsQ8Args a) {
   __shared__ RowSums part[kWarps];
+  __shared__ uint4 turns[WIDE ? 1 : kWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x;
-  const int cols = a.out.cols;
   grid_dependency_wait();
   launch_dependents();
+  const Columns<Piece<T>::V> c{int(threadIdx.x), kThreads, a.out.cols};
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
   const T* r = NORM && a.r ? static_cast<const T*>(a.r) + row * a.ld_r : nullptr;
   T* s = NORM && a.sum ? static_cast<T*>(a.sum) + row * a.ld_sum : nullptr;
-  RowSums sums{0u, 0.f};
-  for (int c = threadIdx.x * V; c < cols; c += kThreads * V) {
-    float v[V], u[V];
-    load_piece<T, V>(x + c, cols - c, wide, v);
+  RowSums sums{0.f, 0.f};
+  Pair ss = pair(0.f, 0.f);
+  uint4* turn = turns[WIDE ? 0 : warp];
+  const int pieces = (c.cols + kThreads * Piece<T>::V - 1) / (kThreads * Piece<T>::V);
+  for (int i = 0; i < pieces; ++i) {
+    Piece<T> v, u;
+    load_piece<WIDE>(v, x, c, i);
     if (r) {
-      load_piece<T, V>(r + c, cols - c, wide, u);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = round_st<T>(v[j] + u[j]);
+      load_piece<WIDE>(u, r, c, i);
+      add_piece(v, u);
     }
-    if (s) store_piece<T, V>(s + c, cols - c, wide, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if constexpr (NORM) {
-        sums.ss += v[j] * v[j];
-        if (a.w) v[j] *= c + j < cols ? __half2float(a.w[c + j]) : 0.f;
-      }
-      sums.top = max(sums.top, __float_as_uint(v[j]) & 0x7fffffffu);
-    }
+    turn_loaded<WIDE>(v, turn);
+    if (s) store_piece<WIDE>(v, s, c, i, turn);
+    sum_piece<NORM, WIDE>(sums, ss, v, a, c, i);
   }
-  sums = row_reduce(sums, kWarps, 0, warp, lane, part);
-  const RowScale sc = row_scale<NORM>(sums, cols, a.eps);
-  T* y = NORM && a.y ? static_cast<T*>(a.y) + row * a.ld_y : nullptr;
-  int8_t* q = a.out.q ? a.out.q + row * a.out.ld : nullptr;
-  for (int c = threadIdx.x * V; c < cols; c += kThreads * V) {
-    float v[V], u[V];
-    load_piece<T, V>(s ? s + c : x + c, cols - c, wide, v);
+  sums.ss = ss.f[0] + ss.f[1];
+  sums = row_reduce(sums, kWarps, warp, lane, part);
+  const RowScale sc = row_scale<NORM>(sums, c.cols, a.eps);
+  for (int i = 0; i < pieces; ++i) {
+    Piece<T> v, u;
+    load_piece<WIDE>(v, s ? s : x, c, i);
     if (r && !s) {
-      load_piece<T, V>(r + c, cols - c, wide, u);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = round_st<T>(v[j] + u[j]);
+      load_piece<WIDE>(u, r, c, i);
+      add_piece(v, u);
     }
-    if constexpr (NORM) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (a.w) v[j] *= c + j < cols ? __half2float(a.w[c + j]) : 0.f;
-        v[j] *= sc.rstd;
-      }
-    }
-    if (y) store_piece<T, V>(y + c, cols - c, wide, v);
-    if (q) store_codes<V>(q + c, cols - c, v, sc);
+    turn_loaded<WIDE>(v, turn);
+    finish_piece<NORM, WIDE>(v, sc, a, row, c, i, turn);
   }
-  if (q && threadIdx.x == 0) a.out.scale[row] = sc.scale;
+  if (a.out.q && threadIdx.x == 0) a.out.scale[row] = sc.scale;
 }
 
 // Codes back to values: a warp takes up to kReadPieces pieces a lane of one row.
 constexpr int kReadPieces = 4;
-template <class T>
+template <class T, bool WIDE>
 __global__ void __launch_bounds__(kThreads)
-    read_kernel(const __grid_constant__ ReadQ8Args a, int segments, int wide) {
+    read_kernel(const __grid_constant__ ReadQ8Args a, int segments) {
   constexpr int V = Piece<T>::V;
+  __shared__ uint4 turns[WIDE ? 1 : kWarps][32];
   const int lane = threadIdx.x & 31;
   const int64_t unit = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   grid_dependency_wait();
   launch_dependents();
   const int64_t i = unit / segments;
   if (i >= a.rows) return;
-  const int col0 = (int(unit - i * segments) * kReadPieces * 32 + lane) * V;
+  const int col0 = int(unit - i * segments) * (kReadPieces * 32 * V);
+  const Columns<V> c{lane, 32, a.src.cols - col0};
   const int64_t row = a.index ? a.index[i] : i;
   const bool inside = row >= 0 && row < a.src.rows;
   if (!inside && row != -1 && lane == 0) atomicOr(a.err, kErrIndex);
   const float scale = inside ? a.src.scale[row] : 0.f;
-  const int8_t* q = a.src.q + (inside ? row : 0) * a.src.ld;
-  T* out = static_cast<T*>(a.out) + i * a.ld_out;
+  const int8_t* q = a.src.q + (inside ? row : 0) * a.src.ld + col0;
+  T* out = static_cast<T*>(a.out) + i * a.ld_out + col0;
   union {
     uint32_t u[V / 4];
     int8_t e[V];
   } w[kReadPieces];
 #pragma unroll
   for (int p = 0; p < kReadPieces; ++p) {
-    const int c = col0 + p * 32 * V, n = a.src.cols - c;
-#pragma unroll
-    for (int j = 0; j < V / 4; ++j) w[p].u[j] = 0;
-    if (!inside) continue;
-    if (n >= V) {
+    if (c.whole(p)) {
       if constexpr (V == 8) {
-        const uint2 u = *reinterpret_cast<const uint2*>(q + c);
+        const uint2 u = *reinterpret_cast<const uint2*>(q + c.at(p));
         w[p].u[0] = u.x;
         w[p].u[1] = u.y;
       } else {
-        w[p].u[0] = *reinterpret_cast<const uint32_t*>(q + c);
+        w[p].u[0] = *reinterpret_cast<const uint32_t*>(q + c.at(p));
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < n) w[p].e[j] = q[c + j];
+      for (int j = 0; j < V; ++j) w[p].e[j] = c.at(p, j) < c.cols ? q[c.at(p, j)] : int8_t(0);
     }
   }
 #pragma unroll
   for (int p = 0; p < kReadPieces; ++p) {
-    const int c = col0 + p * 32 * V, n = a.src.cols - c;
-    float v[V];
+    Piece<T> v;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = inside ? (float(w[p].e[j]) * scale) * a.factor : 0.f;
-    if (n > 0) store_piece<T, V>(out + c, n, wide, v);
+    for (int j = 0; j < V; ++j)
+      v.e[j] = from_f32<T>(inside ? (float(w[p].e[j]) * scale) * a.factor : 0.f);
+    store_piece<WIDE>(v, out, c, p, turns[WIDE ? 0 : threadIdx.x >> 5]);
   }
 }
 
@@ -336,10 +479,11 @@ bool on16(const void* p, int64_t pitch_bytes, int64_t rows) {
   return !p || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (rows == 1 || pitch_bytes % 16 == 0));
 }
 
-cudaError_t launch(const void* fn, int64_t blocks, void** args, cudaStream_t s) {
+cudaError_t launch(const void* fn, int64_t blocks, void** args, cudaStream_t s,
+                   int threads = kThreads) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(blocks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.stream = s;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -349,53 +493,61 @@ cudaError_t launch(const void* fn, int64_t blocks, void** args, cudaStream_t s) 
   return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
-template <class T, bool NORM>
-cudaError_t launch_rows_t(const RowsQ8Args& args, int num_sms, cudaStream_t s) {
+template <class T, bool NORM, bool WIDE>
+cudaError_t launch_rows_t(RowsQ8Args a, int num_sms, cudaStream_t s) {
   constexpr int V = Piece<T>::V, kMost = 32 / V;  // 32 values a lane
-  RowsQ8Args a = args;
-  const int64_t es = sizeof(T), rows = a.out.rows;
-  int wide = on16(a.x, a.ld_x * es, rows) && on16(a.r, a.ld_r * es, rows) &&
-             on16(a.sum, a.ld_sum * es, rows) && on16(a.y, a.ld_y * es, rows);
+  const int64_t rows = a.out.rows;
   const int passes = (a.out.cols + 32 * V - 1) / (32 * V);  // pieces of one warp's lanes
   if (passes > kWarps * kMost) {
-    void* p[] = {&a, &wide};
-    return launch(reinterpret_cast<const void*>(&long_rows_kernel<T, NORM>), rows, p, s);
+    void* p[] = {&a};
+    return launch(reinterpret_cast<const void*>(&long_rows_kernel<T, NORM, WIDE>), rows, p, s);
   }
   int warps = 1;
   while (warps < kWarps && (passes > warps * kMost ||
                             (passes > warps && rows * warps < int64_t(num_sms) * 32)))
     warps *= 2;
   const int np = (passes + warps - 1) / warps;
-  const int64_t blocks = (rows + kWarps / warps - 1) / (kWarps / warps);
-  void* p[] = {&a, &warps, &wide};
-  const void* fn = np <= 1   ? reinterpret_cast<const void*>(&rows_kernel<T, 1, NORM>)
-                   : np <= 2 ? reinterpret_cast<const void*>(&rows_kernel<T, 2, NORM>)
-                   : np <= 4 ? reinterpret_cast<const void*>(&rows_kernel<T, 4, NORM>)
-                             : reinterpret_cast<const void*>(&rows_kernel<T, kMost, NORM>);
-  return launch(fn, blocks, p, s);
+  const int64_t blocks = warps == 1 ? (rows + kWarps - 1) / kWarps : rows;
+  void* p[] = {&a, &warps};
+  const void* fn = np <= 1   ? reinterpret_cast<const void*>(&rows_kernel<T, 1, NORM, WIDE>)
+                   : np <= 2 ? reinterpret_cast<const void*>(&rows_kernel<T, 2, NORM, WIDE>)
+                   : np <= 4 ? reinterpret_cast<const void*>(&rows_kernel<T, 4, NORM, WIDE>)
+                             : reinterpret_cast<const void*>(&rows_kernel<T, kMost, NORM, WIDE>);
+  return launch(fn, blocks, p, s, warps == 1 ? kThreads : 32 * warps);
+}
+
+template <class T>
+cudaError_t launch_rows(const RowsQ8Args& a, int num_sms, cudaStream_t s) {
+  const int64_t es = sizeof(T), rows = a.out.rows;
+  const bool wide = on16(a.x, a.ld_x * es, rows) && on16(a.r, a.ld_r * es, rows) &&
+                    on16(a.sum, a.ld_sum * es, rows) && on16(a.y, a.ld_y * es, rows) &&
+                    on16(a.w, 0, 1);
+  if (a.norm)
+    return wide ? launch_rows_t<T, true, true>(a, num_sms, s)
+                : launch_rows_t<T, true, false>(a, num_sms, s);
+  return wide ? launch_rows_t<T, false, true>(a, num_sms, s)
+              : launch_rows_t<T, false, false>(a, num_sms, s);
 }
 
 }  // namespace
 
 cudaError_t launch_rows_q8(const RowsQ8Args& a, int dtype, int num_sms, cudaStream_t s) {
-  if (dtype == 0)
-    return a.norm ? launch_rows_t<__half, true>(a, num_sms, s)
-                  : launch_rows_t<__half, false>(a, num_sms, s);
-  return a.norm ? launch_rows_t<float, true>(a, num_sms, s)
-                : launch_rows_t<float, false>(a, num_sms, s);
+  return dtype == 0 ? launch_rows<__half>(a, num_sms, s) : launch_rows<float>(a, num_sms, s);
 }
 
 cudaError_t launch_read_q8(const ReadQ8Args& args, int dtype, cudaStream_t s) {
   ReadQ8Args a = args;
   const int es = dtype == 0 ? 2 : 4, per = kReadPieces * 32 * (16 / es);
   int segments = (a.src.cols + per - 1) / per;
-  int wide = on16(a.out, a.ld_out * es, a.rows);
+  const bool wide = on16(a.out, a.ld_out * es, a.rows);
   const int64_t blocks = (a.rows * segments + kWarps - 1) / kWarps;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  void* p[] = {&a, &segments, &wide};
-  return launch(dtype == 0 ? reinterpret_cast<const void*>(&read_kernel<__half>)
-                           : reinterpret_cast<const void*>(&read_kernel<float>),
-                blocks, p, s);
+  void* p[] = {&a, &segments};
+  const void* fn = dtype == 0 ? (wide ? reinterpret_cast<const void*>(&read_kernel<__half, true>)
+                                      : reinterpret_cast<const void*>(&read_kernel<__half, false>))
+                              : (wide ? reinterpret_cast<const void*>(&read_kernel<float, true>)
+                                      : reinterpret_cast<const void*>(&read_kernel<float, false>));
+  return launch(fn, blocks, p, s);
 }
 
 }  // namespace p2p
