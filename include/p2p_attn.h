@@ -441,11 +441,19 @@ p2p_status p2p_quantize_rows_q8(p2p_ctx* ctx, const void* src, int64_t ld_src, i
                                 const p2p_q8_rows* dst, void* stream);
 
 /* out row i [rows][ld_out] (f16 or f32) = (code * scale) * factor of src row index[i] (device int32
- * array; NULL: row i, and then rows <= src->rows), rounded once to out's type.  An index of -1 (what
+ * array; NULL: row i, and then rows <= src.rows), rounded once to out's type.  An index of -1 (what
  * p2p_logits_pick stores where no token is left) gives a row of zeros; another one outside the table
  * gives zeros and P2P_ERR_INVALID_ARG at the next p2p_sync. */
-p2p_status p2p_read_rows_q8(p2p_ctx* ctx, const p2p_q8_rows* src, const int32_t* index, int64_t rows,
-                            float factor, void* out, int64_t ld_out, int32_t dtype, void* stream);
+typedef struct p2p_read_rows {
+  p2p_q8_rows src;
+  const int32_t* index; /* [rows] or NULL */
+  void* out;            /* [rows][ld_out], src.cols values a row */
+  int64_t ld_out;
+  int32_t rows;
+  int32_t dtype; /* P2P_F16 or P2P_F32 */
+  float factor;  /* 0 selects 1 */
+} p2p_read_rows;
+p2p_status p2p_read_rows_q8(p2p_ctx* ctx, const p2p_read_rows* args, void* stream);
 
 /* For every row, in f32:  s = x + residual, rounded to dtype;  y = (s * weight) / sqrt(mean(s^2) + eps);
  * s goes to sum, y (rounded to dtype) to y, and y's codes and scale (of the unrounded y, by the rule of
@@ -466,19 +474,31 @@ typedef struct p2p_add_norm {
 p2p_status p2p_add_norm_q8(p2p_ctx* ctx, const p2p_add_norm* args, void* stream);
 
 /* y[m][n] = (f32(sum_k x[m][k] * w[n][k]) * x.scale[m]) * w.scale[n] (+ bias[n]) (+ residual[m][n]),
- * rounded to y's type (f16 or f32, dtype; the residual has the same type).  The sums are whole numbers,
- * exact in 32 bits (any codes, -128 too).  x->cols = w->cols; y [x->rows][ld_y], w->rows values a row; bias f32
- * or NULL; residual [x->rows][ld_r] or NULL, y itself with ld_r = ld_y included. */
-p2p_status p2p_gemm_q8(p2p_ctx* ctx, const p2p_q8_rows* w, const p2p_q8_rows* x, const float* bias,
-                       const void* residual, int64_t ld_r, void* y, int64_t ld_y, int32_t dtype,
-                       void* stream);
+ * rounded to y's type.  The sums are whole numbers, exact in 32 bits (any codes, -128 too). */
+typedef struct p2p_product {
+  p2p_q8_rows w;        /* [N][K] */
+  p2p_q8_rows x;        /* [M][K] */
+  const float* bias;    /* [N] or NULL */
+  const void* residual; /* [M][ld_r] of y's type, or NULL; y itself with y's pitch is fine */
+  void* y;              /* [M][ld_y] */
+  int64_t ld_r, ld_y;
+  int32_t dtype; /* P2P_F16 or P2P_F32 */
+} p2p_product;
+p2p_status p2p_gemm_q8(p2p_ctx* ctx, const p2p_product* args, void* stream);
 
 /* h[m][n] = f16(act(g) * u), g and u the products of x with gate and up as in p2p_gemm_q8 (f32, no
  * bias): act P2P_ACT_SILU g / (1 + exp(-g)), P2P_ACT_GELU (tanh form) g / (1 + exp(-2c (g + 0.044715 g^3))),
- * c = sqrt(2 / pi).  gate and up have the same rows and cols; h [x->rows][ld_h]. */
+ * c = sqrt(2 / pi). */
 typedef enum p2p_act { P2P_ACT_SILU = 0, P2P_ACT_GELU = 1 } p2p_act;
-p2p_status p2p_gate_q8(p2p_ctx* ctx, const p2p_q8_rows* gate, const p2p_q8_rows* up,
-                       const p2p_q8_rows* x, int32_t act, void* h, int64_t ld_h, void* stream);
+typedef struct p2p_gated {
+  p2p_q8_rows gate; /* [F][K] */
+  p2p_q8_rows up;   /* [F][K] */
+  p2p_q8_rows x;    /* [M][K] */
+  void* h;          /* f16 [M][ld_h] */
+  int64_t ld_h;
+  int32_t act;
+} p2p_gated;
+p2p_status p2p_gate_q8(p2p_ctx* ctx, const p2p_gated* args, void* stream);
 
 /* Converts f16 cache rows [rows][Hkv][D] to the int8 format above (src 16-byte and dst 8-byte
  * aligned; the same restated rule the decode uses when it appends). */

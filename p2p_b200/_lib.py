@@ -123,6 +123,42 @@ class AddNorm(C.Structure):
     ]
 
 
+class ReadRows(C.Structure):
+    _fields_ = [
+        ("src", Q8Rows),
+        ("index", C.c_void_p),
+        ("out", C.c_void_p),
+        ("ld_out", C.c_int64),
+        ("rows", C.c_int32),
+        ("dtype", C.c_int32),
+        ("factor", C.c_float),
+    ]
+
+
+class Product(C.Structure):
+    _fields_ = [
+        ("w", Q8Rows),
+        ("x", Q8Rows),
+        ("bias", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("y", C.c_void_p),
+        ("ld_r", C.c_int64),
+        ("ld_y", C.c_int64),
+        ("dtype", C.c_int32),
+    ]
+
+
+class Gated(C.Structure):
+    _fields_ = [
+        ("gate", Q8Rows),
+        ("up", Q8Rows),
+        ("x", Q8Rows),
+        ("h", C.c_void_p),
+        ("ld_h", C.c_int64),
+        ("act", C.c_int32),
+    ]
+
+
 class Q4Matrix(C.Structure):
     _fields_ = [
         ("qweight", C.c_void_p),
@@ -207,14 +243,12 @@ PROTOTYPES = {
         _st, [_v, _pp, C.POINTER(KvLayout), _v, _i64, _v, _v, _i64, _v, _v, _v, _i32, _i64, _i32,
               _v, _i64, _v]),
     "p2p_logits_pick": (_st, [_v, C.POINTER(Logits), _v]),
-    "p2p_quantize_rows_q8": (_st, [_v, _v, _i64, _i32, C.POINTER(Q8Rows), _v]),
-    "p2p_read_rows_q8": (
-        _st, [_v, C.POINTER(Q8Rows), _v, _i64, C.c_float, _v, _i64, _i32, _v]),
-    "p2p_add_norm_q8": (_st, [_v, C.POINTER(AddNorm), _v]),
-    "p2p_gemm_q8": (
-        _st, [_v, C.POINTER(Q8Rows), C.POINTER(Q8Rows), _v, _v, _i64, _v, _i64, _i32, _v]),
-    "p2p_gate_q8": (
-        _st, [_v, C.POINTER(Q8Rows), C.POINTER(Q8Rows), C.POINTER(Q8Rows), _i32, _v, _i64, _v]),
+    # (the argument structures as plain addresses: the Python layer packs them itself)
+    "p2p_quantize_rows_q8": (_st, [_v, _v, _i64, _i32, _v, _v]),
+    "p2p_read_rows_q8": (_st, [_v, _v, _v]),
+    "p2p_add_norm_q8": (_st, [_v, _v, _v]),
+    "p2p_gemm_q8": (_st, [_v, _v, _v]),
+    "p2p_gate_q8": (_st, [_v, _v, _v]),
     "p2p_kv_quantize_q8": (_st, [_v, _v, _v, _i64, _i32, _v, _i32, _v]),
     "p2p_gemv_q4": (_st, [_v, C.POINTER(Q4Matrix), _v, _v, _i64, _v]),
     "p2p_qkv_gemv_prep": (

@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -71,6 +72,13 @@ _KV_FORMATS = {torch.float16: _lib.P2P_KV_F16, torch.int8: _lib.P2P_KV_I8,
 
 _ROW_TYPES = {torch.float16: _lib.P2P_F16, torch.float32: _lib.P2P_F32}
 _ACTS = {"silu": _lib.P2P_ACT_SILU, "gelu": _lib.P2P_ACT_GELU}
+# Bytes of the C structures of the same order (p2p_q8_rows, p2p_read_rows, p2p_add_norm, p2p_product,
+# p2p_gated), padded to their size.
+_Q8_ROWS = struct.Struct("@PPqii").pack
+_READ_ROWS = struct.Struct("@PPqiiPPqiif4x").pack
+_ADD_NORM = struct.Struct("@PPPPPqqqqPPqiiif").pack
+_PRODUCT = struct.Struct("@PPqiiPPqiiPPPqqi4x").pack
+_GATED = struct.Struct("@PPqiiPPqiiPPqiiPqi4x").pack
 
 
 @functools.lru_cache(maxsize=None)
@@ -620,29 +628,34 @@ class Context:
         return dst
 
     # -- 8-bit rows: the layer around its attention ----------------------------------------------
-    def _values(self, t: torch.Tensor, name: str, dtype=None, rows: int = -1, cols: int = -1) -> int:
-        """Checks f16 or f32 rows (of `dtype`, [rows][cols], where given) and returns their row
-        stride."""
+    # The argument structures of these calls are packed with struct: building them field by field and
+    # converting each argument takes longer than the smallest of the kernels.
+    def _values(self, t: torch.Tensor, name: str, dtype, rows: int, cols: int) -> int:
+        """Checks f16 or f32 rows (of `dtype` where given) [rows][cols] (-1: any) and returns their
+        row stride."""
         shape, dt = t.shape, t.dtype
-        if (dt is not dtype if dtype is not None else dt not in _ROW_TYPES) or \
-                t.get_device() != self.device or len(shape) != 2 or \
-                rows >= 0 and shape[0] != rows or cols >= 0 and shape[1] != cols or \
-                shape[1] > 1 and t.stride(1) != 1:
-            _refuse(f"{name}: {dtype or 'f16 or f32'} [{rows if rows >= 0 else 'rows'}]"
-                    f"[{cols if cols >= 0 else 'cols'}] on device {self.device} needed, "
-                    f"got {tuple(shape)} {dt} on {t.device}")
-        return t.stride(0) if shape[0] > 1 else shape[1]
+        if (dt is dtype or dtype is None and dt in _ROW_TYPES) and \
+                t.get_device() == self.device and len(shape) == 2:
+            m, k = shape
+            ld, one = t.stride()
+            if (rows < 0 or m == rows) and (cols < 0 or k == cols) and (one == 1 or k <= 1):
+                return ld if m > 1 else k
+        _refuse(f"{name}: {dtype or 'f16 or f32'} [{rows if rows >= 0 else 'rows'}]"
+                f"[{cols if cols >= 0 else 'cols'}] on device {self.device} needed, "
+                f"got {tuple(shape)} {dt} on {t.device}")
 
-    def _q8(self, q: torch.Tensor, scale: torch.Tensor, name: str) -> "_lib.Q8Rows":
-        """Checks int8 rows and their scales and returns the C view."""
+    def _q8(self, q: torch.Tensor, scale: torch.Tensor, name: str) -> tuple:
+        """Checks int8 rows and their scales and returns the fields of the C view: codes, scales,
+        pitch, rows, columns."""
         shape = q.shape
-        if q.dtype is not torch.int8 or q.get_device() != self.device or len(shape) != 2 or \
-                shape[1] > 1 and q.stride(1) != 1:
+        if q.dtype is not torch.int8 or q.get_device() != self.device or len(shape) != 2:
             _refuse(f"{name}: int8 [rows][cols] on device {self.device} needed, "
                     f"got {tuple(shape)} {q.dtype} on {q.device}")
         n, k = shape
-        return _lib.Q8Rows(q.data_ptr(), self._floats(scale, n, name + " scales"),
-                           q.stride(0) if n > 1 else (k + 15) & -16, n, k)
+        ld, one = q.stride()
+        if one != 1 and k > 1:
+            _refuse(f"{name}: neighbouring codes of a row needed, strides {q.stride()}")
+        return (q.data_ptr(), self._floats(scale, n, name), ld if n > 1 else (k + 15) & -16, n, k)
 
     def _new_q8(self, q, scale, rows: int, cols: int, device):
         """int8 rows on 16-byte boundaries and their scales, where the caller has none."""
@@ -650,33 +663,38 @@ class Context:
             q = torch.empty((rows, (cols + 15) & -16), dtype=torch.int8, device=device)[:, :cols]
         if scale is None:
             scale = torch.empty(rows, dtype=torch.float32, device=device)
-        if tuple(q.shape) != (rows, cols):
-            _refuse(f"q: [{rows}][{cols}] needed, got {tuple(q.shape)}")
         return q, scale
 
     def quantize_rows_q8(self, src: torch.Tensor, q: Optional[torch.Tensor] = None,
                          scale: Optional[torch.Tensor] = None, stream=None):
         """f16 or f32 rows [rows][cols] -> int8 rows and a scale for each (p2p_quantize_rows_q8):
         (q, scale).  A weight's rows are its output channels."""
-        ld = self._values(src, "src")
-        q, scale = self._new_q8(q, scale, *src.shape, src.device)
+        ld = self._values(src, "src", None, -1, -1)
+        m, k = src.shape
+        if q is None or scale is None:
+            q, scale = self._new_q8(q, scale, m, k, src.device)
         d = self._q8(q, scale, "q")
+        if d[3] != m or d[4] != k:
+            _refuse(f"q: [{m}][{k}] needed, got {tuple(q.shape)}")
         st = lib.p2p_quantize_rows_q8(self.h, src.data_ptr(), ld, _ROW_TYPES[src.dtype],
-                                      C.byref(d), self._stream(stream))
+                                      _Q8_ROWS(*d), self._stream(stream))
         if st:
             self._chk(st)
         return q, scale
 
     def read_rows_q8(self, q: torch.Tensor, scale: torch.Tensor, out: torch.Tensor, *,
                      index: Optional[torch.Tensor] = None, factor: float = 1.0, stream=None):
-        """Rows index[i] (without index: row i) of int8 rows as values times `factor`, into out
-        [rows][cols] (f16 or f32): the embedding lookup (p2p_read_rows_q8).  index -1 gives
+        """Rows index[i] (without index: row i) of int8 rows as values times `factor` (not 0), into
+        out [rows][cols] (f16 or f32): the embedding lookup (p2p_read_rows_q8).  index -1 gives
         zeros."""
         s = self._q8(q, scale, "q")
-        ld, n = self._values(out, "out", cols=s.cols), out.shape[0]
+        ld, n = self._values(out, "out", None, -1, s[4]), out.shape[0]
+        if factor == 0:
+            _refuse("factor: 0")
         st = lib.p2p_read_rows_q8(
-            self.h, C.byref(s), None if index is None else self._ints(index, n, "index"), n,
-            factor, out.data_ptr(), ld, _ROW_TYPES[out.dtype], self._stream(stream))
+            self.h, _READ_ROWS(*s, 0 if index is None else self._ints(index, n, "index"),
+                               out.data_ptr(), ld, n, _ROW_TYPES[out.dtype], factor),
+            self._stream(stream))
         if st:
             self._chk(st)
         return out
@@ -688,24 +706,29 @@ class Context:
                     eps: float = 1e-5, stream=None):
         """Residual addition and RMS norm (p2p_add_norm_q8): sum_out = x + residual (may be
         either of them), y the normed rows, (q, scale) their int8 rows; returns (q, scale)."""
-        dt, (m, k) = x.dtype, x.shape
-        g = _lib.AddNorm()
-        g.x, g.ld_x = x.data_ptr(), self._values(x, "x")
+        dt = x.dtype
+        ld_x = self._values(x, "x", None, -1, -1)
+        m, k = x.shape
+        r_at = w_at = s_at = y_at = ld_r = ld_s = ld_y = 0
         if residual is not None:
-            g.residual, g.ld_r = residual.data_ptr(), self._values(residual, "residual", dt, m, k)
+            r_at, ld_r = residual.data_ptr(), self._values(residual, "residual", dt, m, k)
         if weight is not None:
             if weight.dtype is not torch.float16 or weight.get_device() != self.device or \
                     weight.numel() != k or not weight.is_contiguous():
                 _refuse(f"weight: {k} contiguous f16 values on device {self.device} needed")
-            g.weight = weight.data_ptr()
+            w_at = weight.data_ptr()
         if sum_out is not None:
-            g.sum, g.ld_sum = sum_out.data_ptr(), self._values(sum_out, "sum_out", dt, m, k)
+            s_at, ld_s = sum_out.data_ptr(), self._values(sum_out, "sum_out", dt, m, k)
         if y is not None:
-            g.y, g.ld_y = y.data_ptr(), self._values(y, "y", dt, m, k)
-        q, scale = self._new_q8(q, scale, m, k, x.device)
-        g.out = self._q8(q, scale, "q")
-        g.dtype, g.eps = _ROW_TYPES[dt], eps
-        st = lib.p2p_add_norm_q8(self.h, C.byref(g), self._stream(stream))
+            y_at, ld_y = y.data_ptr(), self._values(y, "y", dt, m, k)
+        if q is None or scale is None:
+            q, scale = self._new_q8(q, scale, m, k, x.device)
+        d = self._q8(q, scale, "q")
+        if d[3] != m or d[4] != k:
+            _refuse(f"q: [{m}][{k}] needed, got {tuple(q.shape)}")
+        st = lib.p2p_add_norm_q8(
+            self.h, _ADD_NORM(x.data_ptr(), r_at, w_at, s_at, y_at, ld_x, ld_r, ld_s, ld_y, *d,
+                              _ROW_TYPES[dt], eps), self._stream(stream))
         if st:
             self._chk(st)
         return q, scale
@@ -716,15 +739,14 @@ class Context:
         """y = x . w^T of int8 rows x [M][K] and w = (codes [N][K], scales), times both scales,
         plus bias [N] (f32) and residual [M][N] (may be y), into y (f16 or f32; p2p_gemm_q8)."""
         wr, xr = self._q8(w[0], w[1], "w"), self._q8(x, x_scale, "x")
-        ld_y, dt = self._values(y, "y", None, xr.rows, wr.rows), y.dtype
-        r_at, ld_r = None, 0
+        m, n, dt = xr[3], wr[3], y.dtype
+        ld_y = self._values(y, "y", None, m, n)
+        r_at = ld_r = 0
         if residual is not None:
-            ld_r = self._values(residual, "residual", dt, xr.rows, wr.rows)
-            r_at = residual.data_ptr()
+            r_at, ld_r = residual.data_ptr(), self._values(residual, "residual", dt, m, n)
         st = lib.p2p_gemm_q8(
-            self.h, C.byref(wr), C.byref(xr),
-            None if bias is None else self._floats(bias, wr.rows, "bias"), r_at, ld_r,
-            y.data_ptr(), ld_y, _ROW_TYPES[dt], self._stream(stream))
+            self.h, _PRODUCT(*wr, *xr, 0 if bias is None else self._floats(bias, n, "bias"), r_at,
+                             y.data_ptr(), ld_r, ld_y, _ROW_TYPES[dt]), self._stream(stream))
         if st:
             self._chk(st)
 
@@ -736,9 +758,9 @@ class Context:
         xr = self._q8(x, x_scale, "x")
         if act not in _ACTS:
             _refuse(f"act: one of {sorted(_ACTS)} needed, got {act!r}")
-        ld_h = self._values(h, "h", torch.float16, xr.rows, gr.rows)
-        st = lib.p2p_gate_q8(self.h, C.byref(gr), C.byref(ur), C.byref(xr), _ACTS[act],
-                             h.data_ptr(), ld_h, self._stream(stream))
+        ld_h = self._values(h, "h", torch.float16, xr[3], gr[3])
+        st = lib.p2p_gate_q8(self.h, _GATED(*gr, *ur, *xr, h.data_ptr(), ld_h, _ACTS[act]),
+                             self._stream(stream))
         if st:
             self._chk(st)
 

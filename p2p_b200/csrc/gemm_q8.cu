@@ -6,9 +6,8 @@
 // result; the scales, the activation and what is added follow in f32.  Two kernels:
 //   wide_kernel    many tokens: a cluster of two CTAs per 256-token tile and one
 //                  tcgen05.mma.cta_group::2 stream, persistent;
-//   narrow_kernel  few tokens, bound by the weights' bytes: the weights are the MMA's 128 rows and the
-//                  tokens its columns, k split over a cluster whose CTAs add their sums through
-//                  distributed shared memory.
+//   narrow_kernel  few tokens, bound by the weights' bytes: the weights are the MMA's rows and the tokens
+//                  its columns.
 // Every mbarrier wait is bounded (about one second): a wait that gives up sets the device error word,
 // every role of the CTA stops, the copies and MMAs in flight are waited for, the TMEM is freed and the
 // CTA returns.
@@ -40,12 +39,12 @@ struct Q8Params {
   void* y;
   int64_t ld_res, ld_y;
   int32_t* err;
+  int32_t tiles_n, items;  // tiles along n; work items in all
   // wide_kernel
-  int32_t tiles_n, whole, items;  // tiles along n; tiles of full width; work items in all
-  int32_t wide;                   // y and res rows on 16-byte boundaries
+  int32_t whole;  // tiles of full width
+  int32_t wide;   // y and res rows on 16-byte boundaries
   // narrow_kernel
-  int32_t tokens;     // columns of a tile
-  int32_t stages;
+  int32_t rows, tokens, stages;  // of a tile; of the ring
 };
 
 // act(g) * u.  The exponential and the quotient are approximations of 2 units in the last place each.
@@ -243,45 +242,47 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   launch_dependents();
 
   if (warp == kTmaWarp) {
-    if (lane == 0) {
-      const CUtensorMap* tm_b = GATE && rank ? &tm_u : &tm_w;
-      prefetch_tensormap(&tm_x);
-      prefetch_tensormap(tm_b);
-      uint32_t g = 0;  // ring slot counter, continuous across items
-      bool ok = true;
-      for (int i = pair; i < p.items && ok; i += pairs) {
-        const Item it = item_of<GATE>(p, i);
-        const int m0 = it.m0 + int(rank) * kRows, half = it.bn / 2;
-        const int n0 = GATE ? it.n0 : it.n0 + int(rank) * half;
-        for (int kt = 0; kt < nk; ++kt, ++g) {
-          const uint32_t st = g % kWideStages;
-          if (g >= kWideStages &&
-              !gemm_wait(s.abort_flag, &s.empty[st], ((g / kWideStages) - 1) & 1, p.err)) {
-            ok = false;
-            break;
-          }
+    // the whole warp walks the ring, so that what the copies take is the same in all its lanes
+    const CUtensorMap* tm_b = GATE && rank ? &tm_u : &tm_w;
+    uint32_t st = 0, round = 0;
+    bool ok = true;
+    for (int i = pair; i < p.items && ok; i += pairs) {
+      const Item it = item_of<GATE>(p, i);
+      const int m0 = it.m0 + int(rank) * kRows, half = it.bn / 2;
+      const int n0 = GATE ? it.n0 : it.n0 + int(rank) * half;
+      for (int kt = 0; kt < nk; ++kt) {
+        if (round > 0 && !(ok = gemm_wait_all(s.abort_flag, &s.empty[st], (round - 1) & 1, p.err)))
+          break;
+        if (elect_one()) {
           const uint32_t full0 = cluster_map(smem_u32(&s.full[st]), 0);
           if (rank == 0) mbar_arrive_expect_tx(&s.full[st], 2 * (kTileBytes + half * kStep));
           tma_load_2d_pair(s.a[st], &tm_x, kt * kStep, m0, full0);
-          for (int r = 0; r < half; r += kBoxRows)
-            tma_load_2d_pair(s.b[st] + r * kStep, tm_b, kt * kStep, n0 + r, full0);
+          tma_load_2d_pair(s.b[st], tm_b, kt * kStep, n0, full0);
+          if (half > kBoxRows)
+            tma_load_2d_pair(s.b[st] + kBoxRows * kStep, tm_b, kt * kStep, n0 + kBoxRows, full0);
         }
-      }
-      if (!ok) {  // let the copies already in flight land before the CTA exits
-        if (rank == 0) {
-          for (uint32_t h = g > kWideStages ? g - kWideStages : 0; h < g; ++h) {
-            const uint64_t t0 = globaltimer_ns();
-            while (!mbar_try_wait(&s.full[h % kWideStages], (h / kWideStages) & 1) &&
-                   globaltimer_ns() - t0 < kGemmWaitNs) {
-            }
-          }
-        } else {  // its loads complete on the even CTA's barriers: give them time to land
-          const uint64_t t0 = globaltimer_ns();
-          while (globaltimer_ns() - t0 < 100000) {
-          }
+        __syncwarp();
+        if (++st == kWideStages) {
+          st = 0;
+          ++round;
         }
       }
     }
+    if (!ok && lane == 0) {  // let the copies already in flight land before the CTA exits
+      if (rank == 0) {
+        for (int h = 0; h < kWideStages; ++h) {
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(&s.full[h], uint32_t(h) < st ? round & 1 : (round - 1) & 1) &&
+                 globaltimer_ns() - t0 < kGemmWaitNs) {
+          }
+        }
+      } else {  // its loads complete on the even CTA's barriers: give them time to land
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 100000) {
+        }
+      }
+    }
+    __syncwarp();
   } else if (warp == kMmaWarp) {
     if (rank == 0) {
       const uint64_t adesc0 = smem_desc_sw128(smem_u32(s.a[0]), 16, 1024);
@@ -292,14 +293,14 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       for (int i = pair; i < p.items && ok; i += pairs, ++n) {
         const int b = n & 1, u = n >> 1;  // accumulator buffer, its use count
         if (u > 0 &&
-            !(ok = gemm_wait_warp(s.abort_flag, &s.acc_empty[b], (u - 1) & 1, p.err, lane)))
+            !(ok = gemm_wait_all(s.abort_flag, &s.acc_empty[b], (u - 1) & 1, p.err)))
           break;
         tc_fence_after();
         const uint32_t idesc = idesc_i8(2 * kRows, item_of<GATE>(p, i).bn);
         const uint32_t acc = tmem + uint32_t(b * kWidth);
         for (int kt = 0; kt < nk; ++kt, ++g) {
           const uint32_t st = g % kWideStages;
-          if (!(ok = gemm_wait_warp(s.abort_flag, &s.full[st], (g / kWideStages) & 1, p.err, lane)))
+          if (!(ok = gemm_wait_all(s.abort_flag, &s.full[st], (g / kWideStages) & 1, p.err)))
             break;
           tc_fence_after();
           if (elect_one()) {
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     for (int i = pair; i < p.items; i += pairs, ++n) {
       const int b = n & 1, u = n >> 1;
       __syncwarp();
-      if (!gemm_wait_warp(s.abort_flag, &s.acc_full[b], u & 1, p.err, lane)) break;
+      if (!gemm_wait_all(s.abort_flag, &s.acc_full[b], u & 1, p.err)) break;
       tc_fence_after();
       const uint32_t empty0 = cluster_map(smem_u32(&s.acc_empty[b]), 0);
       const Item it = item_of<GATE>(p, i);
@@ -353,16 +354,22 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 }
 
 // ---- few tokens -------------------------------------------------------------------------------------
-// A tile: 128 weight rows (GATE: 64 gate rows above 64 up rows) x up to kMostTokens tokens, its k in the
-// hands of the CTAs of one cluster.  Every CTA sums its part of k in TMEM and hands the sums, by token, to
-// the CTA that finishes that token; each CTA adds what it was handed and stores.
-constexpr int kNarrowThreads = 256;
+// The weights' bytes bound these calls, so the weights are the MMA's rows: a tile is `rows` channels (any
+// multiple of 8 up to 128, so that the tiles fill the SMs evenly; the MMA's rows behind them hold whatever
+// lies there and are not looked at) times up to kMostTokens tokens.  GATE: two products of the same
+// tokens, whose sums lie in the same TMEM lanes.  A persistent CTA per SM walks tiles, its ring and two
+// accumulators running on across them.
+//   SPLIT: too few channels for that; a tile's k is cut over a cluster, one tile each.  Every CTA sums its
+// part and hands the sums, by token, to the CTA that finishes that token.
+constexpr int kNarrowThreads = 192;  // TMA, MMA, four epilogue warps
 constexpr int kMostTokens = 128;
 constexpr int kMostSplit = 8;
-constexpr int kMostStages = 12;
+constexpr int kMostStages = 24;
+constexpr int kNarrowSmem = 226 * 1024;
 
 struct NarrowHead {  // in front of the ring and the sums
   uint64_t full[kMostStages], empty[kMostStages];
+  uint64_t acc_full[2], acc_empty[2];
   uint64_t done;
   uint32_t tmem_base;
   volatile int abort_flag;
@@ -373,30 +380,38 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-template <class T, bool GATE>
-__global__ void __launch_bounds__(kNarrowThreads)
+template <class T, bool GATE, bool SPLIT>
+__global__ void __launch_bounds__(kNarrowThreads, 1)
     narrow_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                   const __grid_constant__ CUtensorMap tm_u, const __grid_constant__ Q8Params p) {
+  constexpr int G = GATE ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   NarrowHead& s = *reinterpret_cast<NarrowHead*>(base);
-  uint8_t* ring = base + 1024;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = int(cluster_ctas()), rank = int(cluster_ctarank());
-  const uint32_t stage_bytes = kTileBytes + uint32_t(p.tokens) * kStep;
-  uint32_t* sums = reinterpret_cast<uint32_t*>(ring + p.stages * stage_bytes);  // [split][own][128]
-  const int own = (p.tokens + split - 1) / split;
-  const int tile = blockIdx.x / split;
-  constexpr int kCols = GATE ? 64 : 128;
-  const int n0 = tile % p.tiles_n * kCols, m0 = tile / p.tiles_n * p.tokens;
+  const int split = SPLIT ? int(cluster_ctas()) : 1, rank = SPLIT ? int(cluster_ctarank()) : 0;
+  const int first = SPLIT ? int(blockIdx.x) / split : int(blockIdx.x);
+  const int step = SPLIT ? p.items : int(gridDim.x);
+  const uint32_t w_bytes = uint32_t(p.rows) * kStep, x_bytes = uint32_t(p.tokens) * kStep;
+  const uint32_t stage_bytes = G * w_bytes + x_bytes;
+  const int own = (p.tokens + split - 1) / split;  // SPLIT: tokens finished here
+  uint32_t* sums = reinterpret_cast<uint32_t*>(base + 1024);  // [split][own][G][rows]
+  uint8_t* ring = base + 1024 + (SPLIT ? (split * own * G * p.rows * 4 + 1023) / 1024 * 1024 : 0);
   const int nk = (p.k + kStep - 1) / kStep;
-  const int k0 = int(int64_t(nk) * rank / split), k1 = int(int64_t(nk) * (rank + 1) / split);
-  const uint32_t tmem_cols = p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
+  const int k0 = SPLIT ? int(int64_t(nk) * rank / split) : 0,
+            k1 = SPLIT ? int(int64_t(nk) * (rank + 1) / split) : nk;
+  const uint32_t acc_cols = G * p.tokens;  // of one accumulator buffer
+  const uint32_t need = SPLIT ? acc_cols : 2 * acc_cols;
+  const uint32_t tmem_cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.acc_full[i], 1);
+      mbar_init(&s.acc_empty[i], 4);
     }
     mbar_init(&s.done, 1);
     s.abort_flag = 0;
@@ -408,116 +423,211 @@ __global__ void __launch_bounds__(kNarrowThreads)
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
   // another CTA's shared memory is not touched before that CTA runs
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if constexpr (SPLIT) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   grid_dependency_wait();
   launch_dependents();
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t g = 0;
-      bool ok = true;
-      for (int kt = k0; kt < k1; ++kt, ++g) {
-        const uint32_t st = g % p.stages;
-        if (g >= uint32_t(p.stages) &&
-            !gemm_wait(s.abort_flag, &s.empty[st], ((g / p.stages) - 1) & 1, p.err)) {
-          ok = false;
+    // the whole warp walks the ring, so that what the copies take is the same in all its lanes
+    uint32_t st = 0, round = 0;
+    bool ok = true;
+    for (int t = first; t < p.items && ok; t += step) {
+      const int n0 = t % p.tiles_n * p.rows, m0 = t / p.tiles_n * p.tokens;
+      for (int kt = k0; kt < k1; ++kt) {
+        if (round > 0 && !(ok = gemm_wait_all(s.abort_flag, &s.empty[st], (round - 1) & 1, p.err)))
           break;
+        if (elect_one()) {
+          uint8_t* a = ring + st * stage_bytes;
+          mbar_arrive_expect_tx(&s.full[st], stage_bytes);
+          tma_load_2d(a, &tm_w, kt * kStep, n0, &s.full[st]);
+          if constexpr (GATE) tma_load_2d(a + w_bytes, &tm_u, kt * kStep, n0, &s.full[st]);
+          tma_load_2d(a + G * w_bytes, &tm_x, kt * kStep, m0, &s.full[st]);
         }
-        uint8_t* a = ring + st * stage_bytes;
-        mbar_arrive_expect_tx(&s.full[st], stage_bytes);
-        tma_load_2d(a, &tm_w, kt * kStep, n0, &s.full[st]);
-        if constexpr (GATE) tma_load_2d(a + kTileBytes / 2, &tm_u, kt * kStep, n0, &s.full[st]);
-        else tma_load_2d(a + kTileBytes / 2, &tm_w, kt * kStep, n0 + 64, &s.full[st]);
-        tma_load_2d(a + kTileBytes, &tm_x, kt * kStep, m0, &s.full[st]);
+        __syncwarp();
+        if (++st == uint32_t(p.stages)) {
+          st = 0;
+          ++round;
+        }
       }
-      if (!ok) {  // let the copies already in flight land before the CTA exits
-        for (uint32_t h = g > uint32_t(p.stages) ? g - p.stages : 0; h < g; ++h) {
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(&s.full[h % p.stages], (h / p.stages) & 1) &&
-                 globaltimer_ns() - t0 < kGemmWaitNs) {
-          }
+    }
+    if (!ok && lane == 0) {  // let the copies already in flight land before the CTA exits: those of this
+                             // round in front of st, those of the one before from st on
+      for (int h = 0; h < p.stages; ++h) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&s.full[h], uint32_t(h) < st ? round & 1 : (round - 1) & 1) &&
+               globaltimer_ns() - t0 < kGemmWaitNs) {
         }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    const uint32_t idesc = idesc_i8(128, p.tokens);
-    const uint64_t adesc0 = smem_desc_sw128(smem_u32(ring), 16, 1024);
-    bool ok = true;
-    uint32_t g = 0;
-    for (int kt = k0; kt < k1; ++kt, ++g) {
-      const uint32_t st = g % p.stages;
-      if (!(ok = gemm_wait_warp(s.abort_flag, &s.full[st], (g / p.stages) & 1, p.err, lane))) break;
+    const uint32_t idesc = idesc_i8(p.rows <= 64 ? 64 : 128, p.tokens);
+    const uint64_t desc0 = smem_desc_sw128(smem_u32(ring), 16, 1024);
+    bool ok = true, issued = false;
+    uint32_t st = 0, round = 0;
+    int n = 0;  // tiles of this CTA
+    for (int t = first; t < p.items && ok; t += step, ++n) {
+      const int b = n & 1, u = n >> 1;  // accumulator buffer, its use count
+      if (u > 0 && !(ok = gemm_wait_all(s.abort_flag, &s.acc_empty[b], (u - 1) & 1, p.err)))
+        break;
       tc_fence_after();
-      if (elect_one()) {
-        const uint64_t ad = adesc0 + uint64_t(st) * (stage_bytes >> 4), bd = ad + (kTileBytes >> 4);
+      const uint32_t acc = tmem + uint32_t(b) * acc_cols;
+      for (int kt = k0; kt < k1; ++kt) {
+        if (!(ok = gemm_wait_all(s.abort_flag, &s.full[st], round & 1, p.err))) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t ad = desc0 + uint64_t(st) * (stage_bytes >> 4),
+                         bd = ad + ((G * w_bytes) >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kStep / 32; ++kk)
-          mma_i8_ss(tmem, ad + 2 * kk, bd + 2 * kk, idesc, (g > 0 || kk > 0) ? 1u : 0u);
-        mma_commit(&s.empty[st]);
+          for (int kk = 0; kk < kStep / 32; ++kk) {
+            mma_i8_ss(acc, ad + 2 * kk, bd + 2 * kk, idesc, (kt > k0 || kk > 0) ? 1u : 0u);
+            if constexpr (GATE)
+              mma_i8_ss(acc + p.tokens, ad + (w_bytes >> 4) + 2 * kk, bd + 2 * kk, idesc,
+                        (kt > k0 || kk > 0) ? 1u : 0u);
+          }
+          mma_commit(&s.empty[st]);
+        }
+        issued = true;
+        __syncwarp();
+        if (++st == uint32_t(p.stages)) {
+          st = 0;
+          ++round;
+        }
+      }
+      if (ok && elect_one()) mma_commit(&s.acc_full[b]);
+      __syncwarp();
+    }
+    if (issued) {  // no MMA may still run when the TMEM is freed
+      if (elect_one()) mma_commit(&s.done);
+      __syncwarp();
+      if (lane == 0) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&s.done, 0) && globaltimer_ns() - t0 < kGemmWaitNs) {
+        }
       }
       __syncwarp();
     }
-    // also where a wait gave up: no MMA may still run when the TMEM is freed
-    if (elect_one()) mma_commit(&s.done);
-    __syncwarp();
-    if (!ok && lane == 0) {
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(&s.done, 0) && globaltimer_ns() - t0 < kGemmWaitNs) {
+  } else {
+    // lane of TMEM quarter warp & 3 -> channel: 32 a quarter, or 16 of an MMA of 64 rows
+    const int quarter = warp & 3;
+    const bool tall = p.rows > 64;
+    const int ch = tall ? quarter * 32 + lane : quarter * 16 + lane;
+    const bool mine = ch < p.rows && (tall || lane < 16);
+    int n = 0;
+    for (int t = first; t < p.items; t += step, ++n) {
+      const int b = n & 1, u = n >> 1;
+      const int c = t % p.tiles_n * p.rows + ch, m0 = t / p.tiles_n * p.tokens;
+      const int tokens = min(p.tokens, p.m - m0);
+      const bool live = mine && c < p.n;
+      float ws = 0.f, second = 0.f;
+      if (!SPLIT && live) {
+        ws = p.ws[c];
+        if constexpr (GATE) second = p.us[c];
+        else if (p.bias) second = p.bias[c];
+      }
+      __syncwarp();
+      const bool ok = gemm_wait_all(s.abort_flag, &s.acc_full[b], u & 1, p.err);
+      if constexpr (SPLIT) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t at = tmem + uint32_t(b) * acc_cols + (uint32_t(quarter * 32) << 16);
+      if constexpr (SPLIT) {
+        int to = 0, tl = 0;  // token t0 + j is number tl of CTA `to`
+        for (int t0 = 0; t0 < p.tokens; t0 += 8) {
+          uint32_t r[G][8];
+#pragma unroll
+          for (int g = 0; g < G; ++g) tmem_ld8(at + g * p.tokens + t0, r[g]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t dst = cluster_map(
+                smem_u32(sums + (rank * own + tl) * (G * p.rows) + ch), uint32_t(to));
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+              if (mine) st_cluster(dst + g * p.rows * 4, r[g][j]);
+            if (++tl == own) {
+              tl = 0;
+              ++to;
+            }
+          }
+        }
+      } else {
+        T* y = static_cast<T*>(p.y) + int64_t(m0) * p.ld_y + c;
+        const T* res = static_cast<const T*>(p.res) + int64_t(m0) * p.ld_res + c;
+        float xs32 = 0.f;
+        for (int t0 = 0; t0 < p.tokens; t0 += 8) {
+          if (t0 % 32 == 0) xs32 = t0 + lane < tokens ? p.xs[m0 + t0 + lane] : 0.f;
+          uint32_t r[G][8];
+#pragma unroll
+          for (int g = 0; g < G; ++g) tmem_ld8(at + g * p.tokens + t0, r[g]);
+          float add[8];
+          if constexpr (!GATE) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              add[j] = p.res && live && t0 + j < tokens ? to_f32(res[int64_t(t0 + j) * p.ld_res]) : 0.f;
+          }
+          tmem_ld_wait();
+          if (t0 + 8 >= p.tokens) {  // everything of this warp is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.acc_empty[b]);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float xs = __shfl_sync(0xffffffffu, xs32, (t0 + j) & 31);
+            float v = scaled(r[0][j], xs, ws);
+            if constexpr (GATE) {
+              v = act_mul(v, scaled(r[G - 1][j], xs, second), p.act);
+            } else {
+              if (p.bias) v = __fadd_rn(v, second);
+              if (p.res) v = __fadd_rn(v, add[j]);
+            }
+            if (live && t0 + j < tokens) y[int64_t(t0 + j) * p.ld_y] = from_f32<T>(v);
+          }
+        }
       }
     }
-    __syncwarp();
   }
 
-  // the sums, token by token, to the CTAs that finish them
-  bool ok = true;
-  if (warp >= 4) ok = gemm_wait_warp(s.abort_flag, &s.done, 0, p.err, lane);
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (warp >= 4 && ok) {
-    tc_fence_after();
-    const uint32_t at = tmem + (uint32_t((warp & 3) * 32) << 16);
-    const int ch = (warp & 3) * 32 + lane;
-    for (int t0 = 0; t0 < p.tokens; t0 += 8) {
-      uint32_t r[8];
-      tmem_ld8(at + t0, r);
-      tmem_ld_wait();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int t = t0 + j, to = t / own;
-        st_cluster(cluster_map(smem_u32(sums + (rank * own + t - to * own) * 128 + ch), to), r[j]);
-      }
-    }
+  if constexpr (SPLIT) {
+    if (warp < 2) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (s.abort_flag && lane == 0)  // nothing of a sum that lacks a part is stored
+      for (int i = 0; i < split; ++i)
+        st_cluster(cluster_map(smem_u32(const_cast<int*>(&s.abort_flag)), i), 1u);
+    tc_fence_before();
+    cluster_sync();
+  } else {
+    tc_fence_before();
+    __syncthreads();
   }
-  if (s.abort_flag && lane == 0)  // nothing of a sum that lacks a part is stored
-    for (int i = 0; i < split; ++i)
-      st_cluster(cluster_map(smem_u32(const_cast<int*>(&s.abort_flag)), i), 1u);
-  tc_fence_before();
-  cluster_sync();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, tmem_cols);
   }
-  if (s.abort_flag) return;
-
-  for (int i = threadIdx.x; i < own * kCols; i += kNarrowThreads) {
-    const int c = i % kCols, tl = i / kCols, t = rank * own + tl;
-    const int m = m0 + t, n = n0 + c;
-    if (t >= p.tokens || m >= p.m || n >= p.n) continue;
-    int acc = 0, acc2 = 0;
-    for (int j = 0; j < split; ++j) {
-      acc += int(sums[(j * own + tl) * 128 + c]);
-      if constexpr (GATE) acc2 += int(sums[(j * own + tl) * 128 + 64 + c]);
+  if constexpr (SPLIT) {
+    if (s.abort_flag) return;
+    const int n0 = first % p.tiles_n * p.rows, m0 = first / p.tiles_n * p.tokens;
+    for (int tl = warp; tl < own; tl += kNarrowThreads / 32) {
+      const int m = m0 + rank * own + tl;
+      if (rank * own + tl >= p.tokens || m >= p.m) break;
+      const float xs = p.xs[m];
+      for (int c = lane; c < p.rows && n0 + c < p.n; c += 32) {
+        const int n = n0 + c;
+        int acc[G] = {};
+        for (int j = 0; j < split; ++j)
+#pragma unroll
+          for (int g = 0; g < G; ++g) acc[g] += int(sums[((j * own + tl) * G + g) * p.rows + c]);
+        float v = scaled(uint32_t(acc[0]), xs, p.ws[n]);
+        if constexpr (GATE) {
+          v = act_mul(v, scaled(uint32_t(acc[G - 1]), xs, p.us[n]), p.act);
+        } else {
+          if (p.bias) v = __fadd_rn(v, p.bias[n]);
+          if (p.res)
+            v = __fadd_rn(v, to_f32(static_cast<const T*>(p.res)[int64_t(m) * p.ld_res + n]));
+        }
+        static_cast<T*>(p.y)[int64_t(m) * p.ld_y + n] = from_f32<T>(v);
+      }
     }
-    const float xs = p.xs[m];
-    float y = scaled(uint32_t(acc), xs, p.ws[n]);
-    if constexpr (GATE) {
-      y = act_mul(y, scaled(uint32_t(acc2), xs, p.us[n]), p.act);
-    } else {
-      if (p.bias) y = __fadd_rn(y, p.bias[n]);
-      if (p.res)
-        y = __fadd_rn(y, to_f32(static_cast<const T*>(p.res)[int64_t(m) * p.ld_res + n]));
-    }
-    static_cast<T*>(p.y)[int64_t(m) * p.ld_y + n] = from_f32<T>(y);
   }
 }
 
@@ -599,36 +709,74 @@ cudaError_t launch_wide(Q8Params p, const GemmQ8Args& a, int num_sms, cudaStream
                         stream);
 }
 
-template <class T, bool GATE>
-cudaError_t launch_narrow(Q8Params p, const GemmQ8Args& a, int num_sms, cudaStream_t stream) {
-  // columns of an MMA: 8, 16, 24, or multiples of 16
-  const int tokens = std::min(kMostTokens, p.m <= 24 ? (p.m + 7) / 8 * 8 : (p.m + 15) / 16 * 16);
+// How few tokens are cut up: channels of a tile and CTAs of its k.
+struct NarrowPlan {
+  int rows, split, tokens;
+  double cost;  // cycles
+};
+// The busiest SM's time: its tiles times the longer of what a tile loads (of L2, about kLoad bytes a
+// cycle; an SM's share of the DRAM rate bounds the weights) and what it multiplies (8192 products a cycle
+// with 128 rows, half with 64, and the shared memory that an MMA's weight rows take at 128 bytes a cycle).
+NarrowPlan narrow_plan(int m, int n, int k, int G, int num_sms) {
+  constexpr double kLoad = 50, kDram = 23, kSplitCost = 2500;
+  const int tokens = std::min(kMostTokens, m <= 24 ? (m + 7) / 8 * 8 : (m + 15) / 16 * 16);
+  const int token_tiles = (m + tokens - 1) / tokens, nk = (k + kStep - 1) / kStep;
+  NarrowPlan best{0, 0, tokens, 0};
+  for (int split = 1; split <= std::min(kMostSplit, nk); split *= 2) {
+    for (int rows = 8; rows <= 128; rows += 8) {
+      if (split > 1 && G * rows > 128) break;
+      const int64_t ctas = (int64_t(n) + rows - 1) / rows * token_tiles * split;
+      const double tiles = double((ctas + num_sms - 1) / num_sms);
+      const double steps = double((nk + split - 1) / split);
+      const double load = std::max((G * rows + tokens) * kStep / kLoad, G * rows * kStep / kDram);
+      const double mma = 4.0 * G * std::max(tokens / 2.0, rows <= 64 ? 16.0 : 32.0);
+      double cost = tiles * steps * std::max(load, mma);
+      if (split > 1) cost += tiles * kSplitCost;
+      else cost += tokens * 30.0;  // the last tile's epilogue
+      if (!best.rows || cost < best.cost) best = NarrowPlan{rows, split, tokens, cost};
+    }
+  }
+  return best;
+}
+
+template <class T, bool GATE, bool SPLIT>
+cudaError_t launch_narrow(Q8Params p, const GemmQ8Args& a, const NarrowPlan& plan, int num_sms,
+                          cudaStream_t stream) {
+  constexpr int G = GATE ? 2 : 1;
   CUtensorMap tx, tw, tu;
-  if (!map_codes(&tx, a.x, unsigned(tokens)) || !map_codes(&tw, a.w, 64) ||
-      !map_codes(&tu, GATE ? a.up : a.w, 64))
+  if (!map_codes(&tx, a.x, unsigned(plan.tokens)) || !map_codes(&tw, a.w, unsigned(plan.rows)) ||
+      (GATE && !map_codes(&tu, a.up, unsigned(plan.rows))))
     return cudaErrorInvalidValue;
-  constexpr int kCols = GATE ? 64 : 128;
-  const int64_t tiles_n = (int64_t(p.n) + kCols - 1) / kCols;
-  const int64_t tiles = tiles_n * ((int64_t(p.m) + tokens - 1) / tokens);
+  if (!GATE) tu = tw;
+  p.rows = plan.rows;
+  p.tokens = plan.tokens;
+  p.tiles_n = (p.n + plan.rows - 1) / plan.rows;
+  const int64_t tiles = int64_t(p.tiles_n) * ((int64_t(p.m) + plan.tokens - 1) / plan.tokens);
+  if (tiles * plan.split > INT32_MAX) return cudaErrorInvalidValue;
+  p.items = int32_t(tiles);
   const int nk = (p.k + kStep - 1) / kStep;
-  int split = 1;
-  while (2 * split <= std::min(kMostSplit, nk) && tiles * 2 * split <= 2 * num_sms) split *= 2;
-  const int own = (tokens + split - 1) / split;
-  const int stage = int(kTileBytes) + tokens * kStep, sums = split * own * 128 * 4;
-  const int room = (tokens <= 64 ? 113 : 226) * 1024 - 2048 - sums;
-  const int steps = (nk + split - 1) / split;
-  p.stages = std::max(1, std::min({kMostStages, steps, room / stage}));
-  p.tokens = tokens;
-  p.tiles_n = int32_t(tiles_n);
-  const size_t smem = 2048 + size_t(p.stages) * stage + sums;
-  const void* fn = reinterpret_cast<const void*>(&narrow_kernel<T, GATE>);
+  const int own = (plan.tokens + plan.split - 1) / plan.split;
+  const int stage = (G * plan.rows + plan.tokens) * kStep;
+  const int sums = SPLIT ? (plan.split * own * G * plan.rows * 4 + 1023) / 1024 * 1024 : 0;
+  // behind the ring, what the last stage's MMA reads beyond its rows
+  const int fixed = 2048 + sums + (plan.rows <= 64 ? 64 : 128) * kStep;
+  const int64_t steps = SPLIT ? (nk + plan.split - 1) / plan.split
+                              : nk * ((tiles + num_sms - 1) / num_sms);
+  p.stages = int(std::min<int64_t>({kMostStages, steps, (kNarrowSmem - fixed) / stage}));
+  size_t smem = size_t(fixed) + size_t(p.stages) * stage;
+  // The CTAs of a cluster wait for one another, and an allocation of TMEM waits for whoever holds it: so
+  // never more of them on an SM than its 512 columns serve (at most 4 with up to 128 columns, 2 with 256),
+  // and none beside a pair form's CTA, which takes all columns and over 190 KB of shared memory.
+  if (SPLIT) smem = std::max<size_t>(smem, (G * plan.tokens > 128 ? 78 : 48) * 1024);
+  const void* fn = reinterpret_cast<const void*>(&narrow_kernel<T, GATE, SPLIT>);
   static PerDeviceOnce attrs;
   cudaError_t e = per_device_once(attrs, [&](int&) {
-    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kNarrowSmem);
   });
   if (e != cudaSuccess) return e;
   void* args[] = {&tx, &tw, &tu, &p};
-  return launch_cluster(fn, tiles * split, kNarrowThreads, smem, split, args, stream);
+  return launch_cluster(fn, SPLIT ? tiles * plan.split : std::min<int64_t>(tiles, num_sms),
+                        kNarrowThreads, smem, plan.split, args, stream);
 }
 
 bool on16(const void* p, int64_t pitch_bytes) {
@@ -637,8 +785,10 @@ bool on16(const void* p, int64_t pitch_bytes) {
 
 template <class T, bool GATE>
 cudaError_t launch_q8(const Q8Params& p, const GemmQ8Args& a, int num_sms, cudaStream_t s) {
-  return p.m <= kMostTokens ? launch_narrow<T, GATE>(p, a, num_sms, s)
-                            : launch_wide<T, GATE>(p, a, num_sms, s);
+  if (p.m > kMostTokens) return launch_wide<T, GATE>(p, a, num_sms, s);
+  const NarrowPlan plan = narrow_plan(p.m, p.n, p.k, GATE ? 2 : 1, num_sms);
+  return plan.split > 1 ? launch_narrow<T, GATE, true>(p, a, plan, num_sms, s)
+                        : launch_narrow<T, GATE, false>(p, a, plan, num_sms, s);
 }
 
 }  // namespace

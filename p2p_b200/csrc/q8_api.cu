@@ -140,14 +140,19 @@ p2p_status p2p_quantize_rows_q8(p2p_ctx* ctx, const void* src, int64_t ld_src, i
                   who);
 }
 
-p2p_status p2p_read_rows_q8(p2p_ctx* ctx, const p2p_q8_rows* src, const int32_t* index, int64_t rows,
-                            float factor, void* out, int64_t ld_out, int32_t dtype, void* stream) {
+p2p_status p2p_read_rows_q8(p2p_ctx* ctx, const p2p_read_rows* args, void* stream) {
   if (!ctx) return P2P_ERR_INVALID_ARG;
   const char* who = "read_rows_q8";
+  if (!args) return fail(ctx, P2P_ERR_INVALID_ARG, "%s: arguments are NULL", who);
+  const p2p_q8_rows* src = &args->src;
+  const int32_t* index = args->index;
+  const int64_t rows = args->rows, ld_out = args->ld_out;
+  const int32_t dtype = args->dtype;
+  void* out = args->out;
   p2p_status st;
   if ((st = check_dtype(ctx, dtype, who)) != P2P_OK) return st;
   if ((st = check_q8(ctx, src, "src", who)) != P2P_OK) return st;
-  if (rows < 0 || rows > INT32_MAX || (!index && rows > src->rows) || !aligned(index, 4))
+  if (rows < 0 || (!index && rows > src->rows) || !aligned(index, 4))
     return fail(ctx, P2P_ERR_INVALID_ARG, "%s: %lld rows of %d, index %p", who, (long long)rows,
                 src->rows, (const void*)index);
   if (rows == 0) return P2P_OK;
@@ -157,7 +162,7 @@ p2p_status p2p_read_rows_q8(p2p_ctx* ctx, const p2p_q8_rows* src, const int32_t*
   if ((st = apart(ctx, who, to, {rows_of(src, "src's codes"), scales_of(src, "src's scales"),
                                  {index, 0, 4 * rows, 1, "index"}})) != P2P_OK)
     return st;
-  const p2p::ReadQ8Args a{view(src), index, rows, factor, out, ld_out, p2p::ctx_dev_err(ctx)};
+  const p2p::ReadQ8Args a{view(src), index, rows, args->factor == 0.f ? 1.f : args->factor, out, ld_out, p2p::ctx_dev_err(ctx)};
   OnDevice g(p2p::ctx_device(ctx));
   return launched(ctx, p2p::launch_read_q8(a, dtype, static_cast<cudaStream_t>(stream)), who);
 }
@@ -230,11 +235,16 @@ p2p_status p2p_add_norm_q8(p2p_ctx* ctx, const p2p_add_norm* args, void* stream)
                   who);
 }
 
-p2p_status p2p_gemm_q8(p2p_ctx* ctx, const p2p_q8_rows* w, const p2p_q8_rows* x, const float* bias,
-                       const void* residual, int64_t ld_r, void* y, int64_t ld_y, int32_t dtype,
-                       void* stream) {
+p2p_status p2p_gemm_q8(p2p_ctx* ctx, const p2p_product* args, void* stream) {
   if (!ctx) return P2P_ERR_INVALID_ARG;
   const char* who = "gemm_q8";
+  if (!args) return fail(ctx, P2P_ERR_INVALID_ARG, "%s: arguments are NULL", who);
+  const p2p_q8_rows *w = &args->w, *x = &args->x;
+  const float* bias = args->bias;
+  const void* residual = args->residual;
+  void* y = args->y;
+  const int64_t ld_r = args->ld_r, ld_y = args->ld_y;
+  const int32_t dtype = args->dtype;
   p2p_status st;
   if ((st = check_dtype(ctx, dtype, who)) != P2P_OK) return st;
   if ((st = check_q8(ctx, w, "w", who)) != P2P_OK) return st;
@@ -272,10 +282,14 @@ p2p_status p2p_gemm_q8(p2p_ctx* ctx, const p2p_q8_rows* w, const p2p_q8_rows* x,
                   who);
 }
 
-p2p_status p2p_gate_q8(p2p_ctx* ctx, const p2p_q8_rows* gate, const p2p_q8_rows* up,
-                       const p2p_q8_rows* x, int32_t act, void* h, int64_t ld_h, void* stream) {
+p2p_status p2p_gate_q8(p2p_ctx* ctx, const p2p_gated* args, void* stream) {
   if (!ctx) return P2P_ERR_INVALID_ARG;
   const char* who = "gate_q8";
+  if (!args) return fail(ctx, P2P_ERR_INVALID_ARG, "%s: arguments are NULL", who);
+  const p2p_q8_rows *gate = &args->gate, *up = &args->up, *x = &args->x;
+  void* h = args->h;
+  const int64_t ld_h = args->ld_h;
+  const int32_t act = args->act;
   p2p_status st;
   if (act != P2P_ACT_SILU && act != P2P_ACT_GELU)
     return fail(ctx, P2P_ERR_INVALID_ARG, "%s: act %d", who, act);

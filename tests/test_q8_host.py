@@ -10,7 +10,6 @@ from conftest import ROOT
 torch = pytest.importorskip("torch")
 
 BAD, UNSUPPORTED = 1, 7
-I32_MAX = 2**31 - 1
 MB = 1 << 20
 
 
@@ -54,10 +53,32 @@ def test_null_context_is_a_status():
     from p2p_b200 import _lib, lib
     r, g = _lib.Q8Rows(), _lib.AddNorm()
     assert lib.p2p_quantize_rows_q8(None, None, 0, 0, C.byref(r), None) == BAD
-    assert lib.p2p_read_rows_q8(None, C.byref(r), None, 0, 1.0, None, 0, 0, None) == BAD
+    assert lib.p2p_read_rows_q8(None, C.byref(_lib.ReadRows()), None) == BAD
     assert lib.p2p_add_norm_q8(None, C.byref(g), None) == BAD
-    assert lib.p2p_gemm_q8(None, C.byref(r), C.byref(r), None, None, 0, None, 0, 0, None) == BAD
-    assert lib.p2p_gate_q8(None, C.byref(r), C.byref(r), C.byref(r), 0, None, 0, None) == BAD
+    assert lib.p2p_gemm_q8(None, C.byref(_lib.Product()), None) == BAD
+    assert lib.p2p_gate_q8(None, C.byref(_lib.Gated()), None) == BAD
+
+
+def test_packed_structures_are_the_c_ones():
+    """The Python layer packs the argument structures itself: sizes and offsets have to be the C ones."""
+    from p2p_b200 import _lib, attention as A
+
+    def flat(t, at=0):
+        for name, kind in t._fields_:
+            off = at + getattr(t, name).offset
+            if issubclass(kind, C.Structure):
+                yield from flat(kind, off)
+            else:
+                yield off, kind
+    for pack, t in ((A._Q8_ROWS, _lib.Q8Rows), (A._READ_ROWS, _lib.ReadRows),
+                    (A._ADD_NORM, _lib.AddNorm), (A._PRODUCT, _lib.Product),
+                    (A._GATED, _lib.Gated)):
+        fields = list(flat(t))
+        values = [float(i + 1) if kind is C.c_float else i + 1 for i, (_, kind) in enumerate(fields)]
+        data = pack(*values)
+        assert len(data) == C.sizeof(t)
+        for (off, kind), v in zip(fields, values):
+            assert kind.from_buffer_copy(data, off).value == v, (t, off)
 
 
 def quantize(api, dst, src=MB, ld=64, dtype=0):
@@ -93,8 +114,9 @@ def test_quantize_refusals(api):
 
 
 def read(api, src, n=4, index=None, out=MB, ld=64, dtype=0, factor=1.0):
-    return api.p2p_read_rows_q8(CTX, C.byref(src) if src else None, index, n, factor, out, ld, dtype,
-                                None)
+    from p2p_b200._lib import ReadRows
+    a = ReadRows(src, index, out, ld, n, dtype, factor) if src else None
+    return api.p2p_read_rows_q8(CTX, C.byref(a) if a else None, None)
 
 
 def test_read_refusals(api):
@@ -107,7 +129,6 @@ def test_read_refusals(api):
     said(api, read(api, None), BAD)
     said(api, read(api, good, n=5), BAD)  # more rows than there are, in order
     said(api, read(api, good, n=-1, index=8 * MB), BAD)
-    said(api, read(api, good, n=I32_MAX + 1, index=8 * MB), BAD)
     said(api, read(api, good, index=8 * MB + 2), BAD)
     said(api, read(api, good, dtype=5), UNSUPPORTED)
     said(api, read(api, good, out=None), BAD)
@@ -160,7 +181,8 @@ def test_norm_refusals(api):
 def gemm(api, w=None, x=None, bias=None, res=None, ld_r=0, y=MB, ld_y=32, dtype=0):
     w = w or rows(4 * MB, n=32)
     x = x or rows(8 * MB)
-    return api.p2p_gemm_q8(CTX, C.byref(w), C.byref(x), bias, res, ld_r, y, ld_y, dtype, None)
+    from p2p_b200._lib import Product
+    return api.p2p_gemm_q8(CTX, C.byref(Product(w, x, bias, res, y, ld_r, ld_y, dtype)), None)
 
 
 def test_gemm_refusals(api):
@@ -170,6 +192,7 @@ def test_gemm_refusals(api):
     said(api, gemm(api, res=MB, ld_r=32), 0)  # in place
     said(api, gemm(api, x=rows(8 * MB, n=1), res=MB, ld_r=99), 0)
     assert api.host_launches() == before + 4
+    said(api, api.p2p_gemm_q8(CTX, None, None), BAD)
     said(api, gemm(api, x=rows(8 * MB, n=0), y=None), 0)
     said(api, gemm(api, w=rows(8 * MB, n=0), y=None), 0)
     said(api, gemm(api, x=rows(8 * MB, k=65)), BAD, "64 and 65")
@@ -188,7 +211,8 @@ def gate(api, g=None, u=None, x=None, act=0, h=MB, ld_h=32):
     g = g or rows(4 * MB, n=32)
     u = u or rows(6 * MB, n=32)
     x = x or rows(8 * MB)
-    return api.p2p_gate_q8(CTX, C.byref(g), C.byref(u), C.byref(x), act, h, ld_h, None)
+    from p2p_b200._lib import Gated
+    return api.p2p_gate_q8(CTX, C.byref(Gated(g, u, x, h, ld_h, act)), None)
 
 
 def test_gate_refusals(api):
@@ -197,6 +221,7 @@ def test_gate_refusals(api):
     said(api, gate(api, act=1), 0)
     said(api, gate(api, u=rows(4 * MB, n=32)), 0)  # the same weights twice
     assert api.host_launches() == before + 3
+    said(api, api.p2p_gate_q8(CTX, None, None), BAD)
     said(api, gate(api, x=rows(8 * MB, n=0), h=None), 0)
     for bad in ({"act": 2}, {"act": -1}, {"u": rows(6 * MB, n=31)}, {"u": rows(6 * MB, n=32, k=63)},
                 {"x": rows(8 * MB, k=63)}, {"h": None}, {"h": MB + 1}, {"ld_h": 31},
