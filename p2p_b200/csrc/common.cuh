@@ -132,6 +132,31 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// ---- two f32 operations in one instruction --------------------------------------------------
+union Pair {
+  uint64_t w;
+  float f[2];
+};
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair p;
+  p.f[0] = a;
+  p.f[1] = b;
+  return p;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.w) : "l"(b.w));
+  return a;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.w) : "l"(b.w));
+  return a;
+}
+// a * b + c
+__device__ __forceinline__ Pair mad2(Pair a, Pair b, Pair c) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.w) : "l"(a.w), "l"(b.w));
+  return c;
+}
+
 // ---- q/k RMSNorm + RoPE of one 64-wide head held by one warp ------------------------------
 // Lane l holds elements l and l+32 (the rotate-half partners, kernels.js:257-262).  The
 // sum of squares is folded with xor-butterflies 16, 8, 4, 2, 1 after pairing (l, l+32): every

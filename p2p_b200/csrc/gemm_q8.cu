@@ -44,7 +44,9 @@ struct Q8Params {
   int32_t whole;  // tiles of full width
   int32_t wide;   // y and res rows on 16-byte boundaries
   // narrow_kernel
-  int32_t rows, tokens, stages;  // of a tile; of the ring
+  int32_t rows, tokens, steps;  // of a tile
+  int32_t stages, chunks;       // of the ring; of a stage
+  int32_t deep;                 // the tensor maps' third dimension is k in steps of 128
 };
 
 // act(g) * u.  The exponential and the quotient are approximations of 2 units in the last place each.
@@ -53,8 +55,15 @@ __device__ __forceinline__ float act_mul(float g, float u, int act) {
   return __fdividef(g, 1.f + __expf(-t)) * u;
 }
 
+__device__ __forceinline__ Pair act_mul2(Pair g, Pair u, int act) {
+  return pair(act_mul(g.f[0], u.f[0], act), act_mul(g.f[1], u.f[1], act));
+}
+
 __device__ __forceinline__ float scaled(uint32_t acc, float xs, float ws) {
   return __fmul_rn(__fmul_rn(float(int(acc)), xs), ws);
+}
+__device__ __forceinline__ Pair scaled2(uint32_t a, uint32_t b, Pair xs, Pair ws) {
+  return mul2(mul2(pair(float(int(a)), float(int(b))), xs), ws);
 }
 
 // ---- many tokens ------------------------------------------------------------------------------------
@@ -66,12 +75,15 @@ constexpr int kWideThreads = 32 * (kEpiWarps + 2);
 constexpr int kBoxRows = 64;    // weight rows per TMA box
 constexpr uint32_t kTileBytes = kRows * kStep;          // x, and a CTA's half of the weights
 constexpr int kWideStages = 5;
-constexpr int kPitch = 33;
+// A warp's 32 x 32 outputs change hands through shared memory, so that it stores whole stretches of rows: a
+// row of f32 takes 36 words, one of f16 20 (both keep 16-byte accesses of a column free of conflicts).
+template <class T>
+constexpr int kPitch = sizeof(T) == 4 ? 36 : 20;
 
 struct __align__(1024) WideSmem {
   uint8_t a[kWideStages][kTileBytes];
   uint8_t b[kWideStages][kTileBytes];
-  float turn[kEpiWarps][32 * kPitch];   // a warp's 32 x 32 outputs, to store rows along lanes
+  uint32_t turn[kEpiWarps][32 * kPitch<float>];
   float col[kEpiWarps][2][128];         // a warp's columns: scales, and biases or the up scales
   uint64_t full[kWideStages], empty[kWideStages];
   uint64_t acc_full[2], acc_empty[2];
@@ -102,50 +114,59 @@ __device__ __forceinline__ Item item_of(const Q8Params& p, int i) {
   return it;
 }
 
-// 32 consecutive columns of 32 rows (a row per lane), from n on.
+// 32 consecutive columns, from n on, of 32 rows (a row per lane).  `aligned`: rows on 16-byte boundaries
+// that hold all 32 columns, and what is added has been.
 template <class T>
-__device__ __forceinline__ void store_block(const Q8Params& p, float (&v)[32], int m_base, int lane,
-                                            int n, float* turn) {
-  const int m = m_base + lane;
-  if (p.wide && n + 32 <= p.n) {
-    if (m >= p.m) return;
-    constexpr int V = 16 / sizeof(T);
-    union {
-      uint4 u;
-      T e[V];
-    } w;
-    if (p.res) {
-      const uint4* r = reinterpret_cast<const uint4*>(static_cast<const T*>(p.res) +
-                                                      int64_t(m) * p.ld_res + n);
+__device__ __forceinline__ void store_block(const Q8Params& p, const Pair (&v)[16], int m_base, int lane,
+                                            int n, bool aligned, uint32_t* turn) {
+  if (aligned) {
+    constexpr int kWords = 32 * sizeof(T) / 4, kPieces = kWords / 4;  // of a row
+    uint4* mine = reinterpret_cast<uint4*>(turn + lane * kPitch<T>);
 #pragma unroll
-      for (int i = 0; i < 32 / V; ++i) {
-        w.u = r[i];
+    for (int i = 0; i < kPieces; ++i) {
+      uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[i * V + j] = __fadd_rn(v[i * V + j], to_f32(w.e[j]));
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          w[j] = __float_as_uint(v[2 * i + j / 2].f[j % 2]);
+        } else {
+          const __half2 h = __floats2half2_rn(v[4 * i + j].f[0], v[4 * i + j].f[1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
       }
+      mine[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    uint4* d = reinterpret_cast<uint4*>(static_cast<T*>(p.y) + int64_t(m) * p.ld_y + n);
+    __syncwarp();
+    constexpr int kRowsAtOnce = 32 / kPieces;
+    const int r0 = lane / kPieces, piece = lane % kPieces;
+    T* d = static_cast<T*>(p.y) + int64_t(m_base + r0) * p.ld_y + n;
+    const int64_t ld = kRowsAtOnce * p.ld_y;
 #pragma unroll
-    for (int i = 0; i < 32 / V; ++i) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) w.e[j] = from_f32<T>(v[i * V + j]);
-      d[i] = w.u;
+    for (int i = 0; i < kPieces; ++i, d += ld) {
+      const uint4 w = reinterpret_cast<const uint4*>(turn + (r0 + i * kRowsAtOnce) * kPitch<T>)[piece];
+      if (m_base + r0 + i * kRowsAtOnce < p.m) reinterpret_cast<uint4*>(d)[piece] = w;
     }
+    __syncwarp();
     return;
   }
   // rows that start anywhere, or end inside the block: a row at a time along the lanes
+  float4* mine = reinterpret_cast<float4*>(turn + lane * kPitch<float>);
 #pragma unroll
-  for (int c = 0; c < 32; ++c) turn[lane * kPitch + c] = v[c];
+  for (int i = 0; i < 8; ++i)
+    mine[i] = make_float4(v[2 * i].f[0], v[2 * i].f[1], v[2 * i + 1].f[0], v[2 * i + 1].f[1]);
   __syncwarp();
   const int rows = min(32, p.m - m_base), c = n + lane;
   if (c < p.n) {
     T* d = static_cast<T*>(p.y) + int64_t(m_base) * p.ld_y + c;
-    const T* r = static_cast<const T*>(p.res) + int64_t(m_base) * p.ld_res + c;
-#pragma unroll 4
-    for (int i = 0; i < rows; ++i) {
-      float y = turn[i * kPitch + lane];
-      if (p.res) y = __fadd_rn(y, to_f32(r[int64_t(i) * p.ld_res]));
-      d[int64_t(i) * p.ld_y] = from_f32<T>(y);
+    const float* t = reinterpret_cast<const float*>(turn) + lane;
+    if (p.res) {
+      const T* r = static_cast<const T*>(p.res) + int64_t(m_base) * p.ld_res + c;
+#pragma unroll 8
+      for (int i = 0; i < rows; ++i, d += p.ld_y, r += p.ld_res, t += kPitch<float>)
+        *d = from_f32<T>(__fadd_rn(*t, to_f32(*r)));
+    } else {
+#pragma unroll 8
+      for (int i = 0; i < rows; ++i, d += p.ld_y, t += kPitch<float>) *d = from_f32<T>(*t);
     }
   }
   __syncwarp();
@@ -171,36 +192,66 @@ __device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem& s, ui
     else if (p.bias) second[i] = c < p.n ? p.bias[c] : 0.f;
   }
   __syncwarp();
+  const Pair xs2 = pair(xs, xs);
+  const int m = m_base + lane;
   for (int b = half, i = 0; b < blocks; b += 2, i += 32) {
+    const int n = it.n0 + b * 32;
+    const bool some = m_base < p.m && n < p.n, aligned = p.wide && n + 32 <= p.n;
+    constexpr int kPieces = 32 * sizeof(T) / 16, V = 16 / sizeof(T);
+    union {
+      uint4 u;
+      T e[V];
+    } res[GATE ? 1 : kPieces];
+    const bool add = !GATE && p.res && aligned;
+    if (add) {
+      const uint4* r = reinterpret_cast<const uint4*>(static_cast<const T*>(p.res) +
+                                                      int64_t(m) * p.ld_res + n);
+#pragma unroll
+      for (int j = 0; j < (GATE ? 1 : kPieces); ++j) res[j].u = m < p.m ? r[j] : make_uint4(0, 0, 0, 0);
+    }
     uint32_t r[32];
-    float v[32];
+    Pair v[16];
     tmem_ld32(at + b * 32, r);
     tmem_ld_wait();
+    const float4* w4 = reinterpret_cast<const float4*>(ws + i);
+    const float4* s4 = reinterpret_cast<const float4*>(second + i);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = scaled(r[j], xs, ws[i + j]);
+    for (int j = 0; j < 8; ++j) {
+      const float4 w = w4[j];
+      v[2 * j] = scaled2(r[4 * j], r[4 * j + 1], xs2, pair(w.x, w.y));
+      v[2 * j + 1] = scaled2(r[4 * j + 2], r[4 * j + 3], xs2, pair(w.z, w.w));
+    }
     if constexpr (GATE) {
       tmem_ld32(at + cols + b * 32, r);
       tmem_ld_wait();
-      if (p.act == kActSilu) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          v[j] = act_mul(v[j], scaled(r[j], xs, second[i + j]), kActSilu);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          v[j] = act_mul(v[j], scaled(r[j], xs, second[i + j]), kActGelu);
+      for (int j = 0; j < 8; ++j) {
+        const float4 w = s4[j];
+        const Pair u0 = scaled2(r[4 * j], r[4 * j + 1], xs2, pair(w.x, w.y));
+        const Pair u1 = scaled2(r[4 * j + 2], r[4 * j + 3], xs2, pair(w.z, w.w));
+        v[2 * j] = act_mul2(v[2 * j], u0, p.act);
+        v[2 * j + 1] = act_mul2(v[2 * j + 1], u1, p.act);
       }
     } else if (p.bias) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], second[i + j]);
+      for (int j = 0; j < 8; ++j) {
+        const float4 w = s4[j];
+        v[2 * j] = add2(v[2 * j], pair(w.x, w.y));
+        v[2 * j + 1] = add2(v[2 * j + 1], pair(w.z, w.w));
+      }
     }
     if (b + 2 >= blocks) {  // everything of this warp is in registers
       tc_fence_before();
       __syncwarp();
       release();
     }
-    if (m_base < p.m && it.n0 + b * 32 < p.n)
-      store_block<T>(p, v, m_base, lane, it.n0 + b * 32, s.turn[warp]);
+    if (add) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        v[j] = add2(v[j], pair(to_f32(res[GATE ? 0 : 2 * j / V].e[2 * j % V]),
+                               to_f32(res[GATE ? 0 : 2 * j / V].e[2 * j % V + 1])));
+    }
+    if (some) store_block<T>(p, v, m_base, lane, n, aligned, s.turn[warp]);
     __syncwarp();
   }
 }
@@ -256,10 +307,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         if (elect_one()) {
           const uint32_t full0 = cluster_map(smem_u32(&s.full[st]), 0);
           if (rank == 0) mbar_arrive_expect_tx(&s.full[st], 2 * (kTileBytes + half * kStep));
-          tma_load_2d_pair(s.a[st], &tm_x, kt * kStep, m0, full0);
-          tma_load_2d_pair(s.b[st], tm_b, kt * kStep, n0, full0);
+          tma_load_3d_pair(s.a[st], &tm_x, kt * kStep, m0, 0, full0);
+          tma_load_3d_pair(s.b[st], tm_b, kt * kStep, n0, 0, full0);
           if (half > kBoxRows)
-            tma_load_2d_pair(s.b[st] + kBoxRows * kStep, tm_b, kt * kStep, n0 + kBoxRows, full0);
+            tma_load_3d_pair(s.b[st] + kBoxRows * kStep, tm_b, kt * kStep, n0 + kBoxRows, 0, full0);
         }
         __syncwarp();
         if (++st == kWideStages) {
@@ -361,7 +412,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 // accumulators running on across them.
 //   SPLIT: too few channels for that; a tile's k is cut over a cluster, one tile each.  Every CTA sums its
 // part and hands the sums, by token, to the CTA that finishes that token.
-constexpr int kNarrowThreads = 192;  // TMA, MMA, four epilogue warps
+constexpr int kNarrowEpi = 8;        // epilogue warps: two per TMEM lane quarter
+constexpr int kNarrowThreads = 32 * (2 + kNarrowEpi);  // TMA, MMA, epilogue
 constexpr int kMostTokens = 128;
 constexpr int kMostSplit = 8;
 constexpr int kMostStages = 24;
@@ -393,14 +445,15 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
   const int split = SPLIT ? int(cluster_ctas()) : 1, rank = SPLIT ? int(cluster_ctarank()) : 0;
   const int first = SPLIT ? int(blockIdx.x) / split : int(blockIdx.x);
   const int step = SPLIT ? p.items : int(gridDim.x);
-  const uint32_t w_bytes = uint32_t(p.rows) * kStep, x_bytes = uint32_t(p.tokens) * kStep;
-  const uint32_t stage_bytes = G * w_bytes + x_bytes;
+  // a stage: `chunks` steps of k, [w][chunk][rows][128], GATE: [up] likewise, [x][chunk][tokens][128]
+  const uint32_t w_step = uint32_t(p.rows) * kStep, x_step = uint32_t(p.tokens) * kStep;
+  const uint32_t w_bytes = p.chunks * w_step, stage_bytes = G * w_bytes + p.chunks * x_step;
   const int own = (p.tokens + split - 1) / split;  // SPLIT: tokens finished here
   uint32_t* sums = reinterpret_cast<uint32_t*>(base + 1024);  // [split][own][G][rows]
-  uint8_t* ring = base + 1024 + (SPLIT ? (split * own * G * p.rows * 4 + 1023) / 1024 * 1024 : 0);
-  const int nk = (p.k + kStep - 1) / kStep;
-  const int k0 = SPLIT ? int(int64_t(nk) * rank / split) : 0,
-            k1 = SPLIT ? int(int64_t(nk) * (rank + 1) / split) : nk;
+  constexpr int kScales = kNarrowEpi * kMostTokens * 4;  // each epilogue warp's copy of the tokens' scales
+  uint8_t* ring = base + 1024 + (SPLIT ? (split * own * G * p.rows * 4 + 1023) / 1024 * 1024 : kScales);
+  const int nk = p.steps;  // stages of a tile
+  const int k0 = SPLIT ? nk * rank / split : 0, k1 = SPLIT ? nk * (rank + 1) / split : nk;
   const uint32_t acc_cols = G * p.tokens;  // of one accumulator buffer
   const uint32_t need = SPLIT ? acc_cols : 2 * acc_cols;
   const uint32_t tmem_cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
@@ -411,7 +464,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.acc_full[i], 1);
-      mbar_init(&s.acc_empty[i], 4);
+      mbar_init(&s.acc_empty[i], kNarrowEpi);
     }
     mbar_init(&s.done, 1);
     s.abort_flag = 0;
@@ -433,17 +486,21 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     bool ok = true;
     for (int t = first; t < p.items && ok; t += step) {
       const int n0 = t % p.tiles_n * p.rows, m0 = t / p.tiles_n * p.tokens;
-      for (int kt = k0; kt < k1; ++kt) {
+      // each CTA begins at another part of k: all of them read the same tokens
+      int kt = k0 + first % (k1 - k0);
+      for (int i = k0; i < k1; ++i) {
         if (round > 0 && !(ok = gemm_wait_all(s.abort_flag, &s.empty[st], (round - 1) & 1, p.err)))
           break;
         if (elect_one()) {
           uint8_t* a = ring + st * stage_bytes;
+          const int kx = p.deep ? 0 : kt * kStep, kz = p.deep ? kt * p.chunks : 0;
           mbar_arrive_expect_tx(&s.full[st], stage_bytes);
-          tma_load_2d(a, &tm_w, kt * kStep, n0, &s.full[st]);
-          if constexpr (GATE) tma_load_2d(a + w_bytes, &tm_u, kt * kStep, n0, &s.full[st]);
-          tma_load_2d(a + G * w_bytes, &tm_x, kt * kStep, m0, &s.full[st]);
+          tma_load_3d(a, &tm_w, kx, n0, kz, &s.full[st]);
+          if constexpr (GATE) tma_load_3d(a + w_bytes, &tm_u, kx, n0, kz, &s.full[st]);
+          tma_load_3d(a + G * w_bytes, &tm_x, kx, m0, kz, &s.full[st]);
         }
         __syncwarp();
+        if (++kt == k1) kt = k0;
         if (++st == uint32_t(p.stages)) {
           st = 0;
           ++round;
@@ -476,14 +533,16 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
         if (!(ok = gemm_wait_all(s.abort_flag, &s.full[st], round & 1, p.err))) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t ad = desc0 + uint64_t(st) * (stage_bytes >> 4),
-                         bd = ad + ((G * w_bytes) >> 4);
+          uint64_t ad = desc0 + uint64_t(st) * (stage_bytes >> 4), bd = ad + ((G * w_bytes) >> 4);
+          uint32_t more = kt > k0 ? 1u : 0u;
+          for (int c = 0; c < p.chunks; ++c, ad += w_step >> 4, bd += x_step >> 4) {
 #pragma unroll
-          for (int kk = 0; kk < kStep / 32; ++kk) {
-            mma_i8_ss(acc, ad + 2 * kk, bd + 2 * kk, idesc, (kt > k0 || kk > 0) ? 1u : 0u);
-            if constexpr (GATE)
-              mma_i8_ss(acc + p.tokens, ad + (w_bytes >> 4) + 2 * kk, bd + 2 * kk, idesc,
-                        (kt > k0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < kStep / 32; ++kk) {
+              mma_i8_ss(acc, ad + 2 * kk, bd + 2 * kk, idesc, more);
+              if constexpr (GATE)
+                mma_i8_ss(acc + p.tokens, ad + (w_bytes >> 4) + 2 * kk, bd + 2 * kk, idesc, more);
+              more = 1u;
+            }
           }
           mma_commit(&s.empty[st]);
         }
@@ -508,22 +567,31 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
       __syncwarp();
     }
   } else {
-    // lane of TMEM quarter warp & 3 -> channel: 32 a quarter, or 16 of an MMA of 64 rows
-    const int quarter = warp & 3;
+    // lane of TMEM quarter warp & 3 -> channel: 32 a quarter, or 16 of an MMA of 64 rows.  The two warps of
+    // a quarter take every other eight tokens.
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
     const bool tall = p.rows > 64;
     const int ch = tall ? quarter * 32 + lane : quarter * 16 + lane;
     const bool mine = ch < p.rows && (tall || lane < 16);
-    int n = 0;
+    float* scales = reinterpret_cast<float*>(base + 1024) + (warp - 2) * kMostTokens;
+    int n = 0, have = -1;  // tiles of this CTA; first token of the tile whose scales are there
     for (int t = first; t < p.items; t += step, ++n) {
       const int b = n & 1, u = n >> 1;
       const int c = t % p.tiles_n * p.rows + ch, m0 = t / p.tiles_n * p.tokens;
       const int tokens = min(p.tokens, p.m - m0);
       const bool live = mine && c < p.n;
       float ws = 0.f, second = 0.f;
-      if (!SPLIT && live) {
-        ws = p.ws[c];
-        if constexpr (GATE) second = p.us[c];
-        else if (p.bias) second = p.bias[c];
+      if constexpr (!SPLIT) {
+        if (live) {
+          ws = p.ws[c];
+          if constexpr (GATE) second = p.us[c];
+          else if (p.bias) second = p.bias[c];
+        }
+        if (have != m0) {
+          __syncwarp();
+          for (int i = lane; i < p.tokens; i += 32) scales[i] = i < tokens ? p.xs[m0 + i] : 0.f;
+          have = m0;
+        }
       }
       __syncwarp();
       const bool ok = gemm_wait_all(s.abort_flag, &s.acc_full[b], u & 1, p.err);
@@ -532,11 +600,11 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
       tc_fence_after();
       const uint32_t at = tmem + uint32_t(b) * acc_cols + (uint32_t(quarter * 32) << 16);
       if constexpr (SPLIT) {
-        int to = 0, tl = 0;  // token t0 + j is number tl of CTA `to`
-        for (int t0 = 0; t0 < p.tokens; t0 += 8) {
+        for (int t0 = half * 8; t0 < p.tokens; t0 += 16) {
           uint32_t r[G][8];
 #pragma unroll
           for (int g = 0; g < G; ++g) tmem_ld8(at + g * p.tokens + t0, r[g]);
+          int to = t0 / own, tl = t0 - to * own;  // token t0 + j is number tl of CTA `to`
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -552,39 +620,45 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
           }
         }
       } else {
-        T* y = static_cast<T*>(p.y) + int64_t(m0) * p.ld_y + c;
-        const T* res = static_cast<const T*>(p.res) + int64_t(m0) * p.ld_res + c;
-        float xs32 = 0.f;
-        for (int t0 = 0; t0 < p.tokens; t0 += 8) {
-          if (t0 % 32 == 0) xs32 = t0 + lane < tokens ? p.xs[m0 + t0 + lane] : 0.f;
+        const Pair ws2 = pair(ws, ws), second2 = pair(second, second);
+        T* y = static_cast<T*>(p.y) + int64_t(m0 + half * 8) * p.ld_y + c;
+        const T* res = p.res ? static_cast<const T*>(p.res) + int64_t(m0 + half * 8) * p.ld_res + c : nullptr;
+        for (int t0 = half * 8; t0 < p.tokens; t0 += 16) {
+          const int left = tokens - t0;  // of these eight
           uint32_t r[G][8];
 #pragma unroll
           for (int g = 0; g < G; ++g) tmem_ld8(at + g * p.tokens + t0, r[g]);
           float add[8];
-          if constexpr (!GATE) {
+          if (!GATE && res) {
+            const T* q = res;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              add[j] = p.res && live && t0 + j < tokens ? to_f32(res[int64_t(t0 + j) * p.ld_res]) : 0.f;
+            for (int j = 0; j < 8; ++j, q += p.ld_res) add[j] = live && j < left ? to_f32(*q) : 0.f;
+            res += 16 * p.ld_res;
           }
           tmem_ld_wait();
-          if (t0 + 8 >= p.tokens) {  // everything of this warp is in registers
+          if (t0 + 16 >= p.tokens) {  // everything of this warp is in registers
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.acc_empty[b]);
           }
+          T* d = y;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float xs = __shfl_sync(0xffffffffu, xs32, (t0 + j) & 31);
-            float v = scaled(r[0][j], xs, ws);
+          for (int j = 0; j < 8; j += 2, d += 2 * p.ld_y) {
+            const Pair xs2 = pair(scales[t0 + j], scales[t0 + j + 1]);
+            Pair v = scaled2(r[0][j], r[0][j + 1], xs2, ws2);
             if constexpr (GATE) {
-              v = act_mul(v, scaled(r[G - 1][j], xs, second), p.act);
+              v = act_mul2(v, scaled2(r[G - 1][j], r[G - 1][j + 1], xs2, second2), p.act);
             } else {
-              if (p.bias) v = __fadd_rn(v, second);
-              if (p.res) v = __fadd_rn(v, add[j]);
+              if (p.bias) v = add2(v, second2);
+              if (res) v = add2(v, pair(add[j], add[j + 1]));
             }
-            if (live && t0 + j < tokens) y[int64_t(t0 + j) * p.ld_y] = from_f32<T>(v);
+            if (live && j < left) d[0] = from_f32<T>(v.f[0]);
+            if (live && j + 1 < left) d[p.ld_y] = from_f32<T>(v.f[1]);
           }
+          y += 16 * p.ld_y;
         }
+        // a tile of eight tokens has none for the second warp of a quarter
+        if (half * 8 >= p.tokens && lane == 0) mbar_arrive(&s.acc_empty[b]);
       }
     }
   }
@@ -633,16 +707,20 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
 
 // ---- host -------------------------------------------------------------------------------------------
 // Rows of codes in boxes of 128 codes x box_rows, 128-byte swizzle; what lies outside reads as 0.
-bool map_codes(CUtensorMap* m, const Q8Rows& r, uint32_t box_rows) {
+// chunks > 1: rows of whole steps of 128 codes, the steps a dimension of their own, that many of them in
+// a box.
+bool map_codes(CUtensorMap* m, const Q8Rows& r, int box_rows, int chunks = 1) {
   auto enc = encode_fn();
   if (!enc) return false;
-  cuuint64_t dims[2] = {cuuint64_t(r.cols), cuuint64_t(r.rows)};
-  cuuint64_t strides[1] = {cuuint64_t(r.ld)};
-  cuuint32_t box[2] = {kStep, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r.q, dims, strides, box, estr,
+  const bool deep = chunks > 1;
+  cuuint64_t dims[3] = {cuuint64_t(deep ? kStep : r.cols), cuuint64_t(r.rows),
+                        cuuint64_t(deep ? r.cols / kStep : 1)};
+  cuuint64_t strides[2] = {cuuint64_t(r.ld), kStep};
+  cuuint32_t box[3] = {kStep, cuuint32_t(box_rows), cuuint32_t(chunks)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, r.q, dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -709,31 +787,38 @@ cudaError_t launch_wide(Q8Params p, const GemmQ8Args& a, int num_sms, cudaStream
                         stream);
 }
 
-// How few tokens are cut up: channels of a tile and CTAs of its k.
+// How few tokens are cut up.
 struct NarrowPlan {
-  int rows, split, tokens;
-  double cost;  // cycles
+  int rows, tokens, split;  // channels and tokens of a tile, CTAs of its k
+  int chunks, steps;        // steps of 128 codes in a stage, stages of a tile
+  double cost;              // cycles
 };
-// The busiest SM's time: its tiles times the longer of what a tile loads (of L2, about kLoad bytes a
-// cycle; an SM's share of the DRAM rate bounds the weights) and what it multiplies (8192 products a cycle
-// with 128 rows, half with 64, and the shared memory that an MMA's weight rows take at 128 bytes a cycle).
+// The busiest SM's time: its tiles, their stages, and of a stage the longer of what it loads (from L2
+// about kLoad bytes a cycle; the weights at an SM's share of the DRAM rate), what it multiplies (8192
+// products a cycle with 128 rows, half with 64; an MMA takes its weight rows at 128 bytes a cycle, and kIssue
+// cycles to be issued) and what it takes to hand a stage over.
 NarrowPlan narrow_plan(int m, int n, int k, int G, int num_sms) {
-  constexpr double kLoad = 50, kDram = 23, kSplitCost = 2500;
+  constexpr double kLoad = 50, kDram = 23, kIssue = 22, kHandOver = 250, kSplitCost = 2000;
+  constexpr int kMostChunks = 4, kMostStage = 48 * 1024;
   const int tokens = std::min(kMostTokens, m <= 24 ? (m + 7) / 8 * 8 : (m + 15) / 16 * 16);
   const int token_tiles = (m + tokens - 1) / tokens, nk = (k + kStep - 1) / kStep;
-  NarrowPlan best{0, 0, tokens, 0};
-  for (int split = 1; split <= std::min(kMostSplit, nk); split *= 2) {
-    for (int rows = 8; rows <= 128; rows += 8) {
+  NarrowPlan best{};
+  for (int rows = 8; rows <= 128; rows += 8) {
+    int chunks = 1;  // as many as leave a tile no part of a stage empty
+    if (k % kStep == 0)
+      for (int c = 2; c <= kMostChunks && c * (G * rows + tokens) * kStep <= kMostStage; ++c)
+        if (nk % c == 0) chunks = c;
+    const int steps = nk / chunks;
+    const double load = std::max((G * rows + tokens) * kStep / kLoad, G * rows * kStep / kDram);
+    const double mma = 4.0 * G * std::max({tokens / 2.0, rows <= 64 ? 16.0 : 32.0, kIssue});
+    const double stage = std::max(chunks * std::max(load, mma), kHandOver);
+    for (int split = 1; split <= std::min(kMostSplit, steps); split *= 2) {
       if (split > 1 && G * rows > 128) break;
       const int64_t ctas = (int64_t(n) + rows - 1) / rows * token_tiles * split;
       const double tiles = double((ctas + num_sms - 1) / num_sms);
-      const double steps = double((nk + split - 1) / split);
-      const double load = std::max((G * rows + tokens) * kStep / kLoad, G * rows * kStep / kDram);
-      const double mma = 4.0 * G * std::max(tokens / 2.0, rows <= 64 ? 16.0 : 32.0);
-      double cost = tiles * steps * std::max(load, mma);
-      if (split > 1) cost += tiles * kSplitCost;
-      else cost += tokens * 30.0;  // the last tile's epilogue
-      if (!best.rows || cost < best.cost) best = NarrowPlan{rows, split, tokens, cost};
+      const double cost = tiles * (((steps + split - 1) / split) * stage + (split > 1 ? kSplitCost : 0)) +
+                          (split > 1 ? 0 : tokens * 30.0);  // the last tile's epilogue
+      if (!best.rows || cost < best.cost) best = NarrowPlan{rows, tokens, split, chunks, steps, cost};
     }
   }
   return best;
@@ -744,24 +829,27 @@ cudaError_t launch_narrow(Q8Params p, const GemmQ8Args& a, const NarrowPlan& pla
                           cudaStream_t stream) {
   constexpr int G = GATE ? 2 : 1;
   CUtensorMap tx, tw, tu;
-  if (!map_codes(&tx, a.x, unsigned(plan.tokens)) || !map_codes(&tw, a.w, unsigned(plan.rows)) ||
-      (GATE && !map_codes(&tu, a.up, unsigned(plan.rows))))
+  if (!map_codes(&tx, a.x, plan.tokens, plan.chunks) || !map_codes(&tw, a.w, plan.rows, plan.chunks) ||
+      (GATE && !map_codes(&tu, a.up, plan.rows, plan.chunks)))
     return cudaErrorInvalidValue;
   if (!GATE) tu = tw;
   p.rows = plan.rows;
   p.tokens = plan.tokens;
+  p.steps = plan.steps;
+  p.chunks = plan.chunks;
+  p.deep = plan.chunks > 1;
   p.tiles_n = (p.n + plan.rows - 1) / plan.rows;
   const int64_t tiles = int64_t(p.tiles_n) * ((int64_t(p.m) + plan.tokens - 1) / plan.tokens);
   if (tiles * plan.split > INT32_MAX) return cudaErrorInvalidValue;
   p.items = int32_t(tiles);
-  const int nk = (p.k + kStep - 1) / kStep;
   const int own = (plan.tokens + plan.split - 1) / plan.split;
-  const int stage = (G * plan.rows + plan.tokens) * kStep;
-  const int sums = SPLIT ? (plan.split * own * G * plan.rows * 4 + 1023) / 1024 * 1024 : 0;
+  const int stage = (G * plan.rows + plan.tokens) * kStep * plan.chunks;
+  const int sums = SPLIT ? (plan.split * own * G * plan.rows * 4 + 1023) / 1024 * 1024
+                         : kNarrowEpi * kMostTokens * 4;
   // behind the ring, what the last stage's MMA reads beyond its rows
   const int fixed = 2048 + sums + (plan.rows <= 64 ? 64 : 128) * kStep;
-  const int64_t steps = SPLIT ? (nk + plan.split - 1) / plan.split
-                              : nk * ((tiles + num_sms - 1) / num_sms);
+  const int64_t steps = SPLIT ? (plan.steps + plan.split - 1) / plan.split
+                              : plan.steps * ((tiles + num_sms - 1) / num_sms);
   p.stages = int(std::min<int64_t>({kMostStages, steps, (kNarrowSmem - fixed) / stage}));
   size_t smem = size_t(fixed) + size_t(p.stages) * stage;
   // The CTAs of a cluster wait for one another, and an allocation of TMEM waits for whoever holds it: so

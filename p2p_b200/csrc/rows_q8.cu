@@ -20,29 +20,6 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr float kTiny = 0x1p-100f;  // a row below it counts as zeros (127 / a stays finite)
 
-// Two f32 operations in one instruction.
-union Pair {
-  uint64_t w;
-  float f[2];
-};
-__device__ __forceinline__ Pair pair(float a, float b) {
-  Pair p;
-  p.f[0] = a;
-  p.f[1] = b;
-  return p;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.w) : "l"(b.w));
-  return a;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.w) : "l"(b.w));
-  return a;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.w) : "l"(a.w), "l"(b.w));
-  return c;
-}
 // max(|a|, |b|, |c|), NaN if one of them is.
 __device__ __forceinline__ float max_abs3(float a, float b, float c) {
   float d;
@@ -189,7 +166,7 @@ __device__ __forceinline__ void store_codes(int8_t* row, const Columns<V>& c, in
   for (int i = 0; i < V / 2; ++i) {
     const Pair q = mul2(v[i], inv);
     t[i] = add2(q, up);
-    const Pair d = fma2(add2(t[i], down), minus, q);  // q less its code
+    const Pair d = mad2(add2(t[i], down), minus, q);  // q less its code
     far = max_abs3(far, d.f[0], d.f[1]);
   }
   if (far > 0.49996f) {  // 127 * 2^-22 from a half
@@ -288,7 +265,7 @@ __device__ __forceinline__ void sum_piece(RowSums& sums, Pair& ss, const Piece<T
   for (int j = 0; j < V / 2; ++j) {
     Pair v = x.get(j);
     if constexpr (NORM) {
-      ss = fma2(v, v, ss);
+      ss = mad2(v, v, ss);
       v = mul2(v, wide2(w[j]));
     }
     sums.top = max_abs3(sums.top, v.f[0], v.f[1]);
