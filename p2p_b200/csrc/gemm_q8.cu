@@ -428,8 +428,18 @@ struct NarrowHead {  // in front of the ring and the sums
 };
 static_assert(sizeof(NarrowHead) <= 1024, "the head is one swizzle atom");
 
+__device__ __forceinline__ void st_cluster4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                            uint32_t d) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
 __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+__host__ __device__ inline int split_tokens(int tokens, int split) {
+  return ((tokens + split - 1) / split + 3) / 4 * 4;
 }
 
 template <class T, bool GATE, bool SPLIT>
@@ -448,10 +458,12 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
   // a stage: `chunks` steps of k, [w][chunk][rows][128], GATE: [up] likewise, [x][chunk][tokens][128]
   const uint32_t w_step = uint32_t(p.rows) * kStep, x_step = uint32_t(p.tokens) * kStep;
   const uint32_t w_bytes = p.chunks * w_step, stage_bytes = G * w_bytes + p.chunks * x_step;
-  const int own = (p.tokens + split - 1) / split;  // SPLIT: tokens finished here
-  uint32_t* sums = reinterpret_cast<uint32_t*>(base + 1024);  // [split][own][G][rows]
+  // SPLIT: tokens finished here, in fours, and where the sums lie: [split][G][rows][own + 4] (the four words
+  // between two channels keep 16-byte accesses of neighbouring channels free of conflicts)
+  const int own = split_tokens(p.tokens, split), pitch = own + 4;
+  uint32_t* sums = reinterpret_cast<uint32_t*>(base + 1024);
   constexpr int kScales = kNarrowEpi * kMostTokens * 4;  // each epilogue warp's copy of the tokens' scales
-  uint8_t* ring = base + 1024 + (SPLIT ? (split * own * G * p.rows * 4 + 1023) / 1024 * 1024 : kScales);
+  uint8_t* ring = base + 1024 + (SPLIT ? (split * G * p.rows * pitch * 4 + 1023) / 1024 * 1024 : kScales);
   const int nk = p.steps;  // stages of a tile
   const int k0 = SPLIT ? nk * rank / split : 0, k1 = SPLIT ? nk * (rank + 1) / split : nk;
   const uint32_t acc_cols = G * p.tokens;  // of one accumulator buffer
@@ -479,6 +491,24 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
   if constexpr (SPLIT) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   grid_dependency_wait();
   launch_dependents();
+
+  // SPLIT: what the epilogue warps finish: blocks of 32 channels, a block a warp (or several, each every
+  // so many tokens); scales and biases are fetched now.
+  const int n0 = first % p.tiles_n * p.rows, m0 = first / p.tiles_n * p.tokens;
+  const int blocks = (p.rows + 31) / 32, groups = kNarrowEpi / blocks, group = (warp - 2) / blocks;
+  const int mine = min(own, min(p.tokens, p.m - m0) - rank * own);  // tokens to finish
+  int ln = -1;  // this lane's channel of the tile, if it has one
+  float ws = 0.f, second = 0.f;
+  if (SPLIT && warp >= 2 && group < groups) {
+    ln = (warp - 2) % blocks * 32 + lane;
+    if (ln >= p.rows || n0 + ln >= p.n) ln = -1;
+    if (ln >= 0) {
+      ws = p.ws[n0 + ln];
+      if constexpr (GATE) second = p.us[n0 + ln];
+      else if (p.bias) second = p.bias[n0 + ln];
+    }
+    if (lane < mine) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.xs + m0 + rank * own + lane));
+  }
 
   if (warp == 0) {
     // the whole warp walks the ring, so that what the copies take is the same in all its lanes
@@ -572,14 +602,14 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const bool tall = p.rows > 64;
     const int ch = tall ? quarter * 32 + lane : quarter * 16 + lane;
-    const bool mine = ch < p.rows && (tall || lane < 16);
+    const bool held = ch < p.rows && (tall || lane < 16);
     float* scales = reinterpret_cast<float*>(base + 1024) + (warp - 2) * kMostTokens;
     int n = 0, have = -1;  // tiles of this CTA; first token of the tile whose scales are there
     for (int t = first; t < p.items; t += step, ++n) {
       const int b = n & 1, u = n >> 1;
       const int c = t % p.tiles_n * p.rows + ch, m0 = t / p.tiles_n * p.tokens;
       const int tokens = min(p.tokens, p.m - m0);
-      const bool live = mine && c < p.n;
+      const bool live = held && c < p.n;
       float ws = 0.f, second = 0.f;
       if constexpr (!SPLIT) {
         if (live) {
@@ -604,19 +634,16 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
           uint32_t r[G][8];
 #pragma unroll
           for (int g = 0; g < G; ++g) tmem_ld8(at + g * p.tokens + t0, r[g]);
-          int to = t0 / own, tl = t0 - to * own;  // token t0 + j is number tl of CTA `to`
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < 8; j += 4) {
+            const int to = (t0 + j) / own, tl = t0 + j - to * own;  // number tl of CTA `to`
             const uint32_t dst = cluster_map(
-                smem_u32(sums + (rank * own + tl) * (G * p.rows) + ch), uint32_t(to));
+                smem_u32(sums + (rank * G * p.rows + ch) * pitch + tl), uint32_t(to));
 #pragma unroll
             for (int g = 0; g < G; ++g)
-              if (mine) st_cluster(dst + g * p.rows * 4, r[g][j]);
-            if (++tl == own) {
-              tl = 0;
-              ++to;
-            }
+              if (held)
+                st_cluster4(dst + g * p.rows * pitch * 4, r[g][j], r[g][j + 1], r[g][j + 2], r[g][j + 3]);
           }
         }
       } else {
@@ -679,27 +706,43 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     tmem_dealloc(tmem, tmem_cols);
   }
   if constexpr (SPLIT) {
-    if (s.abort_flag) return;
-    const int n0 = first % p.tiles_n * p.rows, m0 = first / p.tiles_n * p.tokens;
-    for (int tl = warp; tl < own; tl += kNarrowThreads / 32) {
-      const int m = m0 + rank * own + tl;
-      if (rank * own + tl >= p.tokens || m >= p.m) break;
-      const float xs = p.xs[m];
-      for (int c = lane; c < p.rows && n0 + c < p.n; c += 32) {
-        const int n = n0 + c;
-        int acc[G] = {};
-        for (int j = 0; j < split; ++j)
+    if (s.abort_flag || warp < 2) return;
+    if (ln >= 0) {
+      const int n = n0 + ln;
+      T* y = static_cast<T*>(p.y) + int64_t(m0 + rank * own) * p.ld_y + n;
+      const T* res = static_cast<const T*>(p.res) + int64_t(m0 + rank * own) * p.ld_res + n;
+      const Pair ws2 = pair(ws, ws), second2 = pair(second, second);
+      for (int tl = 4 * group; tl < mine; tl += 4 * groups) {
+        Pair xs[2];
+        float add[4];
 #pragma unroll
-          for (int g = 0; g < G; ++g) acc[g] += int(sums[((j * own + tl) * G + g) * p.rows + c]);
-        float v = scaled(uint32_t(acc[0]), xs, p.ws[n]);
-        if constexpr (GATE) {
-          v = act_mul(v, scaled(uint32_t(acc[G - 1]), xs, p.us[n]), p.act);
-        } else {
-          if (p.bias) v = __fadd_rn(v, p.bias[n]);
-          if (p.res)
-            v = __fadd_rn(v, to_f32(static_cast<const T*>(p.res)[int64_t(m) * p.ld_res + n]));
+        for (int j = 0; j < 4; ++j) {
+          xs[j / 2].f[j % 2] = tl + j < mine ? p.xs[m0 + rank * own + tl + j] : 0.f;
+          add[j] = !GATE && p.res && tl + j < mine ? to_f32(res[int64_t(tl + j) * p.ld_res]) : 0.f;
         }
-        static_cast<T*>(p.y)[int64_t(m) * p.ld_y + n] = from_f32<T>(v);
+        int acc[G][4] = {};
+        const uint32_t* q = sums + ln * pitch + tl;
+        for (int k = 0; k < split; ++k)
+#pragma unroll
+          for (int g = 0; g < G; ++g, q += p.rows * pitch) {
+            const uint4 a = *reinterpret_cast<const uint4*>(q);
+            acc[g][0] += int(a.x);
+            acc[g][1] += int(a.y);
+            acc[g][2] += int(a.z);
+            acc[g][3] += int(a.w);
+          }
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          Pair v = scaled2(acc[0][j], acc[0][j + 1], xs[j / 2], ws2);
+          if constexpr (GATE) {
+            v = act_mul2(v, scaled2(acc[G - 1][j], acc[G - 1][j + 1], xs[j / 2], second2), p.act);
+          } else {
+            if (p.bias) v = add2(v, second2);
+            if (p.res) v = add2(v, pair(add[j], add[j + 1]));
+          }
+          if (tl + j < mine) y[int64_t(tl + j) * p.ld_y] = from_f32<T>(v.f[0]);
+          if (tl + j + 1 < mine) y[int64_t(tl + j + 1) * p.ld_y] = from_f32<T>(v.f[1]);
+        }
       }
     }
   }
@@ -793,32 +836,34 @@ struct NarrowPlan {
   int chunks, steps;        // steps of 128 codes in a stage, stages of a tile
   double cost;              // cycles
 };
-// The busiest SM's time: its tiles, their stages, and of a stage the longer of what it loads (from L2
-// about kLoad bytes a cycle; the weights at an SM's share of the DRAM rate), what it multiplies (8192
-// products a cycle with 128 rows, half with 64; an MMA takes its weight rows at 128 bytes a cycle, and kIssue
-// cycles to be issued) and what it takes to hand a stage over.
+// The busiest SM's time, from what was measured over rows 16 to 128 of 8 to 128 tokens: a stage takes the
+// longest of its bytes at 50 a cycle, its weights' at 23 (an SM's share of the DRAM rate), its MMAs (8192
+// products a cycle with 128 rows, half with 64) and their issue (37 cycles each, 260 to hand the stage
+// over); the last tile's epilogue, or the exchange of a cluster's sums, follows.
 NarrowPlan narrow_plan(int m, int n, int k, int G, int num_sms) {
-  constexpr double kLoad = 50, kDram = 23, kIssue = 22, kHandOver = 250, kSplitCost = 2000;
-  constexpr int kMostChunks = 4, kMostStage = 48 * 1024;
+  constexpr double kLoad = 50, kDram = 23, kIssue = 37, kHandOver = 260;
+  constexpr int kMostChunks = 4, kMostStage = 56 * 1024;
   const int tokens = std::min(kMostTokens, m <= 24 ? (m + 7) / 8 * 8 : (m + 15) / 16 * 16);
   const int token_tiles = (m + tokens - 1) / tokens, nk = (k + kStep - 1) / kStep;
   NarrowPlan best{};
   for (int rows = 8; rows <= 128; rows += 8) {
-    int chunks = 1;  // as many as leave a tile no part of a stage empty
-    if (k % kStep == 0)
-      for (int c = 2; c <= kMostChunks && c * (G * rows + tokens) * kStep <= kMostStage; ++c)
-        if (nk % c == 0) chunks = c;
-    const int steps = nk / chunks;
     const double load = std::max((G * rows + tokens) * kStep / kLoad, G * rows * kStep / kDram);
-    const double mma = 4.0 * G * std::max({tokens / 2.0, rows <= 64 ? 16.0 : 32.0, kIssue});
-    const double stage = std::max(chunks * std::max(load, mma), kHandOver);
-    for (int split = 1; split <= std::min(kMostSplit, steps); split *= 2) {
-      if (split > 1 && G * rows > 128) break;
-      const int64_t ctas = (int64_t(n) + rows - 1) / rows * token_tiles * split;
-      const double tiles = double((ctas + num_sms - 1) / num_sms);
-      const double cost = tiles * (((steps + split - 1) / split) * stage + (split > 1 ? kSplitCost : 0)) +
-                          (split > 1 ? 0 : tokens * 30.0);  // the last tile's epilogue
-      if (!best.rows || cost < best.cost) best = NarrowPlan{rows, tokens, split, chunks, steps, cost};
+    const double mma = 4.0 * G * tokens / 2.0;
+    const int64_t tiles = (int64_t(n) + rows - 1) / rows * token_tiles;
+    for (int chunks = 1; chunks <= kMostChunks; ++chunks) {
+      // stages of several steps want rows of whole steps, and leave no part of a stage empty
+      if (chunks > 1 && (k % kStep || nk % chunks || chunks * (G * rows + tokens) * kStep > kMostStage))
+        continue;
+      const int steps = nk / chunks;
+      const double stage = std::max(chunks * std::max(load, mma), chunks * 4 * G * kIssue + kHandOver);
+      for (int split = 1; split <= std::min(kMostSplit, steps); split *= 2) {
+        if (split > 1 && G * rows > 128) break;
+        const double turns = double((tiles * split + num_sms - 1) / num_sms);
+        const int part = (steps + split - 1) / split;
+        const double cost = split > 1 ? turns * (part * stage + 1000 + 43.0 * tokens)
+                                      : turns * (part * stage + 100) + 30.0 * tokens;
+        if (!best.rows || cost < best.cost) best = NarrowPlan{rows, tokens, split, chunks, steps, cost};
+      }
     }
   }
   return best;
@@ -842,9 +887,9 @@ cudaError_t launch_narrow(Q8Params p, const GemmQ8Args& a, const NarrowPlan& pla
   const int64_t tiles = int64_t(p.tiles_n) * ((int64_t(p.m) + plan.tokens - 1) / plan.tokens);
   if (tiles * plan.split > INT32_MAX) return cudaErrorInvalidValue;
   p.items = int32_t(tiles);
-  const int own = (plan.tokens + plan.split - 1) / plan.split;
+  const int own = split_tokens(plan.tokens, plan.split);
   const int stage = (G * plan.rows + plan.tokens) * kStep * plan.chunks;
-  const int sums = SPLIT ? (plan.split * own * G * plan.rows * 4 + 1023) / 1024 * 1024
+  const int sums = SPLIT ? (plan.split * G * plan.rows * (own + 4) * 4 + 1023) / 1024 * 1024
                          : kNarrowEpi * kMostTokens * 4;
   // behind the ring, what the last stage's MMA reads beyond its rows
   const int fixed = 2048 + sums + (plan.rows <= 64 ? 64 : 128) * kStep;
