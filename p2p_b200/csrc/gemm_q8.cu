@@ -59,9 +59,6 @@ __device__ __forceinline__ Pair act_mul2(Pair g, Pair u, int act) {
   return pair(act_mul(g.f[0], u.f[0], act), act_mul(g.f[1], u.f[1], act));
 }
 
-__device__ __forceinline__ float scaled(uint32_t acc, float xs, float ws) {
-  return __fmul_rn(__fmul_rn(float(int(acc)), xs), ws);
-}
 __device__ __forceinline__ Pair scaled2(uint32_t a, uint32_t b, Pair xs, Pair ws) {
   return mul2(mul2(pair(float(int(a)), float(int(b))), xs), ws);
 }
@@ -414,7 +411,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 // part and hands the sums, by token, to the CTA that finishes that token.
 constexpr int kNarrowEpi = 8;        // epilogue warps: two per TMEM lane quarter
 constexpr int kNarrowThreads = 32 * (2 + kNarrowEpi);  // TMA, MMA, epilogue
-constexpr int kMostTokens = 128;
+constexpr int kMostTokens = 128;     // of a tile
+constexpr int kMostNarrow = 512;     // of a call
 constexpr int kMostSplit = 8;
 constexpr int kMostStages = 24;
 constexpr int kNarrowSmem = 226 * 1024;
@@ -834,39 +832,80 @@ cudaError_t launch_wide(Q8Params p, const GemmQ8Args& a, int num_sms, cudaStream
 struct NarrowPlan {
   int rows, tokens, split;  // channels and tokens of a tile, CTAs of its k
   int chunks, steps;        // steps of 128 codes in a stage, stages of a tile
-  double cost;              // cycles
+  float cost;               // cycles
 };
+// Clusters of 2, 4 and 8 CTAs, one CTA an SM, that run at once (148 SMs in groups that hold no multiple of
+// 8): 8 bits each.
+cudaError_t cluster_room(int* room) {
+  static PerDeviceOnce setup;
+  return per_device_once(setup, [](int& packed) {
+    const void* fn = reinterpret_cast<const void*>(&narrow_kernel<__half, false, true>);
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kNarrowSmem);
+    for (int i = 0; i < 3 && e == cudaSuccess; ++i) {
+      cudaLaunchAttribute at{};
+      at.id = cudaLaunchAttributeClusterDimension;
+      at.val.clusterDim.x = 2u << i;
+      at.val.clusterDim.y = 1;
+      at.val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(2u << i);
+      cfg.blockDim = dim3(kNarrowThreads);
+      cfg.dynamicSmemBytes = kNarrowSmem;
+      cfg.attrs = &at;
+      cfg.numAttrs = 1;
+      int n = 0;
+      e = cudaOccupancyMaxActiveClusters(&n, fn, &cfg);
+      packed |= std::min(std::max(n, 1), 255) << (8 * i);
+    }
+    return e;
+  }, room);
+}
 // The busiest SM's time, from what was measured over rows 16 to 128 of 8 to 128 tokens: a stage takes the
-// longest of its bytes at 50 a cycle, its weights' at 23 (an SM's share of the DRAM rate), its MMAs (8192
-// products a cycle with 128 rows, half with 64) and their issue (37 cycles each, 260 to hand the stage
-// over); the last tile's epilogue, or the exchange of a cluster's sums, follows.
-NarrowPlan narrow_plan(int m, int n, int k, int G, int num_sms) {
-  constexpr double kLoad = 50, kDram = 23, kIssue = 37, kHandOver = 260;
-  constexpr int kMostChunks = 4, kMostStage = 56 * 1024;
+// longest of its bytes at 50 a cycle, its weights' at an SM's share of the DRAM rate (23 where all SMs
+// load), and its MMAs (8192 products a cycle with 128 rows, half with 64), and 150 more; or the MMAs'
+// issue, 37 cycles each and 260 to hand the stage over.  The last tile's epilogue, or the exchange of a
+// cluster's sums, follows.
+NarrowPlan narrow_plan(int m, int n, int k, int G, int num_sms, int room) {
+  constexpr float kLoad = 50, kDram = 23, kWait = 150, kIssue = 37, kHandOver = 260;
+  constexpr int kMostChunks = 4, kMostStage = 64 * 1024;
   const int tokens = std::min(kMostTokens, m <= 24 ? (m + 7) / 8 * 8 : (m + 15) / 16 * 16);
   const int token_tiles = (m + tokens - 1) / tokens, nk = (k + kStep - 1) / kStep;
+  const float mma = 4.f * G * tokens / 2.f, sms = float(num_sms);
   NarrowPlan best{};
   for (int rows = 8; rows <= 128; rows += 8) {
-    const double load = std::max((G * rows + tokens) * kStep / kLoad, G * rows * kStep / kDram);
-    const double mma = 4.0 * G * tokens / 2.0;
     const int64_t tiles = (int64_t(n) + rows - 1) / rows * token_tiles;
-    for (int chunks = 1; chunks <= kMostChunks; ++chunks) {
-      // stages of several steps want rows of whole steps, and leave no part of a stage empty
-      if (chunks > 1 && (k % kStep || nk % chunks || chunks * (G * rows + tokens) * kStep > kMostStage))
-        continue;
-      const int steps = nk / chunks;
-      const double stage = std::max(chunks * std::max(load, mma), chunks * 4 * G * kIssue + kHandOver);
-      for (int split = 1; split <= std::min(kMostSplit, steps); split *= 2) {
-        if (split > 1 && G * rows > 128) break;
-        const double turns = double((tiles * split + num_sms - 1) / num_sms);
-        const int part = (steps + split - 1) / split;
-        const double cost = split > 1 ? turns * (part * stage + 1000 + 43.0 * tokens)
-                                      : turns * (part * stage + 100) + 30.0 * tokens;
+    const float all = (G * rows + tokens) * kStep / kLoad, weights = float(G * rows * kStep);
+    for (int split = 1, i = 0; split <= std::min(kMostSplit, nk); split *= 2, ++i) {
+      if (split > 1 && G * rows > 128) break;
+      const int slots = split > 1 ? (room >> (8 * (i - 1))) & 255 : num_sms;
+      const float busy = float(std::min<int64_t>(tiles, slots) * split) / sms;
+      const float bytes = std::max({all, weights / std::min(kLoad, kDram / busy), mma});
+      const float turns = float((tiles + slots - 1) / slots);
+      const float fixed = split > 1 ? turns * (1300 + 0.52f * G * rows * tokens + 12 * tokens)
+                                    : turns * 100 + 30.f * tokens;
+      for (int chunks = 1; chunks <= kMostChunks; ++chunks) {
+        // stages of several steps want rows of whole steps, and leave no part of a stage empty
+        if (chunks > 1 &&
+            (k % kStep || nk % chunks || chunks * (G * rows + tokens) * kStep > kMostStage))
+          continue;
+        const int steps = nk / chunks;
+        if (split > steps) break;
+        const float stage = std::max(chunks * bytes + kWait, chunks * 4 * G * kIssue + kHandOver);
+        const float cost = turns * ((steps + split - 1) / split) * stage + fixed;
         if (!best.rows || cost < best.cost) best = NarrowPlan{rows, tokens, split, chunks, steps, cost};
       }
     }
   }
   return best;
+}
+// The same of wide_kernel: a step of a whole tile takes 512 cycles, of half a tile 305; pairs of CTAs start
+// later.
+double wide_cost(int m, int n, int k, int G, int num_sms) {
+  const int cols = kWidth / G, pairs = std::max(1, num_sms / 2), nk = (k + kStep - 1) / kStep;
+  const int64_t tiles = (int64_t(n) + cols - 1) / cols * ((m + 2 * kRows - 1) / (2 * kRows));
+  const int64_t rest = tiles % pairs;
+  const double whole = double(tiles / pairs + (2 * rest > pairs ? 1 : 0));
+  return 4000 + nk * (512 * whole + (rest && 2 * rest <= pairs ? 305 : 0));
 }
 
 template <class T, bool GATE, bool SPLIT>
@@ -918,8 +957,13 @@ bool on16(const void* p, int64_t pitch_bytes) {
 
 template <class T, bool GATE>
 cudaError_t launch_q8(const Q8Params& p, const GemmQ8Args& a, int num_sms, cudaStream_t s) {
-  if (p.m > kMostTokens) return launch_wide<T, GATE>(p, a, num_sms, s);
-  const NarrowPlan plan = narrow_plan(p.m, p.n, p.k, GATE ? 2 : 1, num_sms);
+  constexpr int G = GATE ? 2 : 1;
+  if (p.m > kMostNarrow) return launch_wide<T, GATE>(p, a, num_sms, s);
+  int room = 0;
+  const cudaError_t e = cluster_room(&room);
+  if (e != cudaSuccess) return e;
+  const NarrowPlan plan = narrow_plan(p.m, p.n, p.k, G, num_sms, room);
+  if (p.m > kMostTokens && plan.cost > wide_cost(p.m, p.n, p.k, G, num_sms)) return launch_wide<T, GATE>(p, a, num_sms, s);
   return plan.split > 1 ? launch_narrow<T, GATE, true>(p, a, plan, num_sms, s)
                         : launch_narrow<T, GATE, false>(p, a, plan, num_sms, s);
 }
