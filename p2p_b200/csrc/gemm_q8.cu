@@ -156,40 +156,62 @@ __device__ __forceinline__ void store_block(const Q8Params& p, const Pair (&v)[1
   if (c < p.n) {
     T* d = static_cast<T*>(p.y) + int64_t(m_base) * p.ld_y + c;
     const float* t = reinterpret_cast<const float*>(turn) + lane;
-    if (p.res) {
-      const T* r = static_cast<const T*>(p.res) + int64_t(m_base) * p.ld_res + c;
-#pragma unroll 8
-      for (int i = 0; i < rows; ++i, d += p.ld_y, r += p.ld_res, t += kPitch<float>)
-        *d = from_f32<T>(__fadd_rn(*t, to_f32(*r)));
-    } else {
-#pragma unroll 8
-      for (int i = 0; i < rows; ++i, d += p.ld_y, t += kPitch<float>) *d = from_f32<T>(*t);
+    const T* r = p.res ? static_cast<const T*>(p.res) + int64_t(m_base) * p.ld_res + c : nullptr;
+    for (int i = 0; i < rows; i += 8, t += 8 * kPitch<float>) {
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = t[j * kPitch<float>];
+      if (r) {
+        float add[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j, r += p.ld_res) add[j] = i + j < rows ? to_f32(*r) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = __fadd_rn(y[j], add[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j, d += p.ld_y)
+        if (i + j < rows) *d = from_f32<T>(y[j]);
     }
   }
   __syncwarp();
+}
+
+// What an epilogue warp multiplies an item's sums with: its token's scale, and by lane the scales of its
+// blocks of columns and their biases or up scales.  Fetched an item ahead.
+struct Ahead {
+  float xs, ws[4], second[4];
+};
+template <bool GATE>
+__device__ __forceinline__ Ahead look_ahead(const Q8Params& p, const Item& it, int m0, int warp,
+                                            int lane) {
+  Ahead a;
+  const int m = m0 + (warp & 3) * 32 + lane, half = warp >> 2;
+  const int blocks = (GATE ? it.bn / 2 : it.bn) / 32;
+  a.xs = m < p.m ? p.xs[m] : 0.f;
+#pragma unroll
+  for (int i = 0; i < (GATE ? 2 : 4); ++i) {
+    const int b = half + 2 * i, c = it.n0 + b * 32 + lane;
+    const bool there = b < blocks && c < p.n;
+    a.ws[i] = there ? p.ws[c] : 0.f;
+    if constexpr (GATE) a.second[i] = there ? p.us[c] : 0.f;
+    else a.second[i] = there && p.bias ? p.bias[c] : 0.f;
+  }
+  return a;
 }
 
 // The epilogue of one item by epilogue warp `warp`: TMEM lane quarter warp & 3, every other block of 32
 // columns.
 template <class T, bool GATE, class Release>
 __device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem& s, uint32_t acc,
-                                              const Item& it, int m0, int warp, int lane,
-                                              Release release) {
+                                              const Item& it, int m0, const Ahead& ahead, int warp,
+                                              int lane, Release release) {
   const int quarter = warp & 3, half = warp >> 2;
   const int cols = GATE ? it.bn / 2 : it.bn, blocks = cols / 32;
   const uint32_t at = acc + (uint32_t(quarter * 32) << 16);
   const int m_base = m0 + quarter * 32;
-  float* ws = s.col[warp][0];
-  float* second = s.col[warp][1];
-  const float xs = m_base + lane < p.m ? p.xs[m_base + lane] : 0.f;
-  for (int b = half, i = lane; b < blocks; b += 2, i += 32) {
-    const int c = it.n0 + b * 32 + lane;
-    ws[i] = c < p.n ? p.ws[c] : 0.f;
-    if constexpr (GATE) second[i] = c < p.n ? p.us[c] : 0.f;
-    else if (p.bias) second[i] = c < p.n ? p.bias[c] : 0.f;
-  }
-  __syncwarp();
-  const Pair xs2 = pair(xs, xs);
+  const float* ws = s.col[warp][0];
+  const float* second = s.col[warp][1];
+  const Pair xs2 = pair(ahead.xs, ahead.xs);
   const int m = m_base + lane;
   for (int b = half, i = 0; b < blocks; b += 2, i += 32) {
     const int n = it.n0 + b * 32;
@@ -206,10 +228,16 @@ __device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem& s, ui
 #pragma unroll
       for (int j = 0; j < (GATE ? 1 : kPieces); ++j) res[j].u = m < p.m ? r[j] : make_uint4(0, 0, 0, 0);
     }
-    uint32_t r[32];
+    uint32_t r[32], ru[GATE ? 32 : 1];
     Pair v[16];
     tmem_ld32(at + b * 32, r);
+    if constexpr (GATE) tmem_ld32(at + cols + b * 32, ru);
     tmem_ld_wait();
+    if (b + 2 >= blocks) {  // everything of this warp is in registers
+      tc_fence_before();
+      __syncwarp();
+      release();
+    }
     const float4* w4 = reinterpret_cast<const float4*>(ws + i);
     const float4* s4 = reinterpret_cast<const float4*>(second + i);
 #pragma unroll
@@ -219,13 +247,11 @@ __device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem& s, ui
       v[2 * j + 1] = scaled2(r[4 * j + 2], r[4 * j + 3], xs2, pair(w.z, w.w));
     }
     if constexpr (GATE) {
-      tmem_ld32(at + cols + b * 32, r);
-      tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float4 w = s4[j];
-        const Pair u0 = scaled2(r[4 * j], r[4 * j + 1], xs2, pair(w.x, w.y));
-        const Pair u1 = scaled2(r[4 * j + 2], r[4 * j + 3], xs2, pair(w.z, w.w));
+        const Pair u0 = scaled2(ru[4 * j], ru[4 * j + 1], xs2, pair(w.x, w.y));
+        const Pair u1 = scaled2(ru[4 * j + 2], ru[4 * j + 3], xs2, pair(w.z, w.w));
         v[2 * j] = act_mul2(v[2 * j], u0, p.act);
         v[2 * j + 1] = act_mul2(v[2 * j + 1], u1, p.act);
       }
@@ -236,11 +262,6 @@ __device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem& s, ui
         v[2 * j] = add2(v[2 * j], pair(w.x, w.y));
         v[2 * j + 1] = add2(v[2 * j + 1], pair(w.z, w.w));
       }
-    }
-    if (b + 2 >= blocks) {  // everything of this warp is in registers
-      tc_fence_before();
-      __syncwarp();
-      release();
     }
     if (add) {
 #pragma unroll
@@ -379,16 +400,33 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
   } else {
     int n = 0;
+    Ahead ahead{};
+    if (pair < p.items) {
+      const Item it = item_of<GATE>(p, pair);
+      ahead = look_ahead<GATE>(p, it, it.m0 + int(rank) * kRows, warp, lane);
+    }
     for (int i = pair; i < p.items; i += pairs, ++n) {
       const int b = n & 1, u = n >> 1;
+      const Item it = item_of<GATE>(p, i);
+      const Ahead now = ahead;
       __syncwarp();
+#pragma unroll
+      for (int j = 0; j < (GATE ? 2 : 4); ++j) {
+        s.col[warp][0][32 * j + lane] = now.ws[j];
+        s.col[warp][1][32 * j + lane] = now.second[j];
+      }
+      __syncwarp();
+      if (i + pairs < p.items) {
+        const Item next = item_of<GATE>(p, i + pairs);
+        ahead = look_ahead<GATE>(p, next, next.m0 + int(rank) * kRows, warp, lane);
+      }
       if (!gemm_wait_all(s.abort_flag, &s.acc_full[b], u & 1, p.err)) break;
       tc_fence_after();
       const uint32_t empty0 = cluster_map(smem_u32(&s.acc_empty[b]), 0);
-      const Item it = item_of<GATE>(p, i);
-      wide_epilogue<T, GATE>(p, s, tmem + uint32_t(b * kWidth), it, it.m0 + int(rank) * kRows, warp,
-                             lane, [&] {
-                               if (lane == 0) mbar_arrive_cluster(empty0);
+      // TMEM loads are ordered by the fence in front of the arrival; nothing else is guarded by it
+      wide_epilogue<T, GATE>(p, s, tmem + uint32_t(b * kWidth), it, it.m0 + int(rank) * kRows, now,
+                             warp, lane, [&] {
+                               if (lane == 0) mbar_arrive_cluster_relaxed(empty0);
                              });
     }
   }

@@ -160,6 +160,12 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
                : "memory");
 }
+// The same without ordering this thread's memory operations in front of it (a release at cluster scope
+// waits for its stores to global memory): where what the barrier guards is ordered otherwise.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+               : "memory");
+}
 // A TMA tile load into this CTA's shared memory whose completion is counted on an mbarrier of
 // either CTA of the pair (its shared::cluster address).  No multicast.
 __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map,
