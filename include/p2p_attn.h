@@ -425,11 +425,12 @@ p2p_status p2p_logits_pick(p2p_ctx* ctx, const p2p_logits* args, void* stream);
  * two rows is neither read nor written); scale 4-byte aligned.  The entry points below refuse (but
  * for what each says) outputs that overlap inputs or each other.  They use no workspace. */
 #define P2P_MAX_Q8_COLS 65536
+#define P2P_MAX_Q8_ROWS (1 << 30)
 typedef struct p2p_q8_rows {
   void* q;       /* int8 [rows][ld] */
   float* scale;  /* [rows] */
   int64_t ld;
-  int32_t rows;
+  int32_t rows;  /* at most P2P_MAX_Q8_ROWS */
   int32_t cols;  /* at most P2P_MAX_Q8_COLS */
 } p2p_q8_rows;
 

@@ -39,6 +39,7 @@ struct Q8Params {
   void* y;
   int64_t ld_res, ld_y;
   int32_t* err;
+  int32_t wait_deficit;    // bytes more than will arrive that the first stage waits for (a test)
   int32_t tiles_n, items;  // tiles along n; work items in all
   // wide_kernel
   int32_t whole;  // tiles of full width
@@ -324,7 +325,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           break;
         if (elect_one()) {
           const uint32_t full0 = cluster_map(smem_u32(&s.full[st]), 0);
-          if (rank == 0) mbar_arrive_expect_tx(&s.full[st], 2 * (kTileBytes + half * kStep));
+          if (rank == 0)
+            mbar_arrive_expect_tx(&s.full[st], 2 * (kTileBytes + half * kStep) +
+                                                   (st + round == 0 ? p.wait_deficit : 0));
           tma_load_3d_pair(s.a[st], &tm_x, kt * kStep, m0, 0, full0);
           tma_load_3d_pair(s.b[st], tm_b, kt * kStep, n0, 0, full0);
           if (half > kBoxRows)
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 constexpr int kNarrowEpi = 8;        // epilogue warps: two per TMEM lane quarter
 constexpr int kNarrowThreads = 32 * (2 + kNarrowEpi);  // TMA, MMA, epilogue
 constexpr int kMostTokens = 128;     // of a tile
-constexpr int kMostNarrow = 512;     // of a call
+constexpr int kMostNarrow = 2048;    // of a call
 constexpr int kMostSplit = 8;
 constexpr int kMostStages = 24;
 constexpr int kNarrowSmem = 226 * 1024;
@@ -560,7 +563,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
         if (elect_one()) {
           uint8_t* a = ring + st * stage_bytes;
           const int kx = p.deep ? 0 : kt * kStep, kz = p.deep ? kt * p.chunks : 0;
-          mbar_arrive_expect_tx(&s.full[st], stage_bytes);
+          mbar_arrive_expect_tx(&s.full[st], stage_bytes + (st + round == 0 ? p.wait_deficit : 0));
           tma_load_3d(a, &tm_w, kx, n0, kz, &s.full[st]);
           if constexpr (GATE) tma_load_3d(a + w_bytes, &tm_u, kx, n0, kz, &s.full[st]);
           tma_load_3d(a + G * w_bytes, &tm_x, kx, m0, kz, &s.full[st]);
@@ -1023,6 +1026,7 @@ cudaError_t launch_gemm_q8(const GemmQ8Args& a, int dtype, int num_sms, cudaStre
   p.ld_res = a.ld_res;
   p.ld_y = a.ld_y;
   p.err = a.err;
+  p.wait_deficit = a.wait_deficit;
   const int64_t es = dtype == 0 ? 2 : 4;
   p.wide = on16(a.y, a.ld_y * es) && (!a.res || on16(a.res, a.ld_res * es));
   if (a.up.q) return launch_q8<__half, true>(p, a, num_sms, s);

@@ -413,6 +413,7 @@ struct GemmQ8Args {
   void* y;
   int64_t ld_y;
   int32_t* err;
+  int32_t wait_deficit;
 };
 cudaError_t launch_gemm_q8(const GemmQ8Args& a, int dtype, int num_sms, cudaStream_t s);
 

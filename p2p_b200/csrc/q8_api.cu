@@ -85,9 +85,9 @@ p2p_status check_dtype(p2p_ctx* ctx, int32_t dtype, const char* who) {
 
 p2p_status check_q8(p2p_ctx* ctx, const p2p_q8_rows* r, const char* name, const char* who) {
   if (!r) return fail(ctx, P2P_ERR_INVALID_ARG, "%s: %s is NULL", who, name);
-  if (r->rows < 0 || r->cols < 1 || r->cols > P2P_MAX_Q8_COLS)
-    return fail(ctx, P2P_ERR_INVALID_ARG, "%s: %s has %d rows of %d codes (1..%d)", who, name, r->rows,
-                r->cols, P2P_MAX_Q8_COLS);
+  if (r->rows < 0 || r->rows > P2P_MAX_Q8_ROWS || r->cols < 1 || r->cols > P2P_MAX_Q8_COLS)
+    return fail(ctx, P2P_ERR_INVALID_ARG, "%s: %s has %d rows (0..%d) of %d codes (1..%d)", who, name,
+                r->rows, P2P_MAX_Q8_ROWS, r->cols, P2P_MAX_Q8_COLS);
   if (r->rows == 0) return P2P_OK;
   if (!r->q || !r->scale)
     return fail(ctx, P2P_ERR_INVALID_ARG, "%s: %s has no codes or no scales", who, name);
@@ -152,7 +152,7 @@ p2p_status p2p_read_rows_q8(p2p_ctx* ctx, const p2p_read_rows* args, void* strea
   p2p_status st;
   if ((st = check_dtype(ctx, dtype, who)) != P2P_OK) return st;
   if ((st = check_q8(ctx, src, "src", who)) != P2P_OK) return st;
-  if (rows < 0 || (!index && rows > src->rows) || !aligned(index, 4))
+  if (rows < 0 || rows > P2P_MAX_Q8_ROWS || (!index && rows > src->rows) || !aligned(index, 4))
     return fail(ctx, P2P_ERR_INVALID_ARG, "%s: %lld rows of %d, index %p", who, (long long)rows,
                 src->rows, (const void*)index);
   if (rows == 0) return P2P_OK;
@@ -177,9 +177,9 @@ p2p_status p2p_add_norm_q8(p2p_ctx* ctx, const p2p_add_norm* args, void* stream)
   const int32_t rows = g.out.rows, cols = g.out.cols;
   if (g.out.q) {
     if ((st = check_q8(ctx, &g.out, "out", who)) != P2P_OK) return st;
-  } else if (rows < 0 || cols < 1 || cols > P2P_MAX_Q8_COLS) {
-    return fail(ctx, P2P_ERR_INVALID_ARG, "%s: %d rows of %d values (1..%d)", who, rows, cols,
-                P2P_MAX_Q8_COLS);
+  } else if (rows < 0 || rows > P2P_MAX_Q8_ROWS || cols < 1 || cols > P2P_MAX_Q8_COLS) {
+    return fail(ctx, P2P_ERR_INVALID_ARG, "%s: %d rows (0..%d) of %d values (1..%d)", who, rows,
+                P2P_MAX_Q8_ROWS, cols, P2P_MAX_Q8_COLS);
   }
   if (rows == 0) return P2P_OK;
   if (!g.sum && !g.y && !g.out.q)
@@ -276,6 +276,7 @@ p2p_status p2p_gemm_q8(p2p_ctx* ctx, const p2p_product* args, void* stream) {
   a.y = y;
   a.ld_y = ld_y;
   a.err = p2p::ctx_dev_err(ctx);
+  a.wait_deficit = p2p::debug_wait_deficit();
   OnDevice g(p2p::ctx_device(ctx));
   return launched(ctx, p2p::launch_gemm_q8(a, dtype, p2p::ctx_num_sms(ctx),
                                            static_cast<cudaStream_t>(stream)),
@@ -314,6 +315,7 @@ p2p_status p2p_gate_q8(p2p_ctx* ctx, const p2p_gated* args, void* stream) {
   a.y = h;
   a.ld_y = ld_h;
   a.err = p2p::ctx_dev_err(ctx);
+  a.wait_deficit = p2p::debug_wait_deficit();
   OnDevice g(p2p::ctx_device(ctx));
   return launched(ctx, p2p::launch_gemm_q8(a, P2P_F16, p2p::ctx_num_sms(ctx),
                                            static_cast<cudaStream_t>(stream)),

@@ -3,11 +3,17 @@
 // src/scripts/lfm-engine/kernels.js:146-182), and read back as values (the embedding lookup).
 //
 // All three move bytes: a row is read once, kept in registers (as it lies in memory, 4 words for 16
-// bytes), reduced and written once.  A code is 127 v / a, a = max |v|, rounded to even.  It is taken as
-// v * (127 / a); a product so near a half that its two roundings could have moved it is divided anew
-// (half of the largest value is exactly 63.5, and rows of f16 hold such values), so that ties of f16
-// rows are ties.  For the norm, v = (s * w) * rstd and rounding is monotone, so max |v| = max |s * w| *
-// rstd exactly: the sum of squares and the maximum go through one reduction.
+// bytes), reduced and written once.  A code is 127 v / a, a = max |v|, rounded to even, taken as
+// v * (127 / a) + 1.5 * 2^23 in one operation.  Of f16 rows ties are exact: with 127 / a rounded up, half
+// of the largest value (63.5 exactly) goes to 64, no other quotient lies so near a half that the factor's
+// last place could move it ((c + 1/2) 2^-18 at least, against (c + 1/2) 2^-23), and rows whose a has a
+// multiple of 127 for its 11 bits, which alone give other ties, are divided value by value.  For the norm,
+// v = (s * w) * rstd and rounding is monotone, so max |v| = max |s * w| * rstd exactly: the sum of squares
+// and the maximum go through one reduction.
+//   A row is in the hands of as few warps as hold it, 4 pieces of 16 bytes a lane: what a warp does once
+// for a row costs as much as 20 to 40 of its values (65536 rows of 1024 f16 values in 36 us by warps, 68
+// by pairs of warps, 131 by eight; blocks that walk rows, with or without the next row on its way, were
+// slower: 39 to 43).
 #include <algorithm>
 
 #include "common.cuh"
@@ -16,8 +22,10 @@
 namespace p2p {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;         // of a block whose warps take a row each
 constexpr int kWarps = kThreads / 32;
+constexpr int kMostWarps = 16;        // of a row
+constexpr int kMostPieces = 4;        // of a lane
 constexpr float kTiny = 0x1p-100f;  // a row below it counts as zeros (127 / a stays finite)
 
 // max(|a|, |b|, |c|), NaN if one of them is.
@@ -151,6 +159,7 @@ __device__ __forceinline__ Pair wide2(__half2 h) {
 // What a row's values are multiplied with, and its scale.  inv 0: all codes are 0.
 struct RowScale {
   float rstd, top, inv, scale;
+  bool divide;
 };
 
 // Adding 1.5 * 2^23 rounds to a whole number, whose low byte is the code.
@@ -158,18 +167,11 @@ template <int V>
 __device__ __forceinline__ void store_codes(int8_t* row, const Columns<V>& c, int piece,
                                             const Pair (&v)[V / 2], const RowScale& sc) {
   constexpr float kRound = 12582912.f;
-  const Pair inv = pair(sc.inv, sc.inv), up = pair(kRound, kRound), down = pair(-kRound, -kRound);
-  const Pair minus = pair(-1.f, -1.f);
+  const Pair inv = pair(sc.inv, sc.inv), up = pair(kRound, kRound);
   Pair t[V / 2];
-  float far = 0.f;
 #pragma unroll
-  for (int i = 0; i < V / 2; ++i) {
-    const Pair q = mul2(v[i], inv);
-    t[i] = add2(q, up);
-    const Pair d = mad2(add2(t[i], down), minus, q);  // q less its code
-    far = max_abs3(far, d.f[0], d.f[1]);
-  }
-  if (far > 0.49996f) {  // 127 * 2^-22 from a half
+  for (int i = 0; i < V / 2; ++i) t[i] = mad2(v[i], inv, up);
+  if (sc.divide) {
 #pragma unroll
     for (int i = 0; i < V / 2; ++i)
 #pragma unroll
@@ -201,25 +203,31 @@ struct RowSums {
 };
 
 // The sums of the threads of a row: a warp, or the `warps` of the block.
+template <bool NORM>
 __device__ __forceinline__ RowSums row_reduce(RowSums r, int warps, int warp, int lane,
                                               RowSums* part) {
   // as whole numbers, infinities and NaN come out largest
   r.top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(r.top)));
+  if constexpr (NORM) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) r.ss += __shfl_xor_sync(0xffffffffu, r.ss, o);
+    for (int o = 16; o; o >>= 1) r.ss += __shfl_xor_sync(0xffffffffu, r.ss, o);
+  }
   if (warps == 1) return r;
   if (lane == 0) part[warp] = r;
   __syncthreads();
-  r = part[0];
-  for (int i = 1; i < warps; ++i) {
-    r.top = max_abs3(r.top, part[i].top, 0.f);
-    r.ss += part[i].ss;
+  r = lane < warps ? part[lane] : RowSums{0.f, 0.f};
+  r.top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(r.top)));
+  if constexpr (NORM) {
+#pragma unroll
+    for (int o = kMostWarps / 2; o; o >>= 1) r.ss += __shfl_xor_sync(0xffffffffu, r.ss, o);
+    r.ss = __shfl_sync(0xffffffffu, r.ss, 0);
   }
   return r;
 }
 
-template <bool NORM>
+template <bool NORM, bool F16>
 __device__ __forceinline__ RowScale row_scale(RowSums r, int cols, float eps) {
+  constexpr bool kTies = F16 && !NORM;
   RowScale s;
   const float nan = __uint_as_float(0x7fffffffu);
   s.rstd = 1.f;
@@ -231,12 +239,13 @@ __device__ __forceinline__ RowScale row_scale(RowSums r, int cols, float eps) {
   if (a < kTiny) {
     s.inv = s.scale = 0.f;
   } else if (a <= 3.4028235e38f) {
-    s.inv = __fdiv_rn(127.f, a);
+    s.inv = kTies ? __fdiv_ru(127.f, a) : __fdiv_rn(127.f, a);
     s.scale = __fdiv_rn(a, 127.f);
   } else {
     s.inv = 0.f;
     s.scale = nan;
   }
+  s.divide = kTies && (((__float_as_uint(a) >> 13) & 0x3ff) | 0x400) % 127 == 0;
   return s;
 }
 
@@ -259,16 +268,22 @@ __device__ __forceinline__ void sum_piece(RowSums& sums, Pair& ss, const Piece<T
                                           const RowsQ8Args& a,
                                           const Columns<Piece<T>::V>& c, int piece) {
   constexpr int V = Piece<T>::V;
-  __half2 w[V / 2];
-  if constexpr (NORM) load_weights<WIDE, V>(w, a.w, c, piece);
+  if constexpr (!NORM && sizeof(T) == 2) {
+    const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(x.h[0]), __habs2(x.h[1])),
+                                  __hmax2_nan(__habs2(x.h[2]), __habs2(x.h[3])));
+    sums.top = max_abs3(sums.top, __low2float(m), __high2float(m));
+  } else {
+    __half2 w[V / 2];
+    if constexpr (NORM) load_weights<WIDE, V>(w, a.w, c, piece);
 #pragma unroll
-  for (int j = 0; j < V / 2; ++j) {
-    Pair v = x.get(j);
-    if constexpr (NORM) {
-      ss = mad2(v, v, ss);
-      v = mul2(v, wide2(w[j]));
+    for (int j = 0; j < V / 2; ++j) {
+      Pair v = x.get(j);
+      if constexpr (NORM) {
+        ss = mad2(v, v, ss);
+        v = mul2(v, wide2(w[j]));
+      }
+      sums.top = max_abs3(sums.top, v.f[0], v.f[1]);
     }
-    sums.top = max_abs3(sums.top, v.f[0], v.f[1]);
   }
 }
 // A piece of what the call stores behind the reduction.
@@ -307,10 +322,10 @@ __device__ __forceinline__ void keep_words(Piece<T>& x) {
 // A row in the registers of a warp (warps 1: a row a warp) or of a block of `warps` warps, NP pieces a
 // lane.
 template <class T, int NP, bool NORM, bool WIDE>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(32 * kMostWarps)
     rows_kernel(const __grid_constant__ RowsQ8Args a, int warps) {
-  __shared__ RowSums part[kWarps];
-  __shared__ uint4 turns[WIDE ? 1 : kWarps][32];
+  __shared__ RowSums part[kMostWarps];
+  __shared__ uint4 turns[WIDE ? 1 : kMostWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = warps == 1 ? int64_t(blockIdx.x) * kWarps + warp : blockIdx.x;
   const int part_of = warps == 1 ? 0 : warp;
@@ -347,10 +362,10 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (int i = 0; i < NP; ++i) sum_piece<NORM, WIDE>(sums, ss, v[i], a, c, i);
   sums.ss = ss.f[0] + ss.f[1];
-  sums = row_reduce(sums, warps, warp, lane, part);
+  sums = row_reduce<NORM>(sums, warps, warp, lane, part);
 #pragma unroll
   for (int i = 0; i < NP; ++i) keep_words(v[i]);
-  const RowScale sc = row_scale<NORM>(sums, a.out.cols, a.eps);
+  const RowScale sc = row_scale<NORM, sizeof(T) == 2>(sums, a.out.cols, a.eps);
 #pragma unroll
   for (int i = 0; i < NP; ++i) finish_piece<NORM, WIDE>(v[i], sc, a, row, c, i, turn);
   if (a.out.q && part_of == 0 && lane == 0) a.out.scale[row] = sc.scale;
@@ -387,8 +402,8 @@ __global__ void __launch_bounds__(kThreads)
     sum_piece<NORM, WIDE>(sums, ss, v, a, c, i);
   }
   sums.ss = ss.f[0] + ss.f[1];
-  sums = row_reduce(sums, kWarps, warp, lane, part);
-  const RowScale sc = row_scale<NORM>(sums, c.cols, a.eps);
+  sums = row_reduce<NORM>(sums, kWarps, warp, lane, part);
+  const RowScale sc = row_scale<NORM, sizeof(T) == 2>(sums, c.cols, a.eps);
   for (int i = 0; i < pieces; ++i) {
     Piece<T> v, u;
     load_piece<WIDE>(v, s ? s : x, c, i);
@@ -402,53 +417,67 @@ __global__ void __launch_bounds__(kThreads)
   if (a.out.q && threadIdx.x == 0) a.out.scale[row] = sc.scale;
 }
 
-// Codes back to values: a warp takes up to kReadPieces pieces a lane of one row.
+// Codes back to values: a warp takes kReadPieces pieces a lane, of a segment of one row, or (SHORT: rows of
+// that many pieces, 1 or 2) of several rows (a row a warp: 33933 rows of 320 in 19.8 us, 13.2 so).
 constexpr int kReadPieces = 4;
-template <class T, bool WIDE>
+template <class T, bool WIDE, int SHORT>
 __global__ void __launch_bounds__(kThreads)
     read_kernel(const __grid_constant__ ReadQ8Args a, int segments) {
-  constexpr int V = Piece<T>::V;
+  constexpr int V = Piece<T>::V, kRows = SHORT ? kReadPieces / SHORT : 1;
   __shared__ uint4 turns[WIDE ? 1 : kWarps][32];
   const int lane = threadIdx.x & 31;
   const int64_t unit = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   grid_dependency_wait();
   launch_dependents();
-  const int64_t i = unit / segments;
-  if (i >= a.rows) return;
-  const int col0 = int(unit - i * segments) * (kReadPieces * 32 * V);
-  const Columns<V> c{lane, 32, a.src.cols - col0};
-  const int64_t row = a.index ? a.index[i] : i;
-  const bool inside = row >= 0 && row < a.src.rows;
-  if (!inside && row != -1 && lane == 0) atomicOr(a.err, kErrIndex);
-  const float scale = inside ? a.src.scale[row] : 0.f;
-  const int8_t* q = a.src.q + (inside ? row : 0) * a.src.ld + col0;
-  T* out = static_cast<T*>(a.out) + i * a.ld_out + col0;
+  const int64_t first = SHORT ? unit * kRows : unit / segments;
+  if (first >= a.rows) return;
+  const int piece0 = SHORT ? 0 : int(unit - first * segments) * kReadPieces;
+  const Columns<V> c{lane, 32, a.src.cols};
+  float scale[kRows];
+  const int8_t* q[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int64_t i = first + r;
+    const int64_t row = i >= a.rows ? -1 : a.index ? a.index[i] : i;
+    const bool inside = row >= 0 && row < a.src.rows;
+    if (!inside && row != -1 && lane == 0) atomicOr(a.err, kErrIndex);
+    scale[r] = inside ? a.src.scale[row] : 0.f;
+    q[r] = inside ? a.src.q + row * a.src.ld : nullptr;
+  }
   union {
     uint32_t u[V / 4];
     int8_t e[V];
   } w[kReadPieces];
 #pragma unroll
   for (int p = 0; p < kReadPieces; ++p) {
-    if (c.whole(p)) {
+    const int piece = SHORT ? p % (SHORT ? SHORT : 1) : piece0 + p;
+    const int8_t* from = q[SHORT ? p / (SHORT ? SHORT : 1) : 0];
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) w[p].u[j] = 0;
+    if (!from) continue;
+    if (c.whole(piece)) {
       if constexpr (V == 8) {
-        const uint2 u = *reinterpret_cast<const uint2*>(q + c.at(p));
+        const uint2 u = *reinterpret_cast<const uint2*>(from + c.at(piece));
         w[p].u[0] = u.x;
         w[p].u[1] = u.y;
       } else {
-        w[p].u[0] = *reinterpret_cast<const uint32_t*>(q + c.at(p));
+        w[p].u[0] = *reinterpret_cast<const uint32_t*>(from + c.at(piece));
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) w[p].e[j] = c.at(p, j) < c.cols ? q[c.at(p, j)] : int8_t(0);
+      for (int j = 0; j < V; ++j)
+        if (c.at(piece, j) < c.cols) w[p].e[j] = from[c.at(piece, j)];
     }
   }
 #pragma unroll
   for (int p = 0; p < kReadPieces; ++p) {
+    const int r = SHORT ? p / (SHORT ? SHORT : 1) : 0;
+    if (first + r >= a.rows) break;
     Piece<T> v;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      v.e[j] = from_f32<T>(inside ? (float(w[p].e[j]) * scale) * a.factor : 0.f);
-    store_piece<WIDE>(v, out, c, p, turns[WIDE ? 0 : threadIdx.x >> 5]);
+    for (int j = 0; j < V; ++j) v.e[j] = from_f32<T>((float(w[p].e[j]) * scale[r]) * a.factor);
+    store_piece<WIDE>(v, static_cast<T*>(a.out) + (first + r) * a.ld_out, c,
+                      SHORT ? p % (SHORT ? SHORT : 1) : piece0 + p, turns[WIDE ? 0 : threadIdx.x >> 5]);
   }
 }
 
@@ -472,24 +501,28 @@ cudaError_t launch(const void* fn, int64_t blocks, void** args, cudaStream_t s,
 
 template <class T, bool NORM, bool WIDE>
 cudaError_t launch_rows_t(RowsQ8Args a, int num_sms, cudaStream_t s) {
-  constexpr int V = Piece<T>::V, kMost = 32 / V;  // 32 values a lane
+  constexpr int V = Piece<T>::V;
   const int64_t rows = a.out.rows;
   const int passes = (a.out.cols + 32 * V - 1) / (32 * V);  // pieces of one warp's lanes
-  if (passes > kWarps * kMost) {
+  if (passes > kMostWarps * kMostPieces) {
     void* p[] = {&a};
     return launch(reinterpret_cast<const void*>(&long_rows_kernel<T, NORM, WIDE>), rows, p, s);
   }
+  // as few warps a row as hold it (one also with eight pieces a lane: 65536 rows of 1024 f32 values are
+  // quantised in 49 us then, 68 by pairs of warps), but where rows are few as many as it has pieces for, up
+  // to 8
   int warps = 1;
-  while (warps < kWarps && (passes > warps * kMost ||
-                            (passes > warps && rows * warps < int64_t(num_sms) * 32)))
+  while (passes > warps * (!NORM && V == 4 && warps == 1 ? 8 : kMostPieces) ||
+         (warps < 8 && passes > warps && rows * warps < int64_t(num_sms) * 32))
     warps *= 2;
   const int np = (passes + warps - 1) / warps;
   const int64_t blocks = warps == 1 ? (rows + kWarps - 1) / kWarps : rows;
   void* p[] = {&a, &warps};
   const void* fn = np <= 1   ? reinterpret_cast<const void*>(&rows_kernel<T, 1, NORM, WIDE>)
                    : np <= 2 ? reinterpret_cast<const void*>(&rows_kernel<T, 2, NORM, WIDE>)
+                   : np <= 3 ? reinterpret_cast<const void*>(&rows_kernel<T, 3, NORM, WIDE>)
                    : np <= 4 ? reinterpret_cast<const void*>(&rows_kernel<T, 4, NORM, WIDE>)
-                             : reinterpret_cast<const void*>(&rows_kernel<T, kMost, NORM, WIDE>);
+                             : reinterpret_cast<const void*>(&rows_kernel<T, NORM || V == 8 ? 4 : 8, NORM, WIDE>);
   return launch(fn, blocks, p, s, warps == 1 ? kThreads : 32 * warps);
 }
 
@@ -506,25 +539,31 @@ cudaError_t launch_rows(const RowsQ8Args& a, int num_sms, cudaStream_t s) {
               : launch_rows_t<T, false, false>(a, num_sms, s);
 }
 
+template <class T, bool WIDE>
+cudaError_t launch_read(ReadQ8Args a, cudaStream_t s) {
+  constexpr int per = 32 * Piece<T>::V;
+  const int pieces = (a.src.cols + per - 1) / per;
+  int segments = (pieces + kReadPieces - 1) / kReadPieces;
+  const int64_t units = pieces <= 2 ? (a.rows * pieces + kReadPieces - 1) / kReadPieces : a.rows * segments;
+  const int64_t blocks = (units + kWarps - 1) / kWarps;
+  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  void* p[] = {&a, &segments};
+  return launch(pieces == 1   ? reinterpret_cast<const void*>(&read_kernel<T, WIDE, 1>)
+                : pieces == 2 ? reinterpret_cast<const void*>(&read_kernel<T, WIDE, 2>)
+                              : reinterpret_cast<const void*>(&read_kernel<T, WIDE, 0>),
+                blocks, p, s);
+}
+
 }  // namespace
 
 cudaError_t launch_rows_q8(const RowsQ8Args& a, int dtype, int num_sms, cudaStream_t s) {
   return dtype == 0 ? launch_rows<__half>(a, num_sms, s) : launch_rows<float>(a, num_sms, s);
 }
 
-cudaError_t launch_read_q8(const ReadQ8Args& args, int dtype, cudaStream_t s) {
-  ReadQ8Args a = args;
-  const int es = dtype == 0 ? 2 : 4, per = kReadPieces * 32 * (16 / es);
-  int segments = (a.src.cols + per - 1) / per;
-  const bool wide = on16(a.out, a.ld_out * es, a.rows);
-  const int64_t blocks = (a.rows * segments + kWarps - 1) / kWarps;
-  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  void* p[] = {&a, &segments};
-  const void* fn = dtype == 0 ? (wide ? reinterpret_cast<const void*>(&read_kernel<__half, true>)
-                                      : reinterpret_cast<const void*>(&read_kernel<__half, false>))
-                              : (wide ? reinterpret_cast<const void*>(&read_kernel<float, true>)
-                                      : reinterpret_cast<const void*>(&read_kernel<float, false>));
-  return launch(fn, blocks, p, s);
+cudaError_t launch_read_q8(const ReadQ8Args& a, int dtype, cudaStream_t s) {
+  const bool wide = on16(a.out, a.ld_out * (dtype == 0 ? 2 : 4), a.rows);
+  if (dtype == 0) return wide ? launch_read<__half, true>(a, s) : launch_read<__half, false>(a, s);
+  return wide ? launch_read<float, true>(a, s) : launch_read<float, false>(a, s);
 }
 
 }  // namespace p2p

@@ -10,6 +10,7 @@ static int g_launches;
 namespace p2p {
 int ctx_device(const p2p_ctx*) { return 0; }
 int ctx_num_sms(const p2p_ctx*) { return 148; }
+int32_t debug_wait_deficit() { return 0; }
 int32_t* ctx_dev_err(const p2p_ctx*) { return nullptr; }
 p2p_status ctx_fail(p2p_ctx*, p2p_status s, const char* msg) {
   g_message = msg;

@@ -272,7 +272,8 @@ SIZES = [(1, 1, 1), (1, 64, 64), (1, 2048, 2048), (2, 100, 33), (3, 257, 1003), 
          (8, 64, 128), (9, 1000, 700), (16, 512, 2048), (17, 384, 160), (31, 128, 65), (32, 4100, 256),
          (33, 129, 129), (48, 640, 8192), (64, 256, 1024), (65, 127, 512), (100, 300, 200),
          (128, 128, 128), (129, 257, 300), (200, 2048, 1024), (255, 512, 96), (256, 1024, 512),
-         (257, 2331, 1531), (400, 96, 2048), (513, 768, 768), (1000, 1333, 640), (2050, 1024, 256)]
+         (257, 2331, 1531), (400, 96, 2048), (513, 768, 768), (1000, 1333, 640), (2050, 1024, 256), (2100, 2331, 300), (2300, 130, 1003),
+         (2304, 768, 512)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -467,6 +468,29 @@ def test_two_streams_at_once(ctx):
             ctx.gemm_q8((w, ws), x, s, y, stream=st)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 64, 1024), (8, 4000, 256), (2100, 700, 1000)])
+def test_a_wait_that_runs_out_is_a_status(ctx, m, n, k):
+    """The first stage of every ring waits for bytes that never come: the call ends, nothing is stored,
+    p2p_sync says so, and the next call is as ever.  (k split over clusters, one CTA a tile, pairs.)"""
+    import p2p_b200
+    g = gen(7)
+    x, xs = codes(g, m, k)
+    w, ws = codes(g, n, k)
+    y = torch.full((m, n), 3.0, device="cuda")
+    p2p_b200.lib.p2p_debug_set_wait_deficit(16)
+    try:
+        ctx.gemm_q8((w, ws), x, xs, y)
+    finally:
+        p2p_b200.lib.p2p_debug_set_wait_deficit(0)
+    with pytest.raises(p2p_b200.P2PError) as e:
+        ctx.sync()
+    assert e.value.status == p2p_b200.P2P_ERR_TIMEOUT
+    assert (y == 3).all()
+    ctx.gemm_q8((w, ws), x, xs, y)
+    check_gemm(y, x, xs, w, ws, None, None, F32)
+    ctx.sync()
 
 
 class Model:

@@ -97,7 +97,7 @@ def test_quantize_refusals(api):
     said(api, quantize(api, good, src=MB + 1), BAD)
     said(api, quantize(api, good, src=MB + 2, dtype=1), BAD)
     said(api, quantize(api, good, ld=63), BAD)
-    for bad in (rows(4 * MB, n=-1), rows(4 * MB, k=0), rows(4 * MB, k=65537), rows(4 * MB + 8),
+    for bad in (rows(4 * MB, n=-1), rows(4 * MB, n=2**30 + 1), rows(4 * MB, k=0), rows(4 * MB, k=65537), rows(4 * MB + 8),
                 rows(4 * MB, ld=72), rows(4 * MB, ld=48), rows(4 * MB, scale=5 * MB + 2),
                 rows(0, scale=MB)):
         said(api, quantize(api, bad), BAD)
@@ -129,6 +129,7 @@ def test_read_refusals(api):
     said(api, read(api, None), BAD)
     said(api, read(api, good, n=5), BAD)  # more rows than there are, in order
     said(api, read(api, good, n=-1, index=8 * MB), BAD)
+    said(api, read(api, good, n=2**30 + 1, index=2**45), BAD)
     said(api, read(api, good, index=8 * MB + 2), BAD)
     said(api, read(api, good, dtype=5), UNSUPPORTED)
     said(api, read(api, good, out=None), BAD)
@@ -164,6 +165,7 @@ def test_norm_refusals(api):
     said(api, norm(api, out=Q8Rows(None, None, 0, 4, 64), sum=None, y=None), BAD, "all NULL")
     said(api, norm(api, out=Q8Rows(None, None, 0, 4, 0)), BAD)
     said(api, norm(api, out=Q8Rows(None, None, 0, -1, 64)), BAD)
+    said(api, norm(api, out=Q8Rows(None, None, 0, 2**30 + 1, 64)), BAD)
     said(api, norm(api, out=rows(4 * MB, ld=72)), BAD)
     said(api, norm(api, dtype=3), UNSUPPORTED)
     for eps in (-1.0, float("nan"), float("inf")):
