@@ -647,15 +647,17 @@ class Context:
     def _q8(self, q: torch.Tensor, scale: torch.Tensor, name: str) -> tuple:
         """Checks int8 rows and their scales and returns the fields of the C view: codes, scales,
         pitch, rows, columns."""
-        shape = q.shape
-        if q.dtype is not torch.int8 or q.get_device() != self.device or len(shape) != 2:
-            _refuse(f"{name}: int8 [rows][cols] on device {self.device} needed, "
-                    f"got {tuple(shape)} {q.dtype} on {q.device}")
-        n, k = shape
-        ld, one = q.stride()
-        if one != 1 and k > 1:
-            _refuse(f"{name}: neighbouring codes of a row needed, strides {q.stride()}")
-        return (q.data_ptr(), self._floats(scale, n, name), ld if n > 1 else (k + 15) & -16, n, k)
+        dev = self.device
+        if q.dtype is torch.int8 and q.get_device() == dev and q.dim() == 2:
+            n, k = q.shape
+            ld, one = q.stride()
+            if one == 1 or k <= 1:
+                if scale.dtype is torch.float32 and scale.get_device() == dev and \
+                        scale.numel() >= n and scale.is_contiguous():
+                    return (q.data_ptr(), scale.data_ptr(), ld if n > 1 else (k + 15) & -16, n, k)
+                _refuse(f"{name}: {n} contiguous f32 scales on device {dev} needed")
+        _refuse(f"{name}: int8 [rows][cols], neighbouring codes of a row, on device {dev} needed, "
+                f"got {tuple(q.shape)} {q.dtype} on {q.device}, strides {q.stride()}")
 
     def _new_q8(self, q, scale, rows: int, cols: int, device):
         """int8 rows on 16-byte boundaries and their scales, where the caller has none."""

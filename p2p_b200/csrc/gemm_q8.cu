@@ -924,16 +924,17 @@ NarrowPlan narrow_plan(int m, int n, int k, int G, int num_sms, int room) {
       const float turns = float((tiles + slots - 1) / slots);
       const float fixed = split > 1 ? turns * (1300 + 0.52f * G * rows * tokens + 12 * tokens)
                                     : turns * 100 + 30.f * tokens;
-      for (int chunks = 1; chunks <= kMostChunks; ++chunks) {
+      for (int chunks = kMostChunks; chunks >= 1; --chunks) {
         // stages of several steps want rows of whole steps, and leave no part of a stage empty
         if (chunks > 1 &&
             (k % kStep || nk % chunks || chunks * (G * rows + tokens) * kStep > kMostStage))
           continue;
         const int steps = nk / chunks;
-        if (split > steps) break;
+        if (split > steps) continue;
         const float stage = std::max(chunks * bytes + kWait, chunks * 4 * G * kIssue + kHandOver);
         const float cost = turns * ((steps + split - 1) / split) * stage + fixed;
         if (!best.rows || cost < best.cost) best = NarrowPlan{rows, tokens, split, chunks, steps, cost};
+        if (steps % split == 0) break;  // smaller stages only wait more often
       }
     }
   }
