@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "gemm_common.cuh"
@@ -50,14 +51,21 @@ struct Q8Params {
   int32_t deep;                 // the tensor maps' third dimension is k in steps of 128
 };
 
-// act(g) * u.  The exponential and the quotient are approximations of 2 units in the last place each.
-__device__ __forceinline__ float act_mul(float g, float u, int act) {
-  const float t = act == kActSilu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-  return __fdividef(g, 1.f + __expf(-t)) * u;
+// act(g) * u, the exponential and the reciprocal as approximations of a few units in the last place, with
+// what is below f32's normal numbers taken as 0 (a reciprocal of more than 2^126 too): f16 has none of it.
+template <bool GELU>
+__device__ __forceinline__ Pair act_mul(Pair g, Pair u) {
+  constexpr float k = GELU ? -1.5957691216057308f * kLog2e : -kLog2e;
+  Pair t = mul2(g, pair(k, k));
+  if constexpr (GELU) t = mul2(t, mad2(mul2(g, g), pair(0.044715f, 0.044715f), pair(1.f, 1.f)));
+  const Pair d = add2(pair(fast_exp2(t.f[0]), fast_exp2(t.f[1])), pair(1.f, 1.f));
+  Pair r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.f[0]) : "f"(d.f[0]));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.f[1]) : "f"(d.f[1]));
+  return mul2(mul2(g, r), u);
 }
-
-__device__ __forceinline__ Pair act_mul2(Pair g, Pair u, int act) {
-  return pair(act_mul(g.f[0], u.f[0], act), act_mul(g.f[1], u.f[1], act));
+__device__ __forceinline__ Pair act_mul(Pair g, Pair u, int act) {
+  return act == kActSilu ? act_mul<false>(g, u) : act_mul<true>(g, u);
 }
 
 __device__ __forceinline__ Pair scaled2(uint32_t a, uint32_t b, Pair xs, Pair ws) {
@@ -248,14 +256,18 @@ __device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem& s, ui
       v[2 * j + 1] = scaled2(r[4 * j + 2], r[4 * j + 3], xs2, pair(w.z, w.w));
     }
     if constexpr (GATE) {
+      const auto finish = [&](auto gelu) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float4 w = s4[j];
-        const Pair u0 = scaled2(ru[4 * j], ru[4 * j + 1], xs2, pair(w.x, w.y));
-        const Pair u1 = scaled2(ru[4 * j + 2], ru[4 * j + 3], xs2, pair(w.z, w.w));
-        v[2 * j] = act_mul2(v[2 * j], u0, p.act);
-        v[2 * j + 1] = act_mul2(v[2 * j + 1], u1, p.act);
-      }
+        for (int j = 0; j < 8; ++j) {
+          const float4 w = s4[j];
+          v[2 * j] = act_mul<gelu.value>(
+              v[2 * j], scaled2(ru[4 * j], ru[4 * j + 1], xs2, pair(w.x, w.y)));
+          v[2 * j + 1] = act_mul<gelu.value>(
+              v[2 * j + 1], scaled2(ru[4 * j + 2], ru[4 * j + 3], xs2, pair(w.z, w.w)));
+        }
+      };
+      if (p.act == kActSilu) finish(std::false_type{});
+      else finish(std::true_type{});
     } else if (p.bias) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -713,7 +725,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
             const Pair xs2 = pair(scales[t0 + j], scales[t0 + j + 1]);
             Pair v = scaled2(r[0][j], r[0][j + 1], xs2, ws2);
             if constexpr (GATE) {
-              v = act_mul2(v, scaled2(r[G - 1][j], r[G - 1][j + 1], xs2, second2), p.act);
+              v = act_mul(v, scaled2(r[G - 1][j], r[G - 1][j + 1], xs2, second2), p.act);
             } else {
               if (p.bias) v = add2(v, second2);
               if (res) v = add2(v, pair(add[j], add[j + 1]));
@@ -774,7 +786,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
         for (int j = 0; j < 4; j += 2) {
           Pair v = scaled2(acc[0][j], acc[0][j + 1], xs[j / 2], ws2);
           if constexpr (GATE) {
-            v = act_mul2(v, scaled2(acc[G - 1][j], acc[G - 1][j + 1], xs[j / 2], second2), p.act);
+            v = act_mul(v, scaled2(acc[G - 1][j], acc[G - 1][j + 1], xs[j / 2], second2), p.act);
           } else {
             if (p.bias) v = add2(v, second2);
             if (p.res) v = add2(v, pair(add[j], add[j + 1]));
