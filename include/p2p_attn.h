@@ -11,6 +11,9 @@
  *   QK_PREP and ATTN of ragged prompt chunks over those caches -> p2p_kv_append,
  *                p2p_attn_chunk_kv; the cached rows back        -> p2p_kv_read
  *   ARGMAX of a batch under penalties, biases and grammar masks -> p2p_logits_pick
+ *   ADD_RMS      src/scripts/lfm-engine/kernels.js:146-182, SILU_MUL :321-339 and the projections
+ *                around the attention in 8-bit integers -> p2p_add_norm_q8, p2p_gate_q8, p2p_gemm_q8,
+ *                p2p_quantize_rows_q8, p2p_read_rows_q8
  *   VISION_ATTN  src/scripts/lfm-engine/vision-kernels.js:176-258 -> p2p_attn_bidir
  *   ropeTable    src/scripts/lfm-engine/engine.js:60-71      -> p2p_rope_table
  *   meta buffer  src/scripts/lfm-engine/engine.js:144,388,422 -> p2p_meta / p2p_meta_write
@@ -422,8 +425,11 @@ p2p_status p2p_logits_pick(p2p_ctx* ctx, const p2p_logits* args, void* stream);
  *   p2p_quantize_rows_q8  weights (once, from p2p_q4_to_f16's rows or any f16 / f32 ones) and
  *                         activations between two products
  * codes: rows of `cols` bytes, ld apart (q 16-byte aligned, ld a multiple of 16; what lies between
- * two rows is neither read nor written); scale 4-byte aligned.  The entry points below refuse (but
- * for what each says) outputs that overlap inputs or each other.  They use no workspace. */
+ * two rows is neither read nor written); scale 4-byte aligned.  f16 / f32 rows need only their type's
+ * alignment; results do not depend on it, rows on 16-byte boundaries are faster.  The entry points below
+ * refuse (but for what each says) outputs that overlap inputs or each other; of operands with different
+ * numbers of rows, ranges of addresses that meet.  They use no workspace and may run on several streams
+ * at once, and be captured from the first call on. */
 #define P2P_MAX_Q8_COLS 65536
 #define P2P_MAX_Q8_ROWS (1 << 30)
 typedef struct p2p_q8_rows {
@@ -459,8 +465,9 @@ p2p_status p2p_read_rows_q8(p2p_ctx* ctx, const p2p_read_rows* args, void* strea
 /* For every row, in f32:  s = x + residual, rounded to dtype;  y = (s * weight) / sqrt(mean(s^2) + eps);
  * s goes to sum, y (rounded to dtype) to y, and y's codes and scale (of the unrounded y, by the rule of
  * p2p_quantize_rows_q8) to out.  residual, weight (then 1), sum, y and out.q may be NULL; without out.q,
- * out.scale is not used.  out.rows and out.cols are the call's in any case.  sum or y may be x or residual themselves, with the same pitch.  A row whose sum of
- * squares is not finite gives y NaN, scale NaN, codes 0.  (f32 rows: values below 2^60.) */
+ * out.scale is not used.  out.rows and out.cols are the call's in any case.  sum or y may be x or residual
+ * themselves, with the same pitch.  A row whose sum of squares is not finite in f32 (f32 values from about
+ * 2^60 on) gives y NaN, scale NaN, codes 0. */
 typedef struct p2p_add_norm {
   const void* x;        /* [rows][ld_x], f16 or f32 */
   const void* residual; /* [rows][ld_r] */

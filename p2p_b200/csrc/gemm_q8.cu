@@ -4,10 +4,16 @@
 //
 // Sums are whole numbers in 32 bits on tcgen05.mma.kind::i8, so every split of them gives the same
 // result; the scales, the activation and what is added follow in f32.  Two kernels:
-//   wide_kernel    many tokens: a cluster of two CTAs per 256-token tile and one
-//                  tcgen05.mma.cta_group::2 stream, persistent;
+//   wide_kernel    many tokens, bound by the MMAs (and, called back to back, by the power limit): a cluster
+//                  of two CTAs per 256 x 256 tile and one tcgen05.mma.cta_group::2 stream, persistent, two
+//                  accumulators, the last wave's tiles halved.  Gate and up of 4096 tokens (8192 x 2048
+//                  each): 76 us alone (3630 TOP/s, 89 % of the tensor pipe's cycles), 86 us among some,
+//                  101 us in long runs; 8192 x 2048 x 8192: 81, 89 and 103 us.
 //   narrow_kernel  few tokens, bound by the weights' bytes: the weights are the MMA's rows and the tokens
-//                  its columns.
+//                  its columns.  The LM head of 32 tokens (65536 x 2048) 24.9 us (5.7 TB/s), gate and up of
+//                  one token (2 x 8192 x 2048) 6.9 us, 48 x 2048 x 8192 7.1 us (15 by pairs of CTAs).
+// A warp that walks a ring does so as a whole: with its loop in one lane the compiler has to treat what a
+// copy takes as different in every lane, and a stage took 200 ns to issue (8192 x 2048 x 8192 98 -> 91 us).
 // Every mbarrier wait is bounded (about one second): a wait that gives up sets the device error word,
 // every role of the CTA stops, the copies and MMAs in flight are waited for, the TMEM is freed and the
 // CTA returns.

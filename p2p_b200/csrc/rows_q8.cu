@@ -508,11 +508,13 @@ cudaError_t launch_rows_t(RowsQ8Args a, int num_sms, cudaStream_t s) {
     void* p[] = {&a};
     return launch(reinterpret_cast<const void*>(&long_rows_kernel<T, NORM, WIDE>), rows, p, s);
   }
-  // as few warps a row as hold it (one also with eight pieces a lane: 65536 rows of 1024 f32 values are
-  // quantised in 49 us then, 68 by pairs of warps), but where rows are few as many as it has pieces for, up
-  // to 8
+  // As few warps a row as hold it in kMostPieces pieces a lane, the norm, which holds x and the residual,
+  // in two (8192 rows of 2048 f16 values 22.5 us, 23.8 in four; 13.8 and 15.2 for 1024), one warp also
+  // with eight pieces a lane (65536 rows of 1024 f32 values are quantised in 49 us then, 68 by pairs of
+  // warps); but where rows are few, as many as the row has pieces for, up to 8.
+  const int most = NORM && passes <= 2 * kMostWarps ? 2 : kMostPieces;
   int warps = 1;
-  while (passes > warps * (!NORM && V == 4 && warps == 1 ? 8 : kMostPieces) ||
+  while (passes > warps * (!NORM && V == 4 && warps == 1 ? 8 : most) ||
          (warps < 8 && passes > warps && rows * warps < int64_t(num_sms) * 32))
     warps *= 2;
   const int np = (passes + warps - 1) / warps;

@@ -213,6 +213,18 @@ def test_norm(ctx, dt, m, k, pad, off, weighted, residual):
         assert torch.equal(q2, q) and torch.equal(r2, total)
 
 
+@pytest.mark.parametrize("k", [512, 1003])
+def test_norm_weights_anywhere(ctx, k):
+    """Weights that start between two 16-byte boundaries, and no codes' neighbours touched."""
+    g = gen(k)
+    x, r = rows_in(g, 50, k, F16), rows_in(g, 50, k, F16)
+    w = (1 + 0.3 * torch.randn(k + 1, generator=g, device="cuda")).half()[1:]
+    q, s = ctx.add_norm_q8(x, w, residual=r)
+    check_norm(x, r, w, 1e-5, F16, q, s)
+    q2, s2 = ctx.add_norm_q8(x, w.clone(), residual=r)
+    assert torch.equal(q, q2) and torch.equal(s, s2)
+
+
 def test_norm_without_codes(ctx):
     from p2p_b200 import _lib, lib
     import ctypes as C
@@ -381,6 +393,16 @@ def test_gate_ends_of_the_activation(ctx, act, m):
     bad = torch.zeros(m, 64, dtype=torch.bool, device="cuda")
     bad[m // 2], bad[:, 9] = True, True
     assert torch.isnan(h[bad]).all() and not torch.isnan(h[~bad]).any()
+
+
+@pytest.mark.parametrize("m", [3, 200, 2100])
+def test_the_same_rows_on_every_side(ctx, m):
+    """One matrix as gate, up and tokens."""
+    q, s = codes(gen(m), m, 256)
+    s = s / 16
+    h = torch.zeros(m, m, device="cuda", dtype=F16)
+    ctx.gate_q8((q, s), (q, s), q, s, h)
+    check_gate(h, q, s, q, s, q, s, "silu")
 
 
 def test_empty_calls(ctx):
