@@ -86,18 +86,22 @@ constexpr int kTmaWarp = kEpiWarps, kMmaWarp = kEpiWarps + 1;
 constexpr int kWideThreads = 32 * (kEpiWarps + 2);
 constexpr int kBoxRows = 64;    // weight rows per TMA box
 constexpr uint32_t kTileBytes = kRows * kStep;          // x, and a CTA's half of the weights
-constexpr int kWideStages = 5;
-// A warp's 32 x 32 outputs change hands through shared memory, so that it stores whole stretches of rows: a
-// row of f32 takes 36 words, one of f16 20 (both keep 16-byte accesses of a column free of conflicts).
+// A warp's 32 x 32 outputs change hands through shared memory, so that it stores whole stretches of rows:
+// 20 words a row of f16, 36 of f32 (both keep 16-byte accesses of a column free of conflicts), and what
+// that leaves goes to the ring (8192 x 2048 x 8192 in 84.0 us with 6 stages, 85.0 with 5, 91 with 4).
 template <class T>
 constexpr int kPitch = sizeof(T) == 4 ? 36 : 20;
+template <class T>
+constexpr int kWideStages = sizeof(T) == 4 ? 5 : 6;
 
+template <class T>
 struct __align__(1024) WideSmem {
-  uint8_t a[kWideStages][kTileBytes];
-  uint8_t b[kWideStages][kTileBytes];
-  uint32_t turn[kEpiWarps][32 * kPitch<float>];
+  static constexpr int kStages = kWideStages<T>;
+  uint8_t a[kStages][kTileBytes];
+  uint8_t b[kStages][kTileBytes];
+  uint32_t turn[kEpiWarps][32 * kPitch<T>];
   float col[kEpiWarps][2][128];         // a warp's columns: scales, and biases or the up scales
-  uint64_t full[kWideStages], empty[kWideStages];
+  uint64_t full[kStages], empty[kStages];
   uint64_t acc_full[2], acc_empty[2];
   uint64_t mma_done;
   uint32_t tmem_base;
@@ -131,64 +135,85 @@ __device__ __forceinline__ Item item_of(const Q8Params& p, int i) {
 template <class T>
 __device__ __forceinline__ void store_block(const Q8Params& p, const Pair (&v)[16], int m_base, int lane,
                                             int n, bool aligned, uint32_t* turn) {
-  if (aligned) {
-    constexpr int kWords = 32 * sizeof(T) / 4, kPieces = kWords / 4;  // of a row
-    uint4* mine = reinterpret_cast<uint4*>(turn + lane * kPitch<T>);
+  constexpr bool kF16 = sizeof(T) == 2;
+  uint4* mine = reinterpret_cast<uint4*>(turn + lane * kPitch<T>);
+  // N pairs of this lane's row, from pair `first` on, as they are or as f16
+  const auto put = [&](int first, auto f16, auto pairs) {
+    constexpr int kEach = f16.value ? 4 : 2;  // pairs in 16 bytes
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < pairs.value / kEach; ++i) {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(T) == 4) {
-          w[j] = __float_as_uint(v[2 * i + j / 2].f[j % 2]);
-        } else {
-          const __half2 h = __floats2half2_rn(v[4 * i + j].f[0], v[4 * i + j].f[1]);
+        if constexpr (f16.value) {
+          const Pair& q = v[first + 4 * i + j];
+          const __half2 h = __floats2half2_rn(q.f[0], q.f[1]);
           w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          w[j] = __float_as_uint(v[first + 2 * i + j / 2].f[j % 2]);
         }
       }
       mine[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __syncwarp();
-    constexpr int kRowsAtOnce = 32 / kPieces;
+  };
+  using All = std::integral_constant<int, 16>;
+  using Half = std::integral_constant<int, 8>;
+  if (aligned) {
+    put(0, std::bool_constant<kF16>{}, All{});
+    constexpr int kPieces = kF16 ? 4 : 8, kRowsAtOnce = 32 / kPieces;  // of 16 bytes in a row
     const int r0 = lane / kPieces, piece = lane % kPieces;
     T* d = static_cast<T*>(p.y) + int64_t(m_base + r0) * p.ld_y + n;
-    const int64_t ld = kRowsAtOnce * p.ld_y;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i, d += ld) {
+    for (int i = 0; i < kPieces; ++i, d += kRowsAtOnce * p.ld_y) {
       const uint4 w = reinterpret_cast<const uint4*>(turn + (r0 + i * kRowsAtOnce) * kPitch<T>)[piece];
       if (m_base + r0 + i * kRowsAtOnce < p.m) reinterpret_cast<uint4*>(d)[piece] = w;
     }
     __syncwarp();
     return;
   }
-  // rows that start anywhere, or end inside the block: a row at a time along the lanes
-  float4* mine = reinterpret_cast<float4*>(turn + lane * kPitch<float>);
+  // Rows that start anywhere, or end inside the block: neighbours in neighbouring lanes, value by value,
+  // eight rows in flight.  From what was put: rows of `each` lanes, U values `pitch` apart.
+  const int rows = min(32, p.m - m_base);
+  const auto take = [&](auto unit, int col0, auto lanes) {
+    using U = decltype(unit);
+    constexpr int kAtOnce = 32 / lanes.value, kRowPitch = kPitch<T> * 4 / sizeof(U) * kAtOnce;
+    const int r0 = lane / lanes.value, c = n + col0 + lane % lanes.value;
+    if (c < p.n) {
+      T* d = static_cast<T*>(p.y) + int64_t(m_base + r0) * p.ld_y + c;
+      const T* r = p.res ? static_cast<const T*>(p.res) + int64_t(m_base + r0) * p.ld_res + c : nullptr;
+      const U* t = reinterpret_cast<const U*>(turn + r0 * kPitch<T>) + lane % lanes.value;
+      for (int i = r0; i < rows; i += 8 * kAtOnce, t += 8 * kRowPitch) {
+        float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    mine[i] = make_float4(v[2 * i].f[0], v[2 * i].f[1], v[2 * i + 1].f[0], v[2 * i + 1].f[1]);
-  __syncwarp();
-  const int rows = min(32, p.m - m_base), c = n + lane;
-  if (c < p.n) {
-    T* d = static_cast<T*>(p.y) + int64_t(m_base) * p.ld_y + c;
-    const float* t = reinterpret_cast<const float*>(turn) + lane;
-    const T* r = p.res ? static_cast<const T*>(p.res) + int64_t(m_base) * p.ld_res + c : nullptr;
-    for (int i = 0; i < rows; i += 8, t += 8 * kPitch<float>) {
-      float y[8];
+        for (int j = 0; j < 8; ++j) y[j] = to_f32(t[j * kRowPitch]);
+        if (r) {
+          float add[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = t[j * kPitch<float>];
-      if (r) {
-        float add[8];
+          for (int j = 0; j < 8; ++j, r += kAtOnce * p.ld_res)
+            add[j] = i + j * kAtOnce < rows ? to_f32(*r) : 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j, r += p.ld_res) add[j] = i + j < rows ? to_f32(*r) : 0.f;
+          for (int j = 0; j < 8; ++j) y[j] = __fadd_rn(y[j], add[j]);
+        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = __fadd_rn(y[j], add[j]);
+        for (int j = 0; j < 8; ++j, d += kAtOnce * p.ld_y)
+          if (i + j * kAtOnce < rows) *d = from_f32<T>(y[j]);
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j, d += p.ld_y)
-        if (i + j < rows) *d = from_f32<T>(y[j]);
     }
+    __syncwarp();
+  };
+  if constexpr (!kF16) {
+    put(0, std::false_type{}, All{});
+    take(0.f, 0, std::integral_constant<int, 32>{});
+  } else if (!p.res) {
+    put(0, std::true_type{}, All{});
+    take(T{}, 0, std::integral_constant<int, 32>{});
+  } else {  // the sums are rounded once, with what is added: half of the columns at a time
+    put(0, std::false_type{}, Half{});
+    take(0.f, 0, std::integral_constant<int, 16>{});
+    put(8, std::false_type{}, Half{});
+    take(0.f, 16, std::integral_constant<int, 16>{});
   }
-  __syncwarp();
 }
 
 // What an epilogue warp multiplies an item's sums with: its token's scale, and by lane the scales of its
@@ -217,7 +242,7 @@ __device__ __forceinline__ Ahead look_ahead(const Q8Params& p, const Item& it, i
 // The epilogue of one item by epilogue warp `warp`: TMEM lane quarter warp & 3, every other block of 32
 // columns.
 template <class T, bool GATE, class Release>
-__device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem& s, uint32_t acc,
+__device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem<T>& s, uint32_t acc,
                                               const Item& it, int m0, const Ahead& ahead, int warp,
                                               int lane, Release release) {
   const int quarter = warp & 3, half = warp >> 2;
@@ -302,14 +327,15 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                 const __grid_constant__ CUtensorMap tm_u, const __grid_constant__ Q8Params p) {
   extern __shared__ uint8_t smem_raw[];
-  WideSmem& s = *reinterpret_cast<WideSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
+  constexpr uint32_t kStages = kWideStages<T>;
+  WideSmem<T>& s = *reinterpret_cast<WideSmem<T>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                   ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = int(cluster_id_x()), pairs = int(cluster_count_x());
   const int nk = (p.k + kStep - 1) / kStep;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kWideStages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], 1);
     }
@@ -352,7 +378,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             tma_load_3d_pair(s.b[st] + kBoxRows * kStep, tm_b, kt * kStep, n0 + kBoxRows, 0, full0);
         }
         __syncwarp();
-        if (++st == kWideStages) {
+        if (++st == kStages) {
           st = 0;
           ++round;
         }
@@ -360,7 +386,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
     if (!ok && lane == 0) {  // let the copies already in flight land before the CTA exits
       if (rank == 0) {
-        for (int h = 0; h < kWideStages; ++h) {
+        for (int h = 0; h < kStages; ++h) {
           const uint64_t t0 = globaltimer_ns();
           while (!mbar_try_wait(&s.full[h], uint32_t(h) < st ? round & 1 : (round - 1) & 1) &&
                  globaltimer_ns() - t0 < kGemmWaitNs) {
@@ -389,8 +415,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const uint32_t idesc = idesc_i8(2 * kRows, item_of<GATE>(p, i).bn);
         const uint32_t acc = tmem + uint32_t(b * kWidth);
         for (int kt = 0; kt < nk; ++kt, ++g) {
-          const uint32_t st = g % kWideStages;
-          if (!(ok = gemm_wait_all(s.abort_flag, &s.full[st], (g / kWideStages) & 1, p.err)))
+          const uint32_t st = g % kStages;
+          if (!(ok = gemm_wait_all(s.abort_flag, &s.full[st], (g / kStages) & 1, p.err)))
             break;
           tc_fence_after();
           if (elect_one()) {
@@ -851,7 +877,7 @@ cudaError_t launch_wide(Q8Params p, const GemmQ8Args& a, int num_sms, cudaStream
       !map_codes(&tu, GATE ? a.up : a.w, kBoxRows))
     return cudaErrorInvalidValue;
   const void* fn = reinterpret_cast<const void*>(&wide_kernel<T, GATE>);
-  const size_t smem = sizeof(WideSmem) + 1024;
+  const size_t smem = sizeof(WideSmem<T>) + 1024;
   static PerDeviceOnce setup;
   int max_pairs = 0;
   cudaError_t e = per_device_once(setup, [&](int& pairs) {
