@@ -440,12 +440,17 @@ typedef struct p2p_q8_rows {
   int32_t cols;  /* at most P2P_MAX_Q8_COLS */
 } p2p_q8_rows;
 
-/* dst row i = codes of src row i (f16 or f32 [dst->rows][ld_src]): with a = max |x| over the row,
+/* dst row i = codes of src row i (f16 or f32 [dst.rows][ld_src]): with a = max |x| over the row,
  * scale = a / 127 and code = roundeven(127 x / a), in f32 (ties of f16 rows are exact).  A row whose a is below 2^-100 has
  * scale 0 and codes 0; one that holds an infinity or a NaN has scale NaN and codes 0 (all that is
  * made of it is NaN). */
-p2p_status p2p_quantize_rows_q8(p2p_ctx* ctx, const void* src, int64_t ld_src, int32_t dtype,
-                                const p2p_q8_rows* dst, void* stream);
+typedef struct p2p_quantize_rows {
+  const void* src; /* [dst.rows][ld_src], dst.cols values a row */
+  int64_t ld_src;
+  p2p_q8_rows dst;
+  int32_t dtype; /* P2P_F16 or P2P_F32 */
+} p2p_quantize_rows;
+p2p_status p2p_quantize_rows_q8(p2p_ctx* ctx, const p2p_quantize_rows* args, void* stream);
 
 /* out row i [rows][ld_out] (f16 or f32) = (code * scale) * factor of src row index[i] (device int32
  * array; NULL: row i, and then rows <= src.rows), rounded once to out's type.  An index of -1 (what

@@ -123,6 +123,15 @@ class AddNorm(C.Structure):
     ]
 
 
+class QuantizeRows(C.Structure):
+    _fields_ = [
+        ("src", C.c_void_p),
+        ("ld_src", C.c_int64),
+        ("dst", Q8Rows),
+        ("dtype", C.c_int32),
+    ]
+
+
 class ReadRows(C.Structure):
     _fields_ = [
         ("src", Q8Rows),
@@ -244,7 +253,7 @@ PROTOTYPES = {
               _v, _i64, _v]),
     "p2p_logits_pick": (_st, [_v, C.POINTER(Logits), _v]),
     # (the argument structures as plain addresses: the Python layer packs them itself)
-    "p2p_quantize_rows_q8": (_st, [_v, _v, _i64, _i32, _v, _v]),
+    "p2p_quantize_rows_q8": (_st, [_v, _v, _v]),
     "p2p_read_rows_q8": (_st, [_v, _v, _v]),
     "p2p_add_norm_q8": (_st, [_v, _v, _v]),
     "p2p_gemm_q8": (_st, [_v, _v, _v]),

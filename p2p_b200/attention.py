@@ -72,9 +72,9 @@ _KV_FORMATS = {torch.float16: _lib.P2P_KV_F16, torch.int8: _lib.P2P_KV_I8,
 
 _ROW_TYPES = {torch.float16: _lib.P2P_F16, torch.float32: _lib.P2P_F32}
 _ACTS = {"silu": _lib.P2P_ACT_SILU, "gelu": _lib.P2P_ACT_GELU}
-# Bytes of the C structures of the same order (p2p_q8_rows, p2p_read_rows, p2p_add_norm, p2p_product,
+# Bytes of the C structures of the same order (p2p_quantize_rows, p2p_read_rows, p2p_add_norm, p2p_product,
 # p2p_gated), padded to their size.
-_Q8_ROWS = struct.Struct("@PPqii").pack
+_QUANTIZE_ROWS = struct.Struct("@PqPPqiii4x").pack
 _READ_ROWS = struct.Struct("@PPqiiPPqiif4x").pack
 _ADD_NORM = struct.Struct("@PPPPPqqqqPPqiiif").pack
 _PRODUCT = struct.Struct("@PPqiiPPqiiPPPqqi4x").pack
@@ -648,8 +648,9 @@ class Context:
         """Checks int8 rows and their scales and returns the fields of the C view: codes, scales,
         pitch, rows, columns."""
         dev = self.device
-        if q.dtype is torch.int8 and q.get_device() == dev and q.dim() == 2:
-            n, k = q.shape
+        shape = q.shape
+        if q.dtype is torch.int8 and q.get_device() == dev and len(shape) == 2:
+            n, k = shape
             ld, one = q.stride()
             if one == 1 or k <= 1:
                 if scale.dtype is torch.float32 and scale.get_device() == dev and \
@@ -657,7 +658,7 @@ class Context:
                     return (q.data_ptr(), scale.data_ptr(), ld if n > 1 else (k + 15) & -16, n, k)
                 _refuse(f"{name}: {n} contiguous f32 scales on device {dev} needed")
         _refuse(f"{name}: int8 [rows][cols], neighbouring codes of a row, on device {dev} needed, "
-                f"got {tuple(q.shape)} {q.dtype} on {q.device}, strides {q.stride()}")
+                f"got {tuple(shape)} {q.dtype} on {q.device}, strides {q.stride()}")
 
     def _new_q8(self, q, scale, rows: int, cols: int, device):
         """int8 rows on 16-byte boundaries and their scales, where the caller has none."""
@@ -678,8 +679,9 @@ class Context:
         d = self._q8(q, scale, "q")
         if d[3] != m or d[4] != k:
             _refuse(f"q: [{m}][{k}] needed, got {tuple(q.shape)}")
-        st = lib.p2p_quantize_rows_q8(self.h, src.data_ptr(), ld, _ROW_TYPES[src.dtype],
-                                      _Q8_ROWS(*d), self._stream(stream))
+        st = lib.p2p_quantize_rows_q8(
+            self.h, _QUANTIZE_ROWS(src.data_ptr(), ld, *d, _ROW_TYPES[src.dtype]),
+            self._stream(stream))
         if st:
             self._chk(st)
         return q, scale

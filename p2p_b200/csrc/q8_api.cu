@@ -116,10 +116,14 @@ p2p::Q8Rows view(const p2p_q8_rows* r) {
 
 extern "C" {
 
-p2p_status p2p_quantize_rows_q8(p2p_ctx* ctx, const void* src, int64_t ld_src, int32_t dtype,
-                                const p2p_q8_rows* dst, void* stream) {
+p2p_status p2p_quantize_rows_q8(p2p_ctx* ctx, const p2p_quantize_rows* args, void* stream) {
   if (!ctx) return P2P_ERR_INVALID_ARG;
   const char* who = "quantize_rows_q8";
+  if (!args) return fail(ctx, P2P_ERR_INVALID_ARG, "%s: arguments are NULL", who);
+  const void* src = args->src;
+  const int64_t ld_src = args->ld_src;
+  const int32_t dtype = args->dtype;
+  const p2p_q8_rows* dst = &args->dst;
   p2p_status st;
   if ((st = check_dtype(ctx, dtype, who)) != P2P_OK) return st;
   if ((st = check_q8(ctx, dst, "dst", who)) != P2P_OK) return st;

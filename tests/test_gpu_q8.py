@@ -515,6 +515,54 @@ def test_a_wait_that_runs_out_is_a_status(ctx, m, n, k):
     ctx.sync()
 
 
+FIRST = """
+import sys
+sys.path.insert(0, {root!r})
+import torch, p2p_b200
+ctx = p2p_b200.Context(0)
+w = torch.randint(-127, 128, (700, 1024), device="cuda").to(torch.int8)
+s = torch.rand(700, device="cuda")
+xs = [torch.randint(-127, 128, (m, 1024), device="cuda").to(torch.int8) for m in (1, 100, 2100)]
+t = torch.rand(2100, device="cuda")
+ys = [torch.zeros(len(x), 700, device="cuda") for x in xs]
+hs = [torch.zeros(len(x), 700, device="cuda", dtype=torch.float16) for x in xs]
+f = torch.randn(2100, 1024, device="cuda", dtype=torch.float16)
+q, c = torch.zeros(2100, 1024, device="cuda", dtype=torch.int8), torch.zeros(2100, device="cuda")
+v = torch.zeros_like(f)
+def calls():
+    for x, y, h in zip(xs, ys, hs):
+        ctx.gemm_q8((w, s), x, t[:len(x)], y)
+        ctx.gate_q8((w, s), (w, s), x, t[:len(x)], h)
+    ctx.add_norm_q8(f, None, q, c)
+    ctx.quantize_rows_q8(f, q, c)
+    ctx.read_rows_q8(q, c, v)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    calls()
+g.replay()
+torch.cuda.synchronize()
+outs = ys + hs + [q, c, v]
+got = [y.clone() for y in outs]
+calls()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, outs))
+assert all((a == a).all() and a.abs().max() > 0 for a in got[:3])
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_captured():
+    """Nothing has to be called before a capture: no workspace, no first call that sets anything up on a
+    stream."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST.format(root=str(ROOT))], capture_output=True,
+                       text=True, timeout=120)
+    assert r.stdout.strip() == "same", r.stderr[-2000:]
+
+
 class Model:
     """A decoder layer of 4 query heads and 2 kv heads with an embedding that is the LM head too,
     every product in 8 bits."""

@@ -51,8 +51,8 @@ CTX = 1  # not NULL
 
 def test_null_context_is_a_status():
     from p2p_b200 import _lib, lib
-    r, g = _lib.Q8Rows(), _lib.AddNorm()
-    assert lib.p2p_quantize_rows_q8(None, None, 0, 0, C.byref(r), None) == BAD
+    g = _lib.AddNorm()
+    assert lib.p2p_quantize_rows_q8(None, C.byref(_lib.QuantizeRows()), None) == BAD
     assert lib.p2p_read_rows_q8(None, C.byref(_lib.ReadRows()), None) == BAD
     assert lib.p2p_add_norm_q8(None, C.byref(g), None) == BAD
     assert lib.p2p_gemm_q8(None, C.byref(_lib.Product()), None) == BAD
@@ -70,7 +70,7 @@ def test_packed_structures_are_the_c_ones():
                 yield from flat(kind, off)
             else:
                 yield off, kind
-    for pack, t in ((A._Q8_ROWS, _lib.Q8Rows), (A._READ_ROWS, _lib.ReadRows),
+    for pack, t in ((A._QUANTIZE_ROWS, _lib.QuantizeRows), (A._READ_ROWS, _lib.ReadRows),
                     (A._ADD_NORM, _lib.AddNorm), (A._PRODUCT, _lib.Product),
                     (A._GATED, _lib.Gated)):
         fields = list(flat(t))
@@ -82,7 +82,9 @@ def test_packed_structures_are_the_c_ones():
 
 
 def quantize(api, dst, src=MB, ld=64, dtype=0):
-    return api.p2p_quantize_rows_q8(CTX, src, ld, dtype, C.byref(dst) if dst else None, None)
+    from p2p_b200._lib import QuantizeRows
+    a = QuantizeRows(src, ld, dst, dtype) if dst else None
+    return api.p2p_quantize_rows_q8(CTX, C.byref(a) if a else None, None)
 
 
 def test_quantize_refusals(api):
