@@ -239,12 +239,35 @@ __device__ __forceinline__ Ahead look_ahead(const Q8Params& p, const Item& it, i
   return a;
 }
 
+// A row's 32 values of what is added to a block, where it can be read in whole pieces.
+template <class T>
+struct Addend {
+  static constexpr int V = 16 / sizeof(T), kPieces = 32 / V;
+  union {
+    uint4 u;
+    T e[V];
+  } w[kPieces];
+};
+template <class T>
+__device__ __forceinline__ void load_addend(Addend<T>& a, const Q8Params& p, int m, int n) {
+  if (p.res && p.wide && n + 32 <= p.n && m < p.m) {
+    const uint4* r = reinterpret_cast<const uint4*>(static_cast<const T*>(p.res) +
+                                                    int64_t(m) * p.ld_res + n);
+#pragma unroll
+    for (int j = 0; j < Addend<T>::kPieces; ++j) a.w[j].u = r[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < Addend<T>::kPieces; ++j) a.w[j].u = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // The epilogue of one item by epilogue warp `warp`: TMEM lane quarter warp & 3, every other block of 32
 // columns.
 template <class T, bool GATE, class Release>
 __device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem<T>& s, uint32_t acc,
-                                              const Item& it, int m0, const Ahead& ahead, int warp,
-                                              int lane, Release release) {
+                                              const Item& it, int m0, const Ahead& ahead,
+                                              Addend<T>& addend, int warp, int lane,
+                                              Release release) {
   const int quarter = warp & 3, half = warp >> 2;
   const int cols = GATE ? it.bn / 2 : it.bn, blocks = cols / 32;
   const uint32_t at = acc + (uint32_t(quarter * 32) << 16);
@@ -256,17 +279,11 @@ __device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem<T>& s,
   for (int b = half, i = 0; b < blocks; b += 2, i += 32) {
     const int n = it.n0 + b * 32;
     const bool some = m_base < p.m && n < p.n, aligned = p.wide && n + 32 <= p.n;
-    constexpr int kPieces = 32 * sizeof(T) / 16, V = 16 / sizeof(T);
-    union {
-      uint4 u;
-      T e[V];
-    } res[GATE ? 1 : kPieces];
     const bool add = !GATE && p.res && aligned;
-    if (add) {
-      const uint4* r = reinterpret_cast<const uint4*>(static_cast<const T*>(p.res) +
-                                                      int64_t(m) * p.ld_res + n);
-#pragma unroll
-      for (int j = 0; j < (GATE ? 1 : kPieces); ++j) res[j].u = m < p.m ? r[j] : make_uint4(0, 0, 0, 0);
+    Addend<T> now;
+    if constexpr (!GATE) {
+      now = addend;
+      if (p.res && b + 2 < blocks) load_addend(addend, p, m, n + 64);
     }
     uint32_t r[32], ru[GATE ? 32 : 1];
     Pair v[16];
@@ -307,11 +324,14 @@ __device__ __forceinline__ void wide_epilogue(const Q8Params& p, WideSmem<T>& s,
         v[2 * j + 1] = add2(v[2 * j + 1], pair(w.z, w.w));
       }
     }
-    if (add) {
+    if constexpr (!GATE) {
+      constexpr int V = Addend<T>::V;
+      if (add) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        v[j] = add2(v[j], pair(to_f32(res[GATE ? 0 : 2 * j / V].e[2 * j % V]),
-                               to_f32(res[GATE ? 0 : 2 * j / V].e[2 * j % V + 1])));
+        for (int j = 0; j < 16; ++j)
+          v[j] = add2(v[j], pair(to_f32(now.w[2 * j / V].e[2 * j % V]),
+                                 to_f32(now.w[2 * j / V].e[2 * j % V + 1])));
+      }
     }
     if (some) store_block<T>(p, v, m_base, lane, n, aligned, s.turn[warp]);
     __syncwarp();
@@ -467,12 +487,17 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const Item next = item_of<GATE>(p, i + pairs);
         ahead = look_ahead<GATE>(p, next, next.m0 + int(rank) * kRows, warp, lane);
       }
+      Addend<T> addend;  // of the first block, on its way while the MMAs run
+      if constexpr (!GATE)
+        if (p.res)
+          load_addend(addend, p, it.m0 + int(rank) * kRows + (warp & 3) * 32 + lane,
+                      it.n0 + (warp >> 2) * 32);
       if (!gemm_wait_all(s.abort_flag, &s.acc_full[b], u & 1, p.err)) break;
       tc_fence_after();
       const uint32_t empty0 = cluster_map(smem_u32(&s.acc_empty[b]), 0);
       // TMEM loads are ordered by the fence in front of the arrival; nothing else is guarded by it
       wide_epilogue<T, GATE>(p, s, tmem + uint32_t(b * kWidth), it, it.m0 + int(rank) * kRows, now,
-                             warp, lane, [&] {
+                             addend, warp, lane, [&] {
                                if (lane == 0) mbar_arrive_cluster_relaxed(empty0);
                              });
     }

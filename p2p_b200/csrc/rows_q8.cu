@@ -322,7 +322,7 @@ __device__ __forceinline__ void keep_words(Piece<T>& x) {
 // A row in the registers of a warp (warps 1: a row a warp) or of a block of `warps` warps, NP pieces a
 // lane.
 template <class T, int NP, bool NORM, bool WIDE>
-__global__ void __launch_bounds__(32 * kMostWarps)
+__global__ void __launch_bounds__(32 * kMostWarps, NP <= 4 ? 3 : 1)
     rows_kernel(const __grid_constant__ RowsQ8Args a, int warps) {
   __shared__ RowSums part[kMostWarps];
   __shared__ uint4 turns[WIDE ? 1 : kMostWarps][32];
