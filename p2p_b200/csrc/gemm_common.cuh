@@ -37,22 +37,25 @@ __device__ __forceinline__ bool gemm_wait_warp(volatile int& abort_flag, uint64_
   return __shfl_sync(0xffffffffu, r ? 1 : 0, 0) != 0;
 }
 
-// A wait of a whole warp, every lane polling: the clock and the abort flag are looked at once in 64 polls
-// only (a poll of one lane with a reading of the clock each, then a shuffle, took 1 us longer over the 16
-// stages of a small product).
+// A wait of a whole warp, every lane polling, with one verdict for all of them: the clock and the abort
+// flag are looked at once in 64 polls only (a poll of one lane with a reading of the clock each, then a
+// shuffle, took 1 us longer over the 16 stages of a small product).
 __device__ __forceinline__ bool gemm_wait_all(volatile int& abort_flag, uint64_t* bar,
                                               uint32_t parity, int32_t* err) {
   uint64_t t0 = 0;
-  for (uint32_t n = 1; !sm100::mbar_try_wait(bar, parity); ++n) {
+  for (uint32_t n = 1; !__all_sync(0xffffffffu, sm100::mbar_try_wait(bar, parity)); ++n) {
     if (n % 64) continue;
-    if (abort_flag) return false;
     const uint64_t now = sm100::globaltimer_ns();
     if (!t0) t0 = now;
-    if (now - t0 > kGemmWaitNs) {
-      abort_flag = 1;
-      atomicOr(err, kErrTimeout);
+    const bool late = now - t0 > kGemmWaitNs;
+    if (__any_sync(0xffffffffu, late)) {
+      if (!abort_flag) {
+        abort_flag = 1;
+        atomicOr(err, kErrTimeout);
+      }
       return false;
     }
+    if (__any_sync(0xffffffffu, abort_flag != 0)) return false;
   }
   return true;
 }

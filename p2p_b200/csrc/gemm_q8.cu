@@ -624,7 +624,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     bool ok = true;
     for (int t = first; t < p.items && ok; t += step) {
       const int n0 = t % p.tiles_n * p.rows, m0 = t / p.tiles_n * p.tokens;
-      // each CTA begins at another part of k: all of them read the same tokens
+      // each CTA begins at another part of k, since all of them read the same tokens (gate and up of one
+      // token, 2 x 8192 x 2048: 6.6 us, 6.9 with all of them at the same part)
       int kt = k0 + first % (k1 - k0);
       for (int i = k0; i < k1; ++i) {
         if (round > 0 && !(ok = gemm_wait_all(s.abort_flag, &s.empty[st], (round - 1) & 1, p.err)))
