@@ -160,8 +160,8 @@ def test_read_outside_the_table(ctx):
 # ---- norm -----------------------------------------------------------------------------------------
 def norm_error(k):
     """Relative error of y: half of the sum of squares' (each thread adds at most 32 values, or
-    k / 256 of a long row, then 5 + 8 sums; a square, a division, an addition), a root, a division,
-    two products."""
+    k / 256 of a long row, then 5 + 4 sums; a square, the mean with eps: 16 in all with some to
+    spare), an inverse root (2^-22.9, 2.2 units), two products."""
     return ((max(32, k / 256 + 16) + 16) / 2 + 5) * U
 
 
