@@ -630,16 +630,17 @@ class Context:
     # -- 8-bit rows: the layer around its attention ----------------------------------------------
     # The argument structures of these calls are packed with struct: building them field by field and
     # converting each argument takes longer than the smallest of the kernels.
-    def _values(self, t: torch.Tensor, name: str, dtype, rows: int, cols: int) -> int:
+    def _values(self, t: torch.Tensor, name: str, dtype, rows: int, cols: int) -> tuple:
         """Checks f16 or f32 rows (of `dtype` where given) [rows][cols] (-1: any) and returns their
-        row stride."""
+        row stride, rows, columns and C type."""
         shape, dt = t.shape, t.dtype
-        if (dt is dtype or dtype is None and dt in _ROW_TYPES) and \
+        code = _ROW_TYPES.get(dt)
+        if code is not None and (dtype is None or dt is dtype) and \
                 t.get_device() == self.device and len(shape) == 2:
             m, k = shape
             ld, one = t.stride()
             if (rows < 0 or m == rows) and (cols < 0 or k == cols) and (one == 1 or k <= 1):
-                return ld if m > 1 else k
+                return ld if m > 1 else k, m, k, code
         _refuse(f"{name}: {dtype or 'f16 or f32'} [{rows if rows >= 0 else 'rows'}]"
                 f"[{cols if cols >= 0 else 'cols'}] on device {self.device} needed, "
                 f"got {tuple(shape)} {dt} on {t.device}")
@@ -672,15 +673,14 @@ class Context:
                          scale: Optional[torch.Tensor] = None, stream=None):
         """f16 or f32 rows [rows][cols] -> int8 rows and a scale for each (p2p_quantize_rows_q8):
         (q, scale).  A weight's rows are its output channels."""
-        ld = self._values(src, "src", None, -1, -1)
-        m, k = src.shape
+        ld, m, k, code = self._values(src, "src", None, -1, -1)
         if q is None or scale is None:
             q, scale = self._new_q8(q, scale, m, k, src.device)
         d = self._q8(q, scale, "q")
         if d[3] != m or d[4] != k:
             _refuse(f"q: [{m}][{k}] needed, got {tuple(q.shape)}")
         st = lib.p2p_quantize_rows_q8(
-            self.h, _QUANTIZE_ROWS(src.data_ptr(), ld, *d, _ROW_TYPES[src.dtype]),
+            self.h, _QUANTIZE_ROWS(src.data_ptr(), ld, *d, code),
             self._stream(stream))
         if st:
             self._chk(st)
@@ -692,12 +692,12 @@ class Context:
         out [rows][cols] (f16 or f32): the embedding lookup (p2p_read_rows_q8).  index -1 gives
         zeros."""
         s = self._q8(q, scale, "q")
-        ld, n = self._values(out, "out", None, -1, s[4]), out.shape[0]
+        ld, n, _, code = self._values(out, "out", None, -1, s[4])
         if factor == 0:
             _refuse("factor: 0")
         st = lib.p2p_read_rows_q8(
             self.h, _READ_ROWS(*s, 0 if index is None else self._ints(index, n, "index"),
-                               out.data_ptr(), ld, n, _ROW_TYPES[out.dtype], factor),
+                               out.data_ptr(), ld, n, code, factor),
             self._stream(stream))
         if st:
             self._chk(st)
@@ -711,20 +711,19 @@ class Context:
         """Residual addition and RMS norm (p2p_add_norm_q8): sum_out = x + residual (may be
         either of them), y the normed rows, (q, scale) their int8 rows; returns (q, scale)."""
         dt = x.dtype
-        ld_x = self._values(x, "x", None, -1, -1)
-        m, k = x.shape
+        ld_x, m, k, code = self._values(x, "x", None, -1, -1)
         r_at = w_at = s_at = y_at = ld_r = ld_s = ld_y = 0
         if residual is not None:
-            r_at, ld_r = residual.data_ptr(), self._values(residual, "residual", dt, m, k)
+            r_at, ld_r = residual.data_ptr(), self._values(residual, "residual", dt, m, k)[0]
         if weight is not None:
             if weight.dtype is not torch.float16 or weight.get_device() != self.device or \
                     weight.numel() != k or not weight.is_contiguous():
                 _refuse(f"weight: {k} contiguous f16 values on device {self.device} needed")
             w_at = weight.data_ptr()
         if sum_out is not None:
-            s_at, ld_s = sum_out.data_ptr(), self._values(sum_out, "sum_out", dt, m, k)
+            s_at, ld_s = sum_out.data_ptr(), self._values(sum_out, "sum_out", dt, m, k)[0]
         if y is not None:
-            y_at, ld_y = y.data_ptr(), self._values(y, "y", dt, m, k)
+            y_at, ld_y = y.data_ptr(), self._values(y, "y", dt, m, k)[0]
         if q is None or scale is None:
             q, scale = self._new_q8(q, scale, m, k, x.device)
         d = self._q8(q, scale, "q")
@@ -732,7 +731,7 @@ class Context:
             _refuse(f"q: [{m}][{k}] needed, got {tuple(q.shape)}")
         st = lib.p2p_add_norm_q8(
             self.h, _ADD_NORM(x.data_ptr(), r_at, w_at, s_at, y_at, ld_x, ld_r, ld_s, ld_y, *d,
-                              _ROW_TYPES[dt], eps), self._stream(stream))
+                              code, eps), self._stream(stream))
         if st:
             self._chk(st)
         return q, scale
@@ -743,14 +742,14 @@ class Context:
         """y = x . w^T of int8 rows x [M][K] and w = (codes [N][K], scales), times both scales,
         plus bias [N] (f32) and residual [M][N] (may be y), into y (f16 or f32; p2p_gemm_q8)."""
         wr, xr = self._q8(w[0], w[1], "w"), self._q8(x, x_scale, "x")
-        m, n, dt = xr[3], wr[3], y.dtype
-        ld_y = self._values(y, "y", None, m, n)
+        m, n = xr[3], wr[3]
+        ld_y, _, _, code = self._values(y, "y", None, m, n)
         r_at = ld_r = 0
         if residual is not None:
-            r_at, ld_r = residual.data_ptr(), self._values(residual, "residual", dt, m, n)
+            r_at, ld_r = residual.data_ptr(), self._values(residual, "residual", y.dtype, m, n)[0]
         st = lib.p2p_gemm_q8(
             self.h, _PRODUCT(*wr, *xr, 0 if bias is None else self._floats(bias, n, "bias"), r_at,
-                             y.data_ptr(), ld_r, ld_y, _ROW_TYPES[dt]), self._stream(stream))
+                             y.data_ptr(), ld_r, ld_y, code), self._stream(stream))
         if st:
             self._chk(st)
 
@@ -762,7 +761,7 @@ class Context:
         xr = self._q8(x, x_scale, "x")
         if act not in _ACTS:
             _refuse(f"act: one of {sorted(_ACTS)} needed, got {act!r}")
-        ld_h = self._values(h, "h", torch.float16, xr[3], gr[3])
+        ld_h = self._values(h, "h", torch.float16, xr[3], gr[3])[0]
         st = lib.p2p_gate_q8(self.h, _GATED(*gr, *ur, *xr, h.data_ptr(), ld_h, _ACTS[act]),
                              self._stream(stream))
         if st:
