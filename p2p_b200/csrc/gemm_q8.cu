@@ -549,6 +549,10 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
 __host__ __device__ inline int split_tokens(int tokens, int split) {
   return ((tokens + split - 1) / split + 3) / 4 * 4;
 }
+// TMEM is allocated in powers of two.
+__host__ __device__ inline uint32_t tmem_columns(uint32_t need) {
+  return need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
+}
 
 template <class T, bool GATE, bool SPLIT>
 __global__ void __launch_bounds__(kNarrowThreads, 1)
@@ -576,7 +580,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
   const int k0 = SPLIT ? nk * rank / split : 0, k1 = SPLIT ? nk * (rank + 1) / split : nk;
   const uint32_t acc_cols = G * p.tokens;  // of one accumulator buffer
   const uint32_t need = SPLIT ? acc_cols : 2 * acc_cols;
-  const uint32_t tmem_cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
+  const uint32_t tmem_cols = tmem_columns(need);
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&s.full[i], 1);
@@ -896,6 +900,21 @@ cudaError_t launch_cluster(const void* fn, int64_t ctas, int threads, size_t sme
   return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
+// Tiles of wide_kernel: the last wave's are halved where their halves still fit one wave.
+struct WideItems {
+  int64_t tiles_n, tiles, whole, items;
+};
+WideItems wide_items(int m, int n, int G, int pairs) {
+  const int cols = kWidth / G;
+  WideItems w;
+  w.tiles_n = (int64_t(n) + cols - 1) / cols;
+  w.tiles = w.tiles_n * ((int64_t(m) + 2 * kRows - 1) / (2 * kRows));
+  const int64_t rest = w.tiles % pairs;
+  w.whole = 2 * rest <= pairs ? w.tiles - rest : w.tiles;
+  w.items = w.whole + 2 * (w.tiles - w.whole);
+  return w;
+}
+
 template <class T, bool GATE>
 cudaError_t launch_wide(Q8Params p, const GemmQ8Args& a, int num_sms, cudaStream_t stream) {
   CUtensorMap tx, tw, tu;
@@ -925,15 +944,11 @@ cudaError_t launch_wide(Q8Params p, const GemmQ8Args& a, int num_sms, cudaStream
   }, &max_pairs);
   if (e != cudaSuccess) return e;
   if (max_pairs <= 0) return cudaErrorInvalidConfiguration;
-  constexpr int kCols = GATE ? kWidth / 2 : kWidth;
-  const int64_t tiles_n = (int64_t(p.n) + kCols - 1) / kCols;
-  const int64_t tiles = tiles_n * ((int64_t(p.m) + 2 * kRows - 1) / (2 * kRows));
-  if (2 * tiles > INT32_MAX) return cudaErrorInvalidValue;
-  // the last wave's tiles are halved where their halves still fit one wave
-  const int64_t rest = tiles % max_pairs;
-  p.tiles_n = int32_t(tiles_n);
-  p.whole = int32_t(2 * rest <= max_pairs ? tiles - rest : tiles);
-  p.items = int32_t(p.whole + 2 * (tiles - p.whole));
+  const WideItems w = wide_items(p.m, p.n, GATE ? 2 : 1, max_pairs);
+  if (2 * w.tiles > INT32_MAX) return cudaErrorInvalidValue;
+  p.tiles_n = int32_t(w.tiles_n);
+  p.whole = int32_t(w.whole);
+  p.items = int32_t(w.items);
   void* args[] = {&tx, &tw, &tu, &p};
   return launch_cluster(fn, 2 * std::min<int64_t>(p.items, max_pairs), kWideThreads, smem, 2, args,
                         stream);
@@ -1020,6 +1035,40 @@ double wide_cost(int m, int n, int k, int G, int num_sms) {
   return 4000 + nk * (512 * whole + (rest && 2 * rest <= pairs ? 305 : 0));
 }
 
+// What a CTA of that plan takes of its SM.
+struct NarrowRoom {
+  int stages;  // of the ring
+  int smem;    // bytes of shared memory asked for
+  int cols;    // of TMEM
+};
+constexpr int kSmemOfSm = 228 * 1024, kKeptOfCta = 1024, kTmemOfSm = 512;  // (kept for the system)
+constexpr int kSplitSmem = 48 * 1024;  // a split CTA's at least
+// The CTAs of a cluster wait for one another, without a bound, and an allocation of TMEM waits for whoever
+// holds the columns.  So the CTAs of clusters that fit on one SM by their shared memory, of any calls on any
+// streams, must find their columns there: a split CTA asks for at least its columns' share of the SM's
+// shared memory (56 KB and the 1 KB kept of each CTA for 128 columns, 113 for 256), and for more than a pair
+// form's CTA, which takes all columns, leaves of it.  (An unsplit CTA waits for nobody that waits for it.)
+NarrowRoom narrow_room(const NarrowPlan& plan, int G, int64_t tiles, int num_sms) {
+  const bool split = plan.split > 1;
+  const int own = split_tokens(plan.tokens, plan.split);
+  const int stage = (G * plan.rows + plan.tokens) * kStep * plan.chunks;
+  const int sums = split ? (plan.split * G * plan.rows * (own + 4) * 4 + 1023) / 1024 * 1024
+                         : kNarrowEpi * kMostTokens * 4;
+  // behind the ring, what the last stage's MMA reads beyond its rows
+  const int fixed = 2048 + sums + (plan.rows <= 64 ? 64 : 128) * kStep;
+  const int64_t steps = split ? (plan.steps + plan.split - 1) / plan.split
+                              : plan.steps * ((tiles + num_sms - 1) / num_sms);
+  NarrowRoom r;
+  r.stages = int(std::min<int64_t>({kMostStages, steps, (kNarrowSmem - fixed) / stage}));
+  r.cols = int(tmem_columns((split ? 1 : 2) * G * plan.tokens));
+  r.smem = fixed + r.stages * stage;
+  if (split) r.smem = std::max({r.smem, kSplitSmem, r.cols * (kSmemOfSm / kTmemOfSm) - kKeptOfCta});
+  return r;
+}
+static_assert(sizeof(WideSmem<__half>) + kSplitSmem > kSmemOfSm &&
+                  sizeof(WideSmem<float>) + kSplitSmem > kSmemOfSm,
+              "no split CTA beside a pair form's");
+
 template <class T, bool GATE, bool SPLIT>
 cudaError_t launch_narrow(Q8Params p, const GemmQ8Args& a, const NarrowPlan& plan, int num_sms,
                           cudaStream_t stream) {
@@ -1038,20 +1087,8 @@ cudaError_t launch_narrow(Q8Params p, const GemmQ8Args& a, const NarrowPlan& pla
   const int64_t tiles = int64_t(p.tiles_n) * ((int64_t(p.m) + plan.tokens - 1) / plan.tokens);
   if (tiles * plan.split > INT32_MAX) return cudaErrorInvalidValue;
   p.items = int32_t(tiles);
-  const int own = split_tokens(plan.tokens, plan.split);
-  const int stage = (G * plan.rows + plan.tokens) * kStep * plan.chunks;
-  const int sums = SPLIT ? (plan.split * G * plan.rows * (own + 4) * 4 + 1023) / 1024 * 1024
-                         : kNarrowEpi * kMostTokens * 4;
-  // behind the ring, what the last stage's MMA reads beyond its rows
-  const int fixed = 2048 + sums + (plan.rows <= 64 ? 64 : 128) * kStep;
-  const int64_t steps = SPLIT ? (plan.steps + plan.split - 1) / plan.split
-                              : plan.steps * ((tiles + num_sms - 1) / num_sms);
-  p.stages = int(std::min<int64_t>({kMostStages, steps, (kNarrowSmem - fixed) / stage}));
-  size_t smem = size_t(fixed) + size_t(p.stages) * stage;
-  // The CTAs of a cluster wait for one another, and an allocation of TMEM waits for whoever holds it: so
-  // never more of them on an SM than its 512 columns serve (at most 4 with up to 128 columns, 2 with 256),
-  // and none beside a pair form's CTA, which takes all columns and over 190 KB of shared memory.
-  if (SPLIT) smem = std::max<size_t>(smem, (G * plan.tokens > 128 ? 78 : 48) * 1024);
+  const NarrowRoom need = narrow_room(plan, G, tiles, num_sms);
+  p.stages = need.stages;
   const void* fn = reinterpret_cast<const void*>(&narrow_kernel<T, GATE, SPLIT>);
   static PerDeviceOnce attrs;
   cudaError_t e = per_device_once(attrs, [&](int&) {
@@ -1060,24 +1097,38 @@ cudaError_t launch_narrow(Q8Params p, const GemmQ8Args& a, const NarrowPlan& pla
   if (e != cudaSuccess) return e;
   void* args[] = {&tx, &tw, &tu, &p};
   return launch_cluster(fn, SPLIT ? tiles * plan.split : std::min<int64_t>(tiles, num_sms),
-                        kNarrowThreads, smem, plan.split, args, stream);
+                        kNarrowThreads, size_t(need.smem), plan.split, args, stream);
 }
 
 bool on16(const void* p, int64_t pitch_bytes) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch_bytes % 16 == 0;
 }
 
+// Which of the two kernels, and how.
+struct Choice {
+  bool wide;
+  NarrowPlan plan;
+};
+Choice choose(int m, int n, int k, int G, int num_sms, int room) {
+  Choice c{m > kMostNarrow, {}};
+  if (c.wide) return c;
+  c.plan = narrow_plan(m, n, k, G, num_sms, room);
+  c.wide = m > kMostTokens && c.plan.cost > wide_cost(m, n, k, G, num_sms);
+  return c;
+}
+
 template <class T, bool GATE>
 cudaError_t launch_q8(const Q8Params& p, const GemmQ8Args& a, int num_sms, cudaStream_t s) {
   constexpr int G = GATE ? 2 : 1;
-  if (p.m > kMostNarrow) return launch_wide<T, GATE>(p, a, num_sms, s);
   int room = 0;
-  const cudaError_t e = cluster_room(&room);
-  if (e != cudaSuccess) return e;
-  const NarrowPlan plan = narrow_plan(p.m, p.n, p.k, G, num_sms, room);
-  if (p.m > kMostTokens && plan.cost > wide_cost(p.m, p.n, p.k, G, num_sms)) return launch_wide<T, GATE>(p, a, num_sms, s);
-  return plan.split > 1 ? launch_narrow<T, GATE, true>(p, a, plan, num_sms, s)
-                        : launch_narrow<T, GATE, false>(p, a, plan, num_sms, s);
+  if (p.m <= kMostNarrow) {
+    const cudaError_t e = cluster_room(&room);
+    if (e != cudaSuccess) return e;
+  }
+  const Choice c = choose(p.m, p.n, p.k, G, num_sms, room);
+  if (c.wide) return launch_wide<T, GATE>(p, a, num_sms, s);
+  return c.plan.split > 1 ? launch_narrow<T, GATE, true>(p, a, c.plan, num_sms, s)
+                          : launch_narrow<T, GATE, false>(p, a, c.plan, num_sms, s);
 }
 
 }  // namespace

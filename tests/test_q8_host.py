@@ -247,3 +247,53 @@ def test_python_refusals():
                  lambda: ctx.gate_q8((q, s), (q, s), q, s, f)):
         with pytest.raises(p2p_b200.P2PError):  # nothing of this is on a device
             call()
+
+
+# ---- how products are cut up --------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    """plan(m, n, k, gate): what gemm_q8.cu makes of a call on 148 SMs that run 74, 35 and 15 clusters of 2, 4
+    and 8 CTAs at once (or those of `room`)."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("p2p_build", ROOT / "p2p_b200" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    so = tmp_path_factory.mktemp("q8_plan") / "q8_plan_host.so"
+    subprocess.run([build.nvcc(), *build.ARCH, *build.NVCC_FLAGS, "-shared", "-cudart", "static",
+                    str(ROOT / "tests" / "q8_plan_host.cu"), "-o", str(so)], check=True,
+                   capture_output=True)
+    lib = C.CDLL(str(so))
+
+    def call(m, n, k, gate=False, room=(74, 35, 15)):
+        o = (C.c_int64 * 10)()
+        lib.host_plan(m, n, k, int(gate), 148, sum(r << (8 * i) for i, r in enumerate(room)), o)
+        if o[0]:
+            return {"kernel": "wide", "whole": o[1], "items": o[2]}
+        names = ("rows", "tokens", "split", "chunks", "steps", "tiles", "stages", "smem", "cols")
+        return {"kernel": "narrow", **dict(zip(names, o[1:]))}
+    return call
+
+
+def shapes(count):
+    import random
+    rng = random.Random(1)
+    for _ in range(count):
+        yield (int(2**rng.uniform(0, 11.1)), int(2**rng.uniform(0, 17)), int(2**rng.uniform(0, 16)),
+               rng.random() < 0.5, rng.choice([(74, 35, 15), (74, 36, 16), (60, 20, 7), (1, 1, 1)]))
+
+
+def test_split_ctas_find_their_tensor_memory(plan):
+    """CTAs of a cluster wait for one another: whatever of them fits on an SM by its 228 KB of shared memory
+    (1 KB of it kept of each) has to fit into its 512 columns too."""
+    seen = set()
+    for m, n, k, gate, room in ((128, 512, 512, True, (74, 35, 15)), (64, 256, 512, False, (74, 35, 15)),
+                                *shapes(4000)):
+        p = plan(m, n, k, gate, room)
+        if p["kernel"] == "wide":
+            continue
+        assert 1 <= p["stages"] <= 24 and p["smem"] <= 227 * 1024 and p["cols"] <= 512
+        if p["split"] > 1:
+            seen.add(p["cols"])
+            assert (p["smem"] + 1024) * 512 >= p["cols"] * 228 * 1024, (m, n, k, gate, p)
+            assert p["smem"] >= 48 * 1024  # none beside a pair form's CTA
+    assert seen == {32, 64, 128, 256}
