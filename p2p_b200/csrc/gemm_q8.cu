@@ -994,11 +994,15 @@ cudaError_t cluster_room(int* room) {
 NarrowPlan narrow_plan(int m, int n, int k, int G, int num_sms, int room) {
   constexpr float kLoad = 50, kDram = 23, kWait = 150, kIssue = 37, kHandOver = 260;
   constexpr int kMostChunks = 4, kMostStage = 64 * 1024;
-  const int tokens = std::min(kMostTokens, m <= 24 ? (m + 7) / 8 * 8 : (m + 15) / 16 * 16);
-  const int token_tiles = (m + tokens - 1) / tokens, nk = (k + kStep - 1) / kStep;
-  const float mma = 4.f * G * tokens / 2.f, sms = float(num_sms);
+  // the MMA's columns: 8 or a multiple of 16; of 64 rows also 24 (which not every list of kind::i8's shapes
+  // has, and with 128 rows nothing needs: 24 x 65536 x 2048 takes 64)
+  const int fewest = std::min(kMostTokens, m <= 24 ? (m + 7) / 8 * 8 : (m + 15) / 16 * 16);
+  const int token_tiles = (m + fewest - 1) / fewest, nk = (k + kStep - 1) / kStep;
+  const float sms = float(num_sms);
   NarrowPlan best{};
   for (int rows = 8; rows <= 128; rows += 8) {
+    const int tokens = rows > 64 && fewest > 8 ? (fewest + 15) / 16 * 16 : fewest;
+    const float mma = 4.f * G * tokens / 2.f;
     const int64_t tiles = (int64_t(n) + rows - 1) / rows * token_tiles;
     const float all = (G * rows + tokens) * kStep / kLoad, weights = float(G * rows * kStep);
     for (int split = 1, i = 0; split <= std::min(kMostSplit, nk); split *= 2, ++i) {

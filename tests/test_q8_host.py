@@ -297,3 +297,16 @@ def test_split_ctas_find_their_tensor_memory(plan):
             assert (p["smem"] + 1024) * 512 >= p["cols"] * 228 * 1024, (m, n, k, gate, p)
             assert p["smem"] >= 48 * 1024  # none beside a pair form's CTA
     assert seen == {32, 64, 128, 256}
+
+
+def test_products_take_known_instruction_shapes(plan):
+    """Integer MMAs of 8 columns or a multiple of 16 (of 64 rows, 24 too), over whole swizzle atoms of rows."""
+    for m in range(1, 131):
+        for n, k, gate in ((65536, 2048, False), (20000, 512, False), (2048, 2048, False),
+                           (30000, 300, True), (8192, 2048, True), (100, 77, True)):
+            p = plan(m, n, k, gate)
+            if p["kernel"] == "narrow":
+                t = p["tokens"]
+                assert t == 8 or t % 16 == 0 or (t == 24 and p["rows"] <= 64), (m, n, k, gate, p)
+                assert min(m, 128) <= t <= 128
+                assert p["rows"] % 8 == 0 and 8 <= p["rows"] <= 128
