@@ -15,6 +15,7 @@ pytestmark = pytest.mark.gpu
 U = 2.0**-24
 HALF = {torch.float16: 2.0**-11, torch.float32: U}
 F16, F32 = torch.float16, torch.float32
+F16_ZERO = torch.zeros((), dtype=F16)
 
 
 @pytest.fixture(scope="module")
@@ -109,6 +110,31 @@ def test_quantize_rows_of_every_kind(ctx, dt, k):
     else:
         check_codes(q[4:5], s[4:5], x[4:5].double(), 0)
     check_codes(q[[5, 7, 8]], s[[5, 7, 8]], x[[5, 7, 8]].double(), 0)
+
+
+@pytest.mark.parametrize("at_once,pad", [(300, 0), (4096, 0), (4096, 7), (16384, 0)])
+@pytest.mark.parametrize("top", ["subnormal", 2.0**-14, 1.0, 2.0**15])
+def test_quantize_ties_of_f16(ctx, top, at_once, pad):
+    """Every f16 significand as a row's largest value, against every f16 value up to it, of both signs: the
+    codes are 127 v / a rounded to even, ties too.  (In 64 bits the quotient is exact at a tie, and no other
+    one lies within 2^-20 of a half.)"""
+    low = 0 if top == "subnormal" else torch.tensor(top, dtype=F16).view(torch.int16).item()
+    largest = torch.arange(low, low + 1024, device="cuda", dtype=torch.int16).view(F16)
+    largest = largest[largest > 0] if low == 0 else largest  # a row of zeros is another test's
+    ties = 0
+    for first in range(0, low + 1024, at_once):
+        v = torch.arange(first, min(first + at_once, low + 1024), device="cuda",
+                         dtype=torch.int16).view(F16)
+        a = largest[:, None]
+        v = torch.where(v <= a, v, F16_ZERO.to("cuda"))
+        whole = torch.zeros(len(largest), 1 + 2 * v.shape[1] + pad, device="cuda", dtype=F16)
+        x = whole[:, :1 + 2 * v.shape[1]]
+        x[:, :1], x[:, 1::2], x[:, 2::2] = a, v, -v
+        q, s = ctx.quantize_rows_q8(x)
+        want = 127 * x.double() / a.double()
+        ties += ((want - want.floor()) == 0.5).sum().item()
+        assert torch.equal(q.double(), torch.round(want))
+    assert ties > 0
 
 
 # ---- codes -> values ------------------------------------------------------------------------------
@@ -263,6 +289,42 @@ def test_norm_rows_of_every_kind(ctx, dt, k):
     check_norm(x[good], r[good], w, 1e-5, dt, q[good], s[good], total[good], y[good])
 
 
+# ---- what lies around the rows ------------------------------------------------------------------------
+def framed(m, k, dt, pad, off):
+    """Rows of nines inside a buffer of nines: `off` values in front, `pad` between two rows, some behind."""
+    buf = torch.full((off + m * (k + pad) + 40,), 9.0, device="cuda", dtype=dt)
+    return buf, buf[off:off + m * (k + pad)].view(m, k + pad)[:, :k]
+
+
+def only_rows_written(buf, rows):
+    outside = buf.clone()
+    outside.as_strided(rows.shape, rows.stride(), rows.storage_offset()).fill_(9.0)
+    return bool((outside == 9).all())
+
+
+@pytest.mark.parametrize("dt", [F16, F32])
+@pytest.mark.parametrize("pad,off", [(0, 0), (1, 1), (8, 8), (3, 0)])
+@pytest.mark.parametrize("m,k", [(1, 1), (5, 7), (9, 128), (33, 250), (7, 257), (40, 512), (6, 520), (11, 1003),
+                                 (5, 2048), (3, 5001), (3, 20001)])
+def test_nothing_around_the_rows_is_written(ctx, dt, m, k, pad, off):
+    """Outputs of any pitch and start: their rows, the same as of rows on 16-byte boundaries, and nothing in
+    front of, between and behind them."""
+    g = gen(m + k)
+    x, r, w = rows_in(g, m, k, dt), rows_in(g, m, k, dt), torch.ones(k, device="cuda", dtype=F16)
+    (sums, total), (ys, y) = framed(m, k, dt, pad, off), framed(m, k, dt, pad, off)
+    q, s = ctx.add_norm_q8(x, w, residual=r, sum_out=total, y=y)
+    check_norm(x, r, w, 1e-5, dt, q, s, total, y)
+    assert only_rows_written(sums, total) and only_rows_written(ys, y)
+    outs, out = framed(m, k, dt, pad, off)
+    straight = torch.zeros(m, (k + 7) // 8 * 8, device="cuda", dtype=dt)[:, :k]
+    ctx.read_rows_q8(q, s, out)
+    ctx.read_rows_q8(q, s, straight)
+    assert only_rows_written(outs, out) and torch.equal(out, straight)
+    outs.fill_(9)
+    ctx.read_rows_q8(q, s, out, index=torch.arange(m, device="cuda", dtype=torch.int32).flip(0))
+    assert only_rows_written(outs, out) and torch.equal(out, straight.flip(0))
+
+
 # ---- products -------------------------------------------------------------------------------------
 def product(x, xs, w, ws):
     return (x.double() @ w.double().T) * xs.double()[:, None] * ws.double()
@@ -307,6 +369,46 @@ def test_gemm(ctx, m, n, k, dt, bias, residual):
         y2.copy_(r)
         ctx.gemm_q8((w, ws), x, xs, y2, bias=b, residual=y2)
         assert torch.equal(y2, y)
+
+
+# Calls whose CTAs (or pairs of them) take several tiles each: a ring and two accumulators that run on across
+# tiles, tokens' scales that change with the tile, MMAs of 128 rows (tests/test_q8_host.py holds which sizes
+# reach what).
+MANY_TILES = [(1, 32001, 256), (7, 65536, 130), (8, 65536, 128), (16, 40001, 700), (20, 20000, 512),
+              (24, 65536, 256), (24, 65536, 2048), (32, 50000, 2048), (32, 40007, 333), (100, 20000, 256),
+              (128, 20001, 257), (300, 20000, 128), (260, 50000, 64), (2304, 5000, 256), (2500, 5003, 128)]
+MANY_GATED = [(1, 30000, 256), (8, 50000, 300), (17, 20003, 128), (33, 20000, 2048), (40, 20000, 512),
+              (128, 20007, 256), (600, 9000, 256), (2300, 3000, 200)]
+
+
+@pytest.mark.parametrize("m,n,k", MANY_TILES)
+@pytest.mark.parametrize("dt,bias,residual", [(F32, False, False), (F16, True, True)])
+def test_gemm_of_many_tiles(ctx, m, n, k, dt, bias, residual):
+    g = gen(m + 3 * n + 5 * k)
+    x, xs = codes(g, m, k, 16)
+    w, ws = codes(g, n, k, 32)
+    b = torch.randn(n, generator=g, device="cuda") if bias else None
+    r = rows_in(g, m, n, dt, 3) if residual else None
+    whole = torch.full((m + 1, n + 8), 7.0, device="cuda", dtype=dt)
+    y = whole[:m, :n]
+    ctx.gemm_q8((w, ws), x, xs, y, bias=b, residual=r)
+    check_gemm(y, x, xs, w, ws, b, r, dt)
+    assert (whole[m:] == 7).all() and (whole[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("m,n,k", MANY_GATED)
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gate_of_many_tiles(ctx, m, n, k, act):
+    g = gen(m + 3 * n + 5 * k)
+    x, xs = codes(g, m, k, 16)
+    (wg, gs), (wu, us) = codes(g, n, k, 32), codes(g, n, k)
+    amp = 40 / (74 * 74 * math.sqrt(k) / 10000)  # outputs of both signs, from far below to far above 1
+    gs, us = gs * amp * torch.rand(n, generator=g, device="cuda"), us * amp / 20
+    whole = torch.full((m + 1, n + 8), 7.0, device="cuda", dtype=F16)
+    h = whole[:m, :n]
+    ctx.gate_q8((wg, gs), (wu, us), x, xs, h, act=act)
+    check_gate(h, x, xs, wg, gs, wu, us, act)
+    assert (whole[m:] == 7).all() and (whole[:, n:] == 7).all()
 
 
 @pytest.mark.parametrize("m", [1, 20, 130, 600])

@@ -310,3 +310,23 @@ def test_products_take_known_instruction_shapes(plan):
                 assert t == 8 or t % 16 == 0 or (t == 24 and p["rows"] <= 64), (m, n, k, gate, p)
                 assert min(m, 128) <= t <= 128
                 assert p["rows"] % 8 == 0 and 8 <= p["rows"] <= 128
+
+
+def test_sizes_of_the_gpu_tests_reach_every_walk(plan):
+    """A CTA's second tile (other accumulator), its third (the first accumulator handed back), a ring that goes
+    round, MMAs of 64 and 128 rows, tiles of few and of many tokens, pairs of CTAs with three items, and
+    clusters: among the sizes that are compared on a GPU."""
+    import test_gpu_q8 as T
+    for gate, many in ((False, T.MANY_TILES), (True, T.MANY_GATED)):
+        plans = [plan(*c, gate) for c in many]
+        walks = [p for p in plans if p["kernel"] == "narrow" and p["split"] == 1 and p["tiles"] > 148]
+        assert any(p["tiles"] > 2 * 148 for p in walks)
+        assert any(p["stages"] < p["steps"] * (p["tiles"] // 148) for p in walks)
+        assert {8, 32, 128} <= {p["tokens"] for p in walks}
+        assert any(p["rows"] > 64 and p["tokens"] == 8 for p in walks)
+        assert any(p["items"] > 2 * 74 for p in plans if p["kernel"] == "wide")
+    assert any(p["rows"] <= 64 for p in (plan(*c) for c in T.MANY_TILES) if p.get("tiles", 0) > 2 * 148)
+    for gate in (False, True):
+        few = [plan(*c, gate) for c in T.SIZES]
+        assert {2, 4, 8} <= {p["split"] for p in few if p["kernel"] == "narrow"}
+        assert any(p["items"] < 74 for p in few if p["kernel"] == "wide")
