@@ -120,6 +120,16 @@ def _params_ref(*fields):
     return C.byref(Params(*fields).c())
 
 
+def _empty(shape, dtype: torch.dtype, device, stream) -> torch.Tensor:
+    """An output that the caller has not brought.  Its memory belongs to the stream that the call runs
+    on: memory of another one could be in use there still, and be given away before the call has
+    written it."""
+    if stream is None:  # the current one, the allocator's too
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 class Context:
     """One p2p_ctx: a CUDA device, its split-KV workspace and its meta buffer."""
 
@@ -661,21 +671,21 @@ class Context:
         _refuse(f"{name}: int8 [rows][cols], neighbouring codes of a row, on device {dev} needed, "
                 f"got {tuple(shape)} {q.dtype} on {q.device}, strides {q.stride()}")
 
-    def _new_q8(self, q, scale, rows: int, cols: int, device):
+    def _new_q8(self, q, scale, rows: int, cols: int, device, stream):
         """int8 rows on 16-byte boundaries and their scales, where the caller has none."""
         if q is None:
-            q = torch.empty((rows, (cols + 15) & -16), dtype=torch.int8, device=device)[:, :cols]
+            q = _empty((rows, (cols + 15) & -16), torch.int8, device, stream)[:, :cols]
         if scale is None:
-            scale = torch.empty(rows, dtype=torch.float32, device=device)
+            scale = _empty(rows, torch.float32, device, stream)
         return q, scale
 
     def quantize_rows_q8(self, src: torch.Tensor, q: Optional[torch.Tensor] = None,
                          scale: Optional[torch.Tensor] = None, stream=None):
         """f16 or f32 rows [rows][cols] -> int8 rows and a scale for each (p2p_quantize_rows_q8):
-        (q, scale).  A weight's rows are its output channels."""
+        (q, scale).  A weight's rows are its output channels.  What is not given is made on `stream`."""
         ld, m, k, code = self._values(src, "src", None, -1, -1)
         if q is None or scale is None:
-            q, scale = self._new_q8(q, scale, m, k, src.device)
+            q, scale = self._new_q8(q, scale, m, k, src.device, stream)
         d = self._q8(q, scale, "q")
         if d[3] != m or d[4] != k:
             _refuse(f"q: [{m}][{k}] needed, got {tuple(q.shape)}")
@@ -709,7 +719,8 @@ class Context:
                     sum_out: Optional[torch.Tensor] = None, y: Optional[torch.Tensor] = None,
                     eps: float = 1e-5, stream=None):
         """Residual addition and RMS norm (p2p_add_norm_q8): sum_out = x + residual (may be
-        either of them), y the normed rows, (q, scale) their int8 rows; returns (q, scale)."""
+        either of them), y the normed rows, (q, scale) their int8 rows; returns (q, scale).  What is
+        not given of them is made on `stream`."""
         dt = x.dtype
         ld_x, m, k, code = self._values(x, "x", None, -1, -1)
         r_at = w_at = s_at = y_at = ld_r = ld_s = ld_y = 0
@@ -725,7 +736,7 @@ class Context:
         if y is not None:
             y_at, ld_y = y.data_ptr(), self._values(y, "y", dt, m, k)[0]
         if q is None or scale is None:
-            q, scale = self._new_q8(q, scale, m, k, x.device)
+            q, scale = self._new_q8(q, scale, m, k, x.device, stream)
         d = self._q8(q, scale, "q")
         if d[3] != m or d[4] != k:
             _refuse(f"q: [{m}][{k}] needed, got {tuple(q.shape)}")

@@ -594,6 +594,25 @@ def test_two_streams_at_once(ctx):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("norm", [False, True])
+def test_outputs_that_a_call_makes_belong_to_its_stream(ctx, norm):
+    """Memory that the current stream still reads is not what a call on another stream writes."""
+    x = rows_in(gen(9), 300, 4096, F16)
+    want = ctx.add_norm_q8(x, None) if norm else ctx.quantize_rows_q8(x)
+    side = torch.cuda.Stream()
+    old, sums = torch.ones(300, 4096, dtype=torch.int8, device="cuda"), torch.ones(300, device="cuda")
+    torch.cuda.synchronize()
+    at = {t.untyped_storage().data_ptr() for t in (old, sums)}
+    torch.cuda._sleep(20000000)
+    copies = old.clone(), sums.clone()
+    del old, sums  # the allocator may give them away on this stream, whose copies have yet to run
+    q, s = ctx.add_norm_q8(x, None, stream=side) if norm else ctx.quantize_rows_q8(x, stream=side)
+    assert not at & {t.untyped_storage().data_ptr() for t in (q, s)}
+    torch.cuda.synchronize()
+    assert torch.equal(q, want[0]) and torch.equal(s, want[1])
+    assert all((c == 1).all() for c in copies)
+
+
 @pytest.mark.parametrize("m,n,k", [(8, 64, 1024), (8, 4000, 256), (2100, 700, 1000)])
 def test_a_wait_that_runs_out_is_a_status(ctx, m, n, k):
     """The first stage of every ring waits for bytes that never come: the call ends, nothing is stored,

@@ -249,6 +249,63 @@ def test_python_refusals():
             call()
 
 
+class Streams:
+    """Stands for the library and torch's streams: which stream was the allocator's at each torch.empty, and
+    the handle that each call got."""
+
+    def __init__(self, monkeypatch):
+        import contextlib
+        from p2p_b200 import attention as A
+        self.current, self.made, self.calls = None, [], []
+        empty = torch.empty
+
+        @contextlib.contextmanager
+        def stream(s):
+            before, self.current = self.current, s
+            yield
+            self.current = before
+
+        def recorded(*a, **kw):
+            self.made.append(self.current)
+            return empty(*a, **kw)
+        monkeypatch.setattr(torch.cuda, "stream", stream)
+        monkeypatch.setattr(torch, "empty", recorded)
+        monkeypatch.setattr(A, "lib", self)
+
+    def __getattr__(self, name):
+        def call(*a):
+            self.calls.append((name, a))
+            return 0
+        return call
+
+
+class Side:
+    cuda_stream = 77
+
+
+def host_context():
+    """A context whose device is that of CPU tensors."""
+    import p2p_b200
+    ctx = object.__new__(p2p_b200.Context)
+    ctx.h, ctx.device = None, -1
+    return ctx
+
+
+def test_outputs_are_made_on_the_stream_of_the_call(monkeypatch):
+    ctx, f, side = host_context(), torch.zeros(3, 64, dtype=torch.float16), Side()
+    q, s = torch.zeros(3, 64, dtype=torch.int8), torch.zeros(3)
+    seen = Streams(monkeypatch)
+    for call, made in ((lambda: ctx.quantize_rows_q8(f, stream=side), 2),
+                       (lambda: ctx.quantize_rows_q8(f, q, stream=side), 1),
+                       (lambda: ctx.add_norm_q8(f, None, stream=side), 2),
+                       (lambda: ctx.add_norm_q8(f, None, scale=s, stream=side), 1),
+                       (lambda: ctx.quantize_rows_q8(f, q, s, stream=side), 0)):
+        seen.made.clear()
+        out = call()
+        assert seen.made == [side] * made and seen.calls[-1][1][-1] == 77
+        assert out[0].shape == (3, 64) and out[1].shape == (3,)
+
+
 # ---- how products are cut up --------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def plan(tmp_path_factory):
