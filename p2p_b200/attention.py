@@ -535,14 +535,14 @@ class Context:
     def kv_quantize_q4(self, src: torch.Tensor, dst: Optional[torch.Tensor] = None,
                        stream=None) -> torch.Tensor:
         """f16 cache rows [..., Hkv, 64] -> the rows [..., kv_q4_row_bytes(Hkv)] (uint8) of a
-        4-bit cache."""
+        4-bit cache; without dst made on `stream`."""
         if src.dtype is not torch.float16 or src.get_device() != self.device or src.dim() < 2 or \
                 src.shape[-1] != HEAD_DIM or not src.is_contiguous():
             _refuse(f"src: contiguous f16 [..., Hkv, {HEAD_DIM}] on device {self.device} needed")
         hkv = src.shape[-2]
         shape = (*src.shape[:-2], kv_q4_row_bytes(hkv))
         if dst is None:
-            dst = torch.empty(shape, dtype=torch.uint8, device=src.device)
+            dst = _empty(shape, torch.uint8, src.device, stream)
         if dst.dtype is not torch.uint8 or tuple(dst.shape) != shape or \
                 dst.get_device() != self.device or not dst.is_contiguous():
             _refuse(f"dst: contiguous uint8 {shape} on device {self.device} needed")
@@ -627,12 +627,13 @@ class Context:
 
     def kv_quantize_q8(self, src: torch.Tensor, scale: torch.Tensor,
                        dst: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
-        """f16 cache rows [..., Hkv, 64] -> int8 (the decode's int8 cache format)."""
+        """f16 cache rows [..., Hkv, 64] -> int8 (the decode's int8 cache format); without dst made
+        on `stream`."""
         assert src.dtype == torch.float16 and scale.dtype == torch.float32
         hkv = src.shape[-2]
         rows = src.numel() // (hkv * HEAD_DIM)
         if dst is None:
-            dst = torch.empty(src.shape, dtype=torch.int8, device=src.device)
+            dst = _empty(src.shape, torch.int8, src.device, stream)
         self._chk(lib.p2p_kv_quantize_q8(self.h, _ptr(src), _ptr(dst), rows, hkv, _ptr(scale),
                                          scale.numel(), _stream(stream)))
         return dst
@@ -826,10 +827,10 @@ class Context:
 
     def q4_to_f16(self, w, dst: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """The resident f16 copy [n][k] of a 4-bit matrix (made once, reused by every call of
-        gemm_f16w / qkv_gemm_prep_f16w)."""
+        gemm_f16w / qkv_gemm_prep_f16w); without dst made on `stream`."""
         mw = self.q4(w)
         if dst is None:
-            dst = torch.empty((mw.n, mw.k), dtype=torch.float16, device="cuda")
+            dst = _empty((mw.n, mw.k), torch.float16, w[0].device, stream)
         self._chk(lib.p2p_q4_to_f16(self.h, C.byref(mw), _ptr(dst), _stream(stream)))
         return dst
 

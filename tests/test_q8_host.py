@@ -306,6 +306,23 @@ def test_outputs_are_made_on_the_stream_of_the_call(monkeypatch):
         assert out[0].shape == (3, 64) and out[1].shape == (3,)
 
 
+def test_copies_in_other_formats_are_made_on_the_stream_of_the_call(monkeypatch):
+    ctx, side = host_context(), Side()
+    rows = torch.zeros(5, 2, 64, dtype=torch.float16)
+    w = (torch.zeros(8, 8, dtype=torch.int32), torch.zeros(8, 2, dtype=torch.float16),
+         torch.zeros(2, dtype=torch.int32))
+    seen = Streams(monkeypatch)
+    monkeypatch.setattr("p2p_b200.attention.kv_q4_row_bytes", lambda hkv: 72 * hkv)
+    for call, shape in ((lambda: ctx.kv_quantize_q4(rows, stream=side), (5, 144)),
+                        (lambda: ctx.kv_quantize_q8(rows, torch.ones(1), stream=side), (5, 2, 64)),
+                        (lambda: ctx.q4_to_f16(w, stream=side), (8, 64))):
+        seen.made.clear()
+        out = call()
+        assert seen.made == [side] and tuple(out.shape) == shape
+        handle = seen.calls[-1][1][-1]
+        assert getattr(handle, "value", handle) == 77
+
+
 # ---- how products are cut up --------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def plan(tmp_path_factory):
