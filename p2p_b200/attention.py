@@ -721,7 +721,10 @@ class Context:
                     eps: float = 1e-5, stream=None):
         """Residual addition and RMS norm (p2p_add_norm_q8): sum_out = x + residual (may be
         either of them), y the normed rows, (q, scale) their int8 rows; returns (q, scale).  What is
-        not given of them is made on `stream`."""
+        not given of them is made on `stream`.  eps is at least 2^-126 (what is 0 in f32 stands for 1e-5
+        in the C structure)."""
+        if not 2.0**-126 <= eps <= 3.4e38:
+            _refuse(f"eps: {eps}")
         dt = x.dtype
         ld_x, m, k, code = self._values(x, "x", None, -1, -1)
         r_at = w_at = s_at = y_at = ld_r = ld_s = ld_y = 0

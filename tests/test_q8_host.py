@@ -323,6 +323,20 @@ def test_copies_in_other_formats_are_made_on_the_stream_of_the_call(monkeypatch)
         assert getattr(handle, "value", handle) == 77
 
 
+def test_no_eps_is_taken_for_another_one(monkeypatch):
+    """0 and what rounds to it select 1e-5 in the C structure: never what a caller of the Python layer means."""
+    import p2p_b200
+    ctx, f = host_context(), torch.zeros(3, 64, dtype=torch.float16)
+    seen = Streams(monkeypatch)
+    for eps in (0.0, -0.0, 0, 1e-50, 1e-39, -1e-5, 1e39, 1e400, float("nan")):
+        with pytest.raises(p2p_b200.P2PError, match="eps"):
+            ctx.add_norm_q8(f, None, eps=eps, stream=Side())
+    assert not seen.calls
+    for eps in (1e-37, 1e-6, 1, 1e38):
+        ctx.add_norm_q8(f, None, eps=eps, stream=Side())
+    assert len(seen.calls) == 4
+
+
 # ---- how products are cut up --------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def plan(tmp_path_factory):
