@@ -463,7 +463,7 @@ typedef struct p2p_read_rows {
   int64_t ld_out;
   int32_t rows;
   int32_t dtype; /* P2P_F16 or P2P_F32 */
-  float factor;  /* 0 selects 1 */
+  float factor;  /* finite; 0 selects 1 */
 } p2p_read_rows;
 p2p_status p2p_read_rows_q8(p2p_ctx* ctx, const p2p_read_rows* args, void* stream);
 

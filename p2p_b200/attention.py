@@ -699,13 +699,13 @@ class Context:
 
     def read_rows_q8(self, q: torch.Tensor, scale: torch.Tensor, out: torch.Tensor, *,
                      index: Optional[torch.Tensor] = None, factor: float = 1.0, stream=None):
-        """Rows index[i] (without index: row i) of int8 rows as values times `factor` (not 0), into
-        out [rows][cols] (f16 or f32): the embedding lookup (p2p_read_rows_q8).  index -1 gives
-        zeros."""
+        """Rows index[i] (without index: row i) of int8 rows as values times `factor` (finite, of 2^-126
+        at least in size: what is 0 in f32 stands for 1 in the C structure), into out [rows][cols] (f16 or
+        f32): the embedding lookup (p2p_read_rows_q8).  index -1 gives zeros."""
+        if not 2.0**-126 <= abs(factor) <= 3.4e38:
+            _refuse(f"factor: {factor}")
         s = self._q8(q, scale, "q")
         ld, n, _, code = self._values(out, "out", None, -1, s[4])
-        if factor == 0:
-            _refuse("factor: 0")
         st = lib.p2p_read_rows_q8(
             self.h, _READ_ROWS(*s, 0 if index is None else self._ints(index, n, "index"),
                                out.data_ptr(), ld, n, code, factor),

@@ -2,6 +2,7 @@
 // front of them, their products).  Host-side checks only.
 #include <cuda_runtime.h>
 
+#include <cfloat>
 #include <cstdarg>
 #include <cstdio>
 
@@ -160,6 +161,9 @@ p2p_status p2p_read_rows_q8(p2p_ctx* ctx, const p2p_read_rows* args, void* strea
     return fail(ctx, P2P_ERR_INVALID_ARG, "%s: %lld rows of %d, index %p", who, (long long)rows,
                 src->rows, (const void*)index);
   if (rows == 0) return P2P_OK;
+  // a row of zeros times an infinity would be NaN
+  if (!(args->factor >= -FLT_MAX && args->factor <= FLT_MAX))
+    return fail(ctx, P2P_ERR_INVALID_ARG, "%s: factor %g", who, double(args->factor));
   const unsigned es = dtype == P2P_F32 ? 4 : 2;
   if ((st = check_rows(ctx, out, ld_out, src->cols, es, "out", who)) != P2P_OK) return st;
   const Span to{out, ld_out * es, int64_t(src->cols) * es, rows, "out"};

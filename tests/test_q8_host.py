@@ -337,6 +337,28 @@ def test_no_eps_is_taken_for_another_one(monkeypatch):
     assert len(seen.calls) == 4
 
 
+def test_no_factor_is_taken_for_another_one(api, monkeypatch):
+    """0 and what rounds to it select 1 in the C structure; an infinity would make NaN of the rows of zeros
+    that an index of -1 gives."""
+    import p2p_b200
+    before, good = api.host_launches(), rows(4 * MB)
+    for factor in (float("inf"), float("-inf"), float("nan")):
+        said(api, read(api, good, factor=factor), BAD, "factor")
+    for factor in (0.0, -2.0, 3.4028234663852886e38):
+        said(api, read(api, good, factor=factor), 0)
+    assert api.host_launches() == before + 3
+    ctx, f = host_context(), torch.zeros(3, 64, dtype=torch.float16)
+    q, s = torch.zeros(3, 64, dtype=torch.int8), torch.zeros(3)
+    seen = Streams(monkeypatch)
+    for factor in (0.0, 1e-50, -1e-50, 1e39, -1e400, float("nan")):
+        with pytest.raises(p2p_b200.P2PError, match="factor"):
+            ctx.read_rows_q8(q, s, f, factor=factor, stream=Side())
+    assert not seen.calls
+    for factor in (1e-37, -1, 1e38):
+        ctx.read_rows_q8(q, s, f, factor=factor, stream=Side())
+    assert len(seen.calls) == 3
+
+
 # ---- how products are cut up --------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def plan(tmp_path_factory):
