@@ -71,6 +71,7 @@ _KV_FORMATS = {torch.float16: _lib.P2P_KV_F16, torch.int8: _lib.P2P_KV_I8,
 
 
 _ROW_TYPES = {torch.float16: _lib.P2P_F16, torch.float32: _lib.P2P_F32}
+_TOO_MANY = 2**31  # rows or columns: the C structures count them in 32 bits
 _ACTS = {"silu": _lib.P2P_ACT_SILU, "gelu": _lib.P2P_ACT_GELU}
 # Bytes of the C structures of the same order (p2p_quantize_rows, p2p_read_rows, p2p_add_norm, p2p_product,
 # p2p_gated), padded to their size.
@@ -650,7 +651,8 @@ class Context:
                 t.get_device() == self.device and len(shape) == 2:
             m, k = shape
             ld, one = t.stride()
-            if (rows < 0 or m == rows) and (cols < 0 or k == cols) and (one == 1 or k <= 1):
+            if (rows < 0 or m == rows) and (cols < 0 or k == cols) and (one == 1 or k <= 1) and \
+                    m < _TOO_MANY:
                 return ld if m > 1 else k, m, k, code
         _refuse(f"{name}: {dtype or 'f16 or f32'} [{rows if rows >= 0 else 'rows'}]"
                 f"[{cols if cols >= 0 else 'cols'}] on device {self.device} needed, "
@@ -664,7 +666,7 @@ class Context:
         if q.dtype is torch.int8 and q.get_device() == dev and len(shape) == 2:
             n, k = shape
             ld, one = q.stride()
-            if one == 1 or k <= 1:
+            if (one == 1 or k <= 1) and n < _TOO_MANY and k < _TOO_MANY:
                 if scale.dtype is torch.float32 and scale.get_device() == dev and \
                         scale.numel() >= n and scale.is_contiguous():
                     return (q.data_ptr(), scale.data_ptr(), ld if n > 1 else (k + 15) & -16, n, k)

@@ -359,6 +359,27 @@ def test_no_factor_is_taken_for_another_one(api, monkeypatch):
     assert len(seen.calls) == 3
 
 
+def test_sizes_beyond_32_bits_are_refused(monkeypatch):
+    """As any other argument, not by an error of the packing."""
+    import p2p_b200
+    ctx, many = host_context(), 2**31
+    ctx.device = torch.empty(1, device="meta").get_device()
+    z = lambda *s, dt=torch.int8: torch.empty(*s, dtype=dt, device="meta")  # noqa: E731
+    f16, f32 = torch.float16, torch.float32
+    tall, wide, one = (z(many, 16), z(many, dt=f32)), (z(1, many), z(1, dt=f32)), (z(1, 16), z(1, dt=f32))
+    seen = Streams(monkeypatch)
+    for call in (lambda: ctx.read_rows_q8(*one, z(many, 16, dt=f16), stream=Side()),
+                 lambda: ctx.read_rows_q8(*tall, z(1, 16, dt=f16), stream=Side()),
+                 lambda: ctx.quantize_rows_q8(z(many, 16, dt=f16), *tall, stream=Side()),
+                 lambda: ctx.quantize_rows_q8(z(1, many, dt=f16), *wide, stream=Side()),
+                 lambda: ctx.add_norm_q8(z(many, 16, dt=f16), None, *tall, stream=Side()),
+                 lambda: ctx.gemm_q8(tall, *one, z(1, many, dt=f16), stream=Side()),
+                 lambda: ctx.gate_q8(one, one, *tall, z(many, 1, dt=f16), stream=Side())):
+        with pytest.raises(p2p_b200.P2PError):
+            call()
+    assert not seen.calls
+
+
 # ---- how products are cut up --------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def plan(tmp_path_factory):
