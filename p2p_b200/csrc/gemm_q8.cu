@@ -57,18 +57,24 @@ struct Q8Params {
   int32_t deep;                 // the tensor maps' third dimension is k in steps of 128
 };
 
-// act(g) * u, the exponential and the reciprocal as approximations of a few units in the last place, with
-// what is below f32's normal numbers taken as 0 (a reciprocal of more than 2^126 too): f16 has none of it.
+// act(g) * u.  The exponential and the reciprocal are approximations of a few units in the last place (the
+// f16 of the result has a 2^-11th) that take what is below f32's normal numbers as 0: 1 / (1 + exp(-t)) is
+// there from t = -87.3 on, where exp(-t) is still a number, and a large u brings the product back.  So a
+// quarter of the sum goes into the reciprocal, and a quarter of that out of it.
 template <bool GELU>
 __device__ __forceinline__ Pair act_mul(Pair g, Pair u) {
   constexpr float k = GELU ? -1.5957691216057308f * kLog2e : -kLog2e;
-  Pair t = mul2(g, pair(k, k));
-  if constexpr (GELU) t = mul2(t, mad2(mul2(g, g), pair(0.044715f, 0.044715f), pair(1.f, 1.f)));
-  const Pair d = add2(pair(fast_exp2(t.f[0]), fast_exp2(t.f[1])), pair(1.f, 1.f));
+  const Pair quarter = pair(0.25f, 0.25f), less = pair(-2.f, -2.f);
+  Pair t;
+  if constexpr (GELU)
+    t = mad2(mul2(g, pair(k, k)), mad2(mul2(g, g), pair(0.044715f, 0.044715f), pair(1.f, 1.f)), less);
+  else
+    t = mad2(g, pair(k, k), less);
+  const Pair d = add2(pair(fast_exp2(t.f[0]), fast_exp2(t.f[1])), quarter);
   Pair r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.f[0]) : "f"(d.f[0]));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.f[1]) : "f"(d.f[1]));
-  return mul2(mul2(g, r), u);
+  return mul2(mul2(g, mul2(r, quarter)), u);
 }
 __device__ __forceinline__ Pair act_mul(Pair g, Pair u, int act) {
   return act == kActSilu ? act_mul<false>(g, u) : act_mul<true>(g, u);

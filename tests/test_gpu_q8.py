@@ -497,6 +497,34 @@ def test_gate_ends_of_the_activation(ctx, act, m):
     assert torch.isnan(h[bad]).all() and not torch.isnan(h[~bad]).any()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("m", [1, 150, 2100])
+def test_gate_of_a_large_up_value(ctx, act, m):
+    """Gate values down to where exp(-t) still is an f32 number: 1 / (1 + exp(-t)) is below f32's normal
+    numbers there, and a large up value brings the product back."""
+    x = torch.zeros(m, 16, dtype=torch.int8, device="cuda")
+    x[:, 0] = 1
+    w = torch.zeros(64, 16, dtype=torch.int8, device="cuda")
+    w[:, 0] = 1
+    xs = torch.ones(m, device="cuda")
+    t = torch.linspace(-88.6, -80, 64, device="cuda", dtype=torch.float64)
+    g = t.clone()
+    if act == "gelu":  # t = 2c (g + 0.044715 g^3), solved for g
+        for _ in range(60):
+            f = 2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g**3) - t
+            g -= f / (2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * g**2))
+    gs, us = g.float(), torch.exp(-t).float()
+    h = torch.zeros(m, 64, device="cuda", dtype=F16)
+    ctx.gate_q8((w, gs), (w, us), x, xs, h, act=act)
+    # (check_gate's 16 |t| roundings stay; its bound on h itself is 2^-11 and no less: nothing here is small)
+    p, u = gs.double(), us.double()
+    t = p if act == "silu" else 2 * math.sqrt(2 / math.pi) * (p + 0.044715 * p**3)
+    want = (p / (1 + torch.exp(-t)) * u).expand(m, 64)
+    assert want.abs().min() > 1
+    # the quotient below 2^-126 keeps 2^-21 or more of itself
+    close(h, want, want.abs() * (2.0**-11 + U * (16 + 16 * t.abs()) + 2.0**-21))
+
+
 @pytest.mark.parametrize("m", [3, 200, 2100])
 def test_the_same_rows_on_every_side(ctx, m):
     """One matrix as gate, up and tokens."""
