@@ -389,7 +389,6 @@ struct RowsQ8Args {  // add_norm, or (norm 0) the quantisation of rows alone
   int64_t ld_x, ld_r, ld_sum, ld_y;
   float eps;
   int32_t norm;
-  float inv_cols;     // set by the launcher
 };
 cudaError_t launch_rows_q8(const RowsQ8Args& a, int dtype, int num_sms, cudaStream_t s);
 struct ReadQ8Args {

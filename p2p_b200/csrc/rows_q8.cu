@@ -225,33 +225,24 @@ __device__ __forceinline__ RowSums row_reduce(RowSums r, int warps, int warp, in
   return r;
 }
 
-// The norm's root and reciprocal are approximations of 2^-22 (a row's warps all come by here, and rounded
-// ones took 60 of 350 instructions for 32 values a lane); rows that are only quantised get rounded
-// quotients.
+// Every operation rounded (as approximations of 2^-22 the norm's root and quotients took 0.9 of 22.5 us for
+// 8192 rows of 2048 f16 values less, and an f32 y and the scales were up to four units in the last place off).
 template <bool NORM, bool F16>
-__device__ __forceinline__ RowScale row_scale(RowSums r, float inv_cols, float eps) {
+__device__ __forceinline__ RowScale row_scale(RowSums r, int cols, float eps) {
   constexpr bool kTies = F16 && !NORM;
   RowScale s;
   const float nan = __uint_as_float(0x7fffffffu);
   s.rstd = 1.f;
-  if constexpr (NORM) {
-    const float mean = fmaxf(fmaf(r.ss, inv_cols, eps), 1.1754944e-38f);
-    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(s.rstd) : "f"(mean));
-    if (!(r.ss <= 3.4028235e38f)) s.rstd = nan;
-  }
+  if constexpr (NORM)
+    s.rstd = r.ss <= 3.4028235e38f
+                 ? __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn(__fdiv_rn(r.ss, float(cols)), eps)))
+                 : nan;
   const float a = s.top = r.top * s.rstd;
   if (a < kTiny) {
     s.inv = s.scale = 0.f;
   } else if (a <= 3.4028235e38f) {
-    if (NORM && a < 0x1p100f) {
-      float inv;
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(a));
-      s.inv = 127.f * inv;
-      s.scale = a * (1.f / 127.f);
-    } else {
-      s.inv = kTies ? __fdiv_ru(127.f, a) : __fdiv_rn(127.f, a);
-      s.scale = __fdiv_rn(a, 127.f);
-    }
+    s.inv = kTies ? __fdiv_ru(127.f, a) : __fdiv_rn(127.f, a);
+    s.scale = __fdiv_rn(a, 127.f);
   } else {
     s.inv = 0.f;
     s.scale = nan;
@@ -376,7 +367,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, NP <= 4 ? 3 : 1)
   sums = row_reduce<NORM>(sums, warps, warp, lane, part);
 #pragma unroll
   for (int i = 0; i < NP; ++i) keep_words(v[i]);
-  const RowScale sc = row_scale<NORM, sizeof(T) == 2>(sums, a.inv_cols, a.eps);
+  const RowScale sc = row_scale<NORM, sizeof(T) == 2>(sums, c.cols, a.eps);
 #pragma unroll
   for (int i = 0; i < NP; ++i) finish_piece<NORM, WIDE>(v[i], sc, a, row, c, i, turn);
   if (a.out.q && part_of == 0 && lane == 0) a.out.scale[row] = sc.scale;
@@ -414,7 +405,7 @@ __global__ void __launch_bounds__(kThreads)
   }
   sums.ss = ss.f[0] + ss.f[1];
   sums = row_reduce<NORM>(sums, kWarps, warp, lane, part);
-  const RowScale sc = row_scale<NORM, sizeof(T) == 2>(sums, a.inv_cols, a.eps);
+  const RowScale sc = row_scale<NORM, sizeof(T) == 2>(sums, c.cols, a.eps);
   for (int i = 0; i < pieces; ++i) {
     Piece<T> v, u;
     load_piece<WIDE>(v, s ? s : x, c, i);
@@ -520,10 +511,9 @@ cudaError_t launch_rows_t(RowsQ8Args a, int num_sms, cudaStream_t s) {
     return launch(reinterpret_cast<const void*>(&long_rows_kernel<T, NORM, WIDE>), rows, p, s);
   }
   // As few warps a row as hold it in kMostPieces pieces a lane, the norm, which holds x and the residual,
-  // in two (8192 rows of 2048 f16 values 22.5 us, 23.8 in four; 13.8 and 15.2 for 1024; 21.6 and 13.3
-  // since), one warp also
-  // with eight pieces a lane (65536 rows of 1024 f32 values are quantised in 49 us then, 68 by pairs of
-  // warps); but where rows are few, as many as the row has pieces for, up to 8.
+  // in two (8192 rows of 2048 f16 values 22.4 us, 23.8 in four; 13.6 and 15.2 for 1024), one warp also with
+  // eight pieces a lane (65536 rows of 1024 f32 values are quantised in 49 us then, 68 by pairs of warps); but
+  // where rows are few, as many as the row has pieces for, up to 8.
   const int most = NORM && passes <= 2 * kMostWarps ? 2 : kMostPieces;
   int warps = 1;
   while (passes > warps * (!NORM && V == 4 && warps == 1 ? 8 : most) ||
@@ -570,9 +560,7 @@ cudaError_t launch_read(ReadQ8Args a, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t launch_rows_q8(const RowsQ8Args& args, int dtype, int num_sms, cudaStream_t s) {
-  RowsQ8Args a = args;
-  a.inv_cols = 1.f / float(a.out.cols);
+cudaError_t launch_rows_q8(const RowsQ8Args& a, int dtype, int num_sms, cudaStream_t s) {
   return dtype == 0 ? launch_rows<__half>(a, num_sms, s) : launch_rows<float>(a, num_sms, s);
 }
 

@@ -239,6 +239,27 @@ def test_norm(ctx, dt, m, k, pad, off, weighted, residual):
         assert torch.equal(q2, q) and torch.equal(r2, total)
 
 
+@pytest.mark.parametrize("m,k,pad", [(3, 1, 0), (200, 64, 0), (500, 1003, 0), (300, 2048, 0), (40, 2048, 1),
+                                     (9, 8192, 0), (4, 20000, 0)])
+def test_norm_is_f32_operations(ctx, m, k, pad):
+    """Of whole numbers, whose squares add up exactly in any order, y and the scales are those of the formula
+    in f32 operations, each rounded: a mean, a root, a quotient, two products; the largest |y| over 127."""
+    g = gen(m + k)
+    x = rows_in(g, m, k, F32, pad)
+    x.copy_(torch.randint(-15, 16, (m, k), generator=g, device="cuda"))
+    x[:, 0] = 13
+    w = (1 + 0.3 * torch.randn(k, generator=g, device="cuda")).half()
+    y = torch.zeros(m, k, device="cuda")
+    q, s = ctx.add_norm_q8(x, w, y=y, eps=0.001953125)
+    f = lambda v: v.float().double()  # noqa: E731  (64 bits are more than twice 24: rounded as once)
+    d = x.double()
+    mean = f(f((d * d).sum(1, keepdim=True) / k) + 0.001953125)
+    rstd = f(1 / f(torch.sqrt(mean)))
+    want = f(f(d * w.double()) * rstd)
+    assert torch.equal(y.double(), want)
+    assert torch.equal(s.double(), f(want.abs().amax(1) / 127))
+
+
 @pytest.mark.parametrize("k", [512, 1003])
 def test_norm_weights_anywhere(ctx, k):
     """Weights that start between two 16-byte boundaries, and no codes' neighbours touched."""
