@@ -8,10 +8,10 @@
 //                  of two CTAs per 256 x 256 tile and one tcgen05.mma.cta_group::2 stream, persistent, two
 //                  accumulators, the last wave's tiles halved.  Gate and up of 4096 tokens (8192 x 2048
 //                  each): 76 us alone (3630 TOP/s, 89 % of the tensor pipe's cycles), 86 us among some,
-//                  101 us in long runs; 8192 x 2048 x 8192: 81, 89 and 103 us.
+//                  103 us in long runs; 8192 x 2048 x 8192: 81, 88 and 104 us.
 //   narrow_kernel  few tokens, bound by the weights' bytes: the weights are the MMA's rows and the tokens
-//                  its columns.  The LM head of 32 tokens (65536 x 2048) 24.9 us (5.7 TB/s), gate and up of
-//                  one token (2 x 8192 x 2048) 6.9 us, 48 x 2048 x 8192 7.1 us (15 by pairs of CTAs).
+//                  its columns.  The LM head of 32 tokens (65536 x 2048) 24.4 us (5.9 TB/s), gate and up of
+//                  one token (2 x 8192 x 2048) 7.0 us, 48 x 2048 x 8192 6.5 us (15 by pairs of CTAs).
 // A warp that walks a ring does so as a whole: with its loop in one lane the compiler has to treat what a
 // copy takes as different in every lane, and a stage took 200 ns to issue (8192 x 2048 x 8192 98 -> 91 us).
 // Every mbarrier wait is bounded (about one second): a wait that gives up sets the device error word,
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1)
     for (int t = first; t < p.items && ok; t += step) {
       const int n0 = t % p.tiles_n * p.rows, m0 = t / p.tiles_n * p.tokens;
       // each CTA begins at another part of k, since all of them read the same tokens (gate and up of one
-      // token, 2 x 8192 x 2048: 6.6 us, 6.9 with all of them at the same part)
+      // token, 2 x 8192 x 2048: 0.3 of 7 us less than with all of them at the same part)
       int kt = k0 + first % (k1 - k0);
       for (int i = k0; i < k1; ++i) {
         if (round > 0 && !(ok = gemm_wait_all(s.abort_flag, &s.empty[st], (round - 1) & 1, p.err)))
