@@ -1000,8 +1000,8 @@ cudaError_t cluster_room(int* room) {
 NarrowPlan narrow_plan(int m, int n, int k, int G, int num_sms, int room) {
   constexpr float kLoad = 50, kDram = 23, kWait = 150, kIssue = 37, kHandOver = 260;
   constexpr int kMostChunks = 4, kMostStage = 64 * 1024;
-  // the MMA's columns: 8 or a multiple of 16; of 64 rows also 24 (which not every list of kind::i8's shapes
-  // has, and with 128 rows nothing needs: 24 x 65536 x 2048 takes 64)
+  // the MMA's columns: 8 or a multiple of 16, with 64 rows also 24 (which not every list of kind::i8's shapes
+  // has; 20 x 2048 x 2048 4.6 us, 4.8 with 32)
   const int fewest = std::min(kMostTokens, m <= 24 ? (m + 7) / 8 * 8 : (m + 15) / 16 * 16);
   const int token_tiles = (m + fewest - 1) / fewest, nk = (k + kStep - 1) / kStep;
   const float sms = float(num_sms);
